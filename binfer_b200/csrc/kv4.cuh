@@ -1,0 +1,43 @@
+// The layout of key/value pages held in 4 bits.
+//
+// A cache of one layer is uint8 [pages][kv_heads][page_size / 8][9 d]: a record of 9 d bytes holds
+// eight tokens of one kv head.  Every KV4_GROUP = 64 numbers of a key or value row share a scale s
+// and a lowest value m (bfloat16 each); a number is m + s c with a code c of 0 to 15, two codes a
+// byte, the lower one in the low half.  Inside a record:
+//
+//   keys' codes     8 tokens x d / 2 bytes   token after token; a row is four parts of d / 8 bytes, part
+//                                            q holds numbers 16 q .. 16 q + 15 of every group
+//   values' codes   8 parts x 8 tokens x d / 16 bytes   part r holds numbers 8 r .. 8 r + 7 of every group
+//   keys' (s, m)    8 tokens x d / 64 pairs
+//   values' (s, m)  the same
+//
+// so that lane 4 r + q of a warp finds what it needs as a tensor-core operand side by side: its part of
+// key r, and its part of the values of tokens 2 q and 2 q + 1.  4.5 bits a number.
+#pragma once
+#include <cuda_bf16.h>
+
+#define KV4_GROUP 64
+#define KV4_EIGHTH 8                       // tokens of a record
+
+__host__ __device__ constexpr int kv4_record(int d) { return 9 * d; }
+__host__ __device__ constexpr int kv4_values_at(int d) { return 4 * d; }
+__host__ __device__ constexpr int kv4_key_params_at(int d) { return 8 * d; }
+__host__ __device__ constexpr int kv4_value_params_at(int d) { return 8 * d + d / 2; }
+
+// Byte (in the record) of the code of number i of token tok's key or value; bit 0 of i chooses the half.
+__host__ __device__ constexpr int kv4_key_byte(int d, int tok, int i) {
+  return tok * (d / 2) + (i % 64) / 16 * (d / 8) + i / 64 * 8 + (i % 16) / 2;
+}
+__host__ __device__ constexpr int kv4_value_byte(int d, int tok, int i) {
+  return 4 * d + (i % 64) / 8 * (d / 2) + tok * (d / 16) + i / 64 * 4 + (i % 8) / 2;
+}
+
+// (s, m) as stored: s in the low half
+__device__ __forceinline__ float kv4_scale(unsigned pair) { return __uint_as_float(pair << 16); }
+__device__ __forceinline__ float kv4_low(unsigned pair) { return __uint_as_float(pair & 0xffff0000u); }
+
+// Whether some row at positions first .. last sees a key of [j0, j1] (window 0: no window).
+__device__ __forceinline__ bool kv4_seen(int j0, int j1, int first, int last, int window, int keep) {
+  if (j0 > last) return false;
+  return window <= 0 || j0 < keep || j1 > first - window;
+}

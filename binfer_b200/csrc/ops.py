@@ -1820,6 +1820,241 @@ def kv_store(proj: torch.Tensor, k_off: int, v_off: int, slots: torch.Tensor,
          _c_int(_dtype_code(proj)), _ptr(err), _stream())
 
 
+# ------------------------------------------------------------- a cache held in 4 bits
+KV4_HEAD_DIMS = (64, 128, 256)
+KV4_GROUP = 64               # numbers of a row that share a scale and a lowest value
+KV4_LOAD_PAGE = 64           # tokens of a page that kv4_load writes
+
+
+def kv4_takes(dtype: torch.dtype, d: int, page_size: int) -> bool:
+    """Whether a cache of heads of ``d`` numbers in pages of ``page_size`` tokens can be held in 4
+    bits beside activations of ``dtype``."""
+    return (dtype == torch.bfloat16 and d in KV4_HEAD_DIMS and 8 <= page_size <= 128
+            and 128 % page_size == 0)
+
+
+def kv4_cache(pages: int, kv_heads: int, page_size: int, d: int, device) -> torch.Tensor:
+    """Zeroed pages for keys and values in 4 bits: ``uint8 [pages, kv_heads, page_size / 8, 9 d]``.
+    The 9 d bytes of eight tokens hold their keys and values as codes of 0 to 15 and, per 64 numbers of
+    a row, a scale s and a lowest value m in bfloat16: a number stands for m + s c (4.5 bits each;
+    ``csrc/kv4.cuh`` has the order of the bytes)."""
+    if not kv4_takes(torch.bfloat16, d, page_size):
+        raise KernelError(f"a cache in 4 bits takes heads of {KV4_HEAD_DIMS} numbers and pages of 8 to "
+                          f"128 tokens that divide 128, not {d} and {page_size}")
+    if pages < 1 or kv_heads < 1:
+        raise KernelError("a cache needs at least one page and one kv head")
+    return torch.zeros((pages, kv_heads, page_size // 8, 9 * d), dtype=torch.uint8, device=device)
+
+
+def _kv4_check(what: str, cache: torch.Tensor, *others) -> Tuple[int, int, int, int]:
+    """(pages, kv heads, page size, head size) of a cache in 4 bits; every tensor on the device that the
+    launch goes to."""
+    if cache.dtype != torch.uint8 or cache.dim() != 4 or not cache.is_contiguous() or cache.data_ptr() % 16:
+        raise KernelError(f"{what}: cache must be contiguous uint8 [pages, kv heads, page_size / 8, 9 d] "
+                          "on a 16-byte boundary")
+    pages, nkv, eighths, rec = cache.shape
+    if rec % 9 or not kv4_takes(torch.bfloat16, rec // 9, 8 * eighths):
+        raise KernelError(f"{what}: pages of {8 * eighths} tokens and records of {rec} bytes are no cache "
+                          "in 4 bits")
+    _same_device(what, cache, *others)
+    return pages, nkv, 8 * eighths, rec // 9
+
+
+def _same_device(what: str, *tensors) -> None:
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise KernelError("the engine's kernels take CUDA tensors only (no CPU path)")
+        if t.device.index != torch.cuda.current_device():
+            raise KernelError(f"{what}: a tensor lies on {t.device}, the launch goes to device "
+                              f"{torch.cuda.current_device()}")
+
+
+def _want_int_table(t: torch.Tensor, what: str, name: str) -> None:
+    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] < 1 or t.shape[1] < 1 or t.stride(1) != 1:
+        raise KernelError(f"{what}: {name} must be int32 with two dimensions and contiguous rows")
+
+
+def kv4_store(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: torch.Tensor,
+              err: torch.Tensor) -> None:
+    """The rows ``k`` and ``v`` ``[T, kv_heads * d]`` (bfloat16; column blocks of wider buffers are fine)
+    into the pages of a cache in 4 bits (``kv4_cache``), token t at ``slots[t]``; a negative slot is not
+    written, one outside the pool sets the error word.  No two tokens have the same slot.
+
+    Of 64 numbers x: m = min x, s = bfloat16((max x - m) / 15), c = (x - m) / s rounded to the nearest
+    whole number (ties to even).  A number that is not finite makes its 64 neighbours read as NaN."""
+    T = k.shape[0] if k.dim() == 2 else -1
+    if (T < 0 or v.dim() != 2 or k.shape != v.shape or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16
+            or (T and (k.stride(1) != 1 or v.stride(1) != 1))):
+        raise KernelError("kv4_store: k and v must be bfloat16 [T, kv heads * d] with contiguous rows")
+    _want(slots, torch.int32, "slots"); _want(err, torch.int32, "err")
+    pages, nkv, ps, d = _kv4_check("kv4_store", cache, k, v, slots, err)
+    if k.shape[1] != nkv * d or slots.numel() != T:
+        raise KernelError(f"kv4_store: rows of {nkv} heads of {d} and a slot per token, got "
+                          f"{tuple(k.shape)} and {slots.numel()} slots")
+    if T == 0:
+        return
+    _run("kv4_store", lib().bf_kv4_store, _ptr(k), _c_ll(k.stride(0)), _ptr(v), _c_ll(v.stride(0)),
+         _ptr(slots), _ptr(cache), _c_int(T), _c_int(nkv), _c_int(d), _c_int(ps), _c_ll(pages * ps),
+         _ptr(err), _stream())
+
+
+def kv4_load(cache: torch.Tensor, block_tables: torch.Tensor, items: torch.Tensor, n_items: int,
+             rows: int, err: torch.Tensor, window: Optional[int] = None, keep_first: int = 0,
+             items_out: Optional[torch.Tensor] = None):
+    """The whole contexts of prompt portions out of a cache in 4 bits, as bfloat16 pages of 64 tokens:
+    ``(k [1 + rows / 64, kv heads, 64, d], v, tables int32 [n_items, rows / 64])``.  ``items`` int32
+    ``[n_items, 4]`` of (request, first token row, rows, first position); ``rows``: the contexts' sum, each
+    rounded up to 64.  Page 0 is zero, so are places behind a context and, with ``window`` and
+    ``keep_first``, keys that no row of the portion sees (pages of nothing else are not written, their
+    place in ``tables`` is page 0).  ``items_out``: takes the items with the portion's number in the
+    request's place, which goes with ``tables``."""
+    _want_int_table(block_tables, "kv4_load", "block_tables")
+    _want(items, torch.int32, "items"); _want(err, torch.int32, "err")
+    pages, nkv, ps, d = _kv4_check("kv4_load", cache, block_tables, items, err, items_out)
+    if n_items < 1 or items.numel() < 4 * n_items or rows < 64 or rows % 64:
+        raise KernelError("kv4_load: items must be [n_items, 4], rows a multiple of 64 tokens")
+    if items_out is not None:
+        _want(items_out, torch.int32, "items_out")
+        if items_out.numel() < 4 * n_items:
+            raise KernelError("kv4_load: items_out must have room for the items")
+    window, keep_first = _kv4_mask("kv4_load", window, keep_first)
+    n = 1 + rows // 64
+    k = torch.empty((n, nkv, KV4_LOAD_PAGE, d), dtype=torch.bfloat16, device=cache.device)
+    v = torch.empty_like(k)
+    tables = torch.empty((n_items, n - 1), dtype=torch.int32, device=cache.device)
+    _run("kv4_load", lib().bf_kv4_load, _ptr(cache), _ptr(block_tables), _c_int(block_tables.stride(0)),
+         _c_int(block_tables.shape[0]), _c_int(block_tables.shape[1]), _ptr(items), _c_int(n_items), _ptr(k),
+         _ptr(v), _ptr(tables), _ptr(items_out), _c_int(n), _c_int(nkv), _c_int(d), _c_int(ps),
+         _c_int(pages), _c_int(window), _c_int(keep_first), _ptr(err), _stream())
+    return k, v, tables
+
+
+def _kv4_mask(what: str, window: Optional[int], keep_first: int) -> Tuple[int, int]:
+    if (window is not None and window < 1) or keep_first < 0:
+        raise KernelError(f"{what}: a window has at least one key, keep_first is not negative")
+    return (int(window), int(keep_first)) if window is not None else (0, 0)
+
+
+def _kv4_attention_check(what, q, cache, block_tables, out, nh, nkv, d, window, keep_first, err, *others):
+    _want_int_table(block_tables, what, "block_tables")
+    _want(err, torch.int32, "err")
+    pages, c_nkv, ps, c_d = _kv4_check(what, cache, q, block_tables, out, err, *others)
+    if (c_nkv, c_d) != (nkv, d) or nh < 1 or nh % nkv:
+        raise KernelError(f"{what}: the cache has {c_nkv} heads of {c_d}, the call names {nkv} of {d} for "
+                          f"{nh} query heads")
+    for name, t in (("q", q), ("out", out)):
+        if (t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape[1] != nh * d or t.stride(1) != 1
+                or t.stride(0) % 8 or t.data_ptr() % 16):
+            raise KernelError(f"{what}: {name} must be bfloat16 [T, heads * d], rows contiguous and on "
+                              "16-byte boundaries")
+    if out.shape[0] < q.shape[0]:
+        raise KernelError(f"{what}: out has fewer rows than q")
+    return (pages, ps) + _kv4_mask(what, window, keep_first)
+
+
+def kv4_decode_attention(q: torch.Tensor, cache: torch.Tensor, rows: Optional[torch.Tensor], n_rows: int,
+                         seq_of_token: torch.Tensor, positions: torch.Tensor, block_tables: torch.Tensor,
+                         out: torch.Tensor, nh: int, nkv: int, d: int, window: Optional[int], scale: float,
+                         err: torch.Tensor, keep_first: int = 0) -> None:
+    """Attention over a cache in 4 bits for rows that bring one token each: ``decode_attention``'s
+    arguments, with ``cache`` (``kv4_cache``) in the pages' place.  A row at position p sees the keys
+    ``j <= p`` of its request; with ``window`` those with ``j > p - window``, and the first ``keep_first``
+    tokens.  ``rows`` lists the token rows to run (None: 0 .. n_rows - 1); other rows of ``out`` are left
+    as they were.  A page id outside the pool sets the error word and its keys are left out."""
+    _want(seq_of_token, torch.int32, "seq_of_token"); _want(positions, torch.int32, "positions")
+    if rows is not None:
+        _want(rows, torch.int32, "rows")
+    pages, ps, w, keep = _kv4_attention_check("kv4_decode_attention", q, cache, block_tables, out, nh, nkv,
+                                              d, window, keep_first, err, rows, seq_of_token, positions)
+    T = q.shape[0]
+    if (n_rows < 0 or (rows is None and n_rows > T) or (rows is not None and rows.numel() < n_rows)
+            or seq_of_token.numel() < T or positions.numel() < T):
+        raise KernelError("kv4_decode_attention: a request and a position per token row, and rows inside q")
+    if n_rows == 0:
+        return
+    _kv4_attention(q, cache, rows, seq_of_token, positions, None, n_rows, 1, block_tables, out, nh, nkv, d,
+                   ps, pages, w, keep, scale, err)
+
+
+def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Tensor, n_items: int,
+                          max_rows: int, block_tables: torch.Tensor, out: torch.Tensor, nh: int, nkv: int,
+                          d: int, window: Optional[int], scale: float, err: torch.Tensor, ctx_rows: int,
+                          max_ctx: int, keep_first: int = 0) -> None:
+    """Causal attention of prompt portions over a cache in 4 bits, their own keys included:
+    ``prefill_attention``'s arguments, with ``cache`` (``kv4_cache``) in the pages' place.  ``ctx_rows``:
+    the portions' contexts added up, each rounded up to 64; ``max_ctx``: the longest of them;
+    ``keep_first``: with a window, the request's first that many tokens stay visible behind it."""
+    _want(items, torch.int32, "items")
+    pages, ps, w, keep = _kv4_attention_check("kv4_prefill_attention", q, cache, block_tables, out, nh, nkv,
+                                              d, window, keep_first, err, items)
+    if n_items < 0 or items.numel() < 4 * n_items or max_rows < 0 or ctx_rows < 0 or ctx_rows % 64:
+        raise KernelError("kv4_prefill_attention: items must be [n_items, 4], ctx_rows a multiple of 64")
+    if n_items == 0 or max_rows == 0:
+        return
+    _kv4_attention(q, cache, None, None, None, items, n_items, max_rows, block_tables, out, nh, nkv, d, ps,
+                   pages, w, keep, scale, err)
+
+
+def _kv4_attention(q, cache, rows, seq_of_token, positions, items, n, max_rows, block_tables, out, nh, nkv, d,
+                   ps, pages, window, keep, scale, err):
+    _run("kv4_attention", lib().bf_kv4_attention, _ptr(q), _c_ll(q.stride(0)), _ptr(cache), _ptr(rows),
+         _ptr(seq_of_token), _ptr(positions), _ptr(items), _c_int(n), _c_int(max_rows), _c_int(q.shape[0]),
+         _ptr(block_tables), _c_int(block_tables.stride(0)), _c_int(block_tables.shape[0]),
+         _c_int(block_tables.shape[1]), _ptr(out), _c_ll(out.stride(0)), _c_int(nh), _c_int(nkv), _c_int(d),
+         _c_int(ps), _c_int(pages), _c_int(window), _c_int(keep), _c_float(scale), _ptr(err), _stream())
+
+
+# ------------------------------------------------------------- a step's description
+def step_tables(master: torch.Tensor, entries: torch.Tensor, new_pages: torch.Tensor, page_size: int,
+                num_pages: int, q_start: torch.Tensor, positions: torch.Tensor, seq_of_token: torch.Tensor,
+                ctx_lens: torch.Tensor, slots: torch.Tensor, tables: torch.Tensor, err: torch.Tensor,
+                decode_rows: Optional[torch.Tensor] = None,
+                prefill_items: Optional[torch.Tensor] = None) -> None:
+    """Describe a step's batch on the device, from its requests' lengths and pages.
+
+    ``entries`` int32 ``[B, 5]``, one per request: (its row of ``master``, its cached tokens, the tokens it
+    brings, the pages its row holds already, where its newly given pages begin in ``new_pages``); no row
+    appears twice, a negative one is a padding entry that reads and writes the scratch page 0.  ``master``
+    int32 ``[requests, places]`` keeps every request's page ids and is extended by the new ones.
+
+    Written (int32): ``q_start [B + 1]`` (first token row of each entry, and their number), ``ctx_lens [B]``
+    (tokens cached after the step), per token ``positions``, ``seq_of_token`` (its entry) and ``slots``
+    (its place in the pool), ``tables [B, width]`` (the pages of each entry, then zeros), and where given
+    ``decode_rows`` (rows of entries that bring one token) and ``prefill_items [n, 4]`` (entry, first token
+    row, tokens, first position) of those that bring more.  Places behind the last token or item are left
+    as they were.  An entry that does not fit (a row, page, place or token outside of what it is given)
+    sets the error word; its table is zero, its slots are -1."""
+    _want_int_table(master, "step_tables", "master")
+    for name, t in (("master", master), ("entries", entries), ("new_pages", new_pages), ("q_start", q_start),
+                    ("positions", positions), ("seq_of_token", seq_of_token), ("ctx_lens", ctx_lens),
+                    ("slots", slots), ("tables", tables), ("err", err)):
+        _want(t, torch.int32, name)
+    for name, t in (("decode_rows", decode_rows), ("prefill_items", prefill_items)):
+        if t is not None:
+            _want(t, torch.int32, name)
+    _same_device("step_tables", master, entries, new_pages, q_start, positions, seq_of_token, ctx_lens, slots,
+                 tables, err, decode_rows, prefill_items)
+    B = entries.shape[0]
+    if entries.dim() != 2 or entries.shape[1] != 5 or page_size < 1 or num_pages < 1:
+        raise KernelError("step_tables: entries must be [B, 5], pages of at least one token")
+    T = min(positions.numel(), seq_of_token.numel(), slots.numel())
+    if (tables.dim() != 2 or tables.shape[0] < B or q_start.numel() < B + 1 or ctx_lens.numel() < B
+            or num_pages * page_size > 1 << 31):
+        raise KernelError("step_tables: tables must be [B, width], q_start [B + 1], ctx_lens [B], and a "
+                          "slot a 32-bit number")
+    if B == 0:
+        return
+    n_dec = decode_rows.numel() if decode_rows is not None else 0
+    n_pf = prefill_items.numel() // 4 if prefill_items is not None else 0
+    _run("step_tables", lib().bf_step_tables, _ptr(master), _c_int(master.shape[0]), _c_int(master.shape[1]),
+         _ptr(entries), _c_int(B), _ptr(new_pages), _c_int(new_pages.numel()), _c_int(page_size),
+         _c_int(num_pages), _ptr(q_start), _ptr(positions), _ptr(seq_of_token), _ptr(ctx_lens), _ptr(slots),
+         _c_int(T), _ptr(tables), _c_int(tables.shape[1]), _ptr(decode_rows), _c_int(n_dec),
+         _ptr(prefill_items), _c_int(n_pf), _ptr(err), _stream())
+
+
 class DiffCombine:
     """What the differential attention kernels do with a head's two maps, besides attending:
     ``o = a1 - lam a2``, ``o <- o / sqrt(mean(o^2) + eps) * out_factor``, times the sigmoid of

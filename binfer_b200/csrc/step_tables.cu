@@ -1,0 +1,109 @@
+// What a step's kernels need to know of its batch, from the requests' lengths and their pages.
+//
+// Entry b of a step is (row, start, count, held, off): the request's row of the page table `master`
+// (negative: a padding entry, whose pages are all the scratch page 0), its cached tokens, the tokens it
+// brings, how many pages its master row holds already, and where its newly given pages begin in
+// `new_pages`.  The entry needs ceil((start + count) / page_size) pages; those from `held` on are new and
+// go into the master row too.  Token i of the entry has position start + i and lies at slot
+// page[p / page_size] page_size + p % page_size.  An entry that brings one token is a decode row, one that
+// brings more a prompt portion (b, first token row, count, start).
+//
+// One launch: block (b, y) sums the counts before b by itself and takes every gridDim.y-th stretch of b's
+// table and tokens.  A new page is always read from `new_pages`, so no block waits for another's write.
+#include "common.cuh"
+
+#define ST_THREADS 128
+
+__global__ void __launch_bounds__(ST_THREADS)
+step_tables_kernel(int* __restrict__ master, int master_rows, int master_width,
+                   const int* __restrict__ entries, int B, const int* __restrict__ new_pages, int n_new,
+                   int page_size, int num_pages, int* __restrict__ q_start, int* __restrict__ positions,
+                   int* __restrict__ seq, int* __restrict__ ctx_lens, int* __restrict__ slots, int T,
+                   int* __restrict__ tables, int width, int* __restrict__ decode_rows, int n_decode,
+                   int* __restrict__ items, int n_items, int* __restrict__ err) {
+  __shared__ long long sums[3][ST_THREADS / 32];
+  const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int* e = entries + 5 * (size_t)b;
+  int row = e[0];
+  const int start = e[1], count = max(e[2], 0), held = e[3], off = e[4];
+  long long tok = 0, dec = 0, por = 0;                      // tokens, decode rows and portions before b
+  for (int i = threadIdx.x; i < b; i += ST_THREADS) {
+    const int n = max(entries[5 * (size_t)i + 2], 0);
+    tok += n, dec += n == 1, por += n > 1;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    tok += __shfl_xor_sync(0xffffffffu, tok, o);
+    dec += __shfl_xor_sync(0xffffffffu, dec, o);
+    por += __shfl_xor_sync(0xffffffffu, por, o);
+  }
+  if (lane == 0) sums[0][warp] = tok, sums[1][warp] = dec, sums[2][warp] = por;
+  __syncthreads();
+  tok = dec = por = 0;
+#pragma unroll
+  for (int w = 0; w < ST_THREADS / 32; ++w) tok += sums[0][w], dec += sums[1][w], por += sums[2][w];
+
+  const bool padding = row < 0;
+  bool bad = start < 0 || held < 0 || row >= master_rows || tok + count > T;
+  const int need = padding ? 0 : (int)(((long long)start + count + page_size - 1) / page_size);
+  bad |= need > width || need > master_width || (need > held && ((long long)off + need - held > n_new || off < 0));
+  if (bad) {                                                // nothing of this entry can be described
+    if (threadIdx.x == 0 && blockIdx.y == 0) atomicOr(err, BF_ERR_PAGE);
+  }
+  if (threadIdx.x == 0 && blockIdx.y == 0) {
+    q_start[b] = (int)tok;
+    if (b == B - 1) q_start[B] = (int)(tok + count);
+    ctx_lens[b] = start + count;
+    if (count == 1 && decode_rows && dec < n_decode) decode_rows[dec] = (int)tok;
+    if (count > 1 && items && por < n_items) {
+      items[4 * por] = b, items[4 * por + 1] = (int)tok;
+      items[4 * por + 2] = count, items[4 * por + 3] = start;
+    }
+    if ((count == 1 && decode_rows && dec >= n_decode) || (count > 1 && items && por >= n_items))
+      atomicOr(err, BF_ERR_PAGE);
+  }
+  auto page_at = [&](int w) {                               // w < need
+    return w < held ? master[(size_t)row * master_width + w] : new_pages[off + w - held];
+  };
+  const int first = blockIdx.y * ST_THREADS + threadIdx.x, step = gridDim.y * ST_THREADS;
+  for (int w = first; w < width; w += step) {
+    int id = 0;
+    if (!bad && w < need) {
+      id = page_at(w);
+      if (w >= held) master[(size_t)row * master_width + w] = id;
+    }
+    tables[(size_t)b * width + w] = id;
+  }
+  for (int i = first; i < count; i += step) {
+    const long long t = tok + i;
+    if (t >= T) break;
+    const int p = start + i;
+    int slot = -1;
+    if (!bad) {
+      const int id = padding ? 0 : page_at(p / page_size);
+      if (id < 0 || id >= num_pages) {
+        atomicOr(err, BF_ERR_PAGE);
+      } else {
+        slot = id * page_size + p % page_size;
+      }
+    }
+    positions[t] = p;
+    seq[t] = b;
+    slots[t] = slot;
+  }
+}
+
+BF_EXPORT int bf_step_tables(int* master, int master_rows, int master_width, const int* entries, int B,
+                             const int* new_pages, int n_new, int page_size, int num_pages, int* q_start,
+                             int* positions, int* seq, int* ctx_lens, int* slots, int T, int* tables,
+                             int width, int* decode_rows, int n_decode, int* items, int n_items, int* err,
+                             cudaStream_t stream) {
+  if (B <= 0) return 0;
+  // a block's share: up to about 512 places of a table, or tokens if portions are long
+  const int per = width > T / B ? width : T / B;
+  const int parts = per <= 512 ? 1 : per / 512 > 16 ? 16 : (per + 511) / 512;
+  step_tables_kernel<<<dim3(B, parts), ST_THREADS, 0, stream>>>(
+      master, master_rows, master_width, entries, B, new_pages, n_new, page_size, num_pages, q_start,
+      positions, seq, ctx_lens, slots, T, tables, width, decode_rows, n_decode, items, n_items, err);
+  return bf_launch_status();
+}

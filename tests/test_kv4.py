@@ -1,0 +1,107 @@
+"""What the operators of a cache held in 4 bits refuse, before anything reaches a GPU."""
+import pytest
+import torch
+
+BF16, I32 = torch.bfloat16, torch.int32
+
+
+@pytest.fixture
+def ops():
+    from binfer_b200.csrc import ops
+    return ops
+
+
+def _i(*shape):
+    return torch.zeros(shape, dtype=I32)
+
+
+def test_cache_layout(ops):
+    c = ops.kv4_cache(5, 2, 16, 128, "cpu")
+    assert tuple(c.shape) == (5, 2, 2, 1152) and c.dtype == torch.uint8 and not c.any()
+    assert ops.kv4_takes(BF16, 128, 16) and not ops.kv4_takes(torch.float32, 128, 16)
+    for d, ps in ((96, 16), (32, 16), (128, 4), (128, 24), (128, 256), (128, 17)):
+        assert not ops.kv4_takes(BF16, d, ps)
+        with pytest.raises(ops.KernelError):
+            ops.kv4_cache(5, 2, ps, d, "cpu")
+    for pages, heads in ((0, 1), (1, 0)):
+        with pytest.raises(ops.KernelError):
+            ops.kv4_cache(pages, heads, 16, 128, "cpu")
+
+
+def test_no_cpu_path(ops):
+    c, k = ops.kv4_cache(3, 1, 16, 64, "cpu"), torch.zeros((2, 64), dtype=BF16)
+    with pytest.raises(ops.KernelError, match="CUDA"):
+        ops.kv4_store(k, k, _i(2), c, _i(1))
+    with pytest.raises(ops.KernelError, match="CUDA"):
+        ops.kv4_load(c, _i(1, 2), _i(1, 4), 1, 64, _i(1))
+    with pytest.raises(ops.KernelError, match="CUDA"):
+        ops.kv4_decode_attention(k, c, None, 2, _i(2), _i(2), _i(1, 2), k, 1, 1, 64, None, 1.0, _i(1))
+    with pytest.raises(ops.KernelError, match="CUDA"):
+        ops.kv4_prefill_attention(k, c, _i(1, 4), 1, 2, _i(1, 2), k, 1, 1, 64, None, 1.0, _i(1), 64, 2)
+    with pytest.raises(ops.KernelError, match="CUDA"):
+        ops.step_tables(_i(2, 4), _i(1, 5), _i(1), 16, 8, _i(2), _i(1), _i(1), _i(1), _i(1), _i(1, 4), _i(1))
+
+
+def _store_args(ops):
+    return dict(k=torch.zeros((2, 128), dtype=BF16), v=torch.zeros((2, 128), dtype=BF16), slots=_i(2),
+                cache=ops.kv4_cache(3, 2, 16, 64, "cpu"), err=_i(1))
+
+
+@pytest.mark.parametrize("change", [dict(k=torch.zeros((2, 128))), dict(v=torch.zeros((3, 128), dtype=BF16)),
+                                    dict(k=torch.zeros((128, 2), dtype=BF16).T), dict(slots=_i(2).long()),
+                                    dict(k=torch.zeros((2, 2, 64), dtype=BF16)), dict(err=torch.zeros(1)),
+                                    dict(cache=torch.zeros((3, 2, 2, 576), dtype=torch.int8)),
+                                    dict(cache=torch.zeros((3, 2, 2, 575), dtype=torch.uint8)),
+                                    dict(cache=torch.zeros((3, 2, 3, 576), dtype=torch.uint8)),
+                                    dict(cache=torch.zeros((6, 2, 576), dtype=torch.uint8)),
+                                    dict(cache=torch.zeros((3, 2, 4, 576), dtype=torch.uint8)[:, :, ::2])])
+def test_store_refuses(ops, change):
+    with pytest.raises(ops.KernelError) as e:
+        ops.kv4_store(**dict(_store_args(ops), **change))
+    assert "CPU path" not in str(e.value)
+
+
+def _attention_args(ops):
+    q = torch.zeros((3, 256), dtype=BF16)
+    return dict(q=q, cache=ops.kv4_cache(3, 2, 16, 64, "cpu"), block_tables=_i(2, 4), out=torch.zeros_like(q),
+                nh=4, nkv=2, d=64, window=None, scale=0.1, err=_i(1))
+
+
+@pytest.mark.parametrize("change", [dict(block_tables=_i(2, 4).long()), dict(block_tables=_i(8)),
+                                    dict(block_tables=_i(4, 2).T), dict(err=torch.zeros(1, dtype=torch.int64))])
+def test_attention_refuses(ops, change):
+    args = dict(_attention_args(ops), **change)
+    decode = dict(rows=None, n_rows=3, seq_of_token=_i(3), positions=_i(3))
+    with pytest.raises(ops.KernelError) as e:
+        ops.kv4_decode_attention(**args, **decode)
+    assert "CPU path" not in str(e.value)
+    with pytest.raises(ops.KernelError) as e:
+        ops.kv4_prefill_attention(**args, items=_i(1, 4), n_items=1, max_rows=3, ctx_rows=64, max_ctx=3)
+    assert "CPU path" not in str(e.value)
+
+
+@pytest.mark.parametrize("change", [dict(seq_of_token=_i(3).long()), dict(positions=torch.zeros(3)),
+                                    dict(rows=torch.zeros(3))])
+def test_decode_attention_refuses(ops, change):
+    args = dict(_attention_args(ops), rows=None, n_rows=3, seq_of_token=_i(3), positions=_i(3))
+    with pytest.raises(ops.KernelError, match="must be"):
+        ops.kv4_decode_attention(**dict(args, **change))
+
+
+def test_items_are_int32(ops):
+    with pytest.raises(ops.KernelError, match="items"):
+        ops.kv4_prefill_attention(**_attention_args(ops), items=_i(1, 4).long(), n_items=1, max_rows=3, ctx_rows=64,
+                                  max_ctx=3)
+    with pytest.raises(ops.KernelError, match="items"):
+        ops.kv4_load(ops.kv4_cache(3, 1, 16, 64, "cpu"), _i(1, 2), torch.zeros((1, 4)), 1, 64, _i(1))
+
+
+@pytest.mark.parametrize("name", ["master", "entries", "new_pages", "q_start", "positions", "seq_of_token",
+                                  "ctx_lens", "slots", "tables", "err", "decode_rows", "prefill_items"])
+def test_step_tables_takes_int32(ops, name):
+    args = dict(master=_i(2, 4), entries=_i(1, 5), new_pages=_i(1), page_size=16, num_pages=8, q_start=_i(2),
+                positions=_i(1), seq_of_token=_i(1), ctx_lens=_i(1), slots=_i(1), tables=_i(1, 4), err=_i(1),
+                decode_rows=_i(1), prefill_items=_i(0, 4))
+    args[name] = args[name].long()
+    with pytest.raises(ops.KernelError, match="int32"):
+        ops.step_tables(**args)
