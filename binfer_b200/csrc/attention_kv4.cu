@@ -1,83 +1,672 @@
-// Attention over pages held in 4 bits (layout: kv4.cuh): a warp per (token row, query head).
+// Attention over pages held in 4 bits (layout: kv4.cuh), for rows that bring one token each and for
+// prompt portions of a few rows.
+//
+// With k_j = m_j + s_j c_j and v_j likewise (s, m per 64 numbers, codes c of 0 to 15),
+//
+//   q . k_j     = sum over groups of  s_j (q . c_j) + m_j sum(q)
+//   sum p_j v_j = sum over groups of  (p_j s_j) . c_j + sum p_j m_j ,
+//
+// so the codes go into the tensor cores as they are and scales and lowest values meet sums only.  A code
+// becomes a bfloat16 operand by a mask alone: the bits 0 .. 7 of a bfloat16 number whose other bits are zero
+// count steps of 2^-133 (subnormal numbers and the first binade above them), and the tensor cores take
+// them as they are.  So (word & 0x000f000f) is two codes, (word & 0x00f000f0) the two beside them times 16,
+// and one shift by 8 gives the other four of eight: five instructions for four operand registers.  Queries
+// and probabilities carry the factor 2^64 (and 2^-4 against the codes times 16), the sums 2^69.
+//
+// Rounding: the probabilities times the value scales go into their product as bfloat16.  Their error meets
+// the codes less 8, since 8 times the sum of the rounded products is taken off again and p (m + 8 s) added
+// in float.  Everything else is float.
+//
+// Work.  A tile is up to 8 NT columns, a column one query head of one token row; its keys go sixteen at a
+// time (a unit), for every kv head.  All units of a call in one row are cut into equal stretches, one a
+// CTA, so that the chip is full whatever the contexts are; the eight warps of a CTA take the units of a tile
+// and head in turn, each with a running maximum of its own, and meet once at its end.  What a CTA does
+// not finish (at most the first and the last tile of its stretch) leaves as a partial result, which a second
+// kernel adds up; scratch is two partials a CTA whatever the contexts are.  A warp fetches its units by
+// itself (16 bytes a lane, asynchronously, three units ahead of the one it computes), so no warp waits
+// for another inside a tile.  The running maximum moves only when a score passes it by 2^8, which no
+// result depends on beyond rounding and which leaves one vote a unit where maxima would take six shuffles.
 #include "common.cuh"
 #include "kv4.cuh"
+#include "mma_utils.cuh"
 
-template <int D>
-__global__ void __launch_bounds__(128)
-kv4_attention_kernel(const __nv_bfloat16* __restrict__ q, long long q_stride, const unsigned char* __restrict__ cache,
-                     const int* __restrict__ rows, const int* __restrict__ seq_of_token,
-                     const int* __restrict__ positions, const int* __restrict__ items,
-                     const int* __restrict__ block_tables, int table_stride, int table_rows,
-                     int table_width, int T, __nv_bfloat16* __restrict__ out, long long out_stride, int nh, int nkv, int page_size, int num_pages,
-                     int window, int keep, float scale, int* __restrict__ err) {
-  constexpr int N = D / 32, NG = D / KV4_GROUP, REC = kv4_record(D);
-  const int lane = threadIdx.x & 31, head = blockIdx.y * 4 + (threadIdx.x >> 5);
-  if (head >= nh) return;
-  int t, b, p;
-  if (items) {
-    const int* it = items + 4 * blockIdx.z;
-    if ((int)blockIdx.x >= it[2]) return;
-    t = it[1] + blockIdx.x, b = it[0], p = it[3] + blockIdx.x;
-  } else {
-    t = rows ? rows[blockIdx.x] : blockIdx.x;
-    const int ok = t >= 0 && t < T;
-    b = ok ? seq_of_token[t] : -1, p = ok ? positions[t] : 0;
+#define KA_WARPS 8
+#define KA_THREADS (KA_WARPS * 32)
+#define KA_STAGES 4
+#define KA_MAX_TILES 512                   // of one launch
+#define KA_UNIT 16                         // keys
+#define KA_MIN_UNITS 8                     // a CTA's share at least, where there is so much
+
+struct KaArgs {
+  const __nv_bfloat16* q;
+  long long q_stride;
+  const unsigned char* cache;
+  const int *rows, *seq_of_token, *positions, *items;
+  int first_tile, n_tiles, tiles_per_item, T;
+  const int* block_tables;
+  int table_stride, table_rows, table_width;
+  __nv_bfloat16* out;
+  long long out_stride;
+  int nh, nkv, group, chunk, chunks, tokens;               // query heads per kv head; in a tile; chunks of them
+  int page_size, num_pages, window, keep;
+  float scale;
+  float* part_o;
+  float2* part_ml;
+  int4* desc;
+  int* err;
+};
+
+struct KaTile {
+  int b, row0, pos0, ntok;
+};
+
+// Units of a tile: sixteen keys each, those of the kept first tokens, then from the window's first on.
+struct KaSpan {
+  int kept, from, units;
+};
+__device__ __forceinline__ KaSpan ka_span(const KaTile& t, int window, int keep) {
+  KaSpan s = {0, 0, 0};
+  if (t.ntok <= 0) return s;
+  if (window > 0) {
+    s.from = max(0, t.pos0 - window + 1) / KA_UNIT;
+    s.kept = min((keep + KA_UNIT - 1) / KA_UNIT, s.from);
   }
-  if (t < 0 || t >= T || b < 0 || b >= table_rows) {
-    if (lane == 0) atomicOr(err, BF_ERR_PAGE);
-    return;
-  }
-  const int h = head / (nh / nkv), i0 = lane * N, g = i0 / 64;
-  float qf[N], o[N], m = -INFINITY, l = 0.f;
-  for (int e = 0; e < N; ++e) qf[e] = __bfloat162float(q[t * q_stride + head * D + i0 + e]), o[e] = 0.f;
-  for (int j = 0; j <= p; ++j) {
-    if (window > 0 && j <= p - window && j >= keep) {
-      j = p - window;
-      continue;
-    }
-    const int at = j / page_size;
-    const int page = at < table_width ? block_tables[(size_t)b * table_stride + at] : -1;
-    if (page < 0 || page >= num_pages) {
-      if (lane == 0) atomicOr(err, BF_ERR_PAGE);
-      continue;
-    }
-    const int off = j % page_size, tok = off % 8;
-    const unsigned char* rec = cache + (((size_t)page * nkv + h) * (page_size / 8) + off / 8) * REC;
-    const unsigned kp = *reinterpret_cast<const unsigned*>(rec + kv4_key_params_at(D) + (tok * NG + g) * 4);
-    const unsigned vp = *reinterpret_cast<const unsigned*>(rec + kv4_value_params_at(D) + (tok * NG + g) * 4);
-    float s = 0.f;
-    for (int e = 0; e < N; ++e) {
-      const int c = rec[kv4_key_byte(D, tok, i0 + e)] >> ((i0 + e) % 2 * 4) & 15;
-      s += qf[e] * fmaf(kv4_scale(kp), (float)c, kv4_low(kp));
-    }
-    s = warp_sum(s) * scale;
-    const float mn = fmaxf(m, s), f = mn == m ? 1.f : __expf(m - mn), w = __expf(s - mn);
-    l = l * f + w;
-    for (int e = 0; e < N; ++e) {
-      const int c = rec[kv4_value_byte(D, tok, i0 + e)] >> ((i0 + e) % 2 * 4) & 15;
-      o[e] = o[e] * f + w * fmaf(kv4_scale(vp), (float)c, kv4_low(vp));
-    }
-    m = mn;
-  }
-  for (int e = 0; e < N; ++e) out[t * out_stride + head * D + i0 + e] = __float2bfloat16_rn(o[e] / l);
+  s.units = (t.pos0 + t.ntok - 1) / KA_UNIT - s.from + 1 + s.kept;
+  return s;
 }
 
-BF_EXPORT int bf_kv4_attention(const void* q, long long q_stride, const void* cache, const int* rows, const int* seq_of_token,
-                               const int* positions, const int* items, int n, int max_rows, int T,
-                               const int* block_tables, int table_stride, int table_rows, int table_width,
-                               void* out, long long out_stride,
-                               int nh, int nkv, int d, int page_size, int num_pages, int window, int keep,
-                               float scale, int* err, cudaStream_t stream) {
+__device__ __forceinline__ float ka_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ unsigned ka_transpose(unsigned x) {
+  unsigned y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+template <int WORDS>
+__device__ __forceinline__ void ka_lds(unsigned (&w)[WORDS], const unsigned char* p) {
+  if constexpr (WORDS >= 4) {
+#pragma unroll
+    for (int i = 0; i < WORDS / 4; ++i) {
+      const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+      w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+    }
+  } else if constexpr (WORDS == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+    w[0] = *reinterpret_cast<const unsigned*>(p);
+  }
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(KA_THREADS, (D <= 128 && NT == 1) ? 2 : 1)
+kv4_attention_kernel(const __grid_constant__ KaArgs a) {
+  constexpr int NG = D / KV4_GROUP, REC = kv4_record(D), UNIT_BYTES = 2 * REC;
+  constexpr int KW = D / 32, COLS = 8 * NT;
+  constexpr float UP = 1.8446744073709551616e19f;           // 2^64
+  constexpr float DOWN = 5.90295810358705651712e20f;        // 2^69
+  constexpr unsigned M0 = 0x000f000fu, M4 = 0x00f000f0u, ONES = 0x00010001u;
+  extern __shared__ __align__(128) unsigned char smem[];
+  unsigned char* ring = smem;                               // also the warps' results at a tile's end
+  float* merge_o = reinterpret_cast<float*>(smem);          // [warps][COLS][D]
+  unsigned char* after = smem + (size_t)KA_WARPS * KA_STAGES * UNIT_BYTES;
+  long long* start = reinterpret_cast<long long*>(after);   // [KA_MAX_TILES + 1]
+  KaTile* tiles = reinterpret_cast<KaTile*>(start + KA_MAX_TILES + 2);
+  float2* merge_ml = reinterpret_cast<float2*>(tiles + KA_MAX_TILES);      // [warps][COLS]
+  __shared__ long long warp_sum_of[KA_WARPS];
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int r = lane >> 2, q4 = lane & 3;
+  const int pairs = a.nkv * a.chunks;
+  bf_pdl_trigger();
+  bf_pdl_wait();
+
+  // tiles and where their units begin
+  long long running = 0;
+  for (int e0 = 0; e0 < a.n_tiles; e0 += KA_THREADS) {
+    const int e = e0 + tid;
+    KaTile t = {0, 0, 0, 0};
+    if (e < a.n_tiles) {
+      if (a.items) {
+        const int id = a.first_tile + e, i = id / a.tiles_per_item, s = id - i * a.tiles_per_item;
+        const int* it = a.items + 4 * (size_t)i;
+        t.b = it[0];
+        t.row0 = it[1] + s * a.tokens;
+        t.pos0 = it[3] + s * a.tokens;
+        t.ntok = min(it[2] - s * a.tokens, a.tokens);
+      } else {
+        const int n = a.first_tile + e;
+        t.row0 = a.rows ? a.rows[n] : n;
+        const bool ok = t.row0 >= 0 && t.row0 < a.T;
+        t.b = ok ? a.seq_of_token[t.row0] : -1;
+        t.pos0 = ok ? a.positions[t.row0] : 0;
+        t.ntok = 1;
+      }
+      if (t.ntok > 0 && (t.b < 0 || t.b >= a.table_rows || t.row0 < 0 || t.row0 + t.ntok > a.T || t.pos0 < 0)) {
+        if (blockIdx.x == 0) atomicOr(a.err, BF_ERR_PAGE);
+        t.ntok = 0;
+      }
+      tiles[e] = t;
+    }
+    const long long n = (long long)ka_span(t, a.window, a.keep).units * pairs;
+    long long incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    if (lane == 31) warp_sum_of[warp] = incl;
+    __syncthreads();
+    long long before = running;
+    for (int w = 0; w < KA_WARPS; ++w) {
+      if (w < warp) before += warp_sum_of[w];
+      running += warp_sum_of[w];
+    }
+    if (e < a.n_tiles) {
+      start[e] = before + incl - n;
+      if (n == 0 && blockIdx.x == 0)
+        for (int i = 0; i < pairs; ++i) a.desc[(size_t)e * pairs + i] = make_int4(-1, -1, 0, 0);
+    }
+    __syncthreads();
+  }
+  if (tid == 0) start[a.n_tiles] = running;
+  __syncthreads();
+  const long long total = running;
+  long long parts = total / KA_MIN_UNITS;
+  parts = parts < 1 ? 1 : parts > gridDim.x ? gridDim.x : parts;
+  const long long cta = blockIdx.x;
+  if (cta >= parts || total == 0) return;
+  long long x = cta * total / parts;
+  const long long x_end = (cta + 1) * total / parts;
+
+  int e;                                                    // the tile that holds unit x
+  {
+    int lo = 0, hi = a.n_tiles - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (start[mid] <= x) lo = mid; else hi = mid - 1;
+    }
+    e = lo;
+  }
+  const float scale_log2 = a.scale * 1.44269504088896341f;
+  const float score_up = scale_log2 * DOWN;
+  const int eighths = a.page_size / KV4_EIGHTH;
+  unsigned char* my_ring = ring + (size_t)warp * KA_STAGES * UNIT_BYTES;
+
+  while (x < x_end) {
+    while (start[e + 1] <= x) ++e;
+    const KaTile t = tiles[e];
+    const KaSpan span = ka_span(t, a.window, a.keep);
+    const long long rel = x - start[e];
+    const int pair = (int)(rel / span.units), u0 = (int)(rel % span.units);
+    const int u1 = (int)(x_end - x < span.units - u0 ? u0 + (x_end - x) : span.units);
+    const int h = pair / a.chunks, head0 = h * a.group + (pair - h * a.chunks) * a.chunk;
+    const int heads = min(a.chunk, (h + 1) * a.group - head0);
+    const int last = t.pos0 + t.ntok - 1;
+    const int first_seen = a.window > 0 ? max(0, t.pos0 - a.window + 1) : 0;
+    const int* table = a.block_tables + (size_t)t.b * a.table_stride;
+    x += u1 - u0;
+
+    // ---- units of this warp: u0 + warp, u0 + warp + 8, ...
+    const int mine = u1 - u0 > warp ? (u1 - u0 - warp + KA_WARPS - 1) / KA_WARPS : 0;
+    auto unit_key = [&](int i) {
+      const int u = u0 + warp + i * KA_WARPS;
+      return (u < span.kept ? u : span.from + u - span.kept) * KA_UNIT;
+    };
+    int rec0 = 0, rec1 = 0;                                 // of unit (32 n + lane): its two records
+    auto look_up = [&](int i) {
+      rec0 = rec1 = 0;
+      if (i >= mine) return;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int j = unit_key(i) + half * 8;
+        int rec = 0;
+        if (kv4_seen(j, j + 7, t.pos0, last, a.window, a.keep)) {
+          const int at = j / a.page_size;
+          const int page = at < a.table_width ? table[at] : -1;
+          if (page < 0 || page >= a.num_pages) {
+            atomicOr(a.err, BF_ERR_PAGE);
+          } else {
+            rec = (page * a.nkv + h) * eighths + (j - at * a.page_size) / 8;
+          }
+        }
+        if (half) rec1 = rec; else rec0 = rec;
+      }
+    };
+    auto issue = [&](int i) {
+      if (i < mine) {
+        if ((i & 31) == 0) look_up(i + lane);
+        const unsigned char* s0 = a.cache + (size_t)__shfl_sync(0xffffffffu, rec0, i & 31) * REC;
+        const unsigned char* s1 = a.cache + (size_t)__shfl_sync(0xffffffffu, rec1, i & 31) * REC;
+        unsigned char* dst = my_ring + (i % KA_STAGES) * UNIT_BYTES;
+        s1 -= REC;
+#pragma unroll
+        for (int c0 = 0; c0 < UNIT_BYTES / 16; c0 += 32) {
+          const int c = c0 + lane;
+          if (c0 + 32 <= UNIT_BYTES / 16 || c < UNIT_BYTES / 16)
+            cp_async16(dst + c * 16, (c < REC / 16 ? s0 : s1) + c * 16, 16);
+        }
+      }
+      cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < KA_STAGES - 1; ++i) issue(i);
+
+    // ---- queries: operand b of the scores' product, and their sums per group
+    unsigned qf[NT][KW][4];
+    float qs[NT][NG][2];
+    int pcol[NT][2];
+    bool live[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int n = nt * 8 + r, ti = n / a.chunk, gi = n - ti * a.chunk;
+      const bool on = ti < t.ntok && gi < heads;
+      const __nv_bfloat16* src = a.q + (long long)(t.row0 + (on ? ti : 0)) * a.q_stride + (size_t)(head0 + (on ? gi : 0)) * D;
+      float sums[NG];
+#pragma unroll
+      for (int g = 0; g < NG; ++g) sums[g] = 0.f;
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+        uint4 raw = *reinterpret_cast<const uint4*>(src + (w >> 1) * 64 + q4 * 16 + (w & 1) * 8);
+        if (!on) raw = make_uint4(0, 0, 0, 0);
+        const unsigned* u = &raw.x;
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f[2 * i] = __uint_as_float(u[i] << 16);
+          f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sums[w >> 1] += f[i];
+        qf[nt][w][0] = pack_bf16(f[0] * UP, f[4] * UP);
+        qf[nt][w][1] = pack_bf16(f[1] * (UP / 16), f[5] * (UP / 16));
+        qf[nt][w][2] = pack_bf16(f[2] * UP, f[6] * UP);
+        qf[nt][w][3] = pack_bf16(f[3] * (UP / 16), f[7] * (UP / 16));
+      }
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 1);
+        sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 2);
+        qs[nt][g][0] = __shfl_sync(0xffffffffu, sums[g], q4 * 8) * scale_log2;
+        qs[nt][g][1] = __shfl_sync(0xffffffffu, sums[g], q4 * 8 + 4) * scale_log2;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int n2 = nt * 8 + 2 * q4 + i, t2 = n2 / a.chunk;
+        live[nt][i] = t2 < t.ntok;
+        pcol[nt][i] = t.pos0 + min(t2, t.ntok - 1);
+      }
+    }
+
+    float o[NT][D / 16][4], ps[NT][NG][4], corr[NT][NG][2], l[NT][2], m[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        ps[nt][g][0] = ps[nt][g][1] = ps[nt][g][2] = ps[nt][g][3] = 0.f;
+        corr[nt][g][0] = corr[nt][g][1] = 0.f;
+      }
+      l[nt][0] = l[nt][1] = 0.f;
+      m[nt][0] = m[nt][1] = -INFINITY;
+    }
+
+    for (int i = 0; i < mine; ++i) {
+      cp_async_wait<KA_STAGES - 2>();
+      __syncwarp();
+      issue(i + KA_STAGES - 1);
+      const unsigned char* s0 = my_ring + (i % KA_STAGES) * UNIT_BYTES;
+      const unsigned char* s1 = s0 + REC;
+      const int key0 = unit_key(i);
+
+      // scores of keys key0 + r and key0 + 8 + r against columns 2 q4, 2 q4 + 1 of every eight
+      float s[NT][4];
+      {
+        unsigned w0[KW], w1[KW], p0[NG], p1[NG];
+        ka_lds<KW>(w0, s0 + r * (D / 2) + q4 * (D / 8));
+        ka_lds<KW>(w1, s1 + r * (D / 2) + q4 * (D / 8));
+        ka_lds<NG>(p0, s0 + kv4_key_params_at(D) + r * NG * 4);
+        ka_lds<NG>(p1, s1 + kv4_key_params_at(D) + r * NG * 4);
+        float low[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+          low[nt][0] = low[nt][1] = low[nt][2] = low[nt][3] = 0.f;
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          float c[NT][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.f;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int w = 2 * g + half;
+            const unsigned a0[4] = {w0[w] & M0, w1[w] & M0, w0[w] & M4, w1[w] & M4};
+            const unsigned h0 = w0[w] >> 8, h1 = w1[w] >> 8;
+            const unsigned a1[4] = {h0 & M0, h1 & M0, h0 & M4, h1 & M4};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma_bf16_16816(c[nt], a0, qf[nt][w][0], qf[nt][w][1]);
+              mma_bf16_16816(c[nt], a1, qf[nt][w][2], qf[nt][w][3]);
+            }
+          }
+          const float sc0 = kv4_scale(p0[g]), sc1 = kv4_scale(p1[g]), lo0 = kv4_low(p0[g]), lo1 = kv4_low(p1[g]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            s[nt][0] += sc0 * c[nt][0];
+            s[nt][1] += sc0 * c[nt][1];
+            s[nt][2] += sc1 * c[nt][2];
+            s[nt][3] += sc1 * c[nt][3];
+            low[nt][0] += lo0 * qs[nt][g][0];
+            low[nt][1] += lo0 * qs[nt][g][1];
+            low[nt][2] += lo1 * qs[nt][g][0];
+            low[nt][3] += lo1 * qs[nt][g][1];
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) s[nt][k] = fmaf(s[nt][k], score_up, low[nt][k]);
+      }
+      // every key seen by every column: not so at the context's end and at the window's edges
+      const bool whole = key0 + KA_UNIT - 1 <= t.pos0 &&
+                         (a.window <= 0 || key0 > last - a.window || key0 + KA_UNIT <= a.keep);
+      unsigned hidden = 0;
+      if (!whole) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int j = key0 + r + (k >> 1) * 8, p = pcol[nt][k & 1];
+            if (j > p || (a.window > 0 && j <= p - a.window && j >= a.keep)) {
+              hidden |= 1u << (nt * 4 + k);
+              s[nt][k] = -INFINITY;
+            }
+          }
+      }
+      bool over = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) over |= fmaxf(s[nt][c], s[nt][c + 2]) > m[nt][c] + 8.f;
+      if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float top = fmaxf(s[nt][c], s[nt][c + 2]);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            top = fmaxf(top, m[nt][c]);
+            const float f = top == m[nt][c] ? 1.f : ka_exp2(m[nt][c] - top);
+            m[nt][c] = top;
+            l[nt][c] *= f;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+              corr[nt][g][c] *= f;
+              ps[nt][g][c] *= f;
+            }
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+              o[nt][d][c] *= f;
+              o[nt][d][c + 2] *= f;
+            }
+          }
+      }
+      {
+        unsigned v0[KW], v1[KW], p0[NG], p1[NG];
+        ka_lds<KW>(v0, s0 + kv4_values_at(D) + r * (D / 2) + q4 * (D / 8));
+        ka_lds<KW>(v1, s1 + kv4_values_at(D) + r * (D / 2) + q4 * (D / 8));
+        ka_lds<NG>(p0, s0 + kv4_value_params_at(D) + r * NG * 4);
+        ka_lds<NG>(p1, s1 + kv4_value_params_at(D) + r * NG * 4);
+        float p[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float top = m[nt][k & 1];
+            p[nt][k] = ka_exp2(s[nt][k] - (top == -INFINITY ? 0.f : top));
+          }
+          l[nt][0] += p[nt][0] + p[nt][2];
+          l[nt][1] += p[nt][1] + p[nt][3];
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const float sc0 = kv4_scale(p0[g]), sc1 = kv4_scale(p1[g]);
+          const float mid0 = fmaf(8.f, sc0, kv4_low(p0[g])), mid1 = fmaf(8.f, sc1, kv4_low(p1[g]));
+          const float up0 = sc0 * UP, up1 = sc1 * UP;
+          unsigned b0[NT], b1[NT];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float w[4] = {p[nt][0] * up0, p[nt][1] * up0, p[nt][2] * up1, p[nt][3] * up1};
+            float z[4] = {p[nt][0] * mid0, p[nt][1] * mid0, p[nt][2] * mid1, p[nt][3] * mid1};
+            if (hidden) {                                   // (a hidden key may be anything: 0 times it is not 0)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (hidden >> (nt * 4 + k) & 1) w[k] = z[k] = 0.f;
+            }
+            corr[nt][g][0] += z[0] + z[2];
+            corr[nt][g][1] += z[1] + z[3];
+            b0[nt] = ka_transpose(pack_bf16(w[0], w[1]));
+            b1[nt] = ka_transpose(pack_bf16(w[2], w[3]));
+            const unsigned ones[4] = {ONES, ONES, ONES, ONES};
+            mma_bf16_16816(ps[nt][g], ones, b0[nt], b1[nt]);
+          }
+          // eight numbers of this lane's part, for tokens 2 q4 and 2 q4 + 1 of either record
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const unsigned sel = half ? 0x7632 : 0x5410;
+            const unsigned x0 = __byte_perm(v0[g], v0[NG + g], sel), x1 = __byte_perm(v1[g], v1[NG + g], sel);
+            const unsigned h0 = x0 >> 8, h1 = x1 >> 8;
+            const unsigned a0[4] = {x0 & M0, x0 & M4, x1 & M0, x1 & M4};
+            const unsigned a1[4] = {h0 & M0, h0 & M4, h1 & M0, h1 & M4};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma_bf16_16816(o[nt][4 * g + 2 * half], a0, b0[nt], b1[nt]);
+              mma_bf16_16816(o[nt][4 * g + 2 * half + 1], a1, b0[nt], b1[nt]);
+            }
+          }
+        }
+      }
+    }
+    cp_async_wait<0>();
+    __syncthreads();                                        // the rings are free: the warps' results go there
+
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int n = nt * 8 + 2 * q4 + c;
+#pragma unroll
+        for (int k = 4; k < 32; k <<= 1) {
+          l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], k);
+#pragma unroll
+          for (int g = 0; g < NG; ++g) corr[nt][g][c] += __shfl_xor_sync(0xffffffffu, corr[nt][g][c], k);
+        }
+        if (r == 0) merge_ml[warp * COLS + n] = make_float2(m[nt][c], l[nt][c]);
+        if (!live[nt][c]) continue;
+        float* dst = merge_o + ((size_t)warp * COLS + n) * D + r * 8;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const float base = fmaf(-8.f * DOWN, ps[nt][g][c], corr[nt][g][c]);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const float* x0 = o[nt][4 * g + 2 * half];
+            const float* x1 = o[nt][4 * g + 2 * half + 1];
+            *reinterpret_cast<float4*>(dst + g * 64 + half * 4) =
+                make_float4(fmaf(x0[c], DOWN, base), fmaf(x0[c + 2], DOWN / 16, base),
+                            fmaf(x1[c], DOWN, base), fmaf(x1[c + 2], DOWN / 16, base));
+          }
+        }
+      }
+    __syncthreads();
+    const bool begins = u0 == 0, ends = u1 == span.units;
+    const int slot = (int)(2 * cta) + (begins ? 1 : 0);
+    for (int i = tid; i < COLS * (D / 4); i += KA_THREADS) {
+      const int n = i / (D / 4), d = (i - n * (D / 4)) * 4, ti = n / a.chunk, gi = n - ti * a.chunk;
+      if (ti >= t.ntok || gi >= heads) continue;
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < KA_WARPS; ++w) top = fmaxf(top, merge_ml[w * COLS + n].x);
+      float sum = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < KA_WARPS; ++w) {
+        const float2 ml = merge_ml[w * COLS + n];
+        const float f = ml.x == top ? 1.f : ka_exp2(ml.x - top);
+        const float4 v = *reinterpret_cast<const float4*>(merge_o + ((size_t)w * COLS + n) * D + d);
+        sum = fmaf(f, ml.y, sum);
+        acc.x = fmaf(f, v.x, acc.x);
+        acc.y = fmaf(f, v.y, acc.y);
+        acc.z = fmaf(f, v.z, acc.z);
+        acc.w = fmaf(f, v.w, acc.w);
+      }
+      if (begins && ends) {
+        uint2 res = make_uint2(pack_bf16(acc.x / sum, acc.y / sum), pack_bf16(acc.z / sum, acc.w / sum));
+        *reinterpret_cast<uint2*>(a.out + (long long)(t.row0 + ti) * a.out_stride + (size_t)(head0 + gi) * D + d) = res;
+      } else {
+        *reinterpret_cast<float4*>(a.part_o + ((size_t)slot * COLS + n) * D + d) = acc;
+        if (d == 0) a.part_ml[slot * COLS + n] = make_float2(top, sum);
+      }
+    }
+    if (begins && tid == 0) {
+      const long long last_unit = start[e] + (long long)(pair + 1) * span.units - 1;
+      const long long end_cta = ((last_unit + 1) * parts - 1) / total;
+      a.desc[(size_t)e * pairs + pair] = ends ? make_int4(-1, -1, 0, 0) : make_int4((int)cta, (int)end_cta, t.row0, t.ntok);
+    }
+    __syncthreads();
+  }
+}
+
+// Adds up what several CTAs left of a (tile, head): a block per column, its warps take the partials in turn.
+template <int D>
+__global__ void __launch_bounds__(256)
+kv4_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml,
+                 const int4* __restrict__ desc, __nv_bfloat16* __restrict__ out, long long out_stride, int group,
+                 int chunk, int chunks, int pairs, int cols) {
+  constexpr int N = D / 32;
+  __shared__ float sh_o[8][D], sh_l[8];
+  bf_pdl_trigger();
+  bf_pdl_wait();
+  const int4 d = desc[blockIdx.x];
+  if (d.x < 0) return;
+  const int pair = blockIdx.x % pairs, h = pair / chunks, head0 = h * group + (pair - h * chunks) * chunk;
+  const int n = blockIdx.y, ti = n / chunk, gi = n - ti * chunk;
+  if (ti >= d.w || gi >= min(chunk, (h + 1) * group - head0)) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int parts = d.y - d.x + 1;
+  auto slot = [&](int i) { return (size_t)(i == 0 ? 2 * d.x + 1 : 2 * (d.x + i)) * cols + n; };
+  float top = -INFINITY;
+  for (int i = lane; i < parts; i += 32) top = fmaxf(top, part_ml[slot(i)].x);
+  top = warp_max(top);
+  float sum = 0.f, acc[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) acc[k] = 0.f;
+#pragma unroll 4
+  for (int i = warp; i < parts; i += 8) {
+    const float2 ml = part_ml[slot(i)];
+    const float f = ml.x == top ? 1.f : ka_exp2(ml.x - top);
+    const float* src = part_o + slot(i) * D + lane;
+    sum = fmaf(f, ml.y, sum);
+#pragma unroll
+    for (int k = 0; k < N; ++k) acc[k] = fmaf(f, src[32 * k], acc[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) sh_o[warp][lane + 32 * k] = acc[k];
+  if (lane == 0) sh_l[warp] = sum;
+  __syncthreads();
+  if (threadIdx.x < D) {
+    float v = 0.f, w = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v += sh_o[k][threadIdx.x], w += sh_l[k];
+    out[(long long)(d.z + ti) * out_stride + (size_t)(head0 + gi) * D + threadIdx.x] = __float2bfloat16_rn(v / w);
+  }
+}
+
+template <int D, int NT>
+static int ka_launch(KaArgs a, int total_tiles, int ctas, cudaStream_t stream) {
+  constexpr size_t smem = (size_t)KA_WARPS * KA_STAGES * 2 * kv4_record(D) + (KA_MAX_TILES + 2) * 8 +
+                          KA_MAX_TILES * sizeof(KaTile) + KA_WARPS * 8 * NT * 8;
+  static_assert((size_t)KA_WARPS * KA_STAGES * 2 * kv4_record(D) >= (size_t)KA_WARPS * 8 * NT * D * 4, "");
+  static bool configured[BF_MAX_DEVICES];
+  const int dev = bf_current_device();
+  if (!configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kv4_attention_kernel<D, NT>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    configured[dev] = true;
+  }
+  const int pairs = a.nkv * a.chunks;
+  for (int first = 0; first < total_tiles; first += KA_MAX_TILES) {
+    a.first_tile = first;
+    a.n_tiles = total_tiles - first < KA_MAX_TILES ? total_tiles - first : KA_MAX_TILES;
+    int e = bf_launch_pdl(kv4_attention_kernel<D, NT>, dim3(ctas), dim3(KA_THREADS), smem, stream, a);
+    if (e) return e;
+    e = bf_launch_pdl(kv4_merge_kernel<D>, dim3(a.n_tiles * pairs, 8 * NT), dim3(256), 0, stream,
+                      (const float*)a.part_o, (const float2*)a.part_ml, (const int4*)a.desc, a.out, a.out_stride,
+                      a.group, a.chunk, a.chunks, pairs, 8 * NT);
+    if (e) return e;
+  }
+  return 0;
+}
+
+// Columns of a tile for `group` query heads per kv head: heads of a chunk, chunks, token rows.
+struct KaShape {
+  int nt, chunk, chunks, tokens;
+};
+static KaShape ka_shape(int group, int d, int max_rows) {
+  // Two sets of eight columns where one would leave heads out or a portion's rows come one by one; heads
+  // of 256 have no registers for a second one.
+  KaShape s;
+  s.nt = d <= 128 && (group > 8 || max_rows > 8 / (group < 8 ? group : 8)) ? 2 : 1;
+  const int cols = 8 * s.nt;
+  s.chunks = (group + cols - 1) / cols;
+  s.chunk = (group + s.chunks - 1) / s.chunks;
+  s.tokens = cols / s.chunk < max_rows ? cols / s.chunk : max_rows;
+  return s;
+}
+
+// Bytes of scratch that a call needs (16-byte aligned): partial results and a note per (tile, head).
+BF_EXPORT long long bf_kv4_attention_scratch(int n, int max_rows, int nh, int nkv, int d, int sms) {
+  const KaShape s = ka_shape(nh / nkv, d, max_rows);
+  const long long slots = 2LL * sms * (d <= 128 && s.nt == 1 ? 2 : 1);
+  long long tiles = (long long)n * ((max_rows + s.tokens - 1) / s.tokens);
+  if (tiles > KA_MAX_TILES) tiles = KA_MAX_TILES;
+  return slots * 8 * s.nt * (d * 4 + 8) + tiles * nkv * s.chunks * 16;
+}
+
+BF_EXPORT int bf_kv4_attention(const void* q, long long q_stride, const void* cache, const int* rows,
+                               const int* seq_of_token, const int* positions, const int* items, int n,
+                               int max_rows, int T, const int* block_tables, int table_stride, int table_rows,
+                               int table_width, void* out, long long out_stride, int nh, int nkv, int d,
+                               int page_size, int num_pages, int window, int keep, float scale, void* scratch,
+                               int sms, int* err, cudaStream_t stream) {
   if (n <= 0 || max_rows <= 0) return 0;
-  const dim3 grid(items ? max_rows : n, (nh + 3) / 4, items ? n : 1);
-  auto run = [&](auto kern) {
-    kern<<<grid, 128, 0, stream>>>((const __nv_bfloat16*)q, q_stride, (const unsigned char*)cache, rows, seq_of_token,
-                                   positions, items, block_tables, table_stride, table_rows, table_width, T,
-                                   (__nv_bfloat16*)out, out_stride, nh, nkv, page_size, num_pages, window, keep, scale, err);
-    return bf_launch_status();
-  };
-  if (d == 64) return run(kv4_attention_kernel<64>);
-  if (d == 128) return run(kv4_attention_kernel<128>);
-  if (d == 256) return run(kv4_attention_kernel<256>);
+  if ((long long)num_pages * nkv * (page_size / 8) > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+  const KaShape s = ka_shape(nh / nkv, d, max_rows);
+  const int ctas = sms * (d <= 128 && s.nt == 1 ? 2 : 1);
+  KaArgs a = {};
+  a.q = (const __nv_bfloat16*)q, a.q_stride = q_stride, a.cache = (const unsigned char*)cache;
+  a.rows = rows, a.seq_of_token = seq_of_token, a.positions = positions, a.items = items;
+  a.tiles_per_item = (max_rows + s.tokens - 1) / s.tokens;
+  a.T = T, a.block_tables = block_tables;
+  a.table_stride = table_stride, a.table_rows = table_rows, a.table_width = table_width;
+  a.out = (__nv_bfloat16*)out, a.out_stride = out_stride;
+  a.nh = nh, a.nkv = nkv, a.group = nh / nkv, a.chunk = s.chunk, a.chunks = s.chunks, a.tokens = s.tokens;
+  a.page_size = page_size, a.num_pages = num_pages, a.window = window, a.keep = keep, a.scale = scale;
+  a.part_o = (float*)scratch;
+  a.part_ml = (float2*)(a.part_o + 2LL * ctas * 8 * s.nt * d);
+  a.desc = (int4*)(a.part_ml + 2LL * ctas * 8 * s.nt);
+  a.err = err;
+  const long long tiles = (long long)n * a.tiles_per_item;
+  if (tiles > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+  if (d == 64) return s.nt == 1 ? ka_launch<64, 1>(a, (int)tiles, ctas, stream) : ka_launch<64, 2>(a, (int)tiles, ctas, stream);
+  if (d == 128) return s.nt == 1 ? ka_launch<128, 1>(a, (int)tiles, ctas, stream) : ka_launch<128, 2>(a, (int)tiles, ctas, stream);
+  if (d == 256) return ka_launch<256, 1>(a, (int)tiles, ctas, stream);
   return (int)cudaErrorInvalidValue;
 }

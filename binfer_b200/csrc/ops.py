@@ -1999,11 +1999,19 @@ def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Ten
 
 def _kv4_attention(q, cache, rows, seq_of_token, positions, items, n, max_rows, block_tables, out, nh, nkv, d,
                    ps, pages, window, keep, scale, err):
+    global _launches
+    sms = num_sms(q.device)
+    size = lib().bf_kv4_attention_scratch
+    size.restype = _c_ll
+    # a call's own, from its stream's pool: two captured graphs share nothing
+    scratch = torch.empty(size(n, max_rows, nh, nkv, d, sms), dtype=torch.uint8, device=q.device)
     _run("kv4_attention", lib().bf_kv4_attention, _ptr(q), _c_ll(q.stride(0)), _ptr(cache), _ptr(rows),
          _ptr(seq_of_token), _ptr(positions), _ptr(items), _c_int(n), _c_int(max_rows), _c_int(q.shape[0]),
          _ptr(block_tables), _c_int(block_tables.stride(0)), _c_int(block_tables.shape[0]),
          _c_int(block_tables.shape[1]), _ptr(out), _c_ll(out.stride(0)), _c_int(nh), _c_int(nkv), _c_int(d),
-         _c_int(ps), _c_int(pages), _c_int(window), _c_int(keep), _c_float(scale), _ptr(err), _stream())
+         _c_int(ps), _c_int(pages), _c_int(window), _c_int(keep), _c_float(scale), _ptr(scratch), _c_int(sms),
+         _ptr(err), _stream())
+    _launches += 1          # two kernels: the stretches of units, and what several of them share
 
 
 # ------------------------------------------------------------- a step's description
