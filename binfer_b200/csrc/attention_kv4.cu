@@ -19,23 +19,23 @@
 //
 // Work.  A tile is up to 8 NT columns, a column one query head of one token row; its keys go sixteen at a
 // time (a unit), for every kv head.  All units of a call in one row are cut into equal stretches, one a
-// CTA, so that the chip is full whatever the contexts are; the eight warps of a CTA take the units of a tile
-// and head in turn, each with a running maximum of its own, and meet once at its end.  What a CTA does
-// not finish (at most the first and the last tile of its stretch) leaves as a partial result, which a second
-// kernel adds up; scratch is two partials a CTA whatever the contexts are.  A warp fetches its units by
-// itself (16 bytes a lane, asynchronously, three units ahead of the one it computes), so no warp waits
-// for another inside a tile.  The running maximum moves only when a score passes it by 2^8, which no
-// result depends on beyond rounding and which leaves one vote a unit where maxima would take six shuffles.
+// warp, so that the chip is full whatever the contexts are.  A warp fetches its units by itself (16 bytes a
+// lane, asynchronously, three units ahead of the two it computes) and waits for no other.  A tile and head
+// that lies within a stretch is written by its warp; what is cut (at most the first and the last of a
+// stretch) leaves as a partial result, which a second kernel adds up in the order of the keys: scratch is
+// two partials a warp whatever the contexts are.  The running maximum moves only when a score passes it by
+// 2^8, which no result depends on beyond rounding and which leaves one vote a step where maxima would take
+// shuffles.
 #include "common.cuh"
 #include "kv4.cuh"
 #include "mma_utils.cuh"
 
 #define KA_WARPS 8
 #define KA_THREADS (KA_WARPS * 32)
-#define KA_STAGES 4
+#define KA_STAGES 5
 #define KA_MAX_TILES 512                   // of one launch
 #define KA_UNIT 16                         // keys
-#define KA_MIN_UNITS 8                     // a CTA's share at least, where there is so much
+#define KA_MIN_UNITS 2                     // a warp's stretch at least
 
 struct KaArgs {
   const __nv_bfloat16* q;
@@ -85,6 +85,10 @@ __device__ __forceinline__ unsigned ka_transpose(unsigned x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
+template <bool B>
+struct Bool {
+  static constexpr bool value = B;
+};
 template <int WORDS>
 __device__ __forceinline__ void ka_lds(unsigned (&w)[WORDS], const unsigned char* p) {
   if constexpr (WORDS >= 4) {
@@ -110,13 +114,9 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   constexpr float DOWN = 5.90295810358705651712e20f;        // 2^69
   constexpr unsigned M0 = 0x000f000fu, M4 = 0x00f000f0u, ONES = 0x00010001u;
   extern __shared__ __align__(128) unsigned char smem[];
-  unsigned char* ring = smem;                               // also the warps' results at a tile's end
-  float* merge_o = reinterpret_cast<float*>(smem);          // [warps][COLS][D]
-  unsigned char* after = smem + (size_t)KA_WARPS * KA_STAGES * UNIT_BYTES;
-  long long* start = reinterpret_cast<long long*>(after);   // [KA_MAX_TILES + 1]
-  KaTile* tiles = reinterpret_cast<KaTile*>(start + KA_MAX_TILES + 2);
-  float2* merge_ml = reinterpret_cast<float2*>(tiles + KA_MAX_TILES);      // [warps][COLS]
-  __shared__ long long warp_sum_of[KA_WARPS];
+  int* start = reinterpret_cast<int*>(smem + (size_t)KA_WARPS * KA_STAGES * UNIT_BYTES);   // [KA_MAX_TILES + 4]
+  KaTile* tiles = reinterpret_cast<KaTile*>(start + KA_MAX_TILES + 4);
+  __shared__ int warp_sum_of[KA_WARPS];
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r = lane >> 2, q4 = lane & 3;
@@ -125,7 +125,7 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   bf_pdl_wait();
 
   // tiles and where their units begin
-  long long running = 0;
+  int running = 0;
   for (int e0 = 0; e0 < a.n_tiles; e0 += KA_THREADS) {
     const int e = e0 + tid;
     KaTile t = {0, 0, 0, 0};
@@ -145,22 +145,23 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
         t.pos0 = ok ? a.positions[t.row0] : 0;
         t.ntok = 1;
       }
-      if (t.ntok > 0 && (t.b < 0 || t.b >= a.table_rows || t.row0 < 0 || t.row0 + t.ntok > a.T || t.pos0 < 0)) {
+      if (t.ntok > 0 && (t.b < 0 || t.b >= a.table_rows || t.row0 < 0 || t.row0 + t.ntok > a.T || t.pos0 < 0 ||
+                         (long long)t.pos0 + t.ntok > (long long)a.table_width * a.page_size)) {
         if (blockIdx.x == 0) atomicOr(a.err, BF_ERR_PAGE);
         t.ntok = 0;
       }
       tiles[e] = t;
     }
-    const long long n = (long long)ka_span(t, a.window, a.keep).units * pairs;
-    long long incl = n;
+    const int n = ka_span(t, a.window, a.keep).units * pairs;
+    int incl = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+      const int up = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += up;
     }
     if (lane == 31) warp_sum_of[warp] = incl;
     __syncthreads();
-    long long before = running;
+    int before = running;
     for (int w = 0; w < KA_WARPS; ++w) {
       if (w < warp) before += warp_sum_of[w];
       running += warp_sum_of[w];
@@ -168,19 +169,19 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
     if (e < a.n_tiles) {
       start[e] = before + incl - n;
       if (n == 0 && blockIdx.x == 0)
-        for (int i = 0; i < pairs; ++i) a.desc[(size_t)e * pairs + i] = make_int4(-1, -1, 0, 0);
+        for (int i = 0; i < pairs; ++i) a.desc[e * pairs + i] = make_int4(-1, -1, 0, 0);
     }
     __syncthreads();
   }
   if (tid == 0) start[a.n_tiles] = running;
   __syncthreads();
-  const long long total = running;
-  long long parts = total / KA_MIN_UNITS;
-  parts = parts < 1 ? 1 : parts > gridDim.x ? gridDim.x : parts;
-  const long long cta = blockIdx.x;
-  if (cta >= parts || total == 0) return;
-  long long x = cta * total / parts;
-  const long long x_end = (cta + 1) * total / parts;
+  const int total = running;
+  const int parts = min(max(total / KA_MIN_UNITS, 1), (int)gridDim.x * KA_WARPS);
+  const int me = warp * gridDim.x + blockIdx.x;             // (few stretches lie on as many SMs)
+  if (me >= parts || total == 0) return;
+  const int each = total / parts, longer = total - each * parts;         // the first `longer` have one more
+  int x = me * each + min(me, longer);
+  const int x_end = x + each + (me < longer ? 1 : 0);
 
   int e;                                                    // the tile that holds unit x
   {
@@ -194,26 +195,37 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   const float scale_log2 = a.scale * 1.44269504088896341f;
   const float score_up = scale_log2 * DOWN;
   const int eighths = a.page_size / KV4_EIGHTH;
-  unsigned char* my_ring = ring + (size_t)warp * KA_STAGES * UNIT_BYTES;
+  unsigned char* my_ring = smem + (size_t)warp * KA_STAGES * UNIT_BYTES;
 
   while (x < x_end) {
     while (start[e + 1] <= x) ++e;
     const KaTile t = tiles[e];
     const KaSpan span = ka_span(t, a.window, a.keep);
-    const long long rel = x - start[e];
-    const int pair = (int)(rel / span.units), u0 = (int)(rel % span.units);
-    const int u1 = (int)(x_end - x < span.units - u0 ? u0 + (x_end - x) : span.units);
+    const int rel = x - start[e], pair = rel / span.units, u0 = rel - pair * span.units;
+    const int mine = min(span.units - u0, x_end - x);
     const int h = pair / a.chunks, head0 = h * a.group + (pair - h * a.chunks) * a.chunk;
     const int heads = min(a.chunk, (h + 1) * a.group - head0);
     const int last = t.pos0 + t.ntok - 1;
     const int first_seen = a.window > 0 ? max(0, t.pos0 - a.window + 1) : 0;
     const int* table = a.block_tables + (size_t)t.b * a.table_stride;
-    x += u1 - u0;
+    x += mine;
+    const bool begins = u0 == 0, ends = u0 + mine == span.units;
 
-    // ---- units of this warp: u0 + warp, u0 + warp + 8, ...
-    const int mine = u1 - u0 > warp ? (u1 - u0 - warp + KA_WARPS - 1) / KA_WARPS : 0;
+    uint4 raw[NT][KW];                                      // the queries, under way while pages are looked up
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int n = nt * 8 + r, ti = n / a.chunk, gi = n - ti * a.chunk;
+      const bool on = ti < t.ntok && gi < heads;
+      const __nv_bfloat16* src = a.q + (long long)(t.row0 + (on ? ti : 0)) * a.q_stride + (size_t)(head0 + (on ? gi : 0)) * D;
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+        raw[nt][w] = *reinterpret_cast<const uint4*>(src + (w >> 1) * 64 + q4 * 16 + (w & 1) * 8);
+        if (!on) raw[nt][w] = make_uint4(0, 0, 0, 0);
+      }
+    }
+    // the stretch's units: u0, u0 + 1, ...
     auto unit_key = [&](int i) {
-      const int u = u0 + warp + i * KA_WARPS;
+      const int u = u0 + i;
       return (u < span.kept ? u : span.from + u - span.kept) * KA_UNIT;
     };
     int rec0 = 0, rec1 = 0;                                 // of unit (32 n + lane): its two records
@@ -253,26 +265,17 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
       cp_async_commit();
     };
 #pragma unroll
-    for (int i = 0; i < KA_STAGES - 1; ++i) issue(i);
+    for (int i = 0; i < KA_STAGES - 2; ++i) issue(i);
 
     // ---- queries: operand b of the scores' product, and their sums per group
-    unsigned qf[NT][KW][4];
-    float qs[NT][NG][2];
+    unsigned qf[NT][KW][4], ql[NT][2];
     int pcol[NT][2];
-    bool live[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int n = nt * 8 + r, ti = n / a.chunk, gi = n - ti * a.chunk;
-      const bool on = ti < t.ntok && gi < heads;
-      const __nv_bfloat16* src = a.q + (long long)(t.row0 + (on ? ti : 0)) * a.q_stride + (size_t)(head0 + (on ? gi : 0)) * D;
-      float sums[NG];
-#pragma unroll
-      for (int g = 0; g < NG; ++g) sums[g] = 0.f;
+      float sums[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < KW; ++w) {
-        uint4 raw = *reinterpret_cast<const uint4*>(src + (w >> 1) * 64 + q4 * 16 + (w & 1) * 8);
-        if (!on) raw = make_uint4(0, 0, 0, 0);
-        const unsigned* u = &raw.x;
+        const unsigned* u = &raw[nt][w].x;
         float f[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -286,21 +289,28 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
         qf[nt][w][2] = pack_bf16(f[2] * UP, f[6] * UP);
         qf[nt][w][3] = pack_bf16(f[3] * (UP / 16), f[7] * (UP / 16));
       }
+      // the sums meet the keys' lowest values in one product: lane q4's share is their q4-th bfloat16 term
+      float term[4];
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 1);
-        sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 2);
-        qs[nt][g][0] = __shfl_sync(0xffffffffu, sums[g], q4 * 8) * scale_log2;
-        qs[nt][g][1] = __shfl_sync(0xffffffffu, sums[g], q4 * 8 + 4) * scale_log2;
+      for (int g = 0; g < 4; ++g) {
+        float v = sums[g];
+        v += __shfl_xor_sync(0xffffffffu, v, 1);
+        v += __shfl_xor_sync(0xffffffffu, v, 2);
+        v *= scale_log2;
+        const float t0 = __bfloat162float(__float2bfloat16_rn(v)), v1 = v - t0;
+        const float t1 = __bfloat162float(__float2bfloat16_rn(v1)), v2 = v1 - t1;
+        term[g] = q4 == 0 ? t0 : q4 == 1 ? t1 : q4 == 2 ? v2 : 0.f;
       }
+      ql[nt][0] = pack_bf16(term[0], term[1]);
+      ql[nt][1] = pack_bf16(term[2], term[3]);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int n2 = nt * 8 + 2 * q4 + i, t2 = n2 / a.chunk;
-        live[nt][i] = t2 < t.ntok;
         pcol[nt][i] = t.pos0 + min(t2, t.ntok - 1);
       }
     }
 
+    // p = 2^(s - m), m some 64 below the largest score so far: the probabilities carry their 2^64 from here
     float o[NT][D / 16][4], ps[NT][NG][4], corr[NT][NG][2], l[NT][2], m[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -312,99 +322,160 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
         corr[nt][g][0] = corr[nt][g][1] = 0.f;
       }
       l[nt][0] = l[nt][1] = 0.f;
-      m[nt][0] = m[nt][1] = -INFINITY;
+      m[nt][0] = m[nt][1] = -1e30f;
     }
 
-    for (int i = 0; i < mine; ++i) {
-      cp_async_wait<KA_STAGES - 2>();
-      __syncwarp();
-      issue(i + KA_STAGES - 1);
-      const unsigned char* s0 = my_ring + (i % KA_STAGES) * UNIT_BYTES;
+    // scores of keys r and 8 + r of a unit against columns 2 q4, 2 q4 + 1 of every eight
+    auto scores = [&](float (&s)[NT][4], const unsigned char* s0) {
       const unsigned char* s1 = s0 + REC;
-      const int key0 = unit_key(i);
-
-      // scores of keys key0 + r and key0 + 8 + r against columns 2 q4, 2 q4 + 1 of every eight
-      float s[NT][4];
-      {
-        unsigned w0[KW], w1[KW], p0[NG], p1[NG];
-        ka_lds<KW>(w0, s0 + r * (D / 2) + q4 * (D / 8));
-        ka_lds<KW>(w1, s1 + r * (D / 2) + q4 * (D / 8));
-        ka_lds<NG>(p0, s0 + kv4_key_params_at(D) + r * NG * 4);
-        ka_lds<NG>(p1, s1 + kv4_key_params_at(D) + r * NG * 4);
-        float low[NT][4];
+      unsigned w0[KW], w1[KW], p0[NG], p1[NG];
+      ka_lds<KW>(w0, s0 + r * (D / 2) + q4 * (D / 8));
+      ka_lds<KW>(w1, s1 + r * (D / 2) + q4 * (D / 8));
+      ka_lds<NG>(p0, s0 + kv4_key_params_at(D) + r * NG * 4);
+      ka_lds<NG>(p1, s1 + kv4_key_params_at(D) + r * NG * 4);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-          low[nt][0] = low[nt][1] = low[nt][2] = low[nt][3] = 0.f;
-        }
+      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          float c[NT][4];
+      for (int g = 0; g < NG; ++g) {
+        float c[NT][4];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.f;
+        for (int nt = 0; nt < NT; ++nt) c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.f;
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int w = 2 * g + half;
-            const unsigned a0[4] = {w0[w] & M0, w1[w] & M0, w0[w] & M4, w1[w] & M4};
-            const unsigned h0 = w0[w] >> 8, h1 = w1[w] >> 8;
-            const unsigned a1[4] = {h0 & M0, h1 & M0, h0 & M4, h1 & M4};
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma_bf16_16816(c[nt], a0, qf[nt][w][0], qf[nt][w][1]);
-              mma_bf16_16816(c[nt], a1, qf[nt][w][2], qf[nt][w][3]);
-            }
-          }
-          const float sc0 = kv4_scale(p0[g]), sc1 = kv4_scale(p1[g]), lo0 = kv4_low(p0[g]), lo1 = kv4_low(p1[g]);
+        for (int half = 0; half < 2; ++half) {
+          const int w = 2 * g + half;
+          const unsigned a0[4] = {w0[w] & M0, w1[w] & M0, w0[w] & M4, w1[w] & M4};
+          const unsigned h0 = w0[w] >> 8, h1 = w1[w] >> 8;
+          const unsigned a1[4] = {h0 & M0, h1 & M0, h0 & M4, h1 & M4};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            s[nt][0] += sc0 * c[nt][0];
-            s[nt][1] += sc0 * c[nt][1];
-            s[nt][2] += sc1 * c[nt][2];
-            s[nt][3] += sc1 * c[nt][3];
-            low[nt][0] += lo0 * qs[nt][g][0];
-            low[nt][1] += lo0 * qs[nt][g][1];
-            low[nt][2] += lo1 * qs[nt][g][0];
-            low[nt][3] += lo1 * qs[nt][g][1];
+            mma_bf16_16816(c[nt], a0, qf[nt][w][0], qf[nt][w][1]);
+            mma_bf16_16816(c[nt], a1, qf[nt][w][2], qf[nt][w][3]);
           }
         }
+        const float sc0 = kv4_scale(p0[g]), sc1 = kv4_scale(p1[g]);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) s[nt][k] = fmaf(s[nt][k], score_up, low[nt][k]);
+        for (int nt = 0; nt < NT; ++nt) {
+          s[nt][0] = fmaf(sc0, c[nt][0], s[nt][0]);
+          s[nt][1] = fmaf(sc0, c[nt][1], s[nt][1]);
+          s[nt][2] = fmaf(sc1, c[nt][2], s[nt][2]);
+          s[nt][3] = fmaf(sc1, c[nt][3], s[nt][3]);
+        }
       }
-      // every key seen by every column: not so at the context's end and at the window's edges
-      const bool whole = key0 + KA_UNIT - 1 <= t.pos0 &&
-                         (a.window <= 0 || key0 > last - a.window || key0 + KA_UNIT <= a.keep);
-      unsigned hidden = 0;
-      if (!whole) {
+      unsigned low[4] = {0u, 0u, 0u, 0u};                   // (m of group 0, m of group 1), of 2 and 3
+      low[0] = NG > 1 ? __byte_perm(p0[0], p0[NG > 1 ? 1 : 0], 0x7632) : p0[0] >> 16;
+      low[1] = NG > 1 ? __byte_perm(p1[0], p1[NG > 1 ? 1 : 0], 0x7632) : p1[0] >> 16;
+      if (NG > 2) {
+        low[2] = __byte_perm(p0[NG > 2 ? 2 : 0], p0[NG > 2 ? 3 : 0], 0x7632);
+        low[3] = __byte_perm(p1[NG > 2 ? 2 : 0], p1[NG > 2 ? 3 : 0], 0x7632);
+      }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        float c[4] = {0.f, 0.f, 0.f, 0.f};
+        mma_bf16_16816(c, low, ql[nt][0], ql[nt][1]);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int j = key0 + r + (k >> 1) * 8, p = pcol[nt][k & 1];
-            if (j > p || (a.window > 0 && j <= p - a.window && j >= a.keep)) {
-              hidden |= 1u << (nt * 4 + k);
-              s[nt][k] = -INFINITY;
-            }
+        for (int k = 0; k < 4; ++k) s[nt][k] = fmaf(s[nt][k], score_up, c[k]);
+      }
+    };
+    // adds a unit's values; `hidden`: bits of elements whose key the column does not see
+    auto values = [&](float (&s)[NT][4], const unsigned char* s0, auto edge, unsigned hidden) {
+      const unsigned char* s1 = s0 + REC;
+      unsigned v0[KW], v1[KW], p0[NG], p1[NG];
+      ka_lds<KW>(v0, s0 + kv4_values_at(D) + r * (D / 2) + q4 * (D / 8));
+      ka_lds<KW>(v1, s1 + kv4_values_at(D) + r * (D / 2) + q4 * (D / 8));
+      ka_lds<NG>(p0, s0 + kv4_value_params_at(D) + r * NG * 4);
+      ka_lds<NG>(p1, s1 + kv4_value_params_at(D) + r * NG * 4);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[nt][k] = ka_exp2(s[nt][k] - m[nt][k & 1]);
+        l[nt][0] += s[nt][0] + s[nt][2];
+        l[nt][1] += s[nt][1] + s[nt][3];
+      }
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const float sc0 = kv4_scale(p0[g]), sc1 = kv4_scale(p1[g]);
+        const float mid0 = fmaf(8.f, sc0, kv4_low(p0[g])), mid1 = fmaf(8.f, sc1, kv4_low(p1[g]));
+        unsigned b0[NT], b1[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float w[4] = {s[nt][0] * sc0, s[nt][1] * sc0, s[nt][2] * sc1, s[nt][3] * sc1};
+          if constexpr (decltype(edge)::value) {            // (a hidden key may be anything: 0 times it is not 0)
+            float z[4] = {s[nt][0] * mid0, s[nt][1] * mid0, s[nt][2] * mid1, s[nt][3] * mid1};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (hidden >> (nt * 4 + k) & 1) w[k] = z[k] = 0.f;
+            corr[nt][g][0] += z[0] + z[2];
+            corr[nt][g][1] += z[1] + z[3];
+          } else {
+            corr[nt][g][0] = fmaf(s[nt][2], mid1, fmaf(s[nt][0], mid0, corr[nt][g][0]));
+            corr[nt][g][1] = fmaf(s[nt][3], mid1, fmaf(s[nt][1], mid0, corr[nt][g][1]));
           }
+          b0[nt] = ka_transpose(pack_bf16(w[0], w[1]));
+          b1[nt] = ka_transpose(pack_bf16(w[2], w[3]));
+          const unsigned ones[4] = {ONES, ONES, ONES, ONES};
+          mma_bf16_16816(ps[nt][g], ones, b0[nt], b1[nt]);
+        }
+        // eight numbers of this lane's part, for tokens 2 q4 and 2 q4 + 1 of either record
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const unsigned sel = half ? 0x7632 : 0x5410;
+          const unsigned x0 = __byte_perm(v0[g], v0[NG + g], sel), x1 = __byte_perm(v1[g], v1[NG + g], sel);
+          const unsigned h0 = x0 >> 8, h1 = x1 >> 8;
+          const unsigned a0[4] = {x0 & M0, x0 & M4, x1 & M0, x1 & M4};
+          const unsigned a1[4] = {h0 & M0, h0 & M4, h1 & M0, h1 & M4};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma_bf16_16816(o[nt][4 * g + 2 * half], a0, b0[nt], b1[nt]);
+            mma_bf16_16816(o[nt][4 * g + 2 * half + 1], a1, b0[nt], b1[nt]);
+          }
+        }
+      }
+    };
+    // two units at a time, so that one's latencies lie under the other's work
+    auto step = [&](int i, auto edge) {
+      const unsigned char* sa = my_ring + (i % KA_STAGES) * UNIT_BYTES;
+      const unsigned char* sb = my_ring + ((i + 1) % KA_STAGES) * UNIT_BYTES;
+      float s[2][NT][4];
+      scores(s[0], sa);
+      scores(s[1], sb);
+      unsigned hidden[2] = {0u, 0u};
+      if constexpr (decltype(edge)::value) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int key = i + u < mine ? unit_key(i + u) : 0x7fffff00;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int j = key + r + (k >> 1) * 8, p = pcol[nt][k & 1];
+              if (j > p || (a.window > 0 && j <= p - a.window && j >= a.keep)) {
+                hidden[u] |= 1u << (nt * 4 + k);
+                s[u][nt][k] = -INFINITY;
+              }
+            }
+        }
       }
       bool over = false;
+      float top[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) over |= fmaxf(s[nt][c], s[nt][c + 2]) > m[nt][c] + 8.f;
+        for (int c = 0; c < 2; ++c) {
+          top[nt][c] = fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]), fmaxf(s[1][nt][c], s[1][nt][c + 2]));
+          over |= top[nt][c] > m[nt][c] + 72.f;
+        }
       if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float top = fmaxf(s[nt][c], s[nt][c + 2]);
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-            top = fmaxf(top, m[nt][c]);
-            const float f = top == m[nt][c] ? 1.f : ka_exp2(m[nt][c] - top);
-            m[nt][c] = top;
+            float x = top[nt][c];
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            x = fmaxf(x - 64.f, m[nt][c]);
+            const float f = ka_exp2(m[nt][c] - x);
+            m[nt][c] = x;
             l[nt][c] *= f;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
@@ -418,132 +489,69 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
             }
           }
       }
-      {
-        unsigned v0[KW], v1[KW], p0[NG], p1[NG];
-        ka_lds<KW>(v0, s0 + kv4_values_at(D) + r * (D / 2) + q4 * (D / 8));
-        ka_lds<KW>(v1, s1 + kv4_values_at(D) + r * (D / 2) + q4 * (D / 8));
-        ka_lds<NG>(p0, s0 + kv4_value_params_at(D) + r * NG * 4);
-        ka_lds<NG>(p1, s1 + kv4_value_params_at(D) + r * NG * 4);
-        float p[NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float top = m[nt][k & 1];
-            p[nt][k] = ka_exp2(s[nt][k] - (top == -INFINITY ? 0.f : top));
-          }
-          l[nt][0] += p[nt][0] + p[nt][2];
-          l[nt][1] += p[nt][1] + p[nt][3];
-        }
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          const float sc0 = kv4_scale(p0[g]), sc1 = kv4_scale(p1[g]);
-          const float mid0 = fmaf(8.f, sc0, kv4_low(p0[g])), mid1 = fmaf(8.f, sc1, kv4_low(p1[g]));
-          const float up0 = sc0 * UP, up1 = sc1 * UP;
-          unsigned b0[NT], b1[NT];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float w[4] = {p[nt][0] * up0, p[nt][1] * up0, p[nt][2] * up1, p[nt][3] * up1};
-            float z[4] = {p[nt][0] * mid0, p[nt][1] * mid0, p[nt][2] * mid1, p[nt][3] * mid1};
-            if (hidden) {                                   // (a hidden key may be anything: 0 times it is not 0)
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                if (hidden >> (nt * 4 + k) & 1) w[k] = z[k] = 0.f;
-            }
-            corr[nt][g][0] += z[0] + z[2];
-            corr[nt][g][1] += z[1] + z[3];
-            b0[nt] = ka_transpose(pack_bf16(w[0], w[1]));
-            b1[nt] = ka_transpose(pack_bf16(w[2], w[3]));
-            const unsigned ones[4] = {ONES, ONES, ONES, ONES};
-            mma_bf16_16816(ps[nt][g], ones, b0[nt], b1[nt]);
-          }
-          // eight numbers of this lane's part, for tokens 2 q4 and 2 q4 + 1 of either record
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const unsigned sel = half ? 0x7632 : 0x5410;
-            const unsigned x0 = __byte_perm(v0[g], v0[NG + g], sel), x1 = __byte_perm(v1[g], v1[NG + g], sel);
-            const unsigned h0 = x0 >> 8, h1 = x1 >> 8;
-            const unsigned a0[4] = {x0 & M0, x0 & M4, x1 & M0, x1 & M4};
-            const unsigned a1[4] = {h0 & M0, h0 & M4, h1 & M0, h1 & M4};
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma_bf16_16816(o[nt][4 * g + 2 * half], a0, b0[nt], b1[nt]);
-              mma_bf16_16816(o[nt][4 * g + 2 * half + 1], a1, b0[nt], b1[nt]);
-            }
-          }
-        }
-      }
+      values(s[0], sa, edge, hidden[0]);
+      values(s[1], sb, edge, hidden[1]);
+    };
+    // every key of a unit seen by every column: not so at the context's end and at the window's edges
+    auto whole = [&](int i) {
+      const int key = unit_key(i);
+      return i < mine && key + KA_UNIT - 1 <= t.pos0 &&
+             (a.window <= 0 || key > last - a.window || key + KA_UNIT <= a.keep);
+    };
+    for (int i = 0; i < mine; i += 2) {
+      cp_async_wait<KA_STAGES - 4>();
+      __syncwarp();
+      issue(i + KA_STAGES - 2);                             // into the places of the two units before these
+      issue(i + KA_STAGES - 1);
+      if (whole(i) && whole(i + 1)) step(i, Bool<false>()); else step(i, Bool<true>());
     }
     cp_async_wait<0>();
-    __syncthreads();                                        // the rings are free: the warps' results go there
 
+    // ---- the result: lane (r, q4) has numbers 8 r .. 8 r + 7 of every group, of two columns of every eight
+    const int slot = 2 * me + (begins ? 1 : 0);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int n = nt * 8 + 2 * q4 + c;
+        const int n = nt * 8 + 2 * q4 + c, ti = n / a.chunk, gi = n - ti * a.chunk;
 #pragma unroll
         for (int k = 4; k < 32; k <<= 1) {
           l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], k);
 #pragma unroll
           for (int g = 0; g < NG; ++g) corr[nt][g][c] += __shfl_xor_sync(0xffffffffu, corr[nt][g][c], k);
         }
-        if (r == 0) merge_ml[warp * COLS + n] = make_float2(m[nt][c], l[nt][c]);
-        if (!live[nt][c]) continue;
-        float* dst = merge_o + ((size_t)warp * COLS + n) * D + r * 8;
+        if (ti >= t.ntok || gi >= heads) continue;
+        const float sum = l[nt][c] * (1.f / UP);
+        const float f = begins && ends ? 1.f / sum : 1.f;
+        if (!(begins && ends) && r == 0) a.part_ml[slot * COLS + n] = make_float2(m[nt][c], sum);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-          const float base = fmaf(-8.f * DOWN, ps[nt][g][c], corr[nt][g][c]);
+          const float base = fmaf(-8.f * DOWN, ps[nt][g][c], corr[nt][g][c] * (1.f / UP));
+          float v[8];
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const float* x0 = o[nt][4 * g + 2 * half];
-            const float* x1 = o[nt][4 * g + 2 * half + 1];
-            *reinterpret_cast<float4*>(dst + g * 64 + half * 4) =
-                make_float4(fmaf(x0[c], DOWN, base), fmaf(x0[c + 2], DOWN / 16, base),
-                            fmaf(x1[c], DOWN, base), fmaf(x1[c + 2], DOWN / 16, base));
+          for (int k = 0; k < 4; ++k) {
+            v[2 * k] = fmaf(o[nt][4 * g + k][c], DOWN, base) * f;
+            v[2 * k + 1] = fmaf(o[nt][4 * g + k][c + 2], DOWN / 16, base) * f;
+          }
+          if (begins && ends) {
+            *reinterpret_cast<uint4*>(a.out + (long long)(t.row0 + ti) * a.out_stride + (size_t)(head0 + gi) * D + g * 64 + r * 8) =
+                make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+          } else {
+            float4* dst = reinterpret_cast<float4*>(a.part_o + ((size_t)slot * COLS + n) * D + g * 64 + r * 8);
+            dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+            dst[1] = make_float4(v[4], v[5], v[6], v[7]);
           }
         }
       }
-    __syncthreads();
-    const bool begins = u0 == 0, ends = u1 == span.units;
-    const int slot = (int)(2 * cta) + (begins ? 1 : 0);
-    for (int i = tid; i < COLS * (D / 4); i += KA_THREADS) {
-      const int n = i / (D / 4), d = (i - n * (D / 4)) * 4, ti = n / a.chunk, gi = n - ti * a.chunk;
-      if (ti >= t.ntok || gi >= heads) continue;
-      float top = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < KA_WARPS; ++w) top = fmaxf(top, merge_ml[w * COLS + n].x);
-      float sum = 0.f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < KA_WARPS; ++w) {
-        const float2 ml = merge_ml[w * COLS + n];
-        const float f = ml.x == top ? 1.f : ka_exp2(ml.x - top);
-        const float4 v = *reinterpret_cast<const float4*>(merge_o + ((size_t)w * COLS + n) * D + d);
-        sum = fmaf(f, ml.y, sum);
-        acc.x = fmaf(f, v.x, acc.x);
-        acc.y = fmaf(f, v.y, acc.y);
-        acc.z = fmaf(f, v.z, acc.z);
-        acc.w = fmaf(f, v.w, acc.w);
-      }
-      if (begins && ends) {
-        uint2 res = make_uint2(pack_bf16(acc.x / sum, acc.y / sum), pack_bf16(acc.z / sum, acc.w / sum));
-        *reinterpret_cast<uint2*>(a.out + (long long)(t.row0 + ti) * a.out_stride + (size_t)(head0 + gi) * D + d) = res;
-      } else {
-        *reinterpret_cast<float4*>(a.part_o + ((size_t)slot * COLS + n) * D + d) = acc;
-        if (d == 0) a.part_ml[slot * COLS + n] = make_float2(top, sum);
-      }
+    if (begins && lane == 0) {
+      const int at = start[e] + (pair + 1) * span.units - 1, edge = longer * (each + 1);   // the last unit's owner
+      const int owner = at < edge ? at / (each + 1) : longer + (at - edge) / each;
+      a.desc[e * pairs + pair] = ends ? make_int4(-1, -1, 0, 0) : make_int4(me, owner, t.row0, t.ntok);
     }
-    if (begins && tid == 0) {
-      const long long last_unit = start[e] + (long long)(pair + 1) * span.units - 1;
-      const long long end_cta = ((last_unit + 1) * parts - 1) / total;
-      a.desc[(size_t)e * pairs + pair] = ends ? make_int4(-1, -1, 0, 0) : make_int4((int)cta, (int)end_cta, t.row0, t.ntok);
-    }
-    __syncthreads();
   }
 }
 
-// Adds up what several CTAs left of a (tile, head): a block per column, its warps take the partials in turn.
+// Adds up what several warps left of a (tile, head): a block per column, its warps take the partials in turn.
 template <int D>
 __global__ void __launch_bounds__(256)
 kv4_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml,
@@ -590,9 +598,8 @@ kv4_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ pa
 
 template <int D, int NT>
 static int ka_launch(KaArgs a, int total_tiles, int ctas, cudaStream_t stream) {
-  constexpr size_t smem = (size_t)KA_WARPS * KA_STAGES * 2 * kv4_record(D) + (KA_MAX_TILES + 2) * 8 +
-                          KA_MAX_TILES * sizeof(KaTile) + KA_WARPS * 8 * NT * 8;
-  static_assert((size_t)KA_WARPS * KA_STAGES * 2 * kv4_record(D) >= (size_t)KA_WARPS * 8 * NT * D * 4, "");
+  constexpr size_t smem = (size_t)KA_WARPS * KA_STAGES * 2 * kv4_record(D) + (KA_MAX_TILES + 4) * 4 +
+                          KA_MAX_TILES * sizeof(KaTile);
   static bool configured[BF_MAX_DEVICES];
   const int dev = bf_current_device();
   if (!configured[dev]) {
@@ -602,9 +609,13 @@ static int ka_launch(KaArgs a, int total_tiles, int ctas, cudaStream_t stream) {
     configured[dev] = true;
   }
   const int pairs = a.nkv * a.chunks;
-  for (int first = 0; first < total_tiles; first += KA_MAX_TILES) {
+  // the units of a launch are counted in 32 bits
+  const long long units = ((long long)a.table_width * a.page_size / KA_UNIT + 2) * pairs;
+  if (units > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+  const int most = 0x7fffffffLL / units < KA_MAX_TILES ? (int)(0x7fffffffLL / units) : KA_MAX_TILES;
+  for (int first = 0; first < total_tiles; first += most) {
     a.first_tile = first;
-    a.n_tiles = total_tiles - first < KA_MAX_TILES ? total_tiles - first : KA_MAX_TILES;
+    a.n_tiles = total_tiles - first < most ? total_tiles - first : most;
     int e = bf_launch_pdl(kv4_attention_kernel<D, NT>, dim3(ctas), dim3(KA_THREADS), smem, stream, a);
     if (e) return e;
     e = bf_launch_pdl(kv4_merge_kernel<D>, dim3(a.n_tiles * pairs, 8 * NT), dim3(256), 0, stream,
@@ -634,7 +645,7 @@ static KaShape ka_shape(int group, int d, int max_rows) {
 // Bytes of scratch that a call needs (16-byte aligned): partial results and a note per (tile, head).
 BF_EXPORT long long bf_kv4_attention_scratch(int n, int max_rows, int nh, int nkv, int d, int sms) {
   const KaShape s = ka_shape(nh / nkv, d, max_rows);
-  const long long slots = 2LL * sms * (d <= 128 && s.nt == 1 ? 2 : 1);
+  const long long slots = 2LL * sms * KA_WARPS * (d <= 128 && s.nt == 1 ? 2 : 1);
   long long tiles = (long long)n * ((max_rows + s.tokens - 1) / s.tokens);
   if (tiles > KA_MAX_TILES) tiles = KA_MAX_TILES;
   return slots * 8 * s.nt * (d * 4 + 8) + tiles * nkv * s.chunks * 16;
@@ -660,8 +671,8 @@ BF_EXPORT int bf_kv4_attention(const void* q, long long q_stride, const void* ca
   a.nh = nh, a.nkv = nkv, a.group = nh / nkv, a.chunk = s.chunk, a.chunks = s.chunks, a.tokens = s.tokens;
   a.page_size = page_size, a.num_pages = num_pages, a.window = window, a.keep = keep, a.scale = scale;
   a.part_o = (float*)scratch;
-  a.part_ml = (float2*)(a.part_o + 2LL * ctas * 8 * s.nt * d);
-  a.desc = (int4*)(a.part_ml + 2LL * ctas * 8 * s.nt);
+  a.part_ml = (float2*)(a.part_o + 2LL * ctas * KA_WARPS * 8 * s.nt * d);
+  a.desc = (int4*)(a.part_ml + 2LL * ctas * KA_WARPS * 8 * s.nt);
   a.err = err;
   const long long tiles = (long long)n * a.tiles_per_item;
   if (tiles > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
