@@ -18,24 +18,25 @@
 // in float.  Everything else is float.
 //
 // Work.  A tile is up to 8 NT columns, a column one query head of one token row; its keys go sixteen at a
-// time (a unit), for every kv head.  All units of a call in one row are cut into equal stretches, one a
-// warp, so that the chip is full whatever the contexts are.  A warp fetches its units by itself (16 bytes a
-// lane, asynchronously, three units ahead of the two it computes) and waits for no other.  A tile and head
-// that lies within a stretch is written by its warp; what is cut (at most the first and the last of a
-// stretch) leaves as a partial result, which a second kernel adds up in the order of the keys: scratch is
-// two partials a warp whatever the contexts are.  The running maximum moves only when a score passes it by
-// 2^8, which no result depends on beyond rounding and which leaves one vote a step where maxima would take
-// shuffles.
+// time (a unit), for every kv head.  A tile and head's units are cut into stretches of nearly equal length,
+// one a warp, as short as the chip's warps allow; a warp fetches its units by itself (16 bytes a lane,
+// asynchronously, two units ahead of the two it computes) and waits for no other.  What is not cut is
+// written by its warp; a cut one leaves a partial result a stretch, which a second kernel adds up in the
+// order of the keys: scratch is one partial a warp whatever the contexts are.  The running maximum moves
+// only when a score passes it by 2^8, which no result depends on beyond rounding and which leaves one vote a
+// step where maxima would take shuffles.
 #include "common.cuh"
 #include "kv4.cuh"
 #include "mma_utils.cuh"
 
 #define KA_WARPS 8
 #define KA_THREADS (KA_WARPS * 32)
-#define KA_STAGES 5
+#define KA_STAGES 4                        // units: two steps
 #define KA_MAX_TILES 512                   // of one launch
 #define KA_UNIT 16                         // keys
-#define KA_MIN_UNITS 2                     // a warp's stretch at least
+#define KA_SPARE_SLOTS 32                  // (the counts of stretches are rounded sums)
+#define KA_MIN_UNITS 2                     // a stretch's length at least
+#define KA_CANDIDATES 8                    // lengths of stretches that are tried
 
 struct KaArgs {
   const __nv_bfloat16* q;
@@ -50,6 +51,7 @@ struct KaArgs {
   int nh, nkv, group, chunk, chunks, tokens;               // query heads per kv head; in a tile; chunks of them
   int page_size, num_pages, window, keep;
   float scale;
+  int slots;
   float* part_o;
   float2* part_ml;
   int4* desc;
@@ -114,9 +116,11 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   constexpr float DOWN = 5.90295810358705651712e20f;        // 2^69
   constexpr unsigned M0 = 0x000f000fu, M4 = 0x00f000f0u, ONES = 0x00010001u;
   extern __shared__ __align__(128) unsigned char smem[];
-  int* start = reinterpret_cast<int*>(smem + (size_t)KA_WARPS * KA_STAGES * UNIT_BYTES);   // [KA_MAX_TILES + 4]
-  KaTile* tiles = reinterpret_cast<KaTile*>(start + KA_MAX_TILES + 4);
-  __shared__ int warp_sum_of[KA_WARPS];
+  KaTile* tiles = reinterpret_cast<KaTile*>(smem + (size_t)KA_WARPS * KA_STAGES * UNIT_BYTES);
+  int* pieces = reinterpret_cast<int*>(tiles + KA_MAX_TILES);              // stretches of a head of the tile
+  int* start = pieces + KA_MAX_TILES;                                      // the tile's first stretch
+  int* cut_start = start + KA_MAX_TILES + 4;                               // and the same of those that are cut
+  __shared__ int sums[KA_WARPS][KA_CANDIDATES + 1];
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r = lane >> 2, q4 = lane & 3;
@@ -124,10 +128,13 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   bf_pdl_trigger();
   bf_pdl_wait();
 
-  // tiles and where their units begin
-  int running = 0;
-  for (int e0 = 0; e0 < a.n_tiles; e0 += KA_THREADS) {
-    const int e = e0 + tid;
+  // ---- tiles, and how their units are cut.  A thread has tiles tid and tid + KA_THREADS.
+  constexpr int MINE = KA_MAX_TILES / KA_THREADS;
+  int units[MINE];
+  int total = 0, filled = 0;
+#pragma unroll
+  for (int k = 0; k < MINE; ++k) {
+    const int e = tid + k * KA_THREADS;
     KaTile t = {0, 0, 0, 0};
     if (e < a.n_tiles) {
       if (a.items) {
@@ -152,64 +159,103 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
       }
       tiles[e] = t;
     }
-    const int n = ka_span(t, a.window, a.keep).units * pairs;
-    int incl = n;
+    units[k] = ka_span(t, a.window, a.keep).units;
+    total += units[k];
+    filled += units[k] > 0;
+  }
+  total = __reduce_add_sync(0xffffffffu, total);
+  filled = __reduce_add_sync(0xffffffffu, filled);
+  if (lane == 0) sums[warp][0] = total, sums[warp][1] = filled;
+  __syncthreads();
+  total = filled = 0;
+#pragma unroll
+  for (int w = 0; w < KA_WARPS; ++w) total += sums[w][0], filled += sums[w][1];
+  __syncthreads();
+  // Stretches of `length` make at most total / length + filled of a head; the shortest of a few lengths
+  // that gives every stretch a warp of its own (with more heads than warps: twice a warp's share).
+  const int warps = gridDim.x * KA_WARPS;
+  const float all = (float)total * pairs, heads_cut = (float)filled * pairs;
+  auto length_of = [&](int i) {
+    const float room = warps - heads_cut * (i * (1.f / (KA_CANDIDATES - 1)));
+    return fmaxf((float)KA_MIN_UNITS, room >= 0.5f * warps ? all / room : 2.f * all / warps);
+  };
+  auto pieces_of = [&](int units, float inverse) {
+    return units ? min(max((int)ceilf(units * inverse), 1), units) : 0;
+  };
+#pragma unroll
+  for (int i = 0; i < KA_CANDIDATES; ++i) {
+    const float inverse = 1.f / length_of(i);
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < MINE; ++k) n += pieces_of(units[k], inverse);
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) sums[warp][i] = n;
+  }
+  __syncthreads();
+  float inverse = 1.f / length_of(KA_CANDIDATES - 1);
+#pragma unroll
+  for (int i = KA_CANDIDATES - 2; i >= 0; --i) {
+    int n = 0;
+#pragma unroll
+    for (int w = 0; w < KA_WARPS; ++w) n += sums[w][i];
+    if (n * pairs <= warps) inverse = 1.f / length_of(i);
+  }
+  __syncthreads();
+  int stretches = 0, cut = 0;
+#pragma unroll
+  for (int k = 0; k < MINE; ++k) {
+    const int e = tid + k * KA_THREADS, mine = pieces_of(units[k], inverse);
+    const int n = mine * pairs, c = mine > 1 ? n : 0;
+    int incl_n = n, incl_c = c;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += up;
+      const int up_n = __shfl_up_sync(0xffffffffu, incl_n, o), up_c = __shfl_up_sync(0xffffffffu, incl_c, o);
+      if (lane >= o) incl_n += up_n, incl_c += up_c;
     }
-    if (lane == 31) warp_sum_of[warp] = incl;
+    if (lane == 31) sums[warp][0] = incl_n, sums[warp][1] = incl_c;
     __syncthreads();
-    int before = running;
+    int before_n = stretches, before_c = cut;
+#pragma unroll
     for (int w = 0; w < KA_WARPS; ++w) {
-      if (w < warp) before += warp_sum_of[w];
-      running += warp_sum_of[w];
+      if (w < warp) before_n += sums[w][0], before_c += sums[w][1];
+      stretches += sums[w][0], cut += sums[w][1];
     }
     if (e < a.n_tiles) {
-      start[e] = before + incl - n;
+      pieces[e] = mine;
+      start[e] = before_n + incl_n - n;
+      cut_start[e] = before_c + incl_c - c;
       if (n == 0 && blockIdx.x == 0)
         for (int i = 0; i < pairs; ++i) a.desc[e * pairs + i] = make_int4(-1, -1, 0, 0);
     }
     __syncthreads();
+    if ((k + 1) * KA_THREADS >= a.n_tiles) break;
   }
-  if (tid == 0) start[a.n_tiles] = running;
-  __syncthreads();
-  const int total = running;
-  const int parts = min(max(total / KA_MIN_UNITS, 1), (int)gridDim.x * KA_WARPS);
-  const int me = warp * gridDim.x + blockIdx.x;             // (few stretches lie on as many SMs)
-  if (me >= parts || total == 0) return;
-  const int each = total / parts, longer = total - each * parts;         // the first `longer` have one more
-  int x = me * each + min(me, longer);
-  const int x_end = x + each + (me < longer ? 1 : 0);
 
-  int e;                                                    // the tile that holds unit x
-  {
-    int lo = 0, hi = a.n_tiles - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (start[mid] <= x) lo = mid; else hi = mid - 1;
-    }
-    e = lo;
-  }
   const float scale_log2 = a.scale * 1.44269504088896341f;
   const float score_up = scale_log2 * DOWN;
   const int eighths = a.page_size / KV4_EIGHTH;
   unsigned char* my_ring = smem + (size_t)warp * KA_STAGES * UNIT_BYTES;
 
-  while (x < x_end) {
-    while (start[e + 1] <= x) ++e;
+  // (few stretches lie on as many SMs)
+  for (int x = warp * gridDim.x + blockIdx.x; x < stretches; x += warps) {
+    int e = 0;                                              // the tile of stretch x: the last that begins at or before it
+    {
+      int hi = a.n_tiles - 1;
+      while (e < hi) {
+        const int mid = (e + hi + 1) >> 1;
+        if (start[mid] <= x) e = mid; else hi = mid - 1;
+      }
+    }
     const KaTile t = tiles[e];
     const KaSpan span = ka_span(t, a.window, a.keep);
-    const int rel = x - start[e], pair = rel / span.units, u0 = rel - pair * span.units;
-    const int mine = min(span.units - u0, x_end - x);
+    const int n_pieces = pieces[e];
+    const int pair = (x - start[e]) / n_pieces, piece = x - start[e] - pair * n_pieces;
+    const int each = span.units / n_pieces, longer = span.units - each * n_pieces;
+    const int u0 = piece * each + min(piece, longer), mine = each + (piece < longer ? 1 : 0);
     const int h = pair / a.chunks, head0 = h * a.group + (pair - h * a.chunks) * a.chunk;
     const int heads = min(a.chunk, (h + 1) * a.group - head0);
     const int last = t.pos0 + t.ntok - 1;
-    const int first_seen = a.window > 0 ? max(0, t.pos0 - a.window + 1) : 0;
     const int* table = a.block_tables + (size_t)t.b * a.table_stride;
-    x += mine;
-    const bool begins = u0 == 0, ends = u0 + mine == span.units;
 
     uint4 raw[NT][KW];                                      // the queries, under way while pages are looked up
 #pragma unroll
@@ -229,43 +275,47 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
       return (u < span.kept ? u : span.from + u - span.kept) * KA_UNIT;
     };
     int rec0 = 0, rec1 = 0;                                 // of unit (32 n + lane): its two records
+    auto record = [&](int j, int n) {                       // of keys j .. j + n - 1, n a page's at most
+      if (!kv4_seen(j, j + n - 1, t.pos0, last, a.window, a.keep)) return 0;
+      const int at = j / a.page_size, page = table[at];
+      if (page >= 0 && page < a.num_pages) return (page * a.nkv + h) * eighths + (j - at * a.page_size) / 8;
+      atomicOr(a.err, BF_ERR_PAGE);
+      return 0;
+    };
     auto look_up = [&](int i) {
       rec0 = rec1 = 0;
       if (i >= mine) return;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int j = unit_key(i) + half * 8;
-        int rec = 0;
-        if (kv4_seen(j, j + 7, t.pos0, last, a.window, a.keep)) {
-          const int at = j / a.page_size;
-          const int page = at < a.table_width ? table[at] : -1;
-          if (page < 0 || page >= a.num_pages) {
-            atomicOr(a.err, BF_ERR_PAGE);
-          } else {
-            rec = (page * a.nkv + h) * eighths + (j - at * a.page_size) / 8;
-          }
-        }
-        if (half) rec1 = rec; else rec0 = rec;
+      if (eighths > 1) {
+        rec0 = record(unit_key(i), KA_UNIT);
+      } else {
+        rec0 = record(unit_key(i), 8);
+        rec1 = record(unit_key(i) + 8, 8);
       }
     };
     auto issue = [&](int i) {
-      if (i < mine) {
-        if ((i & 31) == 0) look_up(i + lane);
-        const unsigned char* s0 = a.cache + (size_t)__shfl_sync(0xffffffffu, rec0, i & 31) * REC;
-        const unsigned char* s1 = a.cache + (size_t)__shfl_sync(0xffffffffu, rec1, i & 31) * REC;
-        unsigned char* dst = my_ring + (i % KA_STAGES) * UNIT_BYTES;
-        s1 -= REC;
+      if (i >= mine) return;
+      unsigned char* dst = my_ring + (i % KA_STAGES) * UNIT_BYTES + lane * 16;
+      const unsigned char* s0 = a.cache + (size_t)__shfl_sync(0xffffffffu, rec0, i & 31) * REC + lane * 16;
+      if (eighths > 1) {
 #pragma unroll
-        for (int c0 = 0; c0 < UNIT_BYTES / 16; c0 += 32) {
-          const int c = c0 + lane;
-          if (c0 + 32 <= UNIT_BYTES / 16 || c < UNIT_BYTES / 16)
-            cp_async16(dst + c * 16, (c < REC / 16 ? s0 : s1) + c * 16, 16);
-        }
+        for (int c0 = 0; c0 < UNIT_BYTES / 16; c0 += 32)
+          if (c0 + 32 <= UNIT_BYTES / 16 || c0 + lane < UNIT_BYTES / 16) cp_async16(dst + c0 * 16, s0 + c0 * 16, 16);
+      } else {                                              // the second record lies in another page
+        const unsigned char* s1 = a.cache + (size_t)__shfl_sync(0xffffffffu, rec1, i & 31) * REC - REC + lane * 16;
+#pragma unroll
+        for (int c0 = 0; c0 < UNIT_BYTES / 16; c0 += 32)
+          if (c0 + 32 <= UNIT_BYTES / 16 || c0 + lane < UNIT_BYTES / 16)
+            cp_async16(dst + c0 * 16, (c0 + lane < REC / 16 ? s0 : s1) + c0 * 16, 16);
       }
+    };
+    auto issue_step = [&](int i) {
+      if ((i & 31) == 0) look_up(i + lane);
+      issue(i);
+      issue(i + 1);
       cp_async_commit();
     };
-#pragma unroll
-    for (int i = 0; i < KA_STAGES - 2; ++i) issue(i);
+    issue_step(0);
+    issue_step(2);
 
     // ---- queries: operand b of the scores' product, and their sums per group
     unsigned qf[NT][KW][4], ql[NT][2];
@@ -434,7 +484,7 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
     // two units at a time, so that one's latencies lie under the other's work
     auto step = [&](int i, auto edge) {
       const unsigned char* sa = my_ring + (i % KA_STAGES) * UNIT_BYTES;
-      const unsigned char* sb = my_ring + ((i + 1) % KA_STAGES) * UNIT_BYTES;
+      const unsigned char* sb = sa + UNIT_BYTES;
       float s[2][NT][4];
       scores(s[0], sa);
       scores(s[1], sb);
@@ -492,23 +542,27 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
       values(s[0], sa, edge, hidden[0]);
       values(s[1], sb, edge, hidden[1]);
     };
-    // every key of a unit seen by every column: not so at the context's end and at the window's edges
-    auto whole = [&](int i) {
-      const int key = unit_key(i);
-      return i < mine && key + KA_UNIT - 1 <= t.pos0 &&
-             (a.window <= 0 || key > last - a.window || key + KA_UNIT <= a.keep);
-    };
+    // units whose every key every column sees: not so at the context's end and at the window's edges
+    const int inner = span.kept - u0;                       // (units of kept tokens count as edges)
+    const int from_i = a.window > 0 ? inner + max(0, (max(0, last - a.window + 1) + KA_UNIT - 1) / KA_UNIT - span.from) : 0;
+    const int to_i = min(mine, inner + (t.pos0 + 1) / KA_UNIT - span.from);
     for (int i = 0; i < mine; i += 2) {
-      cp_async_wait<KA_STAGES - 4>();
+      cp_async_wait<1>();
       __syncwarp();
-      issue(i + KA_STAGES - 2);                             // into the places of the two units before these
-      issue(i + KA_STAGES - 1);
-      if (whole(i) && whole(i + 1)) step(i, Bool<false>()); else step(i, Bool<true>());
+      if (i >= from_i && i + 2 <= to_i) step(i, Bool<false>()); else step(i, Bool<true>());
+      __syncwarp();
+      issue_step(i + 4);
     }
     cp_async_wait<0>();
 
     // ---- the result: lane (r, q4) has numbers 8 r .. 8 r + 7 of every group, of two columns of every eight
-    const int slot = 2 * me + (begins ? 1 : 0);
+    const bool whole = n_pieces == 1;
+    const int slot = cut_start[e] + pair * n_pieces + piece;
+    if (!whole && cut_start[e] + (pair + 1) * n_pieces > a.slots) {        // no room: the lengths above do not let it come to this
+      if (lane == 0) atomicOr(a.err, BF_ERR_SPLITS);
+      if (piece == 0 && lane == 0) a.desc[e * pairs + pair] = make_int4(-1, -1, 0, 0);
+      continue;
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -522,8 +576,8 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
         }
         if (ti >= t.ntok || gi >= heads) continue;
         const float sum = l[nt][c] * (1.f / UP);
-        const float f = begins && ends ? 1.f / sum : 1.f;
-        if (!(begins && ends) && r == 0) a.part_ml[slot * COLS + n] = make_float2(m[nt][c], sum);
+        const float f = whole ? 1.f / sum : 1.f;
+        if (!whole && r == 0) a.part_ml[slot * COLS + n] = make_float2(m[nt][c], sum);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
           const float base = fmaf(-8.f * DOWN, ps[nt][g][c], corr[nt][g][c] * (1.f / UP));
@@ -533,7 +587,7 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
             v[2 * k] = fmaf(o[nt][4 * g + k][c], DOWN, base) * f;
             v[2 * k + 1] = fmaf(o[nt][4 * g + k][c + 2], DOWN / 16, base) * f;
           }
-          if (begins && ends) {
+          if (whole) {
             *reinterpret_cast<uint4*>(a.out + (long long)(t.row0 + ti) * a.out_stride + (size_t)(head0 + gi) * D + g * 64 + r * 8) =
                 make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
           } else {
@@ -543,11 +597,8 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
           }
         }
       }
-    if (begins && lane == 0) {
-      const int at = start[e] + (pair + 1) * span.units - 1, edge = longer * (each + 1);   // the last unit's owner
-      const int owner = at < edge ? at / (each + 1) : longer + (at - edge) / each;
-      a.desc[e * pairs + pair] = ends ? make_int4(-1, -1, 0, 0) : make_int4(me, owner, t.row0, t.ntok);
-    }
+    if (piece == 0 && lane == 0)
+      a.desc[e * pairs + pair] = whole ? make_int4(-1, -1, 0, 0) : make_int4(slot, n_pieces, t.row0, t.ntok);
   }
 }
 
@@ -567,8 +618,8 @@ kv4_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ pa
   const int n = blockIdx.y, ti = n / chunk, gi = n - ti * chunk;
   if (ti >= d.w || gi >= min(chunk, (h + 1) * group - head0)) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int parts = d.y - d.x + 1;
-  auto slot = [&](int i) { return (size_t)(i == 0 ? 2 * d.x + 1 : 2 * (d.x + i)) * cols + n; };
+  const int parts = d.y;
+  auto slot = [&](int i) { return (size_t)(d.x + i) * cols + n; };
   float top = -INFINITY;
   for (int i = lane; i < parts; i += 32) top = fmaxf(top, part_ml[slot(i)].x);
   top = warp_max(top);
@@ -598,8 +649,8 @@ kv4_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ pa
 
 template <int D, int NT>
 static int ka_launch(KaArgs a, int total_tiles, int ctas, cudaStream_t stream) {
-  constexpr size_t smem = (size_t)KA_WARPS * KA_STAGES * 2 * kv4_record(D) + (KA_MAX_TILES + 4) * 4 +
-                          KA_MAX_TILES * sizeof(KaTile);
+  constexpr size_t smem = (size_t)KA_WARPS * KA_STAGES * 2 * kv4_record(D) +
+                          KA_MAX_TILES * (sizeof(KaTile) + 4) + 2 * (KA_MAX_TILES + 4) * 4;
   static bool configured[BF_MAX_DEVICES];
   const int dev = bf_current_device();
   if (!configured[dev]) {
@@ -642,10 +693,13 @@ static KaShape ka_shape(int group, int d, int max_rows) {
   return s;
 }
 
+static int ka_ctas(const KaShape& s, int d, int sms) { return sms * (d <= 128 && s.nt == 1 ? 2 : 1); }
+static long long ka_slots(const KaShape& s, int d, int sms) { return ka_ctas(s, d, sms) * KA_WARPS + KA_SPARE_SLOTS; }
+
 // Bytes of scratch that a call needs (16-byte aligned): partial results and a note per (tile, head).
 BF_EXPORT long long bf_kv4_attention_scratch(int n, int max_rows, int nh, int nkv, int d, int sms) {
   const KaShape s = ka_shape(nh / nkv, d, max_rows);
-  const long long slots = 2LL * sms * KA_WARPS * (d <= 128 && s.nt == 1 ? 2 : 1);
+  const long long slots = ka_slots(s, d, sms);
   long long tiles = (long long)n * ((max_rows + s.tokens - 1) / s.tokens);
   if (tiles > KA_MAX_TILES) tiles = KA_MAX_TILES;
   return slots * 8 * s.nt * (d * 4 + 8) + tiles * nkv * s.chunks * 16;
@@ -660,7 +714,7 @@ BF_EXPORT int bf_kv4_attention(const void* q, long long q_stride, const void* ca
   if (n <= 0 || max_rows <= 0) return 0;
   if ((long long)num_pages * nkv * (page_size / 8) > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
   const KaShape s = ka_shape(nh / nkv, d, max_rows);
-  const int ctas = sms * (d <= 128 && s.nt == 1 ? 2 : 1);
+  const int ctas = ka_ctas(s, d, sms);
   KaArgs a = {};
   a.q = (const __nv_bfloat16*)q, a.q_stride = q_stride, a.cache = (const unsigned char*)cache;
   a.rows = rows, a.seq_of_token = seq_of_token, a.positions = positions, a.items = items;
@@ -670,9 +724,10 @@ BF_EXPORT int bf_kv4_attention(const void* q, long long q_stride, const void* ca
   a.out = (__nv_bfloat16*)out, a.out_stride = out_stride;
   a.nh = nh, a.nkv = nkv, a.group = nh / nkv, a.chunk = s.chunk, a.chunks = s.chunks, a.tokens = s.tokens;
   a.page_size = page_size, a.num_pages = num_pages, a.window = window, a.keep = keep, a.scale = scale;
+  a.slots = (int)ka_slots(s, d, sms);
   a.part_o = (float*)scratch;
-  a.part_ml = (float2*)(a.part_o + 2LL * ctas * KA_WARPS * 8 * s.nt * d);
-  a.desc = (int4*)(a.part_ml + 2LL * ctas * KA_WARPS * 8 * s.nt);
+  a.part_ml = (float2*)(a.part_o + (long long)a.slots * 8 * s.nt * d);
+  a.desc = (int4*)(a.part_ml + (long long)a.slots * 8 * s.nt);
   a.err = err;
   const long long tiles = (long long)n * a.tiles_per_item;
   if (tiles > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
