@@ -29,14 +29,14 @@
 #include "kv4.cuh"
 #include "mma_utils.cuh"
 
-#define KA_WARPS 8
-#define KA_THREADS (KA_WARPS * 32)
 #define KA_STAGES 4                        // units: two steps
 #define KA_MAX_TILES 512                   // of one launch
 #define KA_UNIT 16                         // keys
 #define KA_SPARE_SLOTS 32                  // (the counts of stretches are rounded sums)
 #define KA_MIN_UNITS 2                     // a stretch's length at least
-#define KA_CANDIDATES 8                    // lengths of stretches that are tried
+
+// Warps of a CTA, one CTA an SM: sixteen where 128 registers hold a tile.
+__host__ __device__ constexpr int ka_warps(int d, int nt) { return d <= 128 && nt == 1 ? 16 : 8; }
 
 struct KaArgs {
   const __nv_bfloat16* q;
@@ -108,19 +108,19 @@ __device__ __forceinline__ void ka_lds(unsigned (&w)[WORDS], const unsigned char
 }
 
 template <int D, int NT>
-__global__ void __launch_bounds__(KA_THREADS, (D <= 128 && NT == 1) ? 2 : 1)
+__global__ void __launch_bounds__(32 * ka_warps(D, NT), 1)
 kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   constexpr int NG = D / KV4_GROUP, REC = kv4_record(D), UNIT_BYTES = 2 * REC;
-  constexpr int KW = D / 32, COLS = 8 * NT;
+  constexpr int KW = D / 32, COLS = 8 * NT, WARPS = ka_warps(D, NT);
   constexpr float UP = 1.8446744073709551616e19f;           // 2^64
   constexpr float DOWN = 5.90295810358705651712e20f;        // 2^69
-  constexpr unsigned M0 = 0x000f000fu, M4 = 0x00f000f0u, ONES = 0x00010001u;
+  constexpr unsigned M0 = 0x000f000fu, M4 = 0x00f000f0u, M8 = 0x00ff00ffu, ONES = 0x00010001u;
   extern __shared__ __align__(128) unsigned char smem[];
-  KaTile* tiles = reinterpret_cast<KaTile*>(smem + (size_t)KA_WARPS * KA_STAGES * UNIT_BYTES);
-  int* pieces = reinterpret_cast<int*>(tiles + KA_MAX_TILES);              // stretches of a head of the tile
-  int* start = pieces + KA_MAX_TILES;                                      // the tile's first stretch
+  KaTile* tiles = reinterpret_cast<KaTile*>(smem + (size_t)WARPS * KA_STAGES * UNIT_BYTES);
+  int* units_of = reinterpret_cast<int*>(tiles + KA_MAX_TILES);            // of a head of the tile
+  int* start = units_of + KA_MAX_TILES;                                    // the tile's first stretch
   int* cut_start = start + KA_MAX_TILES + 4;                               // and the same of those that are cut
-  __shared__ int sums[KA_WARPS][KA_CANDIDATES + 1];
+  __shared__ int sums[WARPS];
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r = lane >> 2, q4 = lane & 3;
@@ -128,108 +128,86 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   bf_pdl_trigger();
   bf_pdl_wait();
 
-  // ---- tiles, and how their units are cut.  A thread has tiles tid and tid + KA_THREADS.
-  constexpr int MINE = KA_MAX_TILES / KA_THREADS;
-  int units[MINE];
-  int total = 0, filled = 0;
-#pragma unroll
-  for (int k = 0; k < MINE; ++k) {
-    const int e = tid + k * KA_THREADS;
-    KaTile t = {0, 0, 0, 0};
-    if (e < a.n_tiles) {
-      if (a.items) {
-        const int id = a.first_tile + e, i = id / a.tiles_per_item, s = id - i * a.tiles_per_item;
-        const int* it = a.items + 4 * (size_t)i;
-        t.b = it[0];
-        t.row0 = it[1] + s * a.tokens;
-        t.pos0 = it[3] + s * a.tokens;
-        t.ntok = min(it[2] - s * a.tokens, a.tokens);
-      } else {
-        const int n = a.first_tile + e;
-        t.row0 = a.rows ? a.rows[n] : n;
-        const bool ok = t.row0 >= 0 && t.row0 < a.T;
-        t.b = ok ? a.seq_of_token[t.row0] : -1;
-        t.pos0 = ok ? a.positions[t.row0] : 0;
-        t.ntok = 1;
-      }
-      if (t.ntok > 0 && (t.b < 0 || t.b >= a.table_rows || t.row0 < 0 || t.row0 + t.ntok > a.T || t.pos0 < 0 ||
-                         (long long)t.pos0 + t.ntok > (long long)a.table_width * a.page_size)) {
-        if (blockIdx.x == 0) atomicOr(a.err, BF_ERR_PAGE);
-        t.ntok = 0;
-      }
-      tiles[e] = t;
+  // ---- tiles, and how their units are cut.  (Loops, not unrolled: what a launch runs once waits for its
+  // instructions most of all.)
+#pragma unroll 1
+  for (int e = tid; e < a.n_tiles; e += 32 * WARPS) {
+    KaTile t;
+    if (a.items) {
+      const int id = a.first_tile + e, i = id / a.tiles_per_item, s = id - i * a.tiles_per_item;
+      const int* it = a.items + 4 * (size_t)i;
+      t.b = it[0];
+      t.row0 = it[1] + s * a.tokens;
+      t.pos0 = it[3] + s * a.tokens;
+      t.ntok = min(it[2] - s * a.tokens, a.tokens);
+    } else {
+      const int n = a.first_tile + e;
+      t.row0 = a.rows ? a.rows[n] : n;
+      const bool ok = t.row0 >= 0 && t.row0 < a.T;
+      t.b = ok ? a.seq_of_token[t.row0] : -1;
+      t.pos0 = ok ? a.positions[t.row0] : 0;
+      t.ntok = 1;
     }
-    units[k] = ka_span(t, a.window, a.keep).units;
-    total += units[k];
-    filled += units[k] > 0;
+    if (t.ntok > 0 && (t.b < 0 || t.b >= a.table_rows || t.row0 < 0 || t.row0 + t.ntok > a.T || t.pos0 < 0 ||
+                       (long long)t.pos0 + t.ntok > (long long)a.table_width * a.page_size)) {
+      if (blockIdx.x == 0) atomicOr(a.err, BF_ERR_PAGE);
+      t.ntok = 0;
+    }
+    tiles[e] = t;
+    const int n = ka_span(t, a.window, a.keep).units;
+    units_of[e] = n;
+    if (n == 0 && blockIdx.x == 0)
+      for (int i = 0; i < pairs; ++i) a.desc[e * pairs + i] = make_int4(-1, -1, 0, 0);
   }
+  __syncthreads();
+  // A tile's heads together get pieces in proportion to their units, one each at least.  With `rate`
+  // pieces a unit that makes at most rate total + heads of them: warp w tries a rate, and the highest that
+  // gives every piece a warp of its own is taken (with more heads than warps: half a warp's share each).
+  const int warps = gridDim.x * WARPS;
+  int total = 0, filled = 0;
+#pragma unroll 1
+  for (int e = lane; e < a.n_tiles; e += 32) total += units_of[e], filled += units_of[e] > 0;
   total = __reduce_add_sync(0xffffffffu, total);
   filled = __reduce_add_sync(0xffffffffu, filled);
-  if (lane == 0) sums[warp][0] = total, sums[warp][1] = filled;
-  __syncthreads();
-  total = filled = 0;
-#pragma unroll
-  for (int w = 0; w < KA_WARPS; ++w) total += sums[w][0], filled += sums[w][1];
-  __syncthreads();
-  // Stretches of `length` make at most total / length + filled of a head; the shortest of a few lengths
-  // that gives every stretch a warp of its own (with more heads than warps: twice a warp's share).
-  const int warps = gridDim.x * KA_WARPS;
-  const float all = (float)total * pairs, heads_cut = (float)filled * pairs;
-  auto length_of = [&](int i) {
-    const float room = warps - heads_cut * (i * (1.f / (KA_CANDIDATES - 1)));
-    return fmaxf((float)KA_MIN_UNITS, room >= 0.5f * warps ? all / room : 2.f * all / warps);
+  auto rate_of = [&](int i) {
+    const float room = warps - (float)filled * pairs * (i * (1.f / (WARPS - 1)));
+    return fminf(1.f / KA_MIN_UNITS, (room >= 0.5f * warps ? room : 0.5f * warps) / fmaxf((float)total * pairs, 1.f));
   };
-  auto pieces_of = [&](int units, float inverse) {
-    return units ? min(max((int)ceilf(units * inverse), 1), units) : 0;
-  };
-#pragma unroll
-  for (int i = 0; i < KA_CANDIDATES; ++i) {
-    const float inverse = 1.f / length_of(i);
+  auto pieces_of = [&](int units, float rate) { return units ? max((int)(units * (rate * pairs)), pairs) : 0; };
+  {
+    const float rate = rate_of(warp);
     int n = 0;
-#pragma unroll
-    for (int k = 0; k < MINE; ++k) n += pieces_of(units[k], inverse);
+#pragma unroll 1
+    for (int e = lane; e < a.n_tiles; e += 32) n += pieces_of(units_of[e], rate);
     n = __reduce_add_sync(0xffffffffu, n);
-    if (lane == 0) sums[warp][i] = n;
+    if (lane == 0) sums[warp] = n;
   }
   __syncthreads();
-  float inverse = 1.f / length_of(KA_CANDIDATES - 1);
+  const unsigned fits = __ballot_sync(0xffffffffu, lane < WARPS && sums[lane < WARPS ? lane : 0] <= warps);
+  const float rate = rate_of(fits ? __ffs(fits) - 1 : WARPS - 1);
+  if (warp == 0) {
+    int n_before = 0, c_before = 0;
+#pragma unroll 1
+    for (int e0 = 0; e0 < a.n_tiles; e0 += 32) {
+      const int e = e0 + lane, n = e < a.n_tiles ? pieces_of(units_of[e], rate) : 0;
+      const int c = n >= 2 * pairs ? n : 2 * (n - (n > 0 ? pairs : 0));    // pieces of heads that are cut
+      int n_incl = n, c_incl = c;
 #pragma unroll
-  for (int i = KA_CANDIDATES - 2; i >= 0; --i) {
-    int n = 0;
-#pragma unroll
-    for (int w = 0; w < KA_WARPS; ++w) n += sums[w][i];
-    if (n * pairs <= warps) inverse = 1.f / length_of(i);
+      for (int o = 1; o < 32; o <<= 1) {
+        const int n_up = __shfl_up_sync(0xffffffffu, n_incl, o), c_up = __shfl_up_sync(0xffffffffu, c_incl, o);
+        if (lane >= o) n_incl += n_up, c_incl += c_up;
+      }
+      if (e < a.n_tiles) {
+        start[e] = n_before + n_incl - n;
+        cut_start[e] = c_before + c_incl - c;
+      }
+      n_before += __shfl_sync(0xffffffffu, n_incl, 31);
+      c_before += __shfl_sync(0xffffffffu, c_incl, 31);
+    }
+    if (lane == 0) start[a.n_tiles] = n_before;
   }
   __syncthreads();
-  int stretches = 0, cut = 0;
-#pragma unroll
-  for (int k = 0; k < MINE; ++k) {
-    const int e = tid + k * KA_THREADS, mine = pieces_of(units[k], inverse);
-    const int n = mine * pairs, c = mine > 1 ? n : 0;
-    int incl_n = n, incl_c = c;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int up_n = __shfl_up_sync(0xffffffffu, incl_n, o), up_c = __shfl_up_sync(0xffffffffu, incl_c, o);
-      if (lane >= o) incl_n += up_n, incl_c += up_c;
-    }
-    if (lane == 31) sums[warp][0] = incl_n, sums[warp][1] = incl_c;
-    __syncthreads();
-    int before_n = stretches, before_c = cut;
-#pragma unroll
-    for (int w = 0; w < KA_WARPS; ++w) {
-      if (w < warp) before_n += sums[w][0], before_c += sums[w][1];
-      stretches += sums[w][0], cut += sums[w][1];
-    }
-    if (e < a.n_tiles) {
-      pieces[e] = mine;
-      start[e] = before_n + incl_n - n;
-      cut_start[e] = before_c + incl_c - c;
-      if (n == 0 && blockIdx.x == 0)
-        for (int i = 0; i < pairs; ++i) a.desc[e * pairs + i] = make_int4(-1, -1, 0, 0);
-    }
-    __syncthreads();
-    if ((k + 1) * KA_THREADS >= a.n_tiles) break;
-  }
+  const int stretches = start[a.n_tiles];
 
   const float scale_log2 = a.scale * 1.44269504088896341f;
   const float score_up = scale_log2 * DOWN;
@@ -248,8 +226,11 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
     }
     const KaTile t = tiles[e];
     const KaSpan span = ka_span(t, a.window, a.keep);
-    const int n_pieces = pieces[e];
-    const int pair = (x - start[e]) / n_pieces, piece = x - start[e] - pair * n_pieces;
+    const int y = x - start[e], fewer = (start[e + 1] - start[e]) / pairs, more = start[e + 1] - start[e] - fewer * pairs;
+    const bool longer_cut = y < more * (fewer + 1);         // the first `more` heads have a piece more
+    const int n_pieces = fewer + (longer_cut ? 1 : 0);
+    const int first_y = longer_cut ? 0 : more * (fewer + 1);
+    const int piece = (y - first_y) % n_pieces, pair = (longer_cut ? 0 : more) + (y - first_y) / n_pieces;
     const int each = span.units / n_pieces, longer = span.units - each * n_pieces;
     const int u0 = piece * each + min(piece, longer), mine = each + (piece < longer ? 1 : 0);
     const int h = pair / a.chunks, head0 = h * a.group + (pair - h * a.chunks) * a.chunk;
@@ -322,7 +303,7 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
     int pcol[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float sums[4] = {0.f, 0.f, 0.f, 0.f};
+      float qsum[NG] = {};
 #pragma unroll
       for (int w = 0; w < KW; ++w) {
         const unsigned* u = &raw[nt][w].x;
@@ -333,17 +314,17 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
           f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sums[w >> 1] += f[i];
+        for (int i = 0; i < 8; ++i) qsum[w >> 1] += f[i];
         qf[nt][w][0] = pack_bf16(f[0] * UP, f[4] * UP);
         qf[nt][w][1] = pack_bf16(f[1] * (UP / 16), f[5] * (UP / 16));
         qf[nt][w][2] = pack_bf16(f[2] * UP, f[6] * UP);
         qf[nt][w][3] = pack_bf16(f[3] * (UP / 16), f[7] * (UP / 16));
       }
       // the sums meet the keys' lowest values in one product: lane q4's share is their q4-th bfloat16 term
-      float term[4];
+      float term[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        float v = sums[g];
+      for (int g = 0; g < NG; ++g) {
+        float v = qsum[g];
         v += __shfl_xor_sync(0xffffffffu, v, 1);
         v += __shfl_xor_sync(0xffffffffu, v, 2);
         v *= scale_log2;
@@ -470,9 +451,9 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
         for (int half = 0; half < 2; ++half) {
           const unsigned sel = half ? 0x7632 : 0x5410;
           const unsigned x0 = __byte_perm(v0[g], v0[NG + g], sel), x1 = __byte_perm(v1[g], v1[NG + g], sel);
-          const unsigned h0 = x0 >> 8, h1 = x1 >> 8;
-          const unsigned a0[4] = {x0 & M0, x0 & M4, x1 & M0, x1 & M4};
-          const unsigned a1[4] = {h0 & M0, h0 & M4, h1 & M0, h1 & M4};
+          const unsigned y0 = x0 & M8, y1 = x1 & M8, z0 = __byte_perm(x0, 0u, 0x4341), z1 = __byte_perm(x1, 0u, 0x4341);
+          const unsigned a0[4] = {y0 & M0, y0, y1 & M0, y1};
+          const unsigned a1[4] = {z0 & M0, z0, z1 & M0, z1};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             mma_bf16_16816(o[nt][4 * g + 2 * half], a0, b0[nt], b1[nt]);
@@ -557,8 +538,8 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
 
     // ---- the result: lane (r, q4) has numbers 8 r .. 8 r + 7 of every group, of two columns of every eight
     const bool whole = n_pieces == 1;
-    const int slot = cut_start[e] + pair * n_pieces + piece;
-    if (!whole && cut_start[e] + (pair + 1) * n_pieces > a.slots) {        // no room: the lengths above do not let it come to this
+    const int slot = cut_start[e] + y;
+    if (!whole && slot - piece + n_pieces > a.slots) {        // no room: the lengths above do not let it come to this
       if (lane == 0) atomicOr(a.err, BF_ERR_SPLITS);
       if (piece == 0 && lane == 0) a.desc[e * pairs + pair] = make_int4(-1, -1, 0, 0);
       continue;
@@ -585,7 +566,7 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             v[2 * k] = fmaf(o[nt][4 * g + k][c], DOWN, base) * f;
-            v[2 * k + 1] = fmaf(o[nt][4 * g + k][c + 2], DOWN / 16, base) * f;
+            v[2 * k + 1] = fmaf(o[nt][4 * g + k][c + 2] - o[nt][4 * g + k][c], DOWN / 16, base) * f;
           }
           if (whole) {
             *reinterpret_cast<uint4*>(a.out + (long long)(t.row0 + ti) * a.out_stride + (size_t)(head0 + gi) * D + g * 64 + r * 8) =
@@ -648,8 +629,9 @@ kv4_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ pa
 }
 
 template <int D, int NT>
-static int ka_launch(KaArgs a, int total_tiles, int ctas, cudaStream_t stream) {
-  constexpr size_t smem = (size_t)KA_WARPS * KA_STAGES * 2 * kv4_record(D) +
+static int ka_launch(KaArgs a, int total_tiles, int sms, cudaStream_t stream) {
+  constexpr int threads = 32 * ka_warps(D, NT);
+  constexpr size_t smem = (size_t)ka_warps(D, NT) * KA_STAGES * 2 * kv4_record(D) +
                           KA_MAX_TILES * (sizeof(KaTile) + 4) + 2 * (KA_MAX_TILES + 4) * 4;
   static bool configured[BF_MAX_DEVICES];
   const int dev = bf_current_device();
@@ -667,7 +649,7 @@ static int ka_launch(KaArgs a, int total_tiles, int ctas, cudaStream_t stream) {
   for (int first = 0; first < total_tiles; first += most) {
     a.first_tile = first;
     a.n_tiles = total_tiles - first < most ? total_tiles - first : most;
-    int e = bf_launch_pdl(kv4_attention_kernel<D, NT>, dim3(ctas), dim3(KA_THREADS), smem, stream, a);
+    int e = bf_launch_pdl(kv4_attention_kernel<D, NT>, dim3(sms), dim3(threads), smem, stream, a);
     if (e) return e;
     e = bf_launch_pdl(kv4_merge_kernel<D>, dim3(a.n_tiles * pairs, 8 * NT), dim3(256), 0, stream,
                       (const float*)a.part_o, (const float2*)a.part_ml, (const int4*)a.desc, a.out, a.out_stride,
@@ -693,8 +675,7 @@ static KaShape ka_shape(int group, int d, int max_rows) {
   return s;
 }
 
-static int ka_ctas(const KaShape& s, int d, int sms) { return sms * (d <= 128 && s.nt == 1 ? 2 : 1); }
-static long long ka_slots(const KaShape& s, int d, int sms) { return ka_ctas(s, d, sms) * KA_WARPS + KA_SPARE_SLOTS; }
+static long long ka_slots(const KaShape& s, int d, int sms) { return (long long)sms * ka_warps(d, s.nt) + KA_SPARE_SLOTS; }
 
 // Bytes of scratch that a call needs (16-byte aligned): partial results and a note per (tile, head).
 BF_EXPORT long long bf_kv4_attention_scratch(int n, int max_rows, int nh, int nkv, int d, int sms) {
@@ -714,7 +695,6 @@ BF_EXPORT int bf_kv4_attention(const void* q, long long q_stride, const void* ca
   if (n <= 0 || max_rows <= 0) return 0;
   if ((long long)num_pages * nkv * (page_size / 8) > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
   const KaShape s = ka_shape(nh / nkv, d, max_rows);
-  const int ctas = ka_ctas(s, d, sms);
   KaArgs a = {};
   a.q = (const __nv_bfloat16*)q, a.q_stride = q_stride, a.cache = (const unsigned char*)cache;
   a.rows = rows, a.seq_of_token = seq_of_token, a.positions = positions, a.items = items;
@@ -731,8 +711,8 @@ BF_EXPORT int bf_kv4_attention(const void* q, long long q_stride, const void* ca
   a.err = err;
   const long long tiles = (long long)n * a.tiles_per_item;
   if (tiles > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
-  if (d == 64) return s.nt == 1 ? ka_launch<64, 1>(a, (int)tiles, ctas, stream) : ka_launch<64, 2>(a, (int)tiles, ctas, stream);
-  if (d == 128) return s.nt == 1 ? ka_launch<128, 1>(a, (int)tiles, ctas, stream) : ka_launch<128, 2>(a, (int)tiles, ctas, stream);
-  if (d == 256) return ka_launch<256, 1>(a, (int)tiles, ctas, stream);
+  if (d == 64) return s.nt == 1 ? ka_launch<64, 1>(a, (int)tiles, sms, stream) : ka_launch<64, 2>(a, (int)tiles, sms, stream);
+  if (d == 128) return s.nt == 1 ? ka_launch<128, 1>(a, (int)tiles, sms, stream) : ka_launch<128, 2>(a, (int)tiles, sms, stream);
+  if (d == 256) return ka_launch<256, 1>(a, (int)tiles, sms, stream);
   return (int)cudaErrorInvalidValue;
 }
