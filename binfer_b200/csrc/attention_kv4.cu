@@ -18,13 +18,14 @@
 // in float.  Everything else is float.
 //
 // Work.  A tile is up to 8 NT columns, a column one query head of one token row; its keys go sixteen at a
-// time (a unit), for every kv head.  A tile and head's units are cut into stretches of nearly equal length,
-// one a warp, as short as the chip's warps allow; a warp fetches its units by itself (16 bytes a lane,
-// asynchronously, two units ahead of the two it computes) and waits for no other.  What is not cut is
-// written by its warp; a cut one leaves a partial result a stretch, which a second kernel adds up in the
-// order of the keys: scratch is one partial a warp whatever the contexts are.  The running maximum moves
-// only when a score passes it by 2^8, which no result depends on beyond rounding and which leaves one vote a
-// step where maxima would take shuffles.
+// time (a unit), for every kv head.  Every warp takes one stretch of units, fetches them by itself (16 bytes
+// a lane, asynchronously, two units ahead of the two it computes) and waits for no other.  Where stretches
+// are short, they are pieces of one tile and head, so that a warp begins but once; where they are long, all
+// units in one row are cut into equal ones, whatever heads they cross.  A tile and head that one warp
+// has whole is written by it; a cut one leaves a partial result a piece, which a second kernel adds up in
+// the order of the keys: scratch is two partials a warp whatever the contexts are.  The running maximum moves
+// only when a score passes it by 2^8, which no result depends on beyond rounding and which leaves one
+// vote a step where maxima would take shuffles.
 #include "common.cuh"
 #include "kv4.cuh"
 #include "mma_utils.cuh"
@@ -32,8 +33,8 @@
 #define KA_STAGES 4                        // units: two steps
 #define KA_MAX_TILES 512                   // of one launch
 #define KA_UNIT 16                         // keys
-#define KA_SPARE_SLOTS 32                  // (the counts of stretches are rounded sums)
 #define KA_MIN_UNITS 2                     // a stretch's length at least
+#define KA_LONG 24                         // units of a stretch from which heads are crossed
 
 // Warps of a CTA, one CTA an SM: sixteen where 128 registers hold a tile.
 __host__ __device__ constexpr int ka_warps(int d, int nt) { return d <= 128 && nt == 1 ? 16 : 8; }
@@ -51,7 +52,8 @@ struct KaArgs {
   int nh, nkv, group, chunk, chunks, tokens;               // query heads per kv head; in a tile; chunks of them
   int page_size, num_pages, window, keep;
   float scale;
-  int slots;
+  unsigned chunk_inverse;                                  // n / chunk = n chunk_inverse >> 8 for n < 16
+  int max_pieces;
   float* part_o;
   float2* part_ml;
   int4* desc;
@@ -118,9 +120,9 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   extern __shared__ __align__(128) unsigned char smem[];
   KaTile* tiles = reinterpret_cast<KaTile*>(smem + (size_t)WARPS * KA_STAGES * UNIT_BYTES);
   int* units_of = reinterpret_cast<int*>(tiles + KA_MAX_TILES);            // of a head of the tile
-  int* start = units_of + KA_MAX_TILES;                                    // the tile's first stretch
-  int* cut_start = start + KA_MAX_TILES + 4;                               // and the same of those that are cut
+  int* start = units_of + KA_MAX_TILES;                                    // the tile's first piece, or unit
   __shared__ int sums[WARPS];
+  __shared__ float rates[WARPS];
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r = lane >> 2, q4 = lane & 3;
@@ -160,63 +162,79 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
       for (int i = 0; i < pairs; ++i) a.desc[e * pairs + i] = make_int4(-1, -1, 0, 0);
   }
   __syncthreads();
-  // A tile's heads together get pieces in proportion to their units, one each at least.  With `rate`
-  // pieces a unit that makes at most rate total + heads of them: warp w tries a rate, and the highest that
-  // gives every piece a warp of its own is taken (with more heads than warps: half a warp's share each).
   const int warps = gridDim.x * WARPS;
-  int total = 0, filled = 0;
+  int total = 0, filled = 0, longest = 0;
 #pragma unroll 1
-  for (int e = lane; e < a.n_tiles; e += 32) total += units_of[e], filled += units_of[e] > 0;
-  total = __reduce_add_sync(0xffffffffu, total);
-  filled = __reduce_add_sync(0xffffffffu, filled);
-  auto rate_of = [&](int i) {
-    const float room = warps - (float)filled * pairs * (i * (1.f / (WARPS - 1)));
-    return fminf(1.f / KA_MIN_UNITS, (room >= 0.5f * warps ? room : 0.5f * warps) / fmaxf((float)total * pairs, 1.f));
+  for (int e = lane; e < a.n_tiles; e += 32) {
+    const int n = units_of[e];
+    total += n, filled += n > 0, longest = max(longest, n);
+  }
+  total = __reduce_add_sync(0xffffffffu, total) * pairs;
+  filled = __reduce_add_sync(0xffffffffu, filled) * pairs;
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  if (total == 0) return;
+  // Short stretches: a tile's heads together get pieces in proportion to their units, one each at least.
+  // With `rate` pieces a unit that makes at most rate total + heads of them: warp w tries a rate, and
+  // the highest that gives every piece a warp of its own is taken.
+  bool aligned = total < KA_LONG * warps && filled < warps;
+  float rate = 0.f;
+  if (aligned) {
+    auto rate_of = [&](int i) {
+      const float room = warps - filled * (i * (1.f / (WARPS - 1)));
+      return fminf(1.f / KA_MIN_UNITS, fmaxf(room, 0.f) / total);
+    };
+    rate = rate_of(warp);
+  }
+  auto pieces_of = [&](int units) {
+    return units ? max(min((int)(units * (rate * pairs)), a.max_pieces * pairs), pairs) : 0;
   };
-  auto pieces_of = [&](int units, float rate) { return units ? max((int)(units * (rate * pairs)), pairs) : 0; };
-  {
-    const float rate = rate_of(warp);
+  if (aligned) {
     int n = 0;
 #pragma unroll 1
-    for (int e = lane; e < a.n_tiles; e += 32) n += pieces_of(units_of[e], rate);
+    for (int e = lane; e < a.n_tiles; e += 32) n += pieces_of(units_of[e]);
     n = __reduce_add_sync(0xffffffffu, n);
-    if (lane == 0) sums[warp] = n;
+    if (lane == 0) sums[warp] = n, rates[warp] = rate;
+    __syncthreads();
+    const unsigned fits = __ballot_sync(0xffffffffu, lane < WARPS && sums[lane < WARPS ? lane : 0] <= warps);
+    aligned = fits != 0;
+    if (aligned) rate = rates[__ffs(fits) - 1];
   }
-  __syncthreads();
-  const unsigned fits = __ballot_sync(0xffffffffu, lane < WARPS && sums[lane < WARPS ? lane : 0] <= warps);
-  const float rate = rate_of(fits ? __ffs(fits) - 1 : WARPS - 1);
   if (warp == 0) {
-    int n_before = 0, c_before = 0;
+    int before = 0;
 #pragma unroll 1
     for (int e0 = 0; e0 < a.n_tiles; e0 += 32) {
-      const int e = e0 + lane, n = e < a.n_tiles ? pieces_of(units_of[e], rate) : 0;
-      const int c = n >= 2 * pairs ? n : 2 * (n - (n > 0 ? pairs : 0));    // pieces of heads that are cut
-      int n_incl = n, c_incl = c;
+      const int e = e0 + lane, u = e < a.n_tiles ? units_of[e] : 0, n = aligned ? pieces_of(u) : u * pairs;
+      int incl = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int n_up = __shfl_up_sync(0xffffffffu, n_incl, o), c_up = __shfl_up_sync(0xffffffffu, c_incl, o);
-        if (lane >= o) n_incl += n_up, c_incl += c_up;
+        const int up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
       }
-      if (e < a.n_tiles) {
-        start[e] = n_before + n_incl - n;
-        cut_start[e] = c_before + c_incl - c;
-      }
-      n_before += __shfl_sync(0xffffffffu, n_incl, 31);
-      c_before += __shfl_sync(0xffffffffu, c_incl, 31);
+      if (e < a.n_tiles) start[e] = before + incl - n;
+      before += __shfl_sync(0xffffffffu, incl, 31);
     }
-    if (lane == 0) start[a.n_tiles] = n_before;
+    if (lane == 0) start[a.n_tiles] = before;
   }
   __syncthreads();
-  const int stretches = start[a.n_tiles];
+  const int me = warp * gridDim.x + blockIdx.x;             // (few stretches lie on as many SMs)
+  int each = 1, longer = 0, x = me, x_end = me + 1;         // pieces: one
+  if (!aligned) {
+    const int least = max(KA_MIN_UNITS, (longest + a.max_pieces - 1) / a.max_pieces);
+    const int parts = min(max(total / least, 1), warps);
+    each = total / parts, longer = total - each * parts;    // the first `longer` have a unit more
+    x = me * each + min(me, longer);
+    x_end = me < parts ? x + each + (me < longer ? 1 : 0) : x;
+  } else if (me >= start[a.n_tiles]) {
+    return;
+  }
 
   const float scale_log2 = a.scale * 1.44269504088896341f;
   const float score_up = scale_log2 * DOWN;
   const int eighths = a.page_size / KV4_EIGHTH;
   unsigned char* my_ring = smem + (size_t)warp * KA_STAGES * UNIT_BYTES;
 
-  // (few stretches lie on as many SMs)
-  for (int x = warp * gridDim.x + blockIdx.x; x < stretches; x += warps) {
-    int e = 0;                                              // the tile of stretch x: the last that begins at or before it
+  while (x < x_end) {
+    int e = 0;                                              // the tile of x: the last that begins at or before it
     {
       int hi = a.n_tiles - 1;
       while (e < hi) {
@@ -226,13 +244,30 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
     }
     const KaTile t = tiles[e];
     const KaSpan span = ka_span(t, a.window, a.keep);
-    const int y = x - start[e], fewer = (start[e + 1] - start[e]) / pairs, more = start[e + 1] - start[e] - fewer * pairs;
-    const bool longer_cut = y < more * (fewer + 1);         // the first `more` heads have a piece more
-    const int n_pieces = fewer + (longer_cut ? 1 : 0);
-    const int first_y = longer_cut ? 0 : more * (fewer + 1);
-    const int piece = (y - first_y) % n_pieces, pair = (longer_cut ? 0 : more) + (y - first_y) / n_pieces;
-    const int each = span.units / n_pieces, longer = span.units - each * n_pieces;
-    const int u0 = piece * each + min(piece, longer), mine = each + (piece < longer ? 1 : 0);
+    const int y = x - start[e];
+    int pair, u0, mine, n_pieces;
+    if (aligned) {
+      const int n = start[e + 1] - start[e], fewer = n / pairs, more = n - fewer * pairs;
+      const int edge = more * (fewer + 1);                  // the first `more` heads have a piece more
+      n_pieces = fewer + (y < edge ? 1 : 0);
+      const int z = y < edge ? y : y - edge;
+      pair = z / n_pieces;
+      const int piece = z - pair * n_pieces, units = span.units / n_pieces, over = span.units - units * n_pieces;
+      if (y >= edge) pair += more;
+      u0 = piece * units + min(piece, over);
+      mine = units + (piece < over ? 1 : 0);
+      x = x_end;
+    } else {
+      pair = y / span.units;
+      u0 = y - pair * span.units;
+      mine = min(span.units - u0, x_end - x);
+      n_pieces = 1;
+      if (mine < span.units) {                              // (asked for where u0 is 0: how many warps share the head)
+        const int at = x - u0 + span.units - 1, edge = longer * (each + 1);
+        n_pieces = (at < edge ? at / (each + 1) : longer + (at - edge) / each) - me + 1;
+      }
+      x += mine;
+    }
     const int h = pair / a.chunks, head0 = h * a.group + (pair - h * a.chunks) * a.chunk;
     const int heads = min(a.chunk, (h + 1) * a.group - head0);
     const int last = t.pos0 + t.ntok - 1;
@@ -241,7 +276,7 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
     uint4 raw[NT][KW];                                      // the queries, under way while pages are looked up
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int n = nt * 8 + r, ti = n / a.chunk, gi = n - ti * a.chunk;
+      const int n = nt * 8 + r, ti = n * a.chunk_inverse >> 8, gi = n - ti * a.chunk;
       const bool on = ti < t.ntok && gi < heads;
       const __nv_bfloat16* src = a.q + (long long)(t.row0 + (on ? ti : 0)) * a.q_stride + (size_t)(head0 + (on ? gi : 0)) * D;
 #pragma unroll
@@ -336,7 +371,7 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
       ql[nt][1] = pack_bf16(term[2], term[3]);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int n2 = nt * 8 + 2 * q4 + i, t2 = n2 / a.chunk;
+        const int n2 = nt * 8 + 2 * q4 + i, t2 = n2 * a.chunk_inverse >> 8;
         pcol[nt][i] = t.pos0 + min(t2, t.ntok - 1);
       }
     }
@@ -537,18 +572,13 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
     cp_async_wait<0>();
 
     // ---- the result: lane (r, q4) has numbers 8 r .. 8 r + 7 of every group, of two columns of every eight
-    const bool whole = n_pieces == 1;
-    const int slot = cut_start[e] + y;
-    if (!whole && slot - piece + n_pieces > a.slots) {        // no room: the lengths above do not let it come to this
-      if (lane == 0) atomicOr(a.err, BF_ERR_SPLITS);
-      if (piece == 0 && lane == 0) a.desc[e * pairs + pair] = make_int4(-1, -1, 0, 0);
-      continue;
-    }
+    const bool whole = mine == span.units;
+    const int slot = 2 * me + (u0 == 0 ? 1 : 0);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int n = nt * 8 + 2 * q4 + c, ti = n / a.chunk, gi = n - ti * a.chunk;
+        const int n = nt * 8 + 2 * q4 + c, ti = n * a.chunk_inverse >> 8, gi = n - ti * a.chunk;
 #pragma unroll
         for (int k = 4; k < 32; k <<= 1) {
           l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], k);
@@ -578,53 +608,85 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
           }
         }
       }
-    if (piece == 0 && lane == 0)
-      a.desc[e * pairs + pair] = whole ? make_int4(-1, -1, 0, 0) : make_int4(slot, n_pieces, t.row0, t.ntok);
+    if (u0 == 0 && lane == 0)
+      a.desc[e * pairs + pair] = whole ? make_int4(-1, -1, 0, 0) : make_int4(me, n_pieces, t.row0, t.ntok);
   }
 }
 
-// Adds up what several warps left of a (tile, head): a block per column, its warps take the partials in turn.
-template <int D>
+// Adds up what several warps left of a (tile, head).  A block of eight warps has 8 / PER columns, PER warps
+// take a column's partials in turn (one where a head has few of them).  Partials and their maxima are
+// asked for together; warps meet in shared memory.
+template <int D, int PER>
 __global__ void __launch_bounds__(256)
 kv4_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml,
                  const int4* __restrict__ desc, __nv_bfloat16* __restrict__ out, long long out_stride, int group,
-                 int chunk, int chunks, int pairs, int cols) {
-  constexpr int N = D / 32;
-  __shared__ float sh_o[8][D], sh_l[8];
+                 int chunk, int chunks, unsigned chunk_inverse, int pairs, int cols) {
+  constexpr int N = D / 32, DEPTH = D == 256 ? 2 : 4;
+  __shared__ float sh_o[PER > 1 ? 8 : 1][D], sh_m[8], sh_l[8];
   bf_pdl_trigger();
   bf_pdl_wait();
   const int4 d = desc[blockIdx.x];
   if (d.x < 0) return;
   const int pair = blockIdx.x % pairs, h = pair / chunks, head0 = h * group + (pair - h * chunks) * chunk;
-  const int n = blockIdx.y, ti = n / chunk, gi = n - ti * chunk;
-  if (ti >= d.w || gi >= min(chunk, (h + 1) * group - head0)) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int parts = d.y;
-  auto slot = [&](int i) { return (size_t)(d.x + i) * cols + n; };
-  float top = -INFINITY;
-  for (int i = lane; i < parts; i += 32) top = fmaxf(top, part_ml[slot(i)].x);
-  top = warp_max(top);
-  float sum = 0.f, acc[N];
+  const int n = blockIdx.y * (8 / PER) + warp / PER, ti = n * chunk_inverse >> 8, gi = n - ti * chunk;
+  if (ti >= d.w || gi >= min(chunk, (h + 1) * group - head0)) return;    // (PER > 1: the whole block)
+  float top = -INFINITY, sum = 0.f, acc[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) acc[k] = 0.f;
-#pragma unroll 4
-  for (int i = warp; i < parts; i += 8) {
-    const float2 ml = part_ml[slot(i)];
-    const float f = ml.x == top ? 1.f : ka_exp2(ml.x - top);
-    const float* src = part_o + slot(i) * D + lane;
-    sum = fmaf(f, ml.y, sum);
+  for (int i0 = warp % PER; i0 < d.y; i0 += PER * DEPTH) {
+    float2 ml[DEPTH];
+    float v[DEPTH][N];
 #pragma unroll
-    for (int k = 0; k < N; ++k) acc[k] = fmaf(f, src[32 * k], acc[k]);
+    for (int j = 0; j < DEPTH; ++j) {
+      const int i = i0 + j * PER;
+      ml[j] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[j][k] = 0.f;
+      if (i < d.y) {
+        const size_t slot = (size_t)(2 * (d.x + i) + (i == 0 ? 1 : 0)) * cols + n;
+        ml[j] = part_ml[slot];
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[j][k] = part_o[slot * D + lane + 32 * k];
+      }
+    }
+    float next = top;
+#pragma unroll
+    for (int j = 0; j < DEPTH; ++j) next = fmaxf(next, ml[j].x);
+    const float f = ka_exp2(top - next);                    // (the first time 0 times 0)
+    sum *= f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) acc[k] *= f;
+#pragma unroll
+    for (int j = 0; j < DEPTH; ++j) {
+      const float g = ml[j].x == next ? 1.f : ka_exp2(ml[j].x - next);
+      sum = fmaf(g, ml[j].y, sum);
+#pragma unroll
+      for (int k = 0; k < N; ++k) acc[k] = fmaf(g, v[j][k], acc[k]);
+    }
+    top = next;
+  }
+  __nv_bfloat16* dst = out + (long long)(d.z + ti) * out_stride + (size_t)(head0 + gi) * D;
+  if (PER == 1) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) dst[lane + 32 * k] = __float2bfloat16_rn(acc[k] / sum);
+    return;
   }
 #pragma unroll
   for (int k = 0; k < N; ++k) sh_o[warp][lane + 32 * k] = acc[k];
-  if (lane == 0) sh_l[warp] = sum;
+  if (lane == 0) sh_m[warp] = top, sh_l[warp] = sum;
   __syncthreads();
   if (threadIdx.x < D) {
-    float v = 0.f, w = 0.f;
+    float most = sh_m[0], v = 0.f, w = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v += sh_o[k][threadIdx.x], w += sh_l[k];
-    out[(long long)(d.z + ti) * out_stride + (size_t)(head0 + gi) * D + threadIdx.x] = __float2bfloat16_rn(v / w);
+    for (int k = 1; k < 8; ++k) most = fmaxf(most, sh_m[k]);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float f = sh_m[k] == most ? 1.f : ka_exp2(sh_m[k] - most);
+      v = fmaf(f, sh_o[k][threadIdx.x], v);
+      w = fmaf(f, sh_l[k], w);
+    }
+    dst[threadIdx.x] = __float2bfloat16_rn(v / w);
   }
 }
 
@@ -632,7 +694,7 @@ template <int D, int NT>
 static int ka_launch(KaArgs a, int total_tiles, int sms, cudaStream_t stream) {
   constexpr int threads = 32 * ka_warps(D, NT);
   constexpr size_t smem = (size_t)ka_warps(D, NT) * KA_STAGES * 2 * kv4_record(D) +
-                          KA_MAX_TILES * (sizeof(KaTile) + 4) + 2 * (KA_MAX_TILES + 4) * 4;
+                          KA_MAX_TILES * (sizeof(KaTile) + 4) + (KA_MAX_TILES + 4) * 4;
   static bool configured[BF_MAX_DEVICES];
   const int dev = bf_current_device();
   if (!configured[dev]) {
@@ -649,11 +711,17 @@ static int ka_launch(KaArgs a, int total_tiles, int sms, cudaStream_t stream) {
   for (int first = 0; first < total_tiles; first += most) {
     a.first_tile = first;
     a.n_tiles = total_tiles - first < most ? total_tiles - first : most;
+    // heads with many pieces each (there are few of them): eight warps add a column's up
+    const bool few = (long long)a.n_tiles * pairs * 8 < (long long)sms * ka_warps(D, NT);
+    a.max_pieces = few ? sms * ka_warps(D, NT) : 64;
     int e = bf_launch_pdl(kv4_attention_kernel<D, NT>, dim3(sms), dim3(threads), smem, stream, a);
     if (e) return e;
-    e = bf_launch_pdl(kv4_merge_kernel<D>, dim3(a.n_tiles * pairs, 8 * NT), dim3(256), 0, stream,
-                      (const float*)a.part_o, (const float2*)a.part_ml, (const int4*)a.desc, a.out, a.out_stride,
-                      a.group, a.chunk, a.chunks, pairs, 8 * NT);
+    auto merge = [&](auto kern, int columns) {
+      return bf_launch_pdl(kern, dim3(a.n_tiles * pairs, 8 * NT / columns), dim3(256), 0, stream,
+                           (const float*)a.part_o, (const float2*)a.part_ml, (const int4*)a.desc, a.out,
+                           a.out_stride, a.group, a.chunk, a.chunks, a.chunk_inverse, pairs, 8 * NT);
+    };
+    e = few ? merge(kv4_merge_kernel<D, 8>, 1) : merge(kv4_merge_kernel<D, 1>, 8);
     if (e) return e;
   }
   return 0;
@@ -675,7 +743,7 @@ static KaShape ka_shape(int group, int d, int max_rows) {
   return s;
 }
 
-static long long ka_slots(const KaShape& s, int d, int sms) { return (long long)sms * ka_warps(d, s.nt) + KA_SPARE_SLOTS; }
+static long long ka_slots(const KaShape& s, int d, int sms) { return 2LL * sms * ka_warps(d, s.nt); }
 
 // Bytes of scratch that a call needs (16-byte aligned): partial results and a note per (tile, head).
 BF_EXPORT long long bf_kv4_attention_scratch(int n, int max_rows, int nh, int nkv, int d, int sms) {
@@ -704,10 +772,11 @@ BF_EXPORT int bf_kv4_attention(const void* q, long long q_stride, const void* ca
   a.out = (__nv_bfloat16*)out, a.out_stride = out_stride;
   a.nh = nh, a.nkv = nkv, a.group = nh / nkv, a.chunk = s.chunk, a.chunks = s.chunks, a.tokens = s.tokens;
   a.page_size = page_size, a.num_pages = num_pages, a.window = window, a.keep = keep, a.scale = scale;
-  a.slots = (int)ka_slots(s, d, sms);
+  a.chunk_inverse = (256 + s.chunk - 1) / s.chunk;
+  const long long slots = ka_slots(s, d, sms);
   a.part_o = (float*)scratch;
-  a.part_ml = (float2*)(a.part_o + (long long)a.slots * 8 * s.nt * d);
-  a.desc = (int4*)(a.part_ml + (long long)a.slots * 8 * s.nt);
+  a.part_ml = (float2*)(a.part_o + slots * 8 * s.nt * d);
+  a.desc = (int4*)(a.part_ml + slots * 8 * s.nt);
   a.err = err;
   const long long tiles = (long long)n * a.tiles_per_item;
   if (tiles > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
