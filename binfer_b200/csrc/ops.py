@@ -1902,18 +1902,24 @@ def kv4_store(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: torc
 
 def kv4_load(cache: torch.Tensor, block_tables: torch.Tensor, items: torch.Tensor, n_items: int,
              rows: int, err: torch.Tensor, window: Optional[int] = None, keep_first: int = 0,
-             items_out: Optional[torch.Tensor] = None):
+             items_out: Optional[torch.Tensor] = None, places: int = 0):
     """The whole contexts of prompt portions out of a cache in 4 bits, as bfloat16 pages of 64 tokens:
     ``(k [1 + rows / 64, kv heads, 64, d], v, tables int32 [n_items, rows / 64])``.  ``items`` int32
     ``[n_items, 4]`` of (request, first token row, rows, first position); ``rows``: the contexts' sum, each
     rounded up to 64.  Page 0 is zero, so are places behind a context and, with ``window`` and
     ``keep_first``, keys that no row of the portion sees (pages of nothing else are not written, their
     place in ``tables`` is page 0).  ``items_out``: takes the items with the portion's number in the
-    request's place, which goes with ``tables``."""
+    request's place, which goes with ``tables``; ``places``: the width of ``tables``, where a portion's
+    longest context is known to be shorter than all together."""
+    return _kv4_load(cache, block_tables, items, n_items, rows, err, window, keep_first, items_out, places)
+
+
+def _kv4_load(cache, block_tables, items, n_items, rows, err, window, keep_first, items_out, places,
+              not_finite=None):
     _want_int_table(block_tables, "kv4_load", "block_tables")
     _want(items, torch.int32, "items"); _want(err, torch.int32, "err")
     pages, nkv, ps, d = _kv4_check("kv4_load", cache, block_tables, items, err, items_out)
-    if n_items < 1 or items.numel() < 4 * n_items or rows < 64 or rows % 64:
+    if n_items < 1 or items.numel() < 4 * n_items or rows < 64 or rows % 64 or places < 0:
         raise KernelError("kv4_load: items must be [n_items, 4], rows a multiple of 64 tokens")
     if items_out is not None:
         _want(items_out, torch.int32, "items_out")
@@ -1921,13 +1927,15 @@ def kv4_load(cache: torch.Tensor, block_tables: torch.Tensor, items: torch.Tenso
             raise KernelError("kv4_load: items_out must have room for the items")
     window, keep_first = _kv4_mask("kv4_load", window, keep_first)
     n = 1 + rows // 64
+    places = places or n - 1
     k = torch.empty((n, nkv, KV4_LOAD_PAGE, d), dtype=torch.bfloat16, device=cache.device)
     v = torch.empty_like(k)
-    tables = torch.empty((n_items, n - 1), dtype=torch.int32, device=cache.device)
+    tables = torch.empty((n_items, places), dtype=torch.int32, device=cache.device)
     _run("kv4_load", lib().bf_kv4_load, _ptr(cache), _ptr(block_tables), _c_int(block_tables.stride(0)),
          _c_int(block_tables.shape[0]), _c_int(block_tables.shape[1]), _ptr(items), _c_int(n_items), _ptr(k),
-         _ptr(v), _ptr(tables), _ptr(items_out), _c_int(n), _c_int(nkv), _c_int(d), _c_int(ps),
-         _c_int(pages), _c_int(window), _c_int(keep_first), _ptr(err), _stream())
+         _ptr(v), _ptr(tables), _c_int(places), _ptr(items_out), _ptr(not_finite), _c_int(n), _c_int(nkv),
+         _c_int(d), _c_int(ps), _c_int(pages), _c_int(window), _c_int(keep_first),
+         _c_int(num_sms(cache.device)), _ptr(err), _stream())
     return k, v, tables
 
 
@@ -1981,20 +1989,48 @@ def kv4_decode_attention(q: torch.Tensor, cache: torch.Tensor, rows: Optional[to
 def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Tensor, n_items: int,
                           max_rows: int, block_tables: torch.Tensor, out: torch.Tensor, nh: int, nkv: int,
                           d: int, window: Optional[int], scale: float, err: torch.Tensor, ctx_rows: int,
-                          max_ctx: int, keep_first: int = 0) -> None:
+                          max_ctx: int, keep_first: int = 0, variant: str = "auto") -> None:
     """Causal attention of prompt portions over a cache in 4 bits, their own keys included:
     ``prefill_attention``'s arguments, with ``cache`` (``kv4_cache``) in the pages' place.  ``ctx_rows``:
     the portions' contexts added up, each rounded up to 64; ``max_ctx``: the longest of them;
-    ``keep_first``: with a window, the request's first that many tokens stay visible behind it."""
+    ``keep_first``: with a window, the request's first that many tokens stay visible behind it.
+
+    ``variant``: ``stretches`` (the kernel of single tokens, a few rows at a time; reads the cache as it
+    is), ``load`` (``kv4_load`` into scratch of 4 d bytes a token and kv head, then
+    ``prefill_attention``; q contiguous, and with ``keep_first`` or an ``out`` in a column block heads of
+    128), or ``auto``."""
     _want(items, torch.int32, "items")
     pages, ps, w, keep = _kv4_attention_check("kv4_prefill_attention", q, cache, block_tables, out, nh, nkv,
                                               d, window, keep_first, err, items)
     if n_items < 0 or items.numel() < 4 * n_items or max_rows < 0 or ctx_rows < 0 or ctx_rows % 64:
         raise KernelError("kv4_prefill_attention: items must be [n_items, 4], ctx_rows a multiple of 64")
+    if variant not in ("auto", "stretches", "load"):
+        raise KernelError(f"kv4_prefill_attention: unknown variant {variant!r}")
     if n_items == 0 or max_rows == 0:
+        return
+    load_ok = q.is_contiguous() and (d == 128 or (keep == 0 and out.is_contiguous())) and ctx_rows > 0
+    if variant == "load" and not load_ok:
+        raise KernelError("kv4_prefill_attention: the load variant takes a contiguous q, and keep_first or an "
+                          "out in a column block with heads of 128 only")
+    if variant == "load" or (variant == "auto" and load_ok and _kv4_load_pays(max_rows, nh // nkv)):
+        moved = torch.empty((n_items, 4), dtype=torch.int32, device=q.device)
+        # groups of values that are not finite: a bit a token, see kv4_poison_kernel
+        not_finite = torch.empty((1 + ctx_rows // 64) * nkv * d // 8, dtype=torch.uint8, device=q.device)
+        places = max(1, -(-max_ctx // KV4_LOAD_PAGE))
+        k, v, tables = _kv4_load(cache, block_tables, items, n_items, ctx_rows, err, window, keep_first, moved,
+                                 places, not_finite)
+        prefill_attention(q, k, v, moved, n_items, max_rows, tables, out, nh, nkv, d, window, scale, err,
+                          max_ctx=max_ctx, keep_first=keep)
+        _run("kv4_poison", lib().bf_kv4_poison, _ptr(not_finite), _ptr(moved), _c_int(n_items), _ptr(tables),
+             _c_int(places), _ptr(out), _c_ll(out.stride(0)), _c_int(q.shape[0]), _c_int(nh), _c_int(nkv), _c_int(d),
+             _c_int(w), _c_int(keep), _stream())
         return
     _kv4_attention(q, cache, None, None, None, items, n_items, max_rows, block_tables, out, nh, nkv, d, ps,
                    pages, w, keep, scale, err)
+
+
+def _kv4_load_pays(max_rows: int, group: int) -> bool:
+    return max_rows * group > 64
 
 
 def _kv4_attention(q, cache, rows, seq_of_token, positions, items, n, max_rows, block_tables, out, nh, nkv, d,
