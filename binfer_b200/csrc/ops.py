@@ -1846,34 +1846,55 @@ def kv4_cache(pages: int, kv_heads: int, page_size: int, d: int, device) -> torc
     return torch.zeros((pages, kv_heads, page_size // 8, 9 * d), dtype=torch.uint8, device=device)
 
 
+_kv4_sizes: dict = {}      # shapes that are caches in 4 bits -> (pages, kv heads, page size, head size)
+
+
 def _kv4_check(what: str, cache: torch.Tensor, *others) -> Tuple[int, int, int, int]:
     """(pages, kv heads, page size, head size) of a cache in 4 bits; every tensor on the device that the
     launch goes to."""
     if cache.dtype != torch.uint8 or cache.dim() != 4 or not cache.is_contiguous() or cache.data_ptr() % 16:
         raise KernelError(f"{what}: cache must be contiguous uint8 [pages, kv heads, page_size / 8, 9 d] "
                           "on a 16-byte boundary")
-    pages, nkv, eighths, rec = cache.shape
-    if rec % 9 or not kv4_takes(torch.bfloat16, rec // 9, 8 * eighths):
-        raise KernelError(f"{what}: pages of {8 * eighths} tokens and records of {rec} bytes are no cache "
-                          "in 4 bits")
+    sizes = _kv4_sizes.get(cache.shape)
+    if sizes is None:
+        pages, nkv, eighths, rec = cache.shape
+        if rec % 9 or not kv4_takes(torch.bfloat16, rec // 9, 8 * eighths):
+            raise KernelError(f"{what}: pages of {8 * eighths} tokens and records of {rec} bytes are no cache "
+                              "in 4 bits")
+        if len(_kv4_sizes) > 64:
+            _kv4_sizes.clear()
+        sizes = _kv4_sizes[cache.shape] = (pages, nkv, 8 * eighths, rec // 9)
     _same_device(what, cache, *others)
-    return pages, nkv, 8 * eighths, rec // 9
+    return sizes
 
 
 def _same_device(what: str, *tensors) -> None:
+    here = torch.cuda.current_device() if torch.cuda.is_initialized() else None
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise KernelError("the engine's kernels take CUDA tensors only (no CPU path)")
-        if t.device.index != torch.cuda.current_device():
+        if t is not None and t.get_device() != here:
+            if not t.is_cuda:
+                raise KernelError("the engine's kernels take CUDA tensors only (no CPU path)")
             raise KernelError(f"{what}: a tensor lies on {t.device}, the launch goes to device "
                               f"{torch.cuda.current_device()}")
 
 
 def _want_int_table(t: torch.Tensor, what: str, name: str) -> None:
-    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] < 1 or t.shape[1] < 1 or t.stride(1) != 1:
+    if t.dtype != torch.int32 or t.dim() != 2 or t.stride(1) != 1 or not t.numel():
         raise KernelError(f"{what}: {name} must be int32 with two dimensions and contiguous rows")
+
+
+_plain_fns: dict = {}
+
+
+def _plain_fn(name: str, signature: str):
+    """A launcher whose arguments are Python numbers and addresses: ``p`` an address or None, ``i`` an
+    int, ``l`` a long long, ``f`` a float.  (A ctypes object per argument costs more than the launch.)"""
+    fn = _plain_fns.get(name)
+    if fn is None:
+        fn = getattr(lib(), name)
+        fn.argtypes = [{"p": _c_void_p, "i": _c_int, "l": _c_ll, "f": _c_float}[c] for c in signature]
+        _plain_fns[name] = fn
+    return fn
 
 
 def kv4_store(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: torch.Tensor,
@@ -1895,9 +1916,9 @@ def kv4_store(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: torc
                           f"{tuple(k.shape)} and {slots.numel()} slots")
     if T == 0:
         return
-    _run("kv4_store", lib().bf_kv4_store, _ptr(k), _c_ll(k.stride(0)), _ptr(v), _c_ll(v.stride(0)),
-         _ptr(slots), _ptr(cache), _c_int(T), _c_int(nkv), _c_int(d), _c_int(ps), _c_ll(pages * ps),
-         _ptr(err), _stream())
+    _run("kv4_store", _plain_fn("bf_kv4_store", "plplppiiiilpp"), k.data_ptr(), k.stride(0), v.data_ptr(),
+         v.stride(0), slots.data_ptr(), cache.data_ptr(), T, nkv, d, ps, pages * ps, err.data_ptr(),
+         _stream().value)
 
 
 def kv4_load(cache: torch.Tensor, block_tables: torch.Tensor, items: torch.Tensor, n_items: int,
@@ -1931,11 +1952,12 @@ def _kv4_load(cache, block_tables, items, n_items, rows, err, window, keep_first
     k = torch.empty((n, nkv, KV4_LOAD_PAGE, d), dtype=torch.bfloat16, device=cache.device)
     v = torch.empty_like(k)
     tables = torch.empty((n_items, places), dtype=torch.int32, device=cache.device)
-    _run("kv4_load", lib().bf_kv4_load, _ptr(cache), _ptr(block_tables), _c_int(block_tables.stride(0)),
-         _c_int(block_tables.shape[0]), _c_int(block_tables.shape[1]), _ptr(items), _c_int(n_items), _ptr(k),
-         _ptr(v), _ptr(tables), _c_int(places), _ptr(items_out), _ptr(not_finite), _c_int(n), _c_int(nkv),
-         _c_int(d), _c_int(ps), _c_int(pages), _c_int(window), _c_int(keep_first),
-         _c_int(num_sms(cache.device)), _ptr(err), _stream())
+    _run("kv4_load", _plain_fn("bf_kv4_load", "ppiiipipppippiiiiiiiipp"), cache.data_ptr(),
+         block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[0], block_tables.shape[1],
+         items.data_ptr(), n_items, k.data_ptr(), v.data_ptr(), tables.data_ptr(), places,
+         None if items_out is None else items_out.data_ptr(),
+         None if not_finite is None else not_finite.data_ptr(), n, nkv, d, ps, pages, window, keep_first,
+         num_sms(cache.device), err.data_ptr(), _stream().value)
     return k, v, tables
 
 
@@ -2012,7 +2034,8 @@ def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Ten
     if variant == "load" and not load_ok:
         raise KernelError("kv4_prefill_attention: the load variant takes a contiguous q, and keep_first or an "
                           "out in a column block with heads of 128 only")
-    if variant == "load" or (variant == "auto" and load_ok and _kv4_load_pays(max_rows, nh // nkv)):
+    if variant == "load" or (variant == "auto" and load_ok and _kv4_load_pays(
+            n_items, max_rows, max_ctx, w, keep, nh, nkv, d)):
         moved = torch.empty((n_items, 4), dtype=torch.int32, device=q.device)
         # groups of values that are not finite: a bit a token, see kv4_poison_kernel
         not_finite = torch.empty((1 + ctx_rows // 64) * nkv * d // 8, dtype=torch.uint8, device=q.device)
@@ -2021,32 +2044,60 @@ def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Ten
                                  places, not_finite)
         prefill_attention(q, k, v, moved, n_items, max_rows, tables, out, nh, nkv, d, window, scale, err,
                           max_ctx=max_ctx, keep_first=keep)
-        _run("kv4_poison", lib().bf_kv4_poison, _ptr(not_finite), _ptr(moved), _c_int(n_items), _ptr(tables),
-             _c_int(places), _ptr(out), _c_ll(out.stride(0)), _c_int(q.shape[0]), _c_int(nh), _c_int(nkv), _c_int(d),
-             _c_int(w), _c_int(keep), _stream())
+        _run("kv4_poison", _plain_fn("bf_kv4_poison", "ppipipliiiiiip"), not_finite.data_ptr(), moved.data_ptr(),
+             n_items, tables.data_ptr(), places, out.data_ptr(), out.stride(0), q.shape[0], nh, nkv, d, w, keep,
+             _stream().value)
         return
     _kv4_attention(q, cache, None, None, None, items, n_items, max_rows, block_tables, out, nh, nkv, d, ps,
                    pages, w, keep, scale, err)
 
 
-def _kv4_load_pays(max_rows: int, group: int) -> bool:
-    return max_rows * group > 64
+_kv4_scratch: dict = {}     # bytes of scratch by a call's sizes
+
+
+def _kv4_load_pays(n: int, max_rows: int, max_ctx: int, window: int, keep: int, nh: int, nkv: int,
+                   d: int) -> bool:
+    """Whether a call's portions are faster loaded and attended by ``prefill_attention`` than in stretches
+    of units: microseconds by sizes, fitted to both measured on a B200.  One portion of 32 heads of 128
+    (8 kv heads), stretches against load: 64 rows behind 1,000 keys 23 / 40 us, behind 16,000 101 / 91; 128
+    rows 29 / 44 and 177 / 93; four portions of 64 rows behind 4,000 101 / 87.  16 heads of 64 (4): 128
+    rows behind 16,000 keys 72 / 332; 8 heads of 256 (2) 111 / 852."""
+    seen = min(max_ctx, window + keep + max_rows) if window else max_ctx
+    group, cols = nh // nkv, 8 if d == 256 else 16
+    chunks = -(-group // cols)
+    tiles = n * -(-max_rows // max(1, cols // group)) * chunks
+    # a tile's unit of sixteen keys
+    stretches = 11.0 + {64: 0.44e-3, 128: 0.64e-3, 256: 0.74e-3}[d] * tiles * nkv * (seen - max_rows / 2) / 16
+    if d == 128:          # (keys one tile after the other until they are shared out, then the products)
+        load = 12.0 + 0.025 * min(seen, 1000) + 0.13e-3 * nh * n * seen * -(-max_rows // 256)
+    elif d == 64:         # one tile after the other, 296 blocks of 128 rows at a time
+        load = 12.0 + 0.0205 * seen * max(1.0, nh * n * -(-max_rows // 128) / 296)
+    else:                 # the same of 64 rows
+        load = 12.0 + 0.0525 * seen * max(1.0, nh * n * -(-max_rows // 64) / 296)
+    return load < stretches
 
 
 def _kv4_attention(q, cache, rows, seq_of_token, positions, items, n, max_rows, block_tables, out, nh, nkv, d,
                    ps, pages, window, keep, scale, err):
     global _launches
     sms = num_sms(q.device)
-    size = lib().bf_kv4_attention_scratch
-    size.restype = _c_ll
+    key = (n, max_rows, nh, nkv, d, sms)
+    size = _kv4_scratch.get(key)
+    if size is None:
+        fn = lib().bf_kv4_attention_scratch
+        fn.restype = _c_ll
+        if len(_kv4_scratch) > 4096:
+            _kv4_scratch.clear()
+        size = _kv4_scratch[key] = fn(n, max_rows, nh, nkv, d, sms)
     # a call's own, from its stream's pool: two captured graphs share nothing
-    scratch = torch.empty(size(n, max_rows, nh, nkv, d, sms), dtype=torch.uint8, device=q.device)
-    _run("kv4_attention", lib().bf_kv4_attention, _ptr(q), _c_ll(q.stride(0)), _ptr(cache), _ptr(rows),
-         _ptr(seq_of_token), _ptr(positions), _ptr(items), _c_int(n), _c_int(max_rows), _c_int(q.shape[0]),
-         _ptr(block_tables), _c_int(block_tables.stride(0)), _c_int(block_tables.shape[0]),
-         _c_int(block_tables.shape[1]), _ptr(out), _c_ll(out.stride(0)), _c_int(nh), _c_int(nkv), _c_int(d),
-         _c_int(ps), _c_int(pages), _c_int(window), _c_int(keep), _c_float(scale), _ptr(scratch), _c_int(sms),
-         _ptr(err), _stream())
+    scratch = torch.empty(size, dtype=torch.uint8, device=q.device)
+    _run("kv4_attention", _plain_fn("bf_kv4_attention", "plpppppiiipiiipliiiiiiifpipp"), q.data_ptr(), q.stride(0),
+         cache.data_ptr(), None if rows is None else rows.data_ptr(),
+         None if seq_of_token is None else seq_of_token.data_ptr(),
+         None if positions is None else positions.data_ptr(), None if items is None else items.data_ptr(), n,
+         max_rows, q.shape[0], block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[0],
+         block_tables.shape[1], out.data_ptr(), out.stride(0), nh, nkv, d, ps, pages, window, keep, scale,
+         scratch.data_ptr(), sms, err.data_ptr(), _stream().value)
     _launches += 1          # two kernels: the stretches of units, and what several of them share
 
 
@@ -2071,15 +2122,13 @@ def step_tables(master: torch.Tensor, entries: torch.Tensor, new_pages: torch.Te
     as they were.  An entry that does not fit (a row, page, place or token outside of what it is given)
     sets the error word; its table is zero, its slots are -1."""
     _want_int_table(master, "step_tables", "master")
-    for name, t in (("master", master), ("entries", entries), ("new_pages", new_pages), ("q_start", q_start),
-                    ("positions", positions), ("seq_of_token", seq_of_token), ("ctx_lens", ctx_lens),
-                    ("slots", slots), ("tables", tables), ("err", err)):
-        _want(t, torch.int32, name)
-    for name, t in (("decode_rows", decode_rows), ("prefill_items", prefill_items)):
-        if t is not None:
-            _want(t, torch.int32, name)
-    _same_device("step_tables", master, entries, new_pages, q_start, positions, seq_of_token, ctx_lens, slots,
-                 tables, err, decode_rows, prefill_items)
+    given = (master, entries, new_pages, q_start, positions, seq_of_token, ctx_lens, slots, tables, err,
+             decode_rows, prefill_items)
+    for i, t in enumerate(given):
+        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
+            _want(t, torch.int32, ("master", "entries", "new_pages", "q_start", "positions", "seq_of_token",
+                                   "ctx_lens", "slots", "tables", "err", "decode_rows", "prefill_items")[i])
+    _same_device("step_tables", *given)
     B = entries.shape[0]
     if entries.dim() != 2 or entries.shape[1] != 5 or page_size < 1 or num_pages < 1:
         raise KernelError("step_tables: entries must be [B, 5], pages of at least one token")
@@ -2092,11 +2141,12 @@ def step_tables(master: torch.Tensor, entries: torch.Tensor, new_pages: torch.Te
         return
     n_dec = decode_rows.numel() if decode_rows is not None else 0
     n_pf = prefill_items.numel() // 4 if prefill_items is not None else 0
-    _run("step_tables", lib().bf_step_tables, _ptr(master), _c_int(master.shape[0]), _c_int(master.shape[1]),
-         _ptr(entries), _c_int(B), _ptr(new_pages), _c_int(new_pages.numel()), _c_int(page_size),
-         _c_int(num_pages), _ptr(q_start), _ptr(positions), _ptr(seq_of_token), _ptr(ctx_lens), _ptr(slots),
-         _c_int(T), _ptr(tables), _c_int(tables.shape[1]), _ptr(decode_rows), _c_int(n_dec),
-         _ptr(prefill_items), _c_int(n_pf), _ptr(err), _stream())
+    _run("step_tables", _plain_fn("bf_step_tables", "piipipiiipppppipipipipp"), master.data_ptr(), master.shape[0],
+         master.shape[1], entries.data_ptr(), B, new_pages.data_ptr(), new_pages.numel(), page_size, num_pages,
+         q_start.data_ptr(), positions.data_ptr(), seq_of_token.data_ptr(), ctx_lens.data_ptr(),
+         slots.data_ptr(), T, tables.data_ptr(), tables.shape[1],
+         None if decode_rows is None else decode_rows.data_ptr(), n_dec,
+         None if prefill_items is None else prefill_items.data_ptr(), n_pf, err.data_ptr(), _stream().value)
 
 
 class DiffCombine:

@@ -105,3 +105,70 @@ def test_step_tables_takes_int32(ops, name):
     args[name] = args[name].long()
     with pytest.raises(ops.KernelError, match="int32"):
         ops.step_tables(**args)
+
+
+@pytest.mark.parametrize("change", [dict(variant="fast"), dict(variant="load", keep_first=3, window=5)])
+def test_prefill_variants(ops, change, monkeypatch):
+    """(The checks before a launch, with the device's left out.)"""
+    monkeypatch.setattr(ops, "_same_device", lambda *a: None)
+    args = dict(_attention_args(ops), items=_i(1, 4), n_items=1, max_rows=3, ctx_rows=64, max_ctx=3)
+    with pytest.raises(ops.KernelError, match="variant"):
+        ops.kv4_prefill_attention(**dict(args, **change))
+
+
+@pytest.mark.parametrize("what,change", [
+    ("window", dict(window=0)), ("keep_first", dict(keep_first=-1)), ("heads", dict(nkv=1)), ("heads", dict(d=128)),
+    ("heads", dict(nh=3)), ("q", dict(q=torch.zeros((3, 256)))), ("q", dict(q=torch.zeros((3, 512), dtype=BF16)[:, 1:257])),
+    ("out", dict(out=torch.zeros((3, 255), dtype=BF16))), ("out", dict(out=torch.zeros((2, 256), dtype=BF16)))])
+def test_attention_sizes(ops, what, change, monkeypatch):
+    monkeypatch.setattr(ops, "_same_device", lambda *a: None)
+    args = dict(_attention_args(ops), **change)
+    with pytest.raises(ops.KernelError, match=what):
+        ops.kv4_decode_attention(**args, rows=None, n_rows=3, seq_of_token=_i(3), positions=_i(3))
+    with pytest.raises(ops.KernelError, match=what):
+        ops.kv4_prefill_attention(**args, items=_i(1, 4), n_items=1, max_rows=3, ctx_rows=64, max_ctx=3)
+
+
+@pytest.mark.parametrize("change", [dict(n_rows=4), dict(n_rows=-1), dict(rows=_i(2)), dict(seq_of_token=_i(2)),
+                                    dict(positions=_i(2))])
+def test_decode_rows(ops, change, monkeypatch):
+    monkeypatch.setattr(ops, "_same_device", lambda *a: None)
+    args = dict(_attention_args(ops), rows=None, n_rows=3, seq_of_token=_i(3), positions=_i(3))
+    with pytest.raises(ops.KernelError, match="rows inside q"):
+        ops.kv4_decode_attention(**dict(args, **change))
+
+
+@pytest.mark.parametrize("change", [dict(n_items=2), dict(n_items=-1), dict(ctx_rows=65), dict(max_rows=-1)])
+def test_prefill_items(ops, change, monkeypatch):
+    monkeypatch.setattr(ops, "_same_device", lambda *a: None)
+    args = dict(_attention_args(ops), items=_i(1, 4), n_items=1, max_rows=3, ctx_rows=64, max_ctx=3)
+    with pytest.raises(ops.KernelError, match="items"):
+        ops.kv4_prefill_attention(**dict(args, **change))
+
+
+@pytest.mark.parametrize("change", [dict(rows=63), dict(rows=0), dict(n_items=0), dict(n_items=2), dict(items_out=_i(3)),
+                                    dict(window=0), dict(places=-1)])
+def test_load_sizes(ops, change, monkeypatch):
+    monkeypatch.setattr(ops, "_same_device", lambda *a: None)
+    args = dict(cache=ops.kv4_cache(3, 1, 16, 64, "cpu"), block_tables=_i(1, 2), items=_i(1, 4), n_items=1, rows=64,
+                err=_i(1))
+    with pytest.raises(ops.KernelError):
+        ops.kv4_load(**dict(args, **change))
+
+
+@pytest.mark.parametrize("change", [dict(entries=_i(1, 4)), dict(page_size=0), dict(num_pages=0), dict(tables=_i(0, 4)),
+                                    dict(q_start=_i(1)), dict(ctx_lens=_i(0)), dict(num_pages=1 << 28)])
+def test_step_tables_sizes(ops, change, monkeypatch):
+    monkeypatch.setattr(ops, "_same_device", lambda *a: None)
+    args = dict(master=_i(2, 4), entries=_i(1, 5), new_pages=_i(1), page_size=16, num_pages=8, q_start=_i(2),
+                positions=_i(1), seq_of_token=_i(1), ctx_lens=_i(1), slots=_i(1), tables=_i(1, 4), err=_i(1))
+    with pytest.raises(ops.KernelError, match="step_tables"):
+        ops.step_tables(**dict(args, **change))
+
+
+def test_which_portions_are_loaded(ops):
+    """The rule's two sides at sizes where they are far apart."""
+    pays = ops._kv4_load_pays
+    assert pays(1, 2048, 2048, 0, 0, 32, 8, 128) and pays(1, 256, 8448, 0, 0, 32, 8, 128)
+    assert not pays(6, 5, 3005, 0, 0, 16, 8, 128) and not pays(1, 128, 16000, 0, 0, 16, 4, 64)
+    assert pays(1, 1024, 100000, 512, 0, 32, 8, 128) and not pays(1, 8, 100000, 0, 0, 32, 8, 128)

@@ -582,3 +582,35 @@ def test_a_run_of_steps(cuda_device, window, keep):
             at += counts[b]
             lens[b] = n
         assert int(err.item()) == 0
+
+
+@pytest.mark.parametrize("variant", ["stretches", "load"])
+@pytest.mark.parametrize("nh,nkv,d,ps", [(8, 2, 128, 16), (4, 4, 64, 8), (6, 2, 256, 64), (17, 1, 128, 32)])
+@pytest.mark.parametrize("window,keep", [(None, 0), (64, 0), (100, 11)])
+def test_both_ways_of_a_portion(cuda_device, variant, nh, nkv, d, ps, window, keep):
+    from binfer_b200.csrc import ops
+    if variant == "load" and keep and d != 128:
+        pytest.skip("kept tokens are the 128-sized heads' alone on this way")
+    c = Cache([300, 70, 1], nkv, d, ps, cuda_device, seed=nh)
+    jobs = [(1, 70, 0), (0, 33, 267), (2, 1, 0)]
+    q = _queries(104, nh, d, cuda_device)
+    out = torch.full_like(q, math.nan)
+    items = torch.tensor([(1, 0, 70, 0), (0, 70, 33, 267), (2, 103, 1, 0)], dtype=I32, device=cuda_device)
+    ops.kv4_prefill_attention(q, c.cache, items, 3, 70, c.tables, out, nh, nkv, d, window, d ** -0.5, c.err,
+                              ctx_rows=128 + 320 + 64, max_ctx=300, keep_first=keep, variant=variant)
+    _compare(c, q, out, nh, jobs, window, keep, d ** -0.5)
+
+
+def test_load_without_room_attends_what_fits(cuda_device):
+    """``ctx_rows`` smaller than the contexts: the portions that have no room are flagged and left out."""
+    from binfer_b200.csrc import ops
+    nh, nkv, d = 4, 2, 128
+    c = Cache([100, 200], nkv, d, 16, cuda_device)
+    q = _queries(150, nh, d, cuda_device)
+    out = torch.zeros_like(q)
+    items = torch.tensor([(0, 0, 50, 50), (1, 50, 100, 100)], dtype=I32, device=cuda_device)
+    ops.kv4_prefill_attention(q, c.cache, items, 2, 100, c.tables, out, nh, nkv, d, None, 0.1, c.err, ctx_rows=256,
+                              max_ctx=200, variant="load")
+    assert int(c.err.item()) == 16 and not out[50:].any()
+    c.err.zero_()
+    _compare(c, q[:50], out[:50], nh, [(0, 50, 50)], None, 0, 0.1)
