@@ -35,7 +35,8 @@ class KVNeed:
     left the window AND its block's mean is taken.  ``stride`` > 1 marks such a summary
     group's own need (made by the manager, not by mixers).  ``keep_first``: with a window,
     the request's first that many tokens stay visible for good, so the pages that hold them
-    are never given back while the request lives."""
+    are never given back while the request lives.  ``four_bits``: keys and values are held in 4
+    bits (``csrc.ops.kv4_cache``); both have ``head_dim`` numbers then, and no means are kept."""
 
     num_kv_heads: int
     head_dim: int
@@ -44,6 +45,7 @@ class KVNeed:
     pools: Tuple[int, ...] = ()
     stride: int = 1
     keep_first: int = 0
+    four_bits: bool = False
 
     @property
     def v_dim(self) -> int:
@@ -51,11 +53,19 @@ class KVNeed:
 
     @property
     def group_key(self) -> Tuple:
+        if self.four_bits:
+            return ("four bits", self.num_kv_heads, self.head_dim, self.window, self.kept_tokens)
         if (self.value_dim is None and not self.pools and self.stride == 1
                 and not self.kept_tokens):
             return (self.num_kv_heads, self.head_dim, self.window)
         return (self.num_kv_heads, self.head_dim, self.window, self.v_dim, self.pools,
                 self.stride, self.kept_tokens)
+
+    def page_bytes(self, page_size: int, element_size: int) -> int:
+        """Bytes of a page's keys and values."""
+        if self.four_bits:               # two codes a byte, and two bfloat16 numbers per 64
+            return self.num_kv_heads * page_size * self.head_dim * 9 // 8
+        return self.num_kv_heads * (self.head_dim + self.v_dim) * page_size * element_size
 
     @property
     def kept_tokens(self) -> int:
@@ -65,15 +75,16 @@ class KVNeed:
     def merged(self, other: "KVNeed") -> "KVNeed":
         """The need of a cache that serves this execution and another that reads it: the
         wider window, the pools of both."""
-        if (self.num_kv_heads, self.head_dim, self.v_dim) != (other.num_kv_heads,
-                                                              other.head_dim, other.v_dim):
+        if (self.num_kv_heads, self.head_dim, self.v_dim, self.four_bits) != (
+                other.num_kv_heads, other.head_dim, other.v_dim, other.four_bits):
             raise ValueError("an execution that reads another's cache must have its head "
                              "count and head sizes")
         window = (None if self.window is None or other.window is None
                   else max(self.window, other.window))
         pools = tuple(sorted(set(self.pools) | set(other.pools))) if window is not None else ()
         return KVNeed(self.num_kv_heads, self.head_dim, window, self.value_dim, pools,
-                      keep_first=max(self.kept_tokens, other.kept_tokens))
+                      keep_first=max(self.kept_tokens, other.kept_tokens),
+                      four_bits=self.four_bits)
 
 
 @dataclass(frozen=True)
@@ -136,8 +147,7 @@ def plan_pages(kv_needs: Sequence[Optional[KVNeed]], page_size: int, budget_byte
             max_seq_len, need.window + max(need.pools, default=0) + need.kept_tokens
             + max_tokens_per_step)
         per_request[key] = -(-tokens // page_size) + 2
-        page_bytes[key] = page_bytes.get(key, 0) + (
-            need.num_kv_heads * (need.head_dim + need.v_dim) * page_size * element_size)
+        page_bytes[key] = page_bytes.get(key, 0) + need.page_bytes(page_size, element_size)
         for P in need.pools:         # the summary group of this pool size
             sk = summary_need(need, P).group_key
             per_request[sk] = -(-(max_seq_len // P) // page_size) + 1
@@ -413,14 +423,23 @@ class CacheManager:
     def allocate_storage(self, dtype, device) -> None:
         """Device tensors: per group ``[entries, 2, pages + 1, kv_heads, page_size, head_dim]``
         (keys at index 0, values at 1; page 0 is scratch), or, where keys and values differ in
-        size, a pair of tensors ``[entries, pages + 1, kv_heads, page_size, d]``; and per
+        size, a pair of tensors ``[entries, pages + 1, kv_heads, page_size, d]``, or, held in 4
+        bits, ``uint8 [entries, pages + 1, kv_heads, page_size / 8, 9 head_dim]``; and per
         schedule entry with a :class:`StateNeed` a tensor ``[slots + 1, *shape]`` (the last
         slot is scratch: padded rows of a captured step use it)."""
         import torch
         for g in self.groups:
             n = g.need
             shape = (len(g.entries), g.pool.num_pages + 1, n.num_kv_heads, g.page_size)
-            if n.v_dim == n.head_dim:
+            if n.four_bits:
+                from ..csrc import ops
+                if not ops.kv4_takes(dtype, n.head_dim, g.page_size):
+                    raise ValueError(f"a cache in 4 bits takes a bfloat16 engine, heads of "
+                                     f"{ops.KV4_HEAD_DIMS} numbers and pages of 8 to 128 tokens that divide "
+                                     f"128, not {dtype}, {n.head_dim} and {g.page_size}")
+                g.storage = torch.zeros(shape[:3] + (g.page_size // 8, 9 * n.head_dim),
+                                        dtype=torch.uint8, device=device)
+            elif n.v_dim == n.head_dim:
                 g.storage = torch.zeros((shape[0], 2) + shape[1:] + (n.head_dim,),
                                         dtype=dtype, device=device)
             else:
@@ -442,12 +461,15 @@ class CacheManager:
 
     def kv_view(self, entry: int):
         """(keys, values) storage of schedule entry ``entry``: each
-        ``[pages + 1, kv_heads, page_size, head_dim]``; and its group index."""
+        ``[pages + 1, kv_heads, page_size, head_dim]`` (held in 4 bits: the pages of both, and
+        None); and its group index."""
         gi, ei = self.entry_location[entry]
         return self._kv_of(gi, ei) + (gi,)
 
     def _kv_of(self, gi: int, ei: int):
         st = self.groups[gi].storage
+        if self.groups[gi].need.four_bits:
+            return st[ei], None
         if isinstance(st, tuple):
             return st[0][ei], st[1][ei]
         return st[ei, 0], st[ei, 1]

@@ -34,15 +34,18 @@ class Engine:
                  page_size: int = 16, max_seq_len: int = 4096, max_batch_size: int = 64,
                  max_tokens_per_step: int = 2048, cuda_graphs: bool = True,
                  look_ahead: bool = True, device: str = "cuda:0",
-                 allow_unexpected_tensors: bool = False):
+                 allow_unexpected_tensors: bool = False, kv_cache: str = "auto"):
         """``model``: a folder with config.json and safetensors, or (with
         ``random_seed``) a typed configuration whose weights are drawn on the device.
 
         The cache's size: ``num_pages`` pages per cache group, else ``max_kv_memory_gb``,
         else ``gpu_memory_utilization`` of the device memory that is free once the weights
         are loaded (less 2 GB for activations, logits and graphs), and never more than
-        ``max_batch_size`` requests of ``max_seq_len`` tokens can use."""
-        self.env = make_env(dtype, device)
+        ``max_batch_size`` requests of ``max_seq_len`` tokens can use.
+
+        ``kv_cache``: ``auto`` or ``int4`` (keys and values in 4 bits: 4.5 with their scales, so
+        that 3.5 times as many tokens fit; see ``make_env``)."""
+        self.env = make_env(dtype, device, kv_cache)
         if isinstance(model, str):
             self.config = load_config(model)
             self.model = model_from_dir(model, self.env,

@@ -36,14 +36,21 @@ def parse_dtype(name: Union[str, torch.dtype]) -> torch.dtype:
     return _DTYPES[name]
 
 
-def make_env(dtype: Union[str, torch.dtype], device: Union[str, torch.device] = "cuda:0") -> BuildEnv:
+def make_env(dtype: Union[str, torch.dtype], device: Union[str, torch.device] = "cuda:0",
+             kv_cache: str = "auto") -> BuildEnv:
+    """``kv_cache``: ``auto`` (keys and values as the activations) or ``int4`` (in 4 bits, 4.5 with
+    their scales: bfloat16 engines whose paged layers are plain grouped attention)."""
     device = torch.device(device)
+    if kv_cache not in ("auto", "int4"):
+        raise ValueError(f"unknown kv_cache {kv_cache!r} (auto or int4)")
+    if kv_cache == "int4" and parse_dtype(dtype) != torch.bfloat16:
+        raise ValueError("a cache in 4 bits takes a bfloat16 engine")
     if device.type != "cuda":
         raise RuntimeError("the engine runs on a CUDA device only (there is no CPU path)")
     if not torch.cuda.is_available():
         raise RuntimeError("no CUDA device is available; the engine has no CPU path")
     torch.cuda.set_device(device)
-    return BuildEnv(parse_dtype(dtype), device)
+    return BuildEnv(parse_dtype(dtype), device, kv_cache)
 
 
 def model_from_dir(model_dir: str, env: BuildEnv, allow_unexpected: bool = False) -> DecoderModel:

@@ -11,7 +11,9 @@ product against the concatenated weight; norm, rotation and cache write are one
 kernel; and every key, also those of the step's own tokens, is read from the
 pages, so a prompt can be cut into portions anywhere and portions can share a
 step with decoded tokens (the reference's prefill ignores the cache, :1082-1086).
-An optional window restricts a query at p to keys in (p - window, p].  Changes to
+An optional window restricts a query at p to keys in (p - window, p].  Where the engine holds
+its cache in 4 bits (``BuildEnv.kv_cache``), keys and values pass a second kernel into the pages
+and the attention kernels read the codes.  Changes to
 the scores before the softmax (``AttentionSpec.score``: a soft cap, a bias per
 distance, a sink logit per head) are not Qwen3's; a spec that names one gets the
 generic attention kernel, which applies them, in both precisions.
@@ -41,6 +43,18 @@ FUSE_QKV = os.environ.get("BINFER_B200_FUSE_QKV", "0") != "0"
 FUSE_QKV_FILL = 0.6
 
 
+_each_of: dict = {}
+
+
+def _each(n: int, device) -> torch.Tensor:
+    """int32 0 .. n - 1, kept for good: captured steps read it."""
+    size = max(64, 1 << (n - 1).bit_length())
+    got = _each_of.get((device, size))
+    if got is None:
+        got = _each_of[(device, size)] = torch.arange(size, dtype=torch.int32, device=device)
+    return got[:n]
+
+
 class GQAAttention(Mixer):
     def __init__(self, spec: AttentionSpec, hidden_size: int, prefix: str, env: BuildEnv):
         if spec.num_heads % spec.num_kv_heads:
@@ -61,6 +75,11 @@ class GQAAttention(Mixer):
                 raise ValueError("score.slopes needs one slope per query head")
             self.slopes = torch.tensor(spec.score.slopes, dtype=torch.float32, device=env.device)
         self._qkv_plans = {}
+        # keys and values in 4 bits
+        self.four_bits = env.kv_cache == "int4"
+        if self.four_bits and (spec.score is not None or not ops.kv4_takes(env.dtype, spec.head_dim, 16)):
+            raise ValueError(f"a cache in 4 bits takes bfloat16, heads of {ops.KV4_HEAD_DIMS} numbers and "
+                             f"plain scores")
 
     # ----------------------------------------------------------------- weights
     def param_specs(self) -> List[ParamSpec]:
@@ -95,7 +114,7 @@ class GQAAttention(Mixer):
     # ------------------------------------------------------------------- cache
     def kv_need(self) -> Optional[KVNeed]:
         s = self.spec
-        return KVNeed(s.num_kv_heads, s.head_dim, s.window)
+        return KVNeed(s.num_kv_heads, s.head_dim, s.window, four_bits=self.four_bits)
 
     # ----------------------------------------------------------------- forward
     accepts_scaled_rows = True
@@ -116,7 +135,9 @@ class GQAAttention(Mixer):
         w = self.w_qkv if view.writes_cache else self.w_qkv[: self.q_size]
         if not self._project_fused(x, w, q, row_scale, ctx, view):
             qkv = linear(x, w)
-            if pos is None or pos.inv_freq is not None:
+            if self.four_bits and view.writes_cache:
+                self._encode_four_bits(qkv, q, row_scale, ctx, view)
+            elif pos is None or pos.inv_freq is not None:
                 # head norms, rotation and the store into the pages: one kernel
                 writes = view.writes_cache
                 ops.qk_norm_rope_kv_write(
@@ -136,7 +157,7 @@ class GQAAttention(Mixer):
         store into the pages as one kernel, where the split-K cluster product has a plan with
         tiles of whole heads for this shape.  False, having done nothing, otherwise."""
         s, pos = self.spec, self.position
-        if (not FUSE_QKV or x.dtype != torch.bfloat16 or x.shape[0] > cluster_token_limit()
+        if (not FUSE_QKV or self.four_bits or x.dtype != torch.bfloat16 or x.shape[0] > cluster_token_limit()
                 or (pos is not None and pos.inv_freq is None)):
             return False
         key = (w.shape[0], w.shape[1])
@@ -176,6 +197,38 @@ class GQAAttention(Mixer):
                                       s.num_heads, s.num_kv_heads, s.head_dim, s.qk_norm_eps,
                                       ctx.err)
 
+    def _encode_four_bits(self, qkv, q, row_scale, ctx: StepContext, view: EntryView) -> None:
+        """Head norms and position encoding with the keys and values into rows of bfloat16 (a
+        cache of one-token pages), and those into the pages in 4 bits."""
+        s, T, pos = self.spec, qkv.shape[0], self.position
+        kv = torch.empty((2, T, s.num_kv_heads, 1, s.head_dim), dtype=q.dtype, device=q.device)
+        each = _each(T, q.device)
+        ops.qk_norm_rope_kv_write(
+            qkv, self.q_norm, self.k_norm, pos.inv_freq if pos is not None else None, ctx.positions, each, q,
+            kv[0], kv[1], s.num_heads, s.num_kv_heads, s.head_dim, s.qk_norm_eps, ctx.err, row_scale=row_scale)
+        if pos is not None and pos.inv_freq is None:
+            pos.apply(q.view(T, s.num_heads, s.head_dim), kv[0].view(T, s.num_kv_heads, s.head_dim),
+                      ctx.positions)
+        ops.kv4_store(kv[0].view(T, self.kv_size), kv[1].view(T, self.kv_size), ctx.slots[view.group],
+                      view.k_cache, ctx.err)
+
+    def _attend_four_bits(self, q, out, ctx: StepContext, view: EntryView) -> None:
+        s = self.spec
+        tail = (ctx.block_tables[view.group], out, s.num_heads, s.num_kv_heads, s.head_dim, s.window,
+                s.softmax_scale, ctx.err)
+        if ctx.decode_only or ctx.n_decode:
+            ops.kv4_decode_attention(q, view.k_cache, None if ctx.decode_only else ctx.decode_rows,
+                                     ctx.T if ctx.decode_only else ctx.n_decode, ctx.seq_of_token,
+                                     ctx.positions, *tail)
+        if ctx.n_prefill:
+            rows = ctx.scratch.get("portion_ctx_rows")
+            if rows is None:
+                rows = ctx.scratch["portion_ctx_rows"] = sum(
+                    -(-c // ops.KV4_LOAD_PAGE) * ops.KV4_LOAD_PAGE
+                    for n, c in zip(ctx.q_lens, ctx.ctx_lens_host) if n > 1)
+            ops.kv4_prefill_attention(q, view.k_cache, ctx.prefill_items, ctx.n_prefill, ctx.max_prefill_rows,
+                                      *tail, ctx_rows=rows, max_ctx=ctx.max_ctx_len)
+
     def attend(self, q: torch.Tensor, out: torch.Tensor, ctx: StepContext,
                view: EntryView) -> None:
         """Attention of every token row over its request's pages.
@@ -186,6 +239,9 @@ class GQAAttention(Mixer):
         the rest (and head sizes the tuned kernels do not take) to the generic one.
         """
         s = self.spec
+        if self.four_bits:
+            self._attend_four_bits(q, out, ctx, view)
+            return
         tables = ctx.block_tables[view.group]
         fast = (q.dtype == torch.bfloat16 and s.head_dim in ops.DECODE_HEAD_DIMS
                 and s.score is None)

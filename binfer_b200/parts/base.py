@@ -26,6 +26,7 @@ class BuildEnv:
 
     dtype: torch.dtype            # activations, matrices and cache pages
     device: torch.device
+    kv_cache: str = "auto"        # "int4": keys and values held in 4 bits (KVNeed.four_bits)
 
 
 @dataclass
@@ -155,7 +156,9 @@ class EntryView:
 
     entry: int
     group: Optional[int]               # cache group index, None if the mixer keeps no pages
-    k_cache: Optional[torch.Tensor]    # [pages + 1, kv_heads, page_size, head_dim]
+    # [pages + 1, kv_heads, page_size, head_dim] each; held in 4 bits, k_cache is the pages of both
+    # (``ops.kv4_cache``) and v_cache None
+    k_cache: Optional[torch.Tensor]
     v_cache: Optional[torch.Tensor]
     writes_cache: bool                 # False when the pages belong to another entry
     state: Optional[torch.Tensor]      # [slots + 1, *shape] of the mixer's StateNeed

@@ -149,6 +149,10 @@ class DecoderModel:
         out: List[Optional[KVNeed]] = []
         for entry in self.spec.schedule:
             need = self.blocks[entry.layer].mixer.kv_need()
+            if need is not None and self.env.kv_cache == "int4" and not need.four_bits:
+                raise ValueError(f"layer {entry.layer}: "
+                                 f"{type(self.blocks[entry.layer].mixer).__name__} does not keep its "
+                                 f"keys and values in 4 bits")
             out.append(need if entry.cache_from is None else None)
         # an execution that reads another's pages may look further back, or at pooled blocks
         # of another size: the pages are kept for the widest of them
