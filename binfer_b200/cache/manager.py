@@ -106,6 +106,7 @@ class RequestCache:
     # with `tables` (entries appended; rebuilt after a windowed page was released)
     np_tables: List[object] = field(default_factory=list)
     np_valid: List[int] = field(default_factory=list)
+    device_pages: int = 0      # leading pages of ``tables[0]`` that the runner's device table holds
 
     def table_array(self, g: int):
         """``tables[g]`` as a numpy int32 array (a view of a cached buffer)."""
@@ -482,6 +483,11 @@ class CacheManager:
             if e == entry:
                 out[P] = self._kv_of(gi, ei) + (gi,)
         return out
+
+    @property
+    def keeps_all(self) -> bool:
+        """One group whose requests keep every page until they end: its tables only grow."""
+        return self._plain
 
     @property
     def scratch_slot(self) -> int:

@@ -13,6 +13,7 @@ arrays per call (:2237-2269).
 """
 from __future__ import annotations
 
+import os
 from dataclasses import dataclass, field
 from typing import Hashable, List, Optional, Sequence, Tuple
 
@@ -23,6 +24,10 @@ from ..cache.manager import CacheManager
 from ..cache.pages import OutOfPages
 from ..parts.base import BuildEnv, StepContext
 from ..parts.model import DecoderModel
+
+
+# BINFER_B200_STEP_TABLES=0: captured steps' block tables and positions are made on the host too
+STEP_TABLES = os.environ.get("BINFER_B200_STEP_TABLES", "1") != "0"
 
 
 @dataclass
@@ -84,6 +89,9 @@ class ModelRunner:
         self._staging = _Staging()
         self.steps = 0
         self.h2d_bytes = 0
+        # every request's pages on the device (a row per request slot), from which captured
+        # steps make their tables: the host sends newly given pages only
+        self._master: Optional[torch.Tensor] = None
 
     # --------------------------------------------------------------- requests
     def add_request(self, rid: Hashable) -> None:
@@ -257,6 +265,100 @@ class ModelRunner:
             prefill_items=dview("prefill_items").view(len(pf), 4) if pf else None,
             n_prefill=len(pf), max_prefill_rows=max([q_lens[b] for b in pf], default=0))
 
+    def _build_single(self, items: Sequence[StepItem], bucket: int, st: dict,
+                      device_ids: Optional[torch.Tensor]) -> StepContext:
+        """:meth:`build_context` for a captured step of single tokens of a cache whose tables only
+        grow: the host sends ids, lengths and newly given pages, ``ops.step_tables`` makes the rest
+        on the device.  (Only ahead of a graph, whose launch waits for it: the step's kernels read
+        their description before they wait for the kernel ahead of them.)"""
+        from ..csrc import ops
+        cache, B, n = self.cache, bucket, len(items)
+        ps, width = cache.groups[0].page_size, st["width"]
+        if self._master is None or self._master.shape[1] < width:
+            # (no row is kept: all pages are sent anew)
+            for rc in cache.requests.values():
+                rc.device_pages = 0
+            self._master = torch.zeros((max(1, cache.slots.num_slots), width), dtype=torch.int32,
+                                       device=self.env.device)
+        rcs = [cache.get(it.rid) for it in items]
+        ids: List[int] = []
+        pairs: List[int] = []
+        entries: List[int] = []
+        new: List[int] = []
+        lens: List[int] = []
+        grown: List[Tuple[object, int]] = []
+        for b, (it, rc) in enumerate(zip(items, rcs)):
+            if it.src_row is None:
+                ids.append(it.tokens[0])
+            else:
+                ids.append(0)
+                pairs += (b, it.src_row)
+            start, have = rc.length, rc.device_pages
+            need = start // ps + 1
+            entries += (rc.slot, start, 1, have, len(new))
+            if need > have:
+                new += rc.tables[0][have:need]
+                grown.append((rc, need))
+            lens.append(start + 1)
+        if pairs and device_ids is None:
+            raise ValueError("an item takes its token from the device, but no ids were given")
+        f, sent = st["fields"], st["sent"]
+        total = sent + len(new)
+        host, ring = self._staging.take(total)
+        h = host.numpy()
+        h[:sent] = st["padding"]
+        h[:n] = ids
+        a = f["state_slots"]
+        h[a:a + n] = [rc.slot for rc in rcs]
+        a = f["entries"]
+        h[a:a + 5 * n] = entries
+        a = f["id_pairs"]
+        h[a:a + len(pairs)] = pairs
+        h[sent:total] = new
+        dev = st["dev"]
+        dev[:total].copy_(host[:total], non_blocking=True)
+        self._staging.sent(ring)
+        self.h2d_bytes += total * 4
+        c: StepContext = st["ctx"]
+        if pairs:
+            ops.copy_ids(c.token_ids, device_ids, st["pairs"], len(pairs) // 2)
+        ops.step_tables(self._master, st["entries"], st["new_pages"], ps, cache.groups[0].pool.num_pages + 1,
+                        c.q_start, c.positions, c.seq_of_token, c.ctx_lens, c.slots[0], c.block_tables[0],
+                        self.err)
+        for rc, need in grown:
+            rc.device_pages = need
+        c.ctx_lens_host = lens + [1] * (B - n)
+        return c
+
+    def _single_buffers(self, bucket: int, width: int) -> dict:
+        """The fixed device buffer of a captured step described by :meth:`_build_single`."""
+        B = bucket
+        f, at = {}, 0
+        for name, n in (("token_ids", B), ("state_slots", B), ("logit_rows", B), ("id_pairs", 2 * B),
+                        ("entries", 5 * B), ("new_pages", B * width), ("q_start", B + 1),
+                        ("positions", B), ("seq_of_token", B), ("ctx_lens", B), ("slots", B),
+                        ("tables", B * width)):
+            f[name] = at
+            at += n
+        dev = torch.zeros(at, dtype=torch.int32, device=self.env.device)
+        view = lambda name, n: dev[f[name]:f[name] + n]
+        # what a padding row brings: token 0 at position 0 in the scratch page, no state
+        pad = np.zeros(f["new_pages"], dtype=np.int32)
+        pad[f["state_slots"]:f["state_slots"] + B] = self.cache.scratch_slot
+        pad[f["logit_rows"]:f["logit_rows"] + B] = np.arange(B, dtype=np.int32)
+        pad[f["entries"]:f["entries"] + 5 * B] = np.tile(np.array([-1, 0, 1, 0, 0], np.int32), B)
+        ctx = StepContext(
+            env=self.env, cache=self.cache, T=B, B=B, token_ids=view("token_ids", B),
+            positions=view("positions", B), seq_of_token=view("seq_of_token", B),
+            q_start=view("q_start", B + 1), ctx_lens=view("ctx_lens", B),
+            state_slots=view("state_slots", B), slots=[view("slots", B)],
+            block_tables=[view("tables", B * width).view(B, width)], logit_rows=view("logit_rows", B),
+            err=self.err, q_lens=[1] * B, ctx_lens_host=[1] * B, max_q_len=1,
+            max_ctx_len=self._graph_seq_len, decode_only=True)
+        return {"dev": dev, "graph": None, "logits": None, "fields": f, "sent": f["new_pages"],
+                "padding": pad, "width": width, "ctx": ctx, "pairs": view("id_pairs", 2 * B),
+                "entries": view("entries", 5 * B).view(B, 5), "new_pages": view("new_pages", B * width)}
+
     # ---------------------------------------------------------------- the step
     def reserve(self, items: Sequence[StepItem]) -> None:
         """Pages for every item, or :class:`OutOfPages` with nothing changed."""
@@ -329,15 +431,22 @@ class ModelRunner:
             raise ValueError(f"no graph bucket {bucket} for {B} items")
         widths = [-(-self._graph_seq_len // g.page_size) for g in self.cache.groups]
         st = self._graphs.get(bucket)
+        on_device = STEP_TABLES and self.cache.keeps_all
+        if st is None and on_device:
+            st = self._graphs[bucket] = self._single_buffers(bucket, widths[0])
         if st is None:
             _, total = self._layout(bucket, bucket, bucket, widths)
             st = {"dev": torch.zeros(total, dtype=torch.int32, device=self.env.device),
                   "graph": None, "logits": None}
             self._graphs[bucket] = st
-        ctx = self.build_context(items, pad_to=bucket, widths=widths, dev=st["dev"],
-                                 device_ids=device_ids)
+        if on_device:
+            ctx = self._build_single(items, bucket, st, device_ids)
+        else:
+            ctx = self.build_context(items, pad_to=bucket, widths=widths, dev=st["dev"],
+                                     device_ids=device_ids)
         ctx.max_ctx_len = self._graph_seq_len     # launch shapes must not follow the batch
         if st["graph"] is None:
+            torch.cuda.current_stream().synchronize()         # (see _build_single)
             logits = self.model.forward(ctx, self.views)      # this step's result, eagerly
             torch.cuda.synchronize()
             from ..csrc import ops
