@@ -54,6 +54,10 @@
 // then the window's), and a head may have a sink, a logit that joins its sums in the epilogue or in
 // the merge.  Kept tokens are a fourth instance (KEEP), whose masks the plain one does without.
 //
+// Keys may be fp16 (HALF: those of a cache held in 4 bits, whose numbers bfloat16 would round): the softmax
+// warps then make their Q tile fp16 where it lies before its first product, and a request and kv head
+// with a query beyond fp16's range is noted in `beyond` for the caller to compute otherwise.
+//
 // Every mbarrier wait is bounded.  A barrier whose waiter could fall two phases behind exists
 // once per parity of the tile number, so that its one-bit phase cannot alias: "P V of tile n
 // done" (waited for only when O must be rescaled), and "P of tile n written" (a softmax
@@ -64,6 +68,8 @@
 #include <cuda.h>
 #include <float.h>
 #include <stdint.h>
+
+#include <cuda_fp16.h>
 
 #include "attention_diff.cuh"
 #include "common.cuh"
@@ -98,7 +104,7 @@ __device__ __forceinline__ bool group_all(int id, bool ok) {
   return r != 0;
 }
 
-template <int MODE>
+template <int MODE, bool HALF = false>
 __global__ void __launch_bounds__(A2_THREADS, 1)
 prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
                                const __grid_constant__ CUtensorMap map_k,
@@ -112,7 +118,7 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
                                float* __restrict__ part_o, float* __restrict__ part_ml,
                                int* __restrict__ err, float cap_pre, float cap_post,
                                long long out_stride, float out_scale, BfDiffArgs dd,
-                               const float* __restrict__ sinks, int keep) {
+                               const float* __restrict__ sinks, int keep, int* __restrict__ beyond) {
   constexpr bool DIFF = MODE == A2_DIFF, LATENT = MODE == A2_LATENT, KEEP = MODE == A2_KEEP;
   constexpr int D = A2_D;
   constexpr int HALVES = D / 64;                         // blocks of 64 columns of a V tile
@@ -140,7 +146,8 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
   uint64_t* s_full = kv_empty + STAGES;     // [group][2]: one per S buffer
   uint64_t* p_full = s_full + 4;               // [group][2], 8 arrivals (one a warp): P of the tiles of that parity
   uint64_t* o_done = p_full + 4;               // [group][2]: P V of the tiles of that parity
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 4);
+  uint64_t* q_half = o_done + 4;               // HALF: [group], the Q tile is fp16
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_half + (HALF ? 2 : 0));
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   // with splits > 1 the keys of a block are shared out over `splits` CTAs, each of which leaves
@@ -192,6 +199,8 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
       mbar_init(o_done + s, 1);
       mbar_init(p_full + s, 8);
     }
+    if (HALF)
+      for (int s = 0; s < 2; ++s) mbar_init(q_half + s, 8);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -339,7 +348,7 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
     const int my_tiles = grp == 0 ? tiles_a : (active_b ? tiles : 0);
     {
       // S: a = Q (K-major), b = K tile (K-major), N = 64 keys
-      const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) |
+      const uint32_t idesc_s = (1u << 4) | (HALF ? 0u : (1u << 7) | (1u << 10)) |
                                ((uint32_t)(A2_BN >> 3) << 17) | ((uint32_t)(A2_BM >> 4) << 24);
       // O: a = P (K-major), b = V as stored (MN-major), N = head size
       const uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) |
@@ -358,7 +367,8 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
         }
         umma_commit(s_full + grp * 2 + (n & 1));
       };
-      bool ok = my_tiles == 0 || (mbar_wait_warp(q_full, 0, abort) && mbar_wait_warp(kv_full, 0, abort));
+      bool ok = my_tiles == 0 || (mbar_wait_warp(HALF ? q_half + grp : q_full, 0, abort) &&
+                                  mbar_wait_warp(kv_full, 0, abort));
       if (ok && my_tiles > 0) {
         tc_fence_after();
         issue_s(0);
@@ -407,6 +417,30 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
       // of a tile, in the shape of a tensor-core fragment: a row's scores lie in the four
       // threads of a quad, 16 each, and a thread holds two rows (r and r + 8).  The row's
       // maximum and sum are two shuffles away: the group's warps never wait for each other.
+      if constexpr (HALF) {
+        // the group's Q tile, an eighth a warp: bfloat16 -> fp16, element by element where it lies
+        if (mbar_wait(q_full, 0, abort)) {
+          uint4* tile = reinterpret_cast<uint4*>(Qs + grp * Q_BYTES);
+          uint32_t most = 0;
+#pragma unroll 4
+          for (int i = (warp & 7) * 32 + lane; i < Q_BYTES / 16; i += 256) {
+            uint4 x = tile[i];
+            uint32_t* w = &x.x;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              most = __vmaxu2(most, w[k] & 0x7fff7fffu);
+              const __half2 f = __floats2half2_rn(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
+              w[k] = *reinterpret_cast<const uint32_t*>(&f);
+            }
+            tile[i] = x;
+          }
+          // (0x4780: 65,536; rows behind the portion's last count too, which only costs time)
+          if ((most & 0xffffu) >= 0x4780u || (most >> 16) >= 0x4780u) atomicOr(beyond + (it - items) / 4 * nkv + g, 1);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_half + grp);
+      }
       const int wq = warp & 3, hb = (warp >> 2) & 1;
       const int q4 = lane & 3;
       const uint32_t lane_addr = (uint32_t)(wq * 32 + hb * 16) << 16;
@@ -760,13 +794,14 @@ __global__ void prefill_attention_merge_kernel(const float* __restrict__ part_o,
 // scaled scores, s <- c tanh(s / c) (0: none); the result's rows `out_stride` elements apart
 // (a column block of a wider buffer: a multiple of 8, the block 16-byte aligned) and
 // multiplied by `out_scale`; a logit per head in the softmax's denominator (`sinks`, or null); with a
-// window and one split, the first `keep` tokens that stay visible behind it.
-BF_EXPORT int bf_prefill_attention_umma2_capped(
+// window and one split, the first `keep` tokens that stay visible behind it.  `beyond` (int [n_items, nkv],
+// zero, or null): the keys are fp16, and an entry becomes 1 where a query is beyond fp16's range.
+static int launch_umma2(
     const void* q, const void* k_cache, const void* v_cache, const int* items, int n_items,
     int max_rows, int total_rows, const int* block_tables, int table_stride, void* out, int nh,
     int nkv, int d, int page_size, int num_pages, int window, float scale, int splits,
     float* part_o, float* part_ml, int* err, float softcap, long long out_stride,
-    float out_scale, const float* sinks, int keep, cudaStream_t stream) {
+    float out_scale, const float* sinks, int keep, int* beyond, cudaStream_t stream) {
   if (n_items <= 0 || max_rows <= 0) return 0;
   if (splits < 1 || (splits > 1 && (!part_o || !part_ml))) return (int)cudaErrorInvalidValue;
   if (window <= 0 || keep < 0) keep = 0;
@@ -797,10 +832,12 @@ BF_EXPORT int bf_prefill_attention_umma2_capped(
   if (e) return e;
   // two Q tiles, the stages of K and V, the row sums, barriers
   const size_t smem = 1024 + (size_t)2 * 32768 + (size_t)2 * A2_STAGES * 16384 + 2048 + 256;
-  auto kern = keep > 0 ? prefill_attention_umma2_kernel<A2_KEEP>
-                       : prefill_attention_umma2_kernel<A2_PLAIN>;
-  static bool configured_on[BF_MAX_DEVICES][2];
-  bool& configured = configured_on[bf_current_device()][keep > 0];
+  auto kern = beyond ? (keep > 0 ? prefill_attention_umma2_kernel<A2_KEEP, true>
+                                 : prefill_attention_umma2_kernel<A2_PLAIN, true>)
+                     : (keep > 0 ? prefill_attention_umma2_kernel<A2_KEEP>
+                                 : prefill_attention_umma2_kernel<A2_PLAIN>);
+  static bool configured_on[BF_MAX_DEVICES][4];
+  bool& configured = configured_on[bf_current_device()][(keep > 0 ? 1 : 0) + (beyond ? 2 : 0)];
   if (!configured) {
     cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                           (int)smem);
@@ -813,7 +850,7 @@ BF_EXPORT int bf_prefill_attention_umma2_capped(
                                            (__nv_bfloat16*)out, nh, nkv, page_size, num_pages,
                                            window, scale * log2e, splits, part_o, part_ml, err,
                                            cap_pre, cap_post, out_stride, out_scale,
-                                           BfDiffArgs(), sinks, keep);
+                                           BfDiffArgs(), sinks, keep, beyond);
   if (splits > 1) {
     int st = bf_launch_status();
     if (st) return st;
@@ -821,6 +858,30 @@ BF_EXPORT int bf_prefill_attention_umma2_capped(
         part_o, part_ml, items, (__nv_bfloat16*)out, nh, splits, out_stride, out_scale, sinks);
   }
   return bf_launch_status();
+}
+
+BF_EXPORT int bf_prefill_attention_umma2_capped(
+    const void* q, const void* k_cache, const void* v_cache, const int* items, int n_items,
+    int max_rows, int total_rows, const int* block_tables, int table_stride, void* out, int nh,
+    int nkv, int d, int page_size, int num_pages, int window, float scale, int splits,
+    float* part_o, float* part_ml, int* err, float softcap, long long out_stride,
+    float out_scale, const float* sinks, int keep, cudaStream_t stream) {
+  return launch_umma2(q, k_cache, v_cache, items, n_items, max_rows, total_rows, block_tables, table_stride, out,
+                      nh, nkv, d, page_size, num_pages, window, scale, splits, part_o, part_ml, err, softcap,
+                      out_stride, out_scale, sinks, keep, nullptr, stream);
+}
+
+// bfloat16 queries and values over fp16 keys.
+BF_EXPORT int bf_prefill_attention_umma2_half(
+    const void* q, const void* k_cache, const void* v_cache, const int* items, int n_items,
+    int max_rows, int total_rows, const int* block_tables, int table_stride, void* out, int nh,
+    int nkv, int d, int page_size, int num_pages, int window, float scale, int splits,
+    float* part_o, float* part_ml, int* err, long long out_stride, int keep, int* beyond,
+    cudaStream_t stream) {
+  if (!beyond) return (int)cudaErrorInvalidValue;
+  return launch_umma2(q, k_cache, v_cache, items, n_items, max_rows, total_rows, block_tables, table_stride, out,
+                      nh, nkv, d, page_size, num_pages, window, scale, splits, part_o, part_ml, err, 0.f,
+                      out_stride, 1.f, nullptr, keep, beyond, stream);
 }
 
 BF_EXPORT int bf_prefill_attention_umma2(const void* q, const void* k_cache, const void* v_cache,
@@ -887,7 +948,7 @@ BF_EXPORT int bf_diff_attention_prefill_umma(
   kern<<<grid, A2_THREADS, smem, stream>>>(mq, mk, mv, mkr, mvr, items, block_tables, table_stride,
                                            (__nv_bfloat16*)out, nh, nkv, page_size, num_pages, 0,
                                            scale * 1.4426950408889634f, splits, part_o, part_ml,
-                                           err, 0.f, 0.f, out_stride, 1.f, dd, nullptr, 0);
+                                           err, 0.f, 0.f, out_stride, 1.f, dd, nullptr, 0, nullptr);
   if (splits > 1) {
     int st = bf_launch_status();
     if (st) return st;
@@ -940,6 +1001,6 @@ BF_EXPORT int bf_latent_attention_prefill_umma(
   kern<<<grid, A2_THREADS, smem, stream>>>(mq, mkv, mr, mr, mr, items, kv_base, 0,
                                            (__nv_bfloat16*)out, nh, nh, 1, 1, 0,
                                            scale * 1.4426950408889634f, 1, nullptr, nullptr, err,
-                                           0.f, 0.f, out_stride, 1.f, dd, sinks, 0);
+                                           0.f, 0.f, out_stride, 1.f, dd, sinks, 0, nullptr);
   return bf_launch_status();
 }

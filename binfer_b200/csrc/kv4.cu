@@ -3,6 +3,8 @@
 // Of 64 numbers x of a row: m = min x, s = bf16((max x - min x) / 15), c = (x - m) / s to the nearest
 // whole number (ties to even), at most 15; s = 0 gives c = 0.  A group with a number that is not finite
 // has s = m = NaN: all of it reads as NaN.
+#include <cuda_fp16.h>
+
 #include "common.cuh"
 #include "kv4.cuh"
 
@@ -133,18 +135,29 @@ BF_EXPORT int bf_kv4_store(const void* k, long long k_stride, const void* v, lon
 }
 
 // ------------------------------------------------------------------------------- out of the pages
+template <bool B>
+struct KvBool {
+  static constexpr bool value = B;
+};
+
 // A block takes 64 tokens of one portion's context and every gridDim.y-th kv head and writes them as bfloat16
 // pages [64][d] of keys and of values, a warp a record of eight tokens; the blocks of page 0 write zeros.
 // Where a portion's pages begin is a sum over the portions before it.  What no row of the portion sees is
 // zero (a page of nothing else is left out and its place in the table is page 0).  The blocks of a portion
 // write its row of the table together.
-template <int D>
+//
+// For attention on the tensor cores (HALF) the keys are fp16: a number m + s c has up to twelve bits, of which
+// bfloat16 keeps eight, and the scores' error was the largest part of the result's (0.0036 of its rms
+// against 0.0024).  A byte a record then says whether it holds a key beyond fp16's range, or a value that is
+// not finite (a probability of zero times such a value is NaN: whole tiles would carry it into rows that
+// do not see it); kv4_rest_kernel computes what is concerned.
+template <int D, bool HALF>
 __global__ void __launch_bounds__(256)
 kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__ block_tables,
                 int table_stride, int table_rows, int table_width, const int* __restrict__ items, int n_items,
                 __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out,
                 int* __restrict__ tables_out, int out_width, int* __restrict__ items_out,
-                unsigned char* __restrict__ not_finite, int out_pages, int nkv, int page_size, int num_pages, int window, int keep, int* __restrict__ err) {
+                unsigned char* __restrict__ special, int* __restrict__ beyond, int out_pages, int nkv, int page_size, int num_pages, int window, int keep, int* __restrict__ err) {
   constexpr int NG = D / KV4_GROUP, REC = kv4_record(D);
   bf_pdl_trigger();
   bf_pdl_wait();
@@ -212,6 +225,8 @@ kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
   }
   const int b = sh_of[0], first = sh_of[3], last = first + sh_of[2] - 1;
   const int place = page - 1 - sh_base, n_places = last / 64 + 1;
+  if (HALF && place == 0 && blockIdx.y == 0)
+    for (int h = tid; h < nkv; h += 256) beyond[item * nkv + h] = 0;
   if (blockIdx.y == 0) {                                    // this block's part of the portion's row
     const int w1 = place + 1 < n_places ? (int)((long long)out_width * (place + 1) / n_places) : out_width;
     for (int w = (int)((long long)out_width * place / n_places) + tid; w < w1; w += 256)
@@ -233,14 +248,19 @@ kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
       pid = 0;
     }
   }
-  auto eight = [](unsigned codes, float s, float m) {
+  auto eight = [](unsigned codes, float s, float m, auto half) {
     uint4 o;
     unsigned* w = reinterpret_cast<unsigned*>(&o);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float a = fmaf(s, (float)(codes >> (8 * i) & 15), m), c = fmaf(s, (float)(codes >> (8 * i + 4) & 15), m);
-      __nv_bfloat162 p = __floats2bfloat162_rn(a, c);
-      w[i] = *reinterpret_cast<unsigned*>(&p);
+      if constexpr (decltype(half)::value) {
+        const __half2 p = __floats2half2_rn(a, c);
+        w[i] = *reinterpret_cast<const unsigned*>(&p);
+      } else {
+        const __nv_bfloat162 p = __floats2bfloat162_rn(a, c);
+        w[i] = *reinterpret_cast<const unsigned*>(&p);
+      }
     }
     return o;
   };
@@ -265,38 +285,37 @@ kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
         vp[e][g] = *reinterpret_cast<const unsigned*>(rec + kv4_value_params_at(D) + ((2 * q + e) * NG + g) * 4);
       }
     }
+    bool other = false;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       const float s = kv4_scale(kp[g]), m = kv4_low(kp[g]);
       uint4* dst = reinterpret_cast<uint4*>(ko + r * D + g * 64 + q * 16);
-      dst[0] = on ? eight(kw[g].x, s, m) : zero;
-      dst[1] = on ? eight(kw[g].y, s, m) : zero;
-      unsigned nan = 0;
+      dst[0] = on ? eight(kw[g].x, s, m, KvBool<HALF>()) : zero;
+      dst[1] = on ? eight(kw[g].y, s, m, KvBool<HALF>()) : zero;
+      if (HALF) other |= on && (fabsf(m) > 65000.f || fabsf(fmaf(15.f, s, m)) > 65000.f);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float vs = kv4_scale(vp[e][g]);
-        bool write = v_on[e];
-        if (not_finite && write && vs != vs) {              // noted in its place, see kv4_poison_kernel
-          nan |= 1u << (2 * q + e);
-          write = false;
-        }
         *reinterpret_cast<uint4*>(vo + (2 * q + e) * D + g * 64 + r * 8) =
-            write ? eight(vw[e][g], vs, kv4_low(vp[e][g])) : zero;
+            v_on[e] ? eight(vw[e][g], vs, kv4_low(vp[e][g]), KvBool<false>()) : zero;
+        if (HALF) other |= v_on[e] && vs != vs;
       }
-      if (not_finite) {
-        nan = __reduce_or_sync(0xffffffffu, nan);
-        if (lane == 0) not_finite[((((size_t)page * nkv + h) * NG) + g) * 8 + warp] = (unsigned char)nan;
-      }
+    }
+    if (HALF) {
+      other = __any_sync(0xffffffffu, other);
+      if (lane == 0) special[((size_t)page * nkv + h) * 8 + warp] = other;
     }
   }
 }
 
+// special (8 bytes a page and head) and beyond (n_items x nkv), both or neither: keys in fp16, heads of 128.
 BF_EXPORT int bf_kv4_load(const void* cache, const int* block_tables, int table_stride, int table_rows,
                           int table_width, const int* items, int n_items, void* k_out, void* v_out,
-                          int* tables_out, int out_width, int* items_out, void* not_finite, int out_pages,
-                          int nkv, int d, int page_size, int num_pages, int window, int keep, int sms, int* err,
-                          cudaStream_t stream) {
+                          int* tables_out, int out_width, int* items_out, void* special, int* beyond,
+                          int out_pages, int nkv, int d, int page_size, int num_pages, int window, int keep,
+                          int sms, int* err, cudaStream_t stream) {
   if (n_items <= 0 || out_pages <= 1) return 0;
+  if ((special != nullptr) != (beyond != nullptr) || (special && d != 128)) return (int)cudaErrorInvalidValue;
   // heads apart where pages alone would leave SMs without blocks
   int parts = 1;
   while (parts < nkv && (long long)out_pages * parts < 4LL * sms) parts *= 2;
@@ -305,65 +324,85 @@ BF_EXPORT int bf_kv4_load(const void* cache, const int* block_tables, int table_
     return bf_launch_pdl(kern, dim3(out_pages, parts), dim3(256), 0, stream, (const unsigned char*)cache,
                          block_tables, table_stride, table_rows, table_width, items, n_items,
                          (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, tables_out, out_width, items_out,
-                         (unsigned char*)not_finite, out_pages, nkv, page_size, num_pages, window, keep, err);
+                         (unsigned char*)special, beyond, out_pages, nkv, page_size, num_pages, window, keep, err);
   };
-  if (d == 64) return run(kv4_load_kernel<64>);
-  if (d == 128) return run(kv4_load_kernel<128>);
-  if (d == 256) return run(kv4_load_kernel<256>);
+  if (special) return run(kv4_load_kernel<128, true>);
+  if (d == 64) return run(kv4_load_kernel<64, false>);
+  if (d == 128) return run(kv4_load_kernel<128, false>);
+  if (d == 256) return run(kv4_load_kernel<256, false>);
   return (int)cudaErrorInvalidValue;
 }
 
-// A probability of zero times a value that is not finite is NaN, so a product over whole tiles would
-// carry a token's values into rows that do not see it.  Where the caller attends over the loaded pages, such
-// groups of values are therefore zero in them and noted (a bit a token, [page][head][group][64]), and this
-// kernel writes NaN where a row sees one.  As a rule none is noted and a block only reads a few words.
-template <int NG>
+// What the tensor cores cannot have computed of portions over loaded pages: the rows of a portion and kv head
+// with a record that is noted in `special` or a query in `beyond`, by multiply-adds straight from the
+// cache, a warp a (row, query head).  As a rule nothing is noted and a block only reads a few words; a block
+// that finds something takes its 32 rows.
 __global__ void __launch_bounds__(256)
-kv4_poison_kernel(const unsigned long long* __restrict__ not_finite, const int* __restrict__ items,
-                  const int* __restrict__ tables, int width, __nv_bfloat16* __restrict__ out,
-                  long long out_stride, int T, int nkv, int group, int window, int keep) {
-  const int h = blockIdx.x, item = blockIdx.y;
+kv4_rest_kernel(const unsigned long long* __restrict__ special, const int* __restrict__ beyond,
+                const int* __restrict__ items, const int* __restrict__ moved, const int* __restrict__ tables,
+                int width, const unsigned char* __restrict__ cache, const int* __restrict__ block_tables,
+                int table_stride, const __nv_bfloat16* __restrict__ q, long long q_stride,
+                __nv_bfloat16* __restrict__ out, long long out_stride, int nkv, int group, int page_size,
+                int num_pages, int window, int keep, float scale) {
+  constexpr int D = 128, N = D / 32, NG = 2, REC = kv4_record(D);
   bf_pdl_trigger();
   bf_pdl_wait();
-  const int row0 = items[4 * item + 1], rows = items[4 * item + 2], first = items[4 * item + 3];
-  const int places = min((first + rows + 63) / 64, width);
+  const int h = blockIdx.y, item = blockIdx.z;
+  const int row0 = moved[4 * item + 1], rows = moved[4 * item + 2], first = moved[4 * item + 3];
   const int* table = tables + (size_t)item * width;
-  bool any = false;
-  for (int w = threadIdx.x; w < places; w += 256) {
-    const int page = table[w];
-    if (page <= 0) continue;
-    for (int g = 0; g < NG; ++g) any |= not_finite[((size_t)page * nkv + h) * NG + g] != 0;
-  }
+  if ((int)blockIdx.x * 32 >= rows) return;
+  bool any = threadIdx.x == 0 && beyond[item * nkv + h] != 0;
+  for (int w = threadIdx.x; w < min((first + rows + 63) / 64, width); w += 256)
+    if (table[w] > 0) any |= special[(size_t)table[w] * nkv + h] != 0;
   if (!__syncthreads_or(any)) return;
-  for (int i = threadIdx.x; i < rows * NG; i += 256) {
-    const int row = i / NG, g = i - row * NG, p = first + row;
-    bool sees = false;
-    for (int w = 0; w < places && w * 64 <= p && !sees; ++w) {
-      const int page = table[w];
-      unsigned long long bits = page > 0 ? not_finite[((size_t)page * nkv + h) * NG + g] : 0ULL;
-      for (; bits && !sees; bits &= bits - 1) {
-        const int j = w * 64 + __ffsll(bits) - 1;
-        sees = j <= p && (window <= 0 || j > p - window || j < keep);
+  const int lane = threadIdx.x & 31, i0 = lane * N, g = i0 / 64;
+  const int* request = block_tables + (size_t)items[4 * item] * table_stride;
+  for (int i = threadIdx.x >> 5; i < 32 * group; i += 8) {
+    const int row = blockIdx.x * 32 + i / group, head = h * group + i % group, p = first + row;
+    if (row >= rows) break;
+    const __nv_bfloat16* src = q + (long long)(row0 + row) * q_stride + head * D + i0;
+    float qf[N], o[N], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) qf[e] = __bfloat162float(src[e]), o[e] = 0.f;
+    for (int j = 0; j <= p; ++j) {
+      if (window > 0 && j <= p - window && j >= keep) {
+        j = p - window;
+        continue;
       }
+      const int page = request[j / page_size];
+      if (page < 0 || page >= num_pages) continue;          // (flagged when it was loaded)
+      const int off = j % page_size, tok = off % 8;
+      const unsigned char* rec = cache + (((size_t)page * nkv + h) * (page_size / 8) + off / 8) * REC;
+      const unsigned kp = *reinterpret_cast<const unsigned*>(rec + kv4_key_params_at(D) + (tok * NG + g) * 4);
+      const unsigned vp = *reinterpret_cast<const unsigned*>(rec + kv4_value_params_at(D) + (tok * NG + g) * 4);
+      float s = 0.f, v[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int c = rec[kv4_key_byte(D, tok, i0 + e)] >> ((i0 + e) % 2 * 4) & 15;
+        s += qf[e] * fmaf(kv4_scale(kp), (float)c, kv4_low(kp));
+        v[e] = fmaf(kv4_scale(vp), (float)(rec[kv4_value_byte(D, tok, i0 + e)] >> ((i0 + e) % 2 * 4) & 15), kv4_low(vp));
+      }
+      s = warp_sum(s) * scale;
+      const float top = fmaxf(m, s), f = top == m ? 1.f : expf(m - top), w = expf(s - top);
+      l = l * f + w;
+#pragma unroll
+      for (int e = 0; e < N; ++e) o[e] = o[e] * f + w * v[e];
+      m = top;
     }
-    if (!sees || row0 + row >= T) continue;
-    for (int c = 0; c < group; ++c)
-      for (int e = 0; e < 64; ++e)
-        out[(long long)(row0 + row) * out_stride + ((size_t)(h * group + c) * NG + g) * 64 + e] =
-            __ushort_as_bfloat16(0x7fc0);
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      out[(long long)(row0 + row) * out_stride + head * D + i0 + e] = __float2bfloat16_rn(o[e] / l);
   }
 }
 
-BF_EXPORT int bf_kv4_poison(const void* not_finite, const int* items, int n_items, const int* tables, int width,
-                            void* out, long long out_stride, int T, int nh, int nkv, int d, int window, int keep,
-                            cudaStream_t stream) {
-  if (n_items <= 0) return 0;
-  auto run = [&](auto kern) {
-    return bf_launch_pdl(kern, dim3(nkv, n_items), dim3(256), 0, stream, (const unsigned long long*)not_finite,
-                         items, tables, width, (__nv_bfloat16*)out, out_stride, T, nkv, nh / nkv, window, keep);
-  };
-  if (d == 64) return run(kv4_poison_kernel<1>);
-  if (d == 128) return run(kv4_poison_kernel<2>);
-  if (d == 256) return run(kv4_poison_kernel<4>);
-  return (int)cudaErrorInvalidValue;
+BF_EXPORT int bf_kv4_rest(const void* special, const int* beyond, const int* items, const int* moved, int n_items,
+                          int max_rows, const int* tables, int width, const void* cache, const int* block_tables,
+                          int table_stride, const void* q, long long q_stride, void* out, long long out_stride,
+                          int nh, int nkv, int page_size, int num_pages, int window, int keep, float scale,
+                          cudaStream_t stream) {
+  if (n_items <= 0 || max_rows <= 0) return 0;
+  return bf_launch_pdl(kv4_rest_kernel, dim3((max_rows + 31) / 32, nkv, n_items), dim3(256), 0, stream,
+                       (const unsigned long long*)special, beyond, items, moved, tables, width,
+                       (const unsigned char*)cache, block_tables, table_stride, (const __nv_bfloat16*)q, q_stride,
+                       (__nv_bfloat16*)out, out_stride, nkv, nh / nkv, page_size, num_pages, window, keep, scale);
 }

@@ -1932,11 +1932,6 @@ def kv4_load(cache: torch.Tensor, block_tables: torch.Tensor, items: torch.Tenso
     place in ``tables`` is page 0).  ``items_out``: takes the items with the portion's number in the
     request's place, which goes with ``tables``; ``places``: the width of ``tables``, where a portion's
     longest context is known to be shorter than all together."""
-    return _kv4_load(cache, block_tables, items, n_items, rows, err, window, keep_first, items_out, places)
-
-
-def _kv4_load(cache, block_tables, items, n_items, rows, err, window, keep_first, items_out, places,
-              not_finite=None):
     _want_int_table(block_tables, "kv4_load", "block_tables")
     _want(items, torch.int32, "items"); _want(err, torch.int32, "err")
     pages, nkv, ps, d = _kv4_check("kv4_load", cache, block_tables, items, err, items_out)
@@ -1952,11 +1947,11 @@ def _kv4_load(cache, block_tables, items, n_items, rows, err, window, keep_first
     k = torch.empty((n, nkv, KV4_LOAD_PAGE, d), dtype=torch.bfloat16, device=cache.device)
     v = torch.empty_like(k)
     tables = torch.empty((n_items, places), dtype=torch.int32, device=cache.device)
-    _run("kv4_load", _plain_fn("bf_kv4_load", "ppiiipipppippiiiiiiiipp"), cache.data_ptr(),
+    _run("kv4_load", _plain_fn("bf_kv4_load", "ppiiipipppipppiiiiiiiipp"), cache.data_ptr(),
          block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[0], block_tables.shape[1],
          items.data_ptr(), n_items, k.data_ptr(), v.data_ptr(), tables.data_ptr(), places,
          None if items_out is None else items_out.data_ptr(),
-         None if not_finite is None else not_finite.data_ptr(), n, nkv, d, ps, pages, window, keep_first,
+         None, None, n, nkv, d, ps, pages, window, keep_first,
          num_sms(cache.device), err.data_ptr(), _stream().value)
     return k, v, tables
 
@@ -2018,9 +2013,8 @@ def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Ten
     ``keep_first``: with a window, the request's first that many tokens stay visible behind it.
 
     ``variant``: ``stretches`` (the kernel of single tokens, a few rows at a time; reads the cache as it
-    is), ``load`` (``kv4_load`` into scratch of 4 d bytes a token and kv head, then
-    ``prefill_attention``; q contiguous, and with ``keep_first`` or an ``out`` in a column block heads of
-    128), or ``auto``."""
+    is), ``load`` (heads of 128, a positive scale, q contiguous: the contexts are loaded as ``kv4_load``
+    does, keys in fp16, into scratch of 4 d bytes a token and kv head, and attended on tcgen05), or ``auto``."""
     _want(items, torch.int32, "items")
     pages, ps, w, keep = _kv4_attention_check("kv4_prefill_attention", q, cache, block_tables, out, nh, nkv,
                                               d, window, keep_first, err, items)
@@ -2030,23 +2024,14 @@ def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Ten
         raise KernelError(f"kv4_prefill_attention: unknown variant {variant!r}")
     if n_items == 0 or max_rows == 0:
         return
-    load_ok = q.is_contiguous() and (d == 128 or (keep == 0 and out.is_contiguous())) and ctx_rows > 0
+    load_ok = d == 128 and q.is_contiguous() and ctx_rows > 0 and scale > 0
     if variant == "load" and not load_ok:
-        raise KernelError("kv4_prefill_attention: the load variant takes a contiguous q, and keep_first or an "
-                          "out in a column block with heads of 128 only")
-    if variant == "load" or (variant == "auto" and load_ok and _kv4_load_pays(
-            n_items, max_rows, max_ctx, w, keep, nh, nkv, d)):
-        moved = torch.empty((n_items, 4), dtype=torch.int32, device=q.device)
-        # groups of values that are not finite: a bit a token, see kv4_poison_kernel
-        not_finite = torch.empty((1 + ctx_rows // 64) * nkv * d // 8, dtype=torch.uint8, device=q.device)
-        places = max(1, -(-max_ctx // KV4_LOAD_PAGE))
-        k, v, tables = _kv4_load(cache, block_tables, items, n_items, ctx_rows, err, window, keep_first, moved,
-                                 places, not_finite)
-        prefill_attention(q, k, v, moved, n_items, max_rows, tables, out, nh, nkv, d, window, scale, err,
-                          max_ctx=max_ctx, keep_first=keep)
-        _run("kv4_poison", _plain_fn("bf_kv4_poison", "ppipipliiiiiip"), not_finite.data_ptr(), moved.data_ptr(),
-             n_items, tables.data_ptr(), places, out.data_ptr(), out.stride(0), q.shape[0], nh, nkv, d, w, keep,
-             _stream().value)
+        raise KernelError("kv4_prefill_attention: the load variant takes heads of 128, a contiguous q and a "
+                          "positive scale")
+    if variant == "load" or (variant == "auto" and load_ok
+                             and _kv4_load_pays(n_items, max_rows, max_ctx, w, keep, nh, nkv)):
+        _kv4_loaded_attention(q, cache, items, n_items, max_rows, block_tables, out, nh, nkv, ps, pages, window, w,
+                              keep, scale, err, ctx_rows, max_ctx)
         return
     _kv4_attention(q, cache, None, None, None, items, n_items, max_rows, block_tables, out, nh, nkv, d, ps,
                    pages, w, keep, scale, err)
@@ -2055,26 +2040,60 @@ def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Ten
 _kv4_scratch: dict = {}     # bytes of scratch by a call's sizes
 
 
-def _kv4_load_pays(n: int, max_rows: int, max_ctx: int, window: int, keep: int, nh: int, nkv: int,
-                   d: int) -> bool:
-    """Whether a call's portions are faster loaded and attended by ``prefill_attention`` than in stretches
-    of units: microseconds by sizes, fitted to both measured on a B200.  One portion of 32 heads of 128
+def _kv4_load_pays(n: int, max_rows: int, max_ctx: int, window: int, keep: int, nh: int, nkv: int) -> bool:
+    """Whether a call's portions of heads of 128 are faster loaded and attended on tcgen05 than in
+    stretches of units: microseconds by sizes, fitted to both measured on a B200.  One portion of 32 heads
     (8 kv heads), stretches against load: 64 rows behind 1,000 keys 23 / 40 us, behind 16,000 101 / 91; 128
-    rows 29 / 44 and 177 / 93; four portions of 64 rows behind 4,000 101 / 87.  16 heads of 64 (4): 128
-    rows behind 16,000 keys 72 / 332; 8 heads of 256 (2) 111 / 852."""
+    rows 29 / 44 and 177 / 93; four portions of 64 rows behind 4,000 101 / 87."""
     seen = min(max_ctx, window + keep + max_rows) if window else max_ctx
-    group, cols = nh // nkv, 8 if d == 256 else 16
-    chunks = -(-group // cols)
-    tiles = n * -(-max_rows // max(1, cols // group)) * chunks
-    # a tile's unit of sixteen keys
-    stretches = 11.0 + {64: 0.44e-3, 128: 0.64e-3, 256: 0.74e-3}[d] * tiles * nkv * (seen - max_rows / 2) / 16
-    if d == 128:          # (keys one tile after the other until they are shared out, then the products)
-        load = 12.0 + 0.025 * min(seen, 1000) + 0.13e-3 * nh * n * seen * -(-max_rows // 256)
-    elif d == 64:         # one tile after the other, 296 blocks of 128 rows at a time
-        load = 12.0 + 0.0205 * seen * max(1.0, nh * n * -(-max_rows // 128) / 296)
-    else:                 # the same of 64 rows
-        load = 12.0 + 0.0525 * seen * max(1.0, nh * n * -(-max_rows // 64) / 296)
+    group = nh // nkv
+    tiles = n * -(-max_rows // max(1, 16 // group)) * -(-group // 16)
+    stretches = 11.0 + 0.64e-3 * tiles * nkv * (seen - max_rows / 2) / 16        # (0.64 ns a tile's unit)
+    # keys one tile after the other until they are shared out, then the products
+    load = 12.0 + 0.025 * min(seen, 1000) + 0.13e-3 * nh * n * seen * -(-max_rows // 256)
     return load < stretches
+
+
+def _kv4_loaded_attention(q, cache, items, n_items, max_rows, block_tables, out, nh, nkv, ps, pages, window, w,
+                          keep, scale, err, ctx_rows, max_ctx) -> None:
+    global _launches
+    d, T = 128, q.shape[0]
+    n = 1 + ctx_rows // KV4_LOAD_PAGE
+    places = max(1, -(-max_ctx // KV4_LOAD_PAGE))
+    # few blocks and long contexts: the keys of each block shared out, as ``prefill_attention`` does
+    sms = num_sms(q.device)
+    blocks = -(-max_rows // 256) * nh * n_items
+    splits = max(1, min(8, sms // blocks, max_ctx // 1024)) if not w and 2 * blocks <= sms else 1
+    if T * nh * splits * d * 4 > _PREFILL_SPLIT_BYTES:
+        splits = 1
+    # one piece of scratch for all: keys, values, a byte a record, the pages of each portion, the items,
+    # what is beyond fp16, the shares of the keys
+    sizes = (n * nkv * KV4_LOAD_PAGE * d * 2, n * nkv * KV4_LOAD_PAGE * d * 2, n * nkv * 8, n_items * places * 4,
+             n_items * 16, n_items * nkv * 4, T * nh * splits * d * 4 if splits > 1 else 0,
+             T * nh * splits * 8 if splits > 1 else 0)
+    at, total = [], 0
+    for size in sizes:
+        at.append(total)
+        total += (size + 255) // 256 * 256
+    scratch = torch.empty(total, dtype=torch.uint8, device=q.device)
+    base = scratch.data_ptr()
+    k, v, special, tables, moved, beyond, part_o, part_ml = (base + a for a in at)
+    if splits == 1:
+        part_o = part_ml = None
+    else:
+        _launches += 1
+    table_args = (block_tables.data_ptr(), block_tables.stride(0))
+    item_ptr, cache_ptr, q_ptr, out_ptr, err_ptr = (t.data_ptr() for t in (items, cache, q, out, err))
+    out_stride, stream = out.stride(0), _stream().value
+    _run("kv4_load", _plain_fn("bf_kv4_load", "ppiiipipppipppiiiiiiiipp"), cache_ptr, *table_args,
+         block_tables.shape[0], block_tables.shape[1], item_ptr, n_items, k, v, tables, places, moved, special, beyond,
+         n, nkv, d, ps, pages, w, keep, sms, err_ptr, stream)
+    _run("prefill_attention_umma2", _plain_fn("bf_prefill_attention_umma2_half", "ppppiiipipiiiiiifippplipp"),
+         q_ptr, k, v, moved, n_items, max_rows, T, tables, places, out_ptr, nh, nkv, d, KV4_LOAD_PAGE, n, w, scale,
+         splits, part_o, part_ml, err_ptr, out_stride, keep, beyond, stream)
+    _run("kv4_rest", _plain_fn("bf_kv4_rest", "ppppiipippiplpliiiiiifp"), special, beyond, item_ptr, moved, n_items,
+         max_rows, tables, places, cache_ptr, *table_args, q_ptr, q.stride(0), out_ptr, out_stride, nh, nkv, ps, pages,
+         w, keep, scale, stream)
 
 
 def _kv4_attention(q, cache, rows, seq_of_token, positions, items, n, max_rows, block_tables, out, nh, nkv, d,

@@ -589,8 +589,8 @@ def test_a_run_of_steps(cuda_device, window, keep):
 @pytest.mark.parametrize("window,keep", [(None, 0), (64, 0), (100, 11)])
 def test_both_ways_of_a_portion(cuda_device, variant, nh, nkv, d, ps, window, keep):
     from binfer_b200.csrc import ops
-    if variant == "load" and keep and d != 128:
-        pytest.skip("kept tokens are the 128-sized heads' alone on this way")
+    if variant == "load" and d != 128:
+        pytest.skip("heads of 128 alone go this way")
     c = Cache([300, 70, 1], nkv, d, ps, cuda_device, seed=nh)
     jobs = [(1, 70, 0), (0, 33, 267), (2, 1, 0)]
     q = _queries(104, nh, d, cuda_device)
@@ -614,3 +614,46 @@ def test_load_without_room_attends_what_fits(cuda_device):
     assert int(c.err.item()) == 16 and not out[50:].any()
     c.err.zero_()
     _compare(c, q[:50], out[:50], nh, [(0, 50, 50)], None, 0, 0.1)
+
+
+@pytest.mark.parametrize("what", ["queries", "keys", "both", "one key"])
+@pytest.mark.parametrize("window,keep", [(None, 0), (150, 4)])
+def test_loaded_keys_and_queries_beyond_fp16(cuda_device, what, window, keep):
+    """Numbers that fp16 has no room for, with a scale that makes ordinary scores of them."""
+    from binfer_b200.csrc import ops
+    nh, nkv, d, n, new = 6, 3, 128, 400, 100
+    c = Cache([n], nkv, d, 16, cuda_device, seed=9)
+    q = _queries(new, nh, d, cuda_device)
+    scale = d ** -0.5
+    if what in ("queries", "both"):
+        q, scale = (q.float() * 2.0 ** 17).to(BF16), scale * 2.0 ** -17
+    if what in ("keys", "both"):
+        c.k[0], scale = (c.k[0].float() * 2.0 ** 18).to(BF16), scale * 2.0 ** -18
+    if what == "one key":
+        c.k[0][350, 1, 7] = 70000.0
+        q[:, nh // 3 * d + 7:2 * nh // 3 * d:d] = 2.0 ** -14
+    ops.kv4_store(c.k[0].flatten(1), c.v[0].flatten(1), c.slots[0], c.cache, c.err)
+    out = torch.full_like(q, math.nan)
+    items = torch.tensor([(0, 0, new, n - new)], dtype=I32, device=cuda_device)
+    ops.kv4_prefill_attention(q, c.cache, items, 1, new, c.tables, out, nh, nkv, d, window, scale, c.err,
+                              ctx_rows=448, max_ctx=n, keep_first=keep, variant="load")
+    _compare(c, q, out, nh, [(0, new, n - new)], window, keep, scale)
+
+
+def test_loaded_portions_are_as_close_as_stretches(cuda_device):
+    """Keys in fp16: what is left of the error is that of the probabilities, the values and the result
+    in bfloat16, 1.7e-3 and twice 1.1e-3 of the result's rms (each half a step uniform, 2^-8 / sqrt(3) of a
+    number's upper bound, 0.75 of it on average); 2.3e-3 together, where bfloat16 keys add 2.5e-3 or more."""
+    from binfer_b200.csrc import ops
+    nh, nkv, d, n = 8, 2, 128, 600
+    c = Cache([n], nkv, d, 16, cuda_device, seed=2)
+    q = _queries(300, nh, d, cuda_device) * 1.5
+    items = torch.tensor([(0, 0, 300, 300)], dtype=I32, device=cuda_device)
+    k, v = c.held(0)
+    ref, _ = K4.attend(q.view(300, nh, d).to(F64), k, v, torch.arange(300, 600, device=q.device), None, 0, d ** -0.5)
+    for variant in ("stretches", "load"):
+        out = torch.empty_like(q)
+        ops.kv4_prefill_attention(q, c.cache, items, 1, 300, c.tables, out, nh, nkv, d, None, d ** -0.5, c.err,
+                                  ctx_rows=640, max_ctx=n, variant=variant)
+        off = (out.view(300, nh, d).to(F64) - ref).square().mean().sqrt() / ref.square().mean().sqrt()
+        assert off <= 2.8e-3, (variant, float(off))
