@@ -754,12 +754,27 @@ BF_EXPORT long long bf_kv4_attention_scratch(int n, int max_rows, int nh, int nk
   return slots * 8 * s.nt * (d * 4 + 8) + tiles * nkv * s.chunks * 16;
 }
 
-BF_EXPORT int bf_kv4_attention(const void* q, long long q_stride, const void* cache, const int* rows,
-                               const int* seq_of_token, const int* positions, const int* items, int n,
-                               int max_rows, int T, const int* block_tables, int table_stride, int table_rows,
-                               int table_width, void* out, long long out_stride, int nh, int nkv, int d,
-                               int page_size, int num_pages, int window, int keep, float scale, void* scratch,
-                               int sms, int* err, cudaStream_t stream) {
+struct Kv4AttentionCall {
+  const void* q;
+  long long q_stride;
+  const void* cache;
+  const int* rows, *seq_of_token, *positions, *items;
+  int n, max_rows, T;
+  const int* block_tables;
+  int table_stride, table_rows, table_width;
+  void* out;
+  long long out_stride;
+  int nh, nkv, d, page_size, num_pages, window, keep;
+  float scale;
+  void* scratch;
+  int sms;
+  int* err;
+  cudaStream_t stream;
+};
+BF_EXPORT int bf_kv4_attention(const Kv4AttentionCall* call) {
+  const auto& [q, q_stride, cache, rows, seq_of_token, positions, items, n, max_rows, T, block_tables,
+               table_stride, table_rows, table_width, out, out_stride, nh, nkv, d, page_size, num_pages,
+               window, keep, scale, scratch, sms, err, stream] = *call;
   if (n <= 0 || max_rows <= 0) return 0;
   if ((long long)num_pages * nkv * (page_size / 8) > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
   const KaShape s = ka_shape(nh / nkv, d, max_rows);

@@ -872,12 +872,27 @@ BF_EXPORT int bf_prefill_attention_umma2_capped(
 }
 
 // bfloat16 queries and values over fp16 keys.
-BF_EXPORT int bf_prefill_attention_umma2_half(
-    const void* q, const void* k_cache, const void* v_cache, const int* items, int n_items,
-    int max_rows, int total_rows, const int* block_tables, int table_stride, void* out, int nh,
-    int nkv, int d, int page_size, int num_pages, int window, float scale, int splits,
-    float* part_o, float* part_ml, int* err, long long out_stride, int keep, int* beyond,
-    cudaStream_t stream) {
+struct PrefillAttentionUmma2HalfCall {
+  const void* q, *k_cache, *v_cache;
+  const int* items;
+  int n_items, max_rows, total_rows;
+  const int* block_tables;
+  int table_stride;
+  void* out;
+  int nh, nkv, d, page_size, num_pages, window;
+  float scale;
+  int splits;
+  float* part_o, *part_ml;
+  int* err;
+  long long out_stride;
+  int keep;
+  int* beyond;
+  cudaStream_t stream;
+};
+BF_EXPORT int bf_prefill_attention_umma2_half(const PrefillAttentionUmma2HalfCall* call) {
+  const auto& [q, k_cache, v_cache, items, n_items, max_rows, total_rows, block_tables, table_stride, out,
+               nh, nkv, d, page_size, num_pages, window, scale, splits, part_o, part_ml, err, out_stride,
+               keep, beyond, stream] = *call;
   if (!beyond) return (int)cudaErrorInvalidValue;
   return launch_umma2(q, k_cache, v_cache, items, n_items, max_rows, total_rows, block_tables, table_stride, out,
                       nh, nkv, d, page_size, num_pages, window, scale, splits, part_o, part_ml, err, 0.f,

@@ -109,9 +109,21 @@ kv4_store_kernel(const __nv_bfloat16* __restrict__ k, long long k_stride,
         (unsigned)__bfloat16_as_ushort(sb) | (unsigned)__bfloat16_as_ushort(mb) << 16;
 }
 
-BF_EXPORT int bf_kv4_store(const void* k, long long k_stride, const void* v, long long v_stride,
-                           const int* slots, void* cache, int T, int nkv, int d, int page_size,
-                           long long num_slots, int* err, cudaStream_t stream) {
+struct Kv4StoreCall {
+  const void* k;
+  long long k_stride;
+  const void* v;
+  long long v_stride;
+  const int* slots;
+  void* cache;
+  int T, nkv, d, page_size;
+  long long num_slots;
+  int* err;
+  cudaStream_t stream;
+};
+BF_EXPORT int bf_kv4_store(const Kv4StoreCall* call) {
+  const auto& [k, k_stride, v, v_stride, slots, cache, T, nkv, d, page_size, num_slots, err, stream] =
+               *call;
   if (T <= 0) return 0;
   if ((d != 64 && d != 128 && d != 256) || page_size < 8 || (page_size & (page_size - 1)))
     return (int)cudaErrorInvalidValue;
@@ -309,11 +321,26 @@ kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
 }
 
 // special (8 bytes a page and head) and beyond (n_items x nkv), both or neither: keys in fp16, heads of 128.
-BF_EXPORT int bf_kv4_load(const void* cache, const int* block_tables, int table_stride, int table_rows,
-                          int table_width, const int* items, int n_items, void* k_out, void* v_out,
-                          int* tables_out, int out_width, int* items_out, void* special, int* beyond,
-                          int out_pages, int nkv, int d, int page_size, int num_pages, int window, int keep,
-                          int sms, int* err, cudaStream_t stream) {
+struct Kv4LoadCall {
+  const void* cache;
+  const int* block_tables;
+  int table_stride, table_rows, table_width;
+  const int* items;
+  int n_items;
+  void* k_out, *v_out;
+  int* tables_out;
+  int out_width;
+  int* items_out;
+  void* special;
+  int* beyond;
+  int out_pages, nkv, d, page_size, num_pages, window, keep, sms;
+  int* err;
+  cudaStream_t stream;
+};
+BF_EXPORT int bf_kv4_load(const Kv4LoadCall* call) {
+  const auto& [cache, block_tables, table_stride, table_rows, table_width, items, n_items, k_out, v_out,
+               tables_out, out_width, items_out, special, beyond, out_pages, nkv, d, page_size, num_pages,
+               window, keep, sms, err, stream] = *call;
   if (n_items <= 0 || out_pages <= 1) return 0;
   if ((special != nullptr) != (beyond != nullptr) || (special && d != 128)) return (int)cudaErrorInvalidValue;
   // heads apart where pages alone would leave SMs without blocks
@@ -395,11 +422,27 @@ kv4_rest_kernel(const unsigned long long* __restrict__ special, const int* __res
   }
 }
 
-BF_EXPORT int bf_kv4_rest(const void* special, const int* beyond, const int* items, const int* moved, int n_items,
-                          int max_rows, const int* tables, int width, const void* cache, const int* block_tables,
-                          int table_stride, const void* q, long long q_stride, void* out, long long out_stride,
-                          int nh, int nkv, int page_size, int num_pages, int window, int keep, float scale,
-                          cudaStream_t stream) {
+struct Kv4RestCall {
+  const void* special;
+  const int* beyond, *items, *moved;
+  int n_items, max_rows;
+  const int* tables;
+  int width;
+  const void* cache;
+  const int* block_tables;
+  int table_stride;
+  const void* q;
+  long long q_stride;
+  void* out;
+  long long out_stride;
+  int nh, nkv, page_size, num_pages, window, keep;
+  float scale;
+  cudaStream_t stream;
+};
+BF_EXPORT int bf_kv4_rest(const Kv4RestCall* call) {
+  const auto& [special, beyond, items, moved, n_items, max_rows, tables, width, cache, block_tables,
+               table_stride, q, q_stride, out, out_stride, nh, nkv, page_size, num_pages, window, keep,
+               scale, stream] = *call;
   if (n_items <= 0 || max_rows <= 0) return 0;
   return bf_launch_pdl(kv4_rest_kernel, dim3((max_rows + 31) / 32, nkv, n_items), dim3(256), 0, stream,
                        (const unsigned long long*)special, beyond, items, moved, tables, width,

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -1852,11 +1853,12 @@ _kv4_sizes: dict = {}      # shapes that are caches in 4 bits -> (pages, kv head
 def _kv4_check(what: str, cache: torch.Tensor, *others) -> Tuple[int, int, int, int]:
     """(pages, kv heads, page size, head size) of a cache in 4 bits; every tensor on the device that the
     launch goes to."""
-    if cache.dtype != torch.uint8 or cache.dim() != 4 or not cache.is_contiguous() or cache.data_ptr() % 16:
-        raise KernelError(f"{what}: cache must be contiguous uint8 [pages, kv heads, page_size / 8, 9 d] "
-                          "on a 16-byte boundary")
     sizes = _kv4_sizes.get(cache.shape)
-    if sizes is None:
+    if (sizes is None or cache.dtype != torch.uint8 or not cache.is_contiguous()
+            or cache.data_ptr() % 16):
+        if cache.dtype != torch.uint8 or cache.dim() != 4 or not cache.is_contiguous() or cache.data_ptr() % 16:
+            raise KernelError(f"{what}: cache must be contiguous uint8 [pages, kv heads, page_size / 8, 9 d] "
+                              "on a 16-byte boundary")
         pages, nkv, eighths, rec = cache.shape
         if rec % 9 or not kv4_takes(torch.bfloat16, rec // 9, 8 * eighths):
             raise KernelError(f"{what}: pages of {8 * eighths} tokens and records of {rec} bytes are no cache "
@@ -1878,23 +1880,37 @@ def _same_device(what: str, *tensors) -> None:
                               f"{torch.cuda.current_device()}")
 
 
-def _want_int_table(t: torch.Tensor, what: str, name: str) -> None:
-    if t.dtype != torch.int32 or t.dim() != 2 or t.stride(1) != 1 or not t.numel():
-        raise KernelError(f"{what}: {name} must be int32 with two dimensions and contiguous rows")
+def _want_int_table(t: torch.Tensor, what: str, name: str) -> Tuple[int, int, int]:
+    """(rows, columns, row stride) of an int32 table."""
+    if t.dtype == torch.int32 and t.dim() == 2:
+        rows, columns = t.shape
+        stride, one = t.stride()
+        if one == 1 and rows and columns:
+            return rows, columns, stride
+    raise KernelError(f"{what}: {name} must be int32 with two dimensions and contiguous rows")
 
 
-_plain_fns: dict = {}
+class _Packed:
+    """A launcher that takes its arguments as one struct, packed here: ``P`` an address (0: none), ``q`` a
+    long long, ``i`` an int, ``f`` a float.  (A ctypes object per argument costs more than the launch.)"""
+
+    def __init__(self, name: str, fields: str):
+        self.name, self.pack, self.fn = name, struct.Struct("@" + fields).pack, None
+
+    def __call__(self, *args) -> int:
+        if self.fn is None:
+            fn = getattr(lib(), self.name)
+            fn.argtypes = [ctypes.c_char_p]
+            self.fn = fn
+        return self.fn(self.pack(*args))
 
 
-def _plain_fn(name: str, signature: str):
-    """A launcher whose arguments are Python numbers and addresses: ``p`` an address or None, ``i`` an
-    int, ``l`` a long long, ``f`` a float.  (A ctypes object per argument costs more than the launch.)"""
-    fn = _plain_fns.get(name)
-    if fn is None:
-        fn = getattr(lib(), name)
-        fn.argtypes = [{"p": _c_void_p, "i": _c_int, "l": _c_ll, "f": _c_float}[c] for c in signature]
-        _plain_fns[name] = fn
-    return fn
+_kv4_store_call = _Packed("bf_kv4_store", "PqPqPPiiiiqPP")
+_kv4_load_call = _Packed("bf_kv4_load", "PPiiiPiPPPiPPPiiiiiiiiPP")
+_kv4_rest_call = _Packed("bf_kv4_rest", "PPPPiiPiPPiPqPqiiiiiifP")
+_kv4_attention_call = _Packed("bf_kv4_attention", "PqPPPPPiiiPiiiPqiiiiiiifPiPP")
+_step_tables_call = _Packed("bf_step_tables", "PiiPiPiiiPPPPPiPiPiPiPP")
+_prefill_attention_umma2_half_call = _Packed("bf_prefill_attention_umma2_half", "PPPPiiiPiPiiiiiifiPPPqiPP")
 
 
 def kv4_store(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: torch.Tensor,
@@ -1905,20 +1921,21 @@ def kv4_store(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: torc
 
     Of 64 numbers x: m = min x, s = bfloat16((max x - m) / 15), c = (x - m) / s rounded to the nearest
     whole number (ties to even).  A number that is not finite makes its 64 neighbours read as NaN."""
-    T = k.shape[0] if k.dim() == 2 else -1
-    if (T < 0 or v.dim() != 2 or k.shape != v.shape or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16
-            or (T and (k.stride(1) != 1 or v.stride(1) != 1))):
+    if k.dim() != 2 or k.shape != v.shape or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+        raise KernelError("kv4_store: k and v must be bfloat16 [T, kv heads * d] with contiguous rows")
+    T, width = k.shape
+    (k_stride, k_one), (v_stride, v_one) = k.stride(), v.stride()
+    if T and (k_one != 1 or v_one != 1):
         raise KernelError("kv4_store: k and v must be bfloat16 [T, kv heads * d] with contiguous rows")
     _want(slots, torch.int32, "slots"); _want(err, torch.int32, "err")
     pages, nkv, ps, d = _kv4_check("kv4_store", cache, k, v, slots, err)
-    if k.shape[1] != nkv * d or slots.numel() != T:
+    if width != nkv * d or slots.numel() != T:
         raise KernelError(f"kv4_store: rows of {nkv} heads of {d} and a slot per token, got "
                           f"{tuple(k.shape)} and {slots.numel()} slots")
     if T == 0:
         return
-    _run("kv4_store", _plain_fn("bf_kv4_store", "plplppiiiilpp"), k.data_ptr(), k.stride(0), v.data_ptr(),
-         v.stride(0), slots.data_ptr(), cache.data_ptr(), T, nkv, d, ps, pages * ps, err.data_ptr(),
-         _stream().value)
+    _run("kv4_store", _kv4_store_call, k.data_ptr(), k_stride, v.data_ptr(), v_stride, slots.data_ptr(),
+         cache.data_ptr(), T, nkv, d, ps, pages * ps, err.data_ptr(), _stream().value or 0)
 
 
 def kv4_load(cache: torch.Tensor, block_tables: torch.Tensor, items: torch.Tensor, n_items: int,
@@ -1932,7 +1949,7 @@ def kv4_load(cache: torch.Tensor, block_tables: torch.Tensor, items: torch.Tenso
     place in ``tables`` is page 0).  ``items_out``: takes the items with the portion's number in the
     request's place, which goes with ``tables``; ``places``: the width of ``tables``, where a portion's
     longest context is known to be shorter than all together."""
-    _want_int_table(block_tables, "kv4_load", "block_tables")
+    table_rows, table_width, table_stride = _want_int_table(block_tables, "kv4_load", "block_tables")
     _want(items, torch.int32, "items"); _want(err, torch.int32, "err")
     pages, nkv, ps, d = _kv4_check("kv4_load", cache, block_tables, items, err, items_out)
     if n_items < 1 or items.numel() < 4 * n_items or rows < 64 or rows % 64 or places < 0:
@@ -1942,17 +1959,15 @@ def kv4_load(cache: torch.Tensor, block_tables: torch.Tensor, items: torch.Tenso
         if items_out.numel() < 4 * n_items:
             raise KernelError("kv4_load: items_out must have room for the items")
     window, keep_first = _kv4_mask("kv4_load", window, keep_first)
-    n = 1 + rows // 64
+    n, device = 1 + rows // 64, cache.device
     places = places or n - 1
-    k = torch.empty((n, nkv, KV4_LOAD_PAGE, d), dtype=torch.bfloat16, device=cache.device)
+    k = torch.empty((n, nkv, KV4_LOAD_PAGE, d), dtype=torch.bfloat16, device=device)
     v = torch.empty_like(k)
-    tables = torch.empty((n_items, places), dtype=torch.int32, device=cache.device)
-    _run("kv4_load", _plain_fn("bf_kv4_load", "ppiiipipppipppiiiiiiiipp"), cache.data_ptr(),
-         block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[0], block_tables.shape[1],
-         items.data_ptr(), n_items, k.data_ptr(), v.data_ptr(), tables.data_ptr(), places,
-         None if items_out is None else items_out.data_ptr(),
-         None, None, n, nkv, d, ps, pages, window, keep_first,
-         num_sms(cache.device), err.data_ptr(), _stream().value)
+    tables = torch.empty((n_items, places), dtype=torch.int32, device=device)
+    _run("kv4_load", _kv4_load_call, cache.data_ptr(), block_tables.data_ptr(), table_stride, table_rows,
+         table_width, items.data_ptr(), n_items, k.data_ptr(), v.data_ptr(), tables.data_ptr(), places,
+         items_out.data_ptr() if items_out is not None else 0, 0, 0, n, nkv, d, ps, pages, window, keep_first,
+         num_sms(device), err.data_ptr(), _stream().value or 0)
     return k, v, tables
 
 
@@ -1963,20 +1978,31 @@ def _kv4_mask(what: str, window: Optional[int], keep_first: int) -> Tuple[int, i
 
 
 def _kv4_attention_check(what, q, cache, block_tables, out, nh, nkv, d, window, keep_first, err, *others):
-    _want_int_table(block_tables, what, "block_tables")
+    """Of an attention call: (table rows, columns, stride), (rows of q, strides of q and out), pages, page
+    size, window (0: none), kept tokens."""
+    table = _want_int_table(block_tables, what, "block_tables")
     _want(err, torch.int32, "err")
     pages, c_nkv, ps, c_d = _kv4_check(what, cache, q, block_tables, out, err, *others)
-    if (c_nkv, c_d) != (nkv, d) or nh < 1 or nh % nkv:
+    if c_nkv != nkv or c_d != d or nh < 1 or nh % nkv:
         raise KernelError(f"{what}: the cache has {c_nkv} heads of {c_d}, the call names {nkv} of {d} for "
                           f"{nh} query heads")
-    for name, t in (("q", q), ("out", out)):
-        if (t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape[1] != nh * d or t.stride(1) != 1
-                or t.stride(0) % 8 or t.data_ptr() % 16):
-            raise KernelError(f"{what}: {name} must be bfloat16 [T, heads * d], rows contiguous and on "
-                              "16-byte boundaries")
-    if out.shape[0] < q.shape[0]:
+    sizes = []
+    for t in (q, out):
+        if t.dtype == torch.bfloat16 and t.dim() == 2:
+            rows, width = t.shape
+            stride, one = t.stride()
+            if width == nh * d and one == 1 and not stride % 8 and not t.data_ptr() % 16:
+                sizes += (rows, stride)
+                continue
+        raise KernelError(f"{what}: {'q' if t is q else 'out'} must be bfloat16 [T, heads * d], rows contiguous "
+                          "and on 16-byte boundaries")
+    T, q_stride, out_rows, out_stride = sizes
+    if out_rows < T:
         raise KernelError(f"{what}: out has fewer rows than q")
-    return (pages, ps) + _kv4_mask(what, window, keep_first)
+    if window is None:
+        if keep_first >= 0:
+            return table, (T, q_stride, out_stride), pages, ps, 0, 0
+    return (table, (T, q_stride, out_stride), pages, ps) + _kv4_mask(what, window, keep_first)
 
 
 def kv4_decode_attention(q: torch.Tensor, cache: torch.Tensor, rows: Optional[torch.Tensor], n_rows: int,
@@ -1991,16 +2017,18 @@ def kv4_decode_attention(q: torch.Tensor, cache: torch.Tensor, rows: Optional[to
     _want(seq_of_token, torch.int32, "seq_of_token"); _want(positions, torch.int32, "positions")
     if rows is not None:
         _want(rows, torch.int32, "rows")
-    pages, ps, w, keep = _kv4_attention_check("kv4_decode_attention", q, cache, block_tables, out, nh, nkv,
-                                              d, window, keep_first, err, rows, seq_of_token, positions)
-    T = q.shape[0]
+    table, strides, pages, ps, w, keep = _kv4_attention_check(
+        "kv4_decode_attention", q, cache, block_tables, out, nh, nkv, d, window, keep_first, err, rows,
+        seq_of_token, positions)
+    T = strides[0]
     if (n_rows < 0 or (rows is None and n_rows > T) or (rows is not None and rows.numel() < n_rows)
             or seq_of_token.numel() < T or positions.numel() < T):
         raise KernelError("kv4_decode_attention: a request and a position per token row, and rows inside q")
     if n_rows == 0:
         return
-    _kv4_attention(q, cache, rows, seq_of_token, positions, None, n_rows, 1, block_tables, out, nh, nkv, d,
-                   ps, pages, w, keep, scale, err)
+    _kv4_attention(q, cache, rows.data_ptr() if rows is not None else 0, seq_of_token.data_ptr(),
+                   positions.data_ptr(), 0, n_rows, 1, block_tables, table, strides, out, nh, nkv, d, ps, pages, w,
+                   keep, scale, err)
 
 
 def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Tensor, n_items: int,
@@ -2016,8 +2044,8 @@ def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Ten
     is), ``load`` (heads of 128, a positive scale, q contiguous: the contexts are loaded as ``kv4_load``
     does, keys in fp16, into scratch of 4 d bytes a token and kv head, and attended on tcgen05), or ``auto``."""
     _want(items, torch.int32, "items")
-    pages, ps, w, keep = _kv4_attention_check("kv4_prefill_attention", q, cache, block_tables, out, nh, nkv,
-                                              d, window, keep_first, err, items)
+    table, strides, pages, ps, w, keep = _kv4_attention_check(
+        "kv4_prefill_attention", q, cache, block_tables, out, nh, nkv, d, window, keep_first, err, items)
     if n_items < 0 or items.numel() < 4 * n_items or max_rows < 0 or ctx_rows < 0 or ctx_rows % 64:
         raise KernelError("kv4_prefill_attention: items must be [n_items, 4], ctx_rows a multiple of 64")
     if variant not in ("auto", "stretches", "load"):
@@ -2030,11 +2058,11 @@ def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Ten
                           "positive scale")
     if variant == "load" or (variant == "auto" and load_ok
                              and _kv4_load_pays(n_items, max_rows, max_ctx, w, keep, nh, nkv)):
-        _kv4_loaded_attention(q, cache, items, n_items, max_rows, block_tables, out, nh, nkv, ps, pages, window, w,
-                              keep, scale, err, ctx_rows, max_ctx)
+        _kv4_loaded_attention(q, cache, items, n_items, max_rows, block_tables, table, strides, out, nh, nkv, ps,
+                              pages, w, keep, scale, err, ctx_rows, max_ctx)
         return
-    _kv4_attention(q, cache, None, None, None, items, n_items, max_rows, block_tables, out, nh, nkv, d, ps,
-                   pages, w, keep, scale, err)
+    _kv4_attention(q, cache, 0, 0, 0, items.data_ptr(), n_items, max_rows, block_tables, table, strides, out, nh,
+                   nkv, d, ps, pages, w, keep, scale, err)
 
 
 _kv4_scratch: dict = {}     # bytes of scratch by a call's sizes
@@ -2054,10 +2082,10 @@ def _kv4_load_pays(n: int, max_rows: int, max_ctx: int, window: int, keep: int, 
     return load < stretches
 
 
-def _kv4_loaded_attention(q, cache, items, n_items, max_rows, block_tables, out, nh, nkv, ps, pages, window, w,
+def _kv4_loaded_attention(q, cache, items, n_items, max_rows, block_tables, table, strides, out, nh, nkv, ps, pages, w,
                           keep, scale, err, ctx_rows, max_ctx) -> None:
     global _launches
-    d, T = 128, q.shape[0]
+    d, (T, q_stride, out_stride), (table_rows, table_width, table_stride) = 128, strides, table
     n = 1 + ctx_rows // KV4_LOAD_PAGE
     places = max(1, -(-max_ctx // KV4_LOAD_PAGE))
     # few blocks and long contexts: the keys of each block shared out, as ``prefill_attention`` does
@@ -2079,27 +2107,27 @@ def _kv4_loaded_attention(q, cache, items, n_items, max_rows, block_tables, out,
     base = scratch.data_ptr()
     k, v, special, tables, moved, beyond, part_o, part_ml = (base + a for a in at)
     if splits == 1:
-        part_o = part_ml = None
+        part_o = part_ml = 0
     else:
         _launches += 1
-    table_args = (block_tables.data_ptr(), block_tables.stride(0))
-    item_ptr, cache_ptr, q_ptr, out_ptr, err_ptr = (t.data_ptr() for t in (items, cache, q, out, err))
-    out_stride, stream = out.stride(0), _stream().value
-    _run("kv4_load", _plain_fn("bf_kv4_load", "ppiiipipppipppiiiiiiiipp"), cache_ptr, *table_args,
-         block_tables.shape[0], block_tables.shape[1], item_ptr, n_items, k, v, tables, places, moved, special, beyond,
+    table_ptr, item_ptr, cache_ptr, q_ptr, out_ptr, err_ptr = (t.data_ptr() for t in (block_tables, items, cache, q, out, err))
+    stream = _stream().value or 0
+    _run("kv4_load", _kv4_load_call, cache_ptr, table_ptr, table_stride,
+         table_rows, table_width, item_ptr, n_items, k, v, tables, places, moved, special, beyond,
          n, nkv, d, ps, pages, w, keep, sms, err_ptr, stream)
-    _run("prefill_attention_umma2", _plain_fn("bf_prefill_attention_umma2_half", "ppppiiipipiiiiiifippplipp"),
+    _run("prefill_attention_umma2", _prefill_attention_umma2_half_call,
          q_ptr, k, v, moved, n_items, max_rows, T, tables, places, out_ptr, nh, nkv, d, KV4_LOAD_PAGE, n, w, scale,
          splits, part_o, part_ml, err_ptr, out_stride, keep, beyond, stream)
-    _run("kv4_rest", _plain_fn("bf_kv4_rest", "ppppiipippiplpliiiiiifp"), special, beyond, item_ptr, moved, n_items,
-         max_rows, tables, places, cache_ptr, *table_args, q_ptr, q.stride(0), out_ptr, out_stride, nh, nkv, ps, pages,
+    _run("kv4_rest", _kv4_rest_call, special, beyond, item_ptr, moved, n_items,
+         max_rows, tables, places, cache_ptr, table_ptr, table_stride, q_ptr, q_stride, out_ptr, out_stride, nh, nkv, ps, pages,
          w, keep, scale, stream)
 
 
-def _kv4_attention(q, cache, rows, seq_of_token, positions, items, n, max_rows, block_tables, out, nh, nkv, d,
-                   ps, pages, window, keep, scale, err):
+def _kv4_attention(q, cache, rows, seq, positions, items, n, max_rows, block_tables, table, strides, out, nh,
+                   nkv, d, ps, pages, window, keep, scale, err) -> None:
     global _launches
-    sms = num_sms(q.device)
+    device = q.device
+    sms = num_sms(device)
     key = (n, max_rows, nh, nkv, d, sms)
     size = _kv4_scratch.get(key)
     if size is None:
@@ -2109,14 +2137,13 @@ def _kv4_attention(q, cache, rows, seq_of_token, positions, items, n, max_rows, 
             _kv4_scratch.clear()
         size = _kv4_scratch[key] = fn(n, max_rows, nh, nkv, d, sms)
     # a call's own, from its stream's pool: two captured graphs share nothing
-    scratch = torch.empty(size, dtype=torch.uint8, device=q.device)
-    _run("kv4_attention", _plain_fn("bf_kv4_attention", "plpppppiiipiiipliiiiiiifpipp"), q.data_ptr(), q.stride(0),
-         cache.data_ptr(), None if rows is None else rows.data_ptr(),
-         None if seq_of_token is None else seq_of_token.data_ptr(),
-         None if positions is None else positions.data_ptr(), None if items is None else items.data_ptr(), n,
-         max_rows, q.shape[0], block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[0],
-         block_tables.shape[1], out.data_ptr(), out.stride(0), nh, nkv, d, ps, pages, window, keep, scale,
-         scratch.data_ptr(), sms, err.data_ptr(), _stream().value)
+    scratch = torch.empty(size, dtype=torch.uint8, device=device)
+    table_rows, table_width, table_stride = table
+    T, q_stride, out_stride = strides
+    _run("kv4_attention", _kv4_attention_call, q.data_ptr(), q_stride, cache.data_ptr(), rows, seq, positions,
+         items, n, max_rows, T, block_tables.data_ptr(), table_stride, table_rows, table_width, out.data_ptr(),
+         out_stride, nh, nkv, d, ps, pages, window, keep, scale, scratch.data_ptr(), sms, err.data_ptr(),
+         _stream().value or 0)
     _launches += 1          # two kernels: the stretches of units, and what several of them share
 
 
@@ -2160,12 +2187,12 @@ def step_tables(master: torch.Tensor, entries: torch.Tensor, new_pages: torch.Te
         return
     n_dec = decode_rows.numel() if decode_rows is not None else 0
     n_pf = prefill_items.numel() // 4 if prefill_items is not None else 0
-    _run("step_tables", _plain_fn("bf_step_tables", "piipipiiipppppipipipipp"), master.data_ptr(), master.shape[0],
+    _run("step_tables", _step_tables_call, master.data_ptr(), master.shape[0],
          master.shape[1], entries.data_ptr(), B, new_pages.data_ptr(), new_pages.numel(), page_size, num_pages,
          q_start.data_ptr(), positions.data_ptr(), seq_of_token.data_ptr(), ctx_lens.data_ptr(),
          slots.data_ptr(), T, tables.data_ptr(), tables.shape[1],
-         None if decode_rows is None else decode_rows.data_ptr(), n_dec,
-         None if prefill_items is None else prefill_items.data_ptr(), n_pf, err.data_ptr(), _stream().value)
+         decode_rows.data_ptr() if decode_rows is not None else 0, n_dec,
+         prefill_items.data_ptr() if prefill_items is not None else 0, n_pf, err.data_ptr(), (_stream().value or 0))
 
 
 class DiffCombine:

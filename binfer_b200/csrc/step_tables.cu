@@ -93,11 +93,28 @@ step_tables_kernel(int* __restrict__ master, int master_rows, int master_width,
   }
 }
 
-BF_EXPORT int bf_step_tables(int* master, int master_rows, int master_width, const int* entries, int B,
-                             const int* new_pages, int n_new, int page_size, int num_pages, int* q_start,
-                             int* positions, int* seq, int* ctx_lens, int* slots, int T, int* tables,
-                             int width, int* decode_rows, int n_decode, int* items, int n_items, int* err,
-                             cudaStream_t stream) {
+struct StepTablesCall {
+  int* master;
+  int master_rows, master_width;
+  const int* entries;
+  int B;
+  const int* new_pages;
+  int n_new, page_size, num_pages;
+  int* q_start, *positions, *seq, *ctx_lens, *slots;
+  int T;
+  int* tables;
+  int width;
+  int* decode_rows;
+  int n_decode;
+  int* items;
+  int n_items;
+  int* err;
+  cudaStream_t stream;
+};
+BF_EXPORT int bf_step_tables(const StepTablesCall* call) {
+  const auto& [master, master_rows, master_width, entries, B, new_pages, n_new, page_size, num_pages,
+               q_start, positions, seq, ctx_lens, slots, T, tables, width, decode_rows, n_decode, items,
+               n_items, err, stream] = *call;
   if (B <= 0) return 0;
   // a block's share: up to about 512 places of a table, or tokens if portions are long
   const int per = width > T / B ? width : T / B;
