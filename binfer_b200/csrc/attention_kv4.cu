@@ -93,22 +93,6 @@ template <bool B>
 struct Bool {
   static constexpr bool value = B;
 };
-template <int WORDS>
-__device__ __forceinline__ void ka_lds(unsigned (&w)[WORDS], const unsigned char* p) {
-  if constexpr (WORDS >= 4) {
-#pragma unroll
-    for (int i = 0; i < WORDS / 4; ++i) {
-      const uint4 v = reinterpret_cast<const uint4*>(p)[i];
-      w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
-    }
-  } else if constexpr (WORDS == 2) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    w[0] = v.x, w[1] = v.y;
-  } else {
-    w[0] = *reinterpret_cast<const unsigned*>(p);
-  }
-}
-
 template <int D, int NT>
 __global__ void __launch_bounds__(32 * ka_warps(D, NT), 1)
 kv4_attention_kernel(const __grid_constant__ KaArgs a) {
@@ -395,10 +379,10 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
     auto scores = [&](float (&s)[NT][4], const unsigned char* s0) {
       const unsigned char* s1 = s0 + REC;
       unsigned w0[KW], w1[KW], p0[NG], p1[NG];
-      ka_lds<KW>(w0, s0 + r * (D / 2) + q4 * (D / 8));
-      ka_lds<KW>(w1, s1 + r * (D / 2) + q4 * (D / 8));
-      ka_lds<NG>(p0, s0 + kv4_key_params_at(D) + r * NG * 4);
-      ka_lds<NG>(p1, s1 + kv4_key_params_at(D) + r * NG * 4);
+      kv4_words<KW>(w0, s0 + r * (D / 2) + q4 * (D / 8));
+      kv4_words<KW>(w1, s1 + r * (D / 2) + q4 * (D / 8));
+      kv4_words<NG>(p0, s0 + kv4_key_params_at(D) + r * NG * 4);
+      kv4_words<NG>(p1, s1 + kv4_key_params_at(D) + r * NG * 4);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
 #pragma unroll
@@ -446,10 +430,10 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
     auto values = [&](float (&s)[NT][4], const unsigned char* s0, auto edge, unsigned hidden) {
       const unsigned char* s1 = s0 + REC;
       unsigned v0[KW], v1[KW], p0[NG], p1[NG];
-      ka_lds<KW>(v0, s0 + kv4_values_at(D) + r * (D / 2) + q4 * (D / 8));
-      ka_lds<KW>(v1, s1 + kv4_values_at(D) + r * (D / 2) + q4 * (D / 8));
-      ka_lds<NG>(p0, s0 + kv4_value_params_at(D) + r * NG * 4);
-      ka_lds<NG>(p1, s1 + kv4_value_params_at(D) + r * NG * 4);
+      kv4_words<KW>(v0, s0 + kv4_values_at(D) + r * (D / 2) + q4 * (D / 8));
+      kv4_words<KW>(v1, s1 + kv4_values_at(D) + r * (D / 2) + q4 * (D / 8));
+      kv4_words<NG>(p0, s0 + kv4_value_params_at(D) + r * NG * 4);
+      kv4_words<NG>(p1, s1 + kv4_value_params_at(D) + r * NG * 4);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -621,7 +605,7 @@ __global__ void __launch_bounds__(256)
 kv4_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml,
                  const int4* __restrict__ desc, __nv_bfloat16* __restrict__ out, long long out_stride, int group,
                  int chunk, int chunks, unsigned chunk_inverse, int pairs, int cols) {
-  constexpr int N = D / 32, DEPTH = D == 256 ? 2 : 4;
+  constexpr int N = D / 32, DEPTH = D == 256 ? 4 : 8;
   __shared__ float sh_o[PER > 1 ? 8 : 1][D], sh_m[8], sh_l[8];
   bf_pdl_trigger();
   bf_pdl_wait();

@@ -173,53 +173,44 @@ kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
   constexpr int NG = D / KV4_GROUP, REC = kv4_record(D);
   bf_pdl_trigger();
   bf_pdl_wait();
-  __shared__ int sh_item, sh_base, sh_of[4];
   const int page = blockIdx.x;                              // 0: the zero page; else page - 1 of the contexts
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint4 zero = make_uint4(0, 0, 0, 0);
-  if (warp == 0) {
-    int running = 0, item = -1, base = 0;
-    for (int i0 = 0; i0 < n_items; i0 += 32) {
-      const int i = i0 + lane;
-      int of[4] = {0, 0, 0, 0};
+  // the portion of this page, by every warp for itself
+  int item = -1, base = 0, b = 0, first = 0, n_rows = 0;
+  for (int i0 = 0, running = 0; i0 < n_items; i0 += 32) {
+    const int i = i0 + lane;
+    int of[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (i < n_items) of[k] = items[4 * i + k];
-      const int n = (max(of[2] + of[3], 0) + 63) / 64;
-      int incl = n;
+    for (int k = 0; k < 4; ++k)
+      if (i < n_items) of[k] = items[4 * i + k];
+    const int n = (max(of[2] + of[3], 0) + 63) / 64;
+    int incl = n;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += up;
-      }
-      const unsigned mine = __ballot_sync(0xffffffffu, page - 1 >= running + incl - n && page - 1 < running + incl);
-      if (mine) {
-        const int who = __ffs(mine) - 1;
-        item = i0 + who;
-        base = running + __shfl_sync(0xffffffffu, incl - n, who);
-        if (lane == who) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) sh_of[k] = of[k];
-        }
-      }
-      if (page == 0 && blockIdx.y == 0 && i < n_items) {
-        // a context that the pages or the table have no room for: none of its rows is attended
-        const bool fits = running + incl <= out_pages - 1 && n <= out_width;
-        if (!fits) atomicOr(err, BF_ERR_SPLITS);
-        if (items_out) {
-          items_out[4 * i] = i, items_out[4 * i + 1] = of[1];
-          items_out[4 * i + 2] = fits ? of[2] : 0, items_out[4 * i + 3] = of[3];
-        }
-      }
-      running += __shfl_sync(0xffffffffu, incl, 31);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
     }
-    if (lane == 0) {
-      sh_item = item;
-      sh_base = base;
+    const unsigned mine = __ballot_sync(0xffffffffu, page - 1 >= running + incl - n && page - 1 < running + incl);
+    if (mine) {
+      const int who = __ffs(mine) - 1;
+      item = i0 + who;
+      base = running + __shfl_sync(0xffffffffu, incl - n, who);
+      b = __shfl_sync(0xffffffffu, of[0], who);
+      n_rows = __shfl_sync(0xffffffffu, of[2], who);
+      first = __shfl_sync(0xffffffffu, of[3], who);
     }
+    if (page == 0 && blockIdx.y == 0 && warp == 0 && i < n_items) {
+      // a context that the pages or the table have no room for: none of its rows is attended
+      const bool fits = running + incl <= out_pages - 1 && n <= out_width;
+      if (!fits) atomicOr(err, BF_ERR_SPLITS);
+      if (items_out) {
+        items_out[4 * i] = i, items_out[4 * i + 1] = of[1];
+        items_out[4 * i + 2] = fits ? of[2] : 0, items_out[4 * i + 3] = of[3];
+      }
+    }
+    running += __shfl_sync(0xffffffffu, incl, 31);
   }
-  __syncthreads();
-  const int item = sh_item;
   if (page == 0 && blockIdx.y == 0) {
     for (int i = 0; i < n_items; ++i)                       // (portions without a page of their own)
       if (items[4 * i + 2] + items[4 * i + 3] <= 0)
@@ -235,16 +226,16 @@ kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
     }
     return;
   }
-  const int b = sh_of[0], first = sh_of[3], last = first + sh_of[2] - 1;
-  const int place = page - 1 - sh_base, n_places = last / 64 + 1;
+  const int last = first + n_rows - 1;
+  const int place = page - 1 - base, n_places = last / 64 + 1;
   if (HALF && place == 0 && blockIdx.y == 0)
     for (int h = tid; h < nkv; h += 256) beyond[item * nkv + h] = 0;
   if (blockIdx.y == 0) {                                    // this block's part of the portion's row
     const int w1 = place + 1 < n_places ? (int)((long long)out_width * (place + 1) / n_places) : out_width;
     for (int w = (int)((long long)out_width * place / n_places) + tid; w < w1; w += 256)
       tables_out[(size_t)item * out_width + w] =
-          w < n_places && sh_base + w + 1 < out_pages && kv4_seen(w * 64, w * 64 + 63, first, last, window, keep)
-              ? sh_base + w + 1 : 0;
+          w < n_places && base + w + 1 < out_pages && kv4_seen(w * 64, w * 64 + 63, first, last, window, keep)
+              ? base + w + 1 : 0;
   }
   const int j64 = place * 64;
   if (!kv4_seen(j64, j64 + 63, first, last, window, keep)) return;
@@ -280,36 +271,35 @@ kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
   const bool on = have && kv4_seen(j8 + r, j8 + r, first, last, window, keep);
   const bool v_on[2] = {have && kv4_seen(j8 + 2 * q, j8 + 2 * q, first, last, window, keep),
                         have && kv4_seen(j8 + 2 * q + 1, j8 + 2 * q + 1, first, last, window, keep)};
+  constexpr int KW = D / 32;                                // words of a lane's keys, and of its values
   for (int h = blockIdx.y; h < nkv; h += gridDim.y) {
-    const unsigned char* rec =
-        cache + (((size_t)pid * nkv + h) * (page_size / 8) + j8 % page_size / 8) * REC;
+    const unsigned char* rec = cache + (((size_t)pid * nkv + h) * (page_size / 8) + j8 % page_size / 8) * REC;
     __nv_bfloat16* ko = k_out + (((size_t)page * nkv + h) * 64 + warp * 8) * D;
     __nv_bfloat16* vo = v_out + (((size_t)page * nkv + h) * 64 + warp * 8) * D;
-    uint2 kw[NG];
-    unsigned vw[2][NG], kp[NG], vp[2][NG];
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {                          // keys: lane (r, q) has part q of token r
-      kw[g] = *reinterpret_cast<const uint2*>(rec + r * (D / 2) + q * (D / 8) + g * 8);
-      kp[g] = *reinterpret_cast<const unsigned*>(rec + kv4_key_params_at(D) + (r * NG + g) * 4);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {                         // values: part r of tokens 2 q and 2 q + 1
-        vw[e][g] = *reinterpret_cast<const unsigned*>(rec + 4 * D + r * (D / 2) + (2 * q + e) * (D / 16) + g * 4);
-        vp[e][g] = *reinterpret_cast<const unsigned*>(rec + kv4_value_params_at(D) + ((2 * q + e) * NG + g) * 4);
-      }
-    }
+    // keys: lane (r, q) has part q of token r; values: part r of tokens 2 q and 2 q + 1
+    unsigned kw[KW], vw[KW], kp[NG], vp[2 * NG];
+    kv4_words<KW>(kw, rec + r * (D / 2) + q * (D / 8));
+    kv4_words<NG>(kp, rec + kv4_key_params_at(D) + r * NG * 4);
+    kv4_words<KW>(vw, rec + kv4_values_at(D) + r * (D / 2) + q * (D / 8));
+    kv4_words<2 * NG>(vp, rec + kv4_value_params_at(D) + q * NG * 8);
     bool other = false;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       const float s = kv4_scale(kp[g]), m = kv4_low(kp[g]);
-      uint4* dst = reinterpret_cast<uint4*>(ko + r * D + g * 64 + q * 16);
-      dst[0] = on ? eight(kw[g].x, s, m, KvBool<HALF>()) : zero;
-      dst[1] = on ? eight(kw[g].y, s, m, KvBool<HALF>()) : zero;
+      // a row's four lanes change eights, so that each store fills its 32-byte sectors
+      uint4* dst = reinterpret_cast<uint4*>(ko + r * D + g * 64 + q * 8);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int from = (lane & ~3) | half * 2 | q >> 1;
+        const unsigned w0 = __shfl_sync(0xffffffffu, kw[2 * g], from), w1 = __shfl_sync(0xffffffffu, kw[2 * g + 1], from);
+        dst[half * 4] = on ? eight(q & 1 ? w1 : w0, s, m, KvBool<HALF>()) : zero;
+      }
       if (HALF) other |= on && (fabsf(m) > 65000.f || fabsf(fmaf(15.f, s, m)) > 65000.f);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float vs = kv4_scale(vp[e][g]);
+        const float vs = kv4_scale(vp[e * NG + g]);
         *reinterpret_cast<uint4*>(vo + (2 * q + e) * D + g * 64 + r * 8) =
-            v_on[e] ? eight(vw[e][g], vs, kv4_low(vp[e][g]), KvBool<false>()) : zero;
+            v_on[e] ? eight(vw[e * NG + g], vs, kv4_low(vp[e * NG + g]), KvBool<false>()) : zero;
         if (HALF) other |= v_on[e] && vs != vs;
       }
     }

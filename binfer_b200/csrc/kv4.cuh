@@ -36,6 +36,23 @@ __host__ __device__ constexpr int kv4_value_byte(int d, int tok, int i) {
 __device__ __forceinline__ float kv4_scale(unsigned pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float kv4_low(unsigned pair) { return __uint_as_float(pair & 0xffff0000u); }
 
+// WORDS words at p (aligned as their number allows) by the widest reads.
+template <int WORDS>
+__device__ __forceinline__ void kv4_words(unsigned (&w)[WORDS], const unsigned char* p) {
+  if constexpr (WORDS >= 4) {
+#pragma unroll
+    for (int i = 0; i < WORDS / 4; ++i) {
+      const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+      w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+    }
+  } else if constexpr (WORDS == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+    w[0] = *reinterpret_cast<const unsigned*>(p);
+  }
+}
+
 // Whether some row at positions first .. last sees a key of [j0, j1] (window 0: no window).
 __device__ __forceinline__ bool kv4_seen(int j0, int j1, int first, int last, int window, int keep) {
   if (j0 > last) return false;
