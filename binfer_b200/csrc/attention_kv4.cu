@@ -50,7 +50,7 @@ struct KaArgs {
   __nv_bfloat16* out;
   long long out_stride;
   int nh, nkv, group, chunk, chunks, tokens;               // query heads per kv head; in a tile; chunks of them
-  int page_size, num_pages, window, keep;
+  int page_size, page_shift, num_pages, window, keep;
   float scale;
   unsigned chunk_inverse;                                  // n / chunk = n chunk_inverse >> 8 for n < 16
   int max_pieces;
@@ -72,13 +72,16 @@ __device__ __forceinline__ KaSpan ka_span(const KaTile& t, int window, int keep)
   KaSpan s = {0, 0, 0};
   if (t.ntok <= 0) return s;
   if (window > 0) {
-    s.from = max(0, t.pos0 - window + 1) / KA_UNIT;
-    s.kept = min((keep + KA_UNIT - 1) / KA_UNIT, s.from);
+    s.from = max(0, t.pos0 - window + 1) >> 4;
+    s.kept = min((keep + KA_UNIT - 1) >> 4, s.from);
   }
-  s.units = (t.pos0 + t.ntok - 1) / KA_UNIT - s.from + 1 + s.kept;
+  s.units = ((t.pos0 + t.ntok - 1) >> 4) - s.from + 1 + s.kept;
+  static_assert(KA_UNIT == 16, "the shifts above");
   return s;
 }
 
+// a / b for 0 <= a < 2^20, 0 < b: the half keeps the product off the whole numbers by more than it is wrong
+__device__ __forceinline__ int ka_div(int a, int b) { return (int)(((float)a + 0.5f) * __frcp_rn((float)b)); }
 __device__ __forceinline__ float ka_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -218,25 +221,23 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   unsigned char* my_ring = smem + (size_t)warp * KA_STAGES * UNIT_BYTES;
 
   while (x < x_end) {
-    int e = 0;                                              // the tile of x: the last that begins at or before it
-    {
-      int hi = a.n_tiles - 1;
-      while (e < hi) {
-        const int mid = (e + hi + 1) >> 1;
-        if (start[mid] <= x) e = mid; else hi = mid - 1;
-      }
-    }
+    // the tile of x: the last that begins at or before it, among every sixteenth and then among sixteen
+    int e = lane * 16;
+    e = (31 - __clz(__ballot_sync(0xffffffffu, e < a.n_tiles && start[e] <= x))) * 16;
+    const int e1 = e + (lane & 15);
+    e += 31 - __clz(__ballot_sync(0xffffffffu, lane < 16 && e1 < a.n_tiles && start[e1] <= x));
+    static_assert(KA_MAX_TILES <= 512, "two steps");
     const KaTile t = tiles[e];
     const KaSpan span = ka_span(t, a.window, a.keep);
     const int y = x - start[e];
     int pair, u0, mine, n_pieces;
     if (aligned) {
-      const int n = start[e + 1] - start[e], fewer = n / pairs, more = n - fewer * pairs;
+      const int n = start[e + 1] - start[e], fewer = ka_div(n, pairs), more = n - fewer * pairs;
       const int edge = more * (fewer + 1);                  // the first `more` heads have a piece more
       n_pieces = fewer + (y < edge ? 1 : 0);
       const int z = y < edge ? y : y - edge;
-      pair = z / n_pieces;
-      const int piece = z - pair * n_pieces, units = span.units / n_pieces, over = span.units - units * n_pieces;
+      pair = ka_div(z, n_pieces);
+      const int piece = z - pair * n_pieces, units = ka_div(span.units, n_pieces), over = span.units - units * n_pieces;
       if (y >= edge) pair += more;
       u0 = piece * units + min(piece, over);
       mine = units + (piece < over ? 1 : 0);
@@ -252,7 +253,7 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
       }
       x += mine;
     }
-    const int h = pair / a.chunks, head0 = h * a.group + (pair - h * a.chunks) * a.chunk;
+    const int h = a.chunks == 1 ? pair : pair / a.chunks, head0 = h * a.group + (pair - h * a.chunks) * a.chunk;
     const int heads = min(a.chunk, (h + 1) * a.group - head0);
     const int last = t.pos0 + t.ntok - 1;
     const int* table = a.block_tables + (size_t)t.b * a.table_stride;
@@ -277,8 +278,8 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
     int rec0 = 0, rec1 = 0;                                 // of unit (32 n + lane): its two records
     auto record = [&](int j, int n) {                       // of keys j .. j + n - 1, n a page's at most
       if (!kv4_seen(j, j + n - 1, t.pos0, last, a.window, a.keep)) return 0;
-      const int at = j / a.page_size, page = table[at];
-      if (page >= 0 && page < a.num_pages) return (page * a.nkv + h) * eighths + (j - at * a.page_size) / 8;
+      const int at = j >> a.page_shift, page = table[at];
+      if (page >= 0 && page < a.num_pages) return (page * a.nkv + h) * eighths + ((j - (at << a.page_shift)) >> 3);
       atomicOr(a.err, BF_ERR_PAGE);
       return 0;
     };
@@ -760,7 +761,9 @@ BF_EXPORT int bf_kv4_attention(const Kv4AttentionCall* call) {
                table_stride, table_rows, table_width, out, out_stride, nh, nkv, d, page_size, num_pages,
                window, keep, scale, scratch, sms, err, stream] = *call;
   if (n <= 0 || max_rows <= 0) return 0;
-  if ((long long)num_pages * nkv * (page_size / 8) > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+  if ((long long)num_pages * nkv * (page_size / 8) > 0x7fffffffLL || page_size < 8 || (page_size & (page_size - 1)) ||
+      (long long)table_width * page_size > 1 << 24)        // (a tile's units stay below 2^20)
+    return (int)cudaErrorInvalidValue;
   const KaShape s = ka_shape(nh / nkv, d, max_rows);
   KaArgs a = {};
   a.q = (const __nv_bfloat16*)q, a.q_stride = q_stride, a.cache = (const unsigned char*)cache;
@@ -770,7 +773,9 @@ BF_EXPORT int bf_kv4_attention(const Kv4AttentionCall* call) {
   a.table_stride = table_stride, a.table_rows = table_rows, a.table_width = table_width;
   a.out = (__nv_bfloat16*)out, a.out_stride = out_stride;
   a.nh = nh, a.nkv = nkv, a.group = nh / nkv, a.chunk = s.chunk, a.chunks = s.chunks, a.tokens = s.tokens;
-  a.page_size = page_size, a.num_pages = num_pages, a.window = window, a.keep = keep, a.scale = scale;
+  a.page_size = page_size, a.page_shift = 3;
+  while (1 << a.page_shift < page_size) ++a.page_shift;
+  a.num_pages = num_pages, a.window = window, a.keep = keep, a.scale = scale;
   a.chunk_inverse = (256 + s.chunk - 1) / s.chunk;
   const long long slots = ka_slots(s, d, sms);
   a.part_o = (float*)scratch;

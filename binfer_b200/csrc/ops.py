@@ -1983,6 +1983,8 @@ def _kv4_attention_check(what, q, cache, block_tables, out, nh, nkv, d, window, 
     table = _want_int_table(block_tables, what, "block_tables")
     _want(err, torch.int32, "err")
     pages, c_nkv, ps, c_d = _kv4_check(what, cache, q, block_tables, out, err, *others)
+    if table[1] * ps > 1 << 24:
+        raise KernelError(f"{what}: block tables of more than 2^24 tokens")
     if c_nkv != nkv or c_d != d or nh < 1 or nh % nkv:
         raise KernelError(f"{what}: the cache has {c_nkv} heads of {c_d}, the call names {nkv} of {d} for "
                           f"{nh} query heads")

@@ -119,7 +119,7 @@ def test_prefill_variants(ops, change, monkeypatch):
 @pytest.mark.parametrize("what,change", [
     ("window", dict(window=0)), ("keep_first", dict(keep_first=-1)), ("heads", dict(nkv=1)), ("heads", dict(d=128)),
     ("heads", dict(nh=3)), ("q", dict(q=torch.zeros((3, 256)))), ("q", dict(q=torch.zeros((3, 512), dtype=BF16)[:, 1:257])),
-    ("out", dict(out=torch.zeros((3, 255), dtype=BF16))), ("out", dict(out=torch.zeros((2, 256), dtype=BF16)))])
+    ("tokens", dict(block_tables=_i(1, (1 << 20) + 1))), ("out", dict(out=torch.zeros((3, 255), dtype=BF16))), ("out", dict(out=torch.zeros((2, 256), dtype=BF16)))])
 def test_attention_sizes(ops, what, change, monkeypatch):
     monkeypatch.setattr(ops, "_same_device", lambda *a: None)
     args = dict(_attention_args(ops), **change)
