@@ -35,6 +35,7 @@
 #define KA_UNIT 16                         // keys
 #define KA_MIN_UNITS 2                     // a stretch's length at least
 #define KA_LONG 24                         // units of a stretch from which heads are crossed
+#define KA_BEGIN 6                         // units that a warp could compute while it begins a head
 
 // Warps of a CTA, one CTA an SM: sixteen where 128 registers hold a tile.
 __host__ __device__ constexpr int ka_warps(int d, int nt) { return d <= 128 && nt == 1 ? 16 : 8; }
@@ -190,7 +191,7 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
     int before = 0;
 #pragma unroll 1
     for (int e0 = 0; e0 < a.n_tiles; e0 += 32) {
-      const int e = e0 + lane, u = e < a.n_tiles ? units_of[e] : 0, n = aligned ? pieces_of(u) : u * pairs;
+      const int e = e0 + lane, u = e < a.n_tiles ? units_of[e] : 0, n = aligned ? pieces_of(u) : u ? (u + KA_BEGIN) * pairs : 0;
       int incl = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -206,9 +207,10 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   const int me = warp * gridDim.x + blockIdx.x;             // (few stretches lie on as many SMs)
   int each = 1, longer = 0, x = me, x_end = me + 1;         // pieces: one
   if (!aligned) {
-    const int least = max(KA_MIN_UNITS, (longest + a.max_pieces - 1) / a.max_pieces);
-    const int parts = min(max(total / least, 1), warps);
-    each = total / parts, longer = total - each * parts;    // the first `longer` have a unit more
+    // every head begins with KA_BEGIN places for what that takes
+    const int places = start[a.n_tiles], least = max(KA_LONG, (longest + a.max_pieces - 1) / a.max_pieces);
+    const int parts = min(max(places / least, 1), warps);
+    each = places / parts, longer = places - each * parts;  // the first `longer` have one more
     x = me * each + min(me, longer);
     x_end = me < parts ? x + each + (me < longer ? 1 : 0) : x;
   } else if (me >= start[a.n_tiles]) {
@@ -243,15 +245,18 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
       mine = units + (piece < over ? 1 : 0);
       x = x_end;
     } else {
-      pair = y / span.units;
-      u0 = y - pair * span.units;
-      mine = min(span.units - u0, x_end - x);
+      const int v = span.units + KA_BEGIN;
+      pair = y / v;
+      const int place = y - pair * v, to = min(v, place + x_end - x);
+      u0 = max(place - KA_BEGIN, 0);
+      mine = to - KA_BEGIN - u0;
       n_pieces = 1;
       if (mine < span.units) {                              // (asked for where u0 is 0: how many warps share the head)
-        const int at = x - u0 + span.units - 1, edge = longer * (each + 1);
+        const int at = x - place + v - 1, edge = longer * (each + 1);
         n_pieces = (at < edge ? at / (each + 1) : longer + (at - edge) / each) - me + 1;
       }
-      x += mine;
+      x += to - place;
+      if (mine <= 0) continue;
     }
     const int h = a.chunks == 1 ? pair : pair / a.chunks, head0 = h * a.group + (pair - h * a.chunks) * a.chunk;
     const int heads = min(a.chunk, (h + 1) * a.group - head0);
@@ -690,7 +695,7 @@ static int ka_launch(KaArgs a, int total_tiles, int sms, cudaStream_t stream) {
   }
   const int pairs = a.nkv * a.chunks;
   // the units of a launch are counted in 32 bits
-  const long long units = ((long long)a.table_width * a.page_size / KA_UNIT + 2) * pairs;
+  const long long units = ((long long)a.table_width * a.page_size / KA_UNIT + 2 + KA_BEGIN) * pairs;
   if (units > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
   const int most = 0x7fffffffLL / units < KA_MAX_TILES ? (int)(0x7fffffffLL / units) : KA_MAX_TILES;
   for (int first = 0; first < total_tiles; first += most) {
