@@ -208,7 +208,7 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   int each = 1, longer = 0, x = me, x_end = me + 1;         // pieces: one
   if (!aligned) {
     // every head begins with KA_BEGIN places for what that takes
-    const int places = start[a.n_tiles], least = max(KA_LONG, (longest + a.max_pieces - 1) / a.max_pieces);
+    const int places = start[a.n_tiles], least = max(KA_LONG / 2, (longest + a.max_pieces - 1) / a.max_pieces);
     const int parts = min(max(places / least, 1), warps);
     each = places / parts, longer = places - each * parts;  // the first `longer` have one more
     x = me * each + min(me, longer);

@@ -56,7 +56,8 @@
 //
 // Keys may be fp16 (HALF: those of a cache held in 4 bits, whose numbers bfloat16 would round): the softmax
 // warps then make their Q tile fp16 where it lies before its first product, and a request and kv head
-// with a query beyond fp16's range is noted in `beyond` for the caller to compute otherwise.
+// with a query beyond fp16's range is noted in `beyond` for the caller to compute otherwise.  Heads of 64 go
+// this way too: one block of 64 columns where the others have two, and half of O's tensor memory.
 //
 // Every mbarrier wait is bounded.  A barrier whose waiter could fall two phases behind exists
 // once per parity of the tile number, so that its one-bit phase cannot alias: "P V of tile n
@@ -104,7 +105,7 @@ __device__ __forceinline__ bool group_all(int id, bool ok) {
   return r != 0;
 }
 
-template <int MODE, bool HALF = false>
+template <int MODE, bool HALF = false, int D = A2_D>
 __global__ void __launch_bounds__(A2_THREADS, 1)
 prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
                                const __grid_constant__ CUtensorMap map_k,
@@ -120,7 +121,6 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
                                long long out_stride, float out_scale, BfDiffArgs dd,
                                const float* __restrict__ sinks, int keep, int* __restrict__ beyond) {
   constexpr bool DIFF = MODE == A2_DIFF, LATENT = MODE == A2_LATENT, KEEP = MODE == A2_KEEP;
-  constexpr int D = A2_D;
   constexpr int HALVES = D / 64;                         // blocks of 64 columns of a V tile
   constexpr int KBLOCKS = LATENT ? HALVES + 1 : HALVES;  // ... of a Q or K tile
   constexpr int STAGES = LATENT ? 3 : A2_STAGES;
@@ -806,38 +806,40 @@ static int launch_umma2(
   if (splits < 1 || (splits > 1 && (!part_o || !part_ml))) return (int)cudaErrorInvalidValue;
   if (window <= 0 || keep < 0) keep = 0;
   if (keep > 0 && splits > 1) return (int)cudaErrorInvalidValue;
-  if (d != A2_D || nkv <= 0 || nh % nkv || page_size < 8 || page_size > A2_BN ||
+  if ((d != A2_D && !(d == 64 && beyond && splits == 1)) || nkv <= 0 || nh % nkv || page_size < 8 || page_size > A2_BN ||
       A2_BN % page_size || ((uintptr_t)q & 15) || ((uintptr_t)k_cache & 15) ||
       ((uintptr_t)v_cache & 15) || ((uintptr_t)out & 15) || !(scale > 0.f) || softcap < 0.f ||
-      out_stride < (long long)nh * A2_D || (out_stride & 7))
+      out_stride < (long long)nh * d || (out_stride & 7))
     return (int)cudaErrorInvalidValue;
   const float log2e = 1.4426950408889634f;
   const float cap_pre = softcap > 0.f ? 2.f * log2e * scale / softcap : 0.f;
   const float cap_post = softcap > 0.f ? softcap / scale : 0.f;
   CUtensorMap mq, mk, mv;
-  int e = bf_make_tensor_map_bf16_2d(&mq, q, total_rows, (long long)nh * A2_D,
-                                     (long long)nh * A2_D, A2_BM, 64);
+  int e = bf_make_tensor_map_bf16_2d(&mq, q, total_rows, (long long)nh * d,
+                                     (long long)nh * d, A2_BM, 64);
   if (e) return e;
   const long long cache_rows = (long long)num_pages * nkv * page_size;
-  e = bf_make_tensor_map_bf16_2d(&mk, k_cache, cache_rows, A2_D, A2_D, page_size, 64);
+  e = bf_make_tensor_map_bf16_2d(&mk, k_cache, cache_rows, d, d, page_size, 64);
   if (e) return e;
-  e = bf_make_tensor_map_bf16_2d(&mv, v_cache, cache_rows, A2_D, A2_D, page_size, 64);
+  e = bf_make_tensor_map_bf16_2d(&mv, v_cache, cache_rows, d, d, page_size, 64);
   if (e) return e;
   CUtensorMap mkr, mvr;      // a whole tile of pages that follow one another
-  e = bf_make_tensor_map_pages_bf16(&mkr, k_cache, num_pages, nkv, page_size, A2_D,
+  e = bf_make_tensor_map_pages_bf16(&mkr, k_cache, num_pages, nkv, page_size, d,
                                     A2_BN / page_size);
   if (e) return e;
-  e = bf_make_tensor_map_pages_bf16(&mvr, v_cache, num_pages, nkv, page_size, A2_D,
+  e = bf_make_tensor_map_pages_bf16(&mvr, v_cache, num_pages, nkv, page_size, d,
                                     A2_BN / page_size);
   if (e) return e;
   // two Q tiles, the stages of K and V, the row sums, barriers
   const size_t smem = 1024 + (size_t)2 * 32768 + (size_t)2 * A2_STAGES * 16384 + 2048 + 256;
-  auto kern = beyond ? (keep > 0 ? prefill_attention_umma2_kernel<A2_KEEP, true>
+  auto kern = d == 64 ? (keep > 0 ? prefill_attention_umma2_kernel<A2_KEEP, true, 64>
+                                  : prefill_attention_umma2_kernel<A2_PLAIN, true, 64>)
+              : beyond ? (keep > 0 ? prefill_attention_umma2_kernel<A2_KEEP, true>
                                  : prefill_attention_umma2_kernel<A2_PLAIN, true>)
                      : (keep > 0 ? prefill_attention_umma2_kernel<A2_KEEP>
                                  : prefill_attention_umma2_kernel<A2_PLAIN>);
-  static bool configured_on[BF_MAX_DEVICES][4];
-  bool& configured = configured_on[bf_current_device()][(keep > 0 ? 1 : 0) + (beyond ? 2 : 0)];
+  static bool configured_on[BF_MAX_DEVICES][6];
+  bool& configured = configured_on[bf_current_device()][(keep > 0 ? 1 : 0) + (d == 64 ? 4 : beyond ? 2 : 0)];
   if (!configured) {
     cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                           (int)smem);
@@ -871,7 +873,7 @@ BF_EXPORT int bf_prefill_attention_umma2_capped(
                       out_stride, out_scale, sinks, keep, nullptr, stream);
 }
 
-// bfloat16 queries and values over fp16 keys.
+// bfloat16 queries and values over fp16 keys; heads of 128, or of 64 with one split.
 struct PrefillAttentionUmma2HalfCall {
   const void* q, *k_cache, *v_cache;
   const int* items;

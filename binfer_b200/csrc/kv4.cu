@@ -310,7 +310,7 @@ kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
   }
 }
 
-// special (8 bytes a page and head) and beyond (n_items x nkv), both or neither: keys in fp16, heads of 128.
+// special (8 bytes a page and head) and beyond (n_items x nkv), both or neither: keys in fp16, heads of 64 or 128.
 struct Kv4LoadCall {
   const void* cache;
   const int* block_tables;
@@ -332,7 +332,7 @@ BF_EXPORT int bf_kv4_load(const Kv4LoadCall* call) {
                tables_out, out_width, items_out, special, beyond, out_pages, nkv, d, page_size, num_pages,
                window, keep, sms, err, stream] = *call;
   if (n_items <= 0 || out_pages <= 1) return 0;
-  if ((special != nullptr) != (beyond != nullptr) || (special && d != 128)) return (int)cudaErrorInvalidValue;
+  if ((special != nullptr) != (beyond != nullptr) || (special && d != 128 && d != 64)) return (int)cudaErrorInvalidValue;
   // heads apart where pages alone would leave SMs without blocks
   int parts = 1;
   while (parts < nkv && (long long)out_pages * parts < 4LL * sms) parts *= 2;
@@ -343,7 +343,7 @@ BF_EXPORT int bf_kv4_load(const Kv4LoadCall* call) {
                          (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, tables_out, out_width, items_out,
                          (unsigned char*)special, beyond, out_pages, nkv, page_size, num_pages, window, keep, err);
   };
-  if (special) return run(kv4_load_kernel<128, true>);
+  if (special) return d == 64 ? run(kv4_load_kernel<64, true>) : run(kv4_load_kernel<128, true>);
   if (d == 64) return run(kv4_load_kernel<64, false>);
   if (d == 128) return run(kv4_load_kernel<128, false>);
   if (d == 256) return run(kv4_load_kernel<256, false>);
@@ -354,6 +354,7 @@ BF_EXPORT int bf_kv4_load(const Kv4LoadCall* call) {
 // with a record that is noted in `special` or a query in `beyond`, by multiply-adds straight from the
 // cache, a warp a (row, query head).  As a rule nothing is noted and a block only reads a few words; a block
 // that finds something takes its 32 rows.
+template <int D>
 __global__ void __launch_bounds__(256)
 kv4_rest_kernel(const unsigned long long* __restrict__ special, const int* __restrict__ beyond,
                 const int* __restrict__ items, const int* __restrict__ moved, const int* __restrict__ tables,
@@ -361,7 +362,7 @@ kv4_rest_kernel(const unsigned long long* __restrict__ special, const int* __res
                 int table_stride, const __nv_bfloat16* __restrict__ q, long long q_stride,
                 __nv_bfloat16* __restrict__ out, long long out_stride, int nkv, int group, int page_size,
                 int num_pages, int window, int keep, float scale) {
-  constexpr int D = 128, N = D / 32, NG = 2, REC = kv4_record(D);
+  constexpr int N = D / 32, NG = D / KV4_GROUP, REC = kv4_record(D);
   bf_pdl_trigger();
   bf_pdl_wait();
   const int h = blockIdx.y, item = blockIdx.z;
@@ -425,17 +426,22 @@ struct Kv4RestCall {
   long long q_stride;
   void* out;
   long long out_stride;
-  int nh, nkv, page_size, num_pages, window, keep;
+  int nh, nkv, d, page_size, num_pages, window, keep;
   float scale;
   cudaStream_t stream;
 };
 BF_EXPORT int bf_kv4_rest(const Kv4RestCall* call) {
   const auto& [special, beyond, items, moved, n_items, max_rows, tables, width, cache, block_tables,
-               table_stride, q, q_stride, out, out_stride, nh, nkv, page_size, num_pages, window, keep,
+               table_stride, q, q_stride, out, out_stride, nh, nkv, d, page_size, num_pages, window, keep,
                scale, stream] = *call;
   if (n_items <= 0 || max_rows <= 0) return 0;
-  return bf_launch_pdl(kv4_rest_kernel, dim3((max_rows + 31) / 32, nkv, n_items), dim3(256), 0, stream,
-                       (const unsigned long long*)special, beyond, items, moved, tables, width,
-                       (const unsigned char*)cache, block_tables, table_stride, (const __nv_bfloat16*)q, q_stride,
-                       (__nv_bfloat16*)out, out_stride, nkv, nh / nkv, page_size, num_pages, window, keep, scale);
+  auto run = [&](auto kern) {
+    return bf_launch_pdl(kern, dim3((max_rows + 31) / 32, nkv, n_items), dim3(256), 0, stream,
+                         (const unsigned long long*)special, beyond, items, moved, tables, width,
+                         (const unsigned char*)cache, block_tables, table_stride, (const __nv_bfloat16*)q, q_stride,
+                         (__nv_bfloat16*)out, out_stride, nkv, nh / nkv, page_size, num_pages, window, keep, scale);
+  };
+  if (d == 64) return run(kv4_rest_kernel<64>);
+  if (d == 128) return run(kv4_rest_kernel<128>);
+  return (int)cudaErrorInvalidValue;
 }

@@ -1907,7 +1907,7 @@ class _Packed:
 
 _kv4_store_call = _Packed("bf_kv4_store", "PqPqPPiiiiqPP")
 _kv4_load_call = _Packed("bf_kv4_load", "PPiiiPiPPPiPPPiiiiiiiiPP")
-_kv4_rest_call = _Packed("bf_kv4_rest", "PPPPiiPiPPiPqPqiiiiiifP")
+_kv4_rest_call = _Packed("bf_kv4_rest", "PPPPiiPiPPiPqPqiiiiiiifP")
 _kv4_attention_call = _Packed("bf_kv4_attention", "PqPPPPPiiiPiiiPqiiiiiiifPiPP")
 _step_tables_call = _Packed("bf_step_tables", "PiiPiPiiiPPPPPiPiPiPiPP")
 _prefill_attention_umma2_half_call = _Packed("bf_prefill_attention_umma2_half", "PPPPiiiPiPiiiiiifiPPPqiPP")
@@ -2043,7 +2043,7 @@ def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Ten
     ``keep_first``: with a window, the request's first that many tokens stay visible behind it.
 
     ``variant``: ``stretches`` (the kernel of single tokens, a few rows at a time; reads the cache as it
-    is), ``load`` (heads of 128, a positive scale, q contiguous: the contexts are loaded as ``kv4_load``
+    is), ``load`` (heads of 64 or 128, a positive scale, q contiguous: the contexts are loaded as ``kv4_load``
     does, keys in fp16, into scratch of 4 d bytes a token and kv head, and attended on tcgen05), or ``auto``."""
     _want(items, torch.int32, "items")
     table, strides, pages, ps, w, keep = _kv4_attention_check(
@@ -2054,13 +2054,13 @@ def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Ten
         raise KernelError(f"kv4_prefill_attention: unknown variant {variant!r}")
     if n_items == 0 or max_rows == 0:
         return
-    load_ok = d == 128 and q.is_contiguous() and ctx_rows > 0 and scale > 0
+    load_ok = d in (64, 128) and q.is_contiguous() and ctx_rows > 0 and scale > 0
     if variant == "load" and not load_ok:
-        raise KernelError("kv4_prefill_attention: the load variant takes heads of 128, a contiguous q and a "
+        raise KernelError("kv4_prefill_attention: the load variant takes heads of 64 or 128, a contiguous q and a "
                           "positive scale")
     if variant == "load" or (variant == "auto" and load_ok
-                             and _kv4_load_pays(n_items, max_rows, max_ctx, w, keep, nh, nkv)):
-        _kv4_loaded_attention(q, cache, items, n_items, max_rows, block_tables, table, strides, out, nh, nkv, ps,
+                             and _kv4_load_pays(n_items, max_rows, max_ctx, w, keep, nh, nkv, d)):
+        _kv4_loaded_attention(q, cache, items, n_items, max_rows, block_tables, table, strides, out, nh, nkv, d, ps,
                               pages, w, keep, scale, err, ctx_rows, max_ctx)
         return
     _kv4_attention(q, cache, 0, 0, 0, items.data_ptr(), n_items, max_rows, block_tables, table, strides, out, nh,
@@ -2070,30 +2070,37 @@ def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Ten
 _kv4_scratch: dict = {}     # bytes of scratch by a call's sizes
 
 
-def _kv4_load_pays(n: int, max_rows: int, max_ctx: int, window: int, keep: int, nh: int, nkv: int) -> bool:
-    """Whether a call's portions of heads of 128 are faster loaded and attended on tcgen05 than in
-    stretches of units: microseconds by sizes, fitted to both measured on a B200.  One portion of 32 heads
-    (8 kv heads), stretches against load: 64 rows behind 1,000 keys 23 / 40 us, behind 16,000 101 / 91; 128
-    rows 29 / 44 and 177 / 93; four portions of 64 rows behind 4,000 101 / 87."""
+def _kv4_load_pays(n: int, max_rows: int, max_ctx: int, window: int, keep: int, nh: int, nkv: int,
+                   d: int) -> bool:
+    """Whether a call's portions of heads of 64 or 128 are faster loaded and attended on tcgen05 than in
+    stretches of units: microseconds by sizes, fitted to both measured on a B200 (stretches / load).  32
+    heads of 128 (8 kv heads), one portion: 64 rows behind 1,000 keys 23 / 40, behind 16,000 101 / 91; 128
+    rows 29 / 44 and 177 / 93; four of 64 rows behind 4,000 101 / 87.  16 heads of 64 (4): 256 rows behind
+    4,000 41 / 72, 1,024 rows 141 / 83; behind 16,000 121 / 228 and 463 / 241."""
     seen = min(max_ctx, window + keep + max_rows) if window else max_ctx
     group = nh // nkv
     tiles = n * -(-max_rows // max(1, 16 // group)) * -(-group // 16)
-    stretches = 11.0 + 0.64e-3 * tiles * nkv * (seen - max_rows / 2) / 16        # (0.64 ns a tile's unit)
-    # keys one tile after the other until they are shared out, then the products
-    load = 12.0 + 0.025 * min(seen, 1000) + 0.13e-3 * nh * n * seen * -(-max_rows // 256)
+    # 0.64 ns (heads of 64: 0.44) a unit of a tile and kv head, six units to begin one; 512 tiles a launch
+    stretches = 11.0 * -(-tiles // 512) + (0.64e-3 if d == 128 else 0.44e-3) * tiles * nkv * (
+        (seen - max_rows / 2) / 16 + 6)
+    blocks = nh * n * -(-max_rows // 256)
+    if d == 128:          # keys one tile after the other until they are shared out, then the products
+        load = 12.0 + 0.025 * min(seen, 1000) + 0.13e-3 * seen * blocks
+    else:                 # one tile after the other
+        load = 12.0 + 0.0143 * seen * max(1.0, blocks / 148)
     return load < stretches
 
 
-def _kv4_loaded_attention(q, cache, items, n_items, max_rows, block_tables, table, strides, out, nh, nkv, ps, pages, w,
-                          keep, scale, err, ctx_rows, max_ctx) -> None:
+def _kv4_loaded_attention(q, cache, items, n_items, max_rows, block_tables, table, strides, out, nh, nkv, d, ps, pages,
+                          w, keep, scale, err, ctx_rows, max_ctx) -> None:
     global _launches
-    d, (T, q_stride, out_stride), (table_rows, table_width, table_stride) = 128, strides, table
+    (T, q_stride, out_stride), (table_rows, table_width, table_stride) = strides, table
     n = 1 + ctx_rows // KV4_LOAD_PAGE
     places = max(1, -(-max_ctx // KV4_LOAD_PAGE))
     # few blocks and long contexts: the keys of each block shared out, as ``prefill_attention`` does
     sms = num_sms(q.device)
     blocks = -(-max_rows // 256) * nh * n_items
-    splits = max(1, min(8, sms // blocks, max_ctx // 1024)) if not w and 2 * blocks <= sms else 1
+    splits = max(1, min(8, sms // blocks, max_ctx // 1024)) if d == 128 and not w and 2 * blocks <= sms else 1
     if T * nh * splits * d * 4 > _PREFILL_SPLIT_BYTES:
         splits = 1
     # one piece of scratch for all: keys, values, a byte a record, the pages of each portion, the items,
@@ -2121,8 +2128,8 @@ def _kv4_loaded_attention(q, cache, items, n_items, max_rows, block_tables, tabl
          q_ptr, k, v, moved, n_items, max_rows, T, tables, places, out_ptr, nh, nkv, d, KV4_LOAD_PAGE, n, w, scale,
          splits, part_o, part_ml, err_ptr, out_stride, keep, beyond, stream)
     _run("kv4_rest", _kv4_rest_call, special, beyond, item_ptr, moved, n_items,
-         max_rows, tables, places, cache_ptr, table_ptr, table_stride, q_ptr, q_stride, out_ptr, out_stride, nh, nkv, ps, pages,
-         w, keep, scale, stream)
+         max_rows, tables, places, cache_ptr, table_ptr, table_stride, q_ptr, q_stride, out_ptr, out_stride, nh, nkv, d, ps,
+         pages, w, keep, scale, stream)
 
 
 def _kv4_attention(q, cache, rows, seq, positions, items, n, max_rows, block_tables, table, strides, out, nh,

@@ -107,7 +107,8 @@ def test_step_tables_takes_int32(ops, name):
         ops.step_tables(**args)
 
 
-@pytest.mark.parametrize("change", [dict(variant="fast"), dict(variant="load"), dict(variant="load", scale=0.0)])
+@pytest.mark.parametrize("change", [dict(variant="fast"), dict(variant="load", q=torch.zeros((3, 512), dtype=BF16)[:, :256]),
+                                    dict(variant="load", scale=0.0)])
 def test_prefill_variants(ops, change, monkeypatch):
     """(The checks before a launch, with the device's left out.)"""
     monkeypatch.setattr(ops, "_same_device", lambda *a: None)
@@ -169,6 +170,7 @@ def test_step_tables_sizes(ops, change, monkeypatch):
 def test_which_portions_are_loaded(ops):
     """The rule's two sides at sizes where they are far apart."""
     pays = ops._kv4_load_pays
-    assert pays(1, 2048, 2048, 0, 0, 32, 8) and pays(1, 256, 8448, 0, 0, 32, 8)
-    assert not pays(6, 5, 3005, 0, 0, 16, 8) and not pays(1, 128, 1128, 0, 0, 32, 8)
-    assert pays(1, 1024, 100000, 512, 0, 32, 8) and not pays(1, 8, 100000, 0, 0, 32, 8)
+    assert pays(1, 2048, 2048, 0, 0, 32, 8, 128) and pays(1, 256, 8448, 0, 0, 32, 8, 128)
+    assert not pays(6, 5, 3005, 0, 0, 16, 8, 128) and not pays(1, 128, 1128, 0, 0, 32, 8, 128)
+    assert pays(1, 1024, 5024, 0, 0, 16, 4, 64) and not pays(1, 256, 4256, 0, 0, 16, 4, 64)
+    assert pays(1, 1024, 100000, 512, 0, 32, 8, 128) and not pays(1, 8, 100000, 0, 0, 32, 8, 128)
