@@ -123,26 +123,26 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
 #pragma unroll 1
   for (int e = tid; e < a.n_tiles; e += 32 * WARPS) {
     KaTile t;
+    int rows = 1, skip = 0;                                 // of the portion; before the tile
     if (a.items) {
-      const int id = a.first_tile + e, i = id / a.tiles_per_item, s = id - i * a.tiles_per_item;
+      const int id = a.first_tile + e, i = id / a.tiles_per_item;
       const int* it = a.items + 4 * (size_t)i;
-      t.b = it[0];
-      t.row0 = it[1] + s * a.tokens;
-      t.pos0 = it[3] + s * a.tokens;
-      t.ntok = min(it[2] - s * a.tokens, a.tokens);
+      t.b = it[0], t.row0 = it[1], t.pos0 = it[3];
+      rows = max(it[2], 0), skip = (id - i * a.tiles_per_item) * a.tokens;
     } else {
       const int n = a.first_tile + e;
       t.row0 = a.rows ? a.rows[n] : n;
       const bool ok = t.row0 >= 0 && t.row0 < a.T;
       t.b = ok ? a.seq_of_token[t.row0] : -1;
       t.pos0 = ok ? a.positions[t.row0] : 0;
-      t.ntok = 1;
     }
-    if (t.ntok > 0 && (t.b < 0 || t.b >= a.table_rows || t.row0 < 0 || t.row0 + t.ntok > a.T || t.pos0 < 0 ||
-                       (long long)t.pos0 + t.ntok > (long long)a.table_width * a.page_size)) {
+    t.ntok = min(rows - skip, a.tokens);
+    if (t.ntok > 0 && (t.b < 0 || t.b >= a.table_rows || t.row0 < 0 || t.row0 > a.T - rows || t.pos0 < 0 ||
+                       (long long)t.pos0 + rows > (long long)a.table_width * a.page_size)) {
       if (blockIdx.x == 0) atomicOr(a.err, BF_ERR_PAGE);
       t.ntok = 0;
     }
+    t.row0 += skip, t.pos0 += skip;
     tiles[e] = t;
     const int n = ka_span(t, a.window, a.keep).units;
     units_of[e] = n;

@@ -154,7 +154,8 @@ struct KvBool {
 
 // A block takes 64 tokens of one portion's context and every gridDim.y-th kv head and writes them as bfloat16
 // pages [64][d] of keys and of values, a warp a record of eight tokens; the blocks of page 0 write zeros.
-// Where a portion's pages begin is a sum over the portions before it.  What no row of the portion sees is
+// Where a portion's pages begin is a sum over the portions before it; one that names a request, places or token
+// rows that are not there, or more places than a row of the table has, has none.  What no row of the portion sees is
 // zero (a page of nothing else is left out and its place in the table is page 0).  The blocks of a portion
 // write its row of the table together.
 //
@@ -167,7 +168,7 @@ template <int D, bool HALF>
 __global__ void __launch_bounds__(256)
 kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__ block_tables,
                 int table_stride, int table_rows, int table_width, const int* __restrict__ items, int n_items,
-                __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out,
+                int T, __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out,
                 int* __restrict__ tables_out, int out_width, int* __restrict__ items_out,
                 unsigned char* __restrict__ special, int* __restrict__ beyond, int out_pages, int nkv, int page_size, int num_pages, int window, int keep, int* __restrict__ err) {
   constexpr int NG = D / KV4_GROUP, REC = kv4_record(D);
@@ -176,6 +177,15 @@ kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
   const int page = blockIdx.x;                              // 0: the zero page; else page - 1 of the contexts
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint4 zero = make_uint4(0, 0, 0, 0);
+  // pages of a portion; negative: an error bit
+  auto pages_of = [&](int b, int row0, int rows, int first) {
+    const long long n = (long long)rows + first;
+    if (rows <= 0 && n <= 0) return 0;
+    if (rows < 0 || first < 0 || b < 0 || b >= table_rows || n > (long long)table_width * page_size || row0 < 0 ||
+        row0 > T - rows)
+      return -BF_ERR_PAGE;
+    return n > out_width * 64LL ? -BF_ERR_SPLITS : (int)((n + 63) / 64);
+  };
   // the portion of this page, by every warp for itself
   int item = -1, base = 0, b = 0, first = 0, n_rows = 0;
   for (int i0 = 0, running = 0; i0 < n_items; i0 += 32) {
@@ -184,7 +194,7 @@ kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       if (i < n_items) of[k] = items[4 * i + k];
-    const int n = (max(of[2] + of[3], 0) + 63) / 64;
+    const int found = pages_of(of[0], of[1], of[2], of[3]), n = max(found, 0);
     int incl = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -202,8 +212,8 @@ kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
     }
     if (page == 0 && blockIdx.y == 0 && warp == 0 && i < n_items) {
       // a context that the pages or the table have no room for: none of its rows is attended
-      const bool fits = running + incl <= out_pages - 1 && n <= out_width;
-      if (!fits) atomicOr(err, BF_ERR_SPLITS);
+      const bool fits = found >= 0 && running + incl <= out_pages - 1;
+      if (!fits) atomicOr(err, found < 0 ? -found : BF_ERR_SPLITS);
       if (items_out) {
         items_out[4 * i] = i, items_out[4 * i + 1] = of[1];
         items_out[4 * i + 2] = fits ? of[2] : 0, items_out[4 * i + 3] = of[3];
@@ -213,7 +223,7 @@ kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
   }
   if (page == 0 && blockIdx.y == 0) {
     for (int i = 0; i < n_items; ++i)                       // (portions without a page of their own)
-      if (items[4 * i + 2] + items[4 * i + 3] <= 0)
+      if (pages_of(items[4 * i], items[4 * i + 1], items[4 * i + 2], items[4 * i + 3]) <= 0)
         for (int w = tid; w < out_width; w += 256) tables_out[(size_t)i * out_width + w] = 0;
   }
   if (page == 0 || item < 0) {                              // the zero page, and pages behind the last context
@@ -244,7 +254,7 @@ kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
   int pid = 0;
   if (have) {
     const int at = j8 / page_size;
-    pid = at < table_width && b >= 0 && b < table_rows ? block_tables[(size_t)b * table_stride + at] : -1;
+    pid = at < table_width ? block_tables[(size_t)b * table_stride + at] : -1;
     if (pid < 0 || pid >= num_pages) {
       if (lane == 0 && blockIdx.y == 0) atomicOr(err, BF_ERR_PAGE);
       have = false;
@@ -316,7 +326,7 @@ struct Kv4LoadCall {
   const int* block_tables;
   int table_stride, table_rows, table_width;
   const int* items;
-  int n_items;
+  int n_items, T;
   void* k_out, *v_out;
   int* tables_out;
   int out_width;
@@ -328,7 +338,7 @@ struct Kv4LoadCall {
   cudaStream_t stream;
 };
 BF_EXPORT int bf_kv4_load(const Kv4LoadCall* call) {
-  const auto& [cache, block_tables, table_stride, table_rows, table_width, items, n_items, k_out, v_out,
+  const auto& [cache, block_tables, table_stride, table_rows, table_width, items, n_items, T, k_out, v_out,
                tables_out, out_width, items_out, special, beyond, out_pages, nkv, d, page_size, num_pages,
                window, keep, sms, err, stream] = *call;
   if (n_items <= 0 || out_pages <= 1) return 0;
@@ -339,7 +349,7 @@ BF_EXPORT int bf_kv4_load(const Kv4LoadCall* call) {
   if (parts > nkv) parts = nkv;
   auto run = [&](auto kern) {
     return bf_launch_pdl(kern, dim3(out_pages, parts), dim3(256), 0, stream, (const unsigned char*)cache,
-                         block_tables, table_stride, table_rows, table_width, items, n_items,
+                         block_tables, table_stride, table_rows, table_width, items, n_items, T,
                          (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, tables_out, out_width, items_out,
                          (unsigned char*)special, beyond, out_pages, nkv, page_size, num_pages, window, keep, err);
   };

@@ -1898,15 +1898,19 @@ class _Packed:
         self.name, self.pack, self.fn = name, struct.Struct("@" + fields).pack, None
 
     def __call__(self, *args) -> int:
+        try:
+            packed = self.pack(*args)
+        except struct.error as e:
+            raise KernelError(f"{self.name}: an argument that its type has no room for ({e})") from None
         if self.fn is None:
             fn = getattr(lib(), self.name)
             fn.argtypes = [ctypes.c_char_p]
             self.fn = fn
-        return self.fn(self.pack(*args))
+        return self.fn(packed)
 
 
 _kv4_store_call = _Packed("bf_kv4_store", "PqPqPPiiiiqPP")
-_kv4_load_call = _Packed("bf_kv4_load", "PPiiiPiPPPiPPPiiiiiiiiPP")
+_kv4_load_call = _Packed("bf_kv4_load", "PPiiiPiiPPPiPPPiiiiiiiiPP")
 _kv4_rest_call = _Packed("bf_kv4_rest", "PPPPiiPiPPiPqPqiiiiiiifP")
 _kv4_attention_call = _Packed("bf_kv4_attention", "PqPPPPPiiiPiiiPqiiiiiiifPiPP")
 _step_tables_call = _Packed("bf_step_tables", "PiiPiPiiiPPPPPiPiPiPiPP")
@@ -1946,7 +1950,8 @@ def kv4_load(cache: torch.Tensor, block_tables: torch.Tensor, items: torch.Tenso
     ``[n_items, 4]`` of (request, first token row, rows, first position); ``rows``: the contexts' sum, each
     rounded up to 64.  Page 0 is zero, so are places behind a context and, with ``window`` and
     ``keep_first``, keys that no row of the portion sees (pages of nothing else are not written, their
-    place in ``tables`` is page 0).  ``items_out``: takes the items with the portion's number in the
+    place in ``tables`` is page 0).  A portion of a request or places that the block tables do not have, or
+    without room, sets the error word and has page 0 everywhere.  ``items_out``: takes the items with the portion's number in the
     request's place, which goes with ``tables``; ``places``: the width of ``tables``, where a portion's
     longest context is known to be shorter than all together."""
     table_rows, table_width, table_stride = _want_int_table(block_tables, "kv4_load", "block_tables")
@@ -1965,7 +1970,7 @@ def kv4_load(cache: torch.Tensor, block_tables: torch.Tensor, items: torch.Tenso
     v = torch.empty_like(k)
     tables = torch.empty((n_items, places), dtype=torch.int32, device=device)
     _run("kv4_load", _kv4_load_call, cache.data_ptr(), block_tables.data_ptr(), table_stride, table_rows,
-         table_width, items.data_ptr(), n_items, k.data_ptr(), v.data_ptr(), tables.data_ptr(), places,
+         table_width, items.data_ptr(), n_items, 0x7fffffff, k.data_ptr(), v.data_ptr(), tables.data_ptr(), places,
          items_out.data_ptr() if items_out is not None else 0, 0, 0, n, nkv, d, ps, pages, window, keep_first,
          num_sms(device), err.data_ptr(), _stream().value or 0)
     return k, v, tables
@@ -1974,7 +1979,8 @@ def kv4_load(cache: torch.Tensor, block_tables: torch.Tensor, items: torch.Tenso
 def _kv4_mask(what: str, window: Optional[int], keep_first: int) -> Tuple[int, int]:
     if (window is not None and window < 1) or keep_first < 0:
         raise KernelError(f"{what}: a window has at least one key, keep_first is not negative")
-    return (int(window), int(keep_first)) if window is not None else (0, 0)
+    # (as good as any larger ones: no context is that long)
+    return (min(int(window), 1 << 30), min(int(keep_first), 1 << 30)) if window is not None else (0, 0)
 
 
 def _kv4_attention_check(what, q, cache, block_tables, out, nh, nkv, d, window, keep_first, err, *others):
@@ -2015,7 +2021,10 @@ def kv4_decode_attention(q: torch.Tensor, cache: torch.Tensor, rows: Optional[to
     arguments, with ``cache`` (``kv4_cache``) in the pages' place.  A row at position p sees the keys
     ``j <= p`` of its request; with ``window`` those with ``j > p - window``, and the first ``keep_first``
     tokens.  ``rows`` lists the token rows to run (None: 0 .. n_rows - 1); other rows of ``out`` are left
-    as they were.  A page id outside the pool sets the error word and its keys are left out."""
+    as they were, and so is a listed one whose row, request or position is not there, which sets the error
+    word.  A page id outside the pool sets it too and stands for page 0.
+
+    Queries below 2^62 and values below 2^55 in size: larger ones overflow inside."""
     _want(seq_of_token, torch.int32, "seq_of_token"); _want(positions, torch.int32, "positions")
     if rows is not None:
         _want(rows, torch.int32, "rows")
@@ -2040,7 +2049,9 @@ def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Ten
     """Causal attention of prompt portions over a cache in 4 bits, their own keys included:
     ``prefill_attention``'s arguments, with ``cache`` (``kv4_cache``) in the pages' place.  ``ctx_rows``:
     the portions' contexts added up, each rounded up to 64; ``max_ctx``: the longest of them;
-    ``keep_first``: with a window, the request's first that many tokens stay visible behind it.
+    ``keep_first``: with a window, the request's first that many tokens stay visible behind it.  A portion
+    whose rows, request or places are not there, or that ``ctx_rows`` and ``max_ctx`` have no room for,
+    sets the error word and its rows are left as they were.  Sizes of numbers: as in ``kv4_decode_attention``.
 
     ``variant``: ``stretches`` (the kernel of single tokens, a few rows at a time; reads the cache as it
     is), ``load`` (heads of 64 or 128, a positive scale, q contiguous: the contexts are loaded as ``kv4_load``
@@ -2122,7 +2133,7 @@ def _kv4_loaded_attention(q, cache, items, n_items, max_rows, block_tables, tabl
     table_ptr, item_ptr, cache_ptr, q_ptr, out_ptr, err_ptr = (t.data_ptr() for t in (block_tables, items, cache, q, out, err))
     stream = _stream().value or 0
     _run("kv4_load", _kv4_load_call, cache_ptr, table_ptr, table_stride,
-         table_rows, table_width, item_ptr, n_items, k, v, tables, places, moved, special, beyond,
+         table_rows, table_width, item_ptr, n_items, T, k, v, tables, places, moved, special, beyond,
          n, nkv, d, ps, pages, w, keep, sms, err_ptr, stream)
     _run("prefill_attention_umma2", _prefill_attention_umma2_half_call,
          q_ptr, k, v, moved, n_items, max_rows, T, tables, places, out_ptr, nh, nkv, d, KV4_LOAD_PAGE, n, w, scale,

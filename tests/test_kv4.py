@@ -174,3 +174,9 @@ def test_which_portions_are_loaded(ops):
     assert not pays(6, 5, 3005, 0, 0, 16, 8, 128) and not pays(1, 128, 1128, 0, 0, 32, 8, 128)
     assert pays(1, 1024, 5024, 0, 0, 16, 4, 64) and not pays(1, 256, 4256, 0, 0, 16, 4, 64)
     assert pays(1, 1024, 100000, 512, 0, 32, 8, 128) and not pays(1, 8, 100000, 0, 0, 32, 8, 128)
+
+
+def test_numbers_that_an_argument_has_no_room_for():
+    from binfer_b200.csrc import ops
+    with pytest.raises(ops.KernelError, match="no room"):
+        ops._Packed("bf_kv4_store", "i")(1 << 40)

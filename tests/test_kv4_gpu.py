@@ -616,6 +616,48 @@ def test_load_without_room_attends_what_fits(cuda_device):
     _compare(c, q[:50], out[:50], nh, [(0, 50, 50)], None, 0, 0.1)
 
 
+@pytest.mark.parametrize("variant", ["stretches", "load"])
+@pytest.mark.parametrize("item", [(-1, 40, 30, 20), (2, 40, 30, 20), (2 ** 31 - 1, 40, 30, 20), (1, -1, 30, 20),
+                                  (1, 41, 30, 20), (1, 2 ** 31 - 1, 30, 20), (1, 40, 30, -10), (1, 40, 30, 5000),
+                                  (1, 40, 30, 2 ** 31 - 10)])
+def test_portions_that_are_not_there(cuda_device, variant, item):
+    """A request, token rows or places outside of what the call is given: flagged, and the rows left as they were;
+    the portion beside it is attended, one value that is not finite and all."""
+    from binfer_b200.csrc import ops
+    nh, nkv, d = 4, 2, 128
+    c = Cache([140, 90], nkv, d, 16, cuda_device)
+    c.v[0][120, 1, 3] = math.inf
+    ops.kv4_store(c.k[0].flatten(1), c.v[0].flatten(1), c.slots[0], c.cache, c.err)
+    q = _queries(70, nh, d, cuda_device)
+    out = torch.full_like(q, 7.0)
+    items = torch.tensor([(0, 0, 40, 100), item], dtype=I32, device=cuda_device)
+    ops.kv4_prefill_attention(q, c.cache, items, 2, 40, c.tables, out, nh, nkv, d, None, 0.1, c.err, ctx_rows=384,
+                              max_ctx=192, variant=variant)
+    assert int(c.err.item()) == 4 and (out[40:] == 7).all()
+    c.err.zero_()
+    k, v = c.held(0)
+    ref, allowed = K4.attend(q[:40].view(40, nh, d).to(F64), k, v.nan_to_num(), torch.arange(100, 140, device=q.device),
+                             None, 0, 0.1)
+    got, lost = out[:40].view(40, nh, d), torch.zeros_like(ref, dtype=torch.bool)
+    lost[20:, nh // nkv:, :64] = True
+    assert torch.isnan(got[lost]).all()
+    _check(got[~lost], ref[~lost], allowed[~lost])
+
+
+@pytest.mark.parametrize("variant", ["stretches", "load"])
+def test_a_window_of_any_size(cuda_device, variant):
+    from binfer_b200.csrc import ops
+    nh, nkv, d = 4, 2, 128
+    c = Cache([140], nkv, d, 16, cuda_device)
+    q = _queries(40, nh, d, cuda_device)
+    items = torch.tensor([(0, 0, 40, 100)], dtype=I32, device=cuda_device)
+    for window, keep in ((2 ** 31 - 1, 2 ** 31 - 1), (2 ** 40, 2 ** 40), (1, 2 ** 40)):
+        out = torch.zeros_like(q)
+        ops.kv4_prefill_attention(q, c.cache, items, 1, 40, c.tables, out, nh, nkv, d, window, 0.1, c.err,
+                                  ctx_rows=192, max_ctx=140, keep_first=keep, variant=variant)
+        _compare(c, q, out, nh, [(0, 40, 100)], None, 0, 0.1)
+
+
 @pytest.mark.parametrize("what", ["queries", "keys", "both", "one key"])
 @pytest.mark.parametrize("window,keep,d", [(None, 0, 128), (150, 4, 128), (None, 0, 64)])
 def test_loaded_keys_and_queries_beyond_fp16(cuda_device, what, window, keep, d):
