@@ -54,10 +54,11 @@
 // then the window's), and a head may have a sink, a logit that joins its sums in the epilogue or in
 // the merge.  Kept tokens are a fourth instance (KEEP), whose masks the plain one does without.
 //
-// Keys may be fp16 (HALF: those of a cache held in 4 bits, whose numbers bfloat16 would round): the softmax
-// warps then make their Q tile fp16 where it lies before its first product, and a request and kv head
-// with a query beyond fp16's range is noted in `beyond` for the caller to compute otherwise.  Heads of 64 go
-// this way too: one block of 64 columns where the others have two, and half of O's tensor memory.
+// Keys and values may be fp16 (HALF: those of a cache held in 4 bits, whose numbers bfloat16 would round): the
+// softmax warps then make their Q tile fp16 where it lies before its first product, and a request and kv
+// head with a query beyond fp16's range is noted in `beyond` for the caller to compute otherwise.  P is
+// fp16 as well, times 2^6: at most 2^14, since the reference lies at most 2^8 below the maximum, and what
+// is lost below its smallest number is 2^-31 of the largest.  Heads of 64 go this way too: one block of 64 columns where the others have two, and half of O's tensor memory.
 //
 // Every mbarrier wait is bounded.  A barrier whose waiter could fall two phases behind exists
 // once per parity of the tile number, so that its one-bit phase cannot alias: "P V of tile n
@@ -351,7 +352,7 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
       const uint32_t idesc_s = (1u << 4) | (HALF ? 0u : (1u << 7) | (1u << 10)) |
                                ((uint32_t)(A2_BN >> 3) << 17) | ((uint32_t)(A2_BM >> 4) << 24);
       // O: a = P (K-major), b = V as stored (MN-major), N = head size
-      const uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) |
+      const uint32_t idesc_o = (1u << 4) | (HALF ? 0u : (1u << 7) | (1u << 10)) | (1u << 16) |
                                ((uint32_t)(D >> 3) << 17) | ((uint32_t)(A2_BM >> 4) << 24);
       const uint32_t q_addr = smem_u32(Qs + grp * Q_BYTES);
       auto issue_s = [&](int n) {                        // S of tile n into S buffer n & 1
@@ -563,7 +564,7 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
         float m_use[2], ts[2][2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          m_use[e] = m_ref[e] == -INFINITY ? 0.f : m_ref[e];
+          m_use[e] = m_ref[e] == -INFINITY ? 0.f : HALF ? m_ref[e] - 6.f : m_ref[e];
           ts[e][0] = ts[e][1] = 0.f;
         }
 #pragma unroll
@@ -575,8 +576,13 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
                   DIFF ? row_scale[e] : scale_log2, -m_use[e]);
             const float e0 = ex2_approx(x0), e1 = ex2_approx(x1);
             add2f(ts[e][0], ts[e][1], e0, e1);
-            const __nv_bfloat162 p2 = __floats2bfloat162_rn(e0, e1);
-            packed[2 * c + e] = *reinterpret_cast<const uint32_t*>(&p2);
+            if constexpr (HALF) {
+              const __half2 p2 = __floats2half2_rn(e0, e1);
+              packed[2 * c + e] = *reinterpret_cast<const uint32_t*>(&p2);
+            } else {
+              const __nv_bfloat162 p2 = __floats2bfloat162_rn(e0, e1);
+              packed[2 * c + e] = *reinterpret_cast<const uint32_t*>(&p2);
+            }
           }
 #pragma unroll
         for (int e = 0; e < 2; ++e) lsum[e] = lsum[e] * factor[e] + (ts[e][0] + ts[e][1]);
@@ -873,7 +879,8 @@ BF_EXPORT int bf_prefill_attention_umma2_capped(
                       out_stride, out_scale, sinks, keep, nullptr, stream);
 }
 
-// bfloat16 queries and values over fp16 keys; heads of 128, or of 64 with one split.
+// bfloat16 queries over fp16 keys and values, the result times `out_scale`; heads of 128, or of 64 with one
+// split.
 struct PrefillAttentionUmma2HalfCall {
   const void* q, *k_cache, *v_cache;
   const int* items;
@@ -887,6 +894,7 @@ struct PrefillAttentionUmma2HalfCall {
   float* part_o, *part_ml;
   int* err;
   long long out_stride;
+  float out_scale;
   int keep;
   int* beyond;
   cudaStream_t stream;
@@ -894,11 +902,11 @@ struct PrefillAttentionUmma2HalfCall {
 BF_EXPORT int bf_prefill_attention_umma2_half(const PrefillAttentionUmma2HalfCall* call) {
   const auto& [q, k_cache, v_cache, items, n_items, max_rows, total_rows, block_tables, table_stride, out,
                nh, nkv, d, page_size, num_pages, window, scale, splits, part_o, part_ml, err, out_stride,
-               keep, beyond, stream] = *call;
+               out_scale, keep, beyond, stream] = *call;
   if (!beyond) return (int)cudaErrorInvalidValue;
   return launch_umma2(q, k_cache, v_cache, items, n_items, max_rows, total_rows, block_tables, table_stride, out,
                       nh, nkv, d, page_size, num_pages, window, scale, splits, part_o, part_ml, err, 0.f,
-                      out_stride, 1.f, nullptr, keep, beyond, stream);
+                      out_stride, out_scale, nullptr, keep, beyond, stream);
 }
 
 BF_EXPORT int bf_prefill_attention_umma2(const void* q, const void* k_cache, const void* v_cache,

@@ -9,6 +9,7 @@
 #include "kv4.cuh"
 
 #define KS_THREADS 256
+#define KV4_VALUE_UP 16.f       // fp16 values: 2^-18 is the smallest with all its bits, 4,062 the largest
 
 // z / n for small z, with ceil(2^32 / n) (n = 1: 0, which stands for 2^32)
 __device__ __forceinline__ int ks_row(int z, unsigned inverse) {
@@ -159,11 +160,13 @@ struct KvBool {
 // zero (a page of nothing else is left out and its place in the table is page 0).  The blocks of a portion
 // write its row of the table together.
 //
-// For attention on the tensor cores (HALF) the keys are fp16: a number m + s c has up to twelve bits, of which
-// bfloat16 keeps eight, and the scores' error was the largest part of the result's (0.0036 of its rms
-// against 0.0024).  A byte a record then says whether it holds a key beyond fp16's range, or a value that is
-// not finite (a probability of zero times such a value is NaN: whole tiles would carry it into rows that
-// do not see it); kv4_rest_kernel computes what is concerned.
+// For attention on the tensor cores (HALF) keys and values are fp16, values KV4_VALUE_UP times: a number
+// m + s c has up to twelve bits, of which bfloat16 keeps eight (the result's error was 0.0036 of its rms
+// with both in bfloat16, 0.0027 with the values and probabilities; its own rounding to bfloat16 alone is
+// 0.0017).  A byte a record then says whether it holds a key or value beyond fp16's range, a group of values
+// so small that fp16 has less than half a step of 2^-11 for its largest, or a value that is not finite (a
+// probability of zero times such a value is NaN: whole tiles would carry it into rows that do not see it);
+// kv4_rest_kernel computes what is concerned.
 template <int D, bool HALF>
 __global__ void __launch_bounds__(256)
 kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__ block_tables,
@@ -308,9 +311,13 @@ kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float vs = kv4_scale(vp[e * NG + g]);
+        const float up = HALF ? KV4_VALUE_UP : 1.f, vm = kv4_low(vp[e * NG + g]);
         *reinterpret_cast<uint4*>(vo + (2 * q + e) * D + g * 64 + r * 8) =
-            v_on[e] ? eight(vw[e * NG + g], vs, kv4_low(vp[e * NG + g]), KvBool<false>()) : zero;
-        if (HALF) other |= v_on[e] && vs != vs;
+            v_on[e] ? eight(vw[e * NG + g], vs * up, vm * up, KvBool<HALF>()) : zero;
+        if (HALF) {
+          const float most = fmaxf(fabsf(vm), fabsf(fmaf(15.f, vs, vm)));
+          other |= v_on[e] && (vs != vs || most > 65000.f / KV4_VALUE_UP || (most > 0.f && most < 0x1p-18f));
+        }
       }
     }
     if (HALF) {
@@ -320,7 +327,8 @@ kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
   }
 }
 
-// special (8 bytes a page and head) and beyond (n_items x nkv), both or neither: keys in fp16, heads of 64 or 128.
+// special (8 bytes a page and head) and beyond (n_items x nkv), both or neither: keys and values in fp16, heads
+// of 64 or 128.
 struct Kv4LoadCall {
   const void* cache;
   const int* block_tables;

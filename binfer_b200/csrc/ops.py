@@ -1825,6 +1825,7 @@ def kv_store(proj: torch.Tensor, k_off: int, v_off: int, slots: torch.Tensor,
 KV4_HEAD_DIMS = (64, 128, 256)
 KV4_GROUP = 64               # numbers of a row that share a scale and a lowest value
 KV4_LOAD_PAGE = 64           # tokens of a page that kv4_load writes
+KV4_VALUE_UP = 16            # values in fp16 are so many times themselves (kv4.cu)
 
 
 def kv4_takes(dtype: torch.dtype, d: int, page_size: int) -> bool:
@@ -1914,7 +1915,7 @@ _kv4_load_call = _Packed("bf_kv4_load", "PPiiiPiiPPPiPPPiiiiiiiiPP")
 _kv4_rest_call = _Packed("bf_kv4_rest", "PPPPiiPiPPiPqPqiiiiiiifP")
 _kv4_attention_call = _Packed("bf_kv4_attention", "PqPPPPPiiiPiiiPqiiiiiiifPiPP")
 _step_tables_call = _Packed("bf_step_tables", "PiiPiPiiiPPPPPiPiPiPiPP")
-_prefill_attention_umma2_half_call = _Packed("bf_prefill_attention_umma2_half", "PPPPiiiPiPiiiiiifiPPPqiPP")
+_prefill_attention_umma2_half_call = _Packed("bf_prefill_attention_umma2_half", "PPPPiiiPiPiiiiiifiPPPqfiPP")
 
 
 def kv4_store(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: torch.Tensor,
@@ -2055,7 +2056,7 @@ def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Ten
 
     ``variant``: ``stretches`` (the kernel of single tokens, a few rows at a time; reads the cache as it
     is), ``load`` (heads of 64 or 128, a positive scale, q contiguous: the contexts are loaded as ``kv4_load``
-    does, keys in fp16, into scratch of 4 d bytes a token and kv head, and attended on tcgen05), or ``auto``."""
+    does, in fp16, into scratch of 4 d bytes a token and kv head, and attended on tcgen05), or ``auto``."""
     _want(items, torch.int32, "items")
     table, strides, pages, ps, w, keep = _kv4_attention_check(
         "kv4_prefill_attention", q, cache, block_tables, out, nh, nkv, d, window, keep_first, err, items)
@@ -2137,7 +2138,7 @@ def _kv4_loaded_attention(q, cache, items, n_items, max_rows, block_tables, tabl
          n, nkv, d, ps, pages, w, keep, sms, err_ptr, stream)
     _run("prefill_attention_umma2", _prefill_attention_umma2_half_call,
          q_ptr, k, v, moved, n_items, max_rows, T, tables, places, out_ptr, nh, nkv, d, KV4_LOAD_PAGE, n, w, scale,
-         splits, part_o, part_ml, err_ptr, out_stride, keep, beyond, stream)
+         splits, part_o, part_ml, err_ptr, out_stride, 1.0 / KV4_VALUE_UP, keep, beyond, stream)
     _run("kv4_rest", _kv4_rest_call, special, beyond, item_ptr, moved, n_items,
          max_rows, tables, places, cache_ptr, table_ptr, table_stride, q_ptr, q_stride, out_ptr, out_stride, nh, nkv, d, ps,
          pages, w, keep, scale, stream)

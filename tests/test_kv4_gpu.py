@@ -702,6 +702,43 @@ def test_loaded_portions_are_as_close_as_stretches(cuda_device, d):
         assert off <= 2.8e-3, (variant, float(off))
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n", [600, 9000])
+def test_loaded_portions_lose_little_but_the_result_s_rounding(cuda_device, d, n):
+    """Queries, keys, values and probabilities in fp16 are off by 2^-11 / sqrt(3) each, 5e-4 together; the result's
+    rounding to bfloat16 by 2^-8 / sqrt(3) of a number's upper bound, 1.7e-3 of its rms on average."""
+    from binfer_b200.csrc import ops
+    nh, nkv, new = 8, 2, 300
+    c = Cache([n], nkv, d, 16, cuda_device, seed=2)
+    q = _queries(new, nh, d, cuda_device) * 1.5
+    items = torch.tensor([(0, 0, new, n - new)], dtype=I32, device=cuda_device)
+    k, v = c.held(0)
+    ref, _ = K4.attend(q.view(new, nh, d).to(F64), k, v, torch.arange(n - new, n, device=q.device), None, 0, d ** -0.5)
+    out = torch.empty_like(q)
+    ops.kv4_prefill_attention(q, c.cache, items, 1, new, c.tables, out, nh, nkv, d, None, d ** -0.5, c.err,
+                              ctx_rows=-(-n // 64) * 64, max_ctx=n, variant="load")
+    off = (out.view(new, nh, d).to(F64) - ref).square().mean().sqrt() / ref.square().mean().sqrt()
+    assert off <= 2e-3, float(off)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("size", [2.0 ** -40, 2.0 ** -20, 2.0 ** -16, 2.0 ** -8, 2.0 ** 8, 2.0 ** 11, 2.0 ** 30])
+def test_loaded_values_of_any_size(cuda_device, d, size):
+    """Values that fp16 has no room for, or few bits, among them; the first tokens' are ordinary."""
+    from binfer_b200.csrc import ops
+    nh, nkv, n, new = 4, 2, 300, 100
+    c = Cache([n], nkv, d, 16, cuda_device, seed=4)
+    c.v[0][40:] = (c.v[0][40:].float() * size).to(BF16)
+    ops.kv4_store(c.k[0].flatten(1), c.v[0].flatten(1), c.slots[0], c.cache, c.err)
+    q = _queries(new, nh, d, cuda_device)
+    items = torch.tensor([(0, 0, new, n - new)], dtype=I32, device=cuda_device)
+    for window in (None, 120):                  # (with it no row sees an ordinary value)
+        out = torch.full_like(q, math.nan)
+        ops.kv4_prefill_attention(q, c.cache, items, 1, new, c.tables, out, nh, nkv, d, window, 0.1, c.err,
+                                  ctx_rows=320, max_ctx=n, variant="load")
+        _compare(c, q, out, nh, [(0, new, n - new)], window, 0, 0.1)
+
+
 @pytest.mark.parametrize("nh,nkv,d", [(8, 2, 64), (6, 6, 128), (16, 1, 64)])
 @pytest.mark.parametrize("window,keep", [(None, 0), (300, 0), (500, 70)])
 def test_loaded_long_portions(cuda_device, nh, nkv, d, window, keep):
