@@ -10,6 +10,8 @@
 //
 // One launch: block (b, y) sums the counts before b by itself and takes every gridDim.y-th stretch of b's
 // table and tokens.  A new page is always read from `new_pages`, so no block waits for another's write.
+#include <climits>
+
 #include "common.cuh"
 
 #define ST_THREADS 128
@@ -45,15 +47,16 @@ step_tables_kernel(int* __restrict__ master, int master_rows, int master_width,
 
   const bool padding = row < 0;
   bool bad = start < 0 || held < 0 || row >= master_rows || tok + count > T;
-  const int need = padding ? 0 : (int)(((long long)start + count + page_size - 1) / page_size);
-  bad |= need > width || need > master_width || (need > held && ((long long)off + need - held > n_new || off < 0));
+  const long long after = (long long)start + count, places = padding ? 0 : (after + page_size - 1) / page_size;
+  const int need = (int)min(places, (long long)INT_MAX);
+  bad |= after > INT_MAX || need > width || need > master_width || (need > held && ((long long)off + need - held > n_new || off < 0));
   if (bad) {                                                // nothing of this entry can be described
     if (threadIdx.x == 0 && blockIdx.y == 0) atomicOr(err, BF_ERR_PAGE);
   }
   if (threadIdx.x == 0 && blockIdx.y == 0) {
     q_start[b] = (int)tok;
     if (b == B - 1) q_start[B] = (int)(tok + count);
-    ctx_lens[b] = start + count;
+    ctx_lens[b] = (int)after;
     if (count == 1 && decode_rows && dec < n_decode) decode_rows[dec] = (int)tok;
     if (count > 1 && items && por < n_items) {
       items[4 * por] = b, items[4 * por + 1] = (int)tok;

@@ -514,6 +514,15 @@ def test_step_tables_flags_what_does_not_fit(cuda_device, entry, new_pages):
     assert got["tables"][0].tolist() == [2, 0, 0, 0] and got["tables"][2].tolist() == [2, 0, 0, 0]
 
 
+@pytest.mark.parametrize("start", [2 ** 31 - 2, 2 ** 31 - 4, 2 ** 31 - 5])
+def test_step_tables_flags_positions_past_31_bits(cuda_device, start):
+    """Pages of one token, where the places needed are as many as the tokens."""
+    master = torch.full((3, 4), 2, dtype=I32, device=cuda_device)
+    got, err = _describe(cuda_device, master, [(0, 1, 2, 2, 0), (1, start, 4, 0, 0), (2, 0, 1, 1, 0)], [5], 1, 10, 4)
+    assert err == 4 and got["slots"][:7].tolist() == [2, 5, -1, -1, -1, -1, 2]
+    assert got["tables"].tolist() == [[2, 2, 5, 0], [0] * 4, [2, 0, 0, 0]]
+
+
 def test_step_tables_with_less_room_than_tokens(cuda_device):
     master = torch.full((2, 4), 3, dtype=I32, device=cuda_device)
     got, err = _describe(cuda_device, master, [(0, 0, 3, 1, 0), (1, 0, 6, 1, 0)], [0], 16, 10, 4, T=5)
