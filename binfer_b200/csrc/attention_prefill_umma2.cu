@@ -58,7 +58,9 @@
 // softmax warps then make their Q tile fp16 where it lies before its first product, and a request and kv
 // head with a query beyond fp16's range is noted in `beyond` for the caller to compute otherwise.  P is
 // fp16 as well, times 2^6: at most 2^14, since the reference lies at most 2^8 below the maximum, and what
-// is lost below its smallest number is 2^-31 of the largest.  Heads of 64 go this way too: one block of 64 columns where the others have two, and half of O's tensor memory.
+// is lost below its smallest number is 2^-31 of the largest.  Heads of 64 and 256 go this way
+// too, tiles of one or four blocks of 64 columns where the others have two; 256 leave room in tensor and
+// shared memory for one query tile, with its group, and five tiles of K and V in one ring, in the order in which they are used.
 //
 // Every mbarrier wait is bounded.  A barrier whose waiter could fall two phases behind exists
 // once per parity of the tile number, so that its one-bit phase cannot alias: "P V of tile n
@@ -88,6 +90,7 @@ constexpr int A2_TMA_WARP = 16;
 constexpr int A2_MMA_WARP = 17;  // 17 issues for query tile A, 18 for tile B
 constexpr int A2_D = 128;
 constexpr int A2_PLAIN = 0, A2_DIFF = 1, A2_LATENT = 2, A2_KEEP = 3;   // the instances
+constexpr int A2_RING = 5;       // heads of 256: K and V tiles under way together
 constexpr int A2_ROT = 64;       // LATENT: rotated sizes behind the 128 plain ones
 
 // Barrier among the 256 softmax threads of a group (or THREADS of both) that also ANDs a
@@ -124,8 +127,9 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
   constexpr bool DIFF = MODE == A2_DIFF, LATENT = MODE == A2_LATENT, KEEP = MODE == A2_KEEP;
   constexpr int HALVES = D / 64;                         // blocks of 64 columns of a V tile
   constexpr int KBLOCKS = LATENT ? HALVES + 1 : HALVES;  // ... of a Q or K tile
-  constexpr int STAGES = LATENT ? 3 : A2_STAGES;
-  constexpr int BROWS = DIFF ? A2_BM : 2 * A2_BM;        // query rows of a CTA
+  constexpr bool ONE = D > A2_D;                         // one query tile, one softmax group
+  constexpr int STAGES = LATENT ? 3 : ONE ? A2_RING : A2_STAGES;
+  constexpr int BROWS = DIFF || ONE ? A2_BM : 2 * A2_BM; // query rows of a CTA
   constexpr int TSHIFT = DIFF ? 0 : A2_BM;               // rows from query tile A to tile B
   constexpr int QHALF_BYTES = A2_BM * 128;               // 128 query rows of 128 bytes
   constexpr int KHALF_BYTES = A2_BN * 128;               // 64 key rows of 128 bytes
@@ -135,11 +139,11 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
   constexpr int OH = D / 2;                              // O columns per softmax thread
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint8_t* Qs = base;                                    // [2][Q_BYTES]
-  uint8_t* Ks = Qs + 2 * Q_BYTES;                        // [STAGES][K_BYTES]
-  uint8_t* Vs = Ks + STAGES * K_BYTES;                   // [STAGES][V_BYTES]
-  float* xm = reinterpret_cast<float*>(Vs + STAGES * V_BYTES);   // [sums, references][2 groups][128]
-  float* xss = xm + 4 * 128;                             // DIFF: [4 column quarters][128] sums of squares
+  uint8_t* Qs = base;                                    // [2][Q_BYTES] (ONE: [1])
+  uint8_t* Ks = Qs + (ONE ? 1 : 2) * Q_BYTES;                       // [STAGES][K_BYTES]
+  uint8_t* Vs = Ks + (ONE ? 0 : STAGES * K_BYTES);       // [STAGES][V_BYTES] (ONE: one ring of both)
+  float* xm = reinterpret_cast<float*>(Vs + STAGES * V_BYTES);   // [sums, references][2 groups (ONE: 1)][128]
+  float* xss = xm + (ONE ? 2 : 4) * 128;                             // DIFF: [4 column quarters][128] sums of squares
   uint64_t* bars = reinterpret_cast<uint64_t*>(xss + (DIFF ? 4 * 128 : 0));
   uint64_t* q_full = bars;                     // [1]
   uint64_t* kv_full = bars + 1;                // [STAGES]
@@ -162,7 +166,7 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
   // long block could start late and end alone: 80 us for 2048 tokens from position 0).
   const int qb = (int)gridDim.z - 1 - (int)blockIdx.z, h = blockIdx.x;
   if (qb * BROWS >= qlen) return;
-  const bool active_b = DIFF || qb * BROWS + A2_BM < qlen;
+  const bool active_b = DIFF || (!ONE && qb * BROWS + A2_BM < qlen);
   const int g = h / (nh / nkv);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int* table = block_tables + (size_t)seq * table_stride;
@@ -217,7 +221,7 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  // columns: S of tile A (2 x 64), S of tile B (2 x 64), O of A (128), O of B (128)
+  // columns: S of tile A (2 x 64), S of tile B (2 x 64), O of A (128; ONE: 256), O of B (128)
 
   if (warp == A2_TMA_WARP) {
     // ---------------------------------------------------------------- TMA producer
@@ -228,16 +232,48 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
         for (int t = 0; t < 2; ++t)
           tma_load_2d(Qs + t * Q_BYTES, &map_q, q_full, h * D + t * 64, row0 + qb * BROWS);
       } else {
-        mbar_expect_tx(q_full, 2 * Q_BYTES);
+        mbar_expect_tx(q_full, (ONE ? 1 : 2) * Q_BYTES);
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < (ONE ? 1 : 2); ++t)
 #pragma unroll
           for (int hh = 0; hh < KBLOCKS; ++hh)
             tma_load_2d(Qs + t * Q_BYTES + hh * QHALF_BYTES, &map_q, q_full,
                         h * (KBLOCKS * 64) + hh * 64, row0 + qb * BROWS + t * A2_BM);
       }
     }
-    if constexpr (LATENT) {
+    if constexpr (ONE) {
+      // pages of 64 keys, read whole, in the order K 0, K 1, V 0, K 2, V 1, .. in which they are used
+      bool ok = true;
+      int c = 0;
+      auto fetch = [&](const CUtensorMap& map, int page) {
+        if (lane == 0) {
+          const int st = c % STAGES;
+          ok = ok && (c < STAGES || mbar_wait(kv_empty + st, (uint32_t)(c / STAGES - 1) & 1u, abort));
+          if (ok) {
+            mbar_expect_tx(kv_full + st, (uint32_t)K_BYTES);
+#pragma unroll
+            for (int hh = 0; hh < HALVES; ++hh)
+              tma_load_2d(Ks + st * K_BYTES + hh * KHALF_BYTES, &map, kv_full + st, hh * 64, (page * nkv + g) * A2_BN);
+          }
+        }
+        ++c;
+      };
+      int mine = 0, before = 0;
+      for (int n = 0; n < tiles && !*abort; ++n) {
+        if (n % 32 == 0) {
+          mine = n + lane < tiles ? table[tile_key(n + lane) / A2_BN] : 0;
+          if (mine < 0 || mine >= num_pages) {
+            atomicOr(err, BF_ERR_PAGE);
+            mine = 0;
+          }
+        }
+        const int page = __shfl_sync(0xffffffffu, mine, n % 32);
+        fetch(map_k, page);
+        if (n > 0) fetch(map_v, before);
+        before = page;
+      }
+      if (tiles > 0 && !*abort) fetch(map_v, before);
+    } else if constexpr (LATENT) {
       // a portion's keys begin at a row that is a multiple of 64 of the expanded buffers, which
       // are zero up to the next one; block_tables holds that row per portion
       if (lane == 0) {
@@ -355,9 +391,12 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
       const uint32_t idesc_o = (1u << 4) | (HALF ? 0u : (1u << 7) | (1u << 10)) | (1u << 16) |
                                ((uint32_t)(D >> 3) << 17) | ((uint32_t)(A2_BM >> 4) << 24);
       const uint32_t q_addr = smem_u32(Qs + grp * Q_BYTES);
+      // where K and V of tile n are in the ring, counted on
+      auto k_at = [&](int n) { return !ONE ? n : n == 0 ? 0 : 2 * n - 1; };
+      auto v_at = [&](int n) { return !ONE ? n : n + 1 < tiles ? 2 * n + 2 : 2 * n + 1; };
       auto issue_s = [&](int n) {                        // S of tile n into S buffer n & 1
         const uint32_t k_addr =
-            smem_u32(Ks + (n % STAGES) * K_BYTES + (DIFF ? grp * KHALF_BYTES : 0));
+            smem_u32(Ks + (k_at(n) % STAGES) * K_BYTES + (DIFF ? grp * KHALF_BYTES : 0));
         const uint32_t d_addr = tmem_base + (uint32_t)(grp * 128 + (n & 1) * A2_BN);
 #pragma unroll
         for (int k = 0; k < (DIFF ? 64 : KBLOCKS * 64) / 16; ++k) {
@@ -367,6 +406,7 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
                     idesc_s, k > 0 ? 1u : 0u);
         }
         umma_commit(s_full + grp * 2 + (n & 1));
+        if (ONE) umma_commit(kv_empty + k_at(n) % STAGES);
       };
       bool ok = my_tiles == 0 || (mbar_wait_warp(HALF ? q_half + grp : q_full, 0, abort) &&
                                   mbar_wait_warp(kv_full, 0, abort));
@@ -375,16 +415,17 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
         issue_s(0);
       }
       for (int n = 0; n < my_tiles && ok; ++n) {
-        const int st = n % STAGES;
+        const int st = v_at(n) % STAGES;
         if (n + 1 < my_tiles) {
           // the next tile's product runs under this tile's softmax; its S buffer is free
           // since the group signalled P of the tile before this one
-          const int s1 = (n + 1) % STAGES;
-          if (!(ok = mbar_wait_warp(kv_full + s1, (uint32_t)((n + 1) / STAGES) & 1u, abort))) break;
+          const int k1 = k_at(n + 1);
+          if (!(ok = mbar_wait_warp(kv_full + k1 % STAGES, (uint32_t)(k1 / STAGES) & 1u, abort))) break;
           tc_fence_after();
           issue_s(n + 1);
         }
         if (!(ok = mbar_wait_warp(p_full + grp * 2 + (n & 1), (uint32_t)(n >> 1) & 1u, abort))) break;
+        if (ONE && !(ok = mbar_wait_warp(kv_full + st, (uint32_t)(v_at(n) / STAGES) & 1u, abort))) break;
         tc_fence_after();
         const uint32_t v_addr = smem_u32(Vs + st * V_BYTES);
         const uint32_t d_addr = tmem_base + (uint32_t)(256 + grp * 128);
@@ -398,7 +439,7 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
                            umma_desc_mn_sw128(v_addr + (uint32_t)(k * 2048), KHALF_BYTES),
                            idesc_o, (n > 0 || k > 0) ? 1u : 0u);
         umma_commit(o_done + grp * 2 + (n & 1));
-        umma_commit(kv_empty + st);          // this thread's share: K and V of the tile
+        umma_commit(kv_empty + st);          // this thread's share: K and V of the tile (ONE: V)
       }
       // tile A ends up to two key tiles before B: its thread still owes its arrival for the
       // stages of those tiles, each once the tile has been fetched (so that the arrival
@@ -600,7 +641,7 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
         lsum[e] += __shfl_xor_sync(0xffffffffu, lsum[e], 2);
       }
       float* xl = xm + grp * 128;
-      float* xr = xm + 256 + grp * 128;                    // the rows' exponent references
+      float* xr = xm + (ONE ? 128 : 256) + grp * 128;                    // the rows' exponent references
       if (q4 == 0) {
         xl[wq * 32 + hb * 16 + (lane >> 2)] = lsum[0];
         xl[wq * 32 + hb * 16 + (lane >> 2) + 8] = lsum[1];
@@ -752,8 +793,9 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
 }
 
 // The splits of a (query row, head) made one: out = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M),
-// M the largest reference.  A warp per (row, head), a lane four of the 128 columns, the splits
+// M the largest reference.  A warp per (row, head), a lane four of 128 columns, the splits
 // in ascending order.
+template <int D>
 __global__ void prefill_attention_merge_kernel(const float* __restrict__ part_o,
                                                const float* __restrict__ part_ml,
                                                const int* __restrict__ items,
@@ -767,27 +809,29 @@ __global__ void prefill_attention_merge_kernel(const float* __restrict__ part_o,
   const size_t base = ((size_t)(row0 + r) * nh + h) * splits;
   float M = -INFINITY;
   for (int s = 0; s < splits; ++s) M = fmaxf(M, part_ml[(base + s) * 2]);
-  float L = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s = 0; s < splits; ++s) {
-    const float m = part_ml[(base + s) * 2];
-    if (m == -INFINITY) continue;                          // a share without keys for this row
-    const float w = exp2f(m - M);
-    L += part_ml[(base + s) * 2 + 1] * w;
-    const float4 o = *reinterpret_cast<const float4*>(part_o + (base + s) * A2_D + lane * 4);
-    acc.x += o.x * w;
-    acc.y += o.y * w;
-    acc.z += o.z * w;
-    acc.w += o.w * w;
+#pragma unroll 1
+  for (int col = lane * 4; col < D; col += 128) {
+    float L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < splits; ++s) {
+      const float m = part_ml[(base + s) * 2];
+      if (m == -INFINITY) continue;                        // a share without keys for this row
+      const float w = exp2f(m - M);
+      L += part_ml[(base + s) * 2 + 1] * w;
+      const float4 o = *reinterpret_cast<const float4*>(part_o + (base + s) * D + col);
+      acc.x += o.x * w;
+      acc.y += o.y * w;
+      acc.z += o.z * w;
+      acc.w += o.w * w;
+    }
+    if (sinks) L += exp2f(fmaf(sinks[h], 1.4426950408889634f, -M));
+    const float inv = L > 0.f ? out_scale / L : 0.f;
+    uint2 packed;
+    __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(&packed);
+    o2[0] = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
+    o2[1] = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+    *reinterpret_cast<uint2*>(out + (size_t)(row0 + r) * out_stride + (size_t)h * D + col) = packed;
   }
-  if (sinks) L += exp2f(fmaf(sinks[h], 1.4426950408889634f, -M));
-  const float inv = L > 0.f ? out_scale / L : 0.f;
-  uint2 packed;
-  __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(&packed);
-  o2[0] = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
-  o2[1] = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
-  *reinterpret_cast<uint2*>(out + (size_t)(row0 + r) * out_stride + (size_t)h * A2_D + lane * 4) =
-      packed;
 }
 
 }  // namespace
@@ -812,7 +856,7 @@ static int launch_umma2(
   if (splits < 1 || (splits > 1 && (!part_o || !part_ml))) return (int)cudaErrorInvalidValue;
   if (window <= 0 || keep < 0) keep = 0;
   if (keep > 0 && splits > 1) return (int)cudaErrorInvalidValue;
-  if ((d != A2_D && !(d == 64 && beyond && splits == 1)) || nkv <= 0 || nh % nkv || page_size < 8 || page_size > A2_BN ||
+  if ((d != A2_D && !((d == 64 || d == 256) && beyond)) || (d == 256 && page_size != A2_BN) || nkv <= 0 || nh % nkv || page_size < 8 || page_size > A2_BN ||
       A2_BN % page_size || ((uintptr_t)q & 15) || ((uintptr_t)k_cache & 15) ||
       ((uintptr_t)v_cache & 15) || ((uintptr_t)out & 15) || !(scale > 0.f) || softcap < 0.f ||
       out_stride < (long long)nh * d || (out_stride & 7))
@@ -836,23 +880,28 @@ static int launch_umma2(
   e = bf_make_tensor_map_pages_bf16(&mvr, v_cache, num_pages, nkv, page_size, d,
                                     A2_BN / page_size);
   if (e) return e;
-  // two Q tiles, the stages of K and V, the row sums, barriers
-  const size_t smem = 1024 + (size_t)2 * 32768 + (size_t)2 * A2_STAGES * 16384 + 2048 + 256;
+  // the Q tiles, the stages of K and V (heads of 256: one tile, a ring of tiles), the row sums, barriers
+  const size_t smem = 1024 + (d == 256 ? (size_t)65536 + A2_RING * 32768 + 1024
+                                       : (size_t)2 * 32768 + 2 * A2_STAGES * 16384 + 2048) + 256;
   auto kern = d == 64 ? (keep > 0 ? prefill_attention_umma2_kernel<A2_KEEP, true, 64>
                                   : prefill_attention_umma2_kernel<A2_PLAIN, true, 64>)
+              : d == 256 ? (keep > 0 ? prefill_attention_umma2_kernel<A2_KEEP, true, 256>
+                                     : prefill_attention_umma2_kernel<A2_PLAIN, true, 256>)
               : beyond ? (keep > 0 ? prefill_attention_umma2_kernel<A2_KEEP, true>
-                                 : prefill_attention_umma2_kernel<A2_PLAIN, true>)
-                     : (keep > 0 ? prefill_attention_umma2_kernel<A2_KEEP>
-                                 : prefill_attention_umma2_kernel<A2_PLAIN>);
-  static bool configured_on[BF_MAX_DEVICES][6];
-  bool& configured = configured_on[bf_current_device()][(keep > 0 ? 1 : 0) + (d == 64 ? 4 : beyond ? 2 : 0)];
+                                   : prefill_attention_umma2_kernel<A2_PLAIN, true>)
+                       : (keep > 0 ? prefill_attention_umma2_kernel<A2_KEEP>
+                                   : prefill_attention_umma2_kernel<A2_PLAIN>);
+  static bool configured_on[BF_MAX_DEVICES][8];
+  bool& configured =
+      configured_on[bf_current_device()][(keep > 0 ? 1 : 0) + (d == 64 ? 4 : d == 256 ? 6 : beyond ? 2 : 0)];
   if (!configured) {
     cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                           (int)smem);
     if (ce != cudaSuccess) return (int)ce;
     configured = true;
   }
-  dim3 grid(nh, n_items * splits, (max_rows + 2 * A2_BM - 1) / (2 * A2_BM));
+  const int rows = d == 256 ? A2_BM : 2 * A2_BM;
+  dim3 grid(nh, n_items * splits, (max_rows + rows - 1) / rows);
   if (grid.y > 65535u || grid.z > 65535u) return (int)cudaErrorInvalidValue;
   kern<<<grid, A2_THREADS, smem, stream>>>(mq, mk, mv, mkr, mvr, items, block_tables, table_stride,
                                            (__nv_bfloat16*)out, nh, nkv, page_size, num_pages,
@@ -862,7 +911,9 @@ static int launch_umma2(
   if (splits > 1) {
     int st = bf_launch_status();
     if (st) return st;
-    prefill_attention_merge_kernel<<<dim3((max_rows + 3) / 4, nh, n_items), 128, 0, stream>>>(
+    const auto merge = d == 64 ? prefill_attention_merge_kernel<64> : d == 256 ? prefill_attention_merge_kernel<256>
+                                                                               : prefill_attention_merge_kernel<128>;
+    merge<<<dim3((max_rows + 3) / 4, nh, n_items), 128, 0, stream>>>(
         part_o, part_ml, items, (__nv_bfloat16*)out, nh, splits, out_stride, out_scale, sinks);
   }
   return bf_launch_status();
@@ -879,8 +930,7 @@ BF_EXPORT int bf_prefill_attention_umma2_capped(
                       out_stride, out_scale, sinks, keep, nullptr, stream);
 }
 
-// bfloat16 queries over fp16 keys and values, the result times `out_scale`; heads of 128, or of 64 with one
-// split.
+// bfloat16 queries over fp16 keys and values, the result times `out_scale`; heads of 64, 128 or 256.
 struct PrefillAttentionUmma2HalfCall {
   const void* q, *k_cache, *v_cache;
   const int* items;

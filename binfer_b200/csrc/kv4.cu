@@ -327,8 +327,7 @@ kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
   }
 }
 
-// special (8 bytes a page and head) and beyond (n_items x nkv), both or neither: keys and values in fp16, heads
-// of 64 or 128.
+// special (8 bytes a page and head) and beyond (n_items x nkv), both or neither: keys and values in fp16.
 struct Kv4LoadCall {
   const void* cache;
   const int* block_tables;
@@ -350,7 +349,7 @@ BF_EXPORT int bf_kv4_load(const Kv4LoadCall* call) {
                tables_out, out_width, items_out, special, beyond, out_pages, nkv, d, page_size, num_pages,
                window, keep, sms, err, stream] = *call;
   if (n_items <= 0 || out_pages <= 1) return 0;
-  if ((special != nullptr) != (beyond != nullptr) || (special && d != 128 && d != 64)) return (int)cudaErrorInvalidValue;
+  if ((special != nullptr) != (beyond != nullptr) || (special && d != 64 && d != 128 && d != 256)) return (int)cudaErrorInvalidValue;
   // heads apart where pages alone would leave SMs without blocks
   int parts = 1;
   while (parts < nkv && (long long)out_pages * parts < 4LL * sms) parts *= 2;
@@ -361,7 +360,8 @@ BF_EXPORT int bf_kv4_load(const Kv4LoadCall* call) {
                          (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, tables_out, out_width, items_out,
                          (unsigned char*)special, beyond, out_pages, nkv, page_size, num_pages, window, keep, err);
   };
-  if (special) return d == 64 ? run(kv4_load_kernel<64, true>) : run(kv4_load_kernel<128, true>);
+  if (special)
+    return d == 64 ? run(kv4_load_kernel<64, true>) : d == 128 ? run(kv4_load_kernel<128, true>) : run(kv4_load_kernel<256, true>);
   if (d == 64) return run(kv4_load_kernel<64, false>);
   if (d == 128) return run(kv4_load_kernel<128, false>);
   if (d == 256) return run(kv4_load_kernel<256, false>);
@@ -461,5 +461,6 @@ BF_EXPORT int bf_kv4_rest(const Kv4RestCall* call) {
   };
   if (d == 64) return run(kv4_rest_kernel<64>);
   if (d == 128) return run(kv4_rest_kernel<128>);
+  if (d == 256) return run(kv4_rest_kernel<256>);
   return (int)cudaErrorInvalidValue;
 }

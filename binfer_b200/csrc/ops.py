@@ -2055,7 +2055,7 @@ def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Ten
     sets the error word and its rows are left as they were.  Sizes of numbers: as in ``kv4_decode_attention``.
 
     ``variant``: ``stretches`` (the kernel of single tokens, a few rows at a time; reads the cache as it
-    is), ``load`` (heads of 64 or 128, a positive scale, q contiguous: the contexts are loaded as ``kv4_load``
+    is), ``load`` (a positive scale, q contiguous: the contexts are loaded as ``kv4_load``
     does, in fp16, into scratch of 4 d bytes a token and kv head, and attended on tcgen05), or ``auto``."""
     _want(items, torch.int32, "items")
     table, strides, pages, ps, w, keep = _kv4_attention_check(
@@ -2066,10 +2066,9 @@ def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Ten
         raise KernelError(f"kv4_prefill_attention: unknown variant {variant!r}")
     if n_items == 0 or max_rows == 0:
         return
-    load_ok = d in (64, 128) and q.is_contiguous() and ctx_rows > 0 and scale > 0
+    load_ok = q.is_contiguous() and ctx_rows > 0 and scale > 0
     if variant == "load" and not load_ok:
-        raise KernelError("kv4_prefill_attention: the load variant takes heads of 64 or 128, a contiguous q and a "
-                          "positive scale")
+        raise KernelError("kv4_prefill_attention: the load variant takes a contiguous q and a positive scale")
     if variant == "load" or (variant == "auto" and load_ok
                              and _kv4_load_pays(n_items, max_rows, max_ctx, w, keep, nh, nkv, d)):
         _kv4_loaded_attention(q, cache, items, n_items, max_rows, block_tables, table, strides, out, nh, nkv, d, ps,
@@ -2082,24 +2081,37 @@ def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Ten
 _kv4_scratch: dict = {}     # bytes of scratch by a call's sizes
 
 
+def _kv4_splits(n: int, max_rows: int, max_ctx: int, window: int, nh: int, d: int, sms: int) -> Tuple[int, int]:
+    """Blocks of query rows of loaded portions, and into how many shares a block's keys go: few blocks and
+    long contexts, as ``prefill_attention`` does."""
+    blocks = -(-max_rows // (128 if d == 256 else 256)) * nh * n
+    return blocks, max(1, min(8, sms // blocks, max_ctx // 1024)) if not window and 2 * blocks <= sms else 1
+
+
 def _kv4_load_pays(n: int, max_rows: int, max_ctx: int, window: int, keep: int, nh: int, nkv: int,
                    d: int) -> bool:
-    """Whether a call's portions of heads of 64 or 128 are faster loaded and attended on tcgen05 than in
-    stretches of units: microseconds by sizes, fitted to both measured on a B200 (stretches / load).  32
-    heads of 128 (8 kv heads), one portion: 64 rows behind 1,000 keys 23 / 40, behind 16,000 101 / 91; 128
-    rows 29 / 44 and 177 / 93; four of 64 rows behind 4,000 101 / 87.  16 heads of 64 (4): 256 rows behind
-    4,000 41 / 72, 1,024 rows 141 / 83; behind 16,000 121 / 228 and 463 / 241."""
-    seen = min(max_ctx, window + keep + max_rows) if window else max_ctx
-    group = nh // nkv
-    tiles = n * -(-max_rows // max(1, 16 // group)) * -(-group // 16)
-    # 0.64 ns (heads of 64: 0.44) a unit of a tile and kv head, six units to begin one; 512 tiles a launch
-    stretches = 11.0 * -(-tiles // 512) + (0.64e-3 if d == 128 else 0.44e-3) * tiles * nkv * (
-        (seen - max_rows / 2) / 16 + 6)
-    blocks = nh * n * -(-max_rows // 256)
-    if d == 128:          # keys one tile after the other until they are shared out, then the products
-        load = 12.0 + 0.025 * min(seen, 1000) + 0.13e-3 * seen * blocks
-    else:                 # one tile after the other
-        load = 12.0 + 0.0143 * seen * max(1.0, blocks / 148)
+    """Whether a call's portions are faster loaded and attended on tcgen05 than in stretches of units:
+    microseconds by sizes, fitted to both measured on a B200 (stretches / load; 192 pairs of heads of 64, 128
+    and 256, one and four portions of 16 to 1,024 rows behind up to 16,000 keys, whose slower side the
+    rule took in seven, by 12 to 22 %).  32 heads of 128 (8 kv heads), one portion: 64 rows behind 1,000 keys
+    26 / 30, behind 16,000 99 / 88; 256 rows 41 / 37 and 331 / 106.  16 heads of 64 (4): 256 rows behind 1,000
+    keys 21 / 32, behind 4,000 41 / 37; 8 heads of 256 (2): 31 / 36 and 64 / 41."""
+    group, cols = nh // nkv, 8 if d == 256 else 16
+    seen, per = max_ctx, max_ctx
+    if window:
+        seen = min(max_ctx, window + keep + max_rows)
+        per = min(max_ctx, window + keep + min(max_rows, 256))
+    mean = max(per - max_rows / 2, per / 2)
+    tiles = n * -(-max_rows // max(1, cols // group)) * -(-group // cols)
+    # a unit of a tile and kv head, six units to begin one; 512 tiles a launch
+    unit = 0.44e-3 if d == 64 else 0.64e-3 if d == 128 else 0.70e-3
+    stretches = 11.0 * -(-tiles // 512) + unit * tiles * nkv * (mean / 16 + 6)
+    blocks, splits = _kv4_splits(n, max_rows, max_ctx, window, nh, d, 148)
+    # a block's keys one tile after the other; all blocks' products; the keys and values loaded
+    chain = 0.0165 if d == 256 else 0.013
+    product = 0.10e-3 if d == 64 else 0.115e-3 if d == 128 else 0.109e-3
+    load = 14.0 + max(chain * per / splits, chain * min(per, 1000) + product * mean * blocks) + \
+        0.78e-6 * n * seen * nkv * d
     return load < stretches
 
 
@@ -2109,10 +2121,8 @@ def _kv4_loaded_attention(q, cache, items, n_items, max_rows, block_tables, tabl
     (T, q_stride, out_stride), (table_rows, table_width, table_stride) = strides, table
     n = 1 + ctx_rows // KV4_LOAD_PAGE
     places = max(1, -(-max_ctx // KV4_LOAD_PAGE))
-    # few blocks and long contexts: the keys of each block shared out, as ``prefill_attention`` does
     sms = num_sms(q.device)
-    blocks = -(-max_rows // 256) * nh * n_items
-    splits = max(1, min(8, sms // blocks, max_ctx // 1024)) if d == 128 and not w and 2 * blocks <= sms else 1
+    _, splits = _kv4_splits(n_items, max_rows, max_ctx, w, nh, d, sms)
     if T * nh * splits * d * 4 > _PREFILL_SPLIT_BYTES:
         splits = 1
     # one piece of scratch for all: keys, values, a byte a record, the pages of each portion, the items,

@@ -172,7 +172,8 @@ def test_which_portions_are_loaded(ops):
     pays = ops._kv4_load_pays
     assert pays(1, 2048, 2048, 0, 0, 32, 8, 128) and pays(1, 256, 8448, 0, 0, 32, 8, 128)
     assert not pays(6, 5, 3005, 0, 0, 16, 8, 128) and not pays(1, 128, 1128, 0, 0, 32, 8, 128)
-    assert pays(1, 1024, 5024, 0, 0, 16, 4, 64) and not pays(1, 256, 4256, 0, 0, 16, 4, 64)
+    assert pays(1, 1024, 5024, 0, 0, 16, 4, 64) and not pays(1, 256, 1256, 0, 0, 16, 4, 64)
+    assert pays(1, 1024, 5024, 0, 0, 8, 2, 256) and not pays(1, 64, 1064, 0, 0, 8, 2, 256)
     assert pays(1, 1024, 100000, 512, 0, 32, 8, 128) and not pays(1, 8, 100000, 0, 0, 32, 8, 128)
 
 

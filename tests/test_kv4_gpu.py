@@ -598,8 +598,6 @@ def test_a_run_of_steps(cuda_device, window, keep):
 @pytest.mark.parametrize("window,keep", [(None, 0), (64, 0), (100, 11)])
 def test_both_ways_of_a_portion(cuda_device, variant, nh, nkv, d, ps, window, keep):
     from binfer_b200.csrc import ops
-    if variant == "load" and d == 256:
-        pytest.skip("heads of 64 and 128 alone go this way")
     c = Cache([300, 70, 1], nkv, d, ps, cuda_device, seed=nh)
     jobs = [(1, 70, 0), (0, 33, 267), (2, 1, 0)]
     q = _queries(104, nh, d, cuda_device)
@@ -668,7 +666,7 @@ def test_a_window_of_any_size(cuda_device, variant):
 
 
 @pytest.mark.parametrize("what", ["queries", "keys", "both", "one key"])
-@pytest.mark.parametrize("window,keep,d", [(None, 0, 128), (150, 4, 128), (None, 0, 64)])
+@pytest.mark.parametrize("window,keep,d", [(None, 0, 128), (150, 4, 128), (None, 0, 64), (None, 0, 256), (150, 4, 256)])
 def test_loaded_keys_and_queries_beyond_fp16(cuda_device, what, window, keep, d):
     """Numbers that fp16 has no room for, with a scale that makes ordinary scores of them."""
     from binfer_b200.csrc import ops
@@ -691,7 +689,7 @@ def test_loaded_keys_and_queries_beyond_fp16(cuda_device, what, window, keep, d)
     _compare(c, q, out, nh, [(0, new, n - new)], window, keep, scale)
 
 
-@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("d", [64, 128, 256])
 def test_loaded_portions_are_as_close_as_stretches(cuda_device, d):
     """Keys in fp16: what is left of the error is that of the probabilities, the values and the result
     in bfloat16, 1.7e-3 and twice 1.1e-3 of the result's rms (each half a step uniform, 2^-8 / sqrt(3) of a
@@ -711,7 +709,7 @@ def test_loaded_portions_are_as_close_as_stretches(cuda_device, d):
         assert off <= 2.8e-3, (variant, float(off))
 
 
-@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("n", [600, 9000])
 def test_loaded_portions_lose_little_but_the_result_s_rounding(cuda_device, d, n):
     """Queries, keys, values and probabilities in fp16 are off by 2^-11 / sqrt(3) each, 5e-4 together; the result's
@@ -730,7 +728,7 @@ def test_loaded_portions_lose_little_but_the_result_s_rounding(cuda_device, d, n
     assert off <= 2e-3, float(off)
 
 
-@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("size", [2.0 ** -40, 2.0 ** -20, 2.0 ** -16, 2.0 ** -8, 2.0 ** 8, 2.0 ** 11, 2.0 ** 30])
 def test_loaded_values_of_any_size(cuda_device, d, size):
     """Values that fp16 has no room for, or few bits, among them; the first tokens' are ordinary."""
@@ -748,7 +746,7 @@ def test_loaded_values_of_any_size(cuda_device, d, size):
         _compare(c, q, out, nh, [(0, new, n - new)], window, 0, 0.1)
 
 
-@pytest.mark.parametrize("nh,nkv,d", [(8, 2, 64), (6, 6, 128), (16, 1, 64)])
+@pytest.mark.parametrize("nh,nkv,d", [(8, 2, 64), (6, 6, 128), (16, 1, 64), (8, 2, 256), (9, 3, 256)])
 @pytest.mark.parametrize("window,keep", [(None, 0), (300, 0), (500, 70)])
 def test_loaded_long_portions(cuda_device, nh, nkv, d, window, keep):
     """Several query blocks of 256 rows, tiles that end inside, values and keys of two portions."""
