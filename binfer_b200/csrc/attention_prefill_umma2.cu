@@ -178,17 +178,20 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
   const int j_lo = window > 0 ? max(0, p_first - window + 1) : 0;
   int kt_first = j_lo / A2_BN;
   // key tiles of the tokens that the window keeps, where they lie before the window's first one
-  // (not together with splits)
-  int n_keep = 0;
+  int n_keep = 0, n_first = 0;
   if constexpr (KEEP) n_keep = min(kt_first, (keep + A2_BN - 1) / A2_BN);
   int tiles_a = p_last_a / A2_BN - kt_first + 1 + n_keep;
   int tiles = p_last / A2_BN - kt_first + 1 + n_keep;
   auto tile_key = [&](int n) {                            // the first key of the n-th tile
-    return (KEEP && n < n_keep ? n : kt_first + n - n_keep) * A2_BN;
+    if constexpr (KEEP) {
+      const int m = n + n_first;
+      return (m < n_keep ? m : kt_first + m - n_keep) * A2_BN;
+    }
+    return (kt_first + n) * A2_BN;
   };
   if (splits > 1) {                                       // this CTA's share of the key tiles
     const int b = tiles * split / splits, e = tiles * (split + 1) / splits;
-    kt_first += b;
+    (KEEP ? n_first : kt_first) += b;
     tiles_a = max(0, min(tiles_a, e) - b);
     tiles = e - b;
   }
@@ -844,7 +847,7 @@ __global__ void prefill_attention_merge_kernel(const float* __restrict__ part_o,
 // scaled scores, s <- c tanh(s / c) (0: none); the result's rows `out_stride` elements apart
 // (a column block of a wider buffer: a multiple of 8, the block 16-byte aligned) and
 // multiplied by `out_scale`; a logit per head in the softmax's denominator (`sinks`, or null); with a
-// window and one split, the first `keep` tokens that stay visible behind it.  `beyond` (int [n_items, nkv],
+// window, the first `keep` tokens that stay visible behind it.  `beyond` (int [n_items, nkv],
 // zero, or null): the keys are fp16, and an entry becomes 1 where a query is beyond fp16's range.
 static int launch_umma2(
     const void* q, const void* k_cache, const void* v_cache, const int* items, int n_items,
@@ -855,7 +858,6 @@ static int launch_umma2(
   if (n_items <= 0 || max_rows <= 0) return 0;
   if (splits < 1 || (splits > 1 && (!part_o || !part_ml))) return (int)cudaErrorInvalidValue;
   if (window <= 0 || keep < 0) keep = 0;
-  if (keep > 0 && splits > 1) return (int)cudaErrorInvalidValue;
   if ((d != A2_D && !((d == 64 || d == 256) && beyond)) || (d == 256 && page_size != A2_BN) || nkv <= 0 || nh % nkv || page_size < 8 || page_size > A2_BN ||
       A2_BN % page_size || ((uintptr_t)q & 15) || ((uintptr_t)k_cache & 15) ||
       ((uintptr_t)v_cache & 15) || ((uintptr_t)out & 15) || !(scale > 0.f) || softcap < 0.f ||

@@ -2081,37 +2081,38 @@ def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Ten
 _kv4_scratch: dict = {}     # bytes of scratch by a call's sizes
 
 
-def _kv4_splits(n: int, max_rows: int, max_ctx: int, window: int, nh: int, d: int, sms: int) -> Tuple[int, int]:
-    """Blocks of query rows of loaded portions, and into how many shares a block's keys go: few blocks and
-    long contexts, as ``prefill_attention`` does."""
-    blocks = -(-max_rows // (128 if d == 256 else 256)) * nh * n
-    return blocks, max(1, min(8, sms // blocks, max_ctx // 1024)) if not window and 2 * blocks <= sms else 1
+def _kv4_splits(n: int, max_rows: int, max_ctx: int, window: int, keep: int, nh: int, d: int,
+                sms: int) -> Tuple[int, int, int]:
+    """Of loaded portions: blocks of query rows, keys that a block sees, and into how many shares these go:
+    few blocks and many keys, as ``prefill_attention`` does."""
+    rows = 128 if d == 256 else 256
+    blocks = -(-max_rows // rows) * nh * n
+    keys = min(max_ctx, window + keep + min(max_rows, rows)) if window else max_ctx
+    return blocks, keys, max(1, min(8, sms // blocks, keys // 1024)) if 2 * blocks <= sms else 1
 
 
 def _kv4_load_pays(n: int, max_rows: int, max_ctx: int, window: int, keep: int, nh: int, nkv: int,
                    d: int) -> bool:
     """Whether a call's portions are faster loaded and attended on tcgen05 than in stretches of units:
-    microseconds by sizes, fitted to both measured on a B200 (stretches / load; 192 pairs of heads of 64, 128
-    and 256, one and four portions of 16 to 1,024 rows behind up to 16,000 keys, whose slower side the
-    rule took in seven, by 12 to 22 %).  32 heads of 128 (8 kv heads), one portion: 64 rows behind 1,000 keys
+    microseconds by sizes, fitted to both measured on a B200 (stretches / load; 288 pairs of heads of 64, 128
+    and 256, one and four portions of 16 to 1,024 rows behind up to 16,000 keys or windows, whose slower side the
+    rule took in ten, by 11 to 27 %).  32 heads of 128 (8 kv heads), one portion: 64 rows behind 1,000 keys
     26 / 30, behind 16,000 99 / 88; 256 rows 41 / 37 and 331 / 106.  16 heads of 64 (4): 256 rows behind 1,000
     keys 21 / 32, behind 4,000 41 / 37; 8 heads of 256 (2): 31 / 36 and 64 / 41."""
     group, cols = nh // nkv, 8 if d == 256 else 16
-    seen, per = max_ctx, max_ctx
-    if window:
-        seen = min(max_ctx, window + keep + max_rows)
-        per = min(max_ctx, window + keep + min(max_rows, 256))
+    blocks, per, splits = _kv4_splits(n, max_rows, max_ctx, window, keep, nh, d, 148)
+    seen = min(max_ctx, window + keep + max_rows) if window else max_ctx
     mean = max(per - max_rows / 2, per / 2)
     tiles = n * -(-max_rows // max(1, cols // group)) * -(-group // cols)
     # a unit of a tile and kv head, six units to begin one; 512 tiles a launch
     unit = 0.44e-3 if d == 64 else 0.64e-3 if d == 128 else 0.70e-3
     stretches = 11.0 * -(-tiles // 512) + unit * tiles * nkv * (mean / 16 + 6)
-    blocks, splits = _kv4_splits(n, max_rows, max_ctx, window, nh, d, 148)
-    # a block's keys one tile after the other; all blocks' products; the keys and values loaded
-    chain = 0.0165 if d == 256 else 0.013
-    product = 0.10e-3 if d == 64 else 0.115e-3 if d == 128 else 0.109e-3
-    load = 14.0 + max(chain * per / splits, chain * min(per, 1000) + product * mean * blocks) + \
-        0.78e-6 * n * seen * nkv * d
+    # the first keys of a block, whose latencies nothing hides; then its tiles one after the other; all
+    # blocks' products; the keys and values loaded
+    base, later, chain, product = {64: (12.0, 0.007, 0.013, 0.10e-3), 128: (13.0, 0.007, 0.013, 0.115e-3),
+                                   256: (14.0, 0.012, 0.0165, 0.109e-3)}[d]
+    first = base + 0.03 * min(per, 400) + later * max(0, min(per, 1000) - 400)
+    load = max(base + chain * per / splits, first + product * mean * blocks) + 0.78e-6 * n * seen * nkv * d
     return load < stretches
 
 
@@ -2122,7 +2123,7 @@ def _kv4_loaded_attention(q, cache, items, n_items, max_rows, block_tables, tabl
     n = 1 + ctx_rows // KV4_LOAD_PAGE
     places = max(1, -(-max_ctx // KV4_LOAD_PAGE))
     sms = num_sms(q.device)
-    _, splits = _kv4_splits(n_items, max_rows, max_ctx, w, nh, d, sms)
+    _, _, splits = _kv4_splits(n_items, max_rows, max_ctx, w, keep, nh, d, sms)
     if T * nh * splits * d * 4 > _PREFILL_SPLIT_BYTES:
         splits = 1
     # one piece of scratch for all: keys, values, a byte a record, the pages of each portion, the items,

@@ -758,3 +758,18 @@ def test_loaded_long_portions(cuda_device, nh, nkv, d, window, keep):
     ops.kv4_prefill_attention(q, c.cache, items, 2, 900, c.tables, out, nh, nkv, d, window, d ** -0.5, c.err,
                               ctx_rows=1536 + 704, max_ctx=1500, keep_first=keep, variant="load")
     _compare(c, q, out, nh, [(0, 900, 600), (1, 400, 300)], window, keep, d ** -0.5)
+
+
+@pytest.mark.parametrize("nh,nkv,d", [(4, 2, 64), (4, 2, 128), (2, 1, 256)])
+@pytest.mark.parametrize("window,keep", [(None, 0), (2500, 0), (2500, 70), (2100, 300), (4000, 3000)])
+def test_loaded_portions_with_their_keys_shared_out(cuda_device, nh, nkv, d, window, keep):
+    """Few blocks and some thousand keys each, the kept first tokens among them."""
+    from binfer_b200.csrc import ops
+    assert ops._kv4_splits(2, 300, 4500, window or 0, keep, nh, d, ops.num_sms(cuda_device))[2] > 1
+    c = Cache([4500, 900], nkv, d, 32, cuda_device, seed=d)
+    q = _queries(500, nh, d, cuda_device)
+    out = torch.full_like(q, math.nan)
+    items = torch.tensor([(0, 0, 300, 4200), (1, 300, 200, 700)], dtype=I32, device=cuda_device)
+    ops.kv4_prefill_attention(q, c.cache, items, 2, 300, c.tables, out, nh, nkv, d, window, d ** -0.5, c.err,
+                              ctx_rows=4544 + 960, max_ctx=4500, keep_first=keep, variant="load")
+    _compare(c, q, out, nh, [(0, 300, 4200), (1, 200, 700)], window, keep, d ** -0.5)
