@@ -1872,13 +1872,18 @@ def _kv4_check(what: str, cache: torch.Tensor, *others) -> Tuple[int, int, int, 
 
 
 def _same_device(what: str, *tensors) -> None:
-    here = torch.cuda.current_device() if torch.cuda.is_initialized() else None
+    here = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else None
     for t in tensors:
         if t is not None and t.get_device() != here:
             if not t.is_cuda:
                 raise KernelError("the engine's kernels take CUDA tensors only (no CPU path)")
             raise KernelError(f"{what}: a tensor lies on {t.device}, the launch goes to device "
                               f"{torch.cuda.current_device()}")
+
+
+def _stream_at(t: torch.Tensor) -> int:
+    """The current stream of the device that ``t`` lies on (where the launch goes)."""
+    return _raw_stream(t.get_device()) if _raw_stream is not None else _stream().value or 0
 
 
 def _want_int_table(t: torch.Tensor, what: str, name: str) -> Tuple[int, int, int]:
@@ -1940,7 +1945,7 @@ def kv4_store(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: torc
     if T == 0:
         return
     _run("kv4_store", _kv4_store_call, k.data_ptr(), k_stride, v.data_ptr(), v_stride, slots.data_ptr(),
-         cache.data_ptr(), T, nkv, d, ps, pages * ps, err.data_ptr(), _stream().value or 0)
+         cache.data_ptr(), T, nkv, d, ps, pages * ps, err.data_ptr(), _stream_at(cache))
 
 
 def kv4_load(cache: torch.Tensor, block_tables: torch.Tensor, items: torch.Tensor, n_items: int,
@@ -1967,13 +1972,15 @@ def kv4_load(cache: torch.Tensor, block_tables: torch.Tensor, items: torch.Tenso
     window, keep_first = _kv4_mask("kv4_load", window, keep_first)
     n, device = 1 + rows // 64, cache.device
     places = places or n - 1
-    k = torch.empty((n, nkv, KV4_LOAD_PAGE, d), dtype=torch.bfloat16, device=device)
+    # (the strides spelled out: reading a tuple of sizes alone takes torch twice as long)
+    page = KV4_LOAD_PAGE * d
+    k = torch.empty_strided((n, nkv, KV4_LOAD_PAGE, d), (nkv * page, page, d, 1), dtype=torch.bfloat16, device=device)
     v = torch.empty_like(k)
-    tables = torch.empty((n_items, places), dtype=torch.int32, device=device)
+    tables = torch.empty_strided((n_items, places), (places, 1), dtype=torch.int32, device=device)
     _run("kv4_load", _kv4_load_call, cache.data_ptr(), block_tables.data_ptr(), table_stride, table_rows,
          table_width, items.data_ptr(), n_items, 0x7fffffff, k.data_ptr(), v.data_ptr(), tables.data_ptr(), places,
          items_out.data_ptr() if items_out is not None else 0, 0, 0, n, nkv, d, ps, pages, window, keep_first,
-         num_sms(device), err.data_ptr(), _stream().value or 0)
+         num_sms(device), err.data_ptr(), _stream_at(cache))
     return k, v, tables
 
 
@@ -2143,7 +2150,7 @@ def _kv4_loaded_attention(q, cache, items, n_items, max_rows, block_tables, tabl
     else:
         _launches += 1
     table_ptr, item_ptr, cache_ptr, q_ptr, out_ptr, err_ptr = (t.data_ptr() for t in (block_tables, items, cache, q, out, err))
-    stream = _stream().value or 0
+    stream = _stream_at(q)
     _run("kv4_load", _kv4_load_call, cache_ptr, table_ptr, table_stride,
          table_rows, table_width, item_ptr, n_items, T, k, v, tables, places, moved, special, beyond,
          n, nkv, d, ps, pages, w, keep, sms, err_ptr, stream)
@@ -2175,7 +2182,7 @@ def _kv4_attention(q, cache, rows, seq, positions, items, n, max_rows, block_tab
     _run("kv4_attention", _kv4_attention_call, q.data_ptr(), q_stride, cache.data_ptr(), rows, seq, positions,
          items, n, max_rows, T, block_tables.data_ptr(), table_stride, table_rows, table_width, out.data_ptr(),
          out_stride, nh, nkv, d, ps, pages, window, keep, scale, scratch.data_ptr(), sms, err.data_ptr(),
-         _stream().value or 0)
+         _stream_at(q))
     _launches += 1          # two kernels: the stretches of units, and what several of them share
 
 
@@ -2224,7 +2231,7 @@ def step_tables(master: torch.Tensor, entries: torch.Tensor, new_pages: torch.Te
          q_start.data_ptr(), positions.data_ptr(), seq_of_token.data_ptr(), ctx_lens.data_ptr(),
          slots.data_ptr(), T, tables.data_ptr(), tables.shape[1],
          decode_rows.data_ptr() if decode_rows is not None else 0, n_dec,
-         prefill_items.data_ptr() if prefill_items is not None else 0, n_pf, err.data_ptr(), (_stream().value or 0))
+         prefill_items.data_ptr() if prefill_items is not None else 0, n_pf, err.data_ptr(), _stream_at(master))
 
 
 class DiffCombine:
