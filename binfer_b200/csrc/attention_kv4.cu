@@ -26,6 +26,9 @@
 // the order of the keys: scratch is two partials a warp whatever the contexts are.  The running maximum moves
 // only when a score passes it by 2^8, which no result depends on beyond rounding and which leaves one
 // vote a step where maxima would take shuffles.
+//
+// Where the tables have room for few keys only and heads for one wave of blocks (ka_by_head), a block takes a
+// tile and head whole, its warps leave their partials in shared memory and add them up there: no second kernel.
 #include "common.cuh"
 #include "kv4.cuh"
 #include "mma_utils.cuh"
@@ -97,7 +100,8 @@ template <bool B>
 struct Bool {
   static constexpr bool value = B;
 };
-template <int D, int NT>
+// HEAD: block b takes (tile, head) b whole; its warps share the units and add up in shared memory.
+template <int D, int NT, bool HEAD>
 __global__ void __launch_bounds__(32 * ka_warps(D, NT), 1)
 kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   constexpr int NG = D / KV4_GROUP, REC = kv4_record(D), UNIT_BYTES = 2 * REC;
@@ -118,20 +122,16 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   bf_pdl_trigger();
   bf_pdl_wait();
 
-  // ---- tiles, and how their units are cut.  (Loops, not unrolled: what a launch runs once waits for its
-  // instructions most of all.)
-#pragma unroll 1
-  for (int e = tid; e < a.n_tiles; e += 32 * WARPS) {
+  auto tile_of = [&](int id, bool flag) {
     KaTile t;
     int rows = 1, skip = 0;                                 // of the portion; before the tile
     if (a.items) {
-      const int id = a.first_tile + e, i = id / a.tiles_per_item;
+      const int i = id / a.tiles_per_item;
       const int* it = a.items + 4 * (size_t)i;
       t.b = it[0], t.row0 = it[1], t.pos0 = it[3];
       rows = max(it[2], 0), skip = (id - i * a.tiles_per_item) * a.tokens;
     } else {
-      const int n = a.first_tile + e;
-      t.row0 = a.rows ? a.rows[n] : n;
+      t.row0 = a.rows ? a.rows[id] : id;
       const bool ok = t.row0 >= 0 && t.row0 < a.T;
       t.b = ok ? a.seq_of_token[t.row0] : -1;
       t.pos0 = ok ? a.positions[t.row0] : 0;
@@ -139,10 +139,21 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
     t.ntok = min(rows - skip, a.tokens);
     if (t.ntok > 0 && (t.b < 0 || t.b >= a.table_rows || t.row0 < 0 || t.row0 > a.T - rows || t.pos0 < 0 ||
                        (long long)t.pos0 + rows > (long long)a.table_width * a.page_size)) {
-      if (blockIdx.x == 0) atomicOr(a.err, BF_ERR_PAGE);
+      if (flag) atomicOr(a.err, BF_ERR_PAGE);
       t.ntok = 0;
     }
     t.row0 += skip, t.pos0 += skip;
+    return t;
+  };
+  const int warps = gridDim.x * WARPS;
+  int me = warp, each = 1, longer = 0, x = 0, x_end = 1;
+  bool aligned = true;
+  if constexpr (!HEAD) {
+  // ---- tiles, and how their units are cut.  (Loops, not unrolled: what a launch runs once waits for its
+  // instructions most of all.)
+#pragma unroll 1
+  for (int e = tid; e < a.n_tiles; e += 32 * WARPS) {
+    const KaTile t = tile_of(a.first_tile + e, blockIdx.x == 0);
     tiles[e] = t;
     const int n = ka_span(t, a.window, a.keep).units;
     units_of[e] = n;
@@ -150,7 +161,6 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
       for (int i = 0; i < pairs; ++i) a.desc[e * pairs + i] = make_int4(-1, -1, 0, 0);
   }
   __syncthreads();
-  const int warps = gridDim.x * WARPS;
   int total = 0, filled = 0, longest = 0;
 #pragma unroll 1
   for (int e = lane; e < a.n_tiles; e += 32) {
@@ -164,7 +174,7 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   // Short stretches: a tile's heads together get pieces in proportion to their units, one each at least.
   // With `rate` pieces a unit that makes at most rate total + heads of them: warp w tries a rate, and
   // the highest that gives every piece a warp of its own is taken.
-  bool aligned = total < KA_LONG * warps && filled < warps;
+  aligned = total < KA_LONG * warps && filled < warps;
   float rate = 0.f;
   if (aligned) {
     auto rate_of = [&](int i) {
@@ -204,8 +214,8 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
     if (lane == 0) start[a.n_tiles] = before;
   }
   __syncthreads();
-  const int me = warp * gridDim.x + blockIdx.x;             // (few stretches lie on as many SMs)
-  int each = 1, longer = 0, x = me, x_end = me + 1;         // pieces: one
+  me = warp * gridDim.x + blockIdx.x;                       // (few stretches lie on as many SMs)
+  x = me, x_end = me + 1;                                   // pieces: one
   if (!aligned) {
     // every head begins with KA_BEGIN places for what that takes
     const int places = start[a.n_tiles], least = max(KA_LONG / 2, (longest + a.max_pieces - 1) / a.max_pieces);
@@ -216,6 +226,7 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   } else if (me >= start[a.n_tiles]) {
     return;
   }
+  }
 
   const float scale_log2 = a.scale * 1.44269504088896341f;
   const float score_up = scale_log2 * DOWN;
@@ -223,16 +234,28 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   unsigned char* my_ring = smem + (size_t)warp * KA_STAGES * UNIT_BYTES;
 
   while (x < x_end) {
+    int e, pair, u0, mine, n_pieces;
+    KaTile t;
+    KaSpan span;
+    if constexpr (HEAD) {
+      e = blockIdx.x / pairs, pair = blockIdx.x - e * pairs;
+      t = tile_of(e, pair == 0 && tid == 0);
+      if (t.ntok <= 0) return;
+      span = ka_span(t, a.window, a.keep);
+      const int steps = (span.units + 1) >> 1, few = steps / WARPS, more = steps % WARPS;
+      u0 = 2 * (warp * few + min(warp, more));
+      mine = min(2 * (few + (warp < more ? 1 : 0)), span.units - u0);       // (not below zero where u0 is the end)
+      mine = max(mine, 0), n_pieces = WARPS, x = x_end;
+    } else {
     // the tile of x: the last that begins at or before it, among every sixteenth and then among sixteen
-    int e = lane * 16;
+    e = lane * 16;
     e = (31 - __clz(__ballot_sync(0xffffffffu, e < a.n_tiles && start[e] <= x))) * 16;
     const int e1 = e + (lane & 15);
     e += 31 - __clz(__ballot_sync(0xffffffffu, lane < 16 && e1 < a.n_tiles && start[e1] <= x));
     static_assert(KA_MAX_TILES <= 512, "two steps");
-    const KaTile t = tiles[e];
-    const KaSpan span = ka_span(t, a.window, a.keep);
+    t = tiles[e];
+    span = ka_span(t, a.window, a.keep);
     const int y = x - start[e];
-    int pair, u0, mine, n_pieces;
     if (aligned) {
       const int n = start[e + 1] - start[e], fewer = ka_div(n, pairs), more = n - fewer * pairs;
       const int edge = more * (fewer + 1);                  // the first `more` heads have a piece more
@@ -257,6 +280,7 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
       }
       x += to - place;
       if (mine <= 0) continue;
+    }
     }
     const int h = a.chunks == 1 ? pair : pair / a.chunks, head0 = h * a.group + (pair - h * a.chunks) * a.chunk;
     const int heads = min(a.chunk, (h + 1) * a.group - head0);
@@ -562,8 +586,14 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
     cp_async_wait<0>();
 
     // ---- the result: lane (r, q4) has numbers 8 r .. 8 r + 7 of every group, of two columns of every eight
-    const bool whole = mine == span.units;
-    const int slot = 2 * me + (u0 == 0 ? 1 : 0);
+    const bool whole = !HEAD && mine == span.units;
+    const int slot = HEAD ? warp : 2 * me + (u0 == 0 ? 1 : 0);
+    // (HEAD: over the ring; eight numbers between rows, so that stores meet in two ways only)
+    constexpr int ROW = HEAD ? D + 8 : D;
+    float* part_o = HEAD ? reinterpret_cast<float*>(smem) : a.part_o;
+    float2* part_ml = HEAD ? reinterpret_cast<float2*>(tiles) : a.part_ml;
+    static_assert(!HEAD || (WARPS * COLS * ROW * 4 <= WARPS * KA_STAGES * UNIT_BYTES && WARPS * COLS * 8 <= KA_MAX_TILES * 16), "room");
+    if (HEAD) __syncthreads();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -578,7 +608,7 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
         if (ti >= t.ntok || gi >= heads) continue;
         const float sum = l[nt][c] * (1.f / UP);
         const float f = whole ? 1.f / sum : 1.f;
-        if (!whole && r == 0) a.part_ml[slot * COLS + n] = make_float2(m[nt][c], sum);
+        if (!whole && r == 0) part_ml[slot * COLS + n] = make_float2(m[nt][c], sum);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
           const float base = fmaf(-8.f * DOWN, ps[nt][g][c], corr[nt][g][c] * (1.f / UP));
@@ -592,13 +622,40 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
             *reinterpret_cast<uint4*>(a.out + (long long)(t.row0 + ti) * a.out_stride + (size_t)(head0 + gi) * D + g * 64 + r * 8) =
                 make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
           } else {
-            float4* dst = reinterpret_cast<float4*>(a.part_o + ((size_t)slot * COLS + n) * D + g * 64 + r * 8);
+            float4* dst = reinterpret_cast<float4*>(part_o + ((size_t)slot * COLS + n) * ROW + g * 64 + r * 8);
             dst[0] = make_float4(v[0], v[1], v[2], v[3]);
             dst[1] = make_float4(v[4], v[5], v[6], v[7]);
           }
         }
       }
-    if (u0 == 0 && lane == 0)
+    if constexpr (HEAD) {
+      // a column by one warp, or two warps
+      constexpr int PER = WARPS > COLS ? WARPS / COLS : 1, N = D / PER / 32;
+      __syncthreads();
+      for (int id = warp; id < COLS * PER; id += WARPS) {
+        const int n = id / PER, ti = n * a.chunk_inverse >> 8, gi = n - ti * a.chunk;
+        if (ti >= t.ntok || gi >= heads) continue;
+        const float2 ml = lane < WARPS ? part_ml[lane * COLS + n] : make_float2(-INFINITY, 0.f);
+        float top = ml.x;
+#pragma unroll
+        for (int k = 1; k < WARPS; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+        const float f = ml.x == top ? 1.f : ka_exp2(ml.x - top);
+        float sum = 0.f, acc[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc[k] = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+          const float g = __shfl_sync(0xffffffffu, f, w);
+          sum = fmaf(g, __shfl_sync(0xffffffffu, ml.y, w), sum);
+#pragma unroll
+          for (int k = 0; k < N; ++k)
+            acc[k] = fmaf(g, part_o[(w * COLS + n) * ROW + id % PER * (D / PER) + lane + 32 * k], acc[k]);
+        }
+        __nv_bfloat16* dst = a.out + (long long)(t.row0 + ti) * a.out_stride + (size_t)(head0 + gi) * D + id % PER * (D / PER);
+#pragma unroll
+        for (int k = 0; k < N; ++k) dst[lane + 32 * k] = __float2bfloat16_rn(acc[k] / sum);
+      }
+    } else if (u0 == 0 && lane == 0)
       a.desc[e * pairs + pair] = whole ? make_int4(-1, -1, 0, 0) : make_int4(me, n_pieces, t.row0, t.ntok);
   }
 }
@@ -681,16 +738,17 @@ kv4_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ pa
 }
 
 template <int D, int NT>
-static int ka_launch(KaArgs a, int total_tiles, int sms, cudaStream_t stream) {
+static int ka_launch(KaArgs a, int total_tiles, bool by_head, int sms, cudaStream_t stream) {
   constexpr int threads = 32 * ka_warps(D, NT);
   constexpr size_t smem = (size_t)ka_warps(D, NT) * KA_STAGES * 2 * kv4_record(D) +
                           KA_MAX_TILES * (sizeof(KaTile) + 4) + (KA_MAX_TILES + 4) * 4;
   static bool configured[BF_MAX_DEVICES];
   const int dev = bf_current_device();
   if (!configured[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(kv4_attention_kernel<D, NT>,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return (int)e;
+    for (auto kern : {kv4_attention_kernel<D, NT, false>, kv4_attention_kernel<D, NT, true>}) {
+      const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+      if (e != cudaSuccess) return (int)e;
+    }
     configured[dev] = true;
   }
   const int pairs = a.nkv * a.chunks;
@@ -698,13 +756,15 @@ static int ka_launch(KaArgs a, int total_tiles, int sms, cudaStream_t stream) {
   const long long units = ((long long)a.table_width * a.page_size / KA_UNIT + 2 + KA_BEGIN) * pairs;
   if (units > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
   const int most = 0x7fffffffLL / units < KA_MAX_TILES ? (int)(0x7fffffffLL / units) : KA_MAX_TILES;
+  if (by_head)
+    return bf_launch_pdl(kv4_attention_kernel<D, NT, true>, dim3(total_tiles * pairs), dim3(threads), smem, stream, a);
   for (int first = 0; first < total_tiles; first += most) {
     a.first_tile = first;
     a.n_tiles = total_tiles - first < most ? total_tiles - first : most;
     // heads with many pieces each (there are few of them): eight warps add a column's up
     const bool few = (long long)a.n_tiles * pairs * 8 < (long long)sms * ka_warps(D, NT);
     a.max_pieces = few ? sms * ka_warps(D, NT) : 64;
-    int e = bf_launch_pdl(kv4_attention_kernel<D, NT>, dim3(sms), dim3(threads), smem, stream, a);
+    int e = bf_launch_pdl(kv4_attention_kernel<D, NT, false>, dim3(sms), dim3(threads), smem, stream, a);
     if (e) return e;
     auto merge = [&](auto kern, int columns) {
       return bf_launch_pdl(kern, dim3(a.n_tiles * pairs, 8 * NT / columns), dim3(256), 0, stream,
@@ -735,9 +795,24 @@ static KaShape ka_shape(int group, int d, int max_rows) {
 
 static long long ka_slots(const KaShape& s, int d, int sms) { return 2LL * sms * ka_warps(d, s.nt); }
 
-// Bytes of scratch that a call needs (16-byte aligned): partial results and a note per (tile, head).
-BF_EXPORT long long bf_kv4_attention_scratch(int n, int max_rows, int nh, int nkv, int d, int sms) {
+// Whether every (tile, head) gets a block of its own, whose warps meet in shared memory, rather than stretches
+// of equal work and a second kernel: in one wave of blocks, where few units come on a warp.  `keys`: the most
+// that a tile can see.  Measured for rows of equal length, stretches / blocks in us, replayed from a graph: 8 heads
+// (4 query heads each) of 128 over 512 keys 11.0 / 8.8, 1,024 11.0 / 10.7, 2,048 11.6 / 13.0; 128 heads 14.9 / 8.6,
+// 17.2 / 10.7, 21.0 / 14.7; one head of 16 1,024 12.7 / 12.8; two heads of 256 512 keys 12.2 / 9.9, 1,024 12.7 / 12.7;
+// 192 heads of 128 over 512 keys 17.2 / 13.1, but 384 16.9 / 18.9.  That is, blocks save 5 us and take `unit` us
+// a unit, of which the stretches pay a share that grows with the heads: half of them, as the rows of a batch
+// have different lengths.
+static bool ka_by_head(const KaShape& s, int d, long long heads, int keys, int sms) {
+  const float unit = d == 64 ? (s.nt == 1 ? 0.033f : 0.05f) : d == 128 ? (s.nt == 1 ? 0.056f : 0.088f) : 0.104f;
+  return heads <= sms && (keys / KA_UNIT + 1) * unit * (1.f - 0.5f * heads / sms) < 5.2f;
+}
+
+// Bytes of scratch that a call needs (16-byte aligned): partial results and a note per (tile, head); none where
+// no second kernel runs.  `keys` as the call's.
+BF_EXPORT long long bf_kv4_attention_scratch(int n, int max_rows, int nh, int nkv, int d, int sms, int keys) {
   const KaShape s = ka_shape(nh / nkv, d, max_rows);
+  if (ka_by_head(s, d, (long long)n * ((max_rows + s.tokens - 1) / s.tokens) * nkv * s.chunks, keys, sms)) return 0;
   const long long slots = ka_slots(s, d, sms);
   long long tiles = (long long)n * ((max_rows + s.tokens - 1) / s.tokens);
   if (tiles > KA_MAX_TILES) tiles = KA_MAX_TILES;
@@ -757,14 +832,14 @@ struct Kv4AttentionCall {
   int nh, nkv, d, page_size, num_pages, window, keep;
   float scale;
   void* scratch;
-  int sms;
+  int sms, keys;                                           // keys: the most that a row can see, as to the scratch
   int* err;
   cudaStream_t stream;
 };
 BF_EXPORT int bf_kv4_attention(const Kv4AttentionCall* call) {
   const auto& [q, q_stride, cache, rows, seq_of_token, positions, items, n, max_rows, T, block_tables,
                table_stride, table_rows, table_width, out, out_stride, nh, nkv, d, page_size, num_pages,
-               window, keep, scale, scratch, sms, err, stream] = *call;
+               window, keep, scale, scratch, sms, keys, err, stream] = *call;
   if (n <= 0 || max_rows <= 0) return 0;
   if ((long long)num_pages * nkv * (page_size / 8) > 0x7fffffffLL || page_size < 8 || (page_size & (page_size - 1)) ||
       (long long)table_width * page_size > 1 << 24)        // (a tile's units stay below 2^20)
@@ -789,8 +864,10 @@ BF_EXPORT int bf_kv4_attention(const Kv4AttentionCall* call) {
   a.err = err;
   const long long tiles = (long long)n * a.tiles_per_item;
   if (tiles > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
-  if (d == 64) return s.nt == 1 ? ka_launch<64, 1>(a, (int)tiles, sms, stream) : ka_launch<64, 2>(a, (int)tiles, sms, stream);
-  if (d == 128) return s.nt == 1 ? ka_launch<128, 1>(a, (int)tiles, sms, stream) : ka_launch<128, 2>(a, (int)tiles, sms, stream);
-  if (d == 256) return ka_launch<256, 1>(a, (int)tiles, sms, stream);
+  const bool by_head = ka_by_head(s, d, tiles * nkv * s.chunks, keys, sms);
+  if (!by_head && !scratch) return (int)cudaErrorInvalidValue;
+  if (d == 64) return s.nt == 1 ? ka_launch<64, 1>(a, (int)tiles, by_head, sms, stream) : ka_launch<64, 2>(a, (int)tiles, by_head, sms, stream);
+  if (d == 128) return s.nt == 1 ? ka_launch<128, 1>(a, (int)tiles, by_head, sms, stream) : ka_launch<128, 2>(a, (int)tiles, by_head, sms, stream);
+  if (d == 256) return ka_launch<256, 1>(a, (int)tiles, by_head, sms, stream);
   return (int)cudaErrorInvalidValue;
 }

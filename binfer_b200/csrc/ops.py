@@ -1918,7 +1918,7 @@ class _Packed:
 _kv4_store_call = _Packed("bf_kv4_store", "PqPqPPiiiiqPP")
 _kv4_load_call = _Packed("bf_kv4_load", "PPiiiPiiPPPiPPPiiiiiiiiPP")
 _kv4_rest_call = _Packed("bf_kv4_rest", "PPPPiiPiPPiPqPqiiiiiiifP")
-_kv4_attention_call = _Packed("bf_kv4_attention", "PqPPPPPiiiPiiiPqiiiiiiifPiPP")
+_kv4_attention_call = _Packed("bf_kv4_attention", "PqPPPPPiiiPiiiPqiiiiiiifPiiPP")
 _step_tables_call = _Packed("bf_step_tables", "PiiPiPiiiPPPPPiPiPiPiPP")
 _prefill_attention_umma2_half_call = _Packed("bf_prefill_attention_umma2_half", "PPPPiiiPiPiiiiiifiPPPqfiPP")
 
@@ -2086,6 +2086,7 @@ def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Ten
 
 
 _kv4_scratch: dict = {}     # bytes of scratch by a call's sizes
+_KV4_MANY_KEYS = 1 << 15
 
 
 def _kv4_splits(n: int, max_rows: int, max_ctx: int, window: int, keep: int, nh: int, d: int,
@@ -2167,23 +2168,27 @@ def _kv4_attention(q, cache, rows, seq, positions, items, n, max_rows, block_tab
     global _launches
     device = q.device
     sms = num_sms(device)
-    key = (n, max_rows, nh, nkv, d, sms)
+    table_rows, table_width, table_stride = table
+    # what a row can see at most (beyond some thousand keys any number goes the same way)
+    keys = min(table_width * ps, window + keep + max_rows + 32) if window else table_width * ps
+    keys = min(keys, _KV4_MANY_KEYS) & -16
+    key = (n, max_rows, nh, nkv, d, sms, keys)
     size = _kv4_scratch.get(key)
     if size is None:
         fn = lib().bf_kv4_attention_scratch
         fn.restype = _c_ll
         if len(_kv4_scratch) > 4096:
             _kv4_scratch.clear()
-        size = _kv4_scratch[key] = fn(n, max_rows, nh, nkv, d, sms)
+        size = _kv4_scratch[key] = fn(n, max_rows, nh, nkv, d, sms, keys)
     # a call's own, from its stream's pool: two captured graphs share nothing
-    scratch = torch.empty(size, dtype=torch.uint8, device=device)
-    table_rows, table_width, table_stride = table
+    scratch = torch.empty(size, dtype=torch.uint8, device=device) if size else None
     T, q_stride, out_stride = strides
     _run("kv4_attention", _kv4_attention_call, q.data_ptr(), q_stride, cache.data_ptr(), rows, seq, positions,
          items, n, max_rows, T, block_tables.data_ptr(), table_stride, table_rows, table_width, out.data_ptr(),
-         out_stride, nh, nkv, d, ps, pages, window, keep, scale, scratch.data_ptr(), sms, err.data_ptr(),
-         _stream_at(q))
-    _launches += 1          # two kernels: the stretches of units, and what several of them share
+         out_stride, nh, nkv, d, ps, pages, window, keep, scale, scratch.data_ptr() if size else 0, sms, keys,
+         err.data_ptr(), _stream_at(q))
+    if size:
+        _launches += 1      # two kernels: the stretches of units, and what several of them share
 
 
 # ------------------------------------------------------------- a step's description
