@@ -2,6 +2,8 @@
 
     python -m binfer_b200.microbench decode_attention --batch 8 --ctx 4096
     python -m binfer_b200.microbench prefill_attention --tokens 2048
+    python -m binfer_b200.microbench kv4_decode --batch 8 --ctx 4096
+    python -m binfer_b200.microbench kv4_prefill --tokens 2048 --variant load
     python -m binfer_b200.microbench diff_prefill --tokens 2048 --head-dim 64 --value-dim 128
     python -m binfer_b200.microbench diff_decode --batch 8 --head-dim 64 --value-dim 128
     python -m binfer_b200.microbench gemm --tokens 8 --features 6144 --k 4096 [--library]
@@ -153,6 +155,55 @@ def prefill_attention(a):
     flops = 4.0 * nh * d * (T * start + T * (T + 1) / 2)
     report("prefill_attention", us, flops=flops, tokens=T, start=start, heads=nh, kv_heads=nkv,
            head_dim=d)
+
+
+def _kv4_cache(dev, a, n_req, ctx, sets):
+    """(pages in 4 bits, block tables) as ``_paged_cache``'s, with its numbers stored."""
+    nkv, d, ps = a.kv_heads, a.head_dim, a.page_size
+    err, out = ops.error_word(dev), []
+    for _ in range(sets):
+        (kc, vc, bt), = _paged_cache(dev, n_req, ctx, nkv, d, ps, 1, a.scattered)
+        cache = ops.kv4_cache(kc.shape[0], nkv, ps, d, dev)
+        for p0 in range(0, kc.shape[0], 1024):
+            k, v = (c[p0:p0 + 1024].transpose(1, 2).reshape(-1, nkv * d) for c in (kc, vc))
+            slots = torch.arange(p0 * ps, p0 * ps + k.shape[0], dtype=torch.int32, device=dev)
+            ops.kv4_store(k, v, slots, cache, err)
+        out.append((cache, bt))
+    return out
+
+
+def kv4_decode(a):
+    dev = torch.device("cuda:0")
+    B, ctx, nh, nkv, d = a.batch, a.ctx, a.heads, a.kv_heads, a.head_dim
+    per_set = B * ctx * nkv * d * 9 // 8
+    caches = _kv4_cache(dev, a, B, ctx, max(2, int(3e8 // per_set) + 1))
+    q = torch.randn(B, nh * d, device=dev, dtype=BF16)
+    out = torch.empty_like(q)
+    sot = torch.arange(B, dtype=torch.int32, device=dev)
+    pos = torch.full((B,), ctx - 1, dtype=torch.int32, device=dev)
+    err = ops.error_word(dev)
+    fns = [lambda c=c: ops.kv4_decode_attention(q, c[0], None, B, sot, pos, c[1], out, nh, nkv, d, None,
+                                                d ** -0.5, err) for c in caches]
+    us = timed(fns, a.iters, a.warmup)
+    report("kv4_decode", us, nbytes=per_set, batch=B, ctx=ctx, heads=nh, kv_heads=nkv, head_dim=d,
+           page_size=a.page_size)
+
+
+def kv4_prefill(a):
+    dev = torch.device("cuda:0")
+    T, start, nh, nkv, d = a.tokens, a.start, a.heads, a.kv_heads, a.head_dim
+    ctx = start + T
+    (cache, bt), = _kv4_cache(dev, a, 1, ctx, 1)
+    q = torch.randn(T, nh * d, device=dev, dtype=BF16)
+    out = torch.empty_like(q)
+    items = torch.tensor([[0, 0, T, start]], dtype=torch.int32, device=dev)
+    err = ops.error_word(dev)
+    variant = a.variant if a.variant in ("stretches", "load") else "auto"
+    us = timed([lambda: ops.kv4_prefill_attention(q, cache, items, 1, T, bt, out, nh, nkv, d, None, d ** -0.5,
+                                                  err, ctx_rows=-(-ctx // 64) * 64, max_ctx=ctx, variant=variant)],
+               a.iters, a.warmup)
+    report("kv4_prefill", us, flops=4.0 * nh * d * (T * start + T * (T + 1) / 2), tokens=T, start=start, heads=nh,
+           kv_heads=nkv, head_dim=d, variant=variant)
 
 
 def _diff_cache(dev, a, n_req, ctx, sets):
@@ -478,7 +529,7 @@ def main(argv=None):
     ap.add_argument("kernel", choices=["decode_attention", "prefill_attention", "gemm",
                                        "swiglu", "add_rmsnorm", "step_timeline", "scan",
                                        "diff_decode", "diff_prefill", "add_tanh_norm",
-                                       "out_product", "experts"])
+                                       "out_product", "experts", "kv4_decode", "kv4_prefill"])
     ap.add_argument("--iters", type=int, default=50)
     ap.add_argument("--warmup", type=int, default=5)
     ap.add_argument("--batch", type=int, default=8)
@@ -513,9 +564,9 @@ def main(argv=None):
     ap.add_argument("--cluster", type=int, default=0,
                     help="gemm: split K over clusters of this many CTAs (needs --bn)")
     ap.add_argument("--no-graph", action="store_true", help="launch from the host, no CUDA graph")
-    ap.add_argument("--variant", default="auto", choices=["auto", "persistent", "tma", "cp_async", "umma2", "umma", "mma_sync"],
+    ap.add_argument("--variant", default="auto", choices=["auto", "persistent", "tma", "cp_async", "umma2", "umma", "mma_sync", "stretches", "load"],
                     help="decode attention: tma or cp_async tile loads; prefill attention: "
-                         "umma (tcgen05) or mma_sync")
+                         "umma (tcgen05) or mma_sync; kv4_prefill: stretches or load")
     a = ap.parse_args(argv)
     if not torch.cuda.is_available():
         print("microbench needs a CUDA device", file=sys.stderr)
@@ -527,7 +578,7 @@ def main(argv=None):
      "gemm": gemm, "swiglu": swiglu, "add_rmsnorm": add_rmsnorm,
      "step_timeline": step_timeline, "scan": scan, "diff_decode": diff_decode,
      "diff_prefill": diff_prefill, "add_tanh_norm": add_tanh_norm,
-     "out_product": out_product, "experts": experts}[a.kernel](a)
+     "out_product": out_product, "experts": experts, "kv4_decode": kv4_decode, "kv4_prefill": kv4_prefill}[a.kernel](a)
     return 0
 
 
