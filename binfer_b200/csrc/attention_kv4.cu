@@ -127,8 +127,8 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r = lane >> 2, q4 = lane & 3;
   const int pairs = a.nkv * a.chunks;
-  bf_pdl_trigger();
   bf_pdl_wait();
+  bf_pdl_trigger();
 
   auto tile_of = [&](int id, bool flag) {
     KaTile t;

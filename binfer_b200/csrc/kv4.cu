@@ -16,18 +16,10 @@ __device__ __forceinline__ int ks_row(int z, unsigned inverse) {
   return inverse ? (int)__umulhi((unsigned)z, inverse) : z;
 }
 
-// The code of a number, whatever its size: on x / 4, which is exact, so that no difference of finite numbers
-// overflows.  x - m and s are short enough that the float quotient falls on the side of a border that
-// the exact one falls on.
-__device__ __noinline__ unsigned ks_code(float x, float lo, float s) {
-  return s > 0.f ? (unsigned)fminf(rintf((x * 0.25f - lo * 0.25f) / (s * 0.25f)), 15.f) : 0u;
-}
-
 // Four lanes take a group, a lane the sixteen numbers of its part of a key; units are (token, key or value,
 // kv head, group) in the order in which rows lie in memory.  The kernel is bound by its instructions, so
-// minimum and maximum are taken two bfloat16 numbers at a time and the quotient is a product with 1 / s put
-// right by its remainder (bfloat16 numbers make ties common); only where s or the range leaves the ordinary
-// floats is it computed as above.  2,048 tokens of 8 heads of 128: 5.1 us (10.8 MB, 1.6 at the rate of a copy); 13
+// minimum and maximum are taken two bfloat16 numbers at a time and quotients are products (Kv4Coder; bfloat16
+// numbers make ties common).  2,048 tokens of 8 heads of 128: 5.1 us (10.8 MB, 1.6 at the rate of a copy); 13
 // tokens 2.1, the launch and one round trip.
 template <int D, bool VEC>
 __global__ void __launch_bounds__(KS_THREADS)
@@ -69,31 +61,22 @@ kv4_store_kernel(const __nv_bfloat16* __restrict__ k, long long k_stride,
     if (l == 0) atomicOr(err, BF_ERR_SLOT);
     return;
   }
-  const float lo = __bfloat162float(__hmin_nan(lo2.x, lo2.y)), hi = __bfloat162float(__hmax_nan(hi2.x, hi2.y));
-  const bool finite = hi < INFINITY && lo > -INFINITY;      // (NaN: neither)
-  const __nv_bfloat16 sb = finite ? __float2bfloat16_rn((hi * 0.25f - lo * 0.25f) / 3.75f) : __ushort_as_bfloat16(0x7fc0);
-  const __nv_bfloat16 mb = finite ? __float2bfloat16_rn(lo) : sb;
-  const float s = __bfloat162float(sb);
+  const Kv4Coder coder(__hmin_nan(lo2.x, lo2.y), __hmax_nan(hi2.x, hi2.y));
   unsigned code[2] = {0u, 0u};
-  if (s >= 1e-30f && hi - lo < 3e38f) {
-    // c: the product with 1 / s to the nearest, which is within one of it; the exact remainder says
-    // whether it is the nearest, and of two equally near ones the even one
-    const float inverse = __fdividef(1.f, s), half = 0.5f * s, below = __uint_as_float(__float_as_uint(half) - 1u);
+  if (coder.quick) {
     float sum[4] = {0.f, 0.f, 0.f, 0.f};                    // four codes each, as a whole number
 #pragma unroll
     for (int j = 15; j >= 0; --j) {
       const float x = j & 1 ? __uint_as_float(raw[j >> 1] & 0xffff0000u) : __uint_as_float(raw[j >> 1] << 16);
-      const float y = x - lo, u = fmaf(y, inverse, 12582912.f), c = u - 12582912.f, left = fmaf(-c, s, y);
-      const float limit = __float_as_uint(u) & 1u ? below : half;
-      sum[j >> 2] = fmaf(16.f, sum[j >> 2], fabsf(left) > limit ? c + copysignf(1.f, left) : c);
+      sum[j >> 2] = fmaf(16.f, sum[j >> 2], coder.quick_code(x));
     }
     code[0] = (unsigned)sum[0] | (unsigned)sum[1] << 16;
     code[1] = (unsigned)sum[2] | (unsigned)sum[3] << 16;
-  } else if (finite) {
+  } else if (coder.finite) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
       const float x = j & 1 ? __uint_as_float(raw[j >> 1] & 0xffff0000u) : __uint_as_float(raw[j >> 1] << 16);
-      code[j >> 3] |= ks_code(x, lo, s) << (4 * (j & 7));
+      code[j >> 3] |= kv4_any_code(x, coder.lo, coder.s) << (4 * (j & 7));
     }
   }
   const int h = i / NG, g = i % NG, tok = slot % KV4_EIGHTH;
@@ -107,8 +90,7 @@ kv4_store_kernel(const __nv_bfloat16* __restrict__ k, long long k_stride,
     *reinterpret_cast<uint2*>(rec + tok * (D / 2) + l * (D / 8) + g * 8) = make_uint2(code[0], code[1]);
   }
   if (l == 0)
-    *reinterpret_cast<unsigned*>(rec + (is_v ? kv4_value_params_at(D) : kv4_key_params_at(D)) + (tok * NG + g) * 4) =
-        (unsigned)__bfloat16_as_ushort(sb) | (unsigned)__bfloat16_as_ushort(mb) << 16;
+    *reinterpret_cast<unsigned*>(rec + (is_v ? kv4_value_params_at(D) : kv4_key_params_at(D)) + (tok * NG + g) * 4) = coder.pair;
 }
 
 struct Kv4StoreCall {

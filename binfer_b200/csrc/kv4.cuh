@@ -36,6 +36,41 @@ __host__ __device__ constexpr int kv4_value_byte(int d, int tok, int i) {
 __device__ __forceinline__ float kv4_scale(unsigned pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float kv4_low(unsigned pair) { return __uint_as_float(pair & 0xffff0000u); }
 
+// The code of a number, whatever its size: on x / 4, which is exact, so that no difference of finite numbers
+// overflows.  x - m and s are short enough that the float quotient falls on the side of a border that
+// the exact one falls on.
+static __device__ __noinline__ unsigned kv4_any_code(float x, float lo, float s) {
+  return s > 0.f ? (unsigned)fminf(rintf((x * 0.25f - lo * 0.25f) / (s * 0.25f)), 15.f) : 0u;
+}
+
+// The codes of a group's numbers, from its extremes (NaN if one of them is).  As a rule (`quick`) the quotient is a
+// product with 1 / s put right by its remainder; only where s or the range leaves the ordinary floats is it
+// computed as above.
+struct Kv4Coder {
+  float lo, s, inverse, half, below;
+  unsigned pair;                           // (s, m) as stored
+  bool finite, quick;
+  __device__ __forceinline__ Kv4Coder(__nv_bfloat16 lowest, __nv_bfloat16 highest) {
+    lo = __bfloat162float(lowest);
+    const float hi = __bfloat162float(highest);
+    finite = hi < INFINITY && lo > -INFINITY;               // (NaN: neither)
+    const __nv_bfloat16 sb =
+        finite ? __float2bfloat16_rn((hi * 0.25f - lo * 0.25f) / 3.75f) : __ushort_as_bfloat16(0x7fc0);
+    const __nv_bfloat16 mb = finite ? __float2bfloat16_rn(lo) : sb;
+    pair = (unsigned)__bfloat16_as_ushort(sb) | (unsigned)__bfloat16_as_ushort(mb) << 16;
+    s = __bfloat162float(sb);
+    quick = s >= 1e-30f && hi - lo < 3e38f;
+    inverse = __fdividef(1.f, s), half = 0.5f * s, below = __uint_as_float(__float_as_uint(half) - 1u);
+  }
+  // quick: the product with 1 / s to the nearest, which is within one of it; the exact remainder says
+  // whether it is the nearest, and of two equally near ones the even one
+  __device__ __forceinline__ float quick_code(float x) const {
+    const float y = x - lo, u = fmaf(y, inverse, 12582912.f), c = u - 12582912.f, left = fmaf(-c, s, y);
+    const float limit = __float_as_uint(u) & 1u ? below : half;
+    return fabsf(left) > limit ? c + copysignf(1.f, left) : c;
+  }
+};
+
 // WORDS words at p (aligned as their number allows) by the widest reads.
 template <int WORDS>
 __device__ __forceinline__ void kv4_words(unsigned (&w)[WORDS], const unsigned char* p) {

@@ -1919,6 +1919,7 @@ _kv4_store_call = _Packed("bf_kv4_store", "PqPqPPiiiiqPP")
 _kv4_load_call = _Packed("bf_kv4_load", "PPiiiPiiPPPiPPPiiiiiiiiPP")
 _kv4_rest_call = _Packed("bf_kv4_rest", "PPPPiiPiPPiPqPqiiiiiiifP")
 _kv4_attention_call = _Packed("bf_kv4_attention", "PqPPPPPiiiPiiiPqiiiiiiifPiiPP")
+_qk_norm_rope_kv4_call = _Packed("bf_qk_norm_rope_kv4_store", "PqPPPPPPPiiiiqfPiifPP")
 _step_tables_call = _Packed("bf_step_tables", "PiiPiPiiiPPPPPiPiPiPiPP")
 _prefill_attention_umma2_half_call = _Packed("bf_prefill_attention_umma2_half", "PPPPiiiPiPiiiiiifiPPPqfiPP")
 
@@ -1946,6 +1947,59 @@ def kv4_store(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: torc
         return
     _run("kv4_store", _kv4_store_call, k.data_ptr(), k_stride, v.data_ptr(), v_stride, slots.data_ptr(),
          cache.data_ptr(), T, nkv, d, ps, pages * ps, err.data_ptr(), _stream_at(cache))
+
+
+_token_rows: dict = {}
+
+
+def token_rows(n: int, device) -> torch.Tensor:
+    """int32 0 .. n - 1, kept for good (captured steps read it): the slots of rows as one-token pages."""
+    size = max(64, 1 << (n - 1).bit_length())
+    got = _token_rows.get((device, size))
+    if got is None:
+        got = _token_rows[(device, size)] = torch.arange(size, dtype=torch.int32, device=device)
+    return got[:n]
+
+
+def qk_norm_rope_kv4_store(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w: Optional[torch.Tensor],
+                           inv_freq: Optional[torch.Tensor], positions: torch.Tensor, slots: torch.Tensor,
+                           q_out: torch.Tensor, cache: torch.Tensor, nh: int, nkv: int, d: int, eps: float,
+                           err: torch.Tensor, row_scale: Optional[RowScale] = None) -> None:
+    """``qk_norm_rope_kv_write`` into a cache in 4 bits (``kv4_cache``): per-head RMSNorm of q and k, rotation,
+    q to ``q_out [T, nh * d]``, k and v, rounded to bfloat16, into the pages at ``slots`` as ``kv4_store`` does.
+    One kernel for heads of 128 that are turned whole, two for others."""
+    what = "qk_norm_rope_kv4_store"
+    if (qkv.dim() != 2 or qkv.dtype != torch.bfloat16 or qkv.stride(1) != 1 or q_out.dtype != torch.bfloat16
+            or not q_out.is_contiguous() or qkv.shape[1] != (nh + 2 * nkv) * d
+            or q_out.numel() != qkv.shape[0] * nh * d):
+        raise KernelError(f"{what}: qkv bfloat16 [T, (heads + 2 kv heads) d] with contiguous rows, q_out [T, heads * d]")
+    _want(positions, torch.int32, "positions"); _want(slots, torch.int32, "slots"); _want(err, torch.int32, "err")
+    pages, c_nkv, ps, c_d = _kv4_check(what, cache, qkv, q_w, k_w, inv_freq, positions, slots, q_out, err)
+    T, stride = qkv.shape[0], qkv.stride(0)
+    if c_nkv != nkv or c_d != d or positions.numel() < T or slots.numel() != T:
+        raise KernelError(f"{what}: the cache has {c_nkv} heads of {c_d}, the call names {nkv} of {d}; a position and a "
+                          "slot per token")
+    for w, name, n in ((q_w, "q_w", d), (k_w, "k_w", d), (inv_freq, "inv_freq", 0)):
+        if w is not None and (w.dtype != torch.float32 or not w.is_contiguous() or (w.numel() != n if n else 2 * w.numel() > d)):
+            raise KernelError(f"{what}: {name} must be contiguous float32 of {n or 'at most half the head'} numbers")
+    if T == 0:
+        return
+    address = lambda t: t.data_ptr() if t is not None else 0
+    weights = address(q_w), address(k_w), address(inv_freq)
+    if (d == 128 and inv_freq is not None and inv_freq.numel() == 64 and stride % 4 == 0 and qkv.data_ptr() % 8 == 0
+            and q_out.data_ptr() % 8 == 0 and not any(w % 16 for w in weights)):
+        _row_scale_args(row_scale, T)
+        part, count, width, rs_eps = ((row_scale.partials.data_ptr(), row_scale.partials.shape[1], row_scale.width,
+                                       row_scale.eps) if row_scale is not None else (0, 0, 0, 0.0))
+        _run(what, _qk_norm_rope_kv4_call, qkv.data_ptr(), stride, *weights, positions.data_ptr(), slots.data_ptr(),
+             q_out.data_ptr(), cache.data_ptr(), T, nh, nkv, ps, pages * ps, eps, part, count, width, rs_eps,
+             err.data_ptr(), _stream_at(qkv))
+        return
+    # rows of bfloat16 (a cache of one-token pages), then those into the pages
+    k, v = torch.empty((2, T, nkv, 1, d), dtype=torch.bfloat16, device=qkv.device)
+    qk_norm_rope_kv_write(qkv, q_w, k_w, inv_freq, positions, token_rows(T, qkv.device), q_out, k, v, nh, nkv, d, eps,
+                          err, row_scale=row_scale)
+    kv4_store(k.view(T, nkv * d), v.view(T, nkv * d), slots, cache, err)
 
 
 def kv4_load(cache: torch.Tensor, block_tables: torch.Tensor, items: torch.Tensor, n_items: int,

@@ -13,6 +13,7 @@
 // place is `slot = page * page_size + slot_in_page`, given per token; a negative
 // slot means "do not write".
 #include "common.cuh"
+#include "kv4.cuh"
 
 template <typename A>
 __global__ void qk_norm_rope_kv_write_kernel(
@@ -84,6 +85,10 @@ __global__ void qk_norm_rope_kv_write_kernel(
 // each warp then walks its heads, lane l holding elements 4l..4l+3, whose rotation partners
 // sit in lane l ^ 16.  With few tokens every warp has one head: the kernel is then two
 // dependent round trips long (position, then the head's values) instead of one per head.
+//
+// FOUR: keys and values go into pages held in 4 bits (kv4.cuh; k_cache is the pages of both).  A group's 64 numbers
+// lie in sixteen lanes, which find its extremes in four steps; a lane's four codes are two bytes.
+template <bool FOUR>
 __global__ void qk_norm_rope_kv_write_d128_kernel(
     const __nv_bfloat16* __restrict__ qkv, long long row_stride, const float* __restrict__ q_w,
     const float* __restrict__ k_w, const float* __restrict__ inv_freq,
@@ -94,8 +99,9 @@ __global__ void qk_norm_rope_kv_write_d128_kernel(
   constexpr int D = 128;
   __shared__ float sn_s[64], cs_s[64];
   BF_TRACE_POINT(10 * BF_TR_QKNORM);
-  bf_pdl_trigger();
+  if (!FOUR) bf_pdl_trigger();
   bf_pdl_wait();
+  if (FOUR) bf_pdl_trigger();
   BF_TRACE_POINT(10 * BF_TR_QKNORM + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int t = blockIdx.x;
@@ -186,7 +192,37 @@ __global__ void qk_norm_rope_kv_write_d128_kernel(
       continue;
     }
     const int h = is_k ? hh - nh : hh - nh - nkv;
-    *reinterpret_cast<uint2*>((is_k ? k_cache : v_cache) + kv_base + (size_t)h * kv_head) = o;
+    if constexpr (FOUR) {
+      __nv_bfloat162 lo = __hmin2_nan(o2[0], o2[1]), hi = __hmax2_nan(o2[0], o2[1]);
+#pragma unroll
+      for (int m = 8; m; m >>= 1) {
+        lo = __hmin2_nan(lo, __shfl_xor_sync(0xffffffffu, lo, m));
+        hi = __hmax2_nan(hi, __shfl_xor_sync(0xffffffffu, hi, m));
+      }
+      const Kv4Coder coder(__hmin_nan(lo.x, lo.y), __hmax_nan(hi.x, hi.y));
+      const float2 y0 = __bfloat1622float2(o2[0]), y1 = __bfloat1622float2(o2[1]);
+      const float y[4] = {y0.x, y0.y, y1.x, y1.y};
+      unsigned codes = 0u;
+      if (coder.quick) {
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 3; j >= 0; --j) sum = fmaf(16.f, sum, coder.quick_code(y[j]));
+        codes = (unsigned)sum;
+      } else if (coder.finite) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) codes |= kv4_any_code(y[j], coder.lo, coder.s) << (4 * j);
+      }
+      unsigned char* rec = reinterpret_cast<unsigned char*>(k_cache) +
+                           (((size_t)page * nkv + h) * (page_size / KV4_EIGHTH) + off / KV4_EIGHTH) * kv4_record(D);
+      const int tok = off % KV4_EIGHTH;
+      *reinterpret_cast<unsigned short*>(
+          rec + (is_k ? kv4_key_byte(D, tok, lane * 4) : kv4_value_byte(D, tok, lane * 4))) = (unsigned short)codes;
+      if ((lane & 15) == 0)
+        *reinterpret_cast<unsigned*>(rec + (is_k ? kv4_key_params_at(D) : kv4_value_params_at(D)) +
+                                     (tok * 2 + (lane >> 4)) * 4) = coder.pair;
+    } else {
+      *reinterpret_cast<uint2*>((is_k ? k_cache : v_cache) + kv_base + (size_t)h * kv_head) = o;
+    }
     }
   }
 }
@@ -217,7 +253,7 @@ BF_EXPORT int bf_qk_norm_rope_kv_write(
     // heads' arithmetic: a variant with eight elements a lane and two heads a warp executed
     // 10.4 M and, with fewer warps resident, took 21.6 us.
     const int parts = T <= 64 ? (total * 32 + block - 1) / block : 1;
-    return bf_launch_pdl(qk_norm_rope_kv_write_d128_kernel, dim3(T, parts), dim3(block), 0,
+    return bf_launch_pdl(qk_norm_rope_kv_write_d128_kernel<false>, dim3(T, parts), dim3(block), 0,
                          stream, (const __nv_bfloat16*)qkv,
                          row_stride, q_w, k_w, inv_freq, positions, slots, (__nv_bfloat16*)q_out,
                          (__nv_bfloat16*)k_cache, (__nv_bfloat16*)v_cache, nh, nkv, page_size,
@@ -236,6 +272,40 @@ BF_EXPORT int bf_qk_norm_rope_kv_write(
         (__nv_bfloat16*)q_out, (__nv_bfloat16*)k_cache, (__nv_bfloat16*)v_cache, nh, nkv, d,
         page_size, num_slots, eps, rs, err);
   return bf_launch_status();
+}
+
+// The same into pages held in 4 bits: bfloat16, heads of 128 turned whole, every address a multiple of its loads'
+// size; cudaErrorInvalidValue otherwise (nothing launched).
+struct QkNormRopeKv4Call {
+  const void* qkv;
+  long long row_stride;
+  const float* q_w, *k_w, *inv_freq;
+  const int* positions, *slots;
+  void* q_out;
+  void* cache;
+  int T, nh, nkv, page_size;
+  long long num_slots;
+  float eps;
+  const float* row_partials;
+  int row_count, row_width;
+  float row_eps;
+  int* err;
+  cudaStream_t stream;
+};
+BF_EXPORT int bf_qk_norm_rope_kv4_store(const QkNormRopeKv4Call* call) {
+  const auto& [qkv, row_stride, q_w, k_w, inv_freq, positions, slots, q_out, cache, T, nh, nkv, page_size, num_slots,
+               eps, row_partials, row_count, row_width, row_eps, err, stream] = *call;
+  if (T <= 0) return 0;
+  const BfRowScale rs = {row_partials, row_count, row_width > 0 ? 1.f / (float)row_width : 0.f, row_eps};
+  if (!cache || !inv_freq || row_stride % 4 || ((uintptr_t)qkv & 7) || ((uintptr_t)q_out & 7) || ((uintptr_t)cache & 15) ||
+      ((uintptr_t)inv_freq & 15) || ((uintptr_t)q_w & 15) || ((uintptr_t)k_w & 15) || page_size < 8 || page_size % 8)
+    return (int)cudaErrorInvalidValue;
+  const int total = nh + 2 * nkv, block = total >= 16 ? 256 : 128;
+  const int parts = T <= 64 ? (total * 32 + block - 1) / block : 1;
+  return bf_launch_pdl(qk_norm_rope_kv_write_d128_kernel<true>, dim3(T, parts), dim3(block), 0, stream,
+                       (const __nv_bfloat16*)qkv, row_stride, q_w, k_w, inv_freq, positions, slots,
+                       (__nv_bfloat16*)q_out, (__nv_bfloat16*)cache, (__nv_bfloat16*)nullptr, nh, nkv, page_size,
+                       num_slots, eps, rs, err);
 }
 
 BF_TRACE_READER(bf_trace_read_qkv_post)

@@ -12,8 +12,8 @@ kernel; and every key, also those of the step's own tokens, is read from the
 pages, so a prompt can be cut into portions anywhere and portions can share a
 step with decoded tokens (the reference's prefill ignores the cache, :1082-1086).
 An optional window restricts a query at p to keys in (p - window, p].  Where the engine holds
-its cache in 4 bits (``BuildEnv.kv_cache``), keys and values pass a second kernel into the pages
-and the attention kernels read the codes.  Changes to
+its cache in 4 bits (``BuildEnv.kv_cache``), that kernel writes codes and the attention kernels read
+them.  Changes to
 the scores before the softmax (``AttentionSpec.score``: a soft cap, a bias per
 distance, a sink logit per head) are not Qwen3's; a spec that names one gets the
 generic attention kernel, which applies them, in both precisions.
@@ -41,18 +41,6 @@ from .linear import cluster_token_limit, linear
 FUSE_QKV = os.environ.get("BINFER_B200_FUSE_QKV", "0") != "0"
 # ... and only where those tiles give work to this share of the SMs
 FUSE_QKV_FILL = 0.6
-
-
-_each_of: dict = {}
-
-
-def _each(n: int, device) -> torch.Tensor:
-    """int32 0 .. n - 1, kept for good: captured steps read it."""
-    size = max(64, 1 << (n - 1).bit_length())
-    got = _each_of.get((device, size))
-    if got is None:
-        got = _each_of[(device, size)] = torch.arange(size, dtype=torch.int32, device=device)
-    return got[:n]
 
 
 class GQAAttention(Mixer):
@@ -198,19 +186,21 @@ class GQAAttention(Mixer):
                                       ctx.err)
 
     def _encode_four_bits(self, qkv, q, row_scale, ctx: StepContext, view: EntryView) -> None:
-        """Head norms and position encoding with the keys and values into rows of bfloat16 (a
-        cache of one-token pages), and those into the pages in 4 bits."""
+        """Head norms, position encoding and the store into pages held in 4 bits."""
         s, T, pos = self.spec, qkv.shape[0], self.position
+        slots = ctx.slots[view.group]
+        if pos is None or pos.inv_freq is not None:
+            ops.qk_norm_rope_kv4_store(
+                qkv, self.q_norm, self.k_norm, pos.inv_freq if pos is not None else None, ctx.positions, slots, q,
+                view.k_cache, s.num_heads, s.num_kv_heads, s.head_dim, s.qk_norm_eps, ctx.err, row_scale=row_scale)
+            return
+        # another position encoding: on rows of keys and values (a cache of one-token pages)
         kv = torch.empty((2, T, s.num_kv_heads, 1, s.head_dim), dtype=q.dtype, device=q.device)
-        each = _each(T, q.device)
-        ops.qk_norm_rope_kv_write(
-            qkv, self.q_norm, self.k_norm, pos.inv_freq if pos is not None else None, ctx.positions, each, q,
-            kv[0], kv[1], s.num_heads, s.num_kv_heads, s.head_dim, s.qk_norm_eps, ctx.err, row_scale=row_scale)
-        if pos is not None and pos.inv_freq is None:
-            pos.apply(q.view(T, s.num_heads, s.head_dim), kv[0].view(T, s.num_kv_heads, s.head_dim),
-                      ctx.positions)
-        ops.kv4_store(kv[0].view(T, self.kv_size), kv[1].view(T, self.kv_size), ctx.slots[view.group],
-                      view.k_cache, ctx.err)
+        ops.qk_norm_rope_kv_write(qkv, self.q_norm, self.k_norm, None, ctx.positions, ops.token_rows(T, q.device), q,
+                                  kv[0], kv[1], s.num_heads, s.num_kv_heads, s.head_dim, s.qk_norm_eps, ctx.err,
+                                  row_scale=row_scale)
+        pos.apply(q.view(T, s.num_heads, s.head_dim), kv[0].view(T, s.num_kv_heads, s.head_dim), ctx.positions)
+        ops.kv4_store(kv[0].view(T, self.kv_size), kv[1].view(T, self.kv_size), slots, view.k_cache, ctx.err)
 
     def _attend_four_bits(self, q, out, ctx: StepContext, view: EntryView) -> None:
         s = self.spec

@@ -181,3 +181,16 @@ def test_numbers_that_an_argument_has_no_room_for():
     from binfer_b200.csrc import ops
     with pytest.raises(ops.KernelError, match="no room"):
         ops._Packed("bf_kv4_store", "i")(1 << 40)
+
+
+@pytest.mark.parametrize("change", [dict(nkv=1), dict(d=64), dict(nh=3), dict(qkv=torch.zeros((3, 1024))),
+                                    dict(qkv=torch.zeros((3, 2048), dtype=BF16)[:, ::2]), dict(slots=_i(2)), dict(positions=_i(2)),
+                                    dict(q_w=torch.zeros(64)), dict(inv_freq=torch.zeros(65)), dict(k_w=torch.zeros(128, dtype=BF16)),
+                                    dict(q_out=torch.zeros((3, 256), dtype=BF16)), dict(slots=torch.zeros(3))])
+def test_norm_rotation_and_store_refusals(ops, change, monkeypatch):
+    monkeypatch.setattr(ops, "_same_device", lambda *a: None)
+    args = dict(qkv=torch.zeros((3, 1024), dtype=BF16), q_w=torch.zeros(128), k_w=torch.zeros(128), inv_freq=torch.zeros(64),
+                positions=_i(3), slots=_i(3), q_out=torch.zeros((3, 512), dtype=BF16),
+                cache=torch.zeros((2, 2, 2, 1152), dtype=torch.uint8), nh=4, nkv=2, d=128, eps=1e-6, err=_i(1))
+    with pytest.raises(ops.KernelError):
+        ops.qk_norm_rope_kv4_store(**dict(args, **change))

@@ -188,6 +188,42 @@ def test_load_flags_pages_and_rows_that_do_not_fit(cuda_device):
     assert int(c.err.item()) == 16
 
 
+@pytest.mark.parametrize("T,nh,nkv,d,ps,rot,norms,scaled", [
+    (1, 32, 8, 128, 16, 64, True, False), (1, 2, 2, 128, 8, 64, False, True), (65, 16, 8, 128, 64, 64, True, True),
+    (700, 4, 2, 128, 16, 64, True, False), (33, 6, 3, 128, 128, 32, True, False), (17, 4, 4, 64, 32, 32, True, True),
+    (40, 3, 1, 256, 16, 0, False, False)])
+def test_norm_rotation_and_store_in_one(cuda_device, T, nh, nkv, d, ps, rot, norms, scaled):
+    """The same bits as head norms and rotation into rows of bfloat16, and those stored."""
+    from binfer_b200.csrc import ops
+    dev = cuda_device
+    g = torch.Generator(dev).manual_seed(T)
+    width = (nh + 2 * nkv) * d
+    qkv = torch.randn((T, width + 64), generator=g, device=dev).to(BF16)[:, :width]
+    w = [torch.rand(d, generator=g, device=dev) + 0.5 if norms else None for _ in range(2)]
+    freq = 10000.0 ** (-torch.arange(rot, device=dev) / max(rot, 1)) if rot else None
+    scale = ops.RowScale(torch.rand((T, 3), generator=g, device=dev) + 0.1, 5, 1e-6) if scaled else None
+    positions = torch.randint(0, 9000, (T,), generator=g, device=dev, dtype=I32)
+    pages = -(-T // ps) + 2
+    slots = torch.randperm(pages * ps, generator=g, device=dev)[:T].to(I32)
+    if T > 20:
+        qkv[3, nh * d + 5], qkv[4, -3], qkv[5, nh * d:], qkv[6, -d:-d + 64] = math.inf, math.nan, 0, 3e38
+        qkv[7, -d::2], qkv[8, -d:] = -3e38, 1e-38
+        slots[9], slots[10] = -1, pages * ps
+    want_q, got_q = torch.empty((2, T, nh * d), dtype=BF16, device=dev)
+    k, v = torch.zeros((2, T, nkv, 1, d), dtype=BF16, device=dev)
+    want, got = ops.kv4_cache(pages, nkv, ps, d, dev), ops.kv4_cache(pages, nkv, ps, d, dev)
+    err, err2 = _err(dev), _err(dev)
+    ops.qk_norm_rope_kv_write(qkv, w[0], w[1], freq, positions, torch.arange(T, dtype=I32, device=dev), want_q, k, v,
+                              nh, nkv, d, 1e-6, err, row_scale=scale)
+    ops.kv4_store(k.flatten(1), v.flatten(1), slots, want, err)
+    n = ops.launches()
+    ops.qk_norm_rope_kv4_store(qkv, w[0], w[1], freq, positions, slots, got_q, got, nh, nkv, d, 1e-6, err2, row_scale=scale)
+    assert ops.launches() - n == (1 if d == 128 and rot == 64 else 2)
+    assert got_q.view(torch.int16).equal(want_q.view(torch.int16)) and int(err.item()) == int(err2.item()) == (2 if T > 20 else 0)
+    assert torch.equal(got, want)
+    assert T < 21 or got.any()
+
+
 # ------------------------------------------------------------------------------ attention
 def _attention(c, q, out, nh, jobs, decode, window, keep, scale):
     """``jobs``: (request, rows, first position)."""
