@@ -127,8 +127,13 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r = lane >> 2, q4 = lane & 3;
   const int pairs = a.nkv * a.chunks;
-  bf_pdl_wait();
-  bf_pdl_trigger();
+  // The step's description (rows, positions, requests, tables) is there before the kernel ahead is, so it is read
+  // under that kernel's end.  What waits: queries, pages, whatever is written.  The successor is asked for
+  // after the wait: its blocks, resident any earlier, slow down what runs ahead of this kernel.
+  auto begin = [] {
+    bf_pdl_wait();
+    bf_pdl_trigger();
+  };
 
   auto tile_of = [&](int id, bool flag) {
     KaTile t;
@@ -165,8 +170,6 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
     tiles[e] = t;
     const int n = ka_span(t, a.window, a.keep).units;
     units_of[e] = n;
-    if (n == 0 && blockIdx.x == 0)
-      for (int i = 0; i < pairs; ++i) a.desc[e * pairs + i] = make_int4(-1, -1, 0, 0);
   }
   __syncthreads();
   int total = 0, filled = 0, longest = 0;
@@ -178,7 +181,6 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   total = __reduce_add_sync(0xffffffffu, total) * pairs;
   filled = __reduce_add_sync(0xffffffffu, filled) * pairs;
   longest = __reduce_max_sync(0xffffffffu, longest);
-  if (total == 0) return;
   // Short stretches: a tile's heads together get pieces in proportion to their units, one each at least.
   // With `rate` pieces a unit that makes at most rate total + heads of them: warp w tries a rate, and
   // the highest that gives every piece a warp of its own is taken.
@@ -222,6 +224,13 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
     if (lane == 0) start[a.n_tiles] = before;
   }
   __syncthreads();
+  begin();
+  if (blockIdx.x == 0)
+#pragma unroll 1
+    for (int e = tid; e < a.n_tiles; e += 32 * WARPS)
+      if (units_of[e] == 0)
+        for (int i = 0; i < pairs; ++i) a.desc[e * pairs + i] = make_int4(-1, -1, 0, 0);
+  if (total == 0) return;
   me = warp * gridDim.x + blockIdx.x;                       // (few stretches lie on as many SMs)
   x = me, x_end = me + 1;                                   // pieces: one
   if (!aligned) {
@@ -248,6 +257,7 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
     if constexpr (HEAD) {
       e = blockIdx.x / pairs, pair = blockIdx.x - e * pairs;
       t = tile_of(e, pair == 0 && tid == 0);
+      begin();
       if (t.ntok <= 0) return;
       span = ka_span(t, a.window, a.keep);
       const int steps = (span.units + 1) >> 1, few = steps / WARPS, more = steps % WARPS;
