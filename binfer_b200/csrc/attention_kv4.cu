@@ -27,8 +27,9 @@
 // only when a score passes it by 2^8, which no result depends on beyond rounding and which leaves one
 // vote a step where maxima would take shuffles.
 //
-// Where the tables have room for few keys only and heads for one wave of blocks (ka_by_head), a block takes a
-// tile and head whole, its warps leave their partials in shared memory and add them up there: no second kernel.
+// Where there are few heads, or the tables have room for few keys only (ka_blocks_a_head), a cluster of one to
+// eight blocks takes a tile and head whole: its warps leave their partials in shared memory, each block adds up its
+// own and the blocks theirs over distributed shared memory, and there is no second kernel.
 //
 // Measured (B200).  64 rows of 64 heads of 128 (8) behind 4,096 keys down to 2,700: 55 us and 5 for the second
 // kernel, where the 254 MB take 39 at the rate of a copy, 6.54 TB/s.  While all warps run they read 6.2 TB/s:
@@ -46,6 +47,8 @@
 #define KA_UNIT 16                         // keys
 #define KA_MIN_UNITS 2                     // a stretch's length at least
 #define KA_LONG 24                         // units of a stretch from which heads are crossed
+#define KA_PIECES 30.f                     // a head of U units gets sqrt(30 U) pieces at most
+#define KA_SHARE 8                         // blocks of a cluster at most
 #define KA_BEGIN 6                         // units that a warp could compute while it begins a head
 
 // Warps of a CTA, one CTA an SM: sixteen where 128 registers hold a tile.
@@ -65,7 +68,7 @@ struct KaArgs {
   int page_size, page_shift, num_pages, window, keep;
   float scale;
   unsigned chunk_inverse;                                  // n / chunk = n chunk_inverse >> 8 for n < 16
-  int max_pieces;
+  int max_pieces, share;
   float* part_o;
   float2* part_ml;
   int4* desc;
@@ -108,7 +111,19 @@ template <bool B>
 struct Bool {
   static constexpr bool value = B;
 };
-// HEAD: block b takes (tile, head) b whole; its warps share the units and add up in shared memory.
+__device__ __forceinline__ void ka_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// A number of another block's shared memory, where this block has its own at p.
+__device__ __forceinline__ float ka_peer(const float* p, int rank) {
+  unsigned at;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((unsigned)__cvta_generic_to_shared(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+// HEAD: a cluster of a.share blocks takes a (tile, head) whole; its warps share the units and add up in
+// shared memory.
 template <int D, int NT, bool HEAD>
 __global__ void __launch_bounds__(32 * ka_warps(D, NT), 1)
 kv4_attention_kernel(const __grid_constant__ KaArgs a) {
@@ -183,13 +198,14 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   longest = __reduce_max_sync(0xffffffffu, longest);
   // Short stretches: a tile's heads together get pieces in proportion to their units, one each at least.
   // With `rate` pieces a unit that makes at most rate total + heads of them: warp w tries a rate, and
-  // the highest that gives every piece a warp of its own is taken.
+  // the highest that gives every piece a warp of its own is taken.  Not too many of a head, which the second kernel
+  // adds up: a head's 2,048 units in 1,024 pieces took 33 us, in 248 19.
   aligned = total < KA_LONG * warps && filled < warps;
   float rate = 0.f;
   if (aligned) {
     auto rate_of = [&](int i) {
       const float room = warps - filled * (i * (1.f / (WARPS - 1)));
-      return fminf(1.f / KA_MIN_UNITS, fmaxf(room, 0.f) / total);
+      return fminf(fminf(1.f / KA_MIN_UNITS, sqrtf(KA_PIECES / longest)), fmaxf(room, 0.f) / total);
     };
     rate = rate_of(warp);
   }
@@ -255,15 +271,16 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
     KaTile t;
     KaSpan span;
     if constexpr (HEAD) {
-      e = blockIdx.x / pairs, pair = blockIdx.x - e * pairs;
-      t = tile_of(e, pair == 0 && tid == 0);
+      const int head = blockIdx.x / a.share, rank = blockIdx.x - head * a.share;
+      e = head / pairs, pair = head - e * pairs;
+      t = tile_of(e, pair == 0 && rank == 0 && tid == 0);
       begin();
       if (t.ntok <= 0) return;
       span = ka_span(t, a.window, a.keep);
-      const int steps = (span.units + 1) >> 1, few = steps / WARPS, more = steps % WARPS;
-      u0 = 2 * (warp * few + min(warp, more));
-      mine = min(2 * (few + (warp < more ? 1 : 0)), span.units - u0);       // (not below zero where u0 is the end)
-      mine = max(mine, 0), n_pieces = WARPS, x = x_end;
+      const int steps = (span.units + 1) >> 1, all = WARPS * a.share, w = warp * a.share + rank;
+      const int few = steps / all, more = steps - few * all;
+      u0 = 2 * (w * few + min(w, more));
+      mine = max(min(2 * (few + (w < more ? 1 : 0)), span.units - u0), 0), n_pieces = all, x = x_end;
     } else {
     // the tile of x: the last that begins at or before it, among every sixteenth and then among sixteen
     e = lane * 16;
@@ -647,31 +664,85 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
         }
       }
     if constexpr (HEAD) {
-      // a column by one warp, or two warps
-      constexpr int PER = WARPS > COLS ? WARPS / COLS : 1, N = D / PER / 32;
+      // a column by one warp, or two warps, a warp one or two columns
+      constexpr int PER = WARPS > COLS ? WARPS / COLS : 1, N = D / PER / 32, IDS = COLS * PER / WARPS;
+      static_assert(COLS * PER % WARPS == 0, "columns");
       __syncthreads();
-      for (int id = warp; id < COLS * PER; id += WARPS) {
+      float acc[IDS][N], sum[IDS], top[IDS];
+      auto on = [&](int n) {
+        const int ti = n * a.chunk_inverse >> 8;
+        return ti < t.ntok && n - ti * a.chunk < heads;
+      };
+      auto finish = [&](int id, const float (&v)[N], float l) {
         const int n = id / PER, ti = n * a.chunk_inverse >> 8, gi = n - ti * a.chunk;
-        if (ti >= t.ntok || gi >= heads) continue;
+        __nv_bfloat16* dst = a.out + (long long)(t.row0 + ti) * a.out_stride + (size_t)(head0 + gi) * D + id % PER * (D / PER);
+#pragma unroll
+        for (int k = 0; k < N; ++k) dst[lane + 32 * k] = __float2bfloat16_rn(v[k] / l);
+      };
+#pragma unroll
+      for (int j = 0; j < IDS; ++j) {
+        const int id = warp + j * WARPS, n = id / PER;
+        if (!on(n)) continue;
         const float2 ml = lane < WARPS ? part_ml[lane * COLS + n] : make_float2(-INFINITY, 0.f);
-        float top = ml.x;
+        top[j] = ml.x;
 #pragma unroll
-        for (int k = 1; k < WARPS; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-        const float f = ml.x == top ? 1.f : ka_exp2(ml.x - top);
-        float sum = 0.f, acc[N];
+        for (int k = 1; k < WARPS; k <<= 1) top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], k));
+        const float f = ml.x == top[j] ? 1.f : ka_exp2(ml.x - top[j]);
+        sum[j] = 0.f;
 #pragma unroll
-        for (int k = 0; k < N; ++k) acc[k] = 0.f;
+        for (int k = 0; k < N; ++k) acc[j][k] = 0.f;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
           const float g = __shfl_sync(0xffffffffu, f, w);
-          sum = fmaf(g, __shfl_sync(0xffffffffu, ml.y, w), sum);
+          sum[j] = fmaf(g, __shfl_sync(0xffffffffu, ml.y, w), sum[j]);
 #pragma unroll
           for (int k = 0; k < N; ++k)
-            acc[k] = fmaf(g, part_o[(w * COLS + n) * ROW + id % PER * (D / PER) + lane + 32 * k], acc[k]);
+            acc[j][k] = fmaf(g, part_o[(w * COLS + n) * ROW + id % PER * (D / PER) + lane + 32 * k], acc[j][k]);
         }
-        __nv_bfloat16* dst = a.out + (long long)(t.row0 + ti) * a.out_stride + (size_t)(head0 + gi) * D + id % PER * (D / PER);
+        if (a.share == 1) finish(id, acc[j], sum[j]);
+      }
+      if (a.share > 1) {
+        // the blocks' sums, a column by one warp of one of them
+        const int rank = blockIdx.x % a.share;
+        __syncthreads();
 #pragma unroll
-        for (int k = 0; k < N; ++k) dst[lane + 32 * k] = __float2bfloat16_rn(acc[k] / sum);
+        for (int j = 0; j < IDS; ++j) {
+          const int id = warp + j * WARPS, n = id / PER;
+          if (!on(n)) continue;
+#pragma unroll
+          for (int k = 0; k < N; ++k) part_o[n * D + id % PER * (D / PER) + lane + 32 * k] = acc[j][k];
+          if (id % PER == 0 && lane == 0) part_ml[n] = make_float2(top[j], sum[j]);
+        }
+        ka_cluster_sync();
+#pragma unroll 1
+        for (int id = warp * a.share + rank; id < COLS * PER; id += WARPS * a.share) {
+          const int n = id / PER;
+          if (!on(n)) continue;
+          float m1 = -INFINITY, l1 = 0.f;
+          if (lane < a.share) m1 = ka_peer(&part_ml[n].x, lane), l1 = ka_peer(&part_ml[n].y, lane);
+          float part[KA_SHARE][N];
+#pragma unroll
+          for (int c = 0; c < KA_SHARE; ++c)
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+              part[c][k] = c < a.share ? ka_peer(part_o + n * D + id % PER * (D / PER) + lane + 32 * k, c) : 0.f;
+          float most = m1;
+#pragma unroll
+          for (int k = 1; k < KA_SHARE; k <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, k));
+          const float f = m1 == most ? 1.f : ka_exp2(m1 - most);
+          float l = 0.f, v[N];
+#pragma unroll
+          for (int k = 0; k < N; ++k) v[k] = 0.f;
+#pragma unroll
+          for (int c = 0; c < KA_SHARE; ++c) {
+            const float g = __shfl_sync(0xffffffffu, f, c);
+            l = fmaf(g, __shfl_sync(0xffffffffu, l1, c), l);
+#pragma unroll
+            for (int k = 0; k < N; ++k) v[k] = fmaf(g, part[c][k], v[k]);
+          }
+          finish(id, v, l);
+        }
+        ka_cluster_sync();                                  // (this block's memory may be read until here)
       }
     } else if (u0 == 0 && lane == 0)
       a.desc[e * pairs + pair] = whole ? make_int4(-1, -1, 0, 0) : make_int4(me, n_pieces, t.row0, t.ntok);
@@ -756,7 +827,7 @@ kv4_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ pa
 }
 
 template <int D, int NT>
-static int ka_launch(KaArgs a, int total_tiles, bool by_head, int sms, cudaStream_t stream) {
+static int ka_launch(KaArgs a, int total_tiles, int share, int sms, cudaStream_t stream) {
   constexpr int threads = 32 * ka_warps(D, NT);
   constexpr size_t smem = (size_t)ka_warps(D, NT) * KA_STAGES * 2 * kv4_record(D) +
                           KA_MAX_TILES * (sizeof(KaTile) + 4) + (KA_MAX_TILES + 4) * 4;
@@ -774,8 +845,23 @@ static int ka_launch(KaArgs a, int total_tiles, bool by_head, int sms, cudaStrea
   const long long units = ((long long)a.table_width * a.page_size / KA_UNIT + 2 + KA_BEGIN) * pairs;
   if (units > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
   const int most = 0x7fffffffLL / units < KA_MAX_TILES ? (int)(0x7fffffffLL / units) : KA_MAX_TILES;
-  if (by_head)
-    return bf_launch_pdl(kv4_attention_kernel<D, NT, true>, dim3(total_tiles * pairs), dim3(threads), smem, stream, a);
+  if (share) {
+    a.share = share;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(total_tiles * pairs * share);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = bf_pdl_enabled();
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = share, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_attention_kernel<D, NT, true>, a);
+    return e != cudaSuccess ? (int)e : bf_launch_status();
+  }
   for (int first = 0; first < total_tiles; first += most) {
     a.first_tile = first;
     a.n_tiles = total_tiles - first < most ? total_tiles - first : most;
@@ -813,24 +899,38 @@ static KaShape ka_shape(int group, int d, int max_rows) {
 
 static long long ka_slots(const KaShape& s, int d, int sms) { return 2LL * sms * ka_warps(d, s.nt); }
 
-// Whether every (tile, head) gets a block of its own, whose warps meet in shared memory, rather than stretches
-// of equal work and a second kernel: in one wave of blocks, where few units come on a warp.  `keys`: the most
-// that a tile can see.  Measured for rows of equal length, stretches / blocks in us, replayed from a graph: 8 heads
-// (4 query heads each) of 128 over 512 keys 11.0 / 8.8, 1,024 11.0 / 10.7, 2,048 11.6 / 13.0; 128 heads 14.9 / 8.6,
-// 17.2 / 10.7, 21.0 / 14.7; one head of 16 1,024 12.7 / 12.8; two heads of 256 512 keys 12.2 / 9.9, 1,024 12.7 / 12.7;
-// 192 heads of 128 over 512 keys 17.2 / 13.1, but 384 16.9 / 18.9.  That is, blocks save 5 us and take `unit` us
-// a unit, of which the stretches pay a share that grows with the heads: half of them, as the rows of a batch
-// have different lengths.
-static bool ka_by_head(const KaShape& s, int d, long long heads, int keys, int sms) {
-  const float unit = d == 64 ? (s.nt == 1 ? 0.033f : 0.05f) : d == 128 ? (s.nt == 1 ? 0.056f : 0.088f) : 0.104f;
-  return heads <= sms && (keys / KA_UNIT + 1) * unit * (1.f - 0.5f * heads / sms) < 5.2f;
+// Blocks that each (tile, head) gets for itself, as a cluster whose warps meet in shared memory; 0: stretches of
+// equal work and a second kernel.  `keys`: the most that a tile can see.  The faster by what both take, in us, from a
+// sweep of rows of equal length (replayed from a graph, launch included): a cluster 6.5 (several blocks 8.5) and `unit`
+// for each unit of a block, where all clusters are resident at once (74, 33 and 15 of two, four and eight blocks);
+// stretches `base`, `each` for every unit of all heads, of which a batch has three quarters of what its longest row
+// says, and `piece` for a head's pieces.  Heads of 128 (4 query heads each), stretches / 1, 2, 4, 8 blocks: 8 heads over 512
+// keys 10.7 / 8.6, 8.6, 8.6, 8.6, over 4,096 12.6 / 20.9, 14.8, 12.7, 10.6, over 16,384 19.0 / 62, 36, 23, 15.4; 32 heads over
+// 4,096 16.9 / 20.9, 14.7, 12.7; 72 over 4,096 19.0 / 20.9, 16.3; 128 over 512 14.7 / 8.7, over 4,096 27.2 / 21.0.
+static int ka_blocks_a_head(const KaShape& s, int d, long long tiles, int pairs, int keys, int sms) {
+  struct Times {
+    float unit, base, each, piece;
+  };
+  const Times t = d == 64    ? (s.nt == 1 ? Times{0.033f, 9.2f, 0.5e-3f, 0.011f} : Times{0.05f, 9.5f, 0.8e-3f, 0.011f})
+                  : d == 128 ? (s.nt == 1 ? Times{0.056f, 11.5f, 0.45e-3f, 0.011f} : Times{0.094f, 11.5f, 1.0e-3f, 0.011f})
+                             : Times{0.105f, 12.f, 0.7e-3f, 0.035f};
+  const float units = keys / KA_UNIT + 1, heads = (float)tiles * pairs;
+  const float pieces = fminf(sqrtf(KA_PIECES * units), sms * ka_warps(d, s.nt) / heads);
+  float best = t.base + t.each * units * heads * (tiles > 1 ? 0.75f : 1.f) + t.piece * pieces;
+  int share = 0;
+  for (int c = 1; c <= KA_SHARE; c *= 2) {
+    const int fit = sms * (c < 4 ? 100 : c == 4 ? 90 : 82) / (100 * c);
+    const float time = (c == 1 ? 6.5f : 8.5f) + t.unit * units / c;
+    if (heads <= fit && time < best) best = time, share = c;
+  }
+  return share;
 }
 
 // Bytes of scratch that a call needs (16-byte aligned): partial results and a note per (tile, head); none where
 // no second kernel runs.  `keys` as the call's.
 BF_EXPORT long long bf_kv4_attention_scratch(int n, int max_rows, int nh, int nkv, int d, int sms, int keys) {
   const KaShape s = ka_shape(nh / nkv, d, max_rows);
-  if (ka_by_head(s, d, (long long)n * ((max_rows + s.tokens - 1) / s.tokens) * nkv * s.chunks, keys, sms)) return 0;
+  if (ka_blocks_a_head(s, d, (long long)n * ((max_rows + s.tokens - 1) / s.tokens), nkv * s.chunks, keys, sms)) return 0;
   const long long slots = ka_slots(s, d, sms);
   long long tiles = (long long)n * ((max_rows + s.tokens - 1) / s.tokens);
   if (tiles > KA_MAX_TILES) tiles = KA_MAX_TILES;
@@ -882,10 +982,10 @@ BF_EXPORT int bf_kv4_attention(const Kv4AttentionCall* call) {
   a.err = err;
   const long long tiles = (long long)n * a.tiles_per_item;
   if (tiles > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
-  const bool by_head = ka_by_head(s, d, tiles * nkv * s.chunks, keys, sms);
-  if (!by_head && !scratch) return (int)cudaErrorInvalidValue;
-  if (d == 64) return s.nt == 1 ? ka_launch<64, 1>(a, (int)tiles, by_head, sms, stream) : ka_launch<64, 2>(a, (int)tiles, by_head, sms, stream);
-  if (d == 128) return s.nt == 1 ? ka_launch<128, 1>(a, (int)tiles, by_head, sms, stream) : ka_launch<128, 2>(a, (int)tiles, by_head, sms, stream);
-  if (d == 256) return ka_launch<256, 1>(a, (int)tiles, by_head, sms, stream);
+  const int share = ka_blocks_a_head(s, d, tiles, nkv * s.chunks, keys, sms);
+  if (!share && !scratch) return (int)cudaErrorInvalidValue;
+  if (d == 64) return s.nt == 1 ? ka_launch<64, 1>(a, (int)tiles, share, sms, stream) : ka_launch<64, 2>(a, (int)tiles, share, sms, stream);
+  if (d == 128) return s.nt == 1 ? ka_launch<128, 1>(a, (int)tiles, share, sms, stream) : ka_launch<128, 2>(a, (int)tiles, share, sms, stream);
+  if (d == 256) return ka_launch<256, 1>(a, (int)tiles, share, sms, stream);
   return (int)cudaErrorInvalidValue;
 }
