@@ -68,7 +68,7 @@ struct KaArgs {
   int page_size, page_shift, num_pages, window, keep;
   float scale;
   unsigned chunk_inverse;                                  // n / chunk = n chunk_inverse >> 8 for n < 16
-  int max_pieces, share;
+  int max_pieces, share, early;
   float* part_o;
   float2* part_ml;
   int4* desc;
@@ -142,13 +142,16 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r = lane >> 2, q4 = lane & 3;
   const int pairs = a.nkv * a.chunks;
-  // The step's description (rows, positions, requests, tables) is there before the kernel ahead is, so it is read
-  // under that kernel's end.  What waits: queries, pages, whatever is written.  The successor is asked for
-  // after the wait: its blocks, resident any earlier, slow down what runs ahead of this kernel.
-  auto begin = [] {
+  // Where the step's description (rows, positions, requests, tables) was there before the kernel ahead began
+  // (a.early), it is read under that kernel's end, and queries, pages and all writes wait; else everything waits.
+  // The successor is asked for after the wait: its blocks, resident any earlier, slow down what runs ahead of this
+  // kernel.
+  auto begin = [&](int early) {
+    if (early != a.early) return;
     bf_pdl_wait();
     bf_pdl_trigger();
   };
+  begin(0);
 
   auto tile_of = [&](int id, bool flag) {
     KaTile t;
@@ -240,7 +243,7 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
     if (lane == 0) start[a.n_tiles] = before;
   }
   __syncthreads();
-  begin();
+  begin(1);
   if (blockIdx.x == 0)
 #pragma unroll 1
     for (int e = tid; e < a.n_tiles; e += 32 * WARPS)
@@ -274,7 +277,7 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
       const int head = blockIdx.x / a.share, rank = blockIdx.x - head * a.share;
       e = head / pairs, pair = head - e * pairs;
       t = tile_of(e, pair == 0 && rank == 0 && tid == 0);
-      begin();
+      begin(1);
       if (t.ntok <= 0) return;
       span = ka_span(t, a.window, a.keep);
       const int steps = (span.units + 1) >> 1, all = WARPS * a.share, w = warp * a.share + rank;
@@ -951,13 +954,14 @@ struct Kv4AttentionCall {
   float scale;
   void* scratch;
   int sms, keys;                                           // keys: the most that a row can see, as to the scratch
+  int early;                                               // the description was there before the kernel ahead began
   int* err;
   cudaStream_t stream;
 };
 BF_EXPORT int bf_kv4_attention(const Kv4AttentionCall* call) {
   const auto& [q, q_stride, cache, rows, seq_of_token, positions, items, n, max_rows, T, block_tables,
                table_stride, table_rows, table_width, out, out_stride, nh, nkv, d, page_size, num_pages,
-               window, keep, scale, scratch, sms, keys, err, stream] = *call;
+               window, keep, scale, scratch, sms, keys, early, err, stream] = *call;
   if (n <= 0 || max_rows <= 0) return 0;
   if ((long long)num_pages * nkv * (page_size / 8) > 0x7fffffffLL || page_size < 8 || (page_size & (page_size - 1)) ||
       (long long)table_width * page_size > 1 << 24)        // (a tile's units stay below 2^20)
@@ -974,6 +978,7 @@ BF_EXPORT int bf_kv4_attention(const Kv4AttentionCall* call) {
   a.page_size = page_size, a.page_shift = 3;
   while (1 << a.page_shift < page_size) ++a.page_shift;
   a.num_pages = num_pages, a.window = window, a.keep = keep, a.scale = scale;
+  a.early = early != 0;
   a.chunk_inverse = (256 + s.chunk - 1) / s.chunk;
   const long long slots = ka_slots(s, d, sms);
   a.part_o = (float*)scratch;

@@ -1918,7 +1918,7 @@ class _Packed:
 _kv4_store_call = _Packed("bf_kv4_store", "PqPqPPiiiiqPP")
 _kv4_load_call = _Packed("bf_kv4_load", "PPiiiPiiPPPiPPPiiiiiiiiPP")
 _kv4_rest_call = _Packed("bf_kv4_rest", "PPPPiiPiPPiPqPqiiiiiiifP")
-_kv4_attention_call = _Packed("bf_kv4_attention", "PqPPPPPiiiPiiiPqiiiiiiifPiiPP")
+_kv4_attention_call = _Packed("bf_kv4_attention", "PqPPPPPiiiPiiiPqiiiiiiifPiiiPP")
 _qk_norm_rope_kv4_call = _Packed("bf_qk_norm_rope_kv4_store", "PqPPPPPPPiiiiqfPiifPP")
 _step_tables_call = _Packed("bf_step_tables", "PiiPiPiiiPPPPPiPiPiPiPP")
 _prefill_attention_umma2_half_call = _Packed("bf_prefill_attention_umma2_half", "PPPPiiiPiPiiiiiifiPPPqfiPP")
@@ -2078,13 +2078,16 @@ def _kv4_attention_check(what, q, cache, block_tables, out, nh, nkv, d, window, 
 def kv4_decode_attention(q: torch.Tensor, cache: torch.Tensor, rows: Optional[torch.Tensor], n_rows: int,
                          seq_of_token: torch.Tensor, positions: torch.Tensor, block_tables: torch.Tensor,
                          out: torch.Tensor, nh: int, nkv: int, d: int, window: Optional[int], scale: float,
-                         err: torch.Tensor, keep_first: int = 0) -> None:
+                         err: torch.Tensor, keep_first: int = 0, described: bool = False) -> None:
     """Attention over a cache in 4 bits for rows that bring one token each: ``decode_attention``'s
     arguments, with ``cache`` (``kv4_cache``) in the pages' place.  A row at position p sees the keys
     ``j <= p`` of its request; with ``window`` those with ``j > p - window``, and the first ``keep_first``
     tokens.  ``rows`` lists the token rows to run (None: 0 .. n_rows - 1); other rows of ``out`` are left
     as they were, and so is a listed one whose row, request or position is not there, which sets the error
     word.  A page id outside the pool sets it too and stands for page 0.
+
+    ``described``: rows, requests, positions and tables were complete before the kernel ahead on the stream began
+    (as in a step that is described once and then runs its layers); they are read under that kernel's end.
 
     Queries below 2^62 and values below 2^55 in size: larger ones overflow inside."""
     _want(seq_of_token, torch.int32, "seq_of_token"); _want(positions, torch.int32, "positions")
@@ -2101,19 +2104,20 @@ def kv4_decode_attention(q: torch.Tensor, cache: torch.Tensor, rows: Optional[to
         return
     _kv4_attention(q, cache, rows.data_ptr() if rows is not None else 0, seq_of_token.data_ptr(),
                    positions.data_ptr(), 0, n_rows, 1, block_tables, table, strides, out, nh, nkv, d, ps, pages, w,
-                   keep, scale, err)
+                   keep, scale, err, described)
 
 
 def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Tensor, n_items: int,
                           max_rows: int, block_tables: torch.Tensor, out: torch.Tensor, nh: int, nkv: int,
                           d: int, window: Optional[int], scale: float, err: torch.Tensor, ctx_rows: int,
-                          max_ctx: int, keep_first: int = 0, variant: str = "auto") -> None:
+                          max_ctx: int, keep_first: int = 0, variant: str = "auto", described: bool = False) -> None:
     """Causal attention of prompt portions over a cache in 4 bits, their own keys included:
     ``prefill_attention``'s arguments, with ``cache`` (``kv4_cache``) in the pages' place.  ``ctx_rows``:
     the portions' contexts added up, each rounded up to 64; ``max_ctx``: the longest of them;
     ``keep_first``: with a window, the request's first that many tokens stay visible behind it.  A portion
     whose rows, request or places are not there, or that ``ctx_rows`` and ``max_ctx`` have no room for,
-    sets the error word and its rows are left as they were.  Sizes of numbers: as in ``kv4_decode_attention``.
+    sets the error word and its rows are left as they were.  ``described`` and sizes of numbers: as in
+    ``kv4_decode_attention``.
 
     ``variant``: ``stretches`` (the kernel of single tokens, a few rows at a time; reads the cache as it
     is), ``load`` (a positive scale, q contiguous: the contexts are loaded as ``kv4_load``
@@ -2136,7 +2140,7 @@ def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Ten
                               pages, w, keep, scale, err, ctx_rows, max_ctx)
         return
     _kv4_attention(q, cache, 0, 0, 0, items.data_ptr(), n_items, max_rows, block_tables, table, strides, out, nh,
-                   nkv, d, ps, pages, w, keep, scale, err)
+                   nkv, d, ps, pages, w, keep, scale, err, described)
 
 
 _kv4_scratch: dict = {}     # bytes of scratch by a call's sizes
@@ -2218,7 +2222,7 @@ def _kv4_loaded_attention(q, cache, items, n_items, max_rows, block_tables, tabl
 
 
 def _kv4_attention(q, cache, rows, seq, positions, items, n, max_rows, block_tables, table, strides, out, nh,
-                   nkv, d, ps, pages, window, keep, scale, err) -> None:
+                   nkv, d, ps, pages, window, keep, scale, err, described) -> None:
     global _launches
     device = q.device
     sms = num_sms(device)
@@ -2239,7 +2243,7 @@ def _kv4_attention(q, cache, rows, seq, positions, items, n, max_rows, block_tab
     T, q_stride, out_stride = strides
     _run("kv4_attention", _kv4_attention_call, q.data_ptr(), q_stride, cache.data_ptr(), rows, seq, positions,
          items, n, max_rows, T, block_tables.data_ptr(), table_stride, table_rows, table_width, out.data_ptr(),
-         out_stride, nh, nkv, d, ps, pages, window, keep, scale, scratch.data_ptr() if size else 0, sms, keys,
+         out_stride, nh, nkv, d, ps, pages, window, keep, scale, scratch.data_ptr() if size else 0, sms, keys, described,
          err.data_ptr(), _stream_at(q))
     if size:
         _launches += 1      # two kernels: the stretches of units, and what several of them share

@@ -209,7 +209,7 @@ class GQAAttention(Mixer):
         if ctx.decode_only or ctx.n_decode:
             ops.kv4_decode_attention(q, view.k_cache, None if ctx.decode_only else ctx.decode_rows,
                                      ctx.T if ctx.decode_only else ctx.n_decode, ctx.seq_of_token,
-                                     ctx.positions, *tail)
+                                     ctx.positions, *tail, described=True)
         if ctx.n_prefill:
             rows = ctx.scratch.get("portion_ctx_rows")
             if rows is None:
@@ -217,7 +217,7 @@ class GQAAttention(Mixer):
                     -(-c // ops.KV4_LOAD_PAGE) * ops.KV4_LOAD_PAGE
                     for n, c in zip(ctx.q_lens, ctx.ctx_lens_host) if n > 1)
             ops.kv4_prefill_attention(q, view.k_cache, ctx.prefill_items, ctx.n_prefill, ctx.max_prefill_rows,
-                                      *tail, ctx_rows=rows, max_ctx=ctx.max_ctx_len)
+                                      *tail, ctx_rows=rows, max_ctx=ctx.max_ctx_len, described=True)
 
     def attend(self, q: torch.Tensor, out: torch.Tensor, ctx: StepContext,
                view: EntryView) -> None:

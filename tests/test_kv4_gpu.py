@@ -498,6 +498,54 @@ def test_results_are_the_same_every_time(cuda_device):
     assert all(torch.equal(o, outs[0]) for o in outs)
 
 
+@pytest.mark.usefixtures("tables")
+@pytest.mark.parametrize("rows_new", [1, 5])
+def test_a_chain_of_layers_described_once(cuda_device, rows_new):
+    """Store and attention of several layers in a graph, each reading what the kernel ahead wrote; the rows'
+    description read early or not makes no difference."""
+    from binfer_b200.csrc import ops
+    nh, nkv, d, layers, lens = 8, 2, 128, 6, [700, 70, 2100]
+    c = Cache(lens, nkv, d, 16, cuda_device)
+    T = rows_new * len(lens)
+    slots = torch.cat([c.slots[i][-rows_new:] for i in range(len(lens))])
+    seq = torch.arange(len(lens), device=cuda_device).repeat_interleave(rows_new).to(I32)
+    pos = torch.cat([torch.arange(n - rows_new, n) for n in lens]).to(I32).to(cuda_device)
+    items = torch.tensor([(i, i * rows_new, rows_new, n - rows_new) for i, n in enumerate(lens)], dtype=I32,
+                         device=cuda_device)
+    first = _queries(T, nh, d, cuda_device)
+
+    def run(described):
+        x = first
+        for _ in range(layers):
+            k = x[:, :nkv * d]
+            ops.kv4_store(k, x[:, nkv * d:2 * nkv * d], slots, c.cache, c.err)
+            out = torch.empty_like(x)
+            if rows_new == 1:
+                ops.kv4_decode_attention(x, c.cache, None, T, seq, pos, c.tables, out, nh, nkv, d, None, 0.2, c.err,
+                                         described=described)
+            else:
+                ops.kv4_prefill_attention(x, c.cache, items, len(lens), rows_new, c.tables, out, nh, nkv, d, None, 0.2,
+                                          c.err, ctx_rows=704 + 128 + 2112, max_ctx=2100, described=described)
+            x = out
+        return x
+
+    want = run(False).clone()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        got = run(True)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            got = run(True)
+        for _ in range(20):
+            got.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+    assert int(c.err.item()) == 0 and torch.isfinite(want.float()).all()
+
+
 # ------------------------------------------------------------------------------ a step's description
 def _describe(dev, master, entries, new_pages, ps, num_pages, width, T=None, n_dec=None, n_pf=None, B=None):
     from binfer_b200.csrc import ops
