@@ -157,6 +157,10 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_half + (HALF ? 2 : 0));
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
+  if constexpr (HALF) {                        // (its keys come from the kernel ahead, another looks at its result)
+    bf_pdl_wait();
+    bf_pdl_trigger();
+  }
   // with splits > 1 the keys of a block are shared out over `splits` CTAs, each of which leaves
   // an unnormalised O with its exponent reference and sum for the merge kernel below
   const int split = splits > 1 ? (int)blockIdx.y % splits : 0;
@@ -807,6 +811,8 @@ __global__ void prefill_attention_merge_kernel(const float* __restrict__ part_o,
                                                __nv_bfloat16* __restrict__ out, int nh, int splits,
                                                long long out_stride, float out_scale,
                                                const float* __restrict__ sinks) {
+  bf_pdl_wait();
+  bf_pdl_trigger();
   const int* it = items + 4 * blockIdx.z;
   const int row0 = it[1], qlen = it[2];
   const int r = blockIdx.x * 4 + (threadIdx.x >> 5), h = blockIdx.y, lane = threadIdx.x & 31;
@@ -907,18 +913,30 @@ static int launch_umma2(
   const int rows = d == 256 ? A2_BM : 2 * A2_BM;
   dim3 grid(nh, n_items * splits, (max_rows + rows - 1) / rows);
   if (grid.y > 65535u || grid.z > 65535u) return (int)cudaErrorInvalidValue;
-  kern<<<grid, A2_THREADS, smem, stream>>>(mq, mk, mv, mkr, mvr, items, block_tables, table_stride,
-                                           (__nv_bfloat16*)out, nh, nkv, page_size, num_pages,
-                                           window, scale * log2e, splits, part_o, part_ml, err,
-                                           cap_pre, cap_post, out_stride, out_scale,
-                                           BfDiffArgs(), sinks, keep, beyond);
+  if (beyond) {
+    const int st = bf_launch_pdl(kern, grid, dim3(A2_THREADS), smem, stream, mq, mk, mv, mkr, mvr, items, block_tables,
+                                 table_stride, (__nv_bfloat16*)out, nh, nkv, page_size, num_pages, window,
+                                 scale * log2e, splits, part_o, part_ml, err, cap_pre, cap_post, out_stride, out_scale,
+                                 BfDiffArgs(), sinks, keep, beyond);
+    if (st) return st;
+  } else {
+    kern<<<grid, A2_THREADS, smem, stream>>>(mq, mk, mv, mkr, mvr, items, block_tables, table_stride,
+                                             (__nv_bfloat16*)out, nh, nkv, page_size, num_pages,
+                                             window, scale * log2e, splits, part_o, part_ml, err,
+                                             cap_pre, cap_post, out_stride, out_scale,
+                                             BfDiffArgs(), sinks, keep, beyond);
+  }
   if (splits > 1) {
-    int st = bf_launch_status();
+    const int st = bf_launch_status();
     if (st) return st;
     const auto merge = d == 64 ? prefill_attention_merge_kernel<64> : d == 256 ? prefill_attention_merge_kernel<256>
                                                                                : prefill_attention_merge_kernel<128>;
-    merge<<<dim3((max_rows + 3) / 4, nh, n_items), 128, 0, stream>>>(
-        part_o, part_ml, items, (__nv_bfloat16*)out, nh, splits, out_stride, out_scale, sinks);
+    const dim3 blocks((max_rows + 3) / 4, nh, n_items);
+    if (beyond)
+      return bf_launch_pdl(merge, blocks, dim3(128), 0, stream, (const float*)part_o, (const float*)part_ml, items,
+                           (__nv_bfloat16*)out, nh, splits, out_stride, out_scale, sinks);
+    merge<<<blocks, 128, 0, stream>>>(part_o, part_ml, items, (__nv_bfloat16*)out, nh, splits, out_stride, out_scale,
+                                      sinks);
   }
   return bf_launch_status();
 }
