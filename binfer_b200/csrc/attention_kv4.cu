@@ -35,8 +35,8 @@
 // kernel, where the 254 MB take 39 at the rate of a copy, 6.54 TB/s.  While all warps run they read 6.2 TB/s:
 // some 258 instructions a unit of 2,304 bytes nearly fill the issue slots, so that bytes and instructions are
 // level; the rest is the beginning of the stretches (queries, tables, first units: 4 us) and their end, a wait for
-// the slowest SM.  Eight rows behind 4,096: 12.5 + 3 us (bytes: 5); 30,000 keys behind a window of 4,096, 12 rows of
-// 16 heads: 18 + 3 (8.7).  Tried without gain: partials added up in a block before the second kernel, barriers that
+// the slowest SM.  Eight rows behind 4,096: 12.5 + 3 us (bytes: 5), in clusters of two 15; 30,000 keys behind a
+// window of 4,096, 12 rows of 16 heads: 18 + 3, a block a head 21 (8.7).  Tried without gain: partials added up in a block before the second kernel, barriers that
 // keep a block's warps level, fewer warps with a deeper ring, the lowest values as the product's addend.
 #include "common.cuh"
 #include "kv4.cuh"
@@ -180,88 +180,88 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   int me = warp, each = 1, longer = 0, x = 0, x_end = 1;
   bool aligned = true;
   if constexpr (!HEAD) {
-  // ---- tiles, and how their units are cut.  (Loops, not unrolled: what a launch runs once waits for its
-  // instructions most of all.)
+    // ---- tiles, and how their units are cut.  (Loops, not unrolled: what a launch runs once waits for its
+    // instructions most of all.)
 #pragma unroll 1
-  for (int e = tid; e < a.n_tiles; e += 32 * WARPS) {
-    const KaTile t = tile_of(a.first_tile + e, blockIdx.x == 0);
-    tiles[e] = t;
-    const int n = ka_span(t, a.window, a.keep).units;
-    units_of[e] = n;
-  }
-  __syncthreads();
-  int total = 0, filled = 0, longest = 0;
-#pragma unroll 1
-  for (int e = lane; e < a.n_tiles; e += 32) {
-    const int n = units_of[e];
-    total += n, filled += n > 0, longest = max(longest, n);
-  }
-  total = __reduce_add_sync(0xffffffffu, total) * pairs;
-  filled = __reduce_add_sync(0xffffffffu, filled) * pairs;
-  longest = __reduce_max_sync(0xffffffffu, longest);
-  // Short stretches: a tile's heads together get pieces in proportion to their units, one each at least.
-  // With `rate` pieces a unit that makes at most rate total + heads of them: warp w tries a rate, and
-  // the highest that gives every piece a warp of its own is taken.  Not too many of a head, which the second kernel
-  // adds up: a head's 2,048 units in 1,024 pieces took 33 us, in 248 19.
-  aligned = total < KA_LONG * warps && filled < warps;
-  float rate = 0.f;
-  if (aligned) {
-    auto rate_of = [&](int i) {
-      const float room = warps - filled * (i * (1.f / (WARPS - 1)));
-      return fminf(fminf(1.f / KA_MIN_UNITS, sqrtf(KA_PIECES / longest)), fmaxf(room, 0.f) / total);
-    };
-    rate = rate_of(warp);
-  }
-  auto pieces_of = [&](int units) {
-    return units ? max(min((int)(units * (rate * pairs)), a.max_pieces * pairs), pairs) : 0;
-  };
-  if (aligned) {
-    int n = 0;
-#pragma unroll 1
-    for (int e = lane; e < a.n_tiles; e += 32) n += pieces_of(units_of[e]);
-    n = __reduce_add_sync(0xffffffffu, n);
-    if (lane == 0) sums[warp] = n, rates[warp] = rate;
-    __syncthreads();
-    const unsigned fits = __ballot_sync(0xffffffffu, lane < WARPS && sums[lane < WARPS ? lane : 0] <= warps);
-    aligned = fits != 0;
-    if (aligned) rate = rates[__ffs(fits) - 1];
-  }
-  if (warp == 0) {
-    int before = 0;
-#pragma unroll 1
-    for (int e0 = 0; e0 < a.n_tiles; e0 += 32) {
-      const int e = e0 + lane, u = e < a.n_tiles ? units_of[e] : 0, n = aligned ? pieces_of(u) : u ? (u + KA_BEGIN) * pairs : 0;
-      int incl = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += up;
-      }
-      if (e < a.n_tiles) start[e] = before + incl - n;
-      before += __shfl_sync(0xffffffffu, incl, 31);
+    for (int e = tid; e < a.n_tiles; e += 32 * WARPS) {
+      const KaTile t = tile_of(a.first_tile + e, blockIdx.x == 0);
+      tiles[e] = t;
+      const int n = ka_span(t, a.window, a.keep).units;
+      units_of[e] = n;
     }
-    if (lane == 0) start[a.n_tiles] = before;
-  }
-  __syncthreads();
-  begin(1);
-  if (blockIdx.x == 0)
+    __syncthreads();
+    int total = 0, filled = 0, longest = 0;
 #pragma unroll 1
-    for (int e = tid; e < a.n_tiles; e += 32 * WARPS)
-      if (units_of[e] == 0)
-        for (int i = 0; i < pairs; ++i) a.desc[e * pairs + i] = make_int4(-1, -1, 0, 0);
-  if (total == 0) return;
-  me = warp * gridDim.x + blockIdx.x;                       // (few stretches lie on as many SMs)
-  x = me, x_end = me + 1;                                   // pieces: one
-  if (!aligned) {
-    // every head begins with KA_BEGIN places for what that takes
-    const int places = start[a.n_tiles], least = max(KA_LONG / 2, (longest + a.max_pieces - 1) / a.max_pieces);
-    const int parts = min(max(places / least, 1), warps);
-    each = places / parts, longer = places - each * parts;  // the first `longer` have one more
-    x = me * each + min(me, longer);
-    x_end = me < parts ? x + each + (me < longer ? 1 : 0) : x;
-  } else if (me >= start[a.n_tiles]) {
-    return;
-  }
+    for (int e = lane; e < a.n_tiles; e += 32) {
+      const int n = units_of[e];
+      total += n, filled += n > 0, longest = max(longest, n);
+    }
+    total = __reduce_add_sync(0xffffffffu, total) * pairs;
+    filled = __reduce_add_sync(0xffffffffu, filled) * pairs;
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    // Short stretches: a tile's heads together get pieces in proportion to their units, one each at least.
+    // With `rate` pieces a unit that makes at most rate total + heads of them: warp w tries a rate, and
+    // the highest that gives every piece a warp of its own is taken.  Not too many of a head, which the second kernel
+    // adds up: a head's 2,048 units in 1,024 pieces took 33 us, in 248 19.
+    aligned = total < KA_LONG * warps && filled < warps;
+    float rate = 0.f;
+    if (aligned) {
+      auto rate_of = [&](int i) {
+        const float room = warps - filled * (i * (1.f / (WARPS - 1)));
+        return fminf(fminf(1.f / KA_MIN_UNITS, sqrtf(KA_PIECES / longest)), fmaxf(room, 0.f) / total);
+      };
+      rate = rate_of(warp);
+    }
+    auto pieces_of = [&](int units) {
+      return units ? max(min((int)(units * (rate * pairs)), a.max_pieces * pairs), pairs) : 0;
+    };
+    if (aligned) {
+      int n = 0;
+#pragma unroll 1
+      for (int e = lane; e < a.n_tiles; e += 32) n += pieces_of(units_of[e]);
+      n = __reduce_add_sync(0xffffffffu, n);
+      if (lane == 0) sums[warp] = n, rates[warp] = rate;
+      __syncthreads();
+      const unsigned fits = __ballot_sync(0xffffffffu, lane < WARPS && sums[lane < WARPS ? lane : 0] <= warps);
+      aligned = fits != 0;
+      if (aligned) rate = rates[__ffs(fits) - 1];
+    }
+    if (warp == 0) {
+      int before = 0;
+#pragma unroll 1
+      for (int e0 = 0; e0 < a.n_tiles; e0 += 32) {
+        const int e = e0 + lane, u = e < a.n_tiles ? units_of[e] : 0, n = aligned ? pieces_of(u) : u ? (u + KA_BEGIN) * pairs : 0;
+        int incl = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += up;
+        }
+        if (e < a.n_tiles) start[e] = before + incl - n;
+        before += __shfl_sync(0xffffffffu, incl, 31);
+      }
+      if (lane == 0) start[a.n_tiles] = before;
+    }
+    __syncthreads();
+    begin(1);
+    if (blockIdx.x == 0)
+#pragma unroll 1
+      for (int e = tid; e < a.n_tiles; e += 32 * WARPS)
+        if (units_of[e] == 0)
+          for (int i = 0; i < pairs; ++i) a.desc[e * pairs + i] = make_int4(-1, -1, 0, 0);
+    if (total == 0) return;
+    me = warp * gridDim.x + blockIdx.x;                       // (few stretches lie on as many SMs)
+    x = me, x_end = me + 1;                                   // pieces: one
+    if (!aligned) {
+      // every head begins with KA_BEGIN places for what that takes
+      const int places = start[a.n_tiles], least = max(KA_LONG / 2, (longest + a.max_pieces - 1) / a.max_pieces);
+      const int parts = min(max(places / least, 1), warps);
+      each = places / parts, longer = places - each * parts;  // the first `longer` have one more
+      x = me * each + min(me, longer);
+      x_end = me < parts ? x + each + (me < longer ? 1 : 0) : x;
+    } else if (me >= start[a.n_tiles]) {
+      return;
+    }
   }
 
   const float scale_log2 = a.scale * 1.44269504088896341f;
@@ -285,40 +285,40 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
       u0 = 2 * (w * few + min(w, more));
       mine = max(min(2 * (few + (w < more ? 1 : 0)), span.units - u0), 0), n_pieces = all, x = x_end;
     } else {
-    // the tile of x: the last that begins at or before it, among every sixteenth and then among sixteen
-    e = lane * 16;
-    e = (31 - __clz(__ballot_sync(0xffffffffu, e < a.n_tiles && start[e] <= x))) * 16;
-    const int e1 = e + (lane & 15);
-    e += 31 - __clz(__ballot_sync(0xffffffffu, lane < 16 && e1 < a.n_tiles && start[e1] <= x));
-    static_assert(KA_MAX_TILES <= 512, "two steps");
-    t = tiles[e];
-    span = ka_span(t, a.window, a.keep);
-    const int y = x - start[e];
-    if (aligned) {
-      const int n = start[e + 1] - start[e], fewer = ka_div(n, pairs), more = n - fewer * pairs;
-      const int edge = more * (fewer + 1);                  // the first `more` heads have a piece more
-      n_pieces = fewer + (y < edge ? 1 : 0);
-      const int z = y < edge ? y : y - edge;
-      pair = ka_div(z, n_pieces);
-      const int piece = z - pair * n_pieces, units = ka_div(span.units, n_pieces), over = span.units - units * n_pieces;
-      if (y >= edge) pair += more;
-      u0 = piece * units + min(piece, over);
-      mine = units + (piece < over ? 1 : 0);
-      x = x_end;
-    } else {
-      const int v = span.units + KA_BEGIN;
-      pair = y / v;
-      const int place = y - pair * v, to = min(v, place + x_end - x);
-      u0 = max(place - KA_BEGIN, 0);
-      mine = to - KA_BEGIN - u0;
-      n_pieces = 1;
-      if (mine < span.units) {                              // (asked for where u0 is 0: how many warps share the head)
-        const int at = x - place + v - 1, edge = longer * (each + 1);
-        n_pieces = (at < edge ? at / (each + 1) : longer + (at - edge) / each) - me + 1;
+      // the tile of x: the last that begins at or before it, among every sixteenth and then among sixteen
+      e = lane * 16;
+      e = (31 - __clz(__ballot_sync(0xffffffffu, e < a.n_tiles && start[e] <= x))) * 16;
+      const int e1 = e + (lane & 15);
+      e += 31 - __clz(__ballot_sync(0xffffffffu, lane < 16 && e1 < a.n_tiles && start[e1] <= x));
+      static_assert(KA_MAX_TILES <= 512, "two steps");
+      t = tiles[e];
+      span = ka_span(t, a.window, a.keep);
+      const int y = x - start[e];
+      if (aligned) {
+        const int n = start[e + 1] - start[e], fewer = ka_div(n, pairs), more = n - fewer * pairs;
+        const int edge = more * (fewer + 1);                  // the first `more` heads have a piece more
+        n_pieces = fewer + (y < edge ? 1 : 0);
+        const int z = y < edge ? y : y - edge;
+        pair = ka_div(z, n_pieces);
+        const int piece = z - pair * n_pieces, units = ka_div(span.units, n_pieces), over = span.units - units * n_pieces;
+        if (y >= edge) pair += more;
+        u0 = piece * units + min(piece, over);
+        mine = units + (piece < over ? 1 : 0);
+        x = x_end;
+      } else {
+        const int v = span.units + KA_BEGIN;
+        pair = y / v;
+        const int place = y - pair * v, to = min(v, place + x_end - x);
+        u0 = max(place - KA_BEGIN, 0);
+        mine = to - KA_BEGIN - u0;
+        n_pieces = 1;
+        if (mine < span.units) {                              // (asked for where u0 is 0: how many warps share the head)
+          const int at = x - place + v - 1, edge = longer * (each + 1);
+          n_pieces = (at < edge ? at / (each + 1) : longer + (at - edge) / each) - me + 1;
+        }
+        x += to - place;
+        if (mine <= 0) continue;
       }
-      x += to - place;
-      if (mine <= 0) continue;
-    }
     }
     const int h = a.chunks == 1 ? pair : pair / a.chunks, head0 = h * a.group + (pair - h * a.chunks) * a.chunk;
     const int heads = min(a.chunk, (h + 1) * a.group - head0);
@@ -907,10 +907,10 @@ static long long ka_slots(const KaShape& s, int d, int sms) { return 2LL * sms *
 // sweep of rows of equal length (replayed from a graph, launch included): a cluster 6.5 (several blocks 8.5) and `unit`
 // for each unit of a block, where all clusters are resident at once (74, 33 and 15 of two, four and eight blocks);
 // stretches `base`, `each` for every unit of all heads, of which a batch has three quarters of what its longest row
-// says, and `piece` for a head's pieces.  Heads of 128 (4 query heads each), stretches / 1, 2, 4, 8 blocks: 8 heads over 512
+// says (all of it where a window cuts them to one length, `even`), and `piece` for a head's pieces.  Heads of 128 (4 query heads each), stretches / 1, 2, 4, 8 blocks: 8 heads over 512
 // keys 10.7 / 8.6, 8.6, 8.6, 8.6, over 4,096 12.6 / 20.9, 14.8, 12.7, 10.6, over 16,384 19.0 / 62, 36, 23, 15.4; 32 heads over
 // 4,096 16.9 / 20.9, 14.7, 12.7; 72 over 4,096 19.0 / 20.9, 16.3; 128 over 512 14.7 / 8.7, over 4,096 27.2 / 21.0.
-static int ka_blocks_a_head(const KaShape& s, int d, long long tiles, int pairs, int keys, int sms) {
+static int ka_blocks_a_head(const KaShape& s, int d, long long tiles, int pairs, int keys, bool even, int sms) {
   struct Times {
     float unit, base, each, piece;
   };
@@ -919,7 +919,7 @@ static int ka_blocks_a_head(const KaShape& s, int d, long long tiles, int pairs,
                              : Times{0.105f, 12.f, 0.7e-3f, 0.035f};
   const float units = keys / KA_UNIT + 1, heads = (float)tiles * pairs;
   const float pieces = fminf(sqrtf(KA_PIECES * units), sms * ka_warps(d, s.nt) / heads);
-  float best = t.base + t.each * units * heads * (tiles > 1 ? 0.75f : 1.f) + t.piece * pieces;
+  float best = t.base + t.each * units * heads * (tiles > 1 && !even ? 0.75f : 1.f) + t.piece * pieces;
   int share = 0;
   for (int c = 1; c <= KA_SHARE; c *= 2) {
     const int fit = sms * (c < 4 ? 100 : c == 4 ? 90 : 82) / (100 * c);
@@ -930,10 +930,10 @@ static int ka_blocks_a_head(const KaShape& s, int d, long long tiles, int pairs,
 }
 
 // Bytes of scratch that a call needs (16-byte aligned): partial results and a note per (tile, head); none where
-// no second kernel runs.  `keys` as the call's.
-BF_EXPORT long long bf_kv4_attention_scratch(int n, int max_rows, int nh, int nkv, int d, int sms, int keys) {
+// no second kernel runs.  `keys`, `even` as the call's.
+BF_EXPORT long long bf_kv4_attention_scratch(int n, int max_rows, int nh, int nkv, int d, int sms, int keys, int even) {
   const KaShape s = ka_shape(nh / nkv, d, max_rows);
-  if (ka_blocks_a_head(s, d, (long long)n * ((max_rows + s.tokens - 1) / s.tokens), nkv * s.chunks, keys, sms)) return 0;
+  if (ka_blocks_a_head(s, d, (long long)n * ((max_rows + s.tokens - 1) / s.tokens), nkv * s.chunks, keys, even, sms)) return 0;
   const long long slots = ka_slots(s, d, sms);
   long long tiles = (long long)n * ((max_rows + s.tokens - 1) / s.tokens);
   if (tiles > KA_MAX_TILES) tiles = KA_MAX_TILES;
@@ -953,7 +953,7 @@ struct Kv4AttentionCall {
   int nh, nkv, d, page_size, num_pages, window, keep;
   float scale;
   void* scratch;
-  int sms, keys;                                           // keys: the most that a row can see, as to the scratch
+  int sms, keys, even;                                     // what a row can see, as to the scratch
   int early;                                               // the description was there before the kernel ahead began
   int* err;
   cudaStream_t stream;
@@ -961,7 +961,7 @@ struct Kv4AttentionCall {
 BF_EXPORT int bf_kv4_attention(const Kv4AttentionCall* call) {
   const auto& [q, q_stride, cache, rows, seq_of_token, positions, items, n, max_rows, T, block_tables,
                table_stride, table_rows, table_width, out, out_stride, nh, nkv, d, page_size, num_pages,
-               window, keep, scale, scratch, sms, keys, early, err, stream] = *call;
+               window, keep, scale, scratch, sms, keys, even, early, err, stream] = *call;
   if (n <= 0 || max_rows <= 0) return 0;
   if ((long long)num_pages * nkv * (page_size / 8) > 0x7fffffffLL || page_size < 8 || (page_size & (page_size - 1)) ||
       (long long)table_width * page_size > 1 << 24)        // (a tile's units stay below 2^20)
@@ -987,7 +987,7 @@ BF_EXPORT int bf_kv4_attention(const Kv4AttentionCall* call) {
   a.err = err;
   const long long tiles = (long long)n * a.tiles_per_item;
   if (tiles > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
-  const int share = ka_blocks_a_head(s, d, tiles, nkv * s.chunks, keys, sms);
+  const int share = ka_blocks_a_head(s, d, tiles, nkv * s.chunks, keys, even, sms);
   if (!share && !scratch) return (int)cudaErrorInvalidValue;
   if (d == 64) return s.nt == 1 ? ka_launch<64, 1>(a, (int)tiles, share, sms, stream) : ka_launch<64, 2>(a, (int)tiles, share, sms, stream);
   if (d == 128) return s.nt == 1 ? ka_launch<128, 1>(a, (int)tiles, share, sms, stream) : ka_launch<128, 2>(a, (int)tiles, share, sms, stream);

@@ -1918,8 +1918,8 @@ class _Packed:
 _kv4_store_call = _Packed("bf_kv4_store", "PqPqPPiiiiqPP")
 _kv4_load_call = _Packed("bf_kv4_load", "PPiiiPiiPPPiPPPiiiiiiiiPP")
 _kv4_rest_call = _Packed("bf_kv4_rest", "PPPPiiPiPPiPqPqiiiiiiifP")
-_kv4_attention_call = _Packed("bf_kv4_attention", "PqPPPPPiiiPiiiPqiiiiiiifPiiiPP")
-_qk_norm_rope_kv4_call = _Packed("bf_qk_norm_rope_kv4_store", "PqPPPPPPPiiiiqfPiifPP")
+_kv4_attention_call = _Packed("bf_kv4_attention", "PqPPPPPiiiPiiiPqiiiiiiifPiiiiPP")
+_qk_norm_rope_kv4_call = _Packed("bf_qk_norm_rope_kv4_store", "PqPPPiPPPPiiiiiqfPiifPP")
 _step_tables_call = _Packed("bf_step_tables", "PiiPiPiiiPPPPPiPiPiPiPP")
 _prefill_attention_umma2_half_call = _Packed("bf_prefill_attention_umma2_half", "PPPPiiiPiPiiiiiifiPPPqfiPP")
 
@@ -1966,8 +1966,7 @@ def qk_norm_rope_kv4_store(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w: 
                            q_out: torch.Tensor, cache: torch.Tensor, nh: int, nkv: int, d: int, eps: float,
                            err: torch.Tensor, row_scale: Optional[RowScale] = None) -> None:
     """``qk_norm_rope_kv_write`` into a cache in 4 bits (``kv4_cache``): per-head RMSNorm of q and k, rotation,
-    q to ``q_out [T, nh * d]``, k and v, rounded to bfloat16, into the pages at ``slots`` as ``kv4_store`` does.
-    One kernel for heads of 128 that are turned whole, two for others."""
+    q to ``q_out [T, nh * d]``, k and v, rounded to bfloat16, into the pages at ``slots`` as ``kv4_store`` does."""
     what = "qk_norm_rope_kv4_store"
     if (qkv.dim() != 2 or qkv.dtype != torch.bfloat16 or qkv.stride(1) != 1 or q_out.dtype != torch.bfloat16
             or not q_out.is_contiguous() or qkv.shape[1] != (nh + 2 * nkv) * d
@@ -1985,21 +1984,13 @@ def qk_norm_rope_kv4_store(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w: 
     if T == 0:
         return
     address = lambda t: t.data_ptr() if t is not None else 0
-    weights = address(q_w), address(k_w), address(inv_freq)
-    if (d == 128 and inv_freq is not None and inv_freq.numel() == 64 and stride % 4 == 0 and qkv.data_ptr() % 8 == 0
-            and q_out.data_ptr() % 8 == 0 and not any(w % 16 for w in weights)):
-        _row_scale_args(row_scale, T)
-        part, count, width, rs_eps = ((row_scale.partials.data_ptr(), row_scale.partials.shape[1], row_scale.width,
-                                       row_scale.eps) if row_scale is not None else (0, 0, 0, 0.0))
-        _run(what, _qk_norm_rope_kv4_call, qkv.data_ptr(), stride, *weights, positions.data_ptr(), slots.data_ptr(),
-             q_out.data_ptr(), cache.data_ptr(), T, nh, nkv, ps, pages * ps, eps, part, count, width, rs_eps,
-             err.data_ptr(), _stream_at(qkv))
-        return
-    # rows of bfloat16 (a cache of one-token pages), then those into the pages
-    k, v = torch.empty((2, T, nkv, 1, d), dtype=torch.bfloat16, device=qkv.device)
-    qk_norm_rope_kv_write(qkv, q_w, k_w, inv_freq, positions, token_rows(T, qkv.device), q_out, k, v, nh, nkv, d, eps,
-                          err, row_scale=row_scale)
-    kv4_store(k.view(T, nkv * d), v.view(T, nkv * d), slots, cache, err)
+    _row_scale_args(row_scale, T)
+    part, count, width, rs_eps = ((row_scale.partials.data_ptr(), row_scale.partials.shape[1], row_scale.width,
+                                   row_scale.eps) if row_scale is not None else (0, 0, 0, 0.0))
+    _run(what, _qk_norm_rope_kv4_call, qkv.data_ptr(), stride, address(q_w), address(k_w), address(inv_freq),
+         inv_freq.numel() if inv_freq is not None else 0, positions.data_ptr(), slots.data_ptr(), q_out.data_ptr(),
+         cache.data_ptr(), T, nh, nkv, d, ps, pages * ps, eps, part, count, width, rs_eps, err.data_ptr(),
+         _stream_at(qkv))
 
 
 def kv4_load(cache: torch.Tensor, block_tables: torch.Tensor, items: torch.Tensor, n_items: int,
@@ -2228,22 +2219,23 @@ def _kv4_attention(q, cache, rows, seq, positions, items, n, max_rows, block_tab
     sms = num_sms(device)
     table_rows, table_width, table_stride = table
     # what a row can see at most (beyond some thousand keys any number goes the same way)
-    keys = min(table_width * ps, window + keep + max_rows + 32) if window else table_width * ps
-    keys = min(keys, _KV4_MANY_KEYS) & -16
-    key = (n, max_rows, nh, nkv, d, sms, keys)
+    keys, cut = table_width * ps, window + keep + max_rows + 32
+    even = 0 < window and 2 * cut < keys        # most rows are as long as the window, then
+    keys = min(cut if window else keys, keys, _KV4_MANY_KEYS) & -16
+    key = (n, max_rows, nh, nkv, d, sms, keys, even)
     size = _kv4_scratch.get(key)
     if size is None:
         fn = lib().bf_kv4_attention_scratch
         fn.restype = _c_ll
         if len(_kv4_scratch) > 4096:
             _kv4_scratch.clear()
-        size = _kv4_scratch[key] = fn(n, max_rows, nh, nkv, d, sms, keys)
+        size = _kv4_scratch[key] = fn(n, max_rows, nh, nkv, d, sms, keys, even)
     # a call's own, from its stream's pool: two captured graphs share nothing
     scratch = torch.empty(size, dtype=torch.uint8, device=device) if size else None
     T, q_stride, out_stride = strides
     _run("kv4_attention", _kv4_attention_call, q.data_ptr(), q_stride, cache.data_ptr(), rows, seq, positions,
          items, n, max_rows, T, block_tables.data_ptr(), table_stride, table_rows, table_width, out.data_ptr(),
-         out_stride, nh, nkv, d, ps, pages, window, keep, scale, scratch.data_ptr() if size else 0, sms, keys, described,
+         out_stride, nh, nkv, d, ps, pages, window, keep, scale, scratch.data_ptr() if size else 0, sms, keys, even, described,
          err.data_ptr(), _stream_at(q))
     if size:
         _launches += 1      # two kernels: the stretches of units, and what several of them share

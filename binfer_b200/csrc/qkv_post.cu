@@ -15,7 +15,36 @@
 #include "common.cuh"
 #include "kv4.cuh"
 
-template <typename A>
+// A group's codes from four (or two) numbers of a lane, its extremes among `lanes` neighbouring lanes.
+template <int N>
+__device__ __forceinline__ unsigned kv4_lane_codes(const __nv_bfloat162 (&y)[N / 2], int lanes, unsigned& pair) {
+  __nv_bfloat162 lo = y[0], hi = y[0];
+#pragma unroll
+  for (int j = 1; j < N / 2; ++j) lo = __hmin2_nan(lo, y[j]), hi = __hmax2_nan(hi, y[j]);
+  for (int m = lanes / 2; m; m >>= 1) {
+    lo = __hmin2_nan(lo, __shfl_xor_sync(0xffffffffu, lo, m));
+    hi = __hmax2_nan(hi, __shfl_xor_sync(0xffffffffu, hi, m));
+  }
+  const Kv4Coder coder(__hmin_nan(lo.x, lo.y), __hmax_nan(hi.x, hi.y));
+  pair = coder.pair;
+  unsigned codes = 0u;
+  if (coder.quick) {
+    float sum = 0.f;
+#pragma unroll
+    for (int j = N - 1; j >= 0; --j)
+      sum = fmaf(16.f, sum, coder.quick_code(__bfloat162float(j & 1 ? y[j / 2].y : y[j / 2].x)));
+    codes = (unsigned)sum;
+  } else if (coder.finite) {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      codes |= kv4_any_code(__bfloat162float(j & 1 ? y[j / 2].y : y[j / 2].x), coder.lo, coder.s) << (4 * j);
+  }
+  return codes;
+}
+
+// FOUR: keys and values go into pages held in 4 bits (kv4.cuh; k_cache is the pages of both), rounded to bfloat16
+// first.
+template <typename A, bool FOUR = false>
 __global__ void qk_norm_rope_kv_write_kernel(
     const A* __restrict__ qkv, long long row_stride, const float* __restrict__ q_w,
     const float* __restrict__ k_w, const float* __restrict__ inv_freq, int rot_half,
@@ -75,6 +104,22 @@ __global__ void qk_norm_rope_kv_write_kernel(
   }
   const int h = is_k ? hh - nh : hh - nh - nkv;
   const int page = slot / page_size, off = slot - page * page_size;
+  if constexpr (FOUR) {
+    unsigned char* rec = reinterpret_cast<unsigned char*>(k_cache) +
+                         (((size_t)page * nkv + h) * (page_size / KV4_EIGHTH) + off / KV4_EIGHTH) * kv4_record(d);
+    const int tok = off % KV4_EIGHTH, groups = d / KV4_GROUP;
+    for (int g = 0; g < groups; ++g) {
+      const int i = g * KV4_GROUP + lane * 2;
+      const __nv_bfloat162 y[1] = {__floats2bfloat162_rn(x[i], x[i + 1])};
+      unsigned pair;
+      const unsigned codes = kv4_lane_codes<2>(y, 32, pair);
+      rec[is_k ? kv4_key_byte(d, tok, i) : kv4_value_byte(d, tok, i)] = (unsigned char)codes;
+      if (lane == 0)
+        *reinterpret_cast<unsigned*>(rec + (is_k ? kv4_key_params_at(d) : kv4_value_params_at(d)) +
+                                     (tok * groups + g) * 4) = pair;
+    }
+    return;
+  }
   A* dst = (is_k ? k_cache : v_cache) + (((size_t)page * nkv + h) * page_size + off) * d;
   for (int i = lane; i < d; i += 32) bf_st(dst + i, x[i]);
 }
@@ -86,8 +131,7 @@ __global__ void qk_norm_rope_kv_write_kernel(
 // sit in lane l ^ 16.  With few tokens every warp has one head: the kernel is then two
 // dependent round trips long (position, then the head's values) instead of one per head.
 //
-// FOUR: keys and values go into pages held in 4 bits (kv4.cuh; k_cache is the pages of both).  A group's 64 numbers
-// lie in sixteen lanes, which find its extremes in four steps; a lane's four codes are two bytes.
+// FOUR: as above; a group's 64 numbers lie in sixteen lanes, a lane's four codes are two bytes.
 template <bool FOUR>
 __global__ void qk_norm_rope_kv_write_d128_kernel(
     const __nv_bfloat16* __restrict__ qkv, long long row_stride, const float* __restrict__ q_w,
@@ -193,25 +237,9 @@ __global__ void qk_norm_rope_kv_write_d128_kernel(
     }
     const int h = is_k ? hh - nh : hh - nh - nkv;
     if constexpr (FOUR) {
-      __nv_bfloat162 lo = __hmin2_nan(o2[0], o2[1]), hi = __hmax2_nan(o2[0], o2[1]);
-#pragma unroll
-      for (int m = 8; m; m >>= 1) {
-        lo = __hmin2_nan(lo, __shfl_xor_sync(0xffffffffu, lo, m));
-        hi = __hmax2_nan(hi, __shfl_xor_sync(0xffffffffu, hi, m));
-      }
-      const Kv4Coder coder(__hmin_nan(lo.x, lo.y), __hmax_nan(hi.x, hi.y));
-      const float2 y0 = __bfloat1622float2(o2[0]), y1 = __bfloat1622float2(o2[1]);
-      const float y[4] = {y0.x, y0.y, y1.x, y1.y};
-      unsigned codes = 0u;
-      if (coder.quick) {
-        float sum = 0.f;
-#pragma unroll
-        for (int j = 3; j >= 0; --j) sum = fmaf(16.f, sum, coder.quick_code(y[j]));
-        codes = (unsigned)sum;
-      } else if (coder.finite) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) codes |= kv4_any_code(y[j], coder.lo, coder.s) << (4 * j);
-      }
+      const __nv_bfloat162 y[2] = {o2[0], o2[1]};
+      unsigned pair;
+      const unsigned codes = kv4_lane_codes<4>(y, 16, pair);
       unsigned char* rec = reinterpret_cast<unsigned char*>(k_cache) +
                            (((size_t)page * nkv + h) * (page_size / KV4_EIGHTH) + off / KV4_EIGHTH) * kv4_record(D);
       const int tok = off % KV4_EIGHTH;
@@ -219,7 +247,7 @@ __global__ void qk_norm_rope_kv_write_d128_kernel(
           rec + (is_k ? kv4_key_byte(D, tok, lane * 4) : kv4_value_byte(D, tok, lane * 4))) = (unsigned short)codes;
       if ((lane & 15) == 0)
         *reinterpret_cast<unsigned*>(rec + (is_k ? kv4_key_params_at(D) : kv4_value_params_at(D)) +
-                                     (tok * 2 + (lane >> 4)) * 4) = coder.pair;
+                                     (tok * 2 + (lane >> 4)) * 4) = pair;
     } else {
       *reinterpret_cast<uint2*>((is_k ? k_cache : v_cache) + kv_base + (size_t)h * kv_head) = o;
     }
@@ -274,16 +302,16 @@ BF_EXPORT int bf_qk_norm_rope_kv_write(
   return bf_launch_status();
 }
 
-// The same into pages held in 4 bits: bfloat16, heads of 128 turned whole, every address a multiple of its loads'
-// size; cudaErrorInvalidValue otherwise (nothing launched).
+// The same into pages held in 4 bits, from bfloat16.
 struct QkNormRopeKv4Call {
   const void* qkv;
   long long row_stride;
   const float* q_w, *k_w, *inv_freq;
+  int rot_half;
   const int* positions, *slots;
   void* q_out;
   void* cache;
-  int T, nh, nkv, page_size;
+  int T, nh, nkv, d, page_size;
   long long num_slots;
   float eps;
   const float* row_partials;
@@ -293,19 +321,29 @@ struct QkNormRopeKv4Call {
   cudaStream_t stream;
 };
 BF_EXPORT int bf_qk_norm_rope_kv4_store(const QkNormRopeKv4Call* call) {
-  const auto& [qkv, row_stride, q_w, k_w, inv_freq, positions, slots, q_out, cache, T, nh, nkv, page_size, num_slots,
-               eps, row_partials, row_count, row_width, row_eps, err, stream] = *call;
+  const auto& [qkv, row_stride, q_w, k_w, inv_freq, rot_half, positions, slots, q_out, cache, T, nh, nkv, d, page_size,
+               num_slots, eps, row_partials, row_count, row_width, row_eps, err, stream] = *call;
   if (T <= 0) return 0;
   const BfRowScale rs = {row_partials, row_count, row_width > 0 ? 1.f / (float)row_width : 0.f, row_eps};
-  if (!cache || !inv_freq || row_stride % 4 || ((uintptr_t)qkv & 7) || ((uintptr_t)q_out & 7) || ((uintptr_t)cache & 15) ||
-      ((uintptr_t)inv_freq & 15) || ((uintptr_t)q_w & 15) || ((uintptr_t)k_w & 15) || page_size < 8 || page_size % 8)
+  if (!cache || ((uintptr_t)cache & 15) || page_size < 8 || page_size % 8 || (d != 64 && d != 128 && d != 256) ||
+      2 * rot_half > d || (rot_half && !inv_freq))
     return (int)cudaErrorInvalidValue;
-  const int total = nh + 2 * nkv, block = total >= 16 ? 256 : 128;
-  const int parts = T <= 64 ? (total * 32 + block - 1) / block : 1;
-  return bf_launch_pdl(qk_norm_rope_kv_write_d128_kernel<true>, dim3(T, parts), dim3(block), 0, stream,
-                       (const __nv_bfloat16*)qkv, row_stride, q_w, k_w, inv_freq, positions, slots,
-                       (__nv_bfloat16*)q_out, (__nv_bfloat16*)cache, (__nv_bfloat16*)nullptr, nh, nkv, page_size,
-                       num_slots, eps, rs, err);
+  const int total = nh + 2 * nkv;
+  if (d == 128 && rot_half == 64 && row_stride % 4 == 0 && ((uintptr_t)qkv & 7) == 0 && ((uintptr_t)q_out & 7) == 0 &&
+      ((uintptr_t)inv_freq & 15) == 0 && ((uintptr_t)q_w & 15) == 0 && ((uintptr_t)k_w & 15) == 0) {
+    const int block = total >= 16 ? 256 : 128;
+    const int parts = T <= 64 ? (total * 32 + block - 1) / block : 1;
+    return bf_launch_pdl(qk_norm_rope_kv_write_d128_kernel<true>, dim3(T, parts), dim3(block), 0, stream,
+                         (const __nv_bfloat16*)qkv, row_stride, q_w, k_w, inv_freq, positions, slots,
+                         (__nv_bfloat16*)q_out, (__nv_bfloat16*)cache, (__nv_bfloat16*)nullptr, nh, nkv, page_size,
+                         num_slots, eps, rs, err);
+  }
+  const int warps = 4;
+  qk_norm_rope_kv_write_kernel<__nv_bfloat16, true>
+      <<<dim3(T, (total + warps - 1) / warps), warps * 32, (size_t)warps * d * sizeof(float), stream>>>(
+          (const __nv_bfloat16*)qkv, row_stride, q_w, k_w, inv_freq, rot_half, positions, slots, (__nv_bfloat16*)q_out,
+          (__nv_bfloat16*)cache, nullptr, nh, nkv, d, page_size, num_slots, eps, rs, err);
+  return bf_launch_status();
 }
 
 BF_TRACE_READER(bf_trace_read_qkv_post)
