@@ -2080,7 +2080,7 @@ def kv4_decode_attention(q: torch.Tensor, cache: torch.Tensor, rows: Optional[to
     ``described``: rows, requests, positions and tables were complete before the kernel ahead on the stream began
     (as in a step that is described once and then runs its layers); they are read under that kernel's end.
 
-    Queries below 2^62 and values below 2^55 in size: larger ones overflow inside."""
+    Queries below 2^62, values below 2^55 and scores below 1e30 in size: larger ones overflow inside."""
     _want(seq_of_token, torch.int32, "seq_of_token"); _want(positions, torch.int32, "positions")
     if rows is not None:
         _want(rows, torch.int32, "rows")
