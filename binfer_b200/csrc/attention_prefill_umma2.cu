@@ -56,7 +56,8 @@
 //
 // Keys and values may be fp16 (HALF: those of a cache held in 4 bits, whose numbers bfloat16 would round): the
 // softmax warps then make their Q tile fp16 where it lies before its first product, and a request and kv
-// head with a query beyond fp16's range is noted in `beyond` for the caller to compute otherwise.  P is
+// head with a query beyond fp16's range, or a page that `special` marks, is noted in `beyond` for the caller to
+// compute otherwise.  P is
 // fp16 as well, times 2^6: at most 2^14, since the reference lies at most 2^8 below the maximum, and what
 // is lost below its smallest number is 2^-31 of the largest.  Heads of 64 and 256 go this way
 // too, tiles of one or four blocks of 64 columns where the others have two; 256 leave room in tensor and
@@ -125,7 +126,8 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
                                float* __restrict__ part_o, float* __restrict__ part_ml,
                                int* __restrict__ err, float cap_pre, float cap_post,
                                long long out_stride, float out_scale, BfDiffArgs dd,
-                               const float* __restrict__ sinks, int keep, int* __restrict__ beyond) {
+                               const float* __restrict__ sinks, int keep, int* __restrict__ beyond,
+                               const unsigned long long* __restrict__ special) {
   constexpr bool DIFF = MODE == A2_DIFF, LATENT = MODE == A2_LATENT, KEEP = MODE == A2_KEEP;
   constexpr int HALVES = D / 64;                         // blocks of 64 columns of a V tile
   constexpr int KBLOCKS = LATENT ? HALVES + 1 : HALVES;  // ... of a Q or K tile
@@ -275,6 +277,7 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
             atomicOr(err, BF_ERR_PAGE);
             mine = 0;
           }
+          if (mine > 0 && special[(size_t)mine * nkv + g]) atomicOr(beyond + (it - items) / 4 * nkv + g, 1);
         }
         const int page = __shfl_sync(0xffffffffu, mine, n % 32);
         fetch(map_k, page);
@@ -326,6 +329,8 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
           atomicOr(err, BF_ERR_PAGE);
           page = 0;
         }
+        if constexpr (HALF)
+          if (page > 0 && special[(size_t)page * nkv + g]) atomicOr(beyond + (it - items) / 4 * nkv + g, 1);
       }
       // a tile whose pages lie one after the other in the pool (the pool hands them out so)
       // comes as one box of all its pages per half, instead of one box per page
@@ -856,17 +861,19 @@ __global__ void prefill_attention_merge_kernel(const float* __restrict__ part_o,
 // (a column block of a wider buffer: a multiple of 8, the block 16-byte aligned) and
 // multiplied by `out_scale`; a logit per head in the softmax's denominator (`sinks`, or null); with a
 // window, the first `keep` tokens that stay visible behind it.  `beyond` (int [n_items, nkv],
-// zero, or null): the keys are fp16, and an entry becomes 1 where a query is beyond fp16's range.
+// zero, or null): keys and values are fp16 in pages of 64, and an entry becomes 1 where a query is beyond fp16's
+// range or the portion reads a page of the head whose word of `special` ([num_pages, nkv]) is not zero.
 static int launch_umma2(
     const void* q, const void* k_cache, const void* v_cache, const int* items, int n_items,
     int max_rows, int total_rows, const int* block_tables, int table_stride, void* out, int nh,
     int nkv, int d, int page_size, int num_pages, int window, float scale, int splits,
     float* part_o, float* part_ml, int* err, float softcap, long long out_stride,
-    float out_scale, const float* sinks, int keep, int* beyond, cudaStream_t stream) {
+    float out_scale, const float* sinks, int keep, int* beyond, const unsigned long long* special,
+    cudaStream_t stream) {
   if (n_items <= 0 || max_rows <= 0) return 0;
   if (splits < 1 || (splits > 1 && (!part_o || !part_ml))) return (int)cudaErrorInvalidValue;
   if (window <= 0 || keep < 0) keep = 0;
-  if ((d != A2_D && !((d == 64 || d == 256) && beyond)) || (d == 256 && page_size != A2_BN) || nkv <= 0 || nh % nkv || page_size < 8 || page_size > A2_BN ||
+  if ((d != A2_D && !((d == 64 || d == 256) && beyond)) || (beyond && page_size != A2_BN) || nkv <= 0 || nh % nkv || page_size < 8 || page_size > A2_BN ||
       A2_BN % page_size || ((uintptr_t)q & 15) || ((uintptr_t)k_cache & 15) ||
       ((uintptr_t)v_cache & 15) || ((uintptr_t)out & 15) || !(scale > 0.f) || softcap < 0.f ||
       out_stride < (long long)nh * d || (out_stride & 7))
@@ -917,14 +924,14 @@ static int launch_umma2(
     const int st = bf_launch_pdl(kern, grid, dim3(A2_THREADS), smem, stream, mq, mk, mv, mkr, mvr, items, block_tables,
                                  table_stride, (__nv_bfloat16*)out, nh, nkv, page_size, num_pages, window,
                                  scale * log2e, splits, part_o, part_ml, err, cap_pre, cap_post, out_stride, out_scale,
-                                 BfDiffArgs(), sinks, keep, beyond);
+                                 BfDiffArgs(), sinks, keep, beyond, special);
     if (st) return st;
   } else {
     kern<<<grid, A2_THREADS, smem, stream>>>(mq, mk, mv, mkr, mvr, items, block_tables, table_stride,
                                              (__nv_bfloat16*)out, nh, nkv, page_size, num_pages,
                                              window, scale * log2e, splits, part_o, part_ml, err,
                                              cap_pre, cap_post, out_stride, out_scale,
-                                             BfDiffArgs(), sinks, keep, beyond);
+                                             BfDiffArgs(), sinks, keep, beyond, special);
   }
   if (splits > 1) {
     const int st = bf_launch_status();
@@ -949,7 +956,7 @@ BF_EXPORT int bf_prefill_attention_umma2_capped(
     float out_scale, const float* sinks, int keep, cudaStream_t stream) {
   return launch_umma2(q, k_cache, v_cache, items, n_items, max_rows, total_rows, block_tables, table_stride, out,
                       nh, nkv, d, page_size, num_pages, window, scale, splits, part_o, part_ml, err, softcap,
-                      out_stride, out_scale, sinks, keep, nullptr, stream);
+                      out_stride, out_scale, sinks, keep, nullptr, nullptr, stream);
 }
 
 // bfloat16 queries over fp16 keys and values, the result times `out_scale`; heads of 64, 128 or 256.
@@ -969,16 +976,17 @@ struct PrefillAttentionUmma2HalfCall {
   float out_scale;
   int keep;
   int* beyond;
+  const unsigned long long* special;
   cudaStream_t stream;
 };
 BF_EXPORT int bf_prefill_attention_umma2_half(const PrefillAttentionUmma2HalfCall* call) {
   const auto& [q, k_cache, v_cache, items, n_items, max_rows, total_rows, block_tables, table_stride, out,
                nh, nkv, d, page_size, num_pages, window, scale, splits, part_o, part_ml, err, out_stride,
-               out_scale, keep, beyond, stream] = *call;
-  if (!beyond) return (int)cudaErrorInvalidValue;
+               out_scale, keep, beyond, special, stream] = *call;
+  if (!beyond || !special) return (int)cudaErrorInvalidValue;
   return launch_umma2(q, k_cache, v_cache, items, n_items, max_rows, total_rows, block_tables, table_stride, out,
                       nh, nkv, d, page_size, num_pages, window, scale, splits, part_o, part_ml, err, 0.f,
-                      out_stride, out_scale, nullptr, keep, beyond, stream);
+                      out_stride, out_scale, nullptr, keep, beyond, special, stream);
 }
 
 BF_EXPORT int bf_prefill_attention_umma2(const void* q, const void* k_cache, const void* v_cache,
@@ -1045,7 +1053,7 @@ BF_EXPORT int bf_diff_attention_prefill_umma(
   kern<<<grid, A2_THREADS, smem, stream>>>(mq, mk, mv, mkr, mvr, items, block_tables, table_stride,
                                            (__nv_bfloat16*)out, nh, nkv, page_size, num_pages, 0,
                                            scale * 1.4426950408889634f, splits, part_o, part_ml,
-                                           err, 0.f, 0.f, out_stride, 1.f, dd, nullptr, 0, nullptr);
+                                           err, 0.f, 0.f, out_stride, 1.f, dd, nullptr, 0, nullptr, nullptr);
   if (splits > 1) {
     int st = bf_launch_status();
     if (st) return st;
@@ -1098,6 +1106,6 @@ BF_EXPORT int bf_latent_attention_prefill_umma(
   kern<<<grid, A2_THREADS, smem, stream>>>(mq, mkv, mr, mr, mr, items, kv_base, 0,
                                            (__nv_bfloat16*)out, nh, nh, 1, 1, 0,
                                            scale * 1.4426950408889634f, 1, nullptr, nullptr, err,
-                                           0.f, 0.f, out_stride, 1.f, dd, sinks, 0, nullptr);
+                                           0.f, 0.f, out_stride, 1.f, dd, sinks, 0, nullptr, nullptr);
   return bf_launch_status();
 }

@@ -354,14 +354,12 @@ BF_EXPORT int bf_kv4_load(const Kv4LoadCall* call) {
 }
 
 // What the tensor cores cannot have computed of portions over loaded pages: the rows of a portion and kv head
-// with a record that is noted in `special` or a query in `beyond`, by multiply-adds straight from the
-// cache, a warp a (row, query head).  As a rule nothing is noted and a block only reads a few words (2.4 us); a
-// block that finds something takes its 32 rows.
+// that is noted in `beyond`, by multiply-adds straight from the cache, a warp a (row, query head).  As a rule
+// nothing is noted and a block only reads that.
 template <int D>
 __global__ void __launch_bounds__(256)
-kv4_rest_kernel(const unsigned long long* __restrict__ special, const int* __restrict__ beyond,
-                const int* __restrict__ items, const int* __restrict__ moved, const int* __restrict__ tables,
-                int width, const unsigned char* __restrict__ cache, const int* __restrict__ block_tables,
+kv4_rest_kernel(const int* __restrict__ beyond, const int* __restrict__ items, const int* __restrict__ moved,
+                const unsigned char* __restrict__ cache, const int* __restrict__ block_tables,
                 int table_stride, const __nv_bfloat16* __restrict__ q, long long q_stride,
                 __nv_bfloat16* __restrict__ out, long long out_stride, int nkv, int group, int page_size,
                 int num_pages, int window, int keep, float scale) {
@@ -370,12 +368,7 @@ kv4_rest_kernel(const unsigned long long* __restrict__ special, const int* __res
   bf_pdl_wait();
   const int h = blockIdx.y, item = blockIdx.z;
   const int row0 = moved[4 * item + 1], rows = moved[4 * item + 2], first = moved[4 * item + 3];
-  const int* table = tables + (size_t)item * width;
-  if ((int)blockIdx.x * 32 >= rows) return;
-  bool any = threadIdx.x == 0 && beyond[item * nkv + h] != 0;
-  for (int w = threadIdx.x; w < min((first + rows + 63) / 64, width); w += 256)
-    if (table[w] > 0) any |= special[(size_t)table[w] * nkv + h] != 0;
-  if (!__syncthreads_or(any)) return;
+  if (beyond[item * nkv + h] == 0 || (int)blockIdx.x * 32 >= rows) return;
   const int lane = threadIdx.x & 31, i0 = lane * N, g = i0 / 64;
   const int* request = block_tables + (size_t)items[4 * item] * table_stride;
   for (int i = threadIdx.x >> 5; i < 32 * group; i += 8) {
@@ -417,11 +410,8 @@ kv4_rest_kernel(const unsigned long long* __restrict__ special, const int* __res
 }
 
 struct Kv4RestCall {
-  const void* special;
   const int* beyond, *items, *moved;
   int n_items, max_rows;
-  const int* tables;
-  int width;
   const void* cache;
   const int* block_tables;
   int table_stride;
@@ -434,14 +424,13 @@ struct Kv4RestCall {
   cudaStream_t stream;
 };
 BF_EXPORT int bf_kv4_rest(const Kv4RestCall* call) {
-  const auto& [special, beyond, items, moved, n_items, max_rows, tables, width, cache, block_tables,
+  const auto& [beyond, items, moved, n_items, max_rows, cache, block_tables,
                table_stride, q, q_stride, out, out_stride, nh, nkv, d, page_size, num_pages, window, keep,
                scale, stream] = *call;
   if (n_items <= 0 || max_rows <= 0) return 0;
   auto run = [&](auto kern) {
     return bf_launch_pdl(kern, dim3((max_rows + 31) / 32, nkv, n_items), dim3(256), 0, stream,
-                         (const unsigned long long*)special, beyond, items, moved, tables, width,
-                         (const unsigned char*)cache, block_tables, table_stride, (const __nv_bfloat16*)q, q_stride,
+                         beyond, items, moved, (const unsigned char*)cache, block_tables, table_stride, (const __nv_bfloat16*)q, q_stride,
                          (__nv_bfloat16*)out, out_stride, nkv, nh / nkv, page_size, num_pages, window, keep, scale);
   };
   if (d == 64) return run(kv4_rest_kernel<64>);

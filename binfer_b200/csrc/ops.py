@@ -1917,11 +1917,11 @@ class _Packed:
 
 _kv4_store_call = _Packed("bf_kv4_store", "PqPqPPiiiiqPP")
 _kv4_load_call = _Packed("bf_kv4_load", "PPiiiPiiPPPiPPPiiiiiiiiPP")
-_kv4_rest_call = _Packed("bf_kv4_rest", "PPPPiiPiPPiPqPqiiiiiiifP")
+_kv4_rest_call = _Packed("bf_kv4_rest", "PPPiiPPiPqPqiiiiiiifP")
 _kv4_attention_call = _Packed("bf_kv4_attention", "PqPPPPPiiiPiiiPqiiiiiiifPiiiiPP")
 _qk_norm_rope_kv4_call = _Packed("bf_qk_norm_rope_kv4_store", "PqPPPiPPPPiiiiiqfPiifPP")
 _step_tables_call = _Packed("bf_step_tables", "PiiPiPiiiPPPPPiPiPiPiPP")
-_prefill_attention_umma2_half_call = _Packed("bf_prefill_attention_umma2_half", "PPPPiiiPiPiiiiiifiPPPqfiPP")
+_prefill_attention_umma2_half_call = _Packed("bf_prefill_attention_umma2_half", "PPPPiiiPiPiiiiiifiPPPqfiPPP")
 
 
 def kv4_store(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: torch.Tensor,
@@ -2206,10 +2206,9 @@ def _kv4_loaded_attention(q, cache, items, n_items, max_rows, block_tables, tabl
          n, nkv, d, ps, pages, w, keep, sms, err_ptr, stream)
     _run("prefill_attention_umma2", _prefill_attention_umma2_half_call,
          q_ptr, k, v, moved, n_items, max_rows, T, tables, places, out_ptr, nh, nkv, d, KV4_LOAD_PAGE, n, w, scale,
-         splits, part_o, part_ml, err_ptr, out_stride, 1.0 / KV4_VALUE_UP, keep, beyond, stream)
-    _run("kv4_rest", _kv4_rest_call, special, beyond, item_ptr, moved, n_items,
-         max_rows, tables, places, cache_ptr, table_ptr, table_stride, q_ptr, q_stride, out_ptr, out_stride, nh, nkv, d, ps,
-         pages, w, keep, scale, stream)
+         splits, part_o, part_ml, err_ptr, out_stride, 1.0 / KV4_VALUE_UP, keep, beyond, special, stream)
+    _run("kv4_rest", _kv4_rest_call, beyond, item_ptr, moved, n_items, max_rows, cache_ptr, table_ptr, table_stride,
+         q_ptr, q_stride, out_ptr, out_stride, nh, nkv, d, ps, pages, w, keep, scale, stream)
 
 
 def _kv4_attention(q, cache, rows, seq, positions, items, n, max_rows, block_tables, table, strides, out, nh,
