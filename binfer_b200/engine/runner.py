@@ -13,7 +13,9 @@ arrays per call (:2237-2269).
 """
 from __future__ import annotations
 
+import gc
 import os
+from contextlib import contextmanager
 from dataclasses import dataclass, field
 from typing import Hashable, List, Optional, Sequence, Tuple
 
@@ -28,6 +30,19 @@ from ..parts.model import DecoderModel
 
 # BINFER_B200_STEP_TABLES=0: captured steps' block tables and positions are made on the host too
 STEP_TABLES = os.environ.get("BINFER_B200_STEP_TABLES", "1") != "0"
+
+
+@contextmanager
+def _no_collection():
+    """Garbage collection off: what a collection frees in the middle of a capture (the graphs and pinned memory
+    of an engine that is gone) would end the capture."""
+    on = gc.isenabled()
+    gc.disable()
+    try:
+        yield
+    finally:
+        if on:
+            gc.enable()
 
 
 @dataclass
@@ -452,7 +467,7 @@ class ModelRunner:
             from ..csrc import ops
             graph = torch.cuda.CUDAGraph()
             before = ops.launches()
-            with torch.cuda.graph(graph):
+            with _no_collection(), torch.cuda.graph(graph):
                 st["logits"] = self.model.forward(ctx, self.views)
             st["graph"] = graph
             st["own_kernels"] = ops.launches() - before     # this library's kernels per replay

@@ -108,3 +108,38 @@ def test_generation(cuda_device, tmp_path, monkeypatch, which):
         outs.append(eng.generate(prompts, max_tokens=50, ignore_eos=True))
         assert eng.runner.graph_replays > 0
     assert outs[0] == outs[1]
+
+
+def test_capture_with_an_engine_gone(cuda_device, tmp_path):
+    """An engine that only a reference cycle holds is not collected in the middle of another's capture."""
+    import gc
+    from binfer_b200 import Engine
+    d = H.make_model_dir(tmp_path, "M", torch.bfloat16)
+
+    def engine():
+        e = Engine(d, "bfloat16", num_pages=40, page_size=16, max_seq_len=256, max_batch_size=4)
+        return e, e.generate([[1, 2, 3]], max_tokens=4, ignore_eos=True)
+
+    was = gc.get_threshold()
+    gc.collect()
+    gc.disable()
+    try:
+        old, want = engine()
+        old.itself = old
+        del old
+        new = Engine(d, "bfloat16", num_pages=40, page_size=16, max_seq_len=256, max_batch_size=4)
+        forward, calls = new.model.forward, []
+
+        def collecting(*a, **k):                  # the second forward is the captured one
+            calls.append(gc.isenabled())
+            if gc.isenabled() and torch.cuda.is_current_stream_capturing():
+                gc.collect()
+            return forward(*a, **k)
+
+        new.model.forward = collecting
+        gc.enable()
+        assert new.generate([[1, 2, 3]], max_tokens=4, ignore_eos=True) == want
+        assert False in calls and gc.isenabled() and new.runner.graph_captures == 1
+    finally:
+        gc.enable()
+        gc.set_threshold(*was)
