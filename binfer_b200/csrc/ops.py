@@ -2260,32 +2260,38 @@ def step_tables(master: torch.Tensor, entries: torch.Tensor, new_pages: torch.Te
     row, tokens, first position) of those that bring more.  Places behind the last token or item are left
     as they were.  An entry that does not fit (a row, page, place or token outside of what it is given)
     sets the error word; its table is zero, its slots are -1."""
-    _want_int_table(master, "step_tables", "master")
     given = (master, entries, new_pages, q_start, positions, seq_of_token, ctx_lens, slots, tables, err,
              decode_rows, prefill_items)
-    for i, t in enumerate(given):
-        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
-            _want(t, torch.int32, ("master", "entries", "new_pages", "q_start", "positions", "seq_of_token",
-                                   "ctx_lens", "slots", "tables", "err", "decode_rows", "prefill_items")[i])
-    _same_device("step_tables", *given)
-    B = entries.shape[0]
-    if entries.dim() != 2 or entries.shape[1] != 5 or page_size < 1 or num_pages < 1:
+    here = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else None
+    for t in given:
+        if t is not None and (t.get_device() != here or t.dtype != torch.int32 or not t.is_contiguous()):
+            for u, name in zip(given, ("master", "entries", "new_pages", "q_start", "positions", "seq_of_token",
+                                       "ctx_lens", "slots", "tables", "err", "decode_rows", "prefill_items")):
+                if u is not None:
+                    _want(u, torch.int32, name)
+            _same_device("step_tables", *given)
+            break
+    if master.dim() != 2 or entries.dim() != 2 or tables.dim() != 2 or not master.numel():
+        raise KernelError("step_tables: master, entries and tables must have two dimensions")
+    master_rows, master_width = master.shape
+    (B, five), (table_rows, width) = entries.shape, tables.shape
+    if five != 5 or page_size < 1 or num_pages < 1:
         raise KernelError("step_tables: entries must be [B, 5], pages of at least one token")
     T = min(positions.numel(), seq_of_token.numel(), slots.numel())
-    if (tables.dim() != 2 or tables.shape[0] < B or q_start.numel() < B + 1 or ctx_lens.numel() < B
-            or num_pages * page_size > 1 << 31):
+    if table_rows < B or q_start.numel() < B + 1 or ctx_lens.numel() < B or num_pages * page_size > 1 << 31:
         raise KernelError("step_tables: tables must be [B, width], q_start [B + 1], ctx_lens [B], and a "
                           "slot a 32-bit number")
     if B == 0:
         return
-    n_dec = decode_rows.numel() if decode_rows is not None else 0
-    n_pf = prefill_items.numel() // 4 if prefill_items is not None else 0
-    _run("step_tables", _step_tables_call, master.data_ptr(), master.shape[0],
-         master.shape[1], entries.data_ptr(), B, new_pages.data_ptr(), new_pages.numel(), page_size, num_pages,
-         q_start.data_ptr(), positions.data_ptr(), seq_of_token.data_ptr(), ctx_lens.data_ptr(),
-         slots.data_ptr(), T, tables.data_ptr(), tables.shape[1],
-         decode_rows.data_ptr() if decode_rows is not None else 0, n_dec,
-         prefill_items.data_ptr() if prefill_items is not None else 0, n_pf, err.data_ptr(), _stream_at(master))
+    rows_ptr = n_dec = items_ptr = n_pf = 0
+    if decode_rows is not None:
+        rows_ptr, n_dec = decode_rows.data_ptr(), decode_rows.numel()
+    if prefill_items is not None:
+        items_ptr, n_pf = prefill_items.data_ptr(), prefill_items.numel() // 4
+    _run("step_tables", _step_tables_call, master.data_ptr(), master_rows, master_width, entries.data_ptr(), B,
+         new_pages.data_ptr(), new_pages.numel(), page_size, num_pages, q_start.data_ptr(), positions.data_ptr(),
+         seq_of_token.data_ptr(), ctx_lens.data_ptr(), slots.data_ptr(), T, tables.data_ptr(), width, rows_ptr, n_dec,
+         items_ptr, n_pf, err.data_ptr(), _stream_at(master))
 
 
 class DiffCombine:
