@@ -1,4 +1,5 @@
 """The operators of a paged cache held in 4 bits against their restatement in 64 bits."""
+import gc
 import math
 import random
 
@@ -463,6 +464,7 @@ def test_two_graphs_and_an_eager_call_share_nothing(cuda_device):
     for f, o in ((decode, outs[0]), (prefill, outs[1])):
         f(o)
         torch.cuda.synchronize()
+        gc.collect()                          # (not in the middle of the capture)
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             f(o)
@@ -535,6 +537,7 @@ def test_a_chain_of_layers_described_once(cuda_device, rows_new):
         got = run(True)
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+        gc.collect()                          # (not in the middle of the capture)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=stream):
             got = run(True)
