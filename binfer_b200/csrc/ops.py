@@ -1957,7 +1957,11 @@ def token_rows(n: int, device) -> torch.Tensor:
     size = max(64, 1 << (n - 1).bit_length())
     got = _token_rows.get((device, size))
     if got is None:
-        got = _token_rows[(device, size)] = torch.arange(size, dtype=torch.int32, device=device)
+        got = torch.arange(size, dtype=torch.int32, device=device)
+        if torch.cuda.is_current_stream_capturing():
+            return got[:n]              # the graph's own: it holds nothing before a replay
+        torch.cuda.current_stream().synchronize()           # other streams may read it
+        _token_rows[(device, size)] = got
     return got[:n]
 
 

@@ -225,6 +225,19 @@ def test_norm_rotation_and_store_in_one(cuda_device, T, nh, nkv, d, ps, rot, nor
     assert T < 21 or got.any()
 
 
+def test_token_rows_first_asked_for_in_a_capture(cuda_device):
+    from binfer_b200.csrc import ops
+    ops._token_rows.clear()
+    gc.collect()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        inside = ops.token_rows(100, cuda_device) + 1
+    assert ops.token_rows(100, cuda_device).tolist() == list(range(100))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert inside.tolist() == list(range(1, 101)) and ops.token_rows(70, cuda_device).tolist() == list(range(70))
+
+
 # ------------------------------------------------------------------------------ attention
 def _attention(c, q, out, nh, jobs, decode, window, keep, scale):
     """``jobs``: (request, rows, first position)."""
