@@ -36,8 +36,9 @@
 // some 258 instructions a unit of 2,304 bytes nearly fill the issue slots, so that bytes and instructions are
 // level; the rest is the beginning of the stretches (queries, tables, first units: 4 us) and their end, a wait for
 // the slowest SM.  Eight rows behind 4,096: 12.5 + 3 us (bytes: 5), in clusters of two 15; 30,000 keys behind a
-// window of 4,096, 12 rows of 16 heads: 18 + 3, a block a head 21 (8.7).  Tried without gain: partials added up in a block before the second kernel, barriers that
-// keep a block's warps level, fewer warps with a deeper ring, the lowest values as the product's addend.
+// window of 4,096, 12 rows of 16 heads: 18 + 3, a block a head 21 (8.7).  Tried without gain: partials added up in
+// a block before the second kernel, barriers that keep a block's warps level, fewer warps with a deeper ring, the
+// lowest values as the product's addend.
 #include "common.cuh"
 #include "kv4.cuh"
 #include "mma_utils.cuh"
@@ -230,7 +231,8 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
       int before = 0;
 #pragma unroll 1
       for (int e0 = 0; e0 < a.n_tiles; e0 += 32) {
-        const int e = e0 + lane, u = e < a.n_tiles ? units_of[e] : 0, n = aligned ? pieces_of(u) : u ? (u + KA_BEGIN) * pairs : 0;
+        const int e = e0 + lane, u = e < a.n_tiles ? units_of[e] : 0;
+        const int n = aligned ? pieces_of(u) : u ? (u + KA_BEGIN) * pairs : 0;
         int incl = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -330,7 +332,8 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
     for (int nt = 0; nt < NT; ++nt) {
       const int n = nt * 8 + r, ti = n * a.chunk_inverse >> 8, gi = n - ti * a.chunk;
       const bool on = ti < t.ntok && gi < heads;
-      const __nv_bfloat16* src = a.q + (long long)(t.row0 + (on ? ti : 0)) * a.q_stride + (size_t)(head0 + (on ? gi : 0)) * D;
+      const __nv_bfloat16* src =
+          a.q + (long long)(t.row0 + (on ? ti : 0)) * a.q_stride + (size_t)(head0 + (on ? gi : 0)) * D;
 #pragma unroll
       for (int w = 0; w < KW; ++w) {
         raw[nt][w] = *reinterpret_cast<const uint4*>(src + (w >> 1) * 64 + q4 * 16 + (w & 1) * 8);
@@ -630,7 +633,7 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
     constexpr int ROW = HEAD ? D + 8 : D;
     float* part_o = HEAD ? reinterpret_cast<float*>(smem) : a.part_o;
     float2* part_ml = HEAD ? reinterpret_cast<float2*>(tiles) : a.part_ml;
-    static_assert(!HEAD || (WARPS * COLS * ROW * 4 <= WARPS * KA_STAGES * UNIT_BYTES && WARPS * COLS * 8 <= KA_MAX_TILES * 16), "room");
+    static_assert(!HEAD || (COLS * ROW * 4 <= KA_STAGES * UNIT_BYTES && WARPS * COLS * 8 <= KA_MAX_TILES * 16), "room");
     if (HEAD) __syncthreads();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -678,7 +681,8 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
       };
       auto finish = [&](int id, const float (&v)[N], float l) {
         const int n = id / PER, ti = n * a.chunk_inverse >> 8, gi = n - ti * a.chunk;
-        __nv_bfloat16* dst = a.out + (long long)(t.row0 + ti) * a.out_stride + (size_t)(head0 + gi) * D + id % PER * (D / PER);
+        __nv_bfloat16* dst = a.out + (long long)(t.row0 + ti) * a.out_stride + (size_t)(head0 + gi) * D +
+                             id % PER * (D / PER);
 #pragma unroll
         for (int k = 0; k < N; ++k) dst[lane + 32 * k] = __float2bfloat16_rn(v[k] / l);
       };
@@ -907,8 +911,9 @@ static long long ka_slots(const KaShape& s, int d, int sms) { return 2LL * sms *
 // sweep of rows of equal length (replayed from a graph, launch included): a cluster 6.5 (several blocks 8.5) and `unit`
 // for each unit of a block, where all clusters are resident at once (74, 33 and 15 of two, four and eight blocks);
 // stretches `base`, `each` for every unit of all heads, of which a batch has three quarters of what its longest row
-// says (all of it where a window cuts them to one length, `even`), and `piece` for a head's pieces.  Heads of 128 (4 query heads each), stretches / 1, 2, 4, 8 blocks: 8 heads over 512
-// keys 10.7 / 8.6, 8.6, 8.6, 8.6, over 4,096 12.6 / 20.9, 14.8, 12.7, 10.6, over 16,384 19.0 / 62, 36, 23, 15.4; 32 heads over
+// says (all of it where a window cuts them to one length, `even`), and `piece` for a head's pieces.  Heads of 128
+// (4 query heads each), stretches / 1, 2, 4, 8 blocks: 8 heads over 512 keys 10.7 / 8.6, 8.6, 8.6, 8.6, over 4,096
+// 12.6 / 20.9, 14.8, 12.7, 10.6, over 16,384 19.0 / 62, 36, 23, 15.4; 32 heads over
 // 4,096 16.9 / 20.9, 14.7, 12.7; 72 over 4,096 19.0 / 20.9, 16.3; 128 over 512 14.7 / 8.7, over 4,096 27.2 / 21.0.
 static int ka_blocks_a_head(const KaShape& s, int d, long long tiles, int pairs, int keys, bool even, int sms) {
   struct Times {
@@ -933,7 +938,8 @@ static int ka_blocks_a_head(const KaShape& s, int d, long long tiles, int pairs,
 // no second kernel runs.  `keys`, `even` as the call's.
 BF_EXPORT long long bf_kv4_attention_scratch(int n, int max_rows, int nh, int nkv, int d, int sms, int keys, int even) {
   const KaShape s = ka_shape(nh / nkv, d, max_rows);
-  if (ka_blocks_a_head(s, d, (long long)n * ((max_rows + s.tokens - 1) / s.tokens), nkv * s.chunks, keys, even, sms)) return 0;
+  const long long all = (long long)n * ((max_rows + s.tokens - 1) / s.tokens);
+  if (ka_blocks_a_head(s, d, all, nkv * s.chunks, keys, even, sms)) return 0;
   const long long slots = ka_slots(s, d, sms);
   long long tiles = (long long)n * ((max_rows + s.tokens - 1) / s.tokens);
   if (tiles > KA_MAX_TILES) tiles = KA_MAX_TILES;
@@ -989,8 +995,12 @@ BF_EXPORT int bf_kv4_attention(const Kv4AttentionCall* call) {
   if (tiles > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
   const int share = ka_blocks_a_head(s, d, tiles, nkv * s.chunks, keys, even, sms);
   if (!share && !scratch) return (int)cudaErrorInvalidValue;
-  if (d == 64) return s.nt == 1 ? ka_launch<64, 1>(a, (int)tiles, share, sms, stream) : ka_launch<64, 2>(a, (int)tiles, share, sms, stream);
-  if (d == 128) return s.nt == 1 ? ka_launch<128, 1>(a, (int)tiles, share, sms, stream) : ka_launch<128, 2>(a, (int)tiles, share, sms, stream);
+  if (d == 64)
+    return s.nt == 1 ? ka_launch<64, 1>(a, (int)tiles, share, sms, stream)
+                     : ka_launch<64, 2>(a, (int)tiles, share, sms, stream);
+  if (d == 128)
+    return s.nt == 1 ? ka_launch<128, 1>(a, (int)tiles, share, sms, stream)
+                     : ka_launch<128, 2>(a, (int)tiles, share, sms, stream);
   if (d == 256) return ka_launch<256, 1>(a, (int)tiles, share, sms, stream);
   return (int)cudaErrorInvalidValue;
 }

@@ -90,7 +90,8 @@ kv4_store_kernel(const __nv_bfloat16* __restrict__ k, long long k_stride,
     *reinterpret_cast<uint2*>(rec + tok * (D / 2) + l * (D / 8) + g * 8) = make_uint2(code[0], code[1]);
   }
   if (l == 0)
-    *reinterpret_cast<unsigned*>(rec + (is_v ? kv4_value_params_at(D) : kv4_key_params_at(D)) + (tok * NG + g) * 4) = coder.pair;
+    *reinterpret_cast<unsigned*>(rec + (is_v ? kv4_value_params_at(D) : kv4_key_params_at(D)) + (tok * NG + g) * 4) =
+        coder.pair;
 }
 
 struct Kv4StoreCall {
@@ -158,7 +159,8 @@ kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
                 int table_stride, int table_rows, int table_width, const int* __restrict__ items, int n_items,
                 int T, __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out,
                 int* __restrict__ tables_out, int out_width, int* __restrict__ items_out,
-                unsigned char* __restrict__ special, int* __restrict__ beyond, int out_pages, int nkv, int page_size, int num_pages, int window, int keep, int* __restrict__ err) {
+                unsigned char* __restrict__ special, int* __restrict__ beyond, int out_pages, int nkv, int page_size,
+                int num_pages, int window, int keep, int* __restrict__ err) {
   constexpr int NG = D / KV4_GROUP, REC = kv4_record(D);
   bf_pdl_trigger();
   bf_pdl_wait();
@@ -334,7 +336,7 @@ BF_EXPORT int bf_kv4_load(const Kv4LoadCall* call) {
                tables_out, out_width, items_out, special, beyond, out_pages, nkv, d, page_size, num_pages,
                window, keep, sms, err, stream] = *call;
   if (n_items <= 0 || out_pages <= 1) return 0;
-  if ((special != nullptr) != (beyond != nullptr) || (special && d != 64 && d != 128 && d != 256)) return (int)cudaErrorInvalidValue;
+  if ((special != nullptr) != (beyond != nullptr)) return (int)cudaErrorInvalidValue;
   // heads apart where pages alone would leave SMs without blocks
   int parts = 1;
   while (parts < nkv && (long long)out_pages * parts < 4LL * sms) parts *= 2;
@@ -345,11 +347,9 @@ BF_EXPORT int bf_kv4_load(const Kv4LoadCall* call) {
                          (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, tables_out, out_width, items_out,
                          (unsigned char*)special, beyond, out_pages, nkv, page_size, num_pages, window, keep, err);
   };
-  if (special)
-    return d == 64 ? run(kv4_load_kernel<64, true>) : d == 128 ? run(kv4_load_kernel<128, true>) : run(kv4_load_kernel<256, true>);
-  if (d == 64) return run(kv4_load_kernel<64, false>);
-  if (d == 128) return run(kv4_load_kernel<128, false>);
-  if (d == 256) return run(kv4_load_kernel<256, false>);
+  if (d == 64) return special ? run(kv4_load_kernel<64, true>) : run(kv4_load_kernel<64, false>);
+  if (d == 128) return special ? run(kv4_load_kernel<128, true>) : run(kv4_load_kernel<128, false>);
+  if (d == 256) return special ? run(kv4_load_kernel<256, true>) : run(kv4_load_kernel<256, false>);
   return (int)cudaErrorInvalidValue;
 }
 
