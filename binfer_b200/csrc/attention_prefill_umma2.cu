@@ -155,9 +155,11 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
   uint64_t* s_full = kv_empty + STAGES;     // [group][2]: one per S buffer
   uint64_t* p_full = s_full + 4;               // [group][2], 8 arrivals (one a warp): P of the tiles of that parity
   uint64_t* o_done = p_full + 4;               // [group][2]: P V of the tiles of that parity
-  uint64_t* q_half = o_done + 4;               // HALF: [group], the Q tile is fp16
+  uint64_t* drain = o_done + 4;                // [2], one per MMA thread, for what is in flight when a wait gives up
+  uint64_t* q_half = drain + 2;                // HALF: [group], the Q tile is fp16
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_half + (HALF ? 2 : 0));
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* asked = abort + 1;             // K and V tiles that copies were asked for, once that warp is done
 
   if constexpr (HALF) {                        // (its keys come from the kernel ahead, another looks at its result)
     bf_pdl_wait();
@@ -215,8 +217,10 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
       mbar_init(o_done + s, 1);
       mbar_init(p_full + s, 8);
     }
-    if (HALF)
-      for (int s = 0; s < 2; ++s) mbar_init(q_half + s, 8);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(drain + s, 1);
+      if (HALF) mbar_init(q_half + s, 8);
+    }
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -236,6 +240,7 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
 
   if (warp == A2_TMA_WARP) {
     // ---------------------------------------------------------------- TMA producer
+    int filled = 0;                                      // places of the ring that copies were asked into
     if (lane == 0 && tiles > 0) {                        // (a share of the keys may be empty)
       if constexpr (DIFF) {                              // 64 columns of each map
         mbar_expect_tx(q_full, 2 * QHALF_BYTES);
@@ -254,37 +259,36 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
     }
     if constexpr (ONE) {
       // pages of 64 keys, read whole, in the order K 0, K 1, V 0, K 2, V 1, .. in which they are used
-      bool ok = true;
-      int c = 0;
-      auto fetch = [&](const CUtensorMap& map, int page) {
-        if (lane == 0) {
-          const int st = c % STAGES;
-          ok = ok && (c < STAGES || mbar_wait(kv_empty + st, (uint32_t)(c / STAGES - 1) & 1u, abort));
-          if (ok) {
-            mbar_expect_tx(kv_full + st, (uint32_t)K_BYTES);
+      int c = 0, mine = 0;
+      filled = ring_keys_values(
+          tiles,
+          [&](int n) {
+            if (n % 32 == 0) {
+              mine = n + lane < tiles ? table[tile_key(n + lane) / A2_BN] : 0;
+              if (mine < 0 || mine >= num_pages) {
+                atomicOr(err, BF_ERR_PAGE);
+                mine = 0;
+              }
+              if (mine > 0 && special[(size_t)mine * nkv + g]) atomicOr(beyond + (it - items) / 4 * nkv + g, 1);
+            }
+            return __shfl_sync(0xffffffffu, mine, n % 32);
+          },
+          [&](bool is_value, int page) {
+            bool ok = true;
+            if (lane == 0) {
+              const int st = c % STAGES;
+              ok = c < STAGES || mbar_wait(kv_empty + st, (uint32_t)(c / STAGES - 1) & 1u, abort);
+              if (ok) {
+                mbar_expect_tx(kv_full + st, (uint32_t)K_BYTES);
 #pragma unroll
-            for (int hh = 0; hh < HALVES; ++hh)
-              tma_load_2d(Ks + st * K_BYTES + hh * KHALF_BYTES, &map, kv_full + st, hh * 64, (page * nkv + g) * A2_BN);
-          }
-        }
-        ++c;
-      };
-      int mine = 0, before = 0;
-      for (int n = 0; n < tiles && !*abort; ++n) {
-        if (n % 32 == 0) {
-          mine = n + lane < tiles ? table[tile_key(n + lane) / A2_BN] : 0;
-          if (mine < 0 || mine >= num_pages) {
-            atomicOr(err, BF_ERR_PAGE);
-            mine = 0;
-          }
-          if (mine > 0 && special[(size_t)mine * nkv + g]) atomicOr(beyond + (it - items) / 4 * nkv + g, 1);
-        }
-        const int page = __shfl_sync(0xffffffffu, mine, n % 32);
-        fetch(map_k, page);
-        if (n > 0) fetch(map_v, before);
-        before = page;
-      }
-      if (tiles > 0 && !*abort) fetch(map_v, before);
+                for (int hh = 0; hh < HALVES; ++hh)
+                  tma_load_2d(Ks + st * K_BYTES + hh * KHALF_BYTES, is_value ? &map_v : &map_k, kv_full + st, hh * 64,
+                              (page * nkv + g) * A2_BN);
+              }
+            }
+            ++c;
+            return __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+          });
     } else if constexpr (LATENT) {
       // a portion's keys begin at a row that is a multiple of 64 of the expanded buffers, which
       // are zero up to the next one; block_tables holds that row per portion
@@ -305,6 +309,7 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
                         h * 2 * D + D + hh * 64, y);
           }
           tma_load_2d(Ks + st * K_BYTES + HALVES * KHALF_BYTES, &map_v, kv_full + st, 0, y);
+          filled = n + 1;
         }
       }
     } else {
@@ -317,7 +322,7 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
     const int my_i = lane / pages, my_pg = lane - my_i * pages;
     const unsigned gmask = (pages == 32 ? 0xffffffffu : ((1u << pages) - 1u)) << (my_i * pages);
     bool ok = true;
-    for (int nb = 0; nb < tiles && ok && !*abort; nb += tb) {
+    for (int nb = 0; nb < tiles && ok; nb += tb) {       // (`ok` is the same in all lanes)
       const int n_mine = nb + my_i;
       const int jp = tile_key(n_mine) + my_pg * page_size;
       const bool wanted = my_i < tb && n_mine < tiles && jp <= p_last &&
@@ -345,6 +350,7 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
           ok = mbar_wait(kv_empty + st, (uint32_t)(n / STAGES - 1) & 1u, abort);
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) break;
+        filled = n + 1;
         uint8_t* vb = Vs + st * V_BYTES;
         // V rows of pages that are not fetched must read as zero (the first tile of a
         // window, the last tile of the portion)
@@ -390,6 +396,7 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
       }
     }
     }
+    if (lane == 0) *asked = filled;
   } else if (warp >= A2_MMA_WARP) {
     // ----------------------------------------------------------------- MMA issuers
     // One warp per query tile, converged, one elected lane issuing (umma_utils.cuh).  The two warps'
@@ -797,7 +804,19 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
   }
 
   __syncthreads();
-  if (*abort && threadIdx.x == 0) atomicOr(err, BF_ERR_WAIT);
+  if (*abort) {                                          // what is still in flight lands or ends first
+    if (threadIdx.x == 0) atomicOr(err, BF_ERR_WAIT);
+    if (warp == A2_TMA_WARP && lane == 0) {
+      const int filled = *asked;
+      if (filled > 0) mbar_drain_one(q_full, 0);
+      mbar_drain(kv_full, STAGES, filled % STAGES, (uint32_t)(filled / STAGES) & 1u);
+    }
+    if (warp >= A2_MMA_WARP) {
+      umma_commit(drain + warp - A2_MMA_WARP);
+      mbar_drain_one(drain + warp - A2_MMA_WARP, 0);
+    }
+    __syncthreads();
+  }
   if (warp == A2_MMA_WARP) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base),

@@ -32,3 +32,23 @@ struct OnePlace {
     ring_drain(1, 0, asked & 1u, landed);
   }
 };
+
+// One ring of key and value tiles that a warp fills in the order in which they are used: K 0, K 1, V 0, K 2, V 1, ..
+// page_of(n) and fill(is_value, page) are calls of the whole warp, whose lanes may be apart.  fill answers every lane as
+// the copying lane's wait went, so that all of them leave together: a lane that goes on alone would wait
+// for the others in the next call for good.  Returns how many fills were asked for.
+template <class PageOf, class Fill>
+BF_HOST_DEVICE inline int ring_keys_values(int tiles, PageOf page_of, Fill fill) {
+  int asked = 0, before = 0;
+  for (int n = 0; n < tiles; ++n) {
+    const int page = page_of(n);
+    if (!fill(false, page)) return asked;
+    ++asked;
+    if (n > 0) {
+      if (!fill(true, before)) return asked;
+      ++asked;
+    }
+    before = page;
+  }
+  return tiles > 0 && fill(true, before) ? asked + 1 : asked;
+}
