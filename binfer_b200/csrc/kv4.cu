@@ -140,7 +140,8 @@ struct KvBool {
 // A block takes 64 tokens of one portion's context and every gridDim.y-th kv head and writes them as bfloat16
 // pages [64][d] of keys and of values, a warp a record of eight tokens; the blocks of page 0 write zeros.
 // Where a portion's pages begin is a sum over the portions before it; one that names a request, places or token
-// rows that are not there, or more places than a row of the table has, has none.  What no row of the portion sees is
+// rows that are not there, or more places than a row of the table has, has none, and one that the pages left have no
+// room for has zeros: its row of the table, which no block of its own can be sure to write, and its pages.  What no row of the portion sees is
 // zero (a page of nothing else is left out and its place in the table is page 0).  The blocks of a portion
 // write its row of the table together.  4,096 tokens of 8 heads of 128: 6.0 us (21.5 MB, 3.3 at the rate of a copy),
 // 8,448 10.8 (6.8): a block's way to its page, and stores.  Several heads a block, one after the other, took longer
@@ -212,11 +213,16 @@ kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
     running += __shfl_sync(0xffffffffu, incl, 31);
   }
   if (page == 0 && blockIdx.y == 0) {
-    for (int i = 0; i < n_items; ++i)                       // (portions without a page of their own)
-      if (pages_of(items[4 * i], items[4 * i + 1], items[4 * i + 2], items[4 * i + 3]) <= 0)
+    long long to = 0;                                       // portions without pages, or without room for all of them
+    for (int i = 0; i < n_items; ++i) {
+      const int n = pages_of(items[4 * i], items[4 * i + 1], items[4 * i + 2], items[4 * i + 3]);
+      to += max(n, 0);
+      if (n <= 0 || to > out_pages - 1)
         for (int w = tid; w < out_width; w += 256) tables_out[(size_t)i * out_width + w] = 0;
+    }
   }
-  if (page == 0 || item < 0) {                              // the zero page, and pages behind the last context
+  if (item >= 0 && (long long)base + (n_rows + first - 1) / 64 + 1 > out_pages - 1) item = -1;
+  if (page == 0 || item < 0) {                              // the zero page, and pages of no portion with room
     for (int h = blockIdx.y; h < nkv; h += gridDim.y) {
       const size_t at = ((size_t)page * nkv + h) * 64 * D;
       for (int i = tid; i < 64 * D / 8; i += 256) {
@@ -234,8 +240,7 @@ kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
     const int w1 = place + 1 < n_places ? (int)((long long)out_width * (place + 1) / n_places) : out_width;
     for (int w = (int)((long long)out_width * place / n_places) + tid; w < w1; w += 256)
       tables_out[(size_t)item * out_width + w] =
-          w < n_places && base + w + 1 < out_pages && kv4_seen(w * 64, w * 64 + 63, first, last, window, keep)
-              ? base + w + 1 : 0;
+          w < n_places && kv4_seen(w * 64, w * 64 + 63, first, last, window, keep) ? base + w + 1 : 0;
   }
   const int j64 = place * 64;
   if (!kv4_seen(j64, j64 + 63, first, last, window, keep)) return;

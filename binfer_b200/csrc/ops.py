@@ -2006,9 +2006,10 @@ def kv4_load(cache: torch.Tensor, block_tables: torch.Tensor, items: torch.Tenso
     rounded up to 64.  Page 0 is zero, so are places behind a context and, with ``window`` and
     ``keep_first``, keys that no row of the portion sees (pages of nothing else are not written, their
     place in ``tables`` is page 0).  A portion of a request or places that the block tables do not have, or
-    without room, sets the error word and has page 0 everywhere.  ``items_out``: takes the items with the portion's number in the
-    request's place, which goes with ``tables``; ``places``: the width of ``tables``, where a portion's
-    longest context is known to be shorter than all together."""
+    without room, sets the error word and has page 0 everywhere (one that is longer than ``tables`` are wide takes no
+    room from those behind it).  ``items_out``: takes the items with the portion's number in the
+    request's place, which goes with ``tables``, and no rows where there was no room; ``places``: the width of
+    ``tables``, where a portion's longest context is known to be shorter than all together."""
     table_rows, table_width, table_stride = _want_int_table(block_tables, "kv4_load", "block_tables")
     _want(items, torch.int32, "items"); _want(err, torch.int32, "err")
     pages, nkv, ps, d = _kv4_check("kv4_load", cache, block_tables, items, err, items_out)

@@ -1,0 +1,59 @@
+"""The operators of a cache in 4 bits where they were once wrong."""
+import math
+
+import pytest
+import torch
+
+import kv4_plain as K4
+from test_kv4_gpu import Cache
+
+pytestmark = pytest.mark.gpu
+
+BF16, F64, I32 = torch.bfloat16, torch.float64, torch.int32
+
+
+# ------------------------------------------------------------------------------ portions without room
+@pytest.fixture
+def filled(monkeypatch):
+    """Memory that a call takes is full of what it does not want: 77, and NaN."""
+    real = torch.empty_strided
+
+    def empty(*a, **kw):
+        t = real(*a, **kw)
+        return t.fill_(math.nan) if t.dtype == BF16 else t.fill_(77) if t.dtype == I32 else t
+    monkeypatch.setattr(torch, "empty_strided", empty)
+
+
+@pytest.mark.parametrize("d,ps,nkv", [(128, 16, 2), (64, 8, 1), (256, 128, 3)])
+@pytest.mark.parametrize("lens,rows", [([128, 128], 128), ([100, 128], 192), ([128], 64), ([200, 60], 128),
+                                       ([60, 200, 60], 192), ([64, 64, 64], 192)])
+@pytest.mark.parametrize("places", [0, 9])
+def test_load_of_portions_without_room(cuda_device, filled, d, ps, nkv, lens, rows, places):
+    """A portion without room, or with room for a part of it: page 0 everywhere in its row of the tables, its error bit,
+    no rows; the others whole, and zeros where no portion lies.  A portion that its row of the tables has no places for takes
+    no room from those behind it."""
+    from binfer_b200.csrc import ops
+    width, fit, taken = places or rows // 64, [], 0
+    for n in lens:
+        own = -(-n // 64)
+        taken += own if own <= width else 0
+        fit.append(own <= width and taken <= rows // 64)
+    c = Cache(lens, nkv, d, ps, cuda_device, seed=ps)
+    n = len(lens)
+    items = torch.tensor([(b, 2 * b, 2, lens[b] - 2) for b in range(n)], dtype=I32, device=cuda_device)
+    moved = torch.full_like(items, 77)
+    k, v, tables = ops.kv4_load(c.cache, c.tables, items, n, rows, c.err, items_out=moved, places=places)
+    assert int(c.err.item()) == (0 if all(fit) else 16)
+    assert moved.tolist() == [[b, 2 * b, 2 if fit[b] else 0, lens[b] - 2] for b in range(n)]
+    page = 1
+    for b in range(n):
+        own = -(-lens[b] // 64)
+        want = [page + i if fit[b] and i < own else 0 for i in range(width)]
+        assert tables[b].tolist() == want, b
+        if fit[b]:
+            for x, h in ((k, c.held(b)[0]), (v, c.held(b)[1])):
+                got = x[page:page + own].transpose(1, 2).reshape(-1, nkv, d).to(F64)
+                assert ((got[:lens[b]] - h).abs() <= 1.001 * K4.HALF_STEP * h.abs()).all() and not got[lens[b]:].any()
+            page += own
+    for x in (k, v):
+        assert not x[0].any() and not x[page:].any()
