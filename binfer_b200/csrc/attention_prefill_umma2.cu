@@ -484,20 +484,23 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
         // the group's Q tile, an eighth a warp: bfloat16 -> fp16, element by element where it lies
         if (mbar_wait(q_full, 0, abort)) {
           uint4* tile = reinterpret_cast<uint4*>(Qs + grp * Q_BYTES);
+          // rows behind the portion's last are another request's: they are converted, but do not count
+          const int own = qlen - qb * BROWS - grp * TSHIFT;
           uint32_t most = 0;
 #pragma unroll 4
           for (int i = (warp & 7) * 32 + lane; i < Q_BYTES / 16; i += 256) {
             uint4 x = tile[i];
             uint32_t* w = &x.x;
+            const uint32_t counts = ((i >> 3) & (A2_BM - 1)) < own ? 0x7fff7fffu : 0u;     // (eight lanes a row)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              most = __vmaxu2(most, w[k] & 0x7fff7fffu);
+              most = __vmaxu2(most, w[k] & counts);
               const __half2 f = __floats2half2_rn(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
               w[k] = *reinterpret_cast<const uint32_t*>(&f);
             }
             tile[i] = x;
           }
-          // (0x4780: 65,536; rows behind the portion's last count too, which only costs time)
+          // (0x4780: 65,536)
           if ((most & 0xffffu) >= 0x4780u || (most >> 16) >= 0x4780u) atomicOr(beyond + (it - items) / 4 * nkv + g, 1);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");

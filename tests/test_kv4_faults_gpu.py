@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import kv4_plain as K4
-from test_kv4_gpu import Cache
+from test_kv4_gpu import Cache, _queries
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +57,28 @@ def test_load_of_portions_without_room(cuda_device, filled, d, ps, nkv, lens, ro
             page += own
     for x in (k, v):
         assert not x[0].any() and not x[page:].any()
+
+
+# ------------------------------------------------------------------------------ a portion beside others
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows", [100, 300])
+def test_a_portion_s_bits_do_not_depend_on_the_rows_behind_it(cuda_device, d, rows):
+    """The next request's queries, which the same tile of 128 rows reads: beyond fp16, infinite, not a number."""
+    from binfer_b200.csrc import ops
+    nh, nkv, n = 4, 2, 400
+    c = Cache([n, 50], nkv, d, 16, cuda_device, seed=3)
+    q = _queries(rows + 50, nh, d, cuda_device)
+    items = torch.tensor([(0, 0, rows, n - rows), (1, rows, 50, 0)], dtype=I32, device=cuda_device)
+
+    def run(q):
+        out = torch.zeros_like(q)
+        ops.kv4_prefill_attention(q, c.cache, items, 2, rows, c.tables, out, nh, nkv, d, None, d ** -0.5, c.err,
+                                  ctx_rows=448 + 64, max_ctx=n, variant="load")
+        return out[:rows]
+
+    alone = run(q)
+    for what in (2.0 ** 20, math.inf, math.nan):
+        other = q.clone()
+        other[rows:] = what
+        assert torch.equal(run(other), alone), what
+    assert int(c.err.item()) == 0
