@@ -80,6 +80,7 @@
 
 #include "attention_diff.cuh"
 #include "common.cuh"
+#include "kv4.cuh"
 #include "tma_utils.cuh"
 #include "umma_utils.cuh"
 
@@ -482,26 +483,37 @@ prefill_attention_umma2_kernel(const __grid_constant__ CUtensorMap map_q,
       // maximum and sum are two shuffles away: the group's warps never wait for each other.
       if constexpr (HALF) {
         // the group's Q tile, an eighth a warp: bfloat16 -> fp16, element by element where it lies
-        if (mbar_wait(q_full, 0, abort)) {
+        if (mbar_wait_warp(q_full, 0, abort)) {
           uint4* tile = reinterpret_cast<uint4*>(Qs + grp * Q_BYTES);
           // rows behind the portion's last are another request's: they are converted, but do not count
           const int own = qlen - qb * BROWS - grp * TSHIFT;
-          uint32_t most = 0;
+          // with a large scale a row's 64 numbers that are all below fp16's ordinary ones count too (0x3880: 2^-14)
+          const bool mind_small = scale_log2 > KV4_SMALL_SCALE * 1.4426950408889634f;
+          static_assert(KV4_SMALL == 0x1p-14f, "the bits above");
+          uint32_t most = 0, small = 0;
 #pragma unroll 4
           for (int i = (warp & 7) * 32 + lane; i < Q_BYTES / 16; i += 256) {
             uint4 x = tile[i];
             uint32_t* w = &x.x;
             const uint32_t counts = ((i >> 3) & (A2_BM - 1)) < own ? 0x7fff7fffu : 0u;     // (eight lanes a row)
+            uint32_t top = 0;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              most = __vmaxu2(most, w[k] & counts);
+              top = __vmaxu2(top, w[k] & counts);
               const __half2 f = __floats2half2_rn(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
               w[k] = *reinterpret_cast<const uint32_t*>(&f);
             }
             tile[i] = x;
+            most = __vmaxu2(most, top);
+            if (mind_small) {                              // a byte of a vote is a row's 64
+              const uint32_t some = __ballot_sync(0xffffffffu, top != 0);
+              const uint32_t large = __ballot_sync(0xffffffffu, (top & 0xffffu) >= 0x3880u || (top >> 16) >= 0x3880u);
+              small |= __vcmpne4(some, 0u) & __vcmpeq4(large, 0u);
+            }
           }
           // (0x4780: 65,536)
-          if ((most & 0xffffu) >= 0x4780u || (most >> 16) >= 0x4780u) atomicOr(beyond + (it - items) / 4 * nkv + g, 1);
+          if (small != 0 || (most & 0xffffu) >= 0x4780u || (most >> 16) >= 0x4780u)
+            atomicOr(beyond + (it - items) / 4 * nkv + g, 1);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -884,7 +896,7 @@ __global__ void prefill_attention_merge_kernel(const float* __restrict__ part_o,
 // multiplied by `out_scale`; a logit per head in the softmax's denominator (`sinks`, or null); with a
 // window, the first `keep` tokens that stay visible behind it.  `beyond` (int [n_items, nkv],
 // zero, or null): keys and values are fp16 in pages of 64, and an entry becomes 1 where a query is beyond fp16's
-// range or the portion reads a page of the head whose word of `special` ([num_pages, nkv]) is not zero.
+// range (or, with a scale above KV4_SMALL_SCALE, so small that fp16 has few bits for it) or the portion reads a page of the head whose word of `special` ([num_pages, nkv]) is not zero.
 static int launch_umma2(
     const void* q, const void* k_cache, const void* v_cache, const int* items, int n_items,
     int max_rows, int total_rows, const int* block_tables, int table_stride, void* out, int nh,

@@ -151,7 +151,8 @@ struct KvBool {
 // m + s c has up to twelve bits, of which bfloat16 keeps eight (the result's error was 0.0036 of its rms
 // with both in bfloat16, 0.0027 with the values and probabilities; its own rounding to bfloat16 alone is
 // 0.0017).  A byte a record then says whether it holds a key or value beyond fp16's range, a group of values
-// so small that fp16 has less than half a step of 2^-11 for its largest, or a value that is not finite (a
+// so small that fp16 has less than half a step of 2^-11 for its largest, a group of keys that is (`small_key`,
+// where the scale makes it matter), or a value that is not finite (a
 // probability of zero times such a value is NaN: whole tiles would carry it into rows that do not see it);
 // kv4_rest_kernel computes what is concerned.
 template <int D, bool HALF>
@@ -161,7 +162,7 @@ kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
                 int T, __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out,
                 int* __restrict__ tables_out, int out_width, int* __restrict__ items_out,
                 unsigned char* __restrict__ special, int* __restrict__ beyond, int out_pages, int nkv, int page_size,
-                int num_pages, int window, int keep, int* __restrict__ err) {
+                int num_pages, int window, int keep, float small_key, int* __restrict__ err) {
   constexpr int NG = D / KV4_GROUP, REC = kv4_record(D);
   bf_pdl_trigger();
   bf_pdl_wait();
@@ -299,7 +300,10 @@ kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
         const unsigned w0 = __shfl_sync(0xffffffffu, kw[2 * g], from), w1 = __shfl_sync(0xffffffffu, kw[2 * g + 1], from);
         dst[half * 4] = on ? eight(q & 1 ? w1 : w0, s, m, KvBool<HALF>()) : zero;
       }
-      if (HALF) other |= on && (fabsf(m) > 65000.f || fabsf(fmaf(15.f, s, m)) > 65000.f);
+      if (HALF) {
+        const float most = fmaxf(fabsf(m), fabsf(fmaf(15.f, s, m)));
+        other |= on && (most > 65000.f || (most > 0.f && most < small_key));
+      }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float vs = kv4_scale(vp[e * NG + g]);
@@ -319,7 +323,8 @@ kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
   }
 }
 
-// special (8 bytes a page and head) and beyond (n_items x nkv), both or neither: keys and values in fp16.
+// special (8 bytes a page and head) and beyond (n_items x nkv), both or neither: keys and values in fp16, for scores
+// times `scale`.
 struct Kv4LoadCall {
   const void* cache;
   const int* block_tables;
@@ -333,13 +338,14 @@ struct Kv4LoadCall {
   void* special;
   int* beyond;
   int out_pages, nkv, d, page_size, num_pages, window, keep, sms;
+  float scale;
   int* err;
   cudaStream_t stream;
 };
 BF_EXPORT int bf_kv4_load(const Kv4LoadCall* call) {
   const auto& [cache, block_tables, table_stride, table_rows, table_width, items, n_items, T, k_out, v_out,
                tables_out, out_width, items_out, special, beyond, out_pages, nkv, d, page_size, num_pages,
-               window, keep, sms, err, stream] = *call;
+               window, keep, sms, scale, err, stream] = *call;
   if (n_items <= 0 || out_pages <= 1) return 0;
   if ((special != nullptr) != (beyond != nullptr)) return (int)cudaErrorInvalidValue;
   // heads apart where pages alone would leave SMs without blocks
@@ -350,7 +356,8 @@ BF_EXPORT int bf_kv4_load(const Kv4LoadCall* call) {
     return bf_launch_pdl(kern, dim3(out_pages, parts), dim3(256), 0, stream, (const unsigned char*)cache,
                          block_tables, table_stride, table_rows, table_width, items, n_items, T,
                          (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, tables_out, out_width, items_out,
-                         (unsigned char*)special, beyond, out_pages, nkv, page_size, num_pages, window, keep, err);
+                         (unsigned char*)special, beyond, out_pages, nkv, page_size, num_pages, window, keep,
+                         scale > KV4_SMALL_SCALE ? KV4_SMALL : 0.f, err);
   };
   if (d == 64) return special ? run(kv4_load_kernel<64, true>) : run(kv4_load_kernel<64, false>);
   if (d == 128) return special ? run(kv4_load_kernel<128, true>) : run(kv4_load_kernel<128, false>);

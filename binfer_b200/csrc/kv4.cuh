@@ -19,6 +19,12 @@
 #define KV4_GROUP 64
 #define KV4_EIGHTH 8                       // tokens of a record
 
+// Loaded keys and queries are fp16, which holds a number below 2^-14 to 2^-25 only.  A key or query off by that moves a
+// score by 2^-25 / sqrt(3) times the other's length times the scale: at this scale and the largest numbers that fp16 has,
+// 0.002 for heads of 256, otherwise far less.  With a larger scale, groups of 64 with nothing larger count as beyond fp16.
+#define KV4_SMALL_SCALE 0.125f
+#define KV4_SMALL 0x1p-14f
+
 __host__ __device__ constexpr int kv4_record(int d) { return 9 * d; }
 __host__ __device__ constexpr int kv4_values_at(int d) { return 4 * d; }
 __host__ __device__ constexpr int kv4_key_params_at(int d) { return 8 * d; }

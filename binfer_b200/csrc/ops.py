@@ -1916,7 +1916,7 @@ class _Packed:
 
 
 _kv4_store_call = _Packed("bf_kv4_store", "PqPqPPiiiiqPP")
-_kv4_load_call = _Packed("bf_kv4_load", "PPiiiPiiPPPiPPPiiiiiiiiPP")
+_kv4_load_call = _Packed("bf_kv4_load", "PPiiiPiiPPPiPPPiiiiiiiifPP")
 _kv4_rest_call = _Packed("bf_kv4_rest", "PPPiiPPiPqPqiiiiiiifP")
 _kv4_attention_call = _Packed("bf_kv4_attention", "PqPPPPPiiiPiiiPqiiiiiiifPiiiiPP")
 _qk_norm_rope_kv4_call = _Packed("bf_qk_norm_rope_kv4_store", "PqPPPiPPPPiiiiiqfPiifPP")
@@ -2030,7 +2030,7 @@ def kv4_load(cache: torch.Tensor, block_tables: torch.Tensor, items: torch.Tenso
     _run("kv4_load", _kv4_load_call, cache.data_ptr(), block_tables.data_ptr(), table_stride, table_rows,
          table_width, items.data_ptr(), n_items, 0x7fffffff, k.data_ptr(), v.data_ptr(), tables.data_ptr(), places,
          items_out.data_ptr() if items_out is not None else 0, 0, 0, n, nkv, d, ps, pages, window, keep_first,
-         num_sms(device), err.data_ptr(), _stream_at(cache))
+         num_sms(device), 0.0, err.data_ptr(), _stream_at(cache))
     return k, v, tables
 
 
@@ -2208,7 +2208,7 @@ def _kv4_loaded_attention(q, cache, items, n_items, max_rows, block_tables, tabl
     stream = _stream_at(q)
     _run("kv4_load", _kv4_load_call, cache_ptr, table_ptr, table_stride,
          table_rows, table_width, item_ptr, n_items, T, k, v, tables, places, moved, special, beyond,
-         n, nkv, d, ps, pages, w, keep, sms, err_ptr, stream)
+         n, nkv, d, ps, pages, w, keep, sms, scale, err_ptr, stream)
     _run("prefill_attention_umma2", _prefill_attention_umma2_half_call,
          q_ptr, k, v, moved, n_items, max_rows, T, tables, places, out_ptr, nh, nkv, d, KV4_LOAD_PAGE, n, w, scale,
          splits, part_o, part_ml, err_ptr, out_stride, 1.0 / KV4_VALUE_UP, keep, beyond, special, stream)

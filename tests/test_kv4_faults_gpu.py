@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import kv4_plain as K4
+import kv4_units as U
 from test_kv4_gpu import Cache, _queries
 
 pytestmark = pytest.mark.gpu
@@ -81,4 +82,61 @@ def test_a_portion_s_bits_do_not_depend_on_the_rows_behind_it(cuda_device, d, ro
         other = q.clone()
         other[rows:] = what
         assert torch.equal(run(other), alone), what
+    assert int(c.err.item()) == 0
+
+
+# ------------------------------------------------------------------------------ numbers that fp16 has few bits for
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("variant", ["load", "auto", "stretches"])
+@pytest.mark.parametrize("key_size,query_size", [(-30, 0), (0, -30), (-20, 0), (0, -18), (-16, -16), (-20, -20), (12, -40),
+                                                 (-40, 12)])
+def test_small_keys_and_queries_with_a_large_scale(cuda_device, d, variant, key_size, query_size):
+    """Numbers below fp16's, whose scores a scale makes ordinary."""
+    from binfer_b200.csrc import ops
+    nh, nkv, n, new = 6, 3, 400, 100
+    c = Cache([n], nkv, d, 16, cuda_device, seed=9)
+    c.k[0] = U.keys(n, nkv, d, cuda_device, 1) * 2.0 ** key_size
+    c.v[0] = U.values(n, nkv, d, cuda_device, 2)
+    ops.kv4_store(c.k[0].flatten(1), c.v[0].flatten(1), c.slots[0], c.cache, c.err)
+    q = _queries(new, nh, d, cuda_device) * 2.0 ** query_size
+    scale = d ** -0.5 * 2.0 ** -(key_size + query_size)
+    items = torch.tensor([(0, 0, new, n - new)], dtype=I32, device=cuda_device)
+    out = torch.full_like(q, math.nan)
+    ops.kv4_prefill_attention(q, c.cache, items, 1, new, c.tables, out, nh, nkv, d, None, scale, c.err, ctx_rows=448,
+                              max_ctx=n, variant=variant)
+    k, v = c.held(0)
+    ref, allowed = U.attend(q.view(new, nh, d).to(F64), k, v, torch.arange(n - new, n, device=q.device), None, 0, scale)
+    U.check(out, ref, allowed)
+    assert int(c.err.item()) == 0
+
+
+@pytest.mark.parametrize("what", ["a row of queries", "a key", "a group of keys"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_some_small_keys_and_queries_with_a_large_scale(cuda_device, what, d):
+    """A few small numbers among ordinary ones; zeros, which fp16 has, beside them."""
+    from binfer_b200.csrc import ops
+    nh, nkv, n, new, scale = 4, 2, 300, 140, 64.0
+    c = Cache([n], nkv, d, 16, cuda_device, seed=9)
+    k, q = U.keys(n, nkv, d, cuda_device, 1) * d ** -0.5 / 64, _queries(new, nh, d, cuda_device)
+    c.v[0] = U.values(n, nkv, d, cuda_device, 2)
+    k[::7] = 0
+    q[5] = 0
+    if what == "a row of queries":                      # (the keys that it meets are as much larger)
+        q, k = q * 2.0 ** -10, k * 2.0 ** 10
+        q[133, d:2 * d] *= 2.0 ** -9
+    elif what == "a key":
+        k[201, 1] *= 2.0 ** -11
+        q = q * 2.0 ** 5
+    else:
+        k[:, 1, -64:] *= 2.0 ** -14
+        q.view(new, nh, d)[:, 2:, -64:] *= 2.0 ** 14
+    c.k[0] = k
+    ops.kv4_store(c.k[0].flatten(1), c.v[0].flatten(1), c.slots[0], c.cache, c.err)
+    items = torch.tensor([(0, 0, new, n - new)], dtype=I32, device=cuda_device)
+    kk, v = c.held(0)
+    ref, allowed = U.attend(q.view(new, nh, d).to(F64), kk, v, torch.arange(n - new, n, device=q.device), None, 0, scale)
+    out = torch.full_like(q, math.nan)
+    ops.kv4_prefill_attention(q, c.cache, items, 1, new, c.tables, out, nh, nkv, d, None, scale, c.err, ctx_rows=320,
+                              max_ctx=n, variant="load")
+    U.check(out, ref, allowed)
     assert int(c.err.item()) == 0
