@@ -1826,6 +1826,7 @@ KV4_HEAD_DIMS = (64, 128, 256)
 KV4_GROUP = 64               # numbers of a row that share a scale and a lowest value
 KV4_LOAD_PAGE = 64           # tokens of a page that kv4_load writes
 KV4_VALUE_UP = 16            # values in fp16 are so many times themselves (kv4.cu)
+KV4_MAX_SCALE = 2.0 ** 40    # the stretches' products carry 2^-69, which a scale above 2^58 takes out of a float
 
 
 def kv4_takes(dtype: torch.dtype, d: int, page_size: int) -> bool:
@@ -2041,9 +2042,11 @@ def _kv4_mask(what: str, window: Optional[int], keep_first: int) -> Tuple[int, i
     return (min(int(window), 1 << 30), min(int(keep_first), 1 << 30)) if window is not None else (0, 0)
 
 
-def _kv4_attention_check(what, q, cache, block_tables, out, nh, nkv, d, window, keep_first, err, *others):
+def _kv4_attention_check(what, q, cache, block_tables, out, nh, nkv, d, window, keep_first, scale, err, *others):
     """Of an attention call: (table rows, columns, stride), (rows of q, strides of q and out), pages, page
     size, window (0: none), kept tokens."""
+    if not abs(scale) <= KV4_MAX_SCALE:
+        raise KernelError(f"{what}: a scale of at most 2^40 in size, not {scale}")
     table = _want_int_table(block_tables, what, "block_tables")
     _want(err, torch.int32, "err")
     pages, c_nkv, ps, c_d = _kv4_check(what, cache, q, block_tables, out, err, *others)
@@ -2085,12 +2088,13 @@ def kv4_decode_attention(q: torch.Tensor, cache: torch.Tensor, rows: Optional[to
     ``described``: rows, requests, positions and tables were complete before the kernel ahead on the stream began
     (as in a step that is described once and then runs its layers); they are read under that kernel's end.
 
-    Queries below 2^62, values below 2^55 and scores below 1e30 in size: larger ones overflow inside."""
+    Queries below 2^62, values below 2^55 and scores below 1e30 in size: larger ones overflow inside; queries below
+    2^-48 may count as zero.  A scale above 2^40 in size is refused."""
     _want(seq_of_token, torch.int32, "seq_of_token"); _want(positions, torch.int32, "positions")
     if rows is not None:
         _want(rows, torch.int32, "rows")
     table, strides, pages, ps, w, keep = _kv4_attention_check(
-        "kv4_decode_attention", q, cache, block_tables, out, nh, nkv, d, window, keep_first, err, rows,
+        "kv4_decode_attention", q, cache, block_tables, out, nh, nkv, d, window, keep_first, scale, err, rows,
         seq_of_token, positions)
     T = strides[0]
     if (n_rows < 0 or (rows is None and n_rows > T) or (rows is not None and rows.numel() < n_rows)
@@ -2120,7 +2124,7 @@ def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Ten
     does, in fp16, into scratch of 4 d bytes a token and kv head, and attended on tcgen05), or ``auto``."""
     _want(items, torch.int32, "items")
     table, strides, pages, ps, w, keep = _kv4_attention_check(
-        "kv4_prefill_attention", q, cache, block_tables, out, nh, nkv, d, window, keep_first, err, items)
+        "kv4_prefill_attention", q, cache, block_tables, out, nh, nkv, d, window, keep_first, scale, err, items)
     if n_items < 0 or items.numel() < 4 * n_items or max_rows < 0 or ctx_rows < 0 or ctx_rows % 64:
         raise KernelError("kv4_prefill_attention: items must be [n_items, 4], ctx_rows a multiple of 64")
     if variant not in ("auto", "stretches", "load"):
