@@ -19,7 +19,7 @@ __device__ __forceinline__ int ks_row(int z, unsigned inverse) {
 // Four lanes take a group, a lane the sixteen numbers of its part of a key; units are (token, key or value,
 // kv head, group) in the order in which rows lie in memory.  The kernel is bound by its instructions, so
 // minimum and maximum are taken two bfloat16 numbers at a time and quotients are products (Kv4Coder; bfloat16
-// numbers make ties common).  2,048 tokens of 8 heads of 128: 5.1 us (10.8 MB, 1.6 at the rate of a copy); 13
+// numbers make ties common).  2,048 tokens of 8 heads of 128: 5.5 us (10.8 MB, 1.6 at the rate of a copy); 13
 // tokens 2.1, the launch and one round trip.
 template <int D, bool VEC>
 __global__ void __launch_bounds__(KS_THREADS)

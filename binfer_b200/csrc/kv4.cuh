@@ -42,11 +42,17 @@ __host__ __device__ constexpr int kv4_value_byte(int d, int tok, int i) {
 __device__ __forceinline__ float kv4_scale(unsigned pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float kv4_low(unsigned pair) { return __uint_as_float(pair & 0xffff0000u); }
 
+// x - lo, at least zero.  Where a float does not hold it (numbers of far apart sizes) its last bit is one: it lies on the
+// side of a border between codes, (c + 1/2) s of some thirteen bits, that the exact difference lies on.
+__device__ __forceinline__ float kv4_above(float x, float lo) {
+  const unsigned down = __float_as_uint(__fsub_rd(x, lo)), up = __float_as_uint(__fsub_ru(x, lo));
+  return __uint_as_float(down | ((down ^ up) & 1u));
+}
+
 // The code of a number, whatever its size: on x / 4, which is exact, so that no difference of finite numbers
-// overflows.  x - m and s are short enough that the float quotient falls on the side of a border that
-// the exact one falls on.
+// overflows.  s has eight bits, so that a quotient off a border by the difference's last bit is not rounded onto it.
 static __device__ __noinline__ unsigned kv4_any_code(float x, float lo, float s) {
-  return s > 0.f ? (unsigned)fminf(rintf((x * 0.25f - lo * 0.25f) / (s * 0.25f)), 15.f) : 0u;
+  return s > 0.f ? (unsigned)fminf(rintf(kv4_above(x * 0.25f, lo * 0.25f) / (s * 0.25f)), 15.f) : 0u;
 }
 
 // The codes of a group's numbers, from its extremes (NaN if one of them is).  As a rule (`quick`) the quotient is a
@@ -71,7 +77,7 @@ struct Kv4Coder {
   // quick: the product with 1 / s to the nearest, which is within one of it; the exact remainder says
   // whether it is the nearest, and of two equally near ones the even one
   __device__ __forceinline__ float quick_code(float x) const {
-    const float y = x - lo, u = fmaf(y, inverse, 12582912.f), c = u - 12582912.f, left = fmaf(-c, s, y);
+    const float y = kv4_above(x, lo), u = fmaf(y, inverse, 12582912.f), c = u - 12582912.f, left = fmaf(-c, s, y);
     const float limit = __float_as_uint(u) & 1u ? below : half;
     return fabsf(left) > limit ? c + copysignf(1.f, left) : c;
   }

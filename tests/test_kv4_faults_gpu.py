@@ -1,12 +1,13 @@
 """The operators of a cache in 4 bits where they were once wrong."""
 import math
+from fractions import Fraction
 
 import pytest
 import torch
 
 import kv4_plain as K4
 import kv4_units as U
-from test_kv4_gpu import Cache, _queries
+from test_kv4_gpu import Cache, _err, _queries
 
 pytestmark = pytest.mark.gpu
 
@@ -140,3 +141,62 @@ def test_some_small_keys_and_queries_with_a_large_scale(cuda_device, what, d):
                               max_ctx=n, variant="load")
     U.check(out, ref, allowed)
     assert int(c.err.item()) == 0
+
+
+# ------------------------------------------------------------------------------ codes
+def _border_rows():
+    """Groups whose lowest number is a whole number and a half of steps, with numbers beside zero that no float holds
+    beside it, so that the quotient is next to a border; and lowest numbers beside zero with numbers on a border."""
+    rows = torch.zeros((12, 64), dtype=F64)
+    for r, (low, step) in enumerate([(-3.0, 2.0), (-1.0, 2.0), (-5.0, 2.0), (-0.75, 0.5), (-3.0 * 2.0 ** 40, 2.0 ** 41),
+                                     (-3.0 * 2.0 ** -60, 2.0 ** -59)]):
+        rows[r, 0], rows[r, 1] = low, low + 15 * step
+        tiny = abs(low) * 2.0 ** -torch.arange(20.0, 50.0, dtype=F64)
+        rows[r, 2:32], rows[r, 32:62] = tiny, -tiny
+    for r, (low, step) in enumerate([(-2.0 ** -40, 2.0), (2.0 ** -40, 2.0), (-2.0 ** -60, 0.25), (2.0 ** -60, 0.25),
+                                     (-1e-36, 1e-3), (-2.0 ** 60, 2.0 ** 124)], 6):
+        rows[r] = step * (torch.arange(64, dtype=F64) % 15 + 0.5)
+        rows[r, 0], rows[r, 1] = low, 15 * step
+    return rows.to(torch.float32).to(BF16)
+
+
+def _held_exactly(x):
+    """``K4.held`` with quotients as fractions: 64 bits do not hold 0.125 + 2^-60 either."""
+    out = torch.empty(x.shape, dtype=F64)
+    for r, row in enumerate(x.cpu().to(F64).unflatten(-1, (-1, 64)).flatten(0, -2)):
+        low, high = row.min(), row.max()
+        s = ((high - low) / 15).to(BF16).to(F64)
+        codes = [min(15, round((Fraction(float(n)) - Fraction(float(low))) / Fraction(float(s)))) for n in row]
+        out.view(-1, 64)[r] = low + s * torch.tensor(codes, dtype=F64)
+    return out
+
+
+def test_codes_next_to_a_border(cuda_device):
+    from binfer_b200.csrc import ops
+    x = _border_rows().to(cuda_device)
+    T = x.shape[0]
+    c, err = ops.kv4_cache(3, 1, 8, 64, cuda_device), _err(cuda_device)
+    ops.kv4_store(x, x.flip(0).contiguous(), torch.arange(8, 8 + T, dtype=I32, device=cuda_device), c, err)
+    k, v = K4.unpack(c)
+    want = _held_exactly(x)
+    assert torch.equal(k.reshape(-1, 64)[8:8 + T], want) and torch.equal(v.reshape(-1, 64)[8:8 + T], want.flip(0))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_codes_next_to_a_border_behind_norms_and_rotation(cuda_device, d):
+    """The kernel of a model's layers, heads of 128 by a kernel of their own: the same codes."""
+    from binfer_b200.csrc import ops
+    rows = _border_rows()
+    if d == 128:
+        rows = torch.cat([rows, rows.flip(0)], 1)
+    x = rows.to(cuda_device)
+    T = x.shape[0]
+    qkv = torch.cat([x, x, x], 1)
+    freq = torch.zeros(d // 2, dtype=torch.float32, device=cuda_device)
+    want, got = ops.kv4_cache(3, 1, 8, d, cuda_device), ops.kv4_cache(3, 1, 8, d, cuda_device)
+    slots, err = torch.arange(8, 8 + T, dtype=I32, device=cuda_device), _err(cuda_device)
+    ops.kv4_store(x, x, slots, want, err)
+    ops.qk_norm_rope_kv4_store(qkv, None, None, freq, torch.zeros(T, dtype=I32, device=cuda_device), slots,
+                               torch.empty_like(x), got, 1, 1, d, 1e-6, err)
+    assert torch.equal(got, want)
+    assert torch.equal(K4.unpack(got)[0].reshape(-1, d)[8:8 + T], _held_exactly(x))
