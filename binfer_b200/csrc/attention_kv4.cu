@@ -31,6 +31,12 @@
 // eight blocks takes a tile and head whole: its warps leave their partials in shared memory, each block adds up its
 // own and the blocks theirs over distributed shared memory, and there is no second kernel.
 //
+// Portions that are loaded and attended on tcgen05 leave behind which of them, and which kv heads, fp16 had no room for
+// (kv4.cu): a block an SM takes those heads whole, one after the other, from the codes.  As a rule there are none, and a
+// block only reads that.  Calls of 2,048 rows from position 0, 32 heads of 128 (8): 84 us with nothing noted, 232
+// with one kv head, 371 with all; 256 rows behind 8,192 94, 195 and 299.  (A walk over the keys by multiply-adds took 40 and
+// 85 ms.)
+//
 // Measured (B200).  64 rows of 64 heads of 128 (8) behind 4,096 keys down to 2,700: 55 us and 5 for the second
 // kernel, where the 254 MB take 39 at the rate of a copy, 6.54 TB/s.  While all warps run they read 6.2 TB/s:
 // some 258 instructions a unit of 2,304 bytes nearly fill the issue slots, so that bytes and instructions are
@@ -73,7 +79,16 @@ struct KaArgs {
   float* part_o;
   float2* part_ml;
   int4* desc;
+  const int *beyond, *moved;                               // KA_AGAIN
+  int n_items, heads;
   int* err;
+};
+
+// What a block of the kernel does.
+enum KaForm {
+  KA_STRETCHES,                            // each warp one stretch of units
+  KA_HEAD,                                 // a cluster of a.share blocks takes a (tile, head) whole
+  KA_AGAIN                                 // a block takes (tile, head)s whole, one after the other, of those that `beyond` notes
 };
 
 struct KaTile {
@@ -123,11 +138,11 @@ __device__ __forceinline__ float ka_peer(const float* p, int rank) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
   return v;
 }
-// HEAD: a cluster of a.share blocks takes a (tile, head) whole; its warps share the units and add up in
-// shared memory.
-template <int D, int NT, bool HEAD>
+// HEAD: the warps of the block or cluster share a head's units and add up in shared memory.
+template <int D, int NT, KaForm FORM>
 __global__ void __launch_bounds__(32 * ka_warps(D, NT), 1)
 kv4_attention_kernel(const __grid_constant__ KaArgs a) {
+  constexpr bool HEAD = FORM != KA_STRETCHES, AGAIN = FORM == KA_AGAIN;
   constexpr int NG = D / KV4_GROUP, REC = kv4_record(D), UNIT_BYTES = 2 * REC;
   constexpr int KW = D / 32, COLS = 8 * NT, WARPS = ka_warps(D, NT);
   constexpr float UP = 1.8446744073709551616e19f;           // 2^64
@@ -180,6 +195,12 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   const int warps = gridDim.x * WARPS;
   int me = warp, each = 1, longer = 0, x = 0, x_end = 1;
   bool aligned = true;
+  if constexpr (AGAIN) {                                    // (as a rule nothing is noted)
+    int any = 0;
+    for (int i = tid; i < a.n_items * a.nkv; i += 32 * WARPS) any |= a.beyond[i];
+    if (!__syncthreads_or(any)) return;
+    x = blockIdx.x, x_end = a.heads;
+  }
   if constexpr (!HEAD) {
     // ---- tiles, and how their units are cut.  (Loops, not unrolled: what a launch runs once waits for its
     // instructions most of all.)
@@ -276,16 +297,25 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
     KaTile t;
     KaSpan span;
     if constexpr (HEAD) {
-      const int head = blockIdx.x / a.share, rank = blockIdx.x - head * a.share;
+      const int share = AGAIN ? 1 : a.share;
+      const int head = AGAIN ? x : blockIdx.x / share, rank = AGAIN ? 0 : blockIdx.x - head * share;
       e = head / pairs, pair = head - e * pairs;
-      t = tile_of(e, pair == 0 && rank == 0 && tid == 0);
-      begin(1);
-      if (t.ntok <= 0) return;
+      x = AGAIN ? x + gridDim.x : x_end;
+      if constexpr (AGAIN) {
+        const int i = e / a.tiles_per_item;
+        if (a.beyond[i * a.nkv + pair / a.chunks] == 0 || a.moved[4 * (size_t)i + 2] <= 0) continue;
+      }
+      t = tile_of(e, !AGAIN && pair == 0 && rank == 0 && tid == 0);
+      if (!AGAIN) begin(1);
+      if (t.ntok <= 0) {
+        if (AGAIN) continue;
+        return;
+      }
       span = ka_span(t, a.window, a.keep);
-      const int steps = (span.units + 1) >> 1, all = WARPS * a.share, w = warp * a.share + rank;
+      const int steps = (span.units + 1) >> 1, all = WARPS * share, w = warp * share + rank;
       const int few = steps / all, more = steps - few * all;
       u0 = 2 * (w * few + min(w, more));
-      mine = max(min(2 * (few + (w < more ? 1 : 0)), span.units - u0), 0), n_pieces = all, x = x_end;
+      mine = max(min(2 * (few + (w < more ? 1 : 0)), span.units - u0), 0), n_pieces = all;
     } else {
       // the tile of x: the last that begins at or before it, among every sixteenth and then among sixteen
       e = lane * 16;
@@ -706,9 +736,10 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
           for (int k = 0; k < N; ++k)
             acc[j][k] = fmaf(g, part_o[(w * COLS + n) * ROW + id % PER * (D / PER) + lane + 32 * k], acc[j][k]);
         }
-        if (a.share == 1) finish(id, acc[j], sum[j]);
+        if (AGAIN || a.share == 1) finish(id, acc[j], sum[j]);
       }
-      if (a.share > 1) {
+      if constexpr (AGAIN) __syncthreads();                 // (the next head's ring lies over the partials)
+      if (!AGAIN && a.share > 1) {
         // the blocks' sums, a column by one warp of one of them
         const int rank = blockIdx.x % a.share;
         __syncthreads();
@@ -841,13 +872,21 @@ static int ka_launch(KaArgs a, int total_tiles, int share, int sms, cudaStream_t
   static bool configured[BF_MAX_DEVICES];
   const int dev = bf_current_device();
   if (!configured[dev]) {
-    for (auto kern : {kv4_attention_kernel<D, NT, false>, kv4_attention_kernel<D, NT, true>}) {
+    for (auto kern : {kv4_attention_kernel<D, NT, KA_STRETCHES>, kv4_attention_kernel<D, NT, KA_HEAD>,
+                      kv4_attention_kernel<D, NT, KA_AGAIN>}) {
       const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
       if (e != cudaSuccess) return (int)e;
     }
     configured[dev] = true;
   }
   const int pairs = a.nkv * a.chunks;
+  if (a.beyond) {
+    const long long heads = (long long)total_tiles * pairs;
+    if (heads > 0x7fffffffLL - sms) return (int)cudaErrorInvalidValue;
+    a.heads = (int)heads;
+    return bf_launch_pdl(kv4_attention_kernel<D, NT, KA_AGAIN>, dim3(heads < sms ? (int)heads : sms), dim3(threads),
+                         smem, stream, a);
+  }
   // the units of a launch are counted in 32 bits
   const long long units = ((long long)a.table_width * a.page_size / KA_UNIT + 2 + KA_BEGIN) * pairs;
   if (units > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
@@ -866,7 +905,7 @@ static int ka_launch(KaArgs a, int total_tiles, int share, int sms, cudaStream_t
     attr[1].val.clusterDim.x = share, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_attention_kernel<D, NT, true>, a);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_attention_kernel<D, NT, KA_HEAD>, a);
     return e != cudaSuccess ? (int)e : bf_launch_status();
   }
   for (int first = 0; first < total_tiles; first += most) {
@@ -875,7 +914,7 @@ static int ka_launch(KaArgs a, int total_tiles, int share, int sms, cudaStream_t
     // heads with many pieces each (there are few of them): eight warps add a column's up
     const bool few = (long long)a.n_tiles * pairs * 8 < (long long)sms * ka_warps(D, NT);
     a.max_pieces = few ? sms * ka_warps(D, NT) : 64;
-    int e = bf_launch_pdl(kv4_attention_kernel<D, NT, false>, dim3(sms), dim3(threads), smem, stream, a);
+    int e = bf_launch_pdl(kv4_attention_kernel<D, NT, KA_STRETCHES>, dim3(sms), dim3(threads), smem, stream, a);
     if (e) return e;
     auto merge = [&](auto kern, int columns) {
       return bf_launch_pdl(kern, dim3(a.n_tiles * pairs, 8 * NT / columns), dim3(256), 0, stream,
@@ -963,11 +1002,14 @@ struct Kv4AttentionCall {
   int early;                                               // the description was there before the kernel ahead began
   int* err;
   cudaStream_t stream;
+  // or null: only the portions and kv heads that `beyond` [n, nkv] notes, where `moved` [n, 4] has rows for them (no
+  // scratch)
+  const int *beyond, *moved;
 };
 BF_EXPORT int bf_kv4_attention(const Kv4AttentionCall* call) {
   const auto& [q, q_stride, cache, rows, seq_of_token, positions, items, n, max_rows, T, block_tables,
                table_stride, table_rows, table_width, out, out_stride, nh, nkv, d, page_size, num_pages,
-               window, keep, scale, scratch, sms, keys, even, early, err, stream] = *call;
+               window, keep, scale, scratch, sms, keys, even, early, err, stream, beyond, moved] = *call;
   if (n <= 0 || max_rows <= 0) return 0;
   if ((long long)num_pages * nkv * (page_size / 8) > 0x7fffffffLL || page_size < 8 || (page_size & (page_size - 1)) ||
       (long long)table_width * page_size > 1 << 24)        // (a tile's units stay below 2^20)
@@ -984,7 +1026,8 @@ BF_EXPORT int bf_kv4_attention(const Kv4AttentionCall* call) {
   a.page_size = page_size, a.page_shift = 3;
   while (1 << a.page_shift < page_size) ++a.page_shift;
   a.num_pages = num_pages, a.window = window, a.keep = keep, a.scale = scale;
-  a.early = early != 0;
+  a.early = early != 0 && !beyond;
+  a.beyond = beyond, a.moved = moved, a.n_items = n;
   a.chunk_inverse = (256 + s.chunk - 1) / s.chunk;
   const long long slots = ka_slots(s, d, sms);
   a.part_o = (float*)scratch;
@@ -993,7 +1036,8 @@ BF_EXPORT int bf_kv4_attention(const Kv4AttentionCall* call) {
   a.err = err;
   const long long tiles = (long long)n * a.tiles_per_item;
   if (tiles > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
-  const int share = ka_blocks_a_head(s, d, tiles, nkv * s.chunks, keys, even, sms);
+  if (beyond && (!items || !moved)) return (int)cudaErrorInvalidValue;
+  const int share = beyond ? 1 : ka_blocks_a_head(s, d, tiles, nkv * s.chunks, keys, even, sms);
   if (!share && !scratch) return (int)cudaErrorInvalidValue;
   if (d == 64)
     return s.nt == 1 ? ka_launch<64, 1>(a, (int)tiles, share, sms, stream)

@@ -154,7 +154,7 @@ struct KvBool {
 // so small that fp16 has less than half a step of 2^-11 for its largest, a group of keys that is (`small_key`,
 // where the scale makes it matter), or a value that is not finite (a
 // probability of zero times such a value is NaN: whole tiles would carry it into rows that do not see it);
-// kv4_rest_kernel computes what is concerned.
+// attention_kv4.cu computes what is concerned from the codes.
 template <int D, bool HALF>
 __global__ void __launch_bounds__(256)
 kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__ block_tables,
@@ -214,6 +214,8 @@ kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
     running += __shfl_sync(0xffffffffu, incl, 31);
   }
   if (page == 0 && blockIdx.y == 0) {
+    if (HALF)
+      for (int i = tid; i < n_items * nkv; i += 256) beyond[i] = 0;
     long long to = 0;                                       // portions without pages, or without room for all of them
     for (int i = 0; i < n_items; ++i) {
       const int n = pages_of(items[4 * i], items[4 * i + 1], items[4 * i + 2], items[4 * i + 3]);
@@ -235,8 +237,6 @@ kv4_load_kernel(const unsigned char* __restrict__ cache, const int* __restrict__
   }
   const int last = first + n_rows - 1;
   const int place = page - 1 - base, n_places = last / 64 + 1;
-  if (HALF && place == 0 && blockIdx.y == 0)
-    for (int h = tid; h < nkv; h += 256) beyond[item * nkv + h] = 0;
   if (blockIdx.y == 0) {                                    // this block's part of the portion's row
     const int w1 = place + 1 < n_places ? (int)((long long)out_width * (place + 1) / n_places) : out_width;
     for (int w = (int)((long long)out_width * place / n_places) + tid; w < w1; w += 256)
@@ -362,91 +362,5 @@ BF_EXPORT int bf_kv4_load(const Kv4LoadCall* call) {
   if (d == 64) return special ? run(kv4_load_kernel<64, true>) : run(kv4_load_kernel<64, false>);
   if (d == 128) return special ? run(kv4_load_kernel<128, true>) : run(kv4_load_kernel<128, false>);
   if (d == 256) return special ? run(kv4_load_kernel<256, true>) : run(kv4_load_kernel<256, false>);
-  return (int)cudaErrorInvalidValue;
-}
-
-// What the tensor cores cannot have computed of portions over loaded pages: the rows of a portion and kv head
-// that is noted in `beyond`, by multiply-adds straight from the cache, a warp a (row, query head).  As a rule
-// nothing is noted and a block only reads that.
-template <int D>
-__global__ void __launch_bounds__(256)
-kv4_rest_kernel(const int* __restrict__ beyond, const int* __restrict__ items, const int* __restrict__ moved,
-                const unsigned char* __restrict__ cache, const int* __restrict__ block_tables,
-                int table_stride, const __nv_bfloat16* __restrict__ q, long long q_stride,
-                __nv_bfloat16* __restrict__ out, long long out_stride, int nkv, int group, int page_size,
-                int num_pages, int window, int keep, float scale) {
-  constexpr int N = D / 32, NG = D / KV4_GROUP, REC = kv4_record(D);
-  bf_pdl_trigger();
-  bf_pdl_wait();
-  const int h = blockIdx.y, item = blockIdx.z;
-  const int row0 = moved[4 * item + 1], rows = moved[4 * item + 2], first = moved[4 * item + 3];
-  if (beyond[item * nkv + h] == 0 || (int)blockIdx.x * 32 >= rows) return;
-  const int lane = threadIdx.x & 31, i0 = lane * N, g = i0 / 64;
-  const int* request = block_tables + (size_t)items[4 * item] * table_stride;
-  for (int i = threadIdx.x >> 5; i < 32 * group; i += 8) {
-    const int row = blockIdx.x * 32 + i / group, head = h * group + i % group, p = first + row;
-    if (row >= rows) break;
-    const __nv_bfloat16* src = q + (long long)(row0 + row) * q_stride + head * D + i0;
-    float qf[N], o[N], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int e = 0; e < N; ++e) qf[e] = __bfloat162float(src[e]), o[e] = 0.f;
-    for (int j = 0; j <= p; ++j) {
-      if (window > 0 && j <= p - window && j >= keep) {
-        j = p - window;
-        continue;
-      }
-      const int page = request[j / page_size];
-      if (page < 0 || page >= num_pages) continue;          // (flagged when it was loaded)
-      const int off = j % page_size, tok = off % 8;
-      const unsigned char* rec = cache + (((size_t)page * nkv + h) * (page_size / 8) + off / 8) * REC;
-      const unsigned kp = *reinterpret_cast<const unsigned*>(rec + kv4_key_params_at(D) + (tok * NG + g) * 4);
-      const unsigned vp = *reinterpret_cast<const unsigned*>(rec + kv4_value_params_at(D) + (tok * NG + g) * 4);
-      float s = 0.f, v[N];
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const int c = rec[kv4_key_byte(D, tok, i0 + e)] >> ((i0 + e) % 2 * 4) & 15;
-        s += qf[e] * fmaf(kv4_scale(kp), (float)c, kv4_low(kp));
-        v[e] = fmaf(kv4_scale(vp), (float)(rec[kv4_value_byte(D, tok, i0 + e)] >> ((i0 + e) % 2 * 4) & 15), kv4_low(vp));
-      }
-      s = warp_sum(s) * scale;
-      const float top = fmaxf(m, s), f = top == m ? 1.f : expf(m - top), w = expf(s - top);
-      l = l * f + w;
-#pragma unroll
-      for (int e = 0; e < N; ++e) o[e] = o[e] * f + w * v[e];
-      m = top;
-    }
-#pragma unroll
-    for (int e = 0; e < N; ++e)
-      out[(long long)(row0 + row) * out_stride + head * D + i0 + e] = __float2bfloat16_rn(o[e] / l);
-  }
-}
-
-struct Kv4RestCall {
-  const int* beyond, *items, *moved;
-  int n_items, max_rows;
-  const void* cache;
-  const int* block_tables;
-  int table_stride;
-  const void* q;
-  long long q_stride;
-  void* out;
-  long long out_stride;
-  int nh, nkv, d, page_size, num_pages, window, keep;
-  float scale;
-  cudaStream_t stream;
-};
-BF_EXPORT int bf_kv4_rest(const Kv4RestCall* call) {
-  const auto& [beyond, items, moved, n_items, max_rows, cache, block_tables,
-               table_stride, q, q_stride, out, out_stride, nh, nkv, d, page_size, num_pages, window, keep,
-               scale, stream] = *call;
-  if (n_items <= 0 || max_rows <= 0) return 0;
-  auto run = [&](auto kern) {
-    return bf_launch_pdl(kern, dim3((max_rows + 31) / 32, nkv, n_items), dim3(256), 0, stream,
-                         beyond, items, moved, (const unsigned char*)cache, block_tables, table_stride, (const __nv_bfloat16*)q, q_stride,
-                         (__nv_bfloat16*)out, out_stride, nkv, nh / nkv, page_size, num_pages, window, keep, scale);
-  };
-  if (d == 64) return run(kv4_rest_kernel<64>);
-  if (d == 128) return run(kv4_rest_kernel<128>);
-  if (d == 256) return run(kv4_rest_kernel<256>);
   return (int)cudaErrorInvalidValue;
 }

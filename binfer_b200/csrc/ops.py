@@ -1918,8 +1918,7 @@ class _Packed:
 
 _kv4_store_call = _Packed("bf_kv4_store", "PqPqPPiiiiqPP")
 _kv4_load_call = _Packed("bf_kv4_load", "PPiiiPiiPPPiPPPiiiiiiiifPP")
-_kv4_rest_call = _Packed("bf_kv4_rest", "PPPiiPPiPqPqiiiiiiifP")
-_kv4_attention_call = _Packed("bf_kv4_attention", "PqPPPPPiiiPiiiPqiiiiiiifPiiiiPP")
+_kv4_attention_call = _Packed("bf_kv4_attention", "PqPPPPPiiiPiiiPqiiiiiiifPiiiiPPPP")
 _qk_norm_rope_kv4_call = _Packed("bf_qk_norm_rope_kv4_store", "PqPPPiPPPPiiiiiqfPiifPP")
 _step_tables_call = _Packed("bf_step_tables", "PiiPiPiiiPPPPPiPiPiPiPP")
 _prefill_attention_umma2_half_call = _Packed("bf_prefill_attention_umma2_half", "PPPPiiiPiPiiiiiifiPPPqfiPPP")
@@ -2216,8 +2215,10 @@ def _kv4_loaded_attention(q, cache, items, n_items, max_rows, block_tables, tabl
     _run("prefill_attention_umma2", _prefill_attention_umma2_half_call,
          q_ptr, k, v, moved, n_items, max_rows, T, tables, places, out_ptr, nh, nkv, d, KV4_LOAD_PAGE, n, w, scale,
          splits, part_o, part_ml, err_ptr, out_stride, 1.0 / KV4_VALUE_UP, keep, beyond, special, stream)
-    _run("kv4_rest", _kv4_rest_call, beyond, item_ptr, moved, n_items, max_rows, cache_ptr, table_ptr, table_stride,
-         q_ptr, q_stride, out_ptr, out_stride, nh, nkv, d, ps, pages, w, keep, scale, stream)
+    # what fp16 had no room for, from the codes
+    _run("kv4_attention", _kv4_attention_call, q_ptr, q_stride, cache_ptr, 0, 0, 0, item_ptr, n_items, max_rows, T,
+         table_ptr, table_stride, table_rows, table_width, out_ptr, out_stride, nh, nkv, d, ps, pages, w, keep, scale, 0,
+         sms, 0, 0, 0, err_ptr, stream, beyond, moved)
 
 
 def _kv4_attention(q, cache, rows, seq, positions, items, n, max_rows, block_tables, table, strides, out, nh,
@@ -2244,7 +2245,7 @@ def _kv4_attention(q, cache, rows, seq, positions, items, n, max_rows, block_tab
     _run("kv4_attention", _kv4_attention_call, q.data_ptr(), q_stride, cache.data_ptr(), rows, seq, positions,
          items, n, max_rows, T, block_tables.data_ptr(), table_stride, table_rows, table_width, out.data_ptr(),
          out_stride, nh, nkv, d, ps, pages, window, keep, scale, scratch.data_ptr() if size else 0, sms, keys, even, described,
-         err.data_ptr(), _stream_at(q))
+         err.data_ptr(), _stream_at(q), 0, 0)
     if size:
         _launches += 1      # two kernels: the stretches of units, and what several of them share
 

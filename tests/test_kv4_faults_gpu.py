@@ -200,3 +200,80 @@ def test_codes_next_to_a_border_behind_norms_and_rotation(cuda_device, d):
                                torch.empty_like(x), got, 1, 1, d, 1e-6, err)
     assert torch.equal(got, want)
     assert torch.equal(K4.unpack(got)[0].reshape(-1, d)[8:8 + T], _held_exactly(x))
+
+
+# ------------------------------------------------------------------------------ what fp16 has no room for
+@pytest.mark.parametrize("nh,nkv,d,ps", [(8, 2, 128, 16), (16, 1, 128, 8), (6, 3, 64, 32), (20, 1, 64, 16), (4, 4, 64, 8),
+                                         (4, 1, 256, 128), (18, 2, 256, 16), (3, 3, 128, 64)])
+@pytest.mark.parametrize("window,keep", [(None, 0), (120, 9), (900, 70)])
+@pytest.mark.parametrize("jobs", [[(0, 2, 698)], [(2, 7, 0), (0, 5, 400), (1, 1, 3), (3, 3, 997)],
+                                  [(0, 700, 0), (3, 300, 700)], [(4, 40, 4200), (1, 33, 0)]])
+def test_portions_that_are_computed_from_the_codes(cuda_device, nh, nkv, d, ps, window, keep, jobs):
+    """Keys beyond fp16 in every kv head but the second, whose bits are what they are beside ordinary ones."""
+    from binfer_b200.csrc import ops
+    c = Cache([700, 33, 7, 1000, 4240], nkv, d, ps, cuda_device, seed=d + ps)
+    T, scale = sum(n for _, n, _ in jobs), d ** -0.5
+    q = _queries(T, nh, d, cuda_device)
+    items, at = [], 0
+    for b, n, p in jobs:
+        items.append((b, at, n, p))
+        at += n
+    for i, n in enumerate(c.lens):
+        c.k[i], c.v[i] = U.keys(n, nkv, d, cuda_device, 2 * i), U.values(n, nkv, d, cuda_device, 2 * i + 1)
+
+    def run():
+        for i in range(len(c.lens)):
+            ops.kv4_store(c.k[i].flatten(1), c.v[i].flatten(1), c.slots[i], c.cache, c.err)
+        out = torch.full_like(q, math.nan)
+        ops.kv4_prefill_attention(q, c.cache, torch.tensor(items, dtype=I32, device=cuda_device), len(items),
+                                  max(n for _, n, _ in jobs), c.tables, out, nh, nkv, d, window, scale, c.err,
+                                  ctx_rows=sum(-(-(n + p) // 64) * 64 for _, n, p in jobs),
+                                  max_ctx=max(n + p for _, n, p in jobs), keep_first=keep, variant="load")
+        assert int(c.err.item()) == 0
+        return out
+
+    ordinary = run()
+    up = torch.full((nkv, 1), 2.0 ** 18, device=cuda_device)
+    if nkv > 1:
+        up[1] = 1
+    q = (q.view(T, nkv, -1, d) / up[:, None]).to(BF16).view(T, -1)
+    for i in range(len(c.lens)):
+        c.k[i] = (c.k[i] * up).to(BF16)
+    out = run()
+    at = 0
+    for b, n, p in jobs:
+        k, v = c.held(b)
+        ref, allowed = U.attend(q[at:at + n].view(n, nh, d).to(F64), k[:n + p], v[:n + p],
+                                torch.arange(p, p + n, device=q.device), window, keep, scale)
+        U.check(out[at:at + n], ref, allowed)
+        at += n
+    if nkv > 1:
+        other = slice(nh // nkv * d, 2 * nh // nkv * d)
+        assert torch.equal(out[:, other], ordinary[:, other])
+
+
+@pytest.mark.parametrize("rows,ctx,nh,nkv,d", [(256, 4096, 16, 4, 128), (1024, 1024, 8, 2, 64), (300, 2000, 8, 2, 256)])
+def test_a_value_beyond_fp16_costs_little_more_than_reading_the_codes(cuda_device, rows, ctx, nh, nkv, d):
+    """One value in one token of each head; the kernel that reads the codes of every head takes the same way.  (It was a
+    walk over the keys, one after the other, of some hundred times that.)"""
+    from binfer_b200.csrc import ops
+    c = Cache([ctx], nkv, d, 16, cuda_device)
+    c.v[0][ctx // 2, :, 5] = 5000.0
+    ops.kv4_store(c.k[0].flatten(1), c.v[0].flatten(1), c.slots[0], c.cache, c.err)
+    q = _queries(rows, nh, d, cuda_device)
+    out = torch.empty_like(q)
+    items = torch.tensor([(0, 0, rows, ctx - rows)], dtype=I32, device=cuda_device)
+
+    def time(variant):
+        took = []
+        for _ in range(7):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            ops.kv4_prefill_attention(q, c.cache, items, 1, rows, c.tables, out, nh, nkv, d, None, d ** -0.5, c.err,
+                                      ctx_rows=-(-ctx // 64) * 64, max_ctx=ctx, variant=variant)
+            b.record()
+            torch.cuda.synchronize()
+            took.append(a.elapsed_time(b))
+        return min(took)
+
+    assert time("load") <= 10 * time("stretches")
