@@ -2082,7 +2082,7 @@ def kv4_decode_attention(q: torch.Tensor, cache: torch.Tensor, rows: Optional[to
     ``j <= p`` of its request; with ``window`` those with ``j > p - window``, and the first ``keep_first``
     tokens.  ``rows`` lists the token rows to run (None: 0 .. n_rows - 1); other rows of ``out`` are left
     as they were, and so is a listed one whose row, request or position is not there, which sets the error
-    word.  A page id outside the pool sets it too and stands for page 0.
+    word.  No row is listed twice, and ``out`` does not overlap ``q``.  A page id outside the pool sets it too and stands for page 0.
 
     ``described``: rows, requests, positions and tables were complete before the kernel ahead on the stream began
     (as in a step that is described once and then runs its layers); they are read under that kernel's end.
@@ -2114,13 +2114,15 @@ def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Ten
     ``prefill_attention``'s arguments, with ``cache`` (``kv4_cache``) in the pages' place.  ``ctx_rows``:
     the portions' contexts added up, each rounded up to 64; ``max_ctx``: the longest of them;
     ``keep_first``: with a window, the request's first that many tokens stay visible behind it.  A portion
-    whose rows, request or places are not there, or that ``ctx_rows`` and ``max_ctx`` have no room for,
-    sets the error word and its rows are left as they were.  ``described`` and sizes of numbers: as in
-    ``kv4_decode_attention``.
+    whose rows, request or places are not there, or, loaded, that ``ctx_rows`` and ``max_ctx`` have no room for,
+    sets the error word and its rows are left as they were.  ``out`` does not overlap ``q``.  ``described`` and sizes
+    of numbers: as in ``kv4_decode_attention``.
 
     ``variant``: ``stretches`` (the kernel of single tokens, a few rows at a time; reads the cache as it
     is), ``load`` (a positive scale, q contiguous: the contexts are loaded as ``kv4_load``
-    does, in fp16, into scratch of 4 d bytes a token and kv head, and attended on tcgen05), or ``auto``."""
+    does, in fp16, into scratch of 4 d bytes a token of ``ctx_rows`` and kv head, and attended on tcgen05; portions
+    and kv heads with numbers that fp16 has no room for are computed from the codes), or ``auto``, which loads
+    at most 2 GiB."""
     _want(items, torch.int32, "items")
     table, strides, pages, ps, w, keep = _kv4_attention_check(
         "kv4_prefill_attention", q, cache, block_tables, out, nh, nkv, d, window, keep_first, scale, err, items)
@@ -2134,6 +2136,7 @@ def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Ten
     if variant == "load" and not load_ok:
         raise KernelError("kv4_prefill_attention: the load variant takes a contiguous q and a positive scale")
     if variant == "load" or (variant == "auto" and load_ok
+                             and 4 * d * nkv * ctx_rows <= _KV4_LOAD_BYTES
                              and _kv4_load_pays(n_items, max_rows, max_ctx, w, keep, nh, nkv, d)):
         _kv4_loaded_attention(q, cache, items, n_items, max_rows, block_tables, table, strides, out, nh, nkv, d, ps,
                               pages, w, keep, scale, err, ctx_rows, max_ctx)
@@ -2144,6 +2147,7 @@ def kv4_prefill_attention(q: torch.Tensor, cache: torch.Tensor, items: torch.Ten
 
 _kv4_scratch: dict = {}     # bytes of scratch by a call's sizes
 _KV4_MANY_KEYS = 1 << 15
+_KV4_LOAD_BYTES = 2 << 30    # of loaded contexts that a call chooses to hold beside the pages: what an engine keeps free
 
 
 def _kv4_splits(n: int, max_rows: int, max_ctx: int, window: int, keep: int, nh: int, d: int,
@@ -2161,8 +2165,8 @@ def _kv4_load_pays(n: int, max_rows: int, max_ctx: int, window: int, keep: int, 
     """Whether a call's portions are faster loaded and attended on tcgen05 than in stretches of units:
     microseconds by sizes, fitted to both measured on a B200 (stretches / load; 288 pairs of heads of 64, 128
     and 256, one and four portions of 16 to 1,024 rows behind up to 16,000 keys or windows, whose slower side the
-    rule took in ten, by 11 to 27 %).  32 heads of 128 (8 kv heads), one portion: 64 rows behind 1,000 keys
-    26 / 30, behind 16,000 99 / 88; 256 rows 41 / 37 and 331 / 106.  16 heads of 64 (4): 256 rows behind 1,000
+    rule took in ten, by 11 to 27 %; the times are those of its 148 SMs, and so are the shares they are reckoned
+    with).  32 heads of 128 (8 kv heads), one portion: 64 rows behind 1,000 keys 26 / 30, behind 16,000 99 / 88; 256 rows 41 / 37 and 331 / 106.  16 heads of 64 (4): 256 rows behind 1,000
     keys 21 / 32, behind 4,000 41 / 37; 8 heads of 256 (2): 31 / 36 and 64 / 41."""
     group, cols = nh // nkv, 8 if d == 256 else 16
     blocks, per, splits = _kv4_splits(n, max_rows, max_ctx, window, keep, nh, d, 148)

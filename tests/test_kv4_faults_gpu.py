@@ -277,3 +277,23 @@ def test_a_value_beyond_fp16_costs_little_more_than_reading_the_codes(cuda_devic
         return min(took)
 
     assert time("load") <= 10 * time("stretches")
+
+
+# ------------------------------------------------------------------------------ scratch
+def test_portions_with_room_for_more_than_is_kept_free_are_not_loaded(cuda_device):
+    """``ctx_rows`` of 2^30 tokens, 4 TiB loaded: the choice reads the codes instead."""
+    from binfer_b200.csrc import ops
+    nh, nkv, d, n, rows = 32, 8, 128, 2000, 600
+    c = Cache([n], nkv, d, 16, cuda_device)
+    c.k[0], c.v[0] = U.keys(n, nkv, d, cuda_device, 1), U.values(n, nkv, d, cuda_device, 2)
+    ops.kv4_store(c.k[0].flatten(1), c.v[0].flatten(1), c.slots[0], c.cache, c.err)
+    q = _queries(rows, nh, d, cuda_device)
+    items = torch.tensor([(0, 0, rows, n - rows)], dtype=I32, device=cuda_device)
+    assert ops._kv4_load_pays(1, rows, n, 0, 0, nh, nkv, d)
+    out = torch.full_like(q, math.nan)
+    ops.kv4_prefill_attention(q, c.cache, items, 1, rows, c.tables, out, nh, nkv, d, None, d ** -0.5, c.err,
+                              ctx_rows=1 << 30, max_ctx=n)
+    ref, allowed = U.attend(q.view(rows, nh, d).to(F64), *c.held(0), torch.arange(n - rows, n, device=q.device), None, 0,
+                            d ** -0.5)
+    U.check(out, ref, allowed)
+    assert int(c.err.item()) == 0
