@@ -297,3 +297,58 @@ def test_portions_with_room_for_more_than_is_kept_free_are_not_loaded(cuda_devic
                             d ** -0.5)
     U.check(out, ref, allowed)
     assert int(c.err.item()) == 0
+
+
+def test_loaded_portions_in_a_graph_with_other_items_and_numbers(cuda_device):
+    """A captured call replayed with other portions, with and without numbers beyond fp16, with more context than its room,
+    beside another graph of the same call."""
+    import gc
+    from binfer_b200.csrc import ops
+    nh, nkv, d, lens = 8, 2, 128, [900, 500]
+    c = Cache(lens, nkv, d, 16, cuda_device)
+    q = _queries(300, nh, d, cuda_device)
+    items = torch.tensor([(0, 0, 200, 100), (1, 200, 100, 100)], dtype=I32, device=cuda_device)
+
+    def call(out):
+        ops.kv4_prefill_attention(q, c.cache, items, 2, 200, c.tables, out, nh, nkv, d, None, d ** -0.5, c.err,
+                                  ctx_rows=960 + 512, max_ctx=900, variant="load")
+
+    outs, graphs = [torch.zeros_like(q) for _ in range(2)], []
+    for o in outs:
+        call(o)
+        torch.cuda.synchronize()
+        gc.collect()                          # (not in the middle of the capture)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call(o)
+        graphs.append(g)
+    for jobs, large in (([(0, 0, 200, 700), (1, 200, 100, 400)], 0), ([(1, 0, 100, 400), (0, 100, 200, 700)], 2.0 ** 18),
+                        ([(0, 0, 150, 0), (1, 150, 1, 499)], 0), ([(0, 0, 200, 700), (1, 200, 100, 399)], 2.0 ** 18),
+                        ([(0, 0, 200, 700), (0, 200, 100, 800)], 0)):
+        for i, n in enumerate(lens):
+            c.k[i], c.v[i] = U.keys(n, nkv, d, cuda_device, i), U.values(n, nkv, d, cuda_device, 5 + i)
+            if large:                        # (in one token of one head)
+                c.k[i][17, 1], c.v[i][17, 1] = 0, 0
+                c.v[i][17, 1, 0] = large
+            ops.kv4_store(c.k[i].flatten(1), c.v[i].flatten(1), c.slots[i], c.cache, c.err)
+        items.copy_(torch.tensor(jobs, dtype=I32))
+        c.err.zero_()
+        for g, o in zip(graphs, outs):
+            o.zero_()
+            g.replay()
+        torch.cuda.synchronize()
+        fits = sum(-(-(n + p) // 64) * 64 for _, _, n, p in jobs) <= 960 + 512
+        assert int(c.err.item()) == (0 if fits else 16) and torch.equal(outs[0], outs[1])
+        for i, (b, at, n, p) in enumerate(jobs):
+            if not fits and i:
+                assert not outs[0][at:at + n].any()
+                continue
+            k, v = c.held(b)
+            ref, allowed = U.attend(q[at:at + n].view(n, nh, d).to(F64), k[:n + p], v[:n + p],
+                                    torch.arange(p, p + n, device=q.device), None, 0, d ** -0.5)
+            if large:                        # the numbers that the large one reaches are as far off as it is large
+                ref, got = ref.view(n, nh, d).clone(), outs[0][at:at + n].view(n, nh, d).clone()
+                ref[:, nh // 2:, :64] = got[:, nh // 2:, :64] = 0
+                U.check(got, ref, allowed)
+            else:
+                U.check(outs[0][at:at + n], ref, allowed)
