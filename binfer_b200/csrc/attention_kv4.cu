@@ -37,14 +37,15 @@
 // with one kv head, 371 with all; 256 rows behind 8,192 94, 195 and 299.  (A walk over the keys by multiply-adds took 40 and
 // 85 ms.)
 //
-// Measured (B200).  64 rows of 64 heads of 128 (8) behind 4,096 keys down to 2,700: 55 us and 5 for the second
-// kernel, where the 254 MB take 39 at the rate of a copy, 6.54 TB/s.  While all warps run they read 6.2 TB/s:
-// some 258 instructions a unit of 2,304 bytes nearly fill the issue slots, so that bytes and instructions are
-// level; the rest is the beginning of the stretches (queries, tables, first units: 4 us) and their end, a wait for
-// the slowest SM.  Eight rows behind 4,096: 12.5 + 3 us (bytes: 5), in clusters of two 15; 30,000 keys behind a
-// window of 4,096, 12 rows of 16 heads: 18 + 3, a block a head 21 (8.7).  Tried without gain: partials added up in
-// a block before the second kernel, barriers that keep a block's warps level, fewer warps with a deeper ring, the
-// lowest values as the product's addend.
+// Measured (B200), replayed in a row / with caches cold.  64 rows of 64 heads of 128 (8) behind 4,096 keys down to 2,700:
+// 58.5 / 67.6 us, where the 254 MB take 39 at the rate of a copy, 6.54 TB/s.  All rows behind 2,048, 4,096, 8,192 and
+// 16,384 keys: 42, 66, 114 and 208 us, so that a byte more costs what it takes at 6.3 to 6.4 TB/s and some 19 us stand
+// beside the bytes: the beginning of the stretches (queries, tables, first units), a wait for the slowest SM at their end, the
+// second kernel (5 to 8).  (Issue slots 48 % busy and DRAM 55 % over the attention kernel at 4,096: some 258 instructions
+// a unit of 2,304 bytes are 25 us of all slots.)  Eight rows behind 4,096: clusters of two 16.4 / 20.5 (bytes: 5), stretches 12.5 and 3 for the second kernel; 30,000 keys behind a window of 4,096, 12 rows of 16
+// heads: a block a head 20.6 / 26.6, stretches 18 + 3 (8.7).  Tried without gain: partials added up in a block before the
+// second kernel, barriers that keep a block's warps level, fewer warps with a deeper ring, the lowest values as the
+// product's addend.
 #include "common.cuh"
 #include "kv4.cuh"
 #include "mma_utils.cuh"
@@ -158,8 +159,8 @@ kv4_attention_kernel(const __grid_constant__ KaArgs a) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r = lane >> 2, q4 = lane & 3;
   const int pairs = a.nkv * a.chunks;
-  // Where the step's description (rows, positions, requests, tables) was there before the kernel ahead began
-  // (a.early), it is read under that kernel's end, and queries, pages and all writes wait; else everything waits.
+  // Where the step's description (rows, positions, requests) was there before the kernel ahead began (a.early), it
+  // is read under that kernel's end, and block tables, queries, pages and all writes wait; else everything waits.
   // The successor is asked for after the wait: its blocks, resident any earlier, slow down what runs ahead of this
   // kernel.
   auto begin = [&](int early) {

@@ -2085,7 +2085,8 @@ def kv4_decode_attention(q: torch.Tensor, cache: torch.Tensor, rows: Optional[to
     word.  No row is listed twice, and ``out`` does not overlap ``q``.  A page id outside the pool sets it too and stands for page 0.
 
     ``described``: rows, requests, positions and tables were complete before the kernel ahead on the stream began
-    (as in a step that is described once and then runs its layers); they are read under that kernel's end.
+    (as in a step that is described once and then runs its layers); all but the tables are read under that kernel's
+    end.
 
     Queries below 2^62, values below 2^55 and scores below 1e30 in size: larger ones overflow inside; queries below
     2^-48 may count as zero.  A scale above 2^40 in size is refused."""

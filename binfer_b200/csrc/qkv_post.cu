@@ -131,7 +131,9 @@ __global__ void qk_norm_rope_kv_write_kernel(
 // sit in lane l ^ 16.  With few tokens every warp has one head: the kernel is then two
 // dependent round trips long (position, then the head's values) instead of one per head.
 //
-// FOUR: as above; a group's 64 numbers lie in sixteen lanes, a lane's four codes are two bytes.
+// FOUR: as above; a group's 64 numbers lie in sixteen lanes, a lane's four codes are two bytes.  Beside the store as
+// bfloat16, 32 heads of 128 (8 kv heads): 2.6 us for 2.2 with one token, 3.5 for 3.1 with 64, 23.9 for 16.0 with 2,048 (the
+// codes' instructions); heads of 64 and 256 by the kernel above, 2,048 tokens of 16 (4) 17.8 for 15.8, of 8 (2) 18.3 for 14.1.
 template <bool FOUR>
 __global__ void qk_norm_rope_kv_write_d128_kernel(
     const __nv_bfloat16* __restrict__ qkv, long long row_stride, const float* __restrict__ q_w,
