@@ -42,10 +42,10 @@
 // 16,384 keys: 42, 66, 114 and 208 us, so that a byte more costs what it takes at 6.3 to 6.4 TB/s and some 19 us stand
 // beside the bytes: the beginning of the stretches (queries, tables, first units), a wait for the slowest SM at their end, the
 // second kernel (5 to 8).  (Issue slots 48 % busy and DRAM 55 % over the attention kernel at 4,096: some 258 instructions
-// a unit of 2,304 bytes are 25 us of all slots.)  Eight rows behind 4,096: clusters of two 16.4 / 20.5 (bytes: 5), stretches 12.5 and 3 for the second kernel; 30,000 keys behind a window of 4,096, 12 rows of 16
-// heads: a block a head 20.6 / 26.6, stretches 18 + 3 (8.7).  Tried without gain: partials added up in a block before the
-// second kernel, barriers that keep a block's warps level, fewer warps with a deeper ring, the lowest values as the
-// product's addend.
+// a unit of 2,304 bytes are 25 us of all slots.)  Eight rows behind 4,096: clusters of two 16.4 / 20.5 (bytes: 5),
+// stretches 12.5 and 3 for the second kernel; 30,000 keys behind a window of 4,096, 12 rows of 16 heads: a block a head
+// 20.6 / 26.6, stretches 18 + 3 (8.7).  Tried without gain: partials added up in a block before the second kernel, barriers
+// that keep a block's warps level, fewer warps with a deeper ring, the lowest values as the product's addend.
 #include "common.cuh"
 #include "kv4.cuh"
 #include "mma_utils.cuh"
