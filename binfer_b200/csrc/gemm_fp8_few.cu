@@ -1,0 +1,532 @@
+// Products with weights in 8 bits for few rows a weight: out[m, n] = sum_t sx[m, t] sw[n / 128, t]
+// sum_{k in t} cx[m, k] cw[n, k] over the groups t of 128 columns (the format: fp8.cuh).
+//
+// The weight's rows are the product's rows (128 of them = 128 lanes of tensor memory) and the
+// activations' rows its columns, of which a tile has as many as there are, rounded up to 16: a decode
+// step's eight rows cost a sixteenth of what they would as the product's rows, and an expert with 37
+// rows pays for 48.  One tcgen05.mma.kind::f8f6f4 takes K = 32; the four of a group go into columns of
+// tensor memory of their own, a ring of them, and the epilogue's warps add each group's sums, times its
+// two scales, into registers (float; the scales cannot ride along in tensor memory).
+//
+//   warp 0       TMA: 128 weight rows and NB activation rows x 128 bytes per stage
+//   warp 1       the products; TMEM allocation
+//   warp 2       the factors sx sw of every column of a group, into shared memory
+//   warps 4-11   the sums, times the factors, into registers; the result (wide tiles: these two
+//                warpgroups take 216 registers a thread, which the first leaves them: 128 x 72 +
+//                256 x 216 = 384 x 168)
+//
+// What bounds it with few rows is the weights' bytes; a tile is 128 rows of the weight, so that a
+// narrow weight alone does not give every SM work: then a cluster of `split` CTAs shares a tile, each a
+// part of the groups, and the parts meet in shared memory, added in the order of the ranks.
+// With experts the tiles are dealt out to persistent CTAs.
+//
+// Every wait is bounded; no load uses multicast.
+#include "common.cuh"
+#include "fp8.cuh"
+#include "fp8_umma.cuh"
+
+namespace {
+
+constexpr int FEW_THREADS = 384;            // three warpgroups of 168 registers a thread at launch
+constexpr int FEW_MAX_STAGES = 12;
+constexpr int FEW_BARS = 1024;
+constexpr int FEW_W_BYTES = 128 * FK;
+constexpr size_t FEW_SMEM = 226 * 1024;
+
+template <int NB>
+struct FewShape {
+  static constexpr int SLOTS = 512 / NB < 16 ? 512 / NB : 16;      // groups in tensor memory
+  static constexpr int CH = NB == 16 ? 8 : 16;                     // columns a warp reads at once
+  static constexpr int STAGE = FEW_W_BYTES + NB * FK;
+  // the up rows' sums on their way to the gate rows' warps: two buffers for each half of the warps
+  static constexpr int EXCHANGE = 2 * 2 * CH * 64 * 4;
+};
+
+struct FewParams {
+  int rows, features, K, groups;
+  int experts, tiles_f, w_blocks;      // w_blocks: rows of scales of a matrix
+  const int* starts;                   // null: no experts
+  const float* sx;                     // [groups, lds]
+  long long lds;
+  const float* sw;                     // [experts * (gated ? 2 : 1) * w_blocks, groups]
+  const float* row_w;                  // per row, or null
+  int split, stages, table_bytes;
+  long long ldo;
+  int act;
+  BfGateConst gk;
+  int* err;
+};
+
+__device__ __forceinline__ uint32_t few_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t few_map(uint32_t local_addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local_addr), "r"(rank));
+  return r;
+}
+
+template <int NB, typename OutT, bool GATED>
+__global__ void __launch_bounds__(FEW_THREADS, 1)
+fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+               OutT* __restrict__ out, const FewParams p) {
+  constexpr int SLOTS = FewShape<NB>::SLOTS, CH = FewShape<NB>::CH, CHUNKS = NB / CH / 2;
+  constexpr int STAGE = FewShape<NB>::STAGE;
+  constexpr int HALVES = GATED ? 2 : 1;
+  constexpr int TMEM_COLS = SLOTS * NB;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  bf_pdl_trigger();
+  uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t* full = reinterpret_cast<uint64_t*>(base);
+  uint64_t* empty = full + FEW_MAX_STAGES;
+  uint64_t* acc_full = empty + FEW_MAX_STAGES;           // [SLOTS]: the sums and the factors are there
+  uint64_t* acc_empty = acc_full + SLOTS;
+  uint64_t* drain = acc_empty + SLOTS;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* factors = reinterpret_cast<float*>(base + FEW_BARS);            // [SLOTS][HALVES][NB]
+  float* exchange = factors + SLOTS * HALVES * NB;       // gated: up sums; split: the parts sent here
+  uint8_t* table_smem = reinterpret_cast<uint8_t*>(exchange) +
+                        (p.split > 1 ? ((NB + p.split - 1) / p.split) * p.split * 128 * 4
+                                     : GATED ? FewShape<NB>::EXCHANGE : 0);
+  const RowTables tables = row_tables_at(table_smem, p.experts);
+  uint8_t* tiles = base + (((table_smem - base) + p.table_bytes + 1023) & ~1023);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = p.split > 1 ? (int)few_rank() : 0;
+  const int cluster = (int)blockIdx.x / p.split, clusters = (int)gridDim.x / p.split;
+  const int g0 = (int)((long long)p.groups * rank / p.split);
+  const int g1 = (int)((long long)p.groups * (rank + 1) / p.split);
+  const int STAGES = p.stages;
+  const int w_rows = HALVES * p.features;                // of an expert
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full + s, 1);
+      mbar_init(empty + s, 1);
+    }
+    for (int a = 0; a < SLOTS; ++a) {
+      mbar_init(acc_full + a, 2);              // the products' commit, the factors' warp
+      mbar_init(acc_empty + a, 8);             // a warp of the epilogue each
+    }
+    mbar_init(drain, 1);
+    *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  auto load_w = [&](int stage, int g, int expert, int ft) {
+    uint8_t* dst = tiles + (size_t)stage * STAGE;
+    if (GATED) {
+      tma_load_2d(dst, &map_w, full + stage, g * FK, expert * w_rows + ft * 64);
+      tma_load_2d(dst + 64 * FK, &map_w, full + stage, g * FK, expert * w_rows + p.features + ft * 64);
+    } else {
+      tma_load_2d(dst, &map_w, full + stage, g * FK, expert * w_rows + ft * 128);
+    }
+  };
+  // The weights depend on no kernel of the stream before this one: without experts the first ring of
+  // them is asked for before the wait for those.
+  // (clusters: nothing goes to a CTA that has not begun)
+  if (p.split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  const int pre = p.starts ? 0 : min(STAGES, g1 - g0);
+  if (warp == 0 && lane == 0)
+    for (int i = 0; i < pre; ++i) {
+      mbar_expect_tx(full + i, STAGE);
+      load_w(i, g0 + i, 0, cluster / ((p.rows + NB - 1) / NB));
+    }
+  __syncwarp();
+  bf_pdl_wait();
+  if (p.split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  fill_row_tables(tables, p.starts, p.experts, p.rows, NB);
+  __syncthreads();
+  const int units = tables.before[p.experts] * p.tiles_f;
+
+  int stage = 0;                                 // of this role, with its phase
+  uint32_t phase = 0;
+  if (warp < 4) {
+  if (NB >= 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  if (warp == 0) {
+    // --------------------------------------------------------------- copies
+    if (lane == 0) {
+      int asked = 0;
+      bool ok = true;
+      for (int u = cluster; u < units && ok && !*abort; u += clusters) {
+        const RowTile t = row_tile(tables, p.experts, p.tiles_f, NB, u);
+        for (int g = g0; g < g1; ++g, ++asked) {
+          if (asked >= pre) {
+            if (!mbar_wait(empty + stage, phase ^ 1, abort)) {
+              ok = false;
+              break;
+            }
+            mbar_expect_tx(full + stage, STAGE);
+            load_w(stage, g, t.expert, t.ft);
+          }
+          tma_load_2d(tiles + (size_t)stage * STAGE + FEW_W_BYTES, &map_x, full + stage, g * FK, t.row0);
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------- products
+    int slot = 0;
+    uint32_t slot_phase = 0;
+    bool ok = true;
+    for (int u = cluster; u < units && ok; u += clusters) {
+      const RowTile t = row_tile(tables, p.experts, p.tiles_f, NB, u);
+      const int n = min(NB, (t.row_end - t.row0 + 15) & ~15);
+      const uint32_t idesc = fp8_idesc(128, n);
+      for (int g = g0; g < g1; ++g) {
+        if (!mbar_wait_warp(acc_empty + slot, slot_phase ^ 1, abort) ||
+            !mbar_wait_warp(full + stage, phase, abort)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t a_addr = smem_u32(tiles + (size_t)stage * STAGE);
+        const uint64_t a_desc = umma_desc_k_sw128(a_addr);
+        const uint64_t b_desc = umma_desc_k_sw128(a_addr + FEW_W_BYTES);
+#pragma unroll
+        for (int k = 0; k < FK / 32; ++k)
+          umma_fp8(tmem_base + (uint32_t)(slot * NB), a_desc + (uint64_t)(2 * k), b_desc + (uint64_t)(2 * k),
+                   idesc, k > 0 ? 1u : 0u);
+        umma_commit(empty + stage);
+        umma_commit(acc_full + slot);
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
+        if (++slot == SLOTS) {
+          slot = 0;
+          slot_phase ^= 1;
+        }
+      }
+    }
+  } else if (warp == 2) {
+    // -------------------------------------------------------------- factors
+    constexpr int PER = (NB + 31) / 32;          // columns a lane looks after
+    constexpr int AHEAD = PER == 1 ? 8 : PER == 2 ? 4 : 2;      // groups whose scales are asked for together
+    int slot = 0;
+    uint32_t slot_phase = 0;
+    bool ok = true;
+    for (int u = cluster; u < units && ok; u += clusters) {
+      const RowTile t = row_tile(tables, p.experts, p.tiles_f, NB, u);
+      const long long block = (long long)t.expert * HALVES * p.w_blocks + (GATED ? t.ft >> 1 : t.ft);
+      for (int ga = g0; ga < g1 && ok; ga += AHEAD) {
+        float sx[AHEAD][PER], sw[AHEAD][HALVES];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+          const int g = min(ga + i, g1 - 1);
+#pragma unroll
+          for (int j = 0; j < PER; ++j) {
+            const int row = t.row0 + j * 32 + lane;
+            sx[i][j] = row < t.row_end && j * 32 + lane < NB ? p.sx[(long long)g * p.lds + row] : 0.f;
+          }
+#pragma unroll
+          for (int h = 0; h < HALVES; ++h) sw[i][h] = p.sw[(block + h * p.w_blocks) * p.groups + g];
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+          if (ga + i >= g1 || !ok) break;
+          if (!mbar_wait_warp(acc_empty + slot, slot_phase ^ 1, abort)) {
+            ok = false;
+            break;
+          }
+          float* f = factors + slot * HALVES * NB;
+#pragma unroll
+          for (int j = 0; j < PER; ++j)
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h)
+              if (j * 32 + lane < NB) f[h * NB + j * 32 + lane] = fp8_factor(sx[i][j], sw[i][h]);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(acc_full + slot);
+          if (++slot == SLOTS) {
+            slot = 0;
+            slot_phase ^= 1;
+          }
+        }
+      }
+    }
+  }
+  } else {
+    if (NB >= 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    // ----------------------------------------------------------------- sums
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    const int lane_row = quarter * 32 + lane;            // of the tile's 128 weight rows
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const int which = GATED ? quarter >> 1 : 0;
+    int slot = 0;
+    uint32_t slot_phase = 0;
+    for (int u = cluster; u < units; u += clusters) {
+      const RowTile t = row_tile(tables, p.experts, p.tiles_f, NB, u);
+      const int n = min(NB, t.row_end - t.row0);
+      float acc[CHUNKS][CH];
+#pragma unroll
+      for (int i = 0; i < CHUNKS; ++i)
+#pragma unroll
+        for (int j = 0; j < CH; ++j) acc[i][j] = 0.f;
+      bool ok = true;
+      for (int g = g0; g < g1; ++g) {
+        if (!mbar_wait_warp(acc_full + slot, slot_phase, abort)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const float* f = factors + (slot * HALVES + which) * NB;
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i) {
+          const int c = (2 * i + half) * CH;             // (the two halves take the chunks in turn)
+          if (c < n) {
+            uint32_t r[CH];
+            if constexpr (CH == 8) tmem_ld8(tmem_base + lanes + (uint32_t)(slot * NB + c), r);
+            else tmem_ld16(tmem_base + lanes + (uint32_t)(slot * NB + c), r);
+#pragma unroll
+            for (int j = 0; j < CH; j += 4) {
+              const float4 v = *reinterpret_cast<const float4*>(f + c + j);
+              fma2v(acc[i][j], acc[i][j + 1], r[j], r[j + 1], v.x, v.y);
+              fma2v(acc[i][j + 2], acc[i][j + 3], r[j + 2], r[j + 3], v.z, v.w);
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(acc_empty + slot);
+        if (++slot == SLOTS) {
+          slot = 0;
+          slot_phase ^= 1;
+        }
+      }
+      if (p.split > 1) {
+        // column j goes to rank j % split: [rank][its number there][weight row]
+        const int per = (NB + p.split - 1) / p.split;
+        const uint32_t here = smem_u32(exchange);
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i)
+#pragma unroll
+          for (int j = 0; j < CH; ++j) {
+            const int c = (2 * i + half) * CH + j;
+            if (c < n) {
+              const uint32_t at = here + (uint32_t)(((rank * per + c / p.split) * 128 + lane_row) * 4);
+              asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(few_map(at, (uint32_t)(c % p.split))),
+                           "f"(acc[i][j])
+                           : "memory");
+            }
+          }
+        break;                                           // (a cluster has one tile)
+      }
+      if (GATED) {
+        ok = named_all(1 + half, 128, ok);
+        if (!ok) break;
+        float* xb = exchange + half * 2 * CH * 64;
+        const int o = t.ft * 64 + (quarter & 1) * 32 + lane;
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i) {
+          const int c = (2 * i + half) * CH;
+          if (c < n) {                                   // (the same in the four warps)
+            float* b = xb + (i & 1) * CH * 64 + (quarter & 1) * 32 + lane;
+            if (quarter >= 2) {
+#pragma unroll
+              for (int j = 0; j < CH; ++j) b[j * 64] = acc[i][j];
+            }
+            named_sync(1 + half, 128);
+            if (quarter < 2 && o < p.features) {
+#pragma unroll
+              for (int j = 0; j < CH; ++j)
+                if (c + j < n) {
+                  const int row = t.row0 + c + j;
+                  float v = fp8_gate(p.act, acc[i][j], b[j * 64], p.gk);
+                  if (p.row_w) v *= p.row_w[row];
+                  bf_st(out + (size_t)row * p.ldo + o, v);
+                }
+            }
+          }
+        }
+        // (the next tile's first buffer is this tile's first too: two barriers lie between its uses
+        // only if this tile had more than one chunk)
+        named_sync(1 + half, 128);
+      } else {
+        if (!ok) break;
+        const int o = t.ft * 128 + lane_row;
+        if (o < p.features) {
+#pragma unroll
+          for (int i = 0; i < CHUNKS; ++i)
+#pragma unroll
+            for (int j = 0; j < CH; ++j) {
+              const int c = (2 * i + half) * CH + j;
+              if (c < n) {
+                const int row = t.row0 + c;
+                float v = acc[i][j];
+                if (p.row_w) v *= p.row_w[row];
+                bf_st(out + (size_t)row * p.ldo + o, v);
+              }
+            }
+        }
+      }
+    }
+  }
+  __syncwarp();
+
+  if (p.split > 1) {
+    // every part is in place behind this; then the columns of this rank, parts in the ranks' order
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (cluster < units) {
+      const RowTile t = row_tile(tables, p.experts, p.tiles_f, NB, cluster);
+      const int n = min(NB, t.row_end - t.row0), per = (NB + p.split - 1) / p.split;
+      const int width = GATED ? 64 : 128;
+      const int mine = n > rank ? (n - rank + p.split - 1) / p.split : 0;
+      for (int i = threadIdx.x; i < mine * width; i += FEW_THREADS) {
+        const int o = i % width, c = i / width, row = t.row0 + c * p.split + rank;
+        if (t.ft * width + o >= p.features) continue;
+        float v = 0.f, up = 0.f;
+        for (int r = 0; r < p.split; ++r) {
+          const float* part = exchange + (r * per + c) * 128 + o;
+          v += part[0];
+          if (GATED) up += part[64];
+        }
+        if (GATED) v = fp8_gate(p.act, v, up, p.gk);
+        if (p.row_w) v *= p.row_w[row];
+        bf_st(out + (size_t)row * p.ldo + t.ft * width + o, v);
+      }
+    }
+  }
+
+  // ------------------------------------------------------------------ wind-down
+  __syncthreads();
+  if (*abort) {
+    if (threadIdx.x == 0) atomicOr(p.err, BF_ERR_WAIT);
+    if (warp == 0 && lane == 0) mbar_drain(full, STAGES, stage, phase);
+    if (warp == 1) {
+      umma_commit(drain);
+      const long long t0 = clock64();
+      while (!mbar_try_wait(drain, 0) && clock64() - t0 < WAIT_LIMIT_CYCLES / 16) {
+      }
+    }
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS)
+                 : "memory");
+  }
+}
+
+template <int NB, typename OutT, bool GATED>
+int few_launch(const void* x, long long ldx, const void* w, long long ldw, OutT* out, FewParams p, int num_sms,
+               cudaStream_t stream) {
+  auto kern = fp8_few_kernel<NB, OutT, GATED>;
+  static bool configured_on[BF_MAX_DEVICES];
+  bool& configured = configured_on[bf_current_device()];
+  if (!configured) {
+    const cudaError_t ce =
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FEW_SMEM);
+    if (ce != cudaSuccess) return (int)ce;
+    configured = true;
+  }
+  constexpr int HALVES = GATED ? 2 : 1;
+  p.tiles_f = (p.features + (GATED ? 63 : 127)) / (GATED ? 64 : 128);
+  p.w_blocks = (p.features + 127) / 128;
+  p.groups = (p.K + FK - 1) / FK;
+  p.table_bytes = row_tables_bytes(p.experts);
+  const long long tiles_r = (p.rows + NB - 1) / NB;
+  // (at most: `starts` may hold anything)
+  const long long units = tiles_r * p.experts * p.tiles_f;
+  if (units > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+  if (p.starts || NB > 64 || units * p.split > num_sms || p.split > p.groups) p.split = 1;
+  const size_t extra = p.split > 1 ? (size_t)((NB + p.split - 1) / p.split) * p.split * 128 * 4
+                                   : GATED ? FewShape<NB>::EXCHANGE : 0;
+  size_t fixed = FEW_BARS + (size_t)FewShape<NB>::SLOTS * HALVES * NB * 4 + extra + p.table_bytes;
+  fixed = 1024 + ((fixed + 1023) & ~(size_t)1023);
+  const size_t stage = FEW_W_BYTES + NB * FK;
+  p.stages = (int)((FEW_SMEM - fixed) / stage);
+  if (p.stages > FEW_MAX_STAGES) p.stages = FEW_MAX_STAGES;
+  if (p.stages < 2) return (int)cudaErrorInvalidValue;
+  CUtensorMap mx, mw;
+  int e;
+  if ((e = fp8_map(&mx, x, p.rows, p.K, ldx, NB)) ||
+      (e = fp8_map(&mw, w, (long long)p.experts * HALVES * p.features, p.K, ldw, GATED ? 64 : 128)))
+    return e;
+  const long long work = units * p.split;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.split > 1 || work < num_sms ? work : num_sms));
+  cfg.blockDim = dim3(FEW_THREADS);
+  cfg.dynamicSmemBytes = fixed + p.stages * stage;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = bf_pdl_enabled();
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.split;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.split > 1 ? 2 : 1;
+  const cudaError_t ce = cudaLaunchKernelEx(&cfg, kern, mx, mw, out, p);
+  if (ce != cudaSuccess) return (int)ce;
+  return bf_launch_status();
+}
+
+template <typename OutT, bool GATED>
+int few_by_width(int nb, const void* x, long long ldx, const void* w, long long ldw, OutT* out,
+                 const FewParams& p, int num_sms, cudaStream_t stream) {
+  switch (nb) {
+    case 16: return few_launch<16, OutT, GATED>(x, ldx, w, ldw, out, p, num_sms, stream);
+    case 32: return few_launch<32, OutT, GATED>(x, ldx, w, ldw, out, p, num_sms, stream);
+    case 64: return few_launch<64, OutT, GATED>(x, ldx, w, ldw, out, p, num_sms, stream);
+    case 128: return few_launch<128, OutT, GATED>(x, ldx, w, ldw, out, p, num_sms, stream);
+    case 256: return few_launch<256, OutT, GATED>(x, ldx, w, ldw, out, p, num_sms, stream);
+    default: return (int)cudaErrorInvalidValue;
+  }
+}
+
+}  // namespace
+
+// x codes [rows, K] (rows ldx bytes apart) with scales sx [ceil(K / 128), lds]; w codes [experts,
+// (gated ? 2 : 1) * features, K] (rows ldw bytes apart) with scales sw [experts, (gated ? 2 : 1) *
+// ceil(features / 128), ceil(K / 128)]; starts int [experts + 1] of the experts' first rows, or null for
+// one weight; row_w float [rows] or null; out [rows, features], rows ldo apart.  nb: most rows of a tile
+// (16 to 256, a power of two).  split: CTAs that share a tile (without experts, tiles * split at most
+// num_sms; else 1 is taken).
+BF_EXPORT int bf_gemm_fp8_few(const void* x, long long ldx, const float* sx, long long lds, const void* w,
+                              long long ldw, const float* sw, const int* starts, const float* row_w,
+                              void* out, long long ldo, int out_dtype, int rows, int features, int K,
+                              int experts, int gated, int act, float limit, float slope, float up_offset,
+                              int nb, int split, int num_sms, int* err, cudaStream_t stream) {
+  if (rows <= 0 || features <= 0) return 0;
+  if (K <= 0 || experts < 1 || experts > FP8_MAX_EXPERTS || (!starts && experts != 1) || ldx % 16 || ldw % 16 ||
+      (((uintptr_t)x | (uintptr_t)w) & 15) || split < 1 || split > 8 || num_sms < 1 ||
+      (act != BF_ACT_SILU && act != BF_ACT_CLAMPED) || (gated && out_dtype != BF_DTYPE_BF16))
+    return (int)cudaErrorInvalidValue;
+  FewParams p = {};
+  p.rows = rows;
+  p.features = features;
+  p.K = K;
+  p.experts = experts;
+  p.starts = starts;
+  p.sx = sx;
+  p.lds = lds;
+  p.sw = sw;
+  p.row_w = row_w;
+  p.split = split;
+  p.ldo = ldo;
+  p.act = act;
+  p.gk = BfGateConst{limit, slope, up_offset};
+  p.err = err;
+  if (gated)
+    return few_by_width<__nv_bfloat16, true>(nb, x, ldx, w, ldw, (__nv_bfloat16*)out, p, num_sms, stream);
+  if (out_dtype == BF_DTYPE_F32)
+    return few_by_width<float, false>(nb, x, ldx, w, ldw, (float*)out, p, num_sms, stream);
+  return few_by_width<__nv_bfloat16, false>(nb, x, ldx, w, ldw, (__nv_bfloat16*)out, p, num_sms, stream);
+}

@@ -1,0 +1,424 @@
+// Products with weights in 8 bits for many rows: the sums of gemm_fp8_few.cu on pairs of SMs.
+//
+// Tiles of 256 activation rows x 256 weight rows, a cluster of two CTAs each (tcgen05.mma.cta_group::2.
+// kind::f8f6f4): a CTA holds 128 rows of the activations in its lanes of tensor memory and fetches half
+// of the weight rows.  Here the activations are the product's rows, so that a thread has one row's
+// scale and the weight's scale is one number a group: one multiplication a group of 128 instead of one
+// factor per column.  The sums of a group (256 columns) go into one of two buffers of tensor memory;
+// eight warps per CTA, two to a quarter of the lanes, add them times the factor into 128 registers each
+// while the products fill the other buffer.
+//
+//   warp 0       TMA: 128 activation rows and 128 weight rows x 128 bytes per stage
+//   warp 1       (leader) the products; TMEM allocation
+//   warps 4-11   the sums into registers; the result, turned in shared memory so that a warp writes
+//                whole 128-byte lines (these two warpgroups take 224 registers a thread, which the
+//                first leaves them: 128 x 56 + 256 x 224 = 384 x 168)
+//
+// Gated: a CTA's half of the weight rows are 64 gate rows and the 64 up rows of the same outputs, so a
+// thread holds both.  With experts a tile's rows are one expert's.
+//
+// Every wait is bounded; no load uses multicast.
+#include "common.cuh"
+#include "fp8.cuh"
+#include "fp8_umma.cuh"
+#include "pair_utils.cuh"
+
+namespace {
+
+constexpr int PF_THREADS = 384;             // three warpgroups of 168 registers a thread at launch
+constexpr int PF_TILE = 256;
+constexpr int PF_HALF = 128 * FK;             // a CTA's rows of either operand
+constexpr int PF_STAGE = 2 * PF_HALF;
+constexpr int PF_STAGES = 5;
+constexpr int PF_BARS = 512;
+constexpr int PF_TURN = 32 * 128;             // a warp's rows on their way out: 32 x 128 bytes
+
+struct PairParams {
+  int rows, features, K, groups;
+  int experts, tiles_f, w_blocks, table_bytes;
+  const int* starts;
+  const float* sx;
+  long long lds;
+  const float* sw;
+  const float* row_w;
+  long long ldo;
+  int act;
+  BfGateConst gk;
+  int* err;
+};
+
+__device__ __forceinline__ void pair_umma_fp8(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc,
+                                              uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 32 rows of a warp, 128 bytes each (a lane has a row, `v` its sixteen-byte pieces), to out: row r of the
+// warp goes to dst + r * ldo, as far as there are rows and columns.
+template <typename OutT>
+__device__ __forceinline__ void turn_and_store(uint8_t* buf, const uint4 (&v)[8], OutT* dst, long long ldo,
+                                               int n_rows, int n_cols, bool vec, int lane) {
+  constexpr int PER = 16 / (int)sizeof(OutT);
+#pragma unroll
+  for (int q = 0; q < 8; ++q)
+    *reinterpret_cast<uint4*>(buf + lane * 128 + ((q ^ (lane & 7)) << 4)) = v[q];
+  __syncwarp();
+  const int q = lane & 7;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = i * 4 + (lane >> 3);
+    const uint4 x = *reinterpret_cast<const uint4*>(buf + r * 128 + ((q ^ (r & 7)) << 4));
+    if (r < n_rows && q * PER < n_cols) {
+      OutT* d = dst + (long long)r * ldo + q * PER;
+      if (vec && q * PER + PER <= n_cols) {
+        *reinterpret_cast<uint4*>(d) = x;
+      } else {
+        const OutT* e = reinterpret_cast<const OutT*>(&x);
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+          if (q * PER + j < n_cols) d[j] = e[j];
+      }
+    }
+  }
+  __syncwarp();
+}
+
+template <typename OutT, bool GATED>
+__global__ void __launch_bounds__(PF_THREADS, 1)
+fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                OutT* __restrict__ out, const PairParams p) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  bf_pdl_trigger();
+  uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t* full = reinterpret_cast<uint64_t*>(base);       // waited on in the leader only
+  uint64_t* empty = full + PF_STAGES;
+  uint64_t* acc_full = empty + PF_STAGES;                   // [2]
+  uint64_t* acc_empty = acc_full + 2;                       // [2], waited on in the leader only
+  uint64_t* drain = acc_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const RowTables tables = row_tables_at(base + PF_BARS, p.experts);
+  uint8_t* turn = base + ((PF_BARS + p.table_bytes + 1023) & ~1023);
+  uint8_t* tiles = turn + 8 * PF_TURN;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = pair_rank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int w_rows = (GATED ? 2 : 1) * p.features;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < PF_STAGES; ++s) {
+      mbar_init(full + s, 1);
+      mbar_init(empty + s, 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(acc_full + a, 1);
+      mbar_init(acc_empty + a, 16);            // one arrival per warp of both CTAs' sums
+    }
+    mbar_init(drain, 1);
+    *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  pair_sync();                                 // the peer's barriers exist before anything lands
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  bf_pdl_wait();
+  fill_row_tables(tables, p.starts, p.experts, p.rows, PF_TILE);
+  __syncthreads();
+  const int units = tables.before[p.experts] * p.tiles_f;
+  int next = 0;                                // (copying thread) the stage behind its last fill
+  uint32_t next_phase = 0;
+
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+  if (warp == 0) {
+    // --------------------------------------------------------------- copies
+    if (lane == 0) {
+      const uint32_t full_leader = pair_map(smem_u32(full), 0);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int u = pair; u < units && ok && !*abort; u += pairs) {
+        const RowTile t = row_tile(tables, p.experts, p.tiles_f, PF_TILE, u);
+        for (int g = 0; g < p.groups; ++g) {
+          if (!mbar_wait(empty + stage, phase ^ 1, abort)) {
+            ok = false;
+            break;
+          }
+          uint8_t* dst = tiles + (size_t)stage * PF_STAGE;
+          const uint32_t bar = full_leader + 8u * (uint32_t)stage;
+          if (rank == 0) mbar_expect_tx(full + stage, 2u * (uint32_t)PF_STAGE);
+          pair_tma_load(dst, &map_x, bar, g * FK, t.row0 + (int)rank * 128);
+          if (GATED) {
+            const int o = t.expert * w_rows + t.ft * 128 + (int)rank * 64;
+            pair_tma_load(dst + PF_HALF, &map_w, bar, g * FK, o);
+            pair_tma_load(dst + PF_HALF + PF_HALF / 2, &map_w, bar, g * FK, o + p.features);
+          } else {
+            pair_tma_load(dst + PF_HALF, &map_w, bar, g * FK,
+                          t.expert * w_rows + t.ft * PF_TILE + (int)rank * 128);
+          }
+          if (++stage == PF_STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      next = stage;
+      next_phase = phase;
+      // every arrival that the leader's commits send to this CTA's barriers lands before it ends
+      for (int s = 0; s < PF_STAGES && ok && !*abort; ++s) {
+        ok = mbar_wait(empty + stage, phase ^ 1, abort);
+        if (++stage == PF_STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------- products
+    if (rank == 0) {
+      const uint32_t idesc = fp8_idesc(PF_TILE, 256);
+      int stage = 0, buf = 0;
+      uint32_t phase = 0, buf_phase = 0;
+      bool ok = true;
+      for (int u = pair; u < units && ok; u += pairs) {
+        for (int g = 0; g < p.groups; ++g) {
+          if (!mbar_wait_warp(acc_empty + buf, buf_phase ^ 1, abort) ||
+              !mbar_wait_warp(full + stage, phase, abort)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a_addr = smem_u32(tiles + (size_t)stage * PF_STAGE);
+          const uint64_t a_desc = umma_desc_k_sw128(a_addr);
+          const uint64_t b_desc = umma_desc_k_sw128(a_addr + PF_HALF);
+#pragma unroll
+          for (int k = 0; k < FK / 32; ++k)
+            pair_umma_fp8(tmem_base + (uint32_t)(buf * 256), a_desc + (uint64_t)(2 * k),
+                          b_desc + (uint64_t)(2 * k), idesc, k > 0 ? 1u : 0u);
+          pair_commit_both(empty + stage);
+          pair_commit_both(acc_full + buf);
+          if (++stage == PF_STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+          if (++buf == 2) {
+            buf = 0;
+            buf_phase ^= 1;
+          }
+        }
+      }
+    }
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    // ----------------------------------------------------------------- sums
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    const int lane_row = (int)rank * 128 + quarter * 32 + lane;
+    const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
+    const uint32_t acc_empty_leader = pair_map(smem_u32(acc_empty), 0);
+    uint8_t* my_turn = turn + (warp - 4) * PF_TURN;
+    const bool vec = ((uintptr_t)out & 15) == 0 && p.ldo * (int)sizeof(OutT) % 16 == 0;
+    int buf = 0;
+    uint32_t buf_phase = 0;
+    for (int u = pair; u < units; u += pairs) {
+      const RowTile t = row_tile(tables, p.experts, p.tiles_f, PF_TILE, u);
+      const int row = t.row0 + lane_row;
+      const float* sx = p.sx + min(row, t.row_end - 1);      // (rows behind the last are not stored)
+      // plain: this half's 128 weight rows have one block's scales; gated: 64 gate and 64 up rows
+      const long long block = (long long)t.expert * (GATED ? 2 : 1) * p.w_blocks;
+      const float* swa = p.sw + (block + (GATED ? t.ft : min(t.ft * 2 + half, p.w_blocks - 1))) * p.groups;
+      const float* swb = GATED ? swa + (long long)p.w_blocks * p.groups : swa;
+      float acc[128];
+#pragma unroll
+      for (int j = 0; j < 128; ++j) acc[j] = 0.f;
+      bool ok = true;
+      float s = sx[0], wa = swa[0], wb = swb[0];
+      for (int g = 0; g < p.groups; ++g) {
+        const float fa = fp8_factor(s, wa), fb = GATED ? fp8_factor(s, wb) : fa;
+        if (g + 1 < p.groups) {                              // the next group's, under this one's wait
+          s = sx[(long long)(g + 1) * p.lds];
+          wa = swa[g + 1];
+          if (GATED) wb = swb[g + 1];
+        }
+        if (!mbar_wait_warp(acc_full + buf, buf_phase, abort)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) {
+          uint32_t r[32];
+          tmem_ld32(taddr + (uint32_t)(buf * 256 + c), r);
+          const float f = c < 64 ? fa : fb;
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) fma2v(acc[c + j], acc[c + j + 1], r[j], r[j + 1], f, f);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) pair_arrive_remote(acc_empty_leader + 8u * (uint32_t)buf);
+        if (++buf == 2) {
+          buf = 0;
+          buf_phase ^= 1;
+        }
+      }
+      if (!ok) break;
+      const float w = p.row_w ? p.row_w[min(row, t.row_end - 1)] : 1.f;
+      const int row_w0 = t.row0 + (int)rank * 128 + quarter * 32;      // the warp's first row
+      const int n_rows = t.row_end - row_w0;
+      if (n_rows > 0) {
+        OutT* dst = out + (long long)row_w0 * p.ldo;
+        if constexpr (GATED) {
+          const int o = t.ft * 128 + half * 64;
+          uint4 v[8];
+          uint32_t* v32 = reinterpret_cast<uint32_t*>(v);
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            v32[j] = pack_bf16x2(
+                __float_as_uint(w * fp8_gate(p.act, acc[2 * j], acc[64 + 2 * j], p.gk)),
+                __float_as_uint(w * fp8_gate(p.act, acc[2 * j + 1], acc[65 + 2 * j], p.gk)));
+          turn_and_store<OutT>(my_turn, v, dst + o, p.ldo, n_rows, p.features - o, vec, lane);
+        } else {
+          constexpr int COLS = 128 / (int)sizeof(OutT);      // of 128 bytes
+#pragma unroll
+          for (int c = 0; c < 128; c += COLS) {
+            const int o = t.ft * PF_TILE + half * 128 + c;
+            uint4 v[8];
+            uint32_t* v32 = reinterpret_cast<uint32_t*>(v);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              if constexpr (sizeof(OutT) == 4) v32[j] = __float_as_uint(w * acc[c + j]);
+              else v32[j] = pack_bf16x2(__float_as_uint(w * acc[c + 2 * j]), __float_as_uint(w * acc[c + 2 * j + 1]));
+            }
+            if (o < p.features)
+              turn_and_store<OutT>(my_turn, v, dst + o, p.ldo, n_rows, p.features - o, vec, lane);
+          }
+        }
+      }
+    }
+  }
+
+  // ------------------------------------------------------------------ wind-down
+  __syncthreads();
+  if (*abort) {
+    if (threadIdx.x == 0) {
+      atomicOr(p.err, BF_ERR_WAIT);
+      // the peer leaves its waits at once instead of running each of them out
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(
+                       pair_map(smem_u32(const_cast<int*>(abort)), rank ^ 1u)),
+                   "r"(1)
+                   : "memory");
+    }
+    if (warp == 0 && lane == 0 && rank == 0) mbar_drain(full, PF_STAGES, next, next_phase);
+    if (warp == 1 && rank == 0) {
+      pair_commit_own(drain);
+      const long long t0 = clock64();
+      while (!mbar_try_wait(drain, 0) && clock64() - t0 < WAIT_LIMIT_CYCLES / 16) {
+      }
+    }
+    __syncthreads();
+  }
+  tc_fence_before();
+  pair_sync();                                 // neither CTA's memory goes while the other uses it
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512)
+                 : "memory");
+  }
+}
+
+template <typename OutT, bool GATED>
+int pair_launch(const void* x, long long ldx, const void* w, long long ldw, OutT* out, PairParams p,
+                int num_sms, cudaStream_t stream) {
+  p.tiles_f = (p.features + (GATED ? 127 : PF_TILE - 1)) / (GATED ? 128 : PF_TILE);
+  p.w_blocks = (p.features + 127) / 128;
+  p.groups = (p.K + FK - 1) / FK;
+  p.table_bytes = row_tables_bytes(p.experts);
+  const long long tiles_r = (p.rows + PF_TILE - 1) / PF_TILE;
+  const long long units = tiles_r * p.experts * p.tiles_f;
+  if (units > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+  const size_t smem =
+      1024 + ((PF_BARS + p.table_bytes + 1023) & ~1023) + 8 * PF_TURN + (size_t)PF_STAGES * PF_STAGE;
+  const size_t smem_max =
+      1024 + ((PF_BARS + row_tables_bytes(FP8_MAX_EXPERTS) + 1023) & ~1023) + 8 * PF_TURN +
+      (size_t)PF_STAGES * PF_STAGE;
+  auto kern = fp8_pair_kernel<OutT, GATED>;
+  static bool configured_on[BF_MAX_DEVICES];
+  bool& configured = configured_on[bf_current_device()];
+  if (!configured) {
+    const cudaError_t ce =
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_max);
+    if (ce != cudaSuccess) return (int)ce;
+    configured = true;
+  }
+  CUtensorMap mx, mw;
+  int e;
+  if ((e = fp8_map(&mx, x, p.rows, p.K, ldx, 128)) ||
+      (e = fp8_map(&mw, w, (long long)p.experts * (GATED ? 2 : 1) * p.features, p.K, ldw, GATED ? 64 : 128)))
+    return e;
+  const long long pairs = units < num_sms / 2 ? units : num_sms / 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * pairs));
+  cfg.blockDim = dim3(PF_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = bf_pdl_enabled();
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const cudaError_t ce = cudaLaunchKernelEx(&cfg, kern, mx, mw, out, p);
+  if (ce != cudaSuccess) return (int)ce;
+  return bf_launch_status();
+}
+
+}  // namespace
+
+// Arguments as bf_gemm_fp8_few's.
+BF_EXPORT int bf_gemm_fp8_pair(const void* x, long long ldx, const float* sx, long long lds, const void* w,
+                               long long ldw, const float* sw, const int* starts, const float* row_w,
+                               void* out, long long ldo, int out_dtype, int rows, int features, int K,
+                               int experts, int gated, int act, float limit, float slope, float up_offset,
+                               int num_sms, int* err, cudaStream_t stream) {
+  if (rows <= 0 || features <= 0) return 0;
+  if (K <= 0 || experts < 1 || experts > FP8_MAX_EXPERTS || (!starts && experts != 1) || ldx % 16 || ldw % 16 ||
+      (((uintptr_t)x | (uintptr_t)w) & 15) || num_sms < 2 ||
+      (act != BF_ACT_SILU && act != BF_ACT_CLAMPED) || (gated && out_dtype != BF_DTYPE_BF16))
+    return (int)cudaErrorInvalidValue;
+  PairParams p = {};
+  p.rows = rows;
+  p.features = features;
+  p.K = K;
+  p.experts = experts;
+  p.starts = starts;
+  p.sx = sx;
+  p.lds = lds;
+  p.sw = sw;
+  p.row_w = row_w;
+  p.ldo = ldo;
+  p.act = act;
+  p.gk = BfGateConst{limit, slope, up_offset};
+  p.err = err;
+  if (gated)
+    return pair_launch<__nv_bfloat16, true>(x, ldx, w, ldw, (__nv_bfloat16*)out, p, num_sms, stream);
+  if (out_dtype == BF_DTYPE_F32)
+    return pair_launch<float, false>(x, ldx, w, ldw, (float*)out, p, num_sms, stream);
+  return pair_launch<__nv_bfloat16, false>(x, ldx, w, ldw, (__nv_bfloat16*)out, p, num_sms, stream);
+}

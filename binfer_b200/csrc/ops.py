@@ -2831,6 +2831,216 @@ def gemm_bf16_swiglu(x: torch.Tensor, w_gate_up: torch.Tensor, out: torch.Tensor
     return True
 
 
+# ------------------------------------------------------------------ weights in 8 bits
+FP8_GROUP = 128                # numbers of a row that share a scale; weights: blocks of 128 x 128
+FP8_MAX_EXPERTS = 512
+E4M3 = torch.float8_e4m3fn
+
+_fp8_product_call = _Packed("bf_fp8_product", "PqPqPqPqPPPPqiiiiiiifffiiiPP")
+
+
+def _fp8_empty_codes(shape, device) -> torch.Tensor:
+    """Room for codes ``[..., K]`` whose rows lie on 16-byte boundaries."""
+    *lead, k = shape
+    pitch = -(-k // 16) * 16
+    strides, step = [1], pitch
+    for n in reversed(lead):
+        strides.append(step)
+        step *= n
+    return torch.empty_strided(tuple(shape), tuple(reversed(strides)), dtype=E4M3, device=device)
+
+
+def _fp8_matrix(what: str, name: str, t: torch.Tensor, dims: Tuple[int, ...] = (2,)) -> None:
+    if t.dim() not in dims or t.dtype not in (torch.bfloat16, torch.float32):
+        raise KernelError(f"{what}: {name} must be bfloat16 or float32 with {' or '.join(map(str, dims))} "
+                          f"dimensions, got {t.dtype} {tuple(t.shape)}")
+    if t.shape[-1] < 1:
+        raise KernelError(f"{what}: {name} has no columns")
+    if t.shape[-1] > 1 and t.numel() and t.stride(-1) != 1:
+        raise KernelError(f"{what}: rows of {name} must be contiguous")
+
+
+def _fp8_stacked(t: torch.Tensor) -> bool:
+    """Whether the rows of all of ``[E, N, K]``'s matrices are equally far apart."""
+    return t.dim() == 2 or t.shape[0] < 2 or t.stride(0) == t.shape[1] * t.stride(1)
+
+
+def _fp8_codes_lie(codes: torch.Tensor) -> bool:
+    """Whether codes lie as the kernels take them: rows contiguous and on 16-byte boundaries."""
+    return ((codes.shape[-1] < 2 or codes.stride(-1) == 1) and codes.stride(-2) % 16 == 0
+            and codes.stride(-2) >= codes.shape[-1] and codes.data_ptr() % 16 == 0 and _fp8_stacked(codes))
+
+
+def fp8_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows ``x [T, K]`` (bfloat16 or float32) in 8 bits: ``(codes float8_e4m3fn [T, K], scales float32
+    [ceil(K / 128), T])``.  The 128 numbers of columns 128 g .. 128 g + 127 of row t share the scale
+    ``s = max(float32(a / 448), 2^-100)``, a the largest size among them, and a number's code is the
+    e4m3 value nearest to ``x / s``, ties to even.  A number that is not finite makes its group read as
+    NaN.  (The codes' rows are padded to 16 bytes: ``codes`` need not be contiguous.)"""
+    _fp8_matrix("fp8_rows", "x", x)
+    T, K = x.shape
+    _same_device("fp8_rows", x)
+    codes = _fp8_empty_codes((T, K), x.device)
+    scales = torch.empty((-(-K // FP8_GROUP), T), dtype=torch.float32, device=x.device)
+    if T:
+        _run("fp8_rows", lib().bf_fp8_rows, _ptr(x), _c_ll(x.stride(0)), _c_int(_dtype_code(x)), _ptr(codes),
+             _c_ll(codes.stride(0)), _ptr(scales), _c_ll(T), _c_int(T), _c_int(K), _c_int(num_sms(x.device)),
+             _c_void_p(_stream_at(x)))
+    return codes, scales
+
+
+def fp8_rows_read(codes: torch.Tensor, scales: torch.Tensor, out: torch.Tensor) -> None:
+    """What :func:`fp8_rows`'s codes and scales stand for, into ``out [T, K]`` (bfloat16 or float32)."""
+    _fp8_matrix("fp8_rows_read", "out", out)
+    T, K = out.shape
+    if codes.dtype != E4M3 or tuple(codes.shape) != (T, K) or (T and not _fp8_codes_lie(codes)):
+        raise KernelError("fp8_rows_read: codes must be float8_e4m3fn of out's shape, their rows contiguous and "
+                          "on 16-byte boundaries")
+    if scales.dtype != torch.float32 or tuple(scales.shape) != (-(-K // FP8_GROUP), T) or (
+            T > 1 and scales.stride(1) != 1):
+        raise KernelError("fp8_rows_read: scales must be float32 [ceil(K / 128), T] with contiguous rows")
+    _same_device("fp8_rows_read", codes, scales, out)
+    if T:
+        _run("fp8_read", lib().bf_fp8_read, _ptr(codes), _c_ll(codes.stride(0)), _ptr(scales),
+             _c_ll(scales.stride(0)), _ptr(out), _c_ll(out.stride(0)), _c_int(_dtype_code(out)), _c_ll(T),
+             _c_int(K), _c_int(1), _c_int(T), _c_int(num_sms(out.device)), _c_void_p(_stream_at(out)))
+
+
+class Fp8Weight:
+    """A weight ``[N, K]``, or one per expert ``[E, N, K]``, in 8 bits: ``codes`` float8_e4m3fn of that shape
+    and ``scales`` float32 ``[(E,) blocks, ceil(K / 128)]``, one per 128 x 128 numbers; a number stands for
+    code times scale.  ``gated``: the weight is a gate weight and an up weight of N / 2 rows each, one
+    behind the other, and the up rows' blocks begin anew (blocks = 2 ceil(N / 2 / 128), else ceil(N / 128)).
+    Scales are positive and finite.  Codes whose rows do not lie on 16-byte boundaries are copied."""
+    __slots__ = ("codes", "scales", "gated", "experts", "rows", "features", "K", "device", "_held")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, gated: bool = False):
+        if codes.dtype != E4M3 or codes.dim() not in (2, 3) or not codes.numel():
+            raise KernelError("Fp8Weight: codes must be float8_e4m3fn [N, K] or [E, N, K]")
+        *lead, n, k = codes.shape
+        if gated and n % 2:
+            raise KernelError("Fp8Weight: a gated weight has as many up rows as gate rows")
+        if lead and lead[0] > FP8_MAX_EXPERTS:
+            raise KernelError(f"Fp8Weight: at most {FP8_MAX_EXPERTS} experts")
+        features = n // 2 if gated else n
+        want = (*lead, -(-features // FP8_GROUP) * (2 if gated else 1), -(-k // FP8_GROUP))
+        if scales.dtype != torch.float32 or tuple(scales.shape) != want or not scales.is_contiguous():
+            raise KernelError(f"Fp8Weight: scales must be contiguous float32 {list(want)}, got {scales.dtype} "
+                              f"{list(scales.shape)}")
+        if scales.device != codes.device:
+            raise KernelError("Fp8Weight: codes and scales must lie on one device")
+        if not _fp8_codes_lie(codes):
+            laid = _fp8_empty_codes(codes.shape, codes.device)
+            laid.view(torch.uint8).copy_(codes.view(torch.uint8))
+            codes = laid
+        self.codes, self.scales, self.gated = codes, scales, bool(gated)
+        self.experts = lead[0] if lead else 0
+        self.rows, self.features, self.K, self.device = n, features, k, codes.device
+        self._held = (codes.data_ptr(), codes.stride(-2), scales.data_ptr())
+
+    @property
+    def shape(self):
+        return self.codes.shape
+
+
+def fp8_weight(w: torch.Tensor, gated: bool = False) -> Fp8Weight:
+    """``w [N, K]`` or ``[E, N, K]`` (bfloat16 or float32) as an :class:`Fp8Weight`: of every block of 128 x 128
+    the scale and the codes as :func:`fp8_rows` takes them of 128 numbers."""
+    _fp8_matrix("fp8_weight", "w", w, (2, 3))
+    if not w.numel() or not _fp8_stacked(w) or (gated and w.shape[-2] % 2):
+        raise KernelError("fp8_weight: w must have rows that are equally far apart, a gated one as many up rows "
+                          "as gate rows")
+    _same_device("fp8_weight", w)
+    *lead, n, k = w.shape
+    halves = 2 if gated else 1
+    codes = _fp8_empty_codes(w.shape, w.device)
+    scales = torch.empty((*lead, halves * -(-(n // halves) // FP8_GROUP), -(-k // FP8_GROUP)),
+                         dtype=torch.float32, device=w.device)
+    _run("fp8_blocks", lib().bf_fp8_blocks, _ptr(w), _c_ll(w.stride(-2)), _c_int(_dtype_code(w)), _ptr(codes),
+         _c_ll(codes.stride(-2)), _ptr(scales), _c_int((lead[0] if lead else 1) * halves), _c_int(n // halves),
+         _c_int(k), _c_void_p(_stream_at(w)))
+    return Fp8Weight(codes, scales, gated)
+
+
+def fp8_weight_read(w: Fp8Weight, out: torch.Tensor) -> None:
+    """What an :class:`Fp8Weight` stands for, into ``out`` of its shape (bfloat16 or float32)."""
+    _fp8_matrix("fp8_weight_read", "out", out, (2, 3))
+    if out.shape != w.shape or not _fp8_stacked(out):
+        raise KernelError("fp8_weight_read: out must have the weight's shape, its rows equally far apart")
+    _same_device("fp8_weight_read", w.codes, w.scales, out)
+    _run("fp8_read", lib().bf_fp8_read, _ptr(w.codes), _c_ll(w.codes.stride(-2)), _ptr(w.scales), _c_ll(0),
+         _ptr(out), _c_ll(out.stride(-2)), _c_int(_dtype_code(out)), _c_ll(max(1, w.experts) * w.rows),
+         _c_int(w.K), _c_int(FP8_GROUP), _c_int(w.features), _c_int(num_sms(out.device)),
+         _c_void_p(_stream_at(out)))
+
+
+def _fp8_product(what: str, x, w: Fp8Weight, starts, out, row_w, activation, limit, slope, up_offset, tile,
+                 split) -> None:
+    M, K = x.shape if x.dim() == 2 else (-1, 0)
+    if x.dtype != torch.bfloat16 or K != w.K or (M > 0 and K > 1 and x.stride(1) != 1):
+        raise KernelError(f"{what}: x must be bfloat16 [rows, {w.K}] with contiguous rows, got {x.dtype} "
+                          f"{tuple(x.shape)}")
+    if (out.dtype not in (torch.bfloat16, torch.float32) or tuple(out.shape) != (M, w.features)
+            or (M > 0 and w.features > 1 and out.stride(1) != 1)):
+        raise KernelError(f"{what}: out must be bfloat16 or float32 [{M}, {w.features}] with contiguous rows, got "
+                          f"{out.dtype} {tuple(out.shape)}")
+    if w.gated and (out.dtype != torch.bfloat16 or activation not in FUSED_ACTIVATIONS):
+        raise KernelError(f"{what}: a gated product has a bfloat16 result and one of the activations "
+                          f"{FUSED_ACTIVATIONS}")
+    if row_w is not None:
+        _want(row_w, torch.float32, "row_w")
+        if row_w.numel() != M:
+            raise KernelError(f"{what}: row_w must have a number per row")
+    if tile not in (0, 16, 32, 64, 128, 256, -1) or not 0 <= split <= 8:
+        raise KernelError(f"{what}: no tiles of {tile} rows, shared by {split}")
+    err = error_word(x.device)
+    _same_device(what, x, w.codes, w.scales, starts, out, row_w, err)
+    if M == 0:
+        return
+    # the rows' codes and behind them their scales
+    pitch, groups = -(-K // 16) * 16, -(-K // FP8_GROUP)
+    scratch = torch.empty(M * pitch + 4 * groups * M, dtype=torch.uint8, device=x.device)
+    at = scratch.data_ptr()
+    w_at, w_pitch, sw_at = w._held
+    _run(what, _fp8_product_call, x.data_ptr(), x.stride(0), at, pitch, at + M * pitch, M, w_at, w_pitch, sw_at,
+         starts.data_ptr() if starts is not None else 0, row_w.data_ptr() if row_w is not None else 0,
+         out.data_ptr(), out.stride(0), 0 if out.dtype == torch.float32 else 1, M, w.features, K,
+         max(1, w.experts), w.gated, GATE_ACTIVATIONS[activation] if w.gated else 0, limit, slope, up_offset, tile,
+         split, num_sms(x.device), err.data_ptr(), _stream_at(x))
+    global _launches
+    _launches += 1          # two kernels
+
+
+def fp8_linear(x: torch.Tensor, w: Fp8Weight, out: torch.Tensor, activation: str = "silu",
+               limit: float = 0.0, slope: float = 1.0, up_offset: float = 0.0, tile: int = 0,
+               split: int = 0) -> None:
+    """``out [M, N] = x [M, K] w^T`` for rows in bfloat16 and a weight in 8 bits: the rows go into 8 bits as
+    :func:`fp8_rows` puts them, the products of codes are added up in float and counted with their scales, 128
+    columns after another.  A gated weight: ``out = act(g) u`` of the product's two halves, ``activation`` as
+    in :func:`gated_act_mul` ("silu" or "clamped").  ``out``: bfloat16, or float32 for a weight that is not
+    gated; it may be a column block of a wider buffer.  A row's result does not depend on the other rows'
+    values.  ``tile``, ``split``: rows of a tile (-1: on pairs of SMs) and SMs that share one (0: chosen by the
+    library)."""
+    if w.experts:
+        raise KernelError("fp8_linear: the weight has experts")
+    _fp8_product("fp8_linear", x, w, None, out, None, activation, limit, slope, up_offset, tile, split)
+
+
+def fp8_experts(x: torch.Tensor, w: Fp8Weight, starts: torch.Tensor, out: torch.Tensor,
+                row_w: Optional[torch.Tensor] = None, activation: str = "silu", limit: float = 0.0,
+                slope: float = 1.0, up_offset: float = 0.0, tile: int = 0) -> None:
+    """:func:`fp8_linear` of rows that are sorted by expert: rows ``starts[e] .. starts[e + 1] - 1`` of ``x``
+    against the e-th matrix of ``w [E, N, K]`` (``starts`` int32 ``[E + 1]``, ascending; an expert may have no
+    rows).  Rows in front of the first expert's and behind the last one's are left as they are.  ``row_w``
+    (float32, one per row): the result's rows count so many times."""
+    if not w.experts:
+        raise KernelError("fp8_experts: the weight has no experts")
+    _want(starts, torch.int32, "starts")
+    if starts.dim() != 1 or starts.numel() != w.experts + 1:
+        raise KernelError(f"fp8_experts: starts must have {w.experts + 1} numbers")
+    _fp8_product("fp8_experts", x, w, starts, out, row_w, activation, limit, slope, up_offset, tile, 0)
+
+
 # -------------------------------------------------------------------- sampling
 def repetition_penalty(logits: torch.Tensor, items: torch.Tensor, penalty: torch.Tensor) -> None:
     """items: int32 [n, 3] of (row, token, count)."""

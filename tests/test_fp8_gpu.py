@@ -1,0 +1,389 @@
+"""Weights in 8 bits: quantising, reading back and the products against their restatement in 64 bits."""
+import gc
+
+import pytest
+import torch
+
+import fp8_plain as P8
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32, F64, E4M3 = torch.bfloat16, torch.float32, torch.float64, torch.float8_e4m3fn
+
+
+def _x(T, K, dev, seed=0, dtype=BF16):
+    g = torch.Generator(dev).manual_seed(seed)
+    x = torch.randn((T, K), generator=g, device=dev) * torch.exp(torch.randn(K, generator=g, device=dev))
+    return x.to(dtype)
+
+
+def _w(shape, dev, seed=0):
+    g = torch.Generator(dev).manual_seed(1000 + seed)
+    return (torch.randn(shape, generator=g, device=dev) * shape[-1] ** -0.5).to(BF16)
+
+
+def _same(a, b):
+    """Equal, NaN where the other is."""
+    return torch.equal(torch.nan_to_num(a, nan=-1234.5), torch.nan_to_num(b, nan=-1234.5))
+
+
+def _check(got, ref, off):
+    # a result is rounded to its type: half a step
+    allowed = off + ref.abs() * (torch.finfo(got.dtype).eps / 2)
+    diff = (got.to(F64) - ref).abs()
+    bad = ~(diff <= allowed)
+    assert not bad.any(), (f"{int(bad.sum())} of {bad.numel()} too far off, worst "
+                           f"{float((diff / allowed).nan_to_num(0).max()):.3g} of what is allowed")
+
+
+# ------------------------------------------------------------------------- into 8 bits and back
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T,K", [(1, 1), (1, 128), (3, 129), (7, 16), (33, 1000), (5, 4096), (130, 333)])
+def test_rows(cuda_device, T, K, dtype):
+    from binfer_b200.csrc import ops
+    x = _x(T, K, cuda_device, T + K, dtype)
+    codes, scales = ops.fp8_rows(x)
+    v, s = P8.hold(x, 1)
+    assert torch.equal(scales.t(), s)
+    assert torch.equal(codes.to(F32).to(F64), v)
+    for out_type in (F32, BF16):
+        out = torch.empty((T, K), dtype=out_type, device=cuda_device)
+        ops.fp8_rows_read(codes, scales, out)
+        assert torch.equal(out, P8.dense(v, s, 1).to(F32).to(out_type))
+
+
+@pytest.mark.parametrize("K,off", [(256, 1), (250, 3), (77, 5)])
+def test_rows_of_a_wider_buffer(cuda_device, K, off):
+    from binfer_b200.csrc import ops
+    wide = _x(9, K + 17, cuda_device, K)
+    codes, scales = ops.fp8_rows(wide[:, off:off + K])
+    ref, s = ops.fp8_rows(wide[:, off:off + K].contiguous())
+    assert torch.equal(codes.view(torch.uint8), ref.view(torch.uint8)) and torch.equal(scales, s)
+    out = torch.full((9, K + 17), 7.0, device=cuda_device)
+    ops.fp8_rows_read(codes, scales, out[:, off:off + K])
+    assert (out[:, :off] == 7).all() and (out[:, off + K:] == 7).all()
+    assert torch.equal(out[:, off:off + K], P8.dense(*P8.hold(wide[:, off:off + K], 1), 1).to(F32))
+
+
+def test_rows_next_to_a_border(cuda_device):
+    """Numbers on the middle of two codes and one place to either side of it, for scales of every kind."""
+    from binfer_b200.csrc import ops
+    g = torch.Generator().manual_seed(5)
+    v = P8.values()
+    mid = (v[1:] + v[:-1]) / 2                                    # 126 of them
+    rows = []
+    for i in range(600):
+        top = torch.rand(1, generator=g).item() * 2.0 ** ((i % 60) - 30)
+        s = P8.scale(torch.tensor([top]))
+        x = (mid * s.to(F64)).to(F32)
+        x = torch.nextafter(x, x + [0, 1e30, -1e30][i % 3])
+        rows.append(torch.cat([torch.tensor([top, -top]), x * (1 - 2 * (torch.arange(126) % 2))]).to(F32))
+    x = torch.stack(rows).to(cuda_device)
+    codes, scales = ops.fp8_rows(x)
+    v, s = P8.hold(x, 1)
+    assert torch.equal(scales.t(), s) and torch.equal(codes.to(F32).to(F64), v)
+
+
+@pytest.mark.parametrize("size", [2.0 ** -149, 2.0 ** -130, 2.0 ** -101, 2.0 ** -93, 2.0 ** -60, 2.0 ** 100,
+                                  2.0 ** 127])
+def test_rows_of_any_size(cuda_device, size):
+    from binfer_b200.csrc import ops
+    g = torch.Generator().manual_seed(int(abs(torch.tensor(size).log2())))
+    x = ((torch.rand((8, 256), generator=g, dtype=F64) * 2 - 1) * size * 1.9).to(F32).to(cuda_device)
+    codes, scales = ops.fp8_rows(x)
+    v, s = P8.hold(x, 1)
+    assert torch.equal(scales.t(), s) and torch.equal(codes.to(F32).to(F64), v)
+
+
+def test_rows_that_are_not_finite(cuda_device):
+    from binfer_b200.csrc import ops
+    x = _x(6, 300, cuda_device, 3)
+    x[1, 5], x[2, 140], x[3, 299], x[4] = float("inf"), float("nan"), float("-inf"), 0
+    codes, scales = ops.fp8_rows(x)
+    v, s = P8.hold(x, 1)
+    assert _same(scales.t(), s) and _same(codes.to(F32).to(F64), v)
+    assert int(torch.isnan(s).sum()) == 3 and not codes[4].to(F32).any()
+
+
+@pytest.mark.parametrize("shape,gated", [((1, 1), False), ((128, 128), False), ((300, 200), False),
+                                         ((129, 77), False), ((300, 200), True), ((3, 130, 260), False),
+                                         ((2, 260, 100), True), ((1000, 1111), False)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_weight(cuda_device, shape, gated, dtype):
+    from binfer_b200.csrc import ops
+    w = _w(shape, cuda_device, sum(shape)).to(dtype) * 3
+    h = ops.fp8_weight(w, gated)
+    mats = [w] if w.dim() == 2 else list(w)
+    for i, m in enumerate(mats):
+        v, s = P8.hold_weight(m, gated)
+        hs, hc = (h.scales, h.codes) if w.dim() == 2 else (h.scales[i], h.codes[i])
+        assert torch.equal(hs, s) and torch.equal(hc.to(F32).to(F64), v)
+    for out_type in (F32, BF16):
+        out = torch.empty(shape, dtype=out_type, device=cuda_device)
+        ops.fp8_weight_read(h, out)
+        for i, m in enumerate(mats):
+            ref = P8.dense(*P8.hold_weight(m, gated), 128, gated).to(F32).to(out_type)
+            assert torch.equal(out if w.dim() == 2 else out[i], ref)
+
+
+def test_weight_of_a_wider_buffer(cuda_device):
+    from binfer_b200.csrc import ops
+    wide = _w((300, 263), cuda_device)
+    a, b = ops.fp8_weight(wide[:, 5:205]), ops.fp8_weight(wide[:, 5:205].contiguous())
+    assert torch.equal(a.codes.view(torch.uint8), b.codes.view(torch.uint8)) and torch.equal(a.scales, b.scales)
+    with pytest.raises(ops.KernelError):
+        ops.fp8_weight(wide[:200].view(2, 100, 263)[:, :99])          # the matrices lie further apart
+
+
+# --------------------------------------------------------------------------------- products
+def _linear(dev, M, K, N, gated=False, out_type=BF16, seed=0, **kw):
+    from binfer_b200.csrc import ops
+    x, w = _x(M, K, dev, seed), _w(((2 if gated else 1) * N, K), dev, seed)
+    out = torch.full((M, N), float("nan"), dtype=out_type, device=dev)
+    ops.fp8_linear(x, ops.fp8_weight(w, gated), out, **kw)
+    assert ops.error_word(dev).item() == 0
+    return out, P8.product(x, *P8.hold_weight(w, gated), gated)
+
+
+SIZES = [(1, 128, 128), (1, 16, 16), (3, 1, 5), (8, 384, 640), (16, 1000, 130), (17, 256, 257), (33, 130, 96),
+         (64, 512, 300), (65, 2048, 128), (129, 640, 200), (200, 100, 1000), (257, 384, 513), (300, 1024, 64)]
+
+
+@pytest.mark.parametrize("tile", [16, 32, 64, 128, 256, -1])
+@pytest.mark.parametrize("M,K,N", SIZES)
+def test_linear_of_every_tile(cuda_device, M, K, N, tile):
+    out, ref = _linear(cuda_device, M, K, N, out_type=F32, seed=M + N, tile=tile)
+    _check(out, *ref)
+
+
+@pytest.mark.parametrize("tile", [16, 32, 64, 128, 256, -1])
+@pytest.mark.parametrize("M,K,N", [(1, 128, 64), (5, 300, 100), (16, 512, 128), (40, 256, 200), (130, 640, 65),
+                                   (300, 384, 300), (520, 256, 130)])
+def test_gated_linear_of_every_tile(cuda_device, M, K, N, tile):
+    out, ref = _linear(cuda_device, M, K, N, gated=True, seed=M + N, tile=tile)
+    _check(out, *ref)
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("split", [1, 2, 3, 4, 5, 6, 7, 8])
+@pytest.mark.parametrize("M,K,N", [(1, 1024, 128), (7, 1100, 300), (16, 2048, 640), (33, 1024, 200), (64, 4096, 128)])
+def test_linear_shared_by_a_cluster(cuda_device, M, K, N, split, gated):
+    out, ref = _linear(cuda_device, M, K, N, gated=gated, seed=split, split=split)
+    _check(out, *ref)
+
+
+@pytest.mark.parametrize("M,K,N,gated", [(1, 4096, 6144, False), (8, 12288, 4096, False), (8, 4096, 12288, True),
+                                         (100, 4096, 1024, False), (1030, 2048, 2048, True), (2048, 1024, 4096, False)])
+def test_linear_as_chosen(cuda_device, M, K, N, gated):
+    out, ref = _linear(cuda_device, M, K, N, gated=gated)
+    _check(out, *ref)
+
+
+@pytest.mark.parametrize("M", [3, 40, 150, 300])
+def test_linear_of_strided_rows(cuda_device, M):
+    """Column blocks of wider buffers, at odd offsets, on both sides; what lies beside the result stays."""
+    from binfer_b200.csrc import ops
+    wide, w = _x(M, 400, cuda_device, M), _w((203, 333), cuda_device)
+    x, held = wide[:, 13:346], ops.fp8_weight(w)
+    for out_type, off in ((BF16, 3), (F32, 1), (BF16, 8)):
+        out = torch.full((M, 230), 5.0, dtype=out_type, device=cuda_device)
+        ops.fp8_linear(x, held, out[:, off:off + 203])
+        _check(out[:, off:off + 203], *P8.product(x, *P8.hold_weight(w)))
+        assert (out[:, :off] == 5).all() and (out[:, off + 203:] == 5).all()
+
+
+@pytest.mark.parametrize("M", [4, 50, 300])
+def test_clamped_activation(cuda_device, M):
+    from binfer_b200.csrc import ops
+    x, w = _x(M, 256, cuda_device, M) * 2, _w((400, 256), cuda_device)
+    out = torch.empty((M, 200), dtype=BF16, device=cuda_device)
+    ops.fp8_linear(x, ops.fp8_weight(w, True), out, activation="clamped", limit=1.5, slope=1.7, up_offset=1.0)
+
+    def act(g, u):
+        g, u = g.clamp_max(1.5), u.clamp(-1.5, 1.5) + 1.0
+        return g * torch.sigmoid(1.7 * g), u
+    ref, off = P8.product(x, *P8.hold_weight(w, True), True, act)
+    _check(out, ref, off)
+
+
+@pytest.mark.parametrize("M", [6, 70, 300])
+def test_rows_do_not_touch_one_another(cuda_device, M):
+    """A row with an infinity or a NaN is NaN; the others are what they were.  A row of zeros is zero."""
+    from binfer_b200.csrc import ops
+    x, w = _x(M, 384, cuda_device, M), ops.fp8_weight(_w((300, 384), cuda_device))
+    x[2] = 0
+    a = torch.empty((M, 300), dtype=BF16, device=cuda_device)
+    ops.fp8_linear(x, w, a)
+    assert not a[2].any()
+    x[1, 7], x[4, 300], x[5, 383] = float("inf"), float("nan"), float("-inf")
+    b = torch.empty_like(a)
+    ops.fp8_linear(x, w, b)
+    bad = torch.tensor([1, 4, 5], device=cuda_device)
+    assert torch.isnan(b[bad]).all()
+    rest = torch.ones(M, dtype=torch.bool, device=cuda_device)
+    rest[bad] = False
+    assert torch.equal(a[rest], b[rest])
+
+
+def test_scales_of_any_size(cuda_device):
+    """Products of scales that a float has no room for count with the largest float and leave zeros zero."""
+    from binfer_b200.csrc import ops
+    for M in (3, 300):
+        x = torch.zeros((M, 256), dtype=BF16, device=cuda_device)
+        x[:, 0], x[1, 0] = 2.0 ** 120, 2.0 ** -120
+        w = torch.zeros((128, 256), device=cuda_device)
+        w[:, 1] = 2.0 ** 100
+        w[5, 0] = 2.0 ** -60
+        w[:, 200], x[:, 200] = 1.0, 3.0
+        out = torch.empty((M, 128), dtype=F32, device=cuda_device)
+        ops.fp8_linear(x, ops.fp8_weight(w), out)
+        # (2^-60 is far below a code's step beside 2^100: it reads as zero.  448 x 448 times two scales,
+        # each rounded, their product and the sum too)
+        assert ((out - 3.0).abs() <= 3.0 * 2.0 ** -21).all()
+
+
+def test_empty_calls(cuda_device):
+    from binfer_b200.csrc import ops
+    w = ops.fp8_weight(_w((300, 200), cuda_device))
+    ops.fp8_linear(torch.empty((0, 200), dtype=BF16, device=cuda_device), w,
+                   torch.empty((0, 300), dtype=BF16, device=cuda_device))
+    codes, scales = ops.fp8_rows(torch.empty((0, 200), dtype=BF16, device=cuda_device))
+    assert codes.shape == (0, 200) and scales.shape == (2, 0)
+    ops.fp8_rows_read(codes, scales, torch.empty((0, 200), device=cuda_device))
+
+
+# ---------------------------------------------------------------------------------- experts
+def _experts(dev, counts, K, N, gated=False, out_type=BF16, before=0, behind=0, weighted=False, seed=0, tile=0):
+    from binfer_b200.csrc import ops
+    E, R = len(counts), before + sum(counts) + behind
+    x, w = _x(R, K, dev, seed), _w((E, (2 if gated else 1) * N, K), dev, seed)
+    starts = [before]
+    for c in counts:
+        starts.append(starts[-1] + c)
+    row_w = torch.rand(R, device=dev) if weighted else None
+    out = torch.full((R, N), 9.0, dtype=out_type, device=dev)
+    ops.fp8_experts(x, ops.fp8_weight(w, gated), torch.tensor(starts, dtype=torch.int32, device=dev), out,
+                    row_w=row_w, tile=tile)
+    assert ops.error_word(dev).item() == 0
+    assert (out[:before] == 9).all() and (out[R - behind:] == 9).all()
+    for e, (a, b) in enumerate(zip(starts, starts[1:])):
+        if b > a:
+            ref, off = P8.product(x[a:b], *P8.hold_weight(w[e], gated), gated)
+            if weighted:
+                ref, off = ref * row_w[a:b, None].to(F64), (off + ref.abs() * 2.0 ** -23) * row_w[a:b, None].to(F64)
+            _check(out[a:b], ref, off)
+
+
+@pytest.mark.parametrize("tile", [0, 16, 32, 64, 128, 256, -1])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("counts", [[1], [0, 0, 3], [5, 0, 17, 1, 16, 0], [40, 300, 0, 129, 64], [600, 2]])
+def test_experts(cuda_device, counts, gated, tile):
+    _experts(cuda_device, counts, 384, 200, gated=gated, seed=len(counts), tile=tile)
+
+
+@pytest.mark.parametrize("K,N", [(100, 16), (704, 130), (129, 1)])
+@pytest.mark.parametrize("tile", [0, -1])
+def test_experts_in_part_of_the_rows(cuda_device, K, N, tile):
+    _experts(cuda_device, [7, 0, 30, 260], K, N, before=5, behind=11, weighted=True, out_type=F32, tile=tile)
+    _experts(cuda_device, [3, 4], K, N, before=1, behind=2, weighted=True, gated=True, tile=tile)
+
+
+def test_many_experts(cuda_device):
+    _experts(cuda_device, [(i * 7) % 5 for i in range(512)], 128, 64)
+
+
+def test_no_rows_at_all(cuda_device):
+    _experts(cuda_device, [0, 0, 0], 256, 128, before=4, behind=3)
+    _experts(cuda_device, [0, 0, 0], 256, 128, before=4, behind=3, gated=True, tile=-1)
+
+
+@pytest.mark.parametrize("tile", [16, -1])
+def test_starts_outside_the_rows(cuda_device, tile):
+    """Whatever the starts hold, what is read and written lies inside the rows."""
+    from binfer_b200.csrc import ops
+    x, w = _x(20, 128, cuda_device), ops.fp8_weight(_w((3, 64, 128), cuda_device))
+    out = torch.full((20, 64), 9.0, dtype=BF16, device=cuda_device)
+    s = torch.tensor([-5, 4, 2, 1000], dtype=torch.int32, device=cuda_device)
+    ops.fp8_experts(x, w, s, out, tile=tile)
+    # (the first expert has rows 0 .. 3, the second none, the third 2 .. 19, two rows of which are both's)
+    _check(out[:2], *P8.product(x[:2], w.codes[0].to(F32).to(F64), w.scales[0]))
+    _check(out[4:], *P8.product(x[4:], w.codes[2].to(F32).to(F64), w.scales[2]))
+
+
+# ------------------------------------------------------------------------ streams, graphs, together
+def test_on_another_stream(cuda_device):
+    from binfer_b200.csrc import ops
+    x, w = _x(8, 512, cuda_device), _w((256, 512), cuda_device)
+    side = torch.cuda.Stream(cuda_device)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = torch.empty((8, 256), dtype=BF16, device=cuda_device)
+        for _ in range(20):
+            h = ops.fp8_weight(w * 1.0)               # the weight made right before the product
+            ops.fp8_linear(x, h, out)
+    side.synchronize()
+    _check(out, *P8.product(x, *P8.hold_weight(w)))
+
+
+@pytest.mark.parametrize("M", [8, 300])
+def test_captured_and_replayed(cuda_device, M):
+    """Two graphs of one weight, replayed in turn with other rows."""
+    from binfer_b200.csrc import ops
+    w, e = _w((256, 512), cuda_device), _w((4, 256, 256), cuda_device)
+    held, held_e = ops.fp8_weight(w), ops.fp8_weight(e, True)
+    starts = torch.tensor([0, 2, 2, 5, M], dtype=torch.int32, device=cuda_device)
+
+    def step(x, y, z):
+        ops.fp8_linear(x, held, y)
+        ops.fp8_experts(y, held_e, starts, z)
+    graphs = []
+    for seed in range(2):
+        x = _x(M, 512, cuda_device, seed)
+        y = torch.empty((M, 256), dtype=BF16, device=cuda_device)
+        z = torch.empty((M, 128), dtype=BF16, device=cuda_device)
+        step(x, y, z)
+        torch.cuda.synchronize()
+        gc.collect()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            step(x, y, z)
+        graphs.append((g, x, y, z))
+    for seed in range(4):
+        g, x, y, z = graphs[seed % 2]
+        x.copy_(_x(M, 512, cuda_device, 50 + seed))
+        g.replay()
+        _check(y, *P8.product(x, *P8.hold_weight(w)))
+        s = starts.tolist()
+        for i, (a, b) in enumerate(zip(s, s[1:])):
+            if b > a:
+                _check(z[a:b], *P8.product(y[a:b], *P8.hold_weight(e[i], True), True))
+
+
+def test_a_feed_forward(cuda_device):
+    """The operators one behind the other, as a mixture uses them: rows sorted by expert, gate and up, down."""
+    from binfer_b200.csrc import ops
+    counts = [9, 0, 40, 3]
+    R, starts = sum(counts), torch.tensor([0, 9, 9, 49, 52], dtype=torch.int32, device=cuda_device)
+    x, row_w = _x(R, 256, cuda_device), torch.rand(52, device=cuda_device)
+    gu, dn = _w((4, 384, 256), cuda_device, 1), _w((4, 256, 192), cuda_device, 2)
+    h = torch.empty((R, 192), dtype=BF16, device=cuda_device)
+    y = torch.empty((R, 256), dtype=F32, device=cuda_device)
+    ops.fp8_experts(x, ops.fp8_weight(gu, True), starts, h)
+    ops.fp8_experts(h, ops.fp8_weight(dn), starts, y, row_w=row_w)
+    s = starts.tolist()
+    for e, (a, b) in enumerate(zip(s, s[1:])):
+        if b > a:
+            _check(h[a:b], *P8.product(x[a:b], *P8.hold_weight(gu[e], True), True))
+            ref, off = P8.product(h[a:b], *P8.hold_weight(dn[e]))
+            k = row_w[a:b, None].to(F64)
+            _check(y[a:b], ref * k, (off + ref.abs() * 2.0 ** -23) * k)
+
+
+def test_repeats_bit_for_bit(cuda_device):
+    from binfer_b200.csrc import ops
+    for M in (5, 100, 600):
+        x, w = _x(M, 2048, cuda_device), ops.fp8_weight(_w((512, 2048), cuda_device))
+        outs = [torch.empty((M, 512), dtype=F32, device=cuda_device) for _ in range(5)]
+        for o in outs:
+            ops.fp8_linear(x, w, o)
+        assert all(torch.equal(outs[0], o) for o in outs[1:])
