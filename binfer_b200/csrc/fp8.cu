@@ -1,157 +1,191 @@
 // Activations and weights into 8 bits and back (the format: fp8.cuh).
 //
-// All four kernels pass over the data once, with the numbers of a group in registers between the
-// search for the largest and the rounding; what bounds them is memory.
+// All kernels pass over the data once, with the numbers of a group in registers between the search for
+// the largest and the rounding; what bounds them is memory.
 #include "fp8.cuh"
 
 namespace {
 
-constexpr int ROWS_THREADS = 256;
+constexpr int F8_THREADS = 256;
 
-// 16 lanes hold a group of 128 numbers of a row, eight each; groups of a row side by side.
-// scales [groups, lds]: the rows' scales of one group of columns lie together, as the products that
-// read them want them.
+// How a grid walks the groups of a matrix, `places` of them in a block's hands: `across` groups of a row
+// side by side (a power of two), places / across rows at once; blockIdx.x counts the former, blockIdx.y
+// the latter.
+struct Fp8Walk {
+  int shift;                                     // log2(across)
+  dim3 grid;
+};
+Fp8Walk fp8_walk(int places, long long rows, int groups, int num_sms, int mats) {
+  Fp8Walk w;
+  w.shift = 0;
+  while ((1 << w.shift) < places && (1 << w.shift) < groups) ++w.shift;
+  const int x = (groups + (1 << w.shift) - 1) >> w.shift;
+  const int at_once = places >> w.shift;
+  long long y = (rows + at_once - 1) / at_once;
+  const long long most = (8LL * num_sms + (long long)x * mats - 1) / ((long long)x * mats);   // 8 blocks an SM
+  if (y > most) y = most;
+  if (y > 65535) y = 65535;
+  w.grid = dim3((unsigned)x, (unsigned)y, (unsigned)mats);
+  return w;
+}
+
+__device__ __forceinline__ void fp8_store16(uint8_t* dst, const uint4& c, int n) {
+  if (n >= 16) {
+    *reinterpret_cast<uint4*>(dst) = c;            // (rows of codes lie on 16-byte boundaries)
+  } else {
+    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (j < n) dst[j] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
+  }
+}
+
+// Eight lanes a group, sixteen numbers each.  scales [groups, lds]: the rows' scales of one group of
+// columns lie together, as the products that read them want them.
+constexpr int F8_ROW_PLACES = F8_THREADS / 8;
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(ROWS_THREADS)
+__global__ void __launch_bounds__(F8_THREADS)
 fp8_rows_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ codes, long long ldc,
-                float* __restrict__ scales, long long lds, int rows, int K, int groups) {
+                float* __restrict__ scales, long long lds, int rows, int K, int groups, int shift) {
   bf_pdl_trigger();
+  const int sub = threadIdx.x & 7, place = threadIdx.x >> 3;
+  const int g = (blockIdx.x << shift) + (place & ((1 << shift) - 1));
+  const int at_once = F8_ROW_PLACES >> shift;
+  const int step = (int)gridDim.y * at_once;
+  const int k = g * BF_FP8_GROUP + sub * 16, n = g < groups ? K - k : 0;
+  long long t = (long long)blockIdx.y * at_once + (place >> shift);
+  const T* src = x + t * ldx + k;
+  uint8_t* dst = codes + t * ldc + k;
+  float* at = scales + g * lds + t;
+  // (every lane of a block takes as many turns: the shuffles are the whole warp's)
+  const int turns = (rows - (int)blockIdx.y * at_once + step - 1) / step;
   bf_pdl_wait();
-  const int sub = threadIdx.x & 15;
-  const long long total = (long long)rows * groups;
-  const long long step = (long long)gridDim.x * (ROWS_THREADS / 16);
-  const long long first = (long long)blockIdx.x * (ROWS_THREADS / 16) + threadIdx.x / 16;
-  // (both halves of a warp take as many turns: the shuffles below are the whole warp's)
-  for (long long i = first; i - (first & 1) < total; i += step) {
-    const bool there = i < total;
-    const int t = there ? (int)(i / groups) : 0, g = there ? (int)(i - (long long)t * groups) : 0;
-    const int k = g * BF_FP8_GROUP + sub * 8, n = there ? min(8, K - k) : 0;
-    float v[8];
-    const T* src = x + (long long)t * ldx + k;
-    if (VEC && n == 8) {
-      fp8_load8<true>(src, 8, v);
+  for (int i = 0; i < turns; ++i) {
+    const bool there = t < rows;
+    Fp8Sixteen<T> v;
+    if (VEC && n >= 16 && there) {
+      v.template load<true>(src, 16);
     } else {
-      fp8_load8<false>(src, n, v);
+      v.template load<false>(src, there ? n : 0);
     }
-    uint32_t m = fp8_largest8(v);
+    uint32_t m = v.largest();
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float s = fp8_scale(m), inv = __fdiv_rn(1.f, s);
-    if (n > 0) {
-      const uint2 c = make_uint2(fp8_codes4(v, s, inv), fp8_codes4(v + 4, s, inv));
-      uint8_t* dst = codes + (long long)t * ldc + k;         // (ldc: a multiple of 16)
-      if (n == 8) {
-        *reinterpret_cast<uint2*>(dst) = c;
-      } else {
-        for (int j = 0; j < n; ++j) dst[j] = (uint8_t)((j < 4 ? c.x : c.y) >> (8 * (j & 3)));
-      }
+    for (int o = 4; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const Fp8Scale s = fp8_scale(m);
+    if (there && n > 0) {
+      fp8_store16(dst, v.codes(s), n);
+      if (sub == 0) *at = s.s;
     }
-    if (there && sub == 0) scales[(long long)g * lds + t] = s;
+    t += step;
+    src += step * ldx;
+    dst += step * ldc;
+    at += step;
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(ROWS_THREADS)
+// Sixteen lanes a group.  blockIdx.z: the matrix, of mat_rows rows.  BLOCKS: a scale per 128 rows of it and group, [blocks,
+// groups]; else one per row and group, [groups, lds].
+constexpr int F8_READ_PLACES = F8_THREADS / 16;
+template <typename T, bool BLOCKS>
+__global__ void __launch_bounds__(F8_THREADS)
 fp8_read_kernel(const uint8_t* __restrict__ codes, long long ldc, const float* __restrict__ scales,
-                long long lds, T* __restrict__ out, long long ldo, long long rows, int K, int groups,
-                int block_rows, int mat_rows, int mat_blocks, bool vec) {
+                long long lds, T* __restrict__ out, long long ldo, int mat_rows, int K, int groups, int shift,
+                bool vec) {
   bf_pdl_trigger();
+  const int sub = threadIdx.x & 15, place = threadIdx.x >> 4;
+  const int g = (blockIdx.x << shift) + (place & ((1 << shift) - 1)), r = place >> shift;
+  const int at_once = F8_READ_PLACES >> shift;
+  const long long step = (long long)gridDim.y * at_once;
+  const int k = g * BF_FP8_GROUP + sub * 8, n = g < groups ? min(8, K - k) : 0;
   bf_pdl_wait();
-  const int sub = threadIdx.x & 15;
-  const long long total = rows * groups;
-  for (long long i = (long long)blockIdx.x * (ROWS_THREADS / 16) + threadIdx.x / 16; i < total;
-       i += (long long)gridDim.x * (ROWS_THREADS / 16)) {
-    const long long t = i / groups;
-    const int g = (int)(i - t * groups);
-    const int k = g * BF_FP8_GROUP + sub * 8, n = min(8, K - k);
-    if (n <= 0) continue;
-    // (rows: a scale per row and group, groups first; blocks: one per 128 rows of a matrix and group)
-    const float s = block_rows == 1
-                        ? scales[(long long)g * lds + t]
-                        : scales[((t / mat_rows) * mat_blocks + t % mat_rows / block_rows) * groups + g];
-    const uint8_t* src = codes + t * ldc + k;
-    uint2 c;
-    if (n == 8) {
-      c = *reinterpret_cast<const uint2*>(src);
-    } else {
-      c = make_uint2(0u, 0u);
-      for (int j = 0; j < n; ++j) (j < 4 ? c.x : c.y) |= (uint32_t)src[j] << (8 * (j & 3));
-    }
-    float v[8];
-    fp8_values4(c.x, v);
-    fp8_values4(c.y, v + 4);
+  if (n <= 0) return;
+  codes += (long long)blockIdx.z * mat_rows * ldc;
+  out += (long long)blockIdx.z * mat_rows * ldo;
+  if (BLOCKS) scales += (long long)blockIdx.z * ((mat_rows + BF_FP8_GROUP - 1) / BF_FP8_GROUP) * groups;
+  for (long long t0 = (long long)blockIdx.y * at_once + r; t0 < mat_rows; t0 += 2 * step) {
+    uint2 c[2];
+    float s[2];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= s;
-    T* dst = out + t * ldo + k;
-    if (vec && n == 8) {
-      if constexpr (sizeof(T) == 4) {
-        reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
-      } else {
-        uint4 o;
-        __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(&o);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o2[j] = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-        *reinterpret_cast<uint4*>(dst) = o;
+    for (int i = 0; i < 2; ++i) {
+      const long long t = t0 + i * step;
+      c[i] = make_uint2(0u, 0u);
+      s[i] = 0.f;
+      if (t < mat_rows) {
+        const uint8_t* src = codes + t * ldc + k;
+        s[i] = BLOCKS ? scales[(t / BF_FP8_GROUP) * groups + g] : scales[g * lds + t];
+        if (n == 8) {
+          c[i] = *reinterpret_cast<const uint2*>(src);
+        } else {
+          for (int j = 0; j < n; ++j) (j < 4 ? c[i].x : c[i].y) |= (uint32_t)src[j] << (8 * (j & 3));
+        }
       }
-    } else {
-      for (int j = 0; j < n; ++j) bf_st(dst + j, v[j]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const long long t = t0 + i * step;
+      if (t >= mat_rows) break;
+      float v[8];
+      fp8_values4(c[i].x, v);
+      fp8_values4(c[i].y, v + 4);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= s[i];
+      T* dst = out + t * ldo + k;
+      if (vec && n == 8) {
+        if constexpr (sizeof(T) == 4) {
+          reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
+          reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+          uint4 o;
+          __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(&o);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o2[j] = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+          *reinterpret_cast<uint4*>(dst) = o;
+        }
+      } else {
+        for (int j = 0; j < n; ++j) bf_st(dst + j, v[j]);
+      }
     }
   }
 }
 
-// A block of 128 x 128 per CTA: 16 lanes a row, 16 rows at a time, eight such passes held in registers.
+// A block of 128 x 128 per CTA: 8 lanes a row, 32 rows at a time, four such passes held in registers.
+// blockIdx: (group, block of rows, matrix).
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(F8_THREADS)
 fp8_blocks_kernel(const T* __restrict__ w, long long ldw, uint8_t* __restrict__ codes, long long ldc,
-                  float* __restrict__ scales, int mat_rows, int mat_blocks, int K, int groups) {
-  __shared__ uint32_t warp_max[8];
-  const int sub = threadIdx.x & 15, lead = threadIdx.x >> 4;
-  const int g = blockIdx.x % groups;
-  const long long b = blockIdx.x / groups;                     // block row over all matrices
-  const long long mat = b / mat_blocks;
-  const int r0 = (int)(b - mat * mat_blocks) * BF_FP8_GROUP;
-  const int k = g * BF_FP8_GROUP + sub * 8, n = min(8, K - k);
-  float v[8][8];
+                  float* __restrict__ scales, int mat_rows, int K) {
+  __shared__ uint32_t warp_max[F8_THREADS / 32];
+  const int sub = threadIdx.x & 7, lead = threadIdx.x >> 3;
+  const int g = blockIdx.x, r0 = blockIdx.y * BF_FP8_GROUP;
+  const long long first = (long long)blockIdx.z * mat_rows;
+  const int k = g * BF_FP8_GROUP + sub * 16, n = K - k;
+  Fp8Sixteen<T> v[4];
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = r0 + i * 16 + lead, nn = r < mat_rows ? n : 0;
-    const T* src = w + (mat * mat_rows + r) * ldw + k;
-    if (VEC && nn == 8) {
-      fp8_load8<true>(src, 8, v[i]);
+  for (int i = 0; i < 4; ++i) {
+    const int r = r0 + i * 32 + lead, there = r < mat_rows ? n : 0;
+    const T* src = w + (first + r) * ldw + k;
+    if (VEC && there >= 16) {
+      v[i].template load<true>(src, 16);
     } else {
-      fp8_load8<false>(src, nn, v[i]);
+      v[i].template load<false>(src, there);
     }
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, fp8_largest8(v[i]));
+  for (int i = 0; i < 4; ++i) m = max(m, v[i].largest());
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
   if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = m;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, warp_max[i]);
-  const float s = fp8_scale(m), inv = __fdiv_rn(1.f, s);
-  if (threadIdx.x == 0) scales[b * groups + g] = s;
+  for (int i = 0; i < F8_THREADS / 32; ++i) m = max(m, warp_max[i]);
+  const Fp8Scale s = fp8_scale(m);
+  if (threadIdx.x == 0) scales[((long long)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + g] = s.s;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = r0 + i * 16 + lead;
-    if (r >= mat_rows || n <= 0) continue;
-    const uint2 c = make_uint2(fp8_codes4(v[i], s, inv), fp8_codes4(v[i] + 4, s, inv));
-    uint8_t* dst = codes + (mat * mat_rows + r) * ldc + k;
-    if (n == 8) {
-      *reinterpret_cast<uint2*>(dst) = c;
-    } else {
-      for (int j = 0; j < n; ++j) dst[j] = (uint8_t)((j < 4 ? c.x : c.y) >> (8 * (j & 3)));
-    }
+  for (int i = 0; i < 4; ++i) {
+    const int r = r0 + i * 32 + lead;
+    if (r < mat_rows && n > 0) fp8_store16(codes + (first + r) * ldc + k, v[i].codes(s), n);
   }
-}
-
-int blocks_for(long long items, int num_sms) {
-  const long long blocks = (items + ROWS_THREADS / 16 - 1) / (ROWS_THREADS / 16);
-  const long long most = 8LL * num_sms;                       // 8 blocks of 256 threads an SM
-  return (int)(blocks < most ? blocks : most);
 }
 
 bool on_16(const void* p, long long ld, int size) {
@@ -162,82 +196,102 @@ bool on_16(const void* p, long long ld, int size) {
 
 // x [rows, K] (float or bfloat16, rows ldx apart) -> codes [rows, ldc bytes], scales [ceil(K / 128), lds].
 // codes: on a 16-byte boundary, ldc a multiple of 16.
-BF_EXPORT int bf_fp8_rows(const void* x, long long ldx, int dtype, void* codes, long long ldc,
-                          float* scales, long long lds, int rows, int K, int num_sms,
-                          cudaStream_t stream) {
+struct Fp8RowsCall {
+  const void* x;
+  long long ldx;
+  void* codes;
+  long long ldc;
+  float* scales;
+  long long lds;
+  int dtype, rows, K, num_sms;
+  cudaStream_t stream;
+};
+BF_EXPORT int bf_fp8_rows(const Fp8RowsCall* call) {
+  const auto& [x, ldx, codes, ldc, scales, lds, dtype, rows, K, num_sms, stream] = *call;
   if (rows <= 0 || K <= 0) return 0;
   if (!on_16(codes, ldc, 1)) return (int)cudaErrorInvalidValue;
   const int groups = (K + BF_FP8_GROUP - 1) / BF_FP8_GROUP;
-  const dim3 grid(blocks_for((long long)rows * groups, num_sms));
-  const int size = dtype == BF_DTYPE_F32 ? 4 : 2;
-  const bool vec = on_16(x, ldx, size);
+  const Fp8Walk walk = fp8_walk(F8_ROW_PLACES, rows, groups, num_sms, 1);
   uint8_t* c = (uint8_t*)codes;
-#define BF_GO(T, V)                                                                              \
-  return bf_launch_pdl(fp8_rows_kernel<T, V>, grid, dim3(ROWS_THREADS), 0, stream, (const T*)x, ldx, c, \
-                       ldc, scales, lds, rows, K, groups)
+  auto go = [&](auto kern, auto* src) {
+    return bf_launch_pdl(kern, walk.grid, dim3(F8_THREADS), 0, call->stream, src, call->ldx, c, call->ldc,
+                         call->scales, call->lds, call->rows, call->K, groups, walk.shift);
+  };
   if (dtype == BF_DTYPE_F32) {
-    if (vec) BF_GO(float, true);
-    BF_GO(float, false);
+    const float* f = (const float*)x;
+    return on_16(x, ldx, 4) ? go(fp8_rows_kernel<float, true>, f) : go(fp8_rows_kernel<float, false>, f);
   }
-  if (vec) BF_GO(__nv_bfloat16, true);
-  BF_GO(__nv_bfloat16, false);
-#undef BF_GO
+  const __nv_bfloat16* h = (const __nv_bfloat16*)x;
+  return on_16(x, ldx, 2) ? go(fp8_rows_kernel<__nv_bfloat16, true>, h)
+                          : go(fp8_rows_kernel<__nv_bfloat16, false>, h);
 }
 
 // `mats` matrices of mat_rows x K one behind the other in w (rows ldw apart) -> codes the same way (rows
 // ldc bytes apart), scales [mats, ceil(mat_rows / 128), ceil(K / 128)].
-BF_EXPORT int bf_fp8_blocks(const void* w, long long ldw, int dtype, void* codes, long long ldc,
-                            float* scales, int mats, int mat_rows, int K, cudaStream_t stream) {
+struct Fp8BlocksCall {
+  const void* w;
+  long long ldw;
+  void* codes;
+  long long ldc;
+  float* scales;
+  int dtype, mats, mat_rows, K;
+  cudaStream_t stream;
+};
+BF_EXPORT int bf_fp8_blocks(const Fp8BlocksCall* call) {
+  const auto& [w, ldw, codes, ldc, scales, dtype, mats, mat_rows, K, stream] = *call;
   if (mats <= 0 || mat_rows <= 0 || K <= 0) return 0;
-  if (!on_16(codes, ldc, 1)) return (int)cudaErrorInvalidValue;
   const int groups = (K + BF_FP8_GROUP - 1) / BF_FP8_GROUP;
   const int blocks = (mat_rows + BF_FP8_GROUP - 1) / BF_FP8_GROUP;
-  const long long total = (long long)mats * blocks * groups;
-  if (total > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
-  const dim3 grid((unsigned)total);
-  const int size = dtype == BF_DTYPE_F32 ? 4 : 2;
-  const bool vec = on_16(w, ldw, size);
+  if (!on_16(codes, ldc, 1) || mats > 65535 || blocks > 65535) return (int)cudaErrorInvalidValue;
   uint8_t* c = (uint8_t*)codes;
   // (launched the ordinary way, and no kernel behind it may begin before it has ended: the products
   // ask for weights ahead of their wait for the kernels before them)
-#define BF_GO(T, V)                                                                               \
-  {                                                                                               \
-    fp8_blocks_kernel<T, V><<<grid, 256, 0, stream>>>((const T*)w, ldw, c, ldc, scales, mat_rows, \
-                                                      blocks, K, groups);                         \
-    return bf_launch_status();                                                                    \
-  }
+  auto go = [&](auto kern, auto* src) {
+    kern<<<dim3(groups, blocks, call->mats), F8_THREADS, 0, call->stream>>>(
+        src, call->ldw, c, call->ldc, call->scales, call->mat_rows, call->K);
+    return bf_launch_status();
+  };
   if (dtype == BF_DTYPE_F32) {
-    if (vec) BF_GO(float, true);
-    BF_GO(float, false);
+    const float* f = (const float*)w;
+    return on_16(w, ldw, 4) ? go(fp8_blocks_kernel<float, true>, f) : go(fp8_blocks_kernel<float, false>, f);
   }
-  if (vec) BF_GO(__nv_bfloat16, true);
-  BF_GO(__nv_bfloat16, false);
-#undef BF_GO
+  const __nv_bfloat16* h = (const __nv_bfloat16*)w;
+  return on_16(w, ldw, 2) ? go(fp8_blocks_kernel<__nv_bfloat16, true>, h)
+                          : go(fp8_blocks_kernel<__nv_bfloat16, false>, h);
 }
 
-// What codes and scales stand for, into out (float or bfloat16, rows ldo apart).  block_rows 1: scales
-// [ceil(K / 128), lds]; 128: `rows` rows of matrices of mat_rows each, scales as bf_fp8_blocks leaves them.
-BF_EXPORT int bf_fp8_read(const void* codes, long long ldc, const float* scales, long long lds, void* out,
-                          long long ldo, int dtype, long long rows, int K, int block_rows, int mat_rows,
-                          int num_sms, cudaStream_t stream) {
-  if (rows <= 0 || K <= 0) return 0;
-  if (!on_16(codes, ldc, 1) || (block_rows != 1 && block_rows != BF_FP8_GROUP) || mat_rows <= 0)
-    return (int)cudaErrorInvalidValue;
+// What codes and scales stand for, into out (float or bfloat16, rows ldo apart): `mats` matrices of
+// mat_rows x K one behind the other.  blocks: scales as bf_fp8_blocks leaves them, else as bf_fp8_rows.
+struct Fp8ReadCall {
+  const void* codes;
+  long long ldc;
+  const float* scales;
+  long long lds;
+  void* out;
+  long long ldo;
+  int dtype, blocks, mats, mat_rows, K, num_sms;
+  cudaStream_t stream;
+};
+BF_EXPORT int bf_fp8_read(const Fp8ReadCall* call) {
+  const auto& [codes, ldc, scales, lds, out, ldo, dtype, blocks, mats, mat_rows, K, num_sms, stream] = *call;
+  if (mats <= 0 || mat_rows <= 0 || K <= 0) return 0;
+  if (!on_16(codes, ldc, 1) || mats > 65535 || (!blocks && mats != 1)) return (int)cudaErrorInvalidValue;
   const int groups = (K + BF_FP8_GROUP - 1) / BF_FP8_GROUP;
-  const int mat_blocks = (mat_rows + BF_FP8_GROUP - 1) / BF_FP8_GROUP;
-  const dim3 grid(blocks_for(rows * groups, num_sms));
+  const Fp8Walk walk = fp8_walk(F8_READ_PLACES, (mat_rows + 1LL) / 2, groups, num_sms, mats);
+  auto go = [&](auto kern, auto* dst) {
+    return bf_launch_pdl(kern, walk.grid, dim3(F8_THREADS), 0, call->stream, (const uint8_t*)call->codes,
+                         call->ldc, call->scales, call->lds, dst, call->ldo, call->mat_rows, call->K, groups,
+                         walk.shift, on_16(call->out, call->ldo, (int)sizeof(*dst)));
+  };
   if (dtype == BF_DTYPE_F32)
-    return bf_launch_pdl(fp8_read_kernel<float>, grid, dim3(ROWS_THREADS), 0, stream,
-                         (const uint8_t*)codes, ldc, scales, lds, (float*)out, ldo, rows, K, groups,
-                         block_rows, mat_rows, mat_blocks, on_16(out, ldo, 4));
-  return bf_launch_pdl(fp8_read_kernel<__nv_bfloat16>, grid, dim3(ROWS_THREADS), 0, stream,
-                       (const uint8_t*)codes, ldc, scales, lds, (__nv_bfloat16*)out, ldo, rows, K, groups,
-                       block_rows, mat_rows, mat_blocks, on_16(out, ldo, 2));
+    return blocks ? go(fp8_read_kernel<float, true>, (float*)out) : go(fp8_read_kernel<float, false>, (float*)out);
+  return blocks ? go(fp8_read_kernel<__nv_bfloat16, true>, (__nv_bfloat16*)out)
+                : go(fp8_read_kernel<__nv_bfloat16, false>, (__nv_bfloat16*)out);
 }
 
 extern "C" int bf_gemm_fp8_few(const void*, long long, const float*, long long, const void*, long long,
                                const float*, const int*, const float*, void*, long long, int, int, int, int,
-                               int, int, int, float, float, float, int, int, int, int*, cudaStream_t);
+                               int, int, int, float, float, float, int, int, int, int, int*, cudaStream_t);
 extern "C" int bf_gemm_fp8_pair(const void*, long long, const float*, long long, const void*, long long,
                                 const float*, const int*, const float*, void*, long long, int, int, int, int,
                                 int, int, int, float, float, float, int, int*, cudaStream_t);
@@ -245,18 +299,17 @@ extern "C" int bf_gemm_fp8_pair(const void*, long long, const float*, long long,
 // How a product runs: the most rows of a tile of gemm_fp8_few.cu, or -1 for gemm_fp8_pair.cu.
 static int fp8_tile(int rows, int experts) {
   const int each = (rows + experts - 1) / experts;
-  if (each > 256) return -1;
-  int nb = 16;
-  while (nb < each) nb *= 2;
-  return nb;
+  if (each > (experts > 1 ? 112 : 192)) return -1;
+  return each <= 16 ? 16 : each <= 32 ? 32 : 64;
 }
-// CTAs that share a tile of 128 weight rows: as many as the SMs have room for, each with two groups
+// CTAs that share a tile of 128 weight rows: as many (a power of two: clusters of other sizes leave SMs
+// of a GPC empty) as are resident together, two to an SM, each with two groups at least.
 static int fp8_split(int rows, int features, int K, bool gated, int nb, int num_sms) {
-  const int tiles = ((rows + nb - 1) / nb) * ((features + (gated ? 63 : 127)) / (gated ? 64 : 128));
+  const long long tiles = (long long)((rows + nb - 1) / nb) * ((features + (gated ? 63 : 127)) / (gated ? 64 : 128));
   const int groups = (K + BF_FP8_GROUP - 1) / BF_FP8_GROUP;
   int c = 1;
-  while (c < 8 && tiles * (c + 1) <= num_sms && groups >= 2 * (c + 1)) ++c;
-  return nb <= 64 ? c : 1;
+  while (nb <= 64 && c < 8 && tiles * 2 * c <= 2 * num_sms && groups >= 4 * c) c *= 2;
+  return c;
 }
 
 struct Fp8ProductCall {
@@ -279,22 +332,31 @@ struct Fp8ProductCall {
   int* err;
   cudaStream_t stream;
 };
-// The rows into 8 bits, and their product with a held weight (bf_gemm_fp8_few's arguments).
+// The rows into 8 bits, and their product with a held weight (bf_gemm_fp8_few's arguments).  Without scratch
+// (codes null): as one kernel, or -1 and nothing done where that does not take the sizes.
 BF_EXPORT int bf_fp8_product(const Fp8ProductCall* call) {
   const Fp8ProductCall& c = *call;
   if (c.rows <= 0 || c.features <= 0) return 0;
-  const int e = bf_fp8_rows(c.x, c.ldx, BF_DTYPE_BF16, c.codes, c.ldc, c.scales, c.lds, c.rows, c.K, c.num_sms,
-                            c.stream);
-  if (e) return e;
   const int tile = c.tile ? c.tile : fp8_tile(c.rows, c.experts);
+  const int split = c.starts || tile < 0 ? 1
+                    : c.split ? c.split
+                              : fp8_split(c.rows, c.features, c.K, c.gated != 0, tile, c.num_sms);
+  if (!c.codes) {
+    // asked for without scratch: the rows stay in the CTAs that read them, where they fit
+    if (tile < 0 || tile > 32 || c.rows > tile || c.starts) return -1;
+    return bf_gemm_fp8_few(c.x, c.ldx, nullptr, 0, c.w, c.ldw, c.sw, c.starts, c.row_w, c.out, c.ldo, c.out_dtype,
+                           c.rows, c.features, c.K, c.experts, c.gated, c.act, c.limit, c.slope, c.up_offset,
+                           tile, split, 1, c.num_sms, c.err, c.stream);
+  }
+  const Fp8RowsCall rows = {c.x, c.ldx, c.codes, c.ldc, c.scales, c.lds, BF_DTYPE_BF16, c.rows, c.K, c.num_sms,
+                            c.stream};
+  const int e = bf_fp8_rows(&rows);
+  if (e) return e;
   if (tile < 0)
     return bf_gemm_fp8_pair(c.codes, c.ldc, c.scales, c.lds, c.w, c.ldw, c.sw, c.starts, c.row_w, c.out, c.ldo,
                             c.out_dtype, c.rows, c.features, c.K, c.experts, c.gated, c.act, c.limit, c.slope,
                             c.up_offset, c.num_sms, c.err, c.stream);
-  const int split = c.starts ? 1
-                    : c.split ? c.split
-                              : fp8_split(c.rows, c.features, c.K, c.gated != 0, tile, c.num_sms);
   return bf_gemm_fp8_few(c.codes, c.ldc, c.scales, c.lds, c.w, c.ldw, c.sw, c.starts, c.row_w, c.out, c.ldo,
                          c.out_dtype, c.rows, c.features, c.K, c.experts, c.gated, c.act, c.limit, c.slope,
-                         c.up_offset, tile, split, c.num_sms, c.err, c.stream);
+                         c.up_offset, tile, split, 0, c.num_sms, c.err, c.stream);
 }

@@ -17,36 +17,49 @@
 #define BF_FP8_GROUP 128
 #define BF_FP8_MAX 448.f
 
-// the scale of a group whose largest size has these bits
-__device__ __forceinline__ float fp8_scale(uint32_t largest_bits) {
-  if (largest_bits >= 0x7f800000u) return __uint_as_float(0x7fffffffu);
-  return fmaxf(__fdiv_rn(__uint_as_float(largest_bits), BF_FP8_MAX), 0x1p-100f);
-}
-// A float that rounds to the code of x / s.  q = x * (1 / s) is off by less than 8 of its last places,
-// so it stands unless it is that near to the middle of two codes (one number in 2^15, and those below
-// 2^-6, whose codes lie 2^-9 apart).  Else q is the rounded quotient: where it lies on a middle and the
-// quotient itself does not, the sign of x - q s, which a fused multiply-add gives exactly (q has five
-// bits), says on which side; one last place to that side decides the rounding.
-__device__ __forceinline__ float fp8_quotient(float x, float s, float inv) {
-  float q = x * inv;
-  const uint32_t off = (__float_as_uint(q) + 8u) & 0xfffffu;
-  if ((off >= 0x80000u && off <= 0x80010u) || (fabsf(q) < 0x1p-6f && q != 0.f)) {
-    q = __fdiv_rn(x, s);
-    const float r = fmaf(-q, s, x);
-    const bool middle = fabsf(q) < 0x1p-6f ? q * 1024.f == rintf(q * 1024.f)
-                                           : (__float_as_uint(q) & 0xfffffu) == 0x80000u;
-    if (middle && q != 0.f && r != 0.f)
-      q = __uint_as_float(__float_as_uint(q) + ((r > 0.f) == (q > 0.f) ? 1u : 0xffffffffu));
-  }
-  return q;
+// A group's scale, and its reciprocal from below and above.
+struct Fp8Scale {
+  float s, low, high;
+};
+// ... of a group whose largest size has these bits.  The quotient by 448 is the rounded product with
+// 1 / 448 put right by its remainder, which is exact (it equals the division for every significand).
+__device__ __forceinline__ Fp8Scale fp8_scale(uint32_t largest_bits) {
+  Fp8Scale r;
+  const float a = __uint_as_float(largest_bits), q = a * (1.f / BF_FP8_MAX);
+  r.s = fmaxf(fmaf(fmaf(-q, BF_FP8_MAX, a), 1.f / BF_FP8_MAX, q), 0x1p-100f);
+  if (largest_bits >= 0x7f800000u) r.s = __uint_as_float(0x7fffffffu);
+  float inv;                                       // (off by one place at most)
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(r.s));
+  r.low = inv * (1.f - 0x1p-21f);
+  r.high = inv * (1.f + 0x1p-21f);
+  return r;
 }
 // the codes of two quotients, the first in the lower byte
 __device__ __forceinline__ uint32_t fp8_codes2(float a, float b) {
   return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
-__device__ __forceinline__ uint32_t fp8_codes4(const float* x, float s, float inv) {
-  return fp8_codes2(fp8_quotient(x[0], s, inv), fp8_quotient(x[1], s, inv)) |
-         fp8_codes2(fp8_quotient(x[2], s, inv), fp8_quotient(x[3], s, inv)) << 16;
+// A float that rounds to the code of x / s: the rounded quotient q; where q lies on the middle of two
+// codes and x / s does not, the sign of x - q s, which a fused multiply-add gives exactly (q has five
+// bits), says on which side, and one last place to that side decides the rounding.
+__device__ __forceinline__ float fp8_quotient(float x, float s) {
+  float q = __fdiv_rn(x, s);
+  const float r = fmaf(-q, s, x);
+  const bool middle = fabsf(q) < 0x1p-6f ? q * 1024.f == rintf(q * 1024.f)
+                                         : (__float_as_uint(q) & 0xfffffu) == 0x80000u;
+  if (middle && q != 0.f && r != 0.f)
+    q = __uint_as_float(__float_as_uint(q) + ((r > 0.f) == (q > 0.f) ? 1u : 0xffffffffu));
+  return q;
+}
+// The codes of four numbers.  x / s lies between x * low and x * high (2^-21 to either side covers the
+// three roundings between): where both round to the same code it is that, else (four numbers in 2^14)
+// the quotients are taken.
+__device__ __forceinline__ uint32_t fp8_codes4(const float* x, const Fp8Scale& k) {
+  const uint32_t c = fp8_codes2(x[0] * k.low, x[1] * k.low) | fp8_codes2(x[2] * k.low, x[3] * k.low) << 16;
+  const uint32_t d = fp8_codes2(x[0] * k.high, x[1] * k.high) | fp8_codes2(x[2] * k.high, x[3] * k.high) << 16;
+  if (c == d) return c;
+  return fp8_codes2(fp8_quotient(x[0], k.s), fp8_quotient(x[1], k.s)) |
+        fp8_codes2(fp8_quotient(x[2], k.s), fp8_quotient(x[3], k.s)) << 16;
+  return c;
 }
 // the values of four codes
 __device__ __forceinline__ void fp8_values4(uint32_t codes, float* v) {
@@ -58,41 +71,63 @@ __device__ __forceinline__ void fp8_values4(uint32_t codes, float* v) {
     v[2 * i + 1] = f.y;
   }
 }
-// Eight neighbouring numbers of a row, of which `n` are there (the others read as zero); VEC: the
-// address is on a 16-byte boundary and all eight are there.
-template <bool VEC>
-__device__ __forceinline__ void fp8_load8(const __nv_bfloat16* p, int n, float* v) {
-  if (VEC) {
-    const uint4 raw = *reinterpret_cast<const uint4*>(p);
-    const uint32_t* w = &raw.x;
+// Sixteen neighbouring numbers of a row (as many as 32-bit words hold of them are a register), of which
+// `n` are there (the others read as zero); WHOLE: all sixteen, on a 16-byte boundary.
+template <typename T>
+struct Fp8Sixteen {
+  static constexpr int WORDS = (int)sizeof(T) * 4;
+  uint32_t w[WORDS];
+
+  template <bool WHOLE>
+  __device__ __forceinline__ void load(const T* p, int n) {
+    if (WHOLE) {
+#pragma unroll
+      for (int i = 0; i < WORDS / 4; ++i) {
+        const uint4 q = reinterpret_cast<const uint4*>(p)[i];
+        w[4 * i] = q.x;
+        w[4 * i + 1] = q.y;
+        w[4 * i + 2] = q.z;
+        w[4 * i + 3] = q.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) {
+        if constexpr (sizeof(T) == 4) {
+          w[i] = i < n ? __float_as_uint(p[i]) : 0u;
+        } else {
+          const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+          w[i] = (2 * i < n ? (uint32_t)h[2 * i] : 0u) | (2 * i + 1 < n ? (uint32_t)h[2 * i + 1] << 16 : 0u);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ float value(int i) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+    else return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+  }
+  // the largest size, as the bits of a float (those of a NaN are above an infinity's)
+  __device__ __forceinline__ uint32_t largest() const {
+    uint32_t m = 0u;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) m = max(m, w[i] & 0x7fffffffu);
+      return m;
+    } else {
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) asm("max.u16x2 %0, %0, %1;" : "+r"(m) : "r"(w[i] & 0x7fff7fffu));
+      return max(m << 16, m & 0xffff0000u);
+    }
+  }
+  __device__ __forceinline__ uint4 codes(const Fp8Scale& s) const {
+    uint32_t c[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(w[i] << 16);
-      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      const float x[4] = {value(4 * i), value(4 * i + 1), value(4 * i + 2), value(4 * i + 3)};
+      c[i] = fp8_codes4(x, s);
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? __bfloat162float(p[i]) : 0.f;
+    return make_uint4(c[0], c[1], c[2], c[3]);
   }
-}
-template <bool VEC>
-__device__ __forceinline__ void fp8_load8(const float* p, int n, float* v) {
-  if (VEC) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.f;
-  }
-}
-// the largest size of eight numbers, as bits (those of a NaN are above an infinity's)
-__device__ __forceinline__ uint32_t fp8_largest8(const float* v) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-  return m;
-}
+};
 // The factor of a group's sums: the product of two scales, held at the largest float, so that a sum of
 // zero stays zero where the product alone is out of range.  (NaN stays NaN.)
 __device__ __forceinline__ float fp8_factor(float sx, float sw) {

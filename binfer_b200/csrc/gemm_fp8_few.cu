@@ -11,14 +11,16 @@
 //   warp 0       TMA: 128 weight rows and NB activation rows x 128 bytes per stage
 //   warp 1       the products; TMEM allocation
 //   warp 2       the factors sx sw of every column of a group, into shared memory
-//   warps 4-11   the sums, times the factors, into registers; the result (wide tiles: these two
-//                warpgroups take 216 registers a thread, which the first leaves them: 128 x 72 +
-//                256 x 216 = 384 x 168)
+//   warps 4-11   the sums, times the factors, into registers; the result
 //
 // What bounds it with few rows is the weights' bytes; a tile is 128 rows of the weight, so that a
 // narrow weight alone does not give every SM work: then a cluster of `split` CTAs shares a tile, each a
 // part of the groups, and the parts meet in shared memory, added in the order of the ranks.
 // With experts the tiles are dealt out to persistent CTAs.
+//
+// RESIDENT: few rows come as bfloat16, and every CTA puts its columns of them into 8 bits by itself
+// (warps 4-11, before the first sums, while the first weights are on their way), where they stay: no
+// kernel in front, nothing of them through global memory.
 //
 // Every wait is bounded; no load uses multicast.
 #include "common.cuh"
@@ -27,17 +29,22 @@
 
 namespace {
 
-constexpr int FEW_THREADS = 384;            // three warpgroups of 168 registers a thread at launch
+constexpr int FEW_THREADS = 384;
 constexpr int FEW_MAX_STAGES = 12;
 constexpr int FEW_BARS = 1024;
+constexpr int FEW_READY = 512;                // offset among the barriers of RESIDENT's, one per round
+constexpr int FEW_ROUNDS = (FEW_BARS - FEW_READY) / 8;
 constexpr int FEW_W_BYTES = 128 * FK;
-constexpr size_t FEW_SMEM = 226 * 1024;
+// Two CTAs share an SM: its registers, its shared memory and its tensor memory are dealt out by halves.  A
+// step of eight rows against 24,576 x 4,096 gated took 27.5 us with one, whose 192 tiles ran in two turns.
+constexpr int FEW_PER_SM = 2;
+constexpr size_t FEW_SMEM = 112 * 1024;
+constexpr int FEW_DOES_NOT_FIT = -1;
 
 template <int NB>
 struct FewShape {
-  static constexpr int SLOTS = 512 / NB < 16 ? 512 / NB : 16;      // groups in tensor memory
+  static constexpr int SLOTS = 256 / NB < 16 ? 256 / NB : 16;      // groups in tensor memory
   static constexpr int CH = NB == 16 ? 8 : 16;                     // columns a warp reads at once
-  static constexpr int STAGE = FEW_W_BYTES + NB * FK;
   // the up rows' sums on their way to the gate rows' warps: two buffers for each half of the warps
   static constexpr int EXCHANGE = 2 * 2 * CH * 64 * 4;
 };
@@ -51,6 +58,11 @@ struct FewParams {
   const float* sw;                     // [experts * (gated ? 2 : 1) * w_blocks, groups]
   const float* row_w;                  // per row, or null
   int split, stages, table_bytes;
+  // RESIDENT: the rows, room for res_rows of them (8: the product's second eight columns read the first
+  // eight again), res_groups groups of each
+  const __nv_bfloat16* x;
+  long long ldx;
+  int x_vec, res_rows, res_groups;
   long long ldo;
   int act;
   BfGateConst gk;
@@ -68,12 +80,12 @@ __device__ __forceinline__ uint32_t few_map(uint32_t local_addr, uint32_t rank) 
   return r;
 }
 
-template <int NB, typename OutT, bool GATED>
-__global__ void __launch_bounds__(FEW_THREADS, 1)
+template <int NB, typename OutT, bool GATED, bool RESIDENT>
+__global__ void __launch_bounds__(FEW_THREADS, FEW_PER_SM)
 fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                OutT* __restrict__ out, const FewParams p) {
   constexpr int SLOTS = FewShape<NB>::SLOTS, CH = FewShape<NB>::CH, CHUNKS = NB / CH / 2;
-  constexpr int STAGE = FewShape<NB>::STAGE;
+  constexpr int STAGE = FEW_W_BYTES + (RESIDENT ? 0 : NB * FK);
   constexpr int HALVES = GATED ? 2 : 1;
   constexpr int TMEM_COLS = SLOTS * NB;
   extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -92,7 +104,10 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
                         (p.split > 1 ? ((NB + p.split - 1) / p.split) * p.split * 128 * 4
                                      : GATED ? FewShape<NB>::EXCHANGE : 0);
   const RowTables tables = row_tables_at(table_smem, p.experts);
-  uint8_t* tiles = base + (((table_smem - base) + p.table_bytes + 1023) & ~1023);
+  uint64_t* ready = reinterpret_cast<uint64_t*>(base + FEW_READY);
+  float* res_sx = reinterpret_cast<float*>(table_smem + p.table_bytes);        // [res_groups][NB]
+  uint8_t* res = base + (((table_smem - base) + p.table_bytes + (RESIDENT ? p.res_groups * NB * 4 : 0) + 1023) & ~1023);
+  uint8_t* tiles = res + (RESIDENT ? (p.res_groups * p.res_rows * FK + 1023) & ~1023 : 0);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = p.split > 1 ? (int)few_rank() : 0;
@@ -101,6 +116,10 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   const int g1 = (int)((long long)p.groups * (rank + 1) / p.split);
   const int STAGES = p.stages;
   const int w_rows = HALVES * p.features;                // of an expert
+  // RESIDENT: 32 places of eight lanes, a row and group each: so many groups at once
+  int row_shift = 0;
+  while (RESIDENT && (1 << row_shift) < p.rows) ++row_shift;
+  const int per_round = 32 >> row_shift;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -111,6 +130,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
       mbar_init(acc_full + a, 2);              // the products' commit, the factors' warp
       mbar_init(acc_empty + a, 8);             // a warp of the epilogue each
     }
+    for (int r = 0; RESIDENT && r * per_round < g1 - g0; ++r) mbar_init(ready + r, 8);
     mbar_init(drain, 1);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -154,8 +174,6 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
 
   int stage = 0;                                 // of this role, with its phase
   uint32_t phase = 0;
-  if (warp < 4) {
-  if (NB >= 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
   if (warp == 0) {
     // --------------------------------------------------------------- copies
     if (lane == 0) {
@@ -172,7 +190,8 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
             mbar_expect_tx(full + stage, STAGE);
             load_w(stage, g, t.expert, t.ft);
           }
-          tma_load_2d(tiles + (size_t)stage * STAGE + FEW_W_BYTES, &map_x, full + stage, g * FK, t.row0);
+          if (!RESIDENT)
+            tma_load_2d(tiles + (size_t)stage * STAGE + FEW_W_BYTES, &map_x, full + stage, g * FK, t.row0);
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1;
@@ -182,29 +201,29 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------- products
+    const uint32_t elected = elect_one();
     int slot = 0;
     uint32_t slot_phase = 0;
-    bool ok = true;
+    bool ok = true, seen_empty = false, seen_full = false;       // looks at the next group's barriers
     for (int u = cluster; u < units && ok; u += clusters) {
       const RowTile t = row_tile(tables, p.experts, p.tiles_f, NB, u);
       const int n = min(NB, (t.row_end - t.row0 + 15) & ~15);
       const uint32_t idesc = fp8_idesc(128, n);
       for (int g = g0; g < g1; ++g) {
-        if (!mbar_wait_warp(acc_empty + slot, slot_phase ^ 1, abort) ||
-            !mbar_wait_warp(full + stage, phase, abort)) {
+        if (!mbar_seen_or_wait_warp(seen_empty, acc_empty + slot, slot_phase ^ 1, abort) ||
+            !mbar_seen_or_wait_warp(seen_full, full + stage, phase, abort) ||
+            (RESIDENT && !mbar_wait_warp(ready + (g - g0) / per_round, 0, abort))) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint32_t a_addr = smem_u32(tiles + (size_t)stage * STAGE);
+        const uint32_t a_addr = smem_u32(tiles + (size_t)stage * STAGE), d_tmem = tmem_base + (uint32_t)(slot * NB);
         const uint64_t a_desc = umma_desc_k_sw128(a_addr);
-        const uint64_t b_desc = umma_desc_k_sw128(a_addr + FEW_W_BYTES);
-#pragma unroll
-        for (int k = 0; k < FK / 32; ++k)
-          umma_fp8(tmem_base + (uint32_t)(slot * NB), a_desc + (uint64_t)(2 * k), b_desc + (uint64_t)(2 * k),
-                   idesc, k > 0 ? 1u : 0u);
-        umma_commit(empty + stage);
-        umma_commit(acc_full + slot);
+        const uint64_t b_desc =
+            RESIDENT ? umma_desc_k_sw128_sbo(smem_u32(res + (g - g0) * p.res_rows * FK), p.res_rows == 8 ? 0u : 1024u)
+                     : umma_desc_k_sw128(a_addr + FEW_W_BYTES);
+        uint64_t* const done_stage = empty + stage;
+        uint64_t* const done_slot = acc_full + slot;
         if (++stage == STAGES) {
           stage = 0;
           phase ^= 1;
@@ -213,30 +232,64 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
           slot = 0;
           slot_phase ^= 1;
         }
+        seen_empty = mbar_look(acc_empty + slot, slot_phase ^ 1);
+        seen_full = mbar_look(full + stage, phase);
+#pragma unroll
+        for (int k = 0; k < FK / 32; ++k)
+          umma_fp8(d_tmem, a_desc + (uint64_t)(2 * k), b_desc + (uint64_t)(2 * k), idesc, k > 0 ? 1u : 0u, elected);
+        umma_commit_by(done_stage, elected);
+        umma_commit_by(done_slot, elected);
       }
     }
   } else if (warp == 2) {
     // -------------------------------------------------------------- factors
+    // The scales of AHEAD groups are asked for while the factors of the AHEAD before them are written:
+    // a load takes longer than a group's products.
     constexpr int PER = (NB + 31) / 32;          // columns a lane looks after
-    constexpr int AHEAD = PER == 1 ? 8 : PER == 2 ? 4 : 2;      // groups whose scales are asked for together
+    constexpr int AHEAD = NB <= 32 ? 8 : 4;
     int slot = 0;
     uint32_t slot_phase = 0;
     bool ok = true;
-    for (int u = cluster; u < units && ok; u += clusters) {
-      const RowTile t = row_tile(tables, p.experts, p.tiles_f, NB, u);
+    float sx[AHEAD][PER], sw[AHEAD][HALVES];
+    auto ask = [&](const RowTile& t, int ga) {
       const long long block = (long long)t.expert * HALVES * p.w_blocks + (GATED ? t.ft >> 1 : t.ft);
-      for (int ga = g0; ga < g1 && ok; ga += AHEAD) {
-        float sx[AHEAD][PER], sw[AHEAD][HALVES];
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-          const int g = min(ga + i, g1 - 1);
+      for (int i = 0; i < AHEAD; ++i) {
+        const int g = min(ga + i, g1 - 1);
 #pragma unroll
-          for (int j = 0; j < PER; ++j) {
-            const int row = t.row0 + j * 32 + lane;
+        for (int j = 0; j < PER; ++j) {
+          const int row = t.row0 + j * 32 + lane;
+          if (RESIDENT) {
+            if (i == 0 && j == 0) ok = mbar_wait_warp(ready + (min(ga + AHEAD, g1) - 1 - g0) / per_round, 0, abort);
+            sx[i][j] = row < t.row_end ? res_sx[(g - g0) * NB + row] : 0.f;
+          } else {
             sx[i][j] = row < t.row_end && j * 32 + lane < NB ? p.sx[(long long)g * p.lds + row] : 0.f;
           }
+        }
 #pragma unroll
-          for (int h = 0; h < HALVES; ++h) sw[i][h] = p.sw[(block + h * p.w_blocks) * p.groups + g];
+        for (int h = 0; h < HALVES; ++h) sw[i][h] = p.sw[(block + h * p.w_blocks) * p.groups + g];
+      }
+    };
+    int u = cluster;
+    RowTile t;
+    if (u < units) {
+      t = row_tile(tables, p.experts, p.tiles_f, NB, u);
+      ask(t, g0);
+    }
+    for (; u < units && ok; u += clusters) {
+      for (int ga = g0; ga < g1 && ok; ga += AHEAD) {
+        float f[AHEAD][PER * HALVES];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+          for (int j = 0; j < PER; ++j)
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h) f[i][j * HALVES + h] = fp8_factor(sx[i][j], sw[i][h]);
+        if (ga + AHEAD < g1) {
+          ask(t, ga + AHEAD);
+        } else if (u + clusters < units) {
+          t = row_tile(tables, p.experts, p.tiles_f, NB, u + clusters);
+          ask(t, g0);
         }
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
@@ -245,12 +298,12 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
             ok = false;
             break;
           }
-          float* f = factors + slot * HALVES * NB;
+          float* dst = factors + slot * HALVES * NB;
 #pragma unroll
           for (int j = 0; j < PER; ++j)
 #pragma unroll
             for (int h = 0; h < HALVES; ++h)
-              if (j * 32 + lane < NB) f[h * NB + j * 32 + lane] = fp8_factor(sx[i][j], sw[i][h]);
+              if (j * 32 + lane < NB) dst[h * NB + j * 32 + lane] = f[i][j * HALVES + h];
           __syncwarp();
           if (lane == 0) mbar_arrive(acc_full + slot);
           if (++slot == SLOTS) {
@@ -260,14 +313,45 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
         }
       }
     }
-  }
-  } else {
-    if (NB >= 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+  } else if (warp >= 4) {
     // ----------------------------------------------------------------- sums
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     const int lane_row = quarter * 32 + lane;            // of the tile's 128 weight rows
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const int which = GATED ? quarter >> 1 : 0;
+    if constexpr (RESIDENT) {
+      const int place = (warp - 4) * 4 + (lane >> 3), sub = lane & 7;
+      const int row = place & ((1 << row_shift) - 1);
+      const int rounds = (g1 - g0 + per_round - 1) / per_round;
+      const __nv_bfloat16* src = p.x + row * p.ldx + sub * 16;
+      auto ask = [&](int r, Fp8Sixteen<__nv_bfloat16>& v) {
+        const int k = (g0 + r * per_round + (place >> row_shift)) * FK;
+        const int left = row < p.rows && k < g1 * FK ? p.K - k - sub * 16 : 0;
+        if (p.x_vec && left >= 16) {
+          v.template load<true>(src + k, 16);
+        } else {
+          v.template load<false>(src + k, left);
+        }
+      };
+      Fp8Sixteen<__nv_bfloat16> v, next;
+      ask(0, v);
+      for (int r = 0; r < rounds; ++r) {
+        if (r + 1 < rounds) ask(r + 1, next);
+        const int gl = r * per_round + (place >> row_shift);
+        uint32_t m = v.largest();
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const Fp8Scale sc = fp8_scale(m);
+        if (row < p.rows && gl < g1 - g0) {
+          *reinterpret_cast<uint4*>(res + (gl * p.res_rows + row) * FK + ((sub ^ (row & 7)) << 4)) = v.codes(sc);
+          if (sub == 0) res_sx[gl * NB + row] = sc.s;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ready + r);
+        v = next;
+      }
+    }
     int slot = 0;
     uint32_t slot_phase = 0;
     for (int u = cluster; u < units; u += clusters) {
@@ -286,13 +370,17 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
         }
         tc_fence_after();
         const float* f = factors + (slot * HALVES + which) * NB;
+        // (the two halves of the warps take the chunks in turn; a warp's are all asked for before the first
+        // is waited for: one after the other, a group of 128 columns took 1,030 cycles)
+        const uint32_t at = tmem_base + lanes + (uint32_t)(slot * NB + half * CH);
 #pragma unroll
         for (int i = 0; i < CHUNKS; ++i) {
-          const int c = (2 * i + half) * CH;             // (the two halves take the chunks in turn)
+          const int c = (2 * i + half) * CH;
           if (c < n) {
             uint32_t r[CH];
-            if constexpr (CH == 8) tmem_ld8(tmem_base + lanes + (uint32_t)(slot * NB + c), r);
-            else tmem_ld16(tmem_base + lanes + (uint32_t)(slot * NB + c), r);
+            tmem_ask(at + (uint32_t)(2 * i * CH), r);
+            tmem_got();
+            tmem_have(r);
 #pragma unroll
             for (int j = 0; j < CH; j += 4) {
               const float4 v = *reinterpret_cast<const float4*>(f + c + j);
@@ -423,10 +511,25 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   }
 }
 
-template <int NB, typename OutT, bool GATED>
+// Shared memory in front of the ring, and the ring's stages (fewer than 2: the sizes do not fit).
+template <int NB, bool GATED, bool RESIDENT>
+size_t few_memory(const FewParams& p, int* stages) {
+  const size_t extra = p.split > 1 ? (size_t)((NB + p.split - 1) / p.split) * p.split * 128 * 4
+                                   : GATED ? FewShape<NB>::EXCHANGE : 0;
+  size_t fixed = FEW_BARS + (size_t)FewShape<NB>::SLOTS * (GATED ? 2 : 1) * NB * 4 + extra + p.table_bytes;
+  if (RESIDENT) fixed += (size_t)p.res_groups * NB * 4;
+  fixed = 1024 + ((fixed + 1023) & ~(size_t)1023);
+  if (RESIDENT) fixed += ((size_t)p.res_groups * p.res_rows * FK + 1023) & ~(size_t)1023;
+  const size_t stage = FEW_W_BYTES + (RESIDENT ? 0 : NB * FK);
+  const size_t n = fixed < FEW_SMEM ? (FEW_SMEM - fixed) / stage : 0;
+  *stages = n > FEW_MAX_STAGES ? FEW_MAX_STAGES : (int)n;
+  return fixed + *stages * stage;
+}
+
+template <int NB, typename OutT, bool GATED, bool RESIDENT>
 int few_launch(const void* x, long long ldx, const void* w, long long ldw, OutT* out, FewParams p, int num_sms,
                cudaStream_t stream) {
-  auto kern = fp8_few_kernel<NB, OutT, GATED>;
+  auto kern = fp8_few_kernel<NB, OutT, GATED, RESIDENT>;
   static bool configured_on[BF_MAX_DEVICES];
   bool& configured = configured_on[bf_current_device()];
   if (!configured) {
@@ -440,29 +543,35 @@ int few_launch(const void* x, long long ldx, const void* w, long long ldw, OutT*
   p.w_blocks = (p.features + 127) / 128;
   p.groups = (p.K + FK - 1) / FK;
   p.table_bytes = row_tables_bytes(p.experts);
-  const long long tiles_r = (p.rows + NB - 1) / NB;
+  const long long tiles_r = (p.rows + NB - 1) / NB, room = (long long)FEW_PER_SM * num_sms;
   // (at most: `starts` may hold anything)
   const long long units = tiles_r * p.experts * p.tiles_f;
   if (units > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
-  if (p.starts || NB > 64 || units * p.split > num_sms || p.split > p.groups) p.split = 1;
-  const size_t extra = p.split > 1 ? (size_t)((NB + p.split - 1) / p.split) * p.split * 128 * 4
-                                   : GATED ? FewShape<NB>::EXCHANGE : 0;
-  size_t fixed = FEW_BARS + (size_t)FewShape<NB>::SLOTS * HALVES * NB * 4 + extra + p.table_bytes;
-  fixed = 1024 + ((fixed + 1023) & ~(size_t)1023);
-  const size_t stage = FEW_W_BYTES + NB * FK;
-  p.stages = (int)((FEW_SMEM - fixed) / stage);
-  if (p.stages > FEW_MAX_STAGES) p.stages = FEW_MAX_STAGES;
+  if (p.starts || units * p.split > room || p.split > p.groups) p.split = 1;
+  if (RESIDENT) {
+    p.x = (const __nv_bfloat16*)x;
+    p.ldx = ldx;
+    p.x_vec = ldx % 8 == 0 && ((uintptr_t)x & 15) == 0;
+    p.res_rows = p.rows <= 8 ? 8 : (p.rows + 15) & ~15;
+    p.res_groups = (p.groups + p.split - 1) / p.split;
+    int per_round = 32;
+    while (32 / per_round < p.rows) per_round /= 2;
+    if (p.starts || p.rows > NB || (p.res_groups + per_round - 1) / per_round > FEW_ROUNDS) return FEW_DOES_NOT_FIT;
+  }
+  const size_t smem = few_memory<NB, GATED, RESIDENT>(p, &p.stages);
+  if (RESIDENT && p.stages < 4) return FEW_DOES_NOT_FIT;
   if (p.stages < 2) return (int)cudaErrorInvalidValue;
   CUtensorMap mx, mw;
   int e;
-  if ((e = fp8_map(&mx, x, p.rows, p.K, ldx, NB)) ||
-      (e = fp8_map(&mw, w, (long long)p.experts * HALVES * p.features, p.K, ldw, GATED ? 64 : 128)))
+  if ((e = fp8_map(&mw, w, (long long)p.experts * HALVES * p.features, p.K, ldw, GATED ? 64 : 128)) ||
+      (!RESIDENT && (e = fp8_map(&mx, x, p.rows, p.K, ldx, NB))))
     return e;
+  if (RESIDENT) mx = mw;                           // (not used)
   const long long work = units * p.split;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.split > 1 || work < num_sms ? work : num_sms));
+  cfg.gridDim = dim3((unsigned)(p.split > 1 || work < room ? work : room));
   cfg.blockDim = dim3(FEW_THREADS);
-  cfg.dynamicSmemBytes = fixed + p.stages * stage;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -479,34 +588,39 @@ int few_launch(const void* x, long long ldx, const void* w, long long ldw, OutT*
 }
 
 template <typename OutT, bool GATED>
-int few_by_width(int nb, const void* x, long long ldx, const void* w, long long ldw, OutT* out,
+int few_by_width(int nb, bool resident, const void* x, long long ldx, const void* w, long long ldw, OutT* out,
                  const FewParams& p, int num_sms, cudaStream_t stream) {
+  if (resident) {
+    if (nb == 16) return few_launch<16, OutT, GATED, true>(x, ldx, w, ldw, out, p, num_sms, stream);
+    if (nb == 32) return few_launch<32, OutT, GATED, true>(x, ldx, w, ldw, out, p, num_sms, stream);
+    return FEW_DOES_NOT_FIT;
+  }
   switch (nb) {
-    case 16: return few_launch<16, OutT, GATED>(x, ldx, w, ldw, out, p, num_sms, stream);
-    case 32: return few_launch<32, OutT, GATED>(x, ldx, w, ldw, out, p, num_sms, stream);
-    case 64: return few_launch<64, OutT, GATED>(x, ldx, w, ldw, out, p, num_sms, stream);
-    case 128: return few_launch<128, OutT, GATED>(x, ldx, w, ldw, out, p, num_sms, stream);
-    case 256: return few_launch<256, OutT, GATED>(x, ldx, w, ldw, out, p, num_sms, stream);
+    case 16: return few_launch<16, OutT, GATED, false>(x, ldx, w, ldw, out, p, num_sms, stream);
+    case 32: return few_launch<32, OutT, GATED, false>(x, ldx, w, ldw, out, p, num_sms, stream);
+    case 64: return few_launch<64, OutT, GATED, false>(x, ldx, w, ldw, out, p, num_sms, stream);
     default: return (int)cudaErrorInvalidValue;
   }
 }
 
 }  // namespace
 
-// x codes [rows, K] (rows ldx bytes apart) with scales sx [ceil(K / 128), lds]; w codes [experts,
+// x codes [rows, K] (rows ldx bytes apart) with scales sx [ceil(K / 128), lds], or with `resident` bfloat16
+// (rows ldx numbers apart; -1 is returned, and nothing done, where the rows do not fit); w codes [experts,
 // (gated ? 2 : 1) * features, K] (rows ldw bytes apart) with scales sw [experts, (gated ? 2 : 1) *
 // ceil(features / 128), ceil(K / 128)]; starts int [experts + 1] of the experts' first rows, or null for
 // one weight; row_w float [rows] or null; out [rows, features], rows ldo apart.  nb: most rows of a tile
-// (16 to 256, a power of two).  split: CTAs that share a tile (without experts, tiles * split at most
+// (16, 32 or 64).  split: CTAs that share a tile (without experts, tiles * split at most
 // num_sms; else 1 is taken).
 BF_EXPORT int bf_gemm_fp8_few(const void* x, long long ldx, const float* sx, long long lds, const void* w,
                               long long ldw, const float* sw, const int* starts, const float* row_w,
                               void* out, long long ldo, int out_dtype, int rows, int features, int K,
                               int experts, int gated, int act, float limit, float slope, float up_offset,
-                              int nb, int split, int num_sms, int* err, cudaStream_t stream) {
+                              int nb, int split, int resident, int num_sms, int* err,
+                              cudaStream_t stream) {
   if (rows <= 0 || features <= 0) return 0;
-  if (K <= 0 || experts < 1 || experts > FP8_MAX_EXPERTS || (!starts && experts != 1) || ldx % 16 || ldw % 16 ||
-      (((uintptr_t)x | (uintptr_t)w) & 15) || split < 1 || split > 8 || num_sms < 1 ||
+  if (K <= 0 || experts < 1 || experts > FP8_MAX_EXPERTS || (!starts && experts != 1) || ldw % 16 ||
+      ((uintptr_t)w & 15) || (!resident && (ldx % 16 || ((uintptr_t)x & 15))) || split < 1 || split > 8 || num_sms < 1 ||
       (act != BF_ACT_SILU && act != BF_ACT_CLAMPED) || (gated && out_dtype != BF_DTYPE_BF16))
     return (int)cudaErrorInvalidValue;
   FewParams p = {};
@@ -525,8 +639,8 @@ BF_EXPORT int bf_gemm_fp8_few(const void* x, long long ldx, const float* sx, lon
   p.gk = BfGateConst{limit, slope, up_offset};
   p.err = err;
   if (gated)
-    return few_by_width<__nv_bfloat16, true>(nb, x, ldx, w, ldw, (__nv_bfloat16*)out, p, num_sms, stream);
+    return few_by_width<__nv_bfloat16, true>(nb, resident, x, ldx, w, ldw, (__nv_bfloat16*)out, p, num_sms, stream);
   if (out_dtype == BF_DTYPE_F32)
-    return few_by_width<float, false>(nb, x, ldx, w, ldw, (float*)out, p, num_sms, stream);
-  return few_by_width<__nv_bfloat16, false>(nb, x, ldx, w, ldw, (__nv_bfloat16*)out, p, num_sms, stream);
+    return few_by_width<float, false>(nb, resident, x, ldx, w, ldw, (float*)out, p, num_sms, stream);
+  return few_by_width<__nv_bfloat16, false>(nb, resident, x, ldx, w, ldw, (__nv_bfloat16*)out, p, num_sms, stream);
 }

@@ -11,8 +11,8 @@
 //   warp 0       TMA: 128 activation rows and 128 weight rows x 128 bytes per stage
 //   warp 1       (leader) the products; TMEM allocation
 //   warps 4-11   the sums into registers; the result, turned in shared memory so that a warp writes
-//                whole 128-byte lines (these two warpgroups take 224 registers a thread, which the
-//                first leaves them: 128 x 56 + 256 x 224 = 384 x 168)
+//                whole 128-byte lines (these two warpgroups take 232 registers a thread, which the
+//                first leaves them: 128 x 40 + 256 x 232 = 384 x 168)
 //
 // Gated: a CTA's half of the weight rows are 64 gate rows and the 64 up rows of the same outputs, so a
 // thread holds both.  With experts a tile's rows are one expert's.
@@ -25,13 +25,14 @@
 
 namespace {
 
-constexpr int PF_THREADS = 384;             // three warpgroups of 168 registers a thread at launch
+constexpr int PF_THREADS = 640;             // five warpgroups of 96 registers a thread at launch
+constexpr int PF_SUMS = 16;                 // warps that add up the sums
 constexpr int PF_TILE = 256;
 constexpr int PF_HALF = 128 * FK;             // a CTA's rows of either operand
 constexpr int PF_STAGE = 2 * PF_HALF;
 constexpr int PF_STAGES = 5;
 constexpr int PF_BARS = 512;
-constexpr int PF_TURN = 32 * 128;             // a warp's rows on their way out: 32 x 128 bytes
+constexpr int PF_TURN = 32 * 64;              // a warp's rows on their way out: 32 x 64 bytes
 
 struct PairParams {
   int rows, features, K, groups;
@@ -48,31 +49,49 @@ struct PairParams {
 };
 
 __device__ __forceinline__ void pair_umma_fp8(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc,
-                                              uint32_t idesc, uint32_t accumulate) {
+                                              uint32_t idesc, uint32_t accumulate, uint32_t elected) {
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "elect.sync _|q, 0xffffffff;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
       "@q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(elected)
+      : "memory");
+}
+__device__ __forceinline__ void pair_commit_by(uint64_t* bar, uint32_t elected) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %2, 0;\n\t"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+      "[%0], %1;\n\t}" ::"r"(smem_u32(bar)),
+      "h"((uint16_t)3), "r"(elected)
       : "memory");
 }
 
-// 32 rows of a warp, 128 bytes each (a lane has a row, `v` its sixteen-byte pieces), to out: row r of the
+// An arrival on a barrier of the cluster that orders no memory: what it tells of are reads of tensor
+// memory, which tcgen05.wait::ld and tcgen05.fence have ended.  (With the default, a release at the
+// cluster's scope, the warps stood at a memory barrier for most of a group's time: 2,048 x 4,096 against
+// 8,192 rows gated took 196 us.)
+__device__ __forceinline__ void pair_arrive_relaxed(uint32_t bar_cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr)
+               : "memory");
+}
+
+// 32 rows of a warp, 64 bytes each (a lane has a row, `v` its sixteen-byte pieces), to out: row r of the
 // warp goes to dst + r * ldo, as far as there are rows and columns.
 template <typename OutT>
-__device__ __forceinline__ void turn_and_store(uint8_t* buf, const uint4 (&v)[8], OutT* dst, long long ldo,
+__device__ __forceinline__ void turn_and_store(uint8_t* buf, const uint4 (&v)[4], OutT* dst, long long ldo,
                                                int n_rows, int n_cols, bool vec, int lane) {
   constexpr int PER = 16 / (int)sizeof(OutT);
 #pragma unroll
-  for (int q = 0; q < 8; ++q)
-    *reinterpret_cast<uint4*>(buf + lane * 128 + ((q ^ (lane & 7)) << 4)) = v[q];
+  for (int q = 0; q < 4; ++q)
+    *reinterpret_cast<uint4*>(buf + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) = v[q];
   __syncwarp();
-  const int q = lane & 7;
+  const int q = lane & 3;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = i * 4 + (lane >> 3);
-    const uint4 x = *reinterpret_cast<const uint4*>(buf + r * 128 + ((q ^ (r & 7)) << 4));
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + (lane >> 2);
+    const uint4 x = *reinterpret_cast<const uint4*>(buf + r * 64 + ((q ^ ((r >> 1) & 3)) << 4));
     if (r < n_rows && q * PER < n_cols) {
       OutT* d = dst + (long long)r * ldo + q * PER;
       if (vec && q * PER + PER <= n_cols) {
@@ -104,7 +123,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const RowTables tables = row_tables_at(base + PF_BARS, p.experts);
   uint8_t* turn = base + ((PF_BARS + p.table_bytes + 1023) & ~1023);
-  uint8_t* tiles = turn + 8 * PF_TURN;
+  uint8_t* tiles = turn + PF_SUMS * PF_TURN;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = pair_rank();
@@ -118,7 +137,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(acc_full + a, 1);
-      mbar_init(acc_empty + a, 16);            // one arrival per warp of both CTAs' sums
+      mbar_init(acc_empty + a, 2 * PF_SUMS);   // one arrival per warp of both CTAs' sums
     }
     mbar_init(drain, 1);
     *abort = 0;
@@ -143,7 +162,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   uint32_t next_phase = 0;
 
   if (warp < 4) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
   if (warp == 0) {
     // --------------------------------------------------------------- copies
     if (lane == 0) {
@@ -190,14 +209,14 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   } else if (warp == 1) {
     // ------------------------------------------------------------- products
     if (rank == 0) {
-      const uint32_t idesc = fp8_idesc(PF_TILE, 256);
+      const uint32_t idesc = fp8_idesc(PF_TILE, 256), elected = elect_one();
       int stage = 0, buf = 0;
       uint32_t phase = 0, buf_phase = 0;
-      bool ok = true;
+      bool ok = true, seen = false;                         // a look at the next group's tiles
       for (int u = pair; u < units && ok; u += pairs) {
         for (int g = 0; g < p.groups; ++g) {
-          if (!mbar_wait_warp(acc_empty + buf, buf_phase ^ 1, abort) ||
-              !mbar_wait_warp(full + stage, phase, abort)) {
+          if (!mbar_seen_or_wait_warp(seen, full + stage, phase, abort) ||
+              !mbar_wait_warp(acc_empty + buf, buf_phase ^ 1, abort)) {
             ok = false;
             break;
           }
@@ -208,9 +227,9 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
 #pragma unroll
           for (int k = 0; k < FK / 32; ++k)
             pair_umma_fp8(tmem_base + (uint32_t)(buf * 256), a_desc + (uint64_t)(2 * k),
-                          b_desc + (uint64_t)(2 * k), idesc, k > 0 ? 1u : 0u);
-          pair_commit_both(empty + stage);
-          pair_commit_both(acc_full + buf);
+                          b_desc + (uint64_t)(2 * k), idesc, k > 0 ? 1u : 0u, elected);
+          pair_commit_by(acc_full + buf, elected);
+          pair_commit_by(empty + stage, elected);
           if (++stage == PF_STAGES) {
             stage = 0;
             phase ^= 1;
@@ -219,16 +238,19 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             buf = 0;
             buf_phase ^= 1;
           }
+          seen = mbar_look(full + stage, phase);
         }
       }
     }
   }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
     // ----------------------------------------------------------------- sums
-    const int quarter = warp & 3, half = (warp - 4) >> 2;
-    const int lane_row = (int)rank * 128 + quarter * 32 + lane;
-    const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
+    // A warp's 64 columns: neighbours, or (gated) the gate rows' and the up rows' of 32 outputs.
+    const int quarter = warp & 3, part = (warp - 4) >> 2;
+    const int col_a = GATED ? (part >> 1) * 128 + (part & 1) * 32 : part * 64;
+    const int col_b = col_a + (GATED ? 64 : 32);
+    const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16);
     const uint32_t acc_empty_leader = pair_map(smem_u32(acc_empty), 0);
     uint8_t* my_turn = turn + (warp - 4) * PF_TURN;
     const bool vec = ((uintptr_t)out & 15) == 0 && p.ldo * (int)sizeof(OutT) % 16 == 0;
@@ -236,23 +258,27 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     uint32_t buf_phase = 0;
     for (int u = pair; u < units; u += pairs) {
       const RowTile t = row_tile(tables, p.experts, p.tiles_f, PF_TILE, u);
-      const int row = t.row0 + lane_row;
-      const float* sx = p.sx + min(row, t.row_end - 1);      // (rows behind the last are not stored)
-      // plain: this half's 128 weight rows have one block's scales; gated: 64 gate and 64 up rows
+      const int row_w0 = t.row0 + (int)rank * 128 + quarter * 32;      // the warp's first row
+      const int row = min(row_w0 + lane, t.row_end - 1);               // (rows behind the last are not stored)
+      const float* sx = p.sx + row;
+      // plain: the columns lie in one block of 128 weight rows; gated: in a gate's and an up's
       const long long block = (long long)t.expert * (GATED ? 2 : 1) * p.w_blocks;
-      const float* swa = p.sw + (block + (GATED ? t.ft : min(t.ft * 2 + half, p.w_blocks - 1))) * p.groups;
-      const float* swb = GATED ? swa + (long long)p.w_blocks * p.groups : swa;
-      float acc[128];
+      const float* swa =
+          p.sw + (block + (GATED ? t.ft : min(t.ft * 2 + (part >> 1), p.w_blocks - 1))) * p.groups;
+      const long long to_b = GATED ? (long long)p.w_blocks * p.groups : 0;
+      float acc[64];
 #pragma unroll
-      for (int j = 0; j < 128; ++j) acc[j] = 0.f;
+      for (int j = 0; j < 64; ++j) acc[j] = 0.f;
       bool ok = true;
-      float s = sx[0], wa = swa[0], wb = swb[0];
+      float s = *sx, wa = *swa, wb = GATED ? swa[to_b] : 0.f;
       for (int g = 0; g < p.groups; ++g) {
         const float fa = fp8_factor(s, wa), fb = GATED ? fp8_factor(s, wb) : fa;
         if (g + 1 < p.groups) {                              // the next group's, under this one's wait
-          s = sx[(long long)(g + 1) * p.lds];
-          wa = swa[g + 1];
-          if (GATED) wb = swb[g + 1];
+          sx += p.lds;
+          ++swa;
+          s = *sx;
+          wa = *swa;
+          if (GATED) wb = swa[to_b];
         }
         if (!mbar_wait_warp(acc_full + buf, buf_phase, abort)) {
           ok = false;
@@ -260,52 +286,47 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         }
         tc_fence_after();
 #pragma unroll
-        for (int c = 0; c < 128; c += 32) {
-          uint32_t r[32];
-          tmem_ld32(taddr + (uint32_t)(buf * 256 + c), r);
-          const float f = c < 64 ? fa : fb;
+        for (int c = 0; c < 64; c += 16) {
+          uint32_t r[16];
+          tmem_ld16(taddr + (uint32_t)(buf * 256 + (c < 32 ? col_a + c : col_b + c - 32)), r);
+          if (c == 48) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) pair_arrive_relaxed(acc_empty_leader + 8u * (uint32_t)buf);
+          }
+          const float f = c < 32 ? fa : fb;
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) fma2v(acc[c + j], acc[c + j + 1], r[j], r[j + 1], f, f);
+          for (int j = 0; j < 16; j += 2) fma2v(acc[c + j], acc[c + j + 1], r[j], r[j + 1], f, f);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) pair_arrive_remote(acc_empty_leader + 8u * (uint32_t)buf);
         if (++buf == 2) {
           buf = 0;
           buf_phase ^= 1;
         }
       }
       if (!ok) break;
-      const float w = p.row_w ? p.row_w[min(row, t.row_end - 1)] : 1.f;
-      const int row_w0 = t.row0 + (int)rank * 128 + quarter * 32;      // the warp's first row
+      const float w = p.row_w ? p.row_w[row] : 1.f;
       const int n_rows = t.row_end - row_w0;
       if (n_rows > 0) {
         OutT* dst = out + (long long)row_w0 * p.ldo;
-        if constexpr (GATED) {
-          const int o = t.ft * 128 + half * 64;
-          uint4 v[8];
+        constexpr int COLS = 64 / (int)sizeof(OutT);         // of 64 bytes
+#pragma unroll
+        for (int c = 0; c < (GATED ? 32 : 64); c += COLS) {
+          const int o = GATED ? t.ft * 128 + part * 32 : t.ft * PF_TILE + part * 64 + c;
+          uint4 v[4];
           uint32_t* v32 = reinterpret_cast<uint32_t*>(v);
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            v32[j] = pack_bf16x2(
-                __float_as_uint(w * fp8_gate(p.act, acc[2 * j], acc[64 + 2 * j], p.gk)),
-                __float_as_uint(w * fp8_gate(p.act, acc[2 * j + 1], acc[65 + 2 * j], p.gk)));
-          turn_and_store<OutT>(my_turn, v, dst + o, p.ldo, n_rows, p.features - o, vec, lane);
-        } else {
-          constexpr int COLS = 128 / (int)sizeof(OutT);      // of 128 bytes
-#pragma unroll
-          for (int c = 0; c < 128; c += COLS) {
-            const int o = t.ft * PF_TILE + half * 128 + c;
-            uint4 v[8];
-            uint32_t* v32 = reinterpret_cast<uint32_t*>(v);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              if constexpr (sizeof(OutT) == 4) v32[j] = __float_as_uint(w * acc[c + j]);
-              else v32[j] = pack_bf16x2(__float_as_uint(w * acc[c + 2 * j]), __float_as_uint(w * acc[c + 2 * j + 1]));
-            }
-            if (o < p.features)
-              turn_and_store<OutT>(my_turn, v, dst + o, p.ldo, n_rows, p.features - o, vec, lane);
+          for (int j = 0; j < 16; ++j) {
+            if constexpr (GATED)
+              v32[j] = pack_bf16x2(
+                  __float_as_uint(w * fp8_gate(p.act, acc[2 * j], acc[32 + 2 * j], p.gk)),
+                  __float_as_uint(w * fp8_gate(p.act, acc[2 * j + 1], acc[33 + 2 * j], p.gk)));
+            else if constexpr (sizeof(OutT) == 4)
+              v32[j] = __float_as_uint(w * acc[c + j]);
+            else
+              v32[j] = pack_bf16x2(__float_as_uint(w * acc[c + 2 * j]), __float_as_uint(w * acc[c + 2 * j + 1]));
           }
+          if (o < p.features)
+            turn_and_store<OutT>(my_turn, v, dst + o, p.ldo, n_rows, p.features - o, vec, lane);
         }
       }
     }
@@ -351,9 +372,9 @@ int pair_launch(const void* x, long long ldx, const void* w, long long ldw, OutT
   const long long units = tiles_r * p.experts * p.tiles_f;
   if (units > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
   const size_t smem =
-      1024 + ((PF_BARS + p.table_bytes + 1023) & ~1023) + 8 * PF_TURN + (size_t)PF_STAGES * PF_STAGE;
+      1024 + ((PF_BARS + p.table_bytes + 1023) & ~1023) + PF_SUMS * PF_TURN + (size_t)PF_STAGES * PF_STAGE;
   const size_t smem_max =
-      1024 + ((PF_BARS + row_tables_bytes(FP8_MAX_EXPERTS) + 1023) & ~1023) + 8 * PF_TURN +
+      1024 + ((PF_BARS + row_tables_bytes(FP8_MAX_EXPERTS) + 1023) & ~1023) + PF_SUMS * PF_TURN +
       (size_t)PF_STAGES * PF_STAGE;
   auto kern = fp8_pair_kernel<OutT, GATED>;
   static bool configured_on[BF_MAX_DEVICES];

@@ -2834,8 +2834,13 @@ def gemm_bf16_swiglu(x: torch.Tensor, w_gate_up: torch.Tensor, out: torch.Tensor
 # ------------------------------------------------------------------ weights in 8 bits
 FP8_GROUP = 128                # numbers of a row that share a scale; weights: blocks of 128 x 128
 FP8_MAX_EXPERTS = 512
+# BINFER_B200_FP8_RESIDENT=0: the rows go into 8 bits in a kernel of their own for few rows too
+FP8_RESIDENT = os.environ.get("BINFER_B200_FP8_RESIDENT", "1") != "0"
 E4M3 = torch.float8_e4m3fn
 
+_fp8_rows_call = _Packed("bf_fp8_rows", "PqPqPqiiiiP")
+_fp8_blocks_call = _Packed("bf_fp8_blocks", "PqPqPiiiiP")
+_fp8_read_call = _Packed("bf_fp8_read", "PqPqPqiiiiiiP")
 _fp8_product_call = _Packed("bf_fp8_product", "PqPqPqPqPPPPqiiiiiiifffiiiPP")
 
 
@@ -2883,9 +2888,8 @@ def fp8_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     codes = _fp8_empty_codes((T, K), x.device)
     scales = torch.empty((-(-K // FP8_GROUP), T), dtype=torch.float32, device=x.device)
     if T:
-        _run("fp8_rows", lib().bf_fp8_rows, _ptr(x), _c_ll(x.stride(0)), _c_int(_dtype_code(x)), _ptr(codes),
-             _c_ll(codes.stride(0)), _ptr(scales), _c_ll(T), _c_int(T), _c_int(K), _c_int(num_sms(x.device)),
-             _c_void_p(_stream_at(x)))
+        _run("fp8_rows", _fp8_rows_call, x.data_ptr(), x.stride(0), codes.data_ptr(), codes.stride(0),
+             scales.data_ptr(), T, _dtype_code(x), T, K, num_sms(x.device), _stream_at(x))
     return codes, scales
 
 
@@ -2901,9 +2905,8 @@ def fp8_rows_read(codes: torch.Tensor, scales: torch.Tensor, out: torch.Tensor) 
         raise KernelError("fp8_rows_read: scales must be float32 [ceil(K / 128), T] with contiguous rows")
     _same_device("fp8_rows_read", codes, scales, out)
     if T:
-        _run("fp8_read", lib().bf_fp8_read, _ptr(codes), _c_ll(codes.stride(0)), _ptr(scales),
-             _c_ll(scales.stride(0)), _ptr(out), _c_ll(out.stride(0)), _c_int(_dtype_code(out)), _c_ll(T),
-             _c_int(K), _c_int(1), _c_int(T), _c_int(num_sms(out.device)), _c_void_p(_stream_at(out)))
+        _run("fp8_read", _fp8_read_call, codes.data_ptr(), codes.stride(0), scales.data_ptr(), scales.stride(0),
+             out.data_ptr(), out.stride(0), _dtype_code(out), 0, 1, T, K, num_sms(out.device), _stream_at(out))
 
 
 class Fp8Weight:
@@ -2956,9 +2959,8 @@ def fp8_weight(w: torch.Tensor, gated: bool = False) -> Fp8Weight:
     codes = _fp8_empty_codes(w.shape, w.device)
     scales = torch.empty((*lead, halves * -(-(n // halves) // FP8_GROUP), -(-k // FP8_GROUP)),
                          dtype=torch.float32, device=w.device)
-    _run("fp8_blocks", lib().bf_fp8_blocks, _ptr(w), _c_ll(w.stride(-2)), _c_int(_dtype_code(w)), _ptr(codes),
-         _c_ll(codes.stride(-2)), _ptr(scales), _c_int((lead[0] if lead else 1) * halves), _c_int(n // halves),
-         _c_int(k), _c_void_p(_stream_at(w)))
+    _run("fp8_blocks", _fp8_blocks_call, w.data_ptr(), w.stride(-2), codes.data_ptr(), codes.stride(-2),
+         scales.data_ptr(), _dtype_code(w), (lead[0] if lead else 1) * halves, n // halves, k, _stream_at(w))
     return Fp8Weight(codes, scales, gated)
 
 
@@ -2968,10 +2970,9 @@ def fp8_weight_read(w: Fp8Weight, out: torch.Tensor) -> None:
     if out.shape != w.shape or not _fp8_stacked(out):
         raise KernelError("fp8_weight_read: out must have the weight's shape, its rows equally far apart")
     _same_device("fp8_weight_read", w.codes, w.scales, out)
-    _run("fp8_read", lib().bf_fp8_read, _ptr(w.codes), _c_ll(w.codes.stride(-2)), _ptr(w.scales), _c_ll(0),
-         _ptr(out), _c_ll(out.stride(-2)), _c_int(_dtype_code(out)), _c_ll(max(1, w.experts) * w.rows),
-         _c_int(w.K), _c_int(FP8_GROUP), _c_int(w.features), _c_int(num_sms(out.device)),
-         _c_void_p(_stream_at(out)))
+    at, pitch, scales_at = w._held
+    _run("fp8_read", _fp8_read_call, at, pitch, scales_at, 0, out.data_ptr(), out.stride(-2), _dtype_code(out), 1,
+         max(1, w.experts) * (2 if w.gated else 1), w.features, w.K, num_sms(out.device), _stream_at(out))
 
 
 def _fp8_product(what: str, x, w: Fp8Weight, starts, out, row_w, activation, limit, slope, up_offset, tile,
@@ -2991,23 +2992,35 @@ def _fp8_product(what: str, x, w: Fp8Weight, starts, out, row_w, activation, lim
         _want(row_w, torch.float32, "row_w")
         if row_w.numel() != M:
             raise KernelError(f"{what}: row_w must have a number per row")
-    if tile not in (0, 16, 32, 64, 128, 256, -1) or not 0 <= split <= 8:
+    if tile not in (0, 16, 32, 64, -1) or not 0 <= split <= 8:
         raise KernelError(f"{what}: no tiles of {tile} rows, shared by {split}")
     err = error_word(x.device)
     _same_device(what, x, w.codes, w.scales, starts, out, row_w, err)
     if M == 0:
         return
-    # the rows' codes and behind them their scales
-    pitch, groups = -(-K // 16) * 16, -(-K // FP8_GROUP)
-    scratch = torch.empty(M * pitch + 4 * groups * M, dtype=torch.uint8, device=x.device)
-    at = scratch.data_ptr()
     w_at, w_pitch, sw_at = w._held
-    _run(what, _fp8_product_call, x.data_ptr(), x.stride(0), at, pitch, at + M * pitch, M, w_at, w_pitch, sw_at,
-         starts.data_ptr() if starts is not None else 0, row_w.data_ptr() if row_w is not None else 0,
-         out.data_ptr(), out.stride(0), 0 if out.dtype == torch.float32 else 1, M, w.features, K,
-         max(1, w.experts), w.gated, GATE_ACTIVATIONS[activation] if w.gated else 0, limit, slope, up_offset, tile,
-         split, num_sms(x.device), err.data_ptr(), _stream_at(x))
+    behind = (w_at, w_pitch, sw_at, starts.data_ptr() if starts is not None else 0,
+              row_w.data_ptr() if row_w is not None else 0, out.data_ptr(), out.stride(0),
+              0 if out.dtype == torch.float32 else 1, M, w.features, K, max(1, w.experts), w.gated,
+              GATE_ACTIVATIONS[activation] if w.gated else 0, limit, slope, up_offset, tile, split,
+              num_sms(x.device), err.data_ptr(), _stream_at(x))
     global _launches
+    if M <= 32 and starts is None and FP8_RESIDENT:
+        # few rows: one kernel, where it takes the sizes
+        p = _profiler
+        if p is not None:
+            p.begin(what)
+        code = _fp8_product_call(x.data_ptr(), x.stride(0), 0, 0, 0, 0, *behind)
+        if p is not None:
+            p.end(what)
+        if code != -1:
+            _check(code, what)
+            return
+    # the rows' codes and behind them their scales
+    pitch = -(-K // 16) * 16
+    scratch = torch.empty(M * pitch + 4 * -(-K // FP8_GROUP) * M, dtype=torch.uint8, device=x.device)
+    at = scratch.data_ptr()
+    _run(what, _fp8_product_call, x.data_ptr(), x.stride(0), at, pitch, at + M * pitch, M, *behind)
     _launches += 1          # two kernels
 
 
@@ -3019,8 +3032,8 @@ def fp8_linear(x: torch.Tensor, w: Fp8Weight, out: torch.Tensor, activation: str
     columns after another.  A gated weight: ``out = act(g) u`` of the product's two halves, ``activation`` as
     in :func:`gated_act_mul` ("silu" or "clamped").  ``out``: bfloat16, or float32 for a weight that is not
     gated; it may be a column block of a wider buffer.  A row's result does not depend on the other rows'
-    values.  ``tile``, ``split``: rows of a tile (-1: on pairs of SMs) and SMs that share one (0: chosen by the
-    library)."""
+    values.  ``tile``, ``split``: rows of a tile (16, 32 or 64; -1: on pairs of SMs) and SMs that share one (0: chosen
+    by the library)."""
     if w.experts:
         raise KernelError("fp8_linear: the weight has experts")
     _fp8_product("fp8_linear", x, w, None, out, None, activation, limit, slope, up_offset, tile, split)

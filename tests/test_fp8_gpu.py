@@ -149,14 +149,14 @@ SIZES = [(1, 128, 128), (1, 16, 16), (3, 1, 5), (8, 384, 640), (16, 1000, 130), 
          (64, 512, 300), (65, 2048, 128), (129, 640, 200), (200, 100, 1000), (257, 384, 513), (300, 1024, 64)]
 
 
-@pytest.mark.parametrize("tile", [16, 32, 64, 128, 256, -1])
+@pytest.mark.parametrize("tile", [16, 32, 64, -1])
 @pytest.mark.parametrize("M,K,N", SIZES)
 def test_linear_of_every_tile(cuda_device, M, K, N, tile):
     out, ref = _linear(cuda_device, M, K, N, out_type=F32, seed=M + N, tile=tile)
     _check(out, *ref)
 
 
-@pytest.mark.parametrize("tile", [16, 32, 64, 128, 256, -1])
+@pytest.mark.parametrize("tile", [16, 32, 64, -1])
 @pytest.mark.parametrize("M,K,N", [(1, 128, 64), (5, 300, 100), (16, 512, 128), (40, 256, 200), (130, 640, 65),
                                    (300, 384, 300), (520, 256, 130)])
 def test_gated_linear_of_every_tile(cuda_device, M, K, N, tile):
@@ -274,7 +274,7 @@ def _experts(dev, counts, K, N, gated=False, out_type=BF16, before=0, behind=0, 
             _check(out[a:b], ref, off)
 
 
-@pytest.mark.parametrize("tile", [0, 16, 32, 64, 128, 256, -1])
+@pytest.mark.parametrize("tile", [0, 16, 32, 64, -1])
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("counts", [[1], [0, 0, 3], [5, 0, 17, 1, 16, 0], [40, 300, 0, 129, 64], [600, 2]])
 def test_experts(cuda_device, counts, gated, tile):
@@ -387,3 +387,20 @@ def test_repeats_bit_for_bit(cuda_device):
         for o in outs:
             ops.fp8_linear(x, w, o)
         assert all(torch.equal(outs[0], o) for o in outs[1:])
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("M,K,N", [(1, 4096, 300), (3, 1000, 130), (8, 12288, 256), (9, 4096, 128), (16, 2048, 5000),
+                                   (20, 640, 4000), (32, 4096, 640)])
+def test_one_kernel_or_two(cuda_device, monkeypatch, M, K, N, gated):
+    """Few rows as one kernel and as two: the same codes, the same sums."""
+    from binfer_b200.csrc import ops
+    x, w = _x(M, K + 8, cuda_device, M)[:, 3:3 + K], ops.fp8_weight(_w(((1 + gated) * N, K), cuda_device), gated)
+    for rows in (x, x.contiguous()):
+        outs = []
+        for resident in (True, False):
+            monkeypatch.setattr(ops, "FP8_RESIDENT", resident)
+            out = torch.empty((M, N), dtype=BF16, device=cuda_device)
+            ops.fp8_linear(rows, w, out)
+            outs.append(out)
+        assert torch.equal(*outs)
