@@ -296,11 +296,20 @@ extern "C" int bf_gemm_fp8_pair(const void*, long long, const float*, long long,
                                 const float*, const int*, const float*, void*, long long, int, int, int, int,
                                 int, int, int, float, float, float, int, int*, cudaStream_t);
 
-// How a product runs: the most rows of a tile of gemm_fp8_few.cu, or -1 for gemm_fp8_pair.cu.
-static int fp8_tile(int rows, int experts) {
+// How a product runs: the most rows of a tile of gemm_fp8_few.cu, or -1 for gemm_fp8_pair.cu.  Without
+// experts tiles of 32 rows as long as they are all resident (157 rows, 6,144 x 4,096: 18.6 us against 23.3
+// with tiles of 64 and 22.3 on pairs; 256 rows, 4,096 x 12,288: 42 / 40 / 51), then 64 if those hold all
+// rows (64 rows, 24,576 x 4,096 gated: 28 against 36 and 44), then pairs (157 rows of the same: 61 / 51 /
+// 46).  With experts by the rows that one has on average (64 experts, 2,048 x 2,048 gated, 8 to 128 rows
+// each: 47 / 51 / 55 us with tiles of 16 / 32 / 64 and 84 on pairs, 77 / 62 / 60 / 92, 128 / 90 / 84 / 104,
+// 228 / 156 / 136 / 126).
+static int fp8_tile(int rows, int features, bool gated, int experts, int num_sms) {
   const int each = (rows + experts - 1) / experts;
-  if (each > (experts > 1 ? 112 : 192)) return -1;
-  return each <= 16 ? 16 : each <= 32 ? 32 : 64;
+  if (each <= 16) return 16;
+  if (experts > 1) return each <= 24 ? 32 : each <= 112 ? 64 : -1;
+  const long long tiles = (rows + 31LL) / 32 * ((features + (gated ? 63 : 127)) / (gated ? 64 : 128));
+  if (each <= 32 || tiles <= 2 * num_sms) return 32;
+  return each <= 64 ? 64 : -1;
 }
 // CTAs that share a tile of 128 weight rows: as many (a power of two: clusters of other sizes leave SMs
 // of a GPC empty) as are resident together, two to an SM, each with two groups at least.
@@ -337,13 +346,13 @@ struct Fp8ProductCall {
 BF_EXPORT int bf_fp8_product(const Fp8ProductCall* call) {
   const Fp8ProductCall& c = *call;
   if (c.rows <= 0 || c.features <= 0) return 0;
-  const int tile = c.tile ? c.tile : fp8_tile(c.rows, c.experts);
+  const int tile = c.tile ? c.tile : fp8_tile(c.rows, c.features, c.gated != 0, c.experts, c.num_sms);
   const int split = c.starts || tile < 0 ? 1
                     : c.split ? c.split
                               : fp8_split(c.rows, c.features, c.K, c.gated != 0, tile, c.num_sms);
   if (!c.codes) {
     // asked for without scratch: the rows stay in the CTAs that read them, where they fit
-    if (tile < 0 || tile > 32 || c.rows > tile || c.starts) return -1;
+    if (tile != 16 || c.starts) return -1;
     return bf_gemm_fp8_few(c.x, c.ldx, nullptr, 0, c.w, c.ldw, c.sw, c.starts, c.row_w, c.out, c.ldo, c.out_dtype,
                            c.rows, c.features, c.K, c.experts, c.gated, c.act, c.limit, c.slope, c.up_offset,
                            tile, split, 1, c.num_sms, c.err, c.stream);

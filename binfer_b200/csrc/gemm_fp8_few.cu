@@ -18,9 +18,9 @@
 // part of the groups, and the parts meet in shared memory, added in the order of the ranks.
 // With experts the tiles are dealt out to persistent CTAs.
 //
-// RESIDENT: few rows come as bfloat16, and every CTA puts its columns of them into 8 bits by itself
-// (warps 4-11, before the first sums, while the first weights are on their way), where they stay: no
-// kernel in front, nothing of them through global memory.
+// RESIDENT: at most eight rows come as bfloat16, and every CTA puts its columns of them into 8 bits by
+// itself (warps 4-11, before the first sums, while the first weights are on their way), where they stay:
+// no kernel in front, nothing of them through global memory.
 //
 // Every wait is bounded; no load uses multicast.
 #include "common.cuh"
@@ -32,8 +32,12 @@ namespace {
 constexpr int FEW_THREADS = 384;
 constexpr int FEW_MAX_STAGES = 12;
 constexpr int FEW_BARS = 1024;
-constexpr int FEW_READY = 512;                // offset among the barriers of RESIDENT's, one per round
-constexpr int FEW_ROUNDS = (FEW_BARS - FEW_READY) / 8;
+// RESIDENT: rows, and turns in which the CTA puts its columns of them into 8 bits (32 groups each).  With
+// more turns a kernel in front is faster (a turn is 0.6 us; one row, 4,096 x 2,048 to 12,288: 8.5 to 13.7 us
+// so and 8.0 to 12.8 us with it, but 1,024 x 2,048: 5.0 and 5.5; launched one by one, 4 us of the host's
+// time are gained at every size).
+constexpr int FEW_RES_ROWS = 8;
+constexpr int FEW_ROUNDS = 2;
 constexpr int FEW_W_BYTES = 128 * FK;
 // Two CTAs share an SM: its registers, its shared memory and its tensor memory are dealt out by halves.  A
 // step of eight rows against 24,576 x 4,096 gated took 27.5 us with one, whose 192 tiles ran in two turns.
@@ -58,11 +62,9 @@ struct FewParams {
   const float* sw;                     // [experts * (gated ? 2 : 1) * w_blocks, groups]
   const float* row_w;                  // per row, or null
   int split, stages, table_bytes;
-  // RESIDENT: the rows, room for res_rows of them (8: the product's second eight columns read the first
-  // eight again), res_groups groups of each
-  const __nv_bfloat16* x;
+  const __nv_bfloat16* x;              // RESIDENT: the rows, res_groups groups of each in a CTA
   long long ldx;
-  int x_vec, res_rows, res_groups;
+  int x_vec, res_groups;
   long long ldo;
   int act;
   BfGateConst gk;
@@ -104,10 +106,10 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
                         (p.split > 1 ? ((NB + p.split - 1) / p.split) * p.split * 128 * 4
                                      : GATED ? FewShape<NB>::EXCHANGE : 0);
   const RowTables tables = row_tables_at(table_smem, p.experts);
-  uint64_t* ready = reinterpret_cast<uint64_t*>(base + FEW_READY);
+  uint64_t* ready = drain + 2;                           // [FEW_ROUNDS]
   float* res_sx = reinterpret_cast<float*>(table_smem + p.table_bytes);        // [res_groups][NB]
   uint8_t* res = base + (((table_smem - base) + p.table_bytes + (RESIDENT ? p.res_groups * NB * 4 : 0) + 1023) & ~1023);
-  uint8_t* tiles = res + (RESIDENT ? (p.res_groups * p.res_rows * FK + 1023) & ~1023 : 0);
+  uint8_t* tiles = res + (RESIDENT ? p.res_groups * FEW_RES_ROWS * FK : 0);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = p.split > 1 ? (int)few_rank() : 0;
@@ -116,7 +118,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   const int g1 = (int)((long long)p.groups * (rank + 1) / p.split);
   const int STAGES = p.stages;
   const int w_rows = HALVES * p.features;                // of an expert
-  // RESIDENT: 32 places of eight lanes, a row and group each: so many groups at once
+  // RESIDENT: 32 places of eight lanes, a row and group each: so many groups a turn
   int row_shift = 0;
   while (RESIDENT && (1 << row_shift) < p.rows) ++row_shift;
   const int per_round = 32 >> row_shift;
@@ -220,7 +222,8 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
         const uint32_t a_addr = smem_u32(tiles + (size_t)stage * STAGE), d_tmem = tmem_base + (uint32_t)(slot * NB);
         const uint64_t a_desc = umma_desc_k_sw128(a_addr);
         const uint64_t b_desc =
-            RESIDENT ? umma_desc_k_sw128_sbo(smem_u32(res + (g - g0) * p.res_rows * FK), p.res_rows == 8 ? 0u : 1024u)
+            // (eight rows: the product's second eight columns read them again)
+            RESIDENT ? umma_desc_k_sw128_sbo(smem_u32(res + (g - g0) * FEW_RES_ROWS * FK), 0u)
                      : umma_desc_k_sw128(a_addr + FEW_W_BYTES);
         uint64_t* const done_stage = empty + stage;
         uint64_t* const done_slot = acc_full + slot;
@@ -343,7 +346,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
         for (int o = 4; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
         const Fp8Scale sc = fp8_scale(m);
         if (row < p.rows && gl < g1 - g0) {
-          *reinterpret_cast<uint4*>(res + (gl * p.res_rows + row) * FK + ((sub ^ (row & 7)) << 4)) = v.codes(sc);
+          *reinterpret_cast<uint4*>(res + (gl * FEW_RES_ROWS + row) * FK + ((sub ^ (row & 7)) << 4)) = v.codes(sc);
           if (sub == 0) res_sx[gl * NB + row] = sc.s;
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -519,7 +522,7 @@ size_t few_memory(const FewParams& p, int* stages) {
   size_t fixed = FEW_BARS + (size_t)FewShape<NB>::SLOTS * (GATED ? 2 : 1) * NB * 4 + extra + p.table_bytes;
   if (RESIDENT) fixed += (size_t)p.res_groups * NB * 4;
   fixed = 1024 + ((fixed + 1023) & ~(size_t)1023);
-  if (RESIDENT) fixed += ((size_t)p.res_groups * p.res_rows * FK + 1023) & ~(size_t)1023;
+  if (RESIDENT) fixed += (size_t)p.res_groups * FEW_RES_ROWS * FK;
   const size_t stage = FEW_W_BYTES + (RESIDENT ? 0 : NB * FK);
   const size_t n = fixed < FEW_SMEM ? (FEW_SMEM - fixed) / stage : 0;
   *stages = n > FEW_MAX_STAGES ? FEW_MAX_STAGES : (int)n;
@@ -552,11 +555,10 @@ int few_launch(const void* x, long long ldx, const void* w, long long ldw, OutT*
     p.x = (const __nv_bfloat16*)x;
     p.ldx = ldx;
     p.x_vec = ldx % 8 == 0 && ((uintptr_t)x & 15) == 0;
-    p.res_rows = p.rows <= 8 ? 8 : (p.rows + 15) & ~15;
     p.res_groups = (p.groups + p.split - 1) / p.split;
     int per_round = 32;
     while (32 / per_round < p.rows) per_round /= 2;
-    if (p.starts || p.rows > NB || (p.res_groups + per_round - 1) / per_round > FEW_ROUNDS) return FEW_DOES_NOT_FIT;
+    if (p.starts || p.rows > FEW_RES_ROWS || (p.res_groups + per_round - 1) / per_round > FEW_ROUNDS) return FEW_DOES_NOT_FIT;
   }
   const size_t smem = few_memory<NB, GATED, RESIDENT>(p, &p.stages);
   if (RESIDENT && p.stages < 4) return FEW_DOES_NOT_FIT;
@@ -592,7 +594,6 @@ int few_by_width(int nb, bool resident, const void* x, long long ldx, const void
                  const FewParams& p, int num_sms, cudaStream_t stream) {
   if (resident) {
     if (nb == 16) return few_launch<16, OutT, GATED, true>(x, ldx, w, ldw, out, p, num_sms, stream);
-    if (nb == 32) return few_launch<32, OutT, GATED, true>(x, ldx, w, ldw, out, p, num_sms, stream);
     return FEW_DOES_NOT_FIT;
   }
   switch (nb) {

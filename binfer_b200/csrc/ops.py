@@ -2846,23 +2846,30 @@ _fp8_product_call = _Packed("bf_fp8_product", "PqPqPqPqPPPPqiiiiiiifffiiiPP")
 
 def _fp8_empty_codes(shape, device) -> torch.Tensor:
     """Room for codes ``[..., K]`` whose rows lie on 16-byte boundaries."""
-    *lead, k = shape
-    pitch = -(-k // 16) * 16
-    strides, step = [1], pitch
-    for n in reversed(lead):
+    k = shape[-1]
+    if k % 16 == 0:
+        return torch.empty(shape, dtype=E4M3, device=device)
+    strides, step = [1], -(-k // 16) * 16
+    for n in reversed(shape[:-1]):
         strides.append(step)
         step *= n
     return torch.empty_strided(tuple(shape), tuple(reversed(strides)), dtype=E4M3, device=device)
 
 
-def _fp8_matrix(what: str, name: str, t: torch.Tensor, dims: Tuple[int, ...] = (2,)) -> None:
-    if t.dim() not in dims or t.dtype not in (torch.bfloat16, torch.float32):
+_FP8_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def _fp8_matrix(what: str, name: str, t: torch.Tensor, dims: Tuple[int, ...] = (2,)) -> int:
+    """The code of a matrix's type."""
+    dtype, shape = _FP8_DTYPES.get(t.dtype), t.shape
+    if dtype is None or len(shape) not in dims:
         raise KernelError(f"{what}: {name} must be bfloat16 or float32 with {' or '.join(map(str, dims))} "
-                          f"dimensions, got {t.dtype} {tuple(t.shape)}")
-    if t.shape[-1] < 1:
+                          f"dimensions, got {t.dtype} {tuple(shape)}")
+    if shape[-1] < 1:
         raise KernelError(f"{what}: {name} has no columns")
-    if t.shape[-1] > 1 and t.numel() and t.stride(-1) != 1:
+    if t.stride(-1) != 1 and shape[-1] > 1 and t.numel():
         raise KernelError(f"{what}: rows of {name} must be contiguous")
+    return dtype
 
 
 def _fp8_stacked(t: torch.Tensor) -> bool:
@@ -2872,8 +2879,9 @@ def _fp8_stacked(t: torch.Tensor) -> bool:
 
 def _fp8_codes_lie(codes: torch.Tensor) -> bool:
     """Whether codes lie as the kernels take them: rows contiguous and on 16-byte boundaries."""
-    return ((codes.shape[-1] < 2 or codes.stride(-1) == 1) and codes.stride(-2) % 16 == 0
-            and codes.stride(-2) >= codes.shape[-1] and codes.data_ptr() % 16 == 0 and _fp8_stacked(codes))
+    k, pitch = codes.shape[-1], codes.stride(-2)
+    return ((k < 2 or codes.stride(-1) == 1) and pitch % 16 == 0 and pitch >= k
+            and codes.data_ptr() % 16 == 0 and _fp8_stacked(codes))
 
 
 def fp8_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -2882,31 +2890,33 @@ def fp8_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     ``s = max(float32(a / 448), 2^-100)``, a the largest size among them, and a number's code is the
     e4m3 value nearest to ``x / s``, ties to even.  A number that is not finite makes its group read as
     NaN.  (The codes' rows are padded to 16 bytes: ``codes`` need not be contiguous.)"""
-    _fp8_matrix("fp8_rows", "x", x)
-    T, K = x.shape
+    dtype = _fp8_matrix("fp8_rows", "x", x)
     _same_device("fp8_rows", x)
-    codes = _fp8_empty_codes((T, K), x.device)
-    scales = torch.empty((-(-K // FP8_GROUP), T), dtype=torch.float32, device=x.device)
+    shape, device = x.shape, x.device
+    T, K = shape
+    codes = _fp8_empty_codes(shape, device)
+    scales = torch.empty((-(-K // FP8_GROUP), T), dtype=torch.float32, device=device)
     if T:
-        _run("fp8_rows", _fp8_rows_call, x.data_ptr(), x.stride(0), codes.data_ptr(), codes.stride(0),
-             scales.data_ptr(), T, _dtype_code(x), T, K, num_sms(x.device), _stream_at(x))
+        _run("fp8_rows", _fp8_rows_call, x.data_ptr(), x.stride(0), codes.data_ptr(), -(-K // 16) * 16,
+             scales.data_ptr(), T, dtype, T, K, num_sms(device), _stream_at(x))
     return codes, scales
 
 
 def fp8_rows_read(codes: torch.Tensor, scales: torch.Tensor, out: torch.Tensor) -> None:
     """What :func:`fp8_rows`'s codes and scales stand for, into ``out [T, K]`` (bfloat16 or float32)."""
-    _fp8_matrix("fp8_rows_read", "out", out)
-    T, K = out.shape
-    if codes.dtype != E4M3 or tuple(codes.shape) != (T, K) or (T and not _fp8_codes_lie(codes)):
+    dtype = _fp8_matrix("fp8_rows_read", "out", out)
+    shape = out.shape
+    T, K = shape
+    if codes.dtype != E4M3 or codes.shape != shape or (T and not _fp8_codes_lie(codes)):
         raise KernelError("fp8_rows_read: codes must be float8_e4m3fn of out's shape, their rows contiguous and "
                           "on 16-byte boundaries")
-    if scales.dtype != torch.float32 or tuple(scales.shape) != (-(-K // FP8_GROUP), T) or (
+    if scales.dtype != torch.float32 or scales.shape != (-(-K // FP8_GROUP), T) or (
             T > 1 and scales.stride(1) != 1):
         raise KernelError("fp8_rows_read: scales must be float32 [ceil(K / 128), T] with contiguous rows")
     _same_device("fp8_rows_read", codes, scales, out)
     if T:
         _run("fp8_read", _fp8_read_call, codes.data_ptr(), codes.stride(0), scales.data_ptr(), scales.stride(0),
-             out.data_ptr(), out.stride(0), _dtype_code(out), 0, 1, T, K, num_sms(out.device), _stream_at(out))
+             out.data_ptr(), out.stride(0), dtype, 0, 1, T, K, num_sms(out.device), _stream_at(out))
 
 
 class Fp8Weight:
@@ -2949,7 +2959,7 @@ class Fp8Weight:
 def fp8_weight(w: torch.Tensor, gated: bool = False) -> Fp8Weight:
     """``w [N, K]`` or ``[E, N, K]`` (bfloat16 or float32) as an :class:`Fp8Weight`: of every block of 128 x 128
     the scale and the codes as :func:`fp8_rows` takes them of 128 numbers."""
-    _fp8_matrix("fp8_weight", "w", w, (2, 3))
+    dtype = _fp8_matrix("fp8_weight", "w", w, (2, 3))
     if not w.numel() or not _fp8_stacked(w) or (gated and w.shape[-2] % 2):
         raise KernelError("fp8_weight: w must have rows that are equally far apart, a gated one as many up rows "
                           "as gate rows")
@@ -2960,32 +2970,33 @@ def fp8_weight(w: torch.Tensor, gated: bool = False) -> Fp8Weight:
     scales = torch.empty((*lead, halves * -(-(n // halves) // FP8_GROUP), -(-k // FP8_GROUP)),
                          dtype=torch.float32, device=w.device)
     _run("fp8_blocks", _fp8_blocks_call, w.data_ptr(), w.stride(-2), codes.data_ptr(), codes.stride(-2),
-         scales.data_ptr(), _dtype_code(w), (lead[0] if lead else 1) * halves, n // halves, k, _stream_at(w))
+         scales.data_ptr(), dtype, (lead[0] if lead else 1) * halves, n // halves, k, _stream_at(w))
     return Fp8Weight(codes, scales, gated)
 
 
 def fp8_weight_read(w: Fp8Weight, out: torch.Tensor) -> None:
     """What an :class:`Fp8Weight` stands for, into ``out`` of its shape (bfloat16 or float32)."""
-    _fp8_matrix("fp8_weight_read", "out", out, (2, 3))
+    dtype = _fp8_matrix("fp8_weight_read", "out", out, (2, 3))
     if out.shape != w.shape or not _fp8_stacked(out):
         raise KernelError("fp8_weight_read: out must have the weight's shape, its rows equally far apart")
     _same_device("fp8_weight_read", w.codes, w.scales, out)
     at, pitch, scales_at = w._held
-    _run("fp8_read", _fp8_read_call, at, pitch, scales_at, 0, out.data_ptr(), out.stride(-2), _dtype_code(out), 1,
+    _run("fp8_read", _fp8_read_call, at, pitch, scales_at, 0, out.data_ptr(), out.stride(-2), dtype, 1,
          max(1, w.experts) * (2 if w.gated else 1), w.features, w.K, num_sms(out.device), _stream_at(out))
 
 
 def _fp8_product(what: str, x, w: Fp8Weight, starts, out, row_w, activation, limit, slope, up_offset, tile,
                  split) -> None:
-    M, K = x.shape if x.dim() == 2 else (-1, 0)
-    if x.dtype != torch.bfloat16 or K != w.K or (M > 0 and K > 1 and x.stride(1) != 1):
-        raise KernelError(f"{what}: x must be bfloat16 [rows, {w.K}] with contiguous rows, got {x.dtype} "
-                          f"{tuple(x.shape)}")
-    if (out.dtype not in (torch.bfloat16, torch.float32) or tuple(out.shape) != (M, w.features)
-            or (M > 0 and w.features > 1 and out.stride(1) != 1)):
-        raise KernelError(f"{what}: out must be bfloat16 or float32 [{M}, {w.features}] with contiguous rows, got "
-                          f"{out.dtype} {tuple(out.shape)}")
-    if w.gated and (out.dtype != torch.bfloat16 or activation not in FUSED_ACTIVATIONS):
+    shape, out_shape, K, features = x.shape, out.shape, w.K, w.features
+    M = shape[0] if len(shape) == 2 else -1
+    if x.dtype != torch.bfloat16 or M < 0 or shape[1] != K or (M and K > 1 and x.stride(1) != 1):
+        raise KernelError(f"{what}: x must be bfloat16 [rows, {K}] with contiguous rows, got {x.dtype} "
+                          f"{tuple(shape)}")
+    out_type = _FP8_DTYPES.get(out.dtype)
+    if (out_type is None or out_shape != (M, features) or (M and features > 1 and out.stride(1) != 1)):
+        raise KernelError(f"{what}: out must be bfloat16 or float32 [{M}, {features}] with contiguous rows, got "
+                          f"{out.dtype} {tuple(out_shape)}")
+    if w.gated and (out_type != 1 or activation not in FUSED_ACTIVATIONS):
         raise KernelError(f"{what}: a gated product has a bfloat16 result and one of the activations "
                           f"{FUSED_ACTIVATIONS}")
     if row_w is not None:
@@ -2994,34 +3005,33 @@ def _fp8_product(what: str, x, w: Fp8Weight, starts, out, row_w, activation, lim
             raise KernelError(f"{what}: row_w must have a number per row")
     if tile not in (0, 16, 32, 64, -1) or not 0 <= split <= 8:
         raise KernelError(f"{what}: no tiles of {tile} rows, shared by {split}")
-    err = error_word(x.device)
+    device = x.device
+    err = error_word(device)
     _same_device(what, x, w.codes, w.scales, starts, out, row_w, err)
     if M == 0:
         return
-    w_at, w_pitch, sw_at = w._held
-    behind = (w_at, w_pitch, sw_at, starts.data_ptr() if starts is not None else 0,
-              row_w.data_ptr() if row_w is not None else 0, out.data_ptr(), out.stride(0),
-              0 if out.dtype == torch.float32 else 1, M, w.features, K, max(1, w.experts), w.gated,
-              GATE_ACTIVATIONS[activation] if w.gated else 0, limit, slope, up_offset, tile, split,
-              num_sms(x.device), err.data_ptr(), _stream_at(x))
+    behind = (*w._held, starts.data_ptr() if starts is not None else 0,
+              row_w.data_ptr() if row_w is not None else 0, out.data_ptr(), out.stride(0), out_type, M, features, K,
+              w.experts or 1, w.gated, GATE_ACTIVATIONS[activation] if w.gated else 0, limit, slope, up_offset,
+              tile, split, num_sms(device), err.data_ptr(), _stream_at(x))
     global _launches
-    if M <= 32 and starts is None and FP8_RESIDENT:
-        # few rows: one kernel, where it takes the sizes
-        p = _profiler
-        if p is not None:
-            p.begin(what)
+    p = _profiler
+    if p is not None:
+        p.begin(what)
+    # (few rows: one kernel, where it takes the sizes)
+    code = -1
+    if M <= 8 and starts is None and FP8_RESIDENT:
         code = _fp8_product_call(x.data_ptr(), x.stride(0), 0, 0, 0, 0, *behind)
-        if p is not None:
-            p.end(what)
-        if code != -1:
-            _check(code, what)
-            return
-    # the rows' codes and behind them their scales
-    pitch = -(-K // 16) * 16
-    scratch = torch.empty(M * pitch + 4 * -(-K // FP8_GROUP) * M, dtype=torch.uint8, device=x.device)
-    at = scratch.data_ptr()
-    _run(what, _fp8_product_call, x.data_ptr(), x.stride(0), at, pitch, at + M * pitch, M, *behind)
-    _launches += 1          # two kernels
+    if code == -1:
+        # the rows' codes and behind them their scales
+        pitch = -(-K // 16) * 16
+        scratch = torch.empty(M * pitch + 4 * -(-K // FP8_GROUP) * M, dtype=torch.uint8, device=device)
+        at = scratch.data_ptr()
+        code = _fp8_product_call(x.data_ptr(), x.stride(0), at, pitch, at + M * pitch, M, *behind)
+        _launches += 1          # two kernels
+    if p is not None:
+        p.end(what)
+    _check(code, what)
 
 
 def fp8_linear(x: torch.Tensor, w: Fp8Weight, out: torch.Tensor, activation: str = "silu",
