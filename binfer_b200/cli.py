@@ -25,7 +25,7 @@ VALUE_FLAGS = {
     "--top-k", "--top-p", "-i", "--input", "-o", "--output",
     # additions of this engine
     "--prompt-ids", "--seed", "--repetition-penalty", "--random-weights", "--kv-memory-gb",
-    "--kv-pages", "--kv-cache", "--page-size", "--max-tokens-per-step", "--max-seq-len", "--max-batch-size",
+    "--kv-pages", "--kv-cache", "--weights", "--page-size", "--max-tokens-per-step", "--max-seq-len", "--max-batch-size",
 }
 BOOL_FLAGS = {
     "--chat", "--bench", "--profile", "--no-cache", "-q", "--quiet", "--help", "-h",
@@ -67,6 +67,7 @@ Options:
                            after loading, at most max-batch-size x max-seq-len tokens)
   --kv-pages <n>           Size of the cache in pages instead
   --kv-cache <auto|int4>   Keys and values as the activations (default), or in 4 bits
+  --weights <auto|fp8>     The layers' matrices as the activations (default), or in 8 bits
   --page-size <n>          Tokens per cache page (default: 16)
   --max-tokens-per-step <n>  Token budget of one step (default: 2048)
   --max-seq-len <n>        Longest sequence (default: 4096)
@@ -115,7 +116,7 @@ def parse_args(argv: List[str]) -> dict:
              bench=False, profile=False, trace=None, quiet=False, verbose=False, cuda_graphs=True,
              temperature=0.0, top_k=0, top_p=1.0, repetition_penalty=1.0, seed=None,
              ignore_eos=False, input=None, output=None, use_template=False, random_weights=None,
-             kv_memory_gb=None, kv_pages=None, kv_cache="auto", allow_unexpected_tensors=False, page_size=16, max_tokens_per_step=2048,
+             kv_memory_gb=None, kv_pages=None, kv_cache="auto", weights="auto", allow_unexpected_tensors=False, page_size=16, max_tokens_per_step=2048,
              max_seq_len=4096, max_batch_size=64)
     names = {"--max-tokens": ("max_tokens", int), "--tp": ("tp", str), "--dtype": ("dtype", str),
              "-p": ("prompt", str), "--prompt": ("prompt", str), "--prompt-ids": ("prompt", str),
@@ -125,7 +126,7 @@ def parse_args(argv: List[str]) -> dict:
              "-o": ("output", str), "--output": ("output", str), "--seed": ("seed", int),
              "--repetition-penalty": ("repetition_penalty", float),
              "--random-weights": ("random_weights", int), "--kv-memory-gb": ("kv_memory_gb", float),
-             "--kv-pages": ("kv_pages", int), "--kv-cache": ("kv_cache", str), "--page-size": ("page_size", int),
+             "--kv-pages": ("kv_pages", int), "--kv-cache": ("kv_cache", str), "--weights": ("weights", str), "--page-size": ("page_size", int),
              "--max-tokens-per-step": ("max_tokens_per_step", int),
              "--max-seq-len": ("max_seq_len", int), "--max-batch-size": ("max_batch_size", int)}
     flags = {"--chat": "chat", "--bench": "bench", "--profile": "profile", "-q": "quiet",
@@ -235,7 +236,7 @@ def main(argv: Optional[List[str]] = None) -> int:
     log(f"Loading {args['model']} ...")
     model = args["model"]
     kw = dict(dtype=args["dtype"], max_kv_memory_gb=args["kv_memory_gb"],
-              num_pages=args["kv_pages"], kv_cache=args["kv_cache"], page_size=args["page_size"],
+              num_pages=args["kv_pages"], kv_cache=args["kv_cache"], weights=args["weights"], page_size=args["page_size"],
               max_seq_len=args["max_seq_len"], max_batch_size=args["max_batch_size"],
               max_tokens_per_step=args["max_tokens_per_step"],
               cuda_graphs=args["cuda_graphs"] and not args["profile"] and not args["trace"])

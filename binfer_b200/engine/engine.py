@@ -34,7 +34,8 @@ class Engine:
                  page_size: int = 16, max_seq_len: int = 4096, max_batch_size: int = 64,
                  max_tokens_per_step: int = 2048, cuda_graphs: bool = True,
                  look_ahead: bool = True, device: str = "cuda:0",
-                 allow_unexpected_tensors: bool = False, kv_cache: str = "auto"):
+                 allow_unexpected_tensors: bool = False, kv_cache: str = "auto",
+                 weights: str = "auto"):
         """``model``: a folder with config.json and safetensors, or (with
         ``random_seed``) a typed configuration whose weights are drawn on the device.
 
@@ -44,8 +45,11 @@ class Engine:
         ``max_batch_size`` requests of ``max_seq_len`` tokens can use.
 
         ``kv_cache``: ``auto`` or ``int4`` (keys and values in 4 bits: 4.5 with their scales, so
-        that 3.5 times as many tokens fit; see ``make_env``)."""
-        self.env = make_env(dtype, device, kv_cache)
+        that 3.5 times as many tokens fit; see ``make_env``).
+
+        ``weights``: ``auto`` or ``fp8`` (the layers' matrices in 8 bits: half of the memory, and a decode step
+        reads half of the bytes; see ``make_env``).  The embedding and the output head stay as they are."""
+        self.env = make_env(dtype, device, kv_cache, weights)
         if isinstance(model, str):
             self.config = load_config(model)
             self.model = model_from_dir(model, self.env,

@@ -37,10 +37,17 @@ def parse_dtype(name: Union[str, torch.dtype]) -> torch.dtype:
 
 
 def make_env(dtype: Union[str, torch.dtype], device: Union[str, torch.device] = "cuda:0",
-             kv_cache: str = "auto") -> BuildEnv:
+             kv_cache: str = "auto", weights: str = "auto") -> BuildEnv:
     """``kv_cache``: ``auto`` (keys and values as the activations) or ``int4`` (in 4 bits, 4.5 with
-    their scales: bfloat16 engines whose paged layers are plain grouped attention)."""
+    their scales: bfloat16 engines whose paged layers are plain grouped attention).  ``weights``:
+    ``auto`` (matrices as the activations) or ``fp8`` (the layers' matrices in 8 bits with a scale for
+    each block of 128 x 128, their inputs in 8 bits within the products: bfloat16 engines of pre-norm
+    layers of grouped attention and dense feed-forwards)."""
     device = torch.device(device)
+    if weights not in ("auto", "fp8"):
+        raise ValueError(f"unknown weights {weights!r} (auto or fp8)")
+    if weights == "fp8" and parse_dtype(dtype) != torch.bfloat16:
+        raise ValueError("weights in 8 bits take a bfloat16 engine")
     if kv_cache not in ("auto", "int4"):
         raise ValueError(f"unknown kv_cache {kv_cache!r} (auto or int4)")
     if kv_cache == "int4" and parse_dtype(dtype) != torch.bfloat16:
@@ -50,7 +57,7 @@ def make_env(dtype: Union[str, torch.dtype], device: Union[str, torch.device] = 
     if not torch.cuda.is_available():
         raise RuntimeError("no CUDA device is available; the engine has no CPU path")
     torch.cuda.set_device(device)
-    return BuildEnv(parse_dtype(dtype), device, kv_cache)
+    return BuildEnv(parse_dtype(dtype), device, kv_cache, weights)
 
 
 def model_from_dir(model_dir: str, env: BuildEnv, allow_unexpected: bool = False) -> DecoderModel:

@@ -63,6 +63,7 @@ class GQAAttention(Mixer):
                 raise ValueError("score.slopes needs one slope per query head")
             self.slopes = torch.tensor(spec.score.slopes, dtype=torch.float32, device=env.device)
         self._qkv_plans = {}
+        self.eight_bits = env.weights == "fp8"        # (the projections' weights)
         # keys and values in 4 bits
         self.four_bits = env.kv_cache == "int4"
         if self.four_bits and (spec.score is not None or not ops.kv4_takes(env.dtype, spec.head_dim, 16)):
@@ -91,6 +92,8 @@ class GQAAttention(Mixer):
         self.w_qkv = torch.cat([get(sp["q_proj.weight"]), get(sp["k_proj.weight"]),
                                 get(sp["v_proj.weight"])], dim=0).contiguous()
         self.w_o = get(sp["o_proj.weight"])
+        if self.eight_bits:
+            self.w_qkv, self.w_o = ops.fp8_weight(self.w_qkv), ops.fp8_weight(self.w_o)
         if self.spec.qk_norm:
             self.q_norm = get(sp["q_norm.weight"])
             self.k_norm = get(sp["k_norm.weight"])
@@ -98,6 +101,15 @@ class GQAAttention(Mixer):
             self.sinks = get(sp["sinks"])
         if self.position is not None:
             self.position.load(get)
+
+    holds_eight_bits = True
+
+    def _w_q(self):
+        """The rows of the stacked weight that make the queries."""
+        w, n = self.w_qkv, self.q_size
+        if not self.eight_bits:
+            return w[:n]
+        return ops.Fp8Weight(w.codes[:n], w.scales[:-(-n // ops.FP8_GROUP)])
 
     # ------------------------------------------------------------------- cache
     def kv_need(self) -> Optional[KVNeed]:
@@ -120,7 +132,7 @@ class GQAAttention(Mixer):
         pos = self.position
         q = torch.empty((T, self.q_size), dtype=x.dtype, device=x.device)
         # the pages may belong to another layer execution: only q is needed then
-        w = self.w_qkv if view.writes_cache else self.w_qkv[: self.q_size]
+        w = self.w_qkv if view.writes_cache else self._w_q()
         if not self._project_fused(x, w, q, row_scale, ctx, view):
             qkv = linear(x, w)
             if self.four_bits and view.writes_cache:
@@ -145,7 +157,7 @@ class GQAAttention(Mixer):
         store into the pages as one kernel, where the split-K cluster product has a plan with
         tiles of whole heads for this shape.  False, having done nothing, otherwise."""
         s, pos = self.spec, self.position
-        if (not FUSE_QKV or self.four_bits or x.dtype != torch.bfloat16 or x.shape[0] > cluster_token_limit()
+        if (not FUSE_QKV or self.four_bits or self.eight_bits or x.dtype != torch.bfloat16 or x.shape[0] > cluster_token_limit()
                 or (pos is not None and pos.inv_freq is None)):
             return False
         key = (w.shape[0], w.shape[1])

@@ -27,6 +27,7 @@ class BuildEnv:
     dtype: torch.dtype            # activations, matrices and cache pages
     device: torch.device
     kv_cache: str = "auto"        # "int4": keys and values held in 4 bits (KVNeed.four_bits)
+    weights: str = "auto"         # "fp8": layers' matrices held in 8 bits (Part.holds_eight_bits)
 
 
 @dataclass
@@ -73,6 +74,9 @@ class StepContext:
 
 class Part:
     """Base of every part: tensors it needs, and how it takes them."""
+
+    # whether the part's matrices can be held in 8 bits (``BuildEnv.weights`` "fp8"), which it then does
+    holds_eight_bits = False
 
     def param_specs(self) -> List[ParamSpec]:
         return []

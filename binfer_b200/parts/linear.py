@@ -142,8 +142,13 @@ _plans = {}
 def linear(x: torch.Tensor, w: torch.Tensor, out: Optional[torch.Tensor] = None,
            out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``x [M, K] @ w [N, K]^T -> [M, N]``; ``out_dtype`` float32 keeps a bfloat16
-    product's accumulator precision (used for the logits)."""
+    product's accumulator precision (used for the logits).  ``w`` may be held in 8 bits."""
     M, N = x.shape[0], w.shape[0]
+    if isinstance(w, ops.Fp8Weight):
+        if out is None:
+            out = torch.empty((M, N), dtype=out_dtype or x.dtype, device=x.device)
+        ops.fp8_linear(x, w, out)
+        return out
     if x.dtype == torch.float32:
         if out is None:
             out = torch.empty((M, N), dtype=torch.float32, device=x.device)
@@ -198,8 +203,8 @@ def linear_add_norm(x: torch.Tensor, w: torch.Tensor, resid: torch.Tensor,
     ``rsqrt(mean(resid^2) + eps)`` per row, or None, having done nothing, where the cluster
     kernel does not run (float32, more than 32 tokens, shapes without a plan)."""
     M, (N, K) = x.shape[0], w.shape
-    if (not FUSE_NORM or x.dtype != torch.bfloat16 or w.dtype != torch.bfloat16
-            or not _use_cluster(M, N, K)):
+    if (not FUSE_NORM or isinstance(w, ops.Fp8Weight) or x.dtype != torch.bfloat16
+            or w.dtype != torch.bfloat16 or not _use_cluster(M, N, K)):
         return None
     plan = _plans.get((N, K))
     if plan is None:

@@ -47,6 +47,9 @@ class GatedMLP(FeedForward, StackedOut):
         self.w_gate_up = self.w_out = None
         self.b_gate_up = self.out_bias = None   # float32, with GatedMLPSpec.bias
         self._swiglu_plan = None
+        # the three matrices in 8 bits; the products in that form take no biases
+        self.holds_eight_bits = self.fusable and not spec.bias
+        self.eight_bits = env.weights == "fp8" and self.holds_eight_bits
 
     def param_specs(self) -> List[ParamSpec]:
         p = self.prefix
@@ -64,6 +67,8 @@ class GatedMLP(FeedForward, StackedOut):
         g, u, d, *biases = self.param_specs()
         self.w_gate_up = torch.cat([get(g), get(u)], dim=0).contiguous()
         self.w_out = get(d)
+        if self.eight_bits:
+            self.w_gate_up, self.w_out = ops.fp8_weight(self.w_gate_up, gated=True), ops.fp8_weight(self.w_out)
         if biases:
             bg, bu, bd = (get(b) for b in biases)
             self.b_gate_up, self.out_bias = torch.cat([bg, bu]).contiguous(), bd
@@ -76,7 +81,7 @@ class GatedMLP(FeedForward, StackedOut):
     def forward_deferred(self, x, ctx: StepContext) -> DeferredLinear:
         """Everything but the down projection (see ``GQAAttention.forward_deferred``)."""
         if isinstance(x, ScaledRows) and (self.inter % 8 or self.inter < 256 or not self.silu
-                                          or self.spec.bias):
+                                          or self.spec.bias or self.eight_bits):
             x = x.dense()                  # the activation kernel takes the factor at other sizes only
         x, row_scale = split_scaled(x)
         h = torch.empty((x.shape[0], self.inter), dtype=x.dtype, device=x.device)
@@ -89,6 +94,9 @@ class GatedMLP(FeedForward, StackedOut):
 
     def _inner(self, x, h, row_scale) -> None:
         """Gate, up and activation into ``h`` (which may be a column block of a wider buffer)."""
+        if self.eight_bits:
+            ops.fp8_linear(x, self.w_gate_up, h, **self._act)
+            return
         if self._project_fused(x, h, row_scale):
             return
         gu = linear(x, self.w_gate_up)

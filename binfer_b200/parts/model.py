@@ -51,6 +51,12 @@ class DecoderModel:
         names = spec.names
         self.blocks = [build_block(ls, spec.hidden_size, names, i, env)
                        for i, ls in enumerate(spec.layers)]
+        if env.weights == "fp8":
+            for i, b in enumerate(self.blocks):
+                odd = [b] if type(b) is not _block.PreNormBlock else [
+                    p for p in (b.mixer, b.ffn) if p is not None and not p.holds_eight_bits]
+                if odd:
+                    raise ValueError(f"layer {i}: {type(odd[0]).__name__} does not hold its weights in 8 bits")
         self.final_norm = build_norm(spec.final_norm, spec.hidden_size, names.final_norm, env)
         self.embed_spec = ParamSpec(names.embed, (spec.vocab_size, spec.hidden_size))
         self.head_spec = (None if spec.tie_word_embeddings
@@ -136,7 +142,8 @@ class DecoderModel:
         seen, total = set(), 0
         for obj in [self] + self.blocks + [self.final_norm] + \
                 [p for b in self.blocks for p in (b.parts() if hasattr(b, "parts") else [])]:
-            for v in vars(obj).values():
+            held = [v for v in vars(obj).values() if isinstance(v, ops.Fp8Weight)]
+            for v in (*vars(obj).values(), *(t for w in held for t in (w.codes, w.scales))):
                 # (by storage: a part's weight may be a column block of a stacked one)
                 if isinstance(v, torch.Tensor) and v.untyped_storage().data_ptr() not in seen:
                     seen.add(v.untyped_storage().data_ptr())
