@@ -83,6 +83,74 @@ fp8_rows_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ co
   }
 }
 
+// A block a row: resid (+= delta), RMSNorm, rounding to bfloat16, into 8 bits; eight numbers a thread and
+// trip, sixteen threads a group.  The sums have the order of the norm's own kernel: the codes are those of
+// its output.
+template <int TRIPS>
+__global__ void add_rmsnorm_fp8_kernel(float* __restrict__ resid, const __nv_bfloat16* __restrict__ delta,
+                                       const float* __restrict__ w, uint8_t* __restrict__ codes, long long ldc,
+                                       float* __restrict__ scales, long long lds, int H, float eps) {
+  __shared__ float scratch[33];
+  bf_pdl_trigger();
+  bf_pdl_wait();
+  const int r = blockIdx.x;
+  float* x = resid + (size_t)r * H;
+  const __nv_bfloat16* d = delta ? delta + (size_t)r * H : nullptr;
+  float v[TRIPS][8];
+  float ss = 0.f;
+#pragma unroll
+  for (int k = 0; k < TRIPS; ++k) {
+    const int c = (k * blockDim.x + threadIdx.x) * 8;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[k][j] = 0.f;
+    if (c < H) {
+      const float4 a = *reinterpret_cast<const float4*>(x + c);
+      const float4 b = *reinterpret_cast<const float4*>(x + c + 4);
+      v[k][0] = a.x; v[k][1] = a.y; v[k][2] = a.z; v[k][3] = a.w;
+      v[k][4] = b.x; v[k][5] = b.y; v[k][6] = b.z; v[k][7] = b.w;
+      if (d) {
+        const uint4 q = *reinterpret_cast<const uint4*>(d + c);
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&q);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = __bfloat1622float2(h[j]);
+          v[k][2 * j] += f.x;
+          v[k][2 * j + 1] += f.y;
+        }
+        *reinterpret_cast<float4*>(x + c) = make_float4(v[k][0], v[k][1], v[k][2], v[k][3]);
+        *reinterpret_cast<float4*>(x + c + 4) = make_float4(v[k][4], v[k][5], v[k][6], v[k][7]);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss += v[k][j] * v[k][j];
+    }
+  }
+  ss = block_sum(ss, scratch);
+  const float inv = rsqrtf(ss / (float)H + eps);
+#pragma unroll
+  for (int k = 0; k < TRIPS; ++k) {
+    const int c = (k * blockDim.x + threadIdx.x) * 8;
+    uint32_t m = 0u;
+    if (c < H) {
+      const float4 wa = *reinterpret_cast<const float4*>(w + c);
+      const float4 wb = *reinterpret_cast<const float4*>(w + c + 4);
+      const float f[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[k][j] = __bfloat162float(__float2bfloat16_rn(v[k][j] * inv * f[j]));
+        m = max(m, __float_as_uint(v[k][j]) & 0x7fffffffu);
+      }
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const Fp8Scale s = fp8_scale(m);
+    if (c < H) {
+      *reinterpret_cast<uint2*>(codes + r * ldc + c) =
+          make_uint2(fp8_codes4(v[k], s), fp8_codes4(v[k] + 4, s));
+      if ((threadIdx.x & 15) == 0) scales[(long long)(c / BF_FP8_GROUP) * lds + r] = s.s;
+    }
+  }
+}
+
 // Sixteen lanes a group.  blockIdx.z: the matrix, of mat_rows rows.  BLOCKS: a scale per 128 rows of it and group, [blocks,
 // groups]; else one per row and group, [groups, lds].
 constexpr int F8_READ_PLACES = F8_THREADS / 16;
@@ -289,6 +357,36 @@ BF_EXPORT int bf_fp8_read(const Fp8ReadCall* call) {
                 : go(fp8_read_kernel<__nv_bfloat16, false>, (__nv_bfloat16*)out);
 }
 
+// resid [rows, H] += delta (bfloat16, or null); its RMSNorm times w, rounded to bfloat16, as codes [rows, ldc
+// bytes] and scales [ceil(H / 128), lds].  H: a multiple of 8, at most 8,192; everything on 16-byte boundaries.
+struct AddRmsnormFp8Call {
+  float* resid;
+  const void* delta;
+  const float* w;
+  void* codes;
+  long long ldc;
+  float* scales;
+  long long lds;
+  int rows, H;
+  float eps;
+  cudaStream_t stream;
+};
+BF_EXPORT int bf_add_rmsnorm_fp8(const AddRmsnormFp8Call* call) {
+  const AddRmsnormFp8Call& c = *call;
+  if (c.rows <= 0) return 0;
+  if (c.H % 8 || c.H <= 0 || c.H > 8 * 256 * 4 || c.ldc % 16 ||
+      (((uintptr_t)c.resid | (uintptr_t)c.delta | (uintptr_t)c.w | (uintptr_t)c.codes) & 15))
+    return (int)cudaErrorInvalidValue;
+  const int threads = c.H >= 2048 ? 256 : 128, trips = (c.H / 8 + threads - 1) / threads;
+  auto go = [&](auto kern) {
+    return bf_launch_pdl(kern, dim3(c.rows), dim3(threads), 0, c.stream, c.resid, (const __nv_bfloat16*)c.delta,
+                         c.w, (uint8_t*)c.codes, c.ldc, c.scales, c.lds, c.H, c.eps);
+  };
+  if (trips <= 1) return go(add_rmsnorm_fp8_kernel<1>);
+  if (trips == 2) return go(add_rmsnorm_fp8_kernel<2>);
+  return go(add_rmsnorm_fp8_kernel<4>);
+}
+
 extern "C" int bf_gemm_fp8_few(const void*, long long, const float*, long long, const void*, long long,
                                const float*, const int*, const float*, void*, long long, int, int, int, int,
                                int, int, int, float, float, float, int, int, int, int, int*, cudaStream_t);
@@ -322,7 +420,7 @@ static int fp8_split(int rows, int features, int K, bool gated, int nb, int num_
 }
 
 struct Fp8ProductCall {
-  const void* x;               // bfloat16 [rows, K]
+  const void* x;               // bfloat16 [rows, K], or null: codes and scales hold the rows
   long long ldx;
   void* codes;                 // scratch for the rows' codes and scales
   long long ldc;
@@ -350,7 +448,7 @@ BF_EXPORT int bf_fp8_product(const Fp8ProductCall* call) {
   const int split = c.starts || tile < 0 ? 1
                     : c.split ? c.split
                               : fp8_split(c.rows, c.features, c.K, c.gated != 0, tile, c.num_sms);
-  if (!c.codes) {
+  if (c.x && !c.codes) {
     // asked for without scratch: the rows stay in the CTAs that read them, where they fit
     if (tile != 16 || c.starts) return -1;
     return bf_gemm_fp8_few(c.x, c.ldx, nullptr, 0, c.w, c.ldw, c.sw, c.starts, c.row_w, c.out, c.ldo, c.out_dtype,
@@ -359,7 +457,7 @@ BF_EXPORT int bf_fp8_product(const Fp8ProductCall* call) {
   }
   const Fp8RowsCall rows = {c.x, c.ldx, c.codes, c.ldc, c.scales, c.lds, BF_DTYPE_BF16, c.rows, c.K, c.num_sms,
                             c.stream};
-  const int e = bf_fp8_rows(&rows);
+  const int e = c.x ? bf_fp8_rows(&rows) : 0;
   if (e) return e;
   if (tile < 0)
     return bf_gemm_fp8_pair(c.codes, c.ldc, c.scales, c.lds, c.w, c.ldw, c.sw, c.starts, c.row_w, c.out, c.ldo,

@@ -134,6 +134,12 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
     }
     for (int r = 0; RESIDENT && r * per_round < g1 - g0; ++r) mbar_init(ready + r, 8);
     mbar_init(drain, 1);
+    if (!p.starts) {                           // (all rows are one expert's: nothing of the stream to wait for)
+      tables.first[0] = 0;
+      tables.end[0] = p.rows;
+      tables.before[0] = 0;
+      tables.before[1] = (p.rows + NB - 1) / NB;
+    }
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -170,8 +176,10 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   __syncwarp();
   bf_pdl_wait();
   if (p.split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  fill_row_tables(tables, p.starts, p.experts, p.rows, NB);
-  __syncthreads();
+  if (p.starts) {
+    fill_row_tables(tables, p.starts, p.experts, p.rows, NB);
+    __syncthreads();
+  }
   const int units = tables.before[p.experts] * p.tiles_f;
 
   int stage = 0;                                 // of this role, with its phase
@@ -206,13 +214,16 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
     const uint32_t elected = elect_one();
     int slot = 0;
     uint32_t slot_phase = 0;
-    bool ok = true, seen_empty = false, seen_full = false;       // looks at the next group's barriers
+    bool ok = true, seen_empty = true, seen_full = false;        // looks at the next group's barriers
+    int slots_left = SLOTS;                                      // never used so far: nothing to wait for
+    const int tiles_mine = cluster < units ? (units - cluster + clusters - 1) / clusters : 0;
+    int refills = tiles_mine * (g1 - g0) - STAGES;               // stages that will be filled again
     for (int u = cluster; u < units && ok; u += clusters) {
       const RowTile t = row_tile(tables, p.experts, p.tiles_f, NB, u);
       const int n = min(NB, (t.row_end - t.row0 + 15) & ~15);
       const uint32_t idesc = fp8_idesc(128, n);
       for (int g = g0; g < g1; ++g) {
-        if (!mbar_seen_or_wait_warp(seen_empty, acc_empty + slot, slot_phase ^ 1, abort) ||
+        if (!mbar_seen_or_wait_warp(slots_left > 0 || seen_empty, acc_empty + slot, slot_phase ^ 1, abort) ||
             !mbar_seen_or_wait_warp(seen_full, full + stage, phase, abort) ||
             (RESIDENT && !mbar_wait_warp(ready + (g - g0) / per_round, 0, abort))) {
           ok = false;
@@ -235,13 +246,13 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
           slot = 0;
           slot_phase ^= 1;
         }
-        seen_empty = mbar_look(acc_empty + slot, slot_phase ^ 1);
+        if (--slots_left <= 0) seen_empty = mbar_look(acc_empty + slot, slot_phase ^ 1);
         seen_full = mbar_look(full + stage, phase);
 #pragma unroll
         for (int k = 0; k < FK / 32; ++k)
           umma_fp8(d_tmem, a_desc + (uint64_t)(2 * k), b_desc + (uint64_t)(2 * k), idesc, k > 0 ? 1u : 0u, elected);
-        umma_commit_by(done_stage, elected);
         umma_commit_by(done_slot, elected);
+        if (refills-- > 0) umma_commit_by(done_stage, elected);
       }
     }
   } else if (warp == 2) {
@@ -250,7 +261,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
     // a load takes longer than a group's products.
     constexpr int PER = (NB + 31) / 32;          // columns a lane looks after
     constexpr int AHEAD = NB <= 32 ? 8 : 4;
-    int slot = 0;
+    int slot = 0, slots_left = SLOTS;
     uint32_t slot_phase = 0;
     bool ok = true;
     float sx[AHEAD][PER], sw[AHEAD][HALVES];
@@ -297,7 +308,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
           if (ga + i >= g1 || !ok) break;
-          if (!mbar_wait_warp(acc_empty + slot, slot_phase ^ 1, abort)) {
+          if (--slots_left < 0 && !mbar_wait_warp(acc_empty + slot, slot_phase ^ 1, abort)) {
             ok = false;
             break;
           }

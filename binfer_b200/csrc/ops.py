@@ -9,7 +9,7 @@ from __future__ import annotations
 import ctypes
 import os
 import struct
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -2840,6 +2840,7 @@ E4M3 = torch.float8_e4m3fn
 
 _fp8_rows_call = _Packed("bf_fp8_rows", "PqPqPqiiiiP")
 _fp8_blocks_call = _Packed("bf_fp8_blocks", "PqPqPiiiiP")
+_add_rmsnorm_fp8_call = _Packed("bf_add_rmsnorm_fp8", "PPPPqPqiifP")
 _fp8_read_call = _Packed("bf_fp8_read", "PqPqPqiiiiiiP")
 _fp8_product_call = _Packed("bf_fp8_product", "PqPqPqPqPPPPqiiiiiiifffiiiPP")
 
@@ -2884,7 +2885,26 @@ def _fp8_codes_lie(codes: torch.Tensor) -> bool:
             and codes.data_ptr() % 16 == 0 and _fp8_stacked(codes))
 
 
-def fp8_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+class Fp8Rows(NamedTuple):
+    """Rows in 8 bits, as :func:`fp8_rows` makes them; products with an :class:`Fp8Weight` take them in place of
+    the bfloat16 rows that they stand for."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    @property
+    def shape(self):
+        return self.codes.shape
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    @property
+    def dtype(self):
+        return torch.bfloat16          # (of the rows that they stand for)
+
+
+def fp8_rows(x: torch.Tensor) -> Fp8Rows:
     """Rows ``x [T, K]`` (bfloat16 or float32) in 8 bits: ``(codes float8_e4m3fn [T, K], scales float32
     [ceil(K / 128), T])``.  The 128 numbers of columns 128 g .. 128 g + 127 of row t share the scale
     ``s = max(float32(a / 448), 2^-100)``, a the largest size among them, and a number's code is the
@@ -2899,7 +2919,38 @@ def fp8_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     if T:
         _run("fp8_rows", _fp8_rows_call, x.data_ptr(), x.stride(0), codes.data_ptr(), -(-K // 16) * 16,
              scales.data_ptr(), T, dtype, T, K, num_sms(device), _stream_at(x))
-    return codes, scales
+    return Fp8Rows(codes, scales)
+
+
+def add_rmsnorm_fp8_takes(width: int) -> bool:
+    """Whether :func:`add_rmsnorm_fp8` takes rows of this width."""
+    return width % 8 == 0 and 0 < width <= 8192
+
+
+def add_rmsnorm_fp8(resid: torch.Tensor, delta: Optional[torch.Tensor], weight: torch.Tensor,
+                    eps: float) -> Fp8Rows:
+    """``resid += delta`` and the rows of :func:`add_rmsnorm`'s bfloat16 output in 8 bits, as one kernel: the
+    same codes and scales that :func:`fp8_rows` makes of it."""
+    what = "add_rmsnorm_fp8"
+    _want(resid, torch.float32, "resid"); _want(weight, torch.float32, "weight")
+    if resid.dim() != 2 or weight.numel() != resid.shape[1] or not add_rmsnorm_fp8_takes(resid.shape[1]):
+        raise KernelError(f"{what}: resid must be [T, H] and weight [H], H a multiple of 8 of at most 8,192")
+    if delta is not None:
+        _want(delta, torch.bfloat16, "delta")
+        if delta.shape != resid.shape:
+            raise KernelError(f"{what}: delta must have the stream's shape")
+    for t in (resid, delta, weight):
+        if t is not None and t.data_ptr() % 16:
+            raise KernelError(f"{what}: the tensors must lie on 16-byte boundaries")
+    _same_device(what, resid, delta, weight)
+    (T, H), device = resid.shape, resid.device
+    codes = _fp8_empty_codes((T, H), device)
+    scales = torch.empty((-(-H // FP8_GROUP), T), dtype=torch.float32, device=device)
+    if T:
+        _run(what, _add_rmsnorm_fp8_call, resid.data_ptr(), delta.data_ptr() if delta is not None else 0,
+             weight.data_ptr(), codes.data_ptr(), codes.stride(0), scales.data_ptr(), T, T, H, eps,
+             _stream_at(resid))
+    return Fp8Rows(codes, scales)
 
 
 def fp8_rows_read(codes: torch.Tensor, scales: torch.Tensor, out: torch.Tensor) -> None:
@@ -2989,7 +3040,15 @@ def _fp8_product(what: str, x, w: Fp8Weight, starts, out, row_w, activation, lim
                  split) -> None:
     shape, out_shape, K, features = x.shape, out.shape, w.K, w.features
     M = shape[0] if len(shape) == 2 else -1
-    if x.dtype != torch.bfloat16 or M < 0 or shape[1] != K or (M and K > 1 and x.stride(1) != 1):
+    held = isinstance(x, Fp8Rows)
+    if held:
+        codes, scales = x
+        if (codes.dtype != E4M3 or M < 0 or shape[1] != K or (M and not _fp8_codes_lie(codes))
+                or scales.dtype != torch.float32 or scales.shape != (-(-K // FP8_GROUP), M)
+                or (M > 1 and scales.stride(1) != 1)):
+            raise KernelError(f"{what}: rows in 8 bits must be [rows, {K}] as fp8_rows makes them, got {codes.dtype} "
+                              f"{tuple(shape)} and scales {tuple(scales.shape)}")
+    elif x.dtype != torch.bfloat16 or M < 0 or shape[1] != K or (M and K > 1 and x.stride(1) != 1):
         raise KernelError(f"{what}: x must be bfloat16 [rows, {K}] with contiguous rows, got {x.dtype} "
                           f"{tuple(shape)}")
     out_type = _FP8_DTYPES.get(out.dtype)
@@ -3007,22 +3066,24 @@ def _fp8_product(what: str, x, w: Fp8Weight, starts, out, row_w, activation, lim
         raise KernelError(f"{what}: no tiles of {tile} rows, shared by {split}")
     device = x.device
     err = error_word(device)
-    _same_device(what, x, w.codes, w.scales, starts, out, row_w, err)
+    _same_device(what, *(x if held else (x,)), w.codes, w.scales, starts, out, row_w, err)
     if M == 0:
         return
     behind = (*w._held, starts.data_ptr() if starts is not None else 0,
               row_w.data_ptr() if row_w is not None else 0, out.data_ptr(), out.stride(0), out_type, M, features, K,
               w.experts or 1, w.gated, GATE_ACTIVATIONS[activation] if w.gated else 0, limit, slope, up_offset,
-              tile, split, num_sms(device), err.data_ptr(), _stream_at(x))
+              tile, split, num_sms(device), err.data_ptr(), _stream_at(out))
     global _launches
     p = _profiler
     if p is not None:
         p.begin(what)
     # (few rows: one kernel, where it takes the sizes)
     code = -1
-    if M <= 8 and starts is None and FP8_RESIDENT:
+    if held:
+        code = _fp8_product_call(0, 0, codes.data_ptr(), codes.stride(0), scales.data_ptr(), scales.stride(0), *behind)
+    elif M <= 8 and starts is None and FP8_RESIDENT:
         code = _fp8_product_call(x.data_ptr(), x.stride(0), 0, 0, 0, 0, *behind)
-    if code == -1:
+    if code == -1 and not held:
         # the rows' codes and behind them their scales
         pitch = -(-K // 16) * 16
         scratch = torch.empty(M * pitch + 4 * -(-K // FP8_GROUP) * M, dtype=torch.uint8, device=device)
@@ -3038,7 +3099,7 @@ def fp8_linear(x: torch.Tensor, w: Fp8Weight, out: torch.Tensor, activation: str
                limit: float = 0.0, slope: float = 1.0, up_offset: float = 0.0, tile: int = 0,
                split: int = 0) -> None:
     """``out [M, N] = x [M, K] w^T`` for rows in bfloat16 and a weight in 8 bits: the rows go into 8 bits as
-    :func:`fp8_rows` puts them, the products of codes are added up in float and counted with their scales, 128
+    :func:`fp8_rows` puts them (or are there already: ``x`` an :class:`Fp8Rows`), the products of codes are added up in float and counted with their scales, 128
     columns after another.  A gated weight: ``out = act(g) u`` of the product's two halves, ``activation`` as
     in :func:`gated_act_mul` ("silu" or "clamped").  ``out``: bfloat16, or float32 for a weight that is not
     gated; it may be a column block of a wider buffer.  A row's result does not depend on the other rows'

@@ -50,7 +50,7 @@ class PreNormBlock(Part):
                 successor: Optional[Part] = None) -> None:
         """``successor``: the block that runs next on this stream, if any; its input norm
         can then be prepared by this block's last product."""
-        h = self._for(self.mixer, self.input_norm.forward(stream))
+        h = self._read(self.mixer, self.input_norm, stream)
         deferred = getattr(self.mixer, "forward_deferred", None)
         if self.ffn is None:
             if deferred is not None:
@@ -62,7 +62,7 @@ class PreNormBlock(Part):
             stream.add_linear(deferred(h, ctx, view), self.post_norm, self.ffn)
         else:
             stream.add(self.mixer.forward(h, ctx, view))
-        h = self._for(self.ffn, self.post_norm.forward(stream))
+        h = self._read(self.ffn, self.post_norm, stream)
         deferred = getattr(self.ffn, "forward_deferred", None)
         if deferred is not None:
             stream.add_linear(deferred(h, ctx), *self._reads_next(successor))
@@ -75,6 +75,13 @@ class PreNormBlock(Part):
         one part alone."""
         return (getattr(successor, "first_norm", None),
                 successor.mixer if isinstance(successor, PreNormBlock) else None)
+
+    @classmethod
+    def _read(cls, part, norm, stream: ResidualStream):
+        """``norm`` over the stream, as ``part`` can take it."""
+        if getattr(part, "eight_bits", False) and hasattr(norm, "forward_eight_bits"):
+            return cls._for(part, norm.forward_eight_bits(stream))
+        return cls._for(part, norm.forward(stream))
 
     @staticmethod
     def _for(part, h):

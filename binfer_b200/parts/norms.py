@@ -63,6 +63,18 @@ class RMSNorm(Norm):
         return out
 
 
+    def forward_eight_bits(self, stream: ResidualStream):
+        """:meth:`forward` of every row, in 8 bits (``ops.Fp8Rows``), for parts whose products take their rows
+        so; the bfloat16 rows themselves where the kernel does not take the width."""
+        if stream.ready_for is self or not ops.add_rmsnorm_fp8_takes(self.size):
+            return self.forward(stream)
+        if stream.pending2 is not None or stream.pending_bias is not None:
+            stream.flush()
+        stream.ready = stream.ready_for = None
+        out = ops.add_rmsnorm_fp8(stream.x, stream.pending, self.weight, self.eps)
+        stream.pending = None
+        return out
+
     def add_normed(self, stream: ResidualStream, y: torch.Tensor,
                    next_norm: Optional[Norm] = None) -> None:
         """``stream.x += y * rsqrt(mean(y^2) + eps) * w`` in one kernel, which also leaves the

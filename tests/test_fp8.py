@@ -149,3 +149,27 @@ def test_read_refuses(ops):
     w = ops.Fp8Weight(_codes(4, 32), torch.ones(1, 1))
     with pytest.raises(ops.KernelError, match="shape"):
         ops.fp8_weight_read(w, torch.zeros(4, 31))
+
+
+def test_rows_in_8_bits_refused(ops):
+    w, out = ops.Fp8Weight(_codes(300, 256), torch.ones(3, 2)), torch.zeros(2, 300, dtype=BF16)
+    for codes, scales in ((_codes(2, 256), torch.ones(2, 3)), (_codes(2, 256), torch.ones(2, 2, dtype=F64)),
+                          (_codes(2, 255), torch.ones(2, 2)), (_codes(2, 256).view(torch.uint8), torch.ones(2, 2)),
+                          (_codes(2, 512)[:, 1:257], torch.ones(2, 2)), (_codes(256, 2).t(), torch.ones(2, 2))):
+        with pytest.raises(ops.KernelError) as e:
+            ops.fp8_linear(ops.Fp8Rows(codes, scales), w, out)
+        assert "CUDA" not in str(e.value)
+
+
+def test_norm_into_8_bits_refuses(ops):
+    ok = dict(resid=torch.zeros(2, 64), delta=torch.zeros(2, 64, dtype=BF16), weight=torch.ones(64), eps=1e-6)
+    for change in (dict(resid=torch.zeros(2, 60), delta=None, weight=torch.ones(60)), dict(weight=torch.ones(32)),
+                   dict(delta=torch.zeros(2, 64)), dict(delta=torch.zeros(3, 64, dtype=BF16)),
+                   dict(resid=torch.zeros(2, 64, dtype=BF16)), dict(resid=torch.zeros(64)),
+                   dict(resid=torch.zeros(130)[1:129].view(2, 64)),
+                   dict(resid=torch.zeros(2, 8200), delta=None, weight=torch.ones(8200))):
+        with pytest.raises(ops.KernelError) as e:
+            ops.add_rmsnorm_fp8(**dict(ok, **change))
+        assert "CUDA" not in str(e.value)
+    with pytest.raises(ops.KernelError, match="CUDA"):
+        ops.add_rmsnorm_fp8(**ok)

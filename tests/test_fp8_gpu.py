@@ -404,3 +404,34 @@ def test_one_kernel_or_two(cuda_device, monkeypatch, M, K, N, gated):
             ops.fp8_linear(rows, w, out)
             outs.append(out)
         assert torch.equal(*outs)
+
+
+@pytest.mark.parametrize("T,H", [(1, 8), (3, 200), (8, 4096), (17, 2048), (300, 1000), (5, 8192)])
+def test_norm_into_8_bits(cuda_device, T, H):
+    """The codes and scales of the norm's bfloat16 output, and the stream as the norm leaves it."""
+    from binfer_b200.csrc import ops
+    g = torch.Generator(cuda_device).manual_seed(T + H)
+    w = 1 + 0.1 * torch.randn(H, generator=g, device=cuda_device)
+    for delta in (None, _x(T, H, cuda_device, 5)):
+        a = torch.randn((T, H), generator=g, device=cuda_device)
+        b, y = a.clone(), torch.empty((T, H), dtype=BF16, device=cuda_device)
+        ops.add_rmsnorm(a, delta, w, y, 1e-6)
+        rows = ops.add_rmsnorm_fp8(b, delta, w, 1e-6)
+        ref = ops.fp8_rows(y)
+        assert torch.equal(a, b) and torch.equal(rows.scales, ref.scales)
+        assert torch.equal(rows.codes.view(torch.uint8), ref.codes.view(torch.uint8))
+
+
+@pytest.mark.parametrize("M", [1, 8, 40, 300])
+def test_rows_that_are_there_already(cuda_device, M):
+    from binfer_b200.csrc import ops
+    for K in (384, 1000):
+        x, w = _x(M, K, cuda_device, M), ops.fp8_weight(_w((300, K), cuda_device))
+        e, starts = ops.fp8_weight(_w((2, 64, K), cuda_device)), torch.tensor([0, M // 2, M], dtype=torch.int32,
+                                                                              device=cuda_device)
+        rows = ops.fp8_rows(x)
+        for call in (lambda r, o: ops.fp8_linear(r, w, o[:, :300]), lambda r, o: ops.fp8_experts(r, e, starts, o[:, :64])):
+            a, b = (torch.zeros((M, 304), dtype=BF16, device=cuda_device) for _ in range(2))
+            call(x, a)
+            call(rows, b)
+            assert torch.equal(a, b) and a.any()
