@@ -206,3 +206,6 @@ __device__ __forceinline__ void bf_trace_point(int code) {
 #define BF_TR_ATTN 4
 #define BF_TR_MERGE 5
 #define BF_TR_GEMM 6
+#define BF_TR_FP8_ROWS 7
+#define BF_TR_FP8_NORM 8
+#define BF_TR_FP8_GEMM 9

@@ -29,14 +29,18 @@ Fp8Walk fp8_walk(int places, long long rows, int groups, int num_sms, int mats) 
   return w;
 }
 
+// the codes of Fp8Sixteen<., 64>, of which `n` are there
 __device__ __forceinline__ void fp8_store16(uint8_t* dst, const uint4& c, int n) {
-  if (n >= 16) {
-    *reinterpret_cast<uint4*>(dst) = c;            // (rows of codes lie on 16-byte boundaries)
+  if (n >= 72) {
+    *reinterpret_cast<uint2*>(dst) = make_uint2(c.x, c.y);            // (rows of codes lie on 16-byte boundaries)
+    *reinterpret_cast<uint2*>(dst + 64) = make_uint2(c.z, c.w);
   } else {
     const uint32_t w[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (j < n) dst[j] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
+    for (int j = 0; j < 16; ++j) {
+      const int at = j < 8 ? j : 56 + j;
+      if (at < n) dst[at] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
+    }
   }
 }
 
@@ -47,40 +51,35 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(F8_THREADS)
 fp8_rows_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ codes, long long ldc,
                 float* __restrict__ scales, long long lds, int rows, int K, int groups, int shift) {
+  BF_TRACE_POINT(10 * BF_TR_FP8_ROWS);
   bf_pdl_trigger();
   const int sub = threadIdx.x & 7, place = threadIdx.x >> 3;
   const int g = (blockIdx.x << shift) + (place & ((1 << shift) - 1));
   const int at_once = F8_ROW_PLACES >> shift;
   const int step = (int)gridDim.y * at_once;
-  const int k = g * BF_FP8_GROUP + sub * 16, n = g < groups ? K - k : 0;
-  long long t = (long long)blockIdx.y * at_once + (place >> shift);
-  const T* src = x + t * ldx + k;
-  uint8_t* dst = codes + t * ldc + k;
-  float* at = scales + g * lds + t;
+  const int k = g * BF_FP8_GROUP + sub * 8, n = g < groups ? K - k : 0;
+  const long long t0 = (long long)blockIdx.y * at_once + (place >> shift);
   // (every lane of a block takes as many turns: the shuffles are the whole warp's)
   const int turns = (rows - (int)blockIdx.y * at_once + step - 1) / step;
   bf_pdl_wait();
+  BF_TRACE_POINT(10 * BF_TR_FP8_ROWS + 1);
   for (int i = 0; i < turns; ++i) {
-    const bool there = t < rows;
-    Fp8Sixteen<T> v;
-    if (VEC && n >= 16 && there) {
-      v.template load<true>(src, 16);
+    const long long t = t0 + (long long)i * step;
+    Fp8Sixteen<T, 64> v;
+    const T* src = x + t * ldx + k;
+    if (VEC && n >= 72 && t < rows) {
+      v.template load<true>(src, n);
     } else {
-      v.template load<false>(src, there ? n : 0);
+      v.template load<false>(src, t < rows ? n : 0);
     }
     uint32_t m = v.largest();
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     const Fp8Scale s = fp8_scale(m);
-    if (there && n > 0) {
-      fp8_store16(dst, v.codes(s), n);
-      if (sub == 0) *at = s.s;
-    }
-    t += step;
-    src += step * ldx;
-    dst += step * ldc;
-    at += step;
+    if (t < rows && n > 0) fp8_store16(codes + t * ldc + k, v.codes(s), n);
+    if (t < rows && g < groups && sub == 0) scales[g * lds + t] = s.s;
   }
+  BF_TRACE_POINT(10 * BF_TR_FP8_ROWS + 2);
 }
 
 // A block a row: resid (+= delta), RMSNorm, rounding to bfloat16, into 8 bits; eight numbers a thread and
@@ -91,8 +90,22 @@ __global__ void add_rmsnorm_fp8_kernel(float* __restrict__ resid, const __nv_bfl
                                        const float* __restrict__ w, uint8_t* __restrict__ codes, long long ldc,
                                        float* __restrict__ scales, long long lds, int H, float eps) {
   __shared__ float scratch[33];
+  BF_TRACE_POINT(10 * BF_TR_FP8_NORM);
   bf_pdl_trigger();
+  // (the norm's weight depends on no kernel of the stream)
+  float f[TRIPS][8];
+#pragma unroll
+  for (int k = 0; k < TRIPS; ++k) {
+    const int c = (k * blockDim.x + threadIdx.x) * 8;
+    if (c < H) {
+      const float4 wa = *reinterpret_cast<const float4*>(w + c);
+      const float4 wb = *reinterpret_cast<const float4*>(w + c + 4);
+      f[k][0] = wa.x; f[k][1] = wa.y; f[k][2] = wa.z; f[k][3] = wa.w;
+      f[k][4] = wb.x; f[k][5] = wb.y; f[k][6] = wb.z; f[k][7] = wb.w;
+    }
+  }
   bf_pdl_wait();
+  BF_TRACE_POINT(10 * BF_TR_FP8_NORM + 1);
   const int r = blockIdx.x;
   float* x = resid + (size_t)r * H;
   const __nv_bfloat16* d = delta ? delta + (size_t)r * H : nullptr;
@@ -131,83 +144,89 @@ __global__ void add_rmsnorm_fp8_kernel(float* __restrict__ resid, const __nv_bfl
     const int c = (k * blockDim.x + threadIdx.x) * 8;
     uint32_t m = 0u;
     if (c < H) {
-      const float4 wa = *reinterpret_cast<const float4*>(w + c);
-      const float4 wb = *reinterpret_cast<const float4*>(w + c + 4);
-      const float f[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        v[k][j] = __bfloat162float(__float2bfloat16_rn(v[k][j] * inv * f[j]));
+        v[k][j] = __bfloat162float(__float2bfloat16_rn(v[k][j] * inv * f[k][j]));
         m = max(m, __float_as_uint(v[k][j]) & 0x7fffffffu);
       }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[k][j] = 0.f;
     }
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     const Fp8Scale s = fp8_scale(m);
     if (c < H) {
-      *reinterpret_cast<uint2*>(codes + r * ldc + c) =
-          make_uint2(fp8_codes4(v[k], s), fp8_codes4(v[k] + 4, s));
+      uint32_t q[2], sg[2] = {0u, 0u};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        sg[j >> 2] |= (__float_as_uint(v[k][j]) >> 31) << (8 * (j & 3) + 7);
+        v[k][j] = fabsf(v[k][j]);
+      }
+      fp8_codes(v[k], sg, s, q);
+      *reinterpret_cast<uint2*>(codes + r * ldc + c) = make_uint2(q[0], q[1]);
       if ((threadIdx.x & 15) == 0) scales[(long long)(c / BF_FP8_GROUP) * lds + r] = s.s;
     }
   }
+  BF_TRACE_POINT(10 * BF_TR_FP8_NORM + 2);
 }
 
-// Sixteen lanes a group.  blockIdx.z: the matrix, of mat_rows rows.  BLOCKS: a scale per 128 rows of it and group, [blocks,
-// groups]; else one per row and group, [groups, lds].
-constexpr int F8_READ_PLACES = F8_THREADS / 16;
+// A warp a group, four numbers a lane, four rows a turn: a warp's loads and stores are whole lines.
+// blockIdx.z: the matrix, of mat_rows rows.  BLOCKS: a scale per 128 rows of it and group, [blocks, groups];
+// else one per row and group, [groups, lds].
+constexpr int F8_READ_PLACES = F8_THREADS / 32;
 template <typename T, bool BLOCKS>
 __global__ void __launch_bounds__(F8_THREADS)
 fp8_read_kernel(const uint8_t* __restrict__ codes, long long ldc, const float* __restrict__ scales,
                 long long lds, T* __restrict__ out, long long ldo, int mat_rows, int K, int groups, int shift,
                 bool vec) {
   bf_pdl_trigger();
-  const int sub = threadIdx.x & 15, place = threadIdx.x >> 4;
+  const int lane = threadIdx.x & 31, place = threadIdx.x >> 5;
   const int g = (blockIdx.x << shift) + (place & ((1 << shift) - 1)), r = place >> shift;
   const int at_once = F8_READ_PLACES >> shift;
   const long long step = (long long)gridDim.y * at_once;
-  const int k = g * BF_FP8_GROUP + sub * 8, n = g < groups ? min(8, K - k) : 0;
+  const int k = g * BF_FP8_GROUP + lane * 4, n = g < groups ? min(4, K - k) : 0;
   bf_pdl_wait();
   if (n <= 0) return;
   codes += (long long)blockIdx.z * mat_rows * ldc;
   out += (long long)blockIdx.z * mat_rows * ldo;
   if (BLOCKS) scales += (long long)blockIdx.z * ((mat_rows + BF_FP8_GROUP - 1) / BF_FP8_GROUP) * groups;
-  for (long long t0 = (long long)blockIdx.y * at_once + r; t0 < mat_rows; t0 += 2 * step) {
-    uint2 c[2];
-    float s[2];
+  for (long long t0 = (long long)blockIdx.y * at_once + r; t0 < mat_rows; t0 += 4 * step) {
+    uint32_t c[4];
+    float s[4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       const long long t = t0 + i * step;
-      c[i] = make_uint2(0u, 0u);
+      c[i] = 0u;
       s[i] = 0.f;
       if (t < mat_rows) {
         const uint8_t* src = codes + t * ldc + k;
         s[i] = BLOCKS ? scales[(t / BF_FP8_GROUP) * groups + g] : scales[g * lds + t];
-        if (n == 8) {
-          c[i] = *reinterpret_cast<const uint2*>(src);
+        if (n == 4) {
+          c[i] = *reinterpret_cast<const uint32_t*>(src);
         } else {
-          for (int j = 0; j < n; ++j) (j < 4 ? c[i].x : c[i].y) |= (uint32_t)src[j] << (8 * (j & 3));
+          for (int j = 0; j < n; ++j) c[i] |= (uint32_t)src[j] << (8 * j);
         }
       }
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       const long long t = t0 + i * step;
       if (t >= mat_rows) break;
-      float v[8];
-      fp8_values4(c[i].x, v);
-      fp8_values4(c[i].y, v + 4);
+      float v[4];
+      fp8_values4(c[i], v);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] *= s[i];
+      for (int j = 0; j < 4; ++j) v[j] *= s[i];
       T* dst = out + t * ldo + k;
-      if (vec && n == 8) {
+      if (vec && n == 4) {
         if constexpr (sizeof(T) == 4) {
-          reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
-          reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
+          *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
         } else {
-          uint4 o;
+          uint2 o;
           __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(&o);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o2[j] = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-          *reinterpret_cast<uint4*>(dst) = o;
+          o2[0] = __floats2bfloat162_rn(v[0], v[1]);
+          o2[1] = __floats2bfloat162_rn(v[2], v[3]);
+          *reinterpret_cast<uint2*>(dst) = o;
         }
       } else {
         for (int j = 0; j < n; ++j) bf_st(dst + j, v[j]);
@@ -226,15 +245,15 @@ fp8_blocks_kernel(const T* __restrict__ w, long long ldw, uint8_t* __restrict__ 
   const int sub = threadIdx.x & 7, lead = threadIdx.x >> 3;
   const int g = blockIdx.x, r0 = blockIdx.y * BF_FP8_GROUP;
   const long long first = (long long)blockIdx.z * mat_rows;
-  const int k = g * BF_FP8_GROUP + sub * 16, n = K - k;
-  Fp8Sixteen<T> v[4];
+  const int k = g * BF_FP8_GROUP + sub * 8, n = K - k;
+  Fp8Sixteen<T, 64> v[4];
   uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = r0 + i * 32 + lead, there = r < mat_rows ? n : 0;
     const T* src = w + (first + r) * ldw + k;
-    if (VEC && there >= 16) {
-      v[i].template load<true>(src, 16);
+    if (VEC && there >= 72) {
+      v[i].template load<true>(src, there);
     } else {
       v[i].template load<false>(src, there);
     }
@@ -345,7 +364,7 @@ BF_EXPORT int bf_fp8_read(const Fp8ReadCall* call) {
   if (mats <= 0 || mat_rows <= 0 || K <= 0) return 0;
   if (!on_16(codes, ldc, 1) || mats > 65535 || (!blocks && mats != 1)) return (int)cudaErrorInvalidValue;
   const int groups = (K + BF_FP8_GROUP - 1) / BF_FP8_GROUP;
-  const Fp8Walk walk = fp8_walk(F8_READ_PLACES, (mat_rows + 1LL) / 2, groups, num_sms, mats);
+  const Fp8Walk walk = fp8_walk(F8_READ_PLACES, (mat_rows + 3LL) / 4, groups, num_sms, mats);
   auto go = [&](auto kern, auto* dst) {
     return bf_launch_pdl(kern, walk.grid, dim3(F8_THREADS), 0, call->stream, (const uint8_t*)call->codes,
                          call->ldc, call->scales, call->lds, dst, call->ldo, call->mat_rows, call->K, groups,
@@ -467,3 +486,5 @@ BF_EXPORT int bf_fp8_product(const Fp8ProductCall* call) {
                          c.out_dtype, c.rows, c.features, c.K, c.experts, c.gated, c.act, c.limit, c.slope,
                          c.up_offset, tile, split, 0, c.num_sms, c.err, c.stream);
 }
+
+BF_TRACE_READER(bf_trace_read_fp8)

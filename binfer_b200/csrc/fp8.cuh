@@ -17,9 +17,9 @@
 #define BF_FP8_GROUP 128
 #define BF_FP8_MAX 448.f
 
-// A group's scale, and its reciprocal from below and above.
+// A group's scale, and its reciprocal (off by one place at most).
 struct Fp8Scale {
-  float s, low, high;
+  float s, inv;
 };
 // ... of a group whose largest size has these bits.  The quotient by 448 is the rounded product with
 // 1 / 448 put right by its remainder, which is exact (it equals the division for every significand).
@@ -28,38 +28,35 @@ __device__ __forceinline__ Fp8Scale fp8_scale(uint32_t largest_bits) {
   const float a = __uint_as_float(largest_bits), q = a * (1.f / BF_FP8_MAX);
   r.s = fmaxf(fmaf(fmaf(-q, BF_FP8_MAX, a), 1.f / BF_FP8_MAX, q), 0x1p-100f);
   if (largest_bits >= 0x7f800000u) r.s = __uint_as_float(0x7fffffffu);
-  float inv;                                       // (off by one place at most)
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(r.s));
-  r.low = inv * (1.f - 0x1p-21f);
-  r.high = inv * (1.f + 0x1p-21f);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.inv) : "f"(r.s));
   return r;
 }
-// the codes of two quotients, the first in the lower byte
+// the codes of two numbers, the first in the lower byte
 __device__ __forceinline__ uint32_t fp8_codes2(float a, float b) {
   return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
-// A float that rounds to the code of x / s: the rounded quotient q; where q lies on the middle of two
-// codes and x / s does not, the sign of x - q s, which a fused multiply-add gives exactly (q has five
-// bits), says on which side, and one last place to that side decides the rounding.
-__device__ __forceinline__ float fp8_quotient(float x, float s) {
-  float q = __fdiv_rn(x, s);
-  const float r = fmaf(-q, s, x);
-  const bool middle = fabsf(q) < 0x1p-6f ? q * 1024.f == rintf(q * 1024.f)
-                                         : (__float_as_uint(q) & 0xfffffu) == 0x80000u;
-  if (middle && q != 0.f && r != 0.f)
-    q = __uint_as_float(__float_as_uint(q) + ((r > 0.f) == (q > 0.f) ? 1u : 0xffffffffu));
-  return q;
+// A float that rounds to the code of a / s, for a >= 0.  Codes and the middles between them are among the
+// floats of five significant bits; t is the one nearest to a * (1 / s).  A fused multiply-add gives the sign
+// of a - t s exactly (t s has 29 bits), and one last place to that side of t decides as the quotient itself
+// does: nothing where t is a code, the side where it is a middle, the tie where a / s is t.  (Middles are
+// no rarity: of two bfloat16 numbers, the largest and another, the quotient is one every few dozen times.)
+__device__ __forceinline__ float fp8_side(float a, const Fp8Scale& k) {
+  const uint32_t t = (__float_as_uint(a * k.inv) + 0x40000u) & 0xfff80000u;
+  const int side = (int)__float_as_uint(fmaf(-__uint_as_float(t), k.s, a));
+  return __uint_as_float(t + (uint32_t)max(min(side, 1), -1));
 }
-// The codes of four numbers.  x / s lies between x * low and x * high (2^-21 to either side covers the
-// three roundings between): where both round to the same code it is that, else (four numbers in 2^14)
-// the quotients are taken.
-__device__ __forceinline__ uint32_t fp8_codes4(const float* x, const Fp8Scale& k) {
-  const uint32_t c = fp8_codes2(x[0] * k.low, x[1] * k.low) | fp8_codes2(x[2] * k.low, x[3] * k.low) << 16;
-  const uint32_t d = fp8_codes2(x[0] * k.high, x[1] * k.high) | fp8_codes2(x[2] * k.high, x[3] * k.high) << 16;
-  if (c == d) return c;
-  return fp8_codes2(fp8_quotient(x[0], k.s), fp8_quotient(x[1], k.s)) |
-        fp8_codes2(fp8_quotient(x[2], k.s), fp8_quotient(x[3], k.s)) << 16;
-  return c;
+// The codes of N numbers (a multiple of 4), four a word, from their sizes; `signs` has the signs in the
+// codes' places.
+template <int N>
+__device__ __forceinline__ void fp8_codes(const float (&a)[N], const uint32_t (&signs)[N / 4], const Fp8Scale& k,
+                                          uint32_t (&c)[N / 4]) {
+  const bool finite = k.s == k.s;
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    const uint32_t v = fp8_codes2(fp8_side(a[i], k), fp8_side(a[i + 1], k)) |
+                       fp8_codes2(fp8_side(a[i + 2], k), fp8_side(a[i + 3], k)) << 16;
+    c[i / 4] = finite ? v | (signs[i / 4] & 0x80808080u) : 0x7f7f7f7fu;
+  }
 }
 // the values of four codes
 __device__ __forceinline__ void fp8_values4(uint32_t codes, float* v) {
@@ -71,9 +68,10 @@ __device__ __forceinline__ void fp8_values4(uint32_t codes, float* v) {
     v[2 * i + 1] = f.y;
   }
 }
-// Sixteen neighbouring numbers of a row (as many as 32-bit words hold of them are a register), of which
-// `n` are there (the others read as zero); WHOLE: all sixteen, on a 16-byte boundary.
-template <typename T>
+// Sixteen numbers of a row in the registers' own form, two runs of eight that lie `GAP` apart (8: sixteen
+// neighbours; 64: eight lanes' loads and stores of either run are one line each).  `n` numbers are there from
+// the first on, counting the gap (the others read as zero); WHOLE: all of them, on 16-byte boundaries.
+template <typename T, int GAP>
 struct Fp8Sixteen {
   static constexpr int WORDS = (int)sizeof(T) * 4;
   uint32_t w[WORDS];
@@ -83,7 +81,8 @@ struct Fp8Sixteen {
     if (WHOLE) {
 #pragma unroll
       for (int i = 0; i < WORDS / 4; ++i) {
-        const uint4 q = reinterpret_cast<const uint4*>(p)[i];
+        const T* at = i < WORDS / 8 ? p + i * (16 / (int)sizeof(T)) : p + GAP + (i - WORDS / 8) * (16 / (int)sizeof(T));
+        const uint4 q = *reinterpret_cast<const uint4*>(at);
         w[4 * i] = q.x;
         w[4 * i + 1] = q.y;
         w[4 * i + 2] = q.z;
@@ -93,17 +92,26 @@ struct Fp8Sixteen {
 #pragma unroll
       for (int i = 0; i < WORDS; ++i) {
         if constexpr (sizeof(T) == 4) {
-          w[i] = i < n ? __float_as_uint(p[i]) : 0u;
+          const int at = i < 8 ? i : GAP + i - 8;
+          w[i] = at < n ? __float_as_uint(p[at]) : 0u;
         } else {
           const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
-          w[i] = (2 * i < n ? (uint32_t)h[2 * i] : 0u) | (2 * i + 1 < n ? (uint32_t)h[2 * i + 1] << 16 : 0u);
+          const int at = i < 4 ? 2 * i : GAP + 2 * i - 8;
+          w[i] = (at < n ? (uint32_t)h[at] : 0u) | (at + 1 < n ? (uint32_t)h[at + 1] << 16 : 0u);
         }
       }
     }
   }
-  __device__ __forceinline__ float value(int i) const {
-    if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
-    else return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+  // the size of a number, and the signs of four
+  __device__ __forceinline__ float size(int i) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[i] & 0x7fffffffu);
+    else return __uint_as_float(i & 1 ? w[i / 2] & 0x7fff0000u : (w[i / 2] & 0x7fffu) << 16);
+  }
+  __device__ __forceinline__ uint32_t signs(int i) const {            // (of numbers 4 i .., in the bytes' tops)
+    if constexpr (sizeof(T) == 4)
+      return __byte_perm(__byte_perm(w[4 * i], w[4 * i + 1], 0x0073), __byte_perm(w[4 * i + 2], w[4 * i + 3], 0x0073),
+                         0x5410);
+    else return __byte_perm(w[2 * i], w[2 * i + 1], 0x7531);
   }
   // the largest size, as the bits of a float (those of a NaN are above an infinity's)
   __device__ __forceinline__ uint32_t largest() const {
@@ -119,12 +127,13 @@ struct Fp8Sixteen {
     }
   }
   __device__ __forceinline__ uint4 codes(const Fp8Scale& s) const {
-    uint32_t c[4];
+    float a[16];
+    uint32_t sg[4], c[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float x[4] = {value(4 * i), value(4 * i + 1), value(4 * i + 2), value(4 * i + 3)};
-      c[i] = fp8_codes4(x, s);
-    }
+    for (int i = 0; i < 16; ++i) a[i] = size(i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sg[i] = signs(i);
+    fp8_codes(a, sg, s, c);
     return make_uint4(c[0], c[1], c[2], c[3]);
   }
 };

@@ -91,6 +91,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   constexpr int HALVES = GATED ? 2 : 1;
   constexpr int TMEM_COLS = SLOTS * NB;
   extern __shared__ __align__(16) uint8_t smem_raw[];
+  BF_TRACE_POINT(10 * BF_TR_FP8_GEMM);
   bf_pdl_trigger();
   uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t* full = reinterpret_cast<uint64_t*>(base);
@@ -175,6 +176,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
     }
   __syncwarp();
   bf_pdl_wait();
+  BF_TRACE_POINT(10 * BF_TR_FP8_GEMM + 1);
   if (p.split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (p.starts) {
     fill_row_tables(tables, p.starts, p.experts, p.rows, NB);
@@ -338,7 +340,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
       const int row = place & ((1 << row_shift) - 1);
       const int rounds = (g1 - g0 + per_round - 1) / per_round;
       const __nv_bfloat16* src = p.x + row * p.ldx + sub * 16;
-      auto ask = [&](int r, Fp8Sixteen<__nv_bfloat16>& v) {
+      auto ask = [&](int r, Fp8Sixteen<__nv_bfloat16, 8>& v) {
         const int k = (g0 + r * per_round + (place >> row_shift)) * FK;
         const int left = row < p.rows && k < g1 * FK ? p.K - k - sub * 16 : 0;
         if (p.x_vec && left >= 16) {
@@ -347,7 +349,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
           v.template load<false>(src + k, left);
         }
       };
-      Fp8Sixteen<__nv_bfloat16> v, next;
+      Fp8Sixteen<__nv_bfloat16, 8> v, next;
       ask(0, v);
       for (int r = 0; r < rounds; ++r) {
         if (r + 1 < rounds) ask(r + 1, next);
@@ -480,6 +482,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
     }
   }
   __syncwarp();
+  BF_TRACE_POINT(10 * BF_TR_FP8_GEMM + 5);
 
   if (p.split > 1) {
     // every part is in place behind this; then the columns of this rank, parts in the ranks' order
@@ -507,6 +510,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
 
   // ------------------------------------------------------------------ wind-down
   __syncthreads();
+  BF_TRACE_POINT(10 * BF_TR_FP8_GEMM + 2);
   if (*abort) {
     if (threadIdx.x == 0) atomicOr(p.err, BF_ERR_WAIT);
     if (warp == 0 && lane == 0) mbar_drain(full, STAGES, stage, phase);
@@ -656,3 +660,5 @@ BF_EXPORT int bf_gemm_fp8_few(const void* x, long long ldx, const float* sx, lon
     return few_by_width<float, false>(nb, resident, x, ldx, w, ldw, (float*)out, p, num_sms, stream);
   return few_by_width<__nv_bfloat16, false>(nb, resident, x, ldx, w, ldw, (__nv_bfloat16*)out, p, num_sms, stream);
 }
+
+BF_TRACE_READER(bf_trace_read_gemm_fp8_few)

@@ -3077,11 +3077,13 @@ def _fp8_product(what: str, x, w: Fp8Weight, starts, out, row_w, activation, lim
     p = _profiler
     if p is not None:
         p.begin(what)
-    # (few rows: one kernel, where it takes the sizes)
+    # Few rows launched one by one go as one kernel, where it takes the sizes (4 us of the host's time less: 7.5
+    # against 12); in a captured graph, where the host does not count, as two (a decode step of one request, 36
+    # layers of the 8B shape: 2.74 ms against 2.93).  The results are the same.
     code = -1
     if held:
         code = _fp8_product_call(0, 0, codes.data_ptr(), codes.stride(0), scales.data_ptr(), scales.stride(0), *behind)
-    elif M <= 8 and starts is None and FP8_RESIDENT:
+    elif M <= 8 and starts is None and FP8_RESIDENT and not torch.cuda.is_current_stream_capturing():
         code = _fp8_product_call(x.data_ptr(), x.stride(0), 0, 0, 0, 0, *behind)
     if code == -1 and not held:
         # the rows' codes and behind them their scales

@@ -4,6 +4,7 @@
     python -m binfer_b200.microbench prefill_attention --tokens 2048
     python -m binfer_b200.microbench kv4_decode --batch 8 --ctx 4096
     python -m binfer_b200.microbench kv4_prefill --tokens 2048 --variant load
+    python -m binfer_b200.microbench fp8_linear --tokens 8 --features 12288 --gated   # weights in 8 bits
     python -m binfer_b200.microbench diff_prefill --tokens 2048 --head-dim 64 --value-dim 128
     python -m binfer_b200.microbench diff_decode --batch 8 --head-dim 64 --value-dim 128
     python -m binfer_b200.microbench gemm --tokens 8 --features 6144 --k 4096 [--library]
@@ -456,6 +457,18 @@ def scan(a):
     assert int(err.item()) == 0
 
 
+def fp8_linear(a):
+    dev = torch.device("cuda:0")
+    T, N, K = a.tokens, a.features, a.k
+    rows = N * (2 if a.gated else 1)
+    weights = [ops.fp8_weight(torch.randn((rows, K), device=dev, dtype=BF16) * 0.02, a.gated)
+               for _ in range(max(2, int(3e8 // (rows * K)) + 1))]
+    x, out = torch.randn((T, K), device=dev, dtype=BF16), torch.empty((T, N), dtype=BF16, device=dev)
+    us = timed([lambda w=w: ops.fp8_linear(x, w, out) for w in weights], a.iters, a.warmup)
+    report("fp8_linear", us, nbytes=rows * K + 2 * T * (K + N), flops=2.0 * T * rows * K, tokens=T, features=N, k=K,
+           gated=a.gated)
+
+
 def step_timeline(a):
     import ctypes
     from . import Engine
@@ -476,7 +489,8 @@ def step_timeline(a):
     cfg = Qwen3Config.from_dict(raw)
     ps = a.page_size
     eng = Engine(cfg, "bfloat16", random_seed=0, num_pages=B * (-(-ctx // ps)) + 64, page_size=ps,
-                 max_seq_len=ctx, max_batch_size=B, max_tokens_per_step=2048, cuda_graphs=True)
+                 max_seq_len=ctx, max_batch_size=B, max_tokens_per_step=2048, cuda_graphs=True,
+                 weights=a.weights)
     runner, sampler = eng.runner, eng.sampler
     gen = torch.Generator().manual_seed(0)
     steps = 8
@@ -492,7 +506,7 @@ def step_timeline(a):
     torch.cuda.synchronize()
     readers = [getattr(ops.lib(), "bf_trace_read_" + f) for f in
                ("elementwise", "qkv_post", "attention_decode_persistent", "attention_decode",
-                "gemm_tcgen05_cluster")]
+                "gemm_tcgen05_cluster", "fp8", "gemm_fp8_few")]
     times = (ctypes.c_ulonglong * 8192)()
     codes = (ctypes.c_int * 8192)()
     events = []
@@ -510,7 +524,7 @@ def step_timeline(a):
         events += [(times[i], codes[i]) for i in range(n)]
     events.sort()
     names = {1: "add_rmsnorm", 2: "silu_mul", 3: "qk_norm_rope", 4: "decode_attention",
-             5: "attention_merge", 6: "gemm_cluster"}
+             5: "attention_merge", 6: "gemm_cluster", 7: "fp8_rows", 8: "add_rmsnorm_fp8", 9: "fp8_linear"}
     phases = ["first block starts", "wait returns", "ends", "partial sums sent",
               "cluster barrier passed", "products done"]
     t0 = prev = events[0][0]
@@ -529,7 +543,8 @@ def main(argv=None):
     ap.add_argument("kernel", choices=["decode_attention", "prefill_attention", "gemm",
                                        "swiglu", "add_rmsnorm", "step_timeline", "scan",
                                        "diff_decode", "diff_prefill", "add_tanh_norm",
-                                       "out_product", "experts", "kv4_decode", "kv4_prefill"])
+                                       "out_product", "experts", "kv4_decode", "kv4_prefill",
+                                       "fp8_linear"])
     ap.add_argument("--iters", type=int, default=50)
     ap.add_argument("--warmup", type=int, default=5)
     ap.add_argument("--batch", type=int, default=8)
@@ -550,6 +565,8 @@ def main(argv=None):
     ap.add_argument("--chunked", action="store_true", help="scan: long portions in chunks")
     ap.add_argument("--state", type=int, default=128, help="scan: size of a key (the state's rows)")
     ap.add_argument("--layers", type=int, default=6, help="step_timeline: layers of the model")
+    ap.add_argument("--weights", default="auto", choices=["auto", "fp8"], help="step_timeline: the layers' matrices")
+    ap.add_argument("--gated", action="store_true", help="fp8_linear: a gate and up projection")
     ap.add_argument("--intermediate", type=int, default=12288)
     ap.add_argument("--vocab", type=int, default=151936)
     ap.add_argument("--features", type=int, default=6144)
@@ -578,7 +595,8 @@ def main(argv=None):
      "gemm": gemm, "swiglu": swiglu, "add_rmsnorm": add_rmsnorm,
      "step_timeline": step_timeline, "scan": scan, "diff_decode": diff_decode,
      "diff_prefill": diff_prefill, "add_tanh_norm": add_tanh_norm,
-     "out_product": out_product, "experts": experts, "kv4_decode": kv4_decode, "kv4_prefill": kv4_prefill}[a.kernel](a)
+     "out_product": out_product, "experts": experts, "kv4_decode": kv4_decode, "kv4_prefill": kv4_prefill,
+     "fp8_linear": fp8_linear}[a.kernel](a)
     return 0
 
 
