@@ -37,7 +37,7 @@ constexpr int FEW_BARS = 1024;
 // so and 8.0 to 12.8 us with it, but 1,024 x 2,048: 5.0 and 5.5; launched one by one, 4 us of the host's
 // time are gained at every size).
 constexpr int FEW_RES_ROWS = 8;
-constexpr int FEW_ROUNDS = 2;
+constexpr int FEW_ROUNDS = 4;
 constexpr int FEW_W_BYTES = 128 * FK;
 // Two CTAs share an SM: its registers, its shared memory and its tensor memory are dealt out by halves.  A
 // step of eight rows against 24,576 x 4,096 gated took 27.5 us with one, whose 192 tiles ran in two turns.

@@ -2847,14 +2847,18 @@ _fp8_product_call = _Packed("bf_fp8_product", "PqPqPqPqPPPPqiiiiiiifffiiiPP")
 
 def _fp8_empty_codes(shape, device) -> torch.Tensor:
     """Room for codes ``[..., K]`` whose rows lie on 16-byte boundaries."""
-    k = shape[-1]
-    if k % 16 == 0:
-        return torch.empty(shape, dtype=E4M3, device=device)
-    strides, step = [1], -(-k // 16) * 16
+    strides, step = [1], -(-shape[-1] // 16) * 16
     for n in reversed(shape[:-1]):
         strides.append(step)
         step *= n
-    return torch.empty_strided(tuple(shape), tuple(reversed(strides)), dtype=E4M3, device=device)
+    strides.reverse()
+    return torch.empty_strided(shape, strides, dtype=E4M3, device=device)
+
+
+def _fp8_empty_rows(T: int, K: int, device) -> Tuple[torch.Tensor, torch.Tensor]:
+    # (the strides spelled out: torch takes half of the time)
+    return (torch.empty_strided((T, K), (-(-K // 16) * 16, 1), dtype=E4M3, device=device),
+            torch.empty_strided((-(-K // FP8_GROUP), T), (T, 1), dtype=torch.float32, device=device))
 
 
 _FP8_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
@@ -2914,8 +2918,7 @@ def fp8_rows(x: torch.Tensor) -> Fp8Rows:
     _same_device("fp8_rows", x)
     shape, device = x.shape, x.device
     T, K = shape
-    codes = _fp8_empty_codes(shape, device)
-    scales = torch.empty((-(-K // FP8_GROUP), T), dtype=torch.float32, device=device)
+    codes, scales = _fp8_empty_rows(T, K, device)
     if T:
         _run("fp8_rows", _fp8_rows_call, x.data_ptr(), x.stride(0), codes.data_ptr(), -(-K // 16) * 16,
              scales.data_ptr(), T, dtype, T, K, num_sms(device), _stream_at(x))
@@ -2944,8 +2947,7 @@ def add_rmsnorm_fp8(resid: torch.Tensor, delta: Optional[torch.Tensor], weight: 
             raise KernelError(f"{what}: the tensors must lie on 16-byte boundaries")
     _same_device(what, resid, delta, weight)
     (T, H), device = resid.shape, resid.device
-    codes = _fp8_empty_codes((T, H), device)
-    scales = torch.empty((-(-H // FP8_GROUP), T), dtype=torch.float32, device=device)
+    codes, scales = _fp8_empty_rows(T, H, device)
     if T:
         _run(what, _add_rmsnorm_fp8_call, resid.data_ptr(), delta.data_ptr() if delta is not None else 0,
              weight.data_ptr(), codes.data_ptr(), codes.stride(0), scales.data_ptr(), T, T, H, eps,
@@ -2976,7 +2978,7 @@ class Fp8Weight:
     code times scale.  ``gated``: the weight is a gate weight and an up weight of N / 2 rows each, one
     behind the other, and the up rows' blocks begin anew (blocks = 2 ceil(N / 2 / 128), else ceil(N / 128)).
     Scales are positive and finite.  Codes whose rows do not lie on 16-byte boundaries are copied."""
-    __slots__ = ("codes", "scales", "gated", "experts", "rows", "features", "K", "device", "_held")
+    __slots__ = ("codes", "scales", "gated", "experts", "rows", "features", "K", "device", "_held", "_index")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, gated: bool = False):
         if codes.dtype != E4M3 or codes.dim() not in (2, 3) or not codes.numel():
@@ -3001,6 +3003,7 @@ class Fp8Weight:
         self.experts = lead[0] if lead else 0
         self.rows, self.features, self.K, self.device = n, features, k, codes.device
         self._held = (codes.data_ptr(), codes.stride(-2), scales.data_ptr())
+        self._index = codes.get_device()
 
     @property
     def shape(self):
@@ -3038,7 +3041,7 @@ def fp8_weight_read(w: Fp8Weight, out: torch.Tensor) -> None:
 
 def _fp8_product(what: str, x, w: Fp8Weight, starts, out, row_w, activation, limit, slope, up_offset, tile,
                  split) -> None:
-    shape, out_shape, K, features = x.shape, out.shape, w.K, w.features
+    shape, K, features = x.shape, w.K, w.features
     M = shape[0] if len(shape) == 2 else -1
     held = isinstance(x, Fp8Rows)
     if held:
@@ -3048,31 +3051,41 @@ def _fp8_product(what: str, x, w: Fp8Weight, starts, out, row_w, activation, lim
                 or (M > 1 and scales.stride(1) != 1)):
             raise KernelError(f"{what}: rows in 8 bits must be [rows, {K}] as fp8_rows makes them, got {codes.dtype} "
                               f"{tuple(shape)} and scales {tuple(scales.shape)}")
-    elif x.dtype != torch.bfloat16 or M < 0 or shape[1] != K or (M and K > 1 and x.stride(1) != 1):
-        raise KernelError(f"{what}: x must be bfloat16 [rows, {K}] with contiguous rows, got {x.dtype} "
-                          f"{tuple(shape)}")
+        others = (codes, scales)
+    else:
+        if x.dtype != torch.bfloat16 or M < 0 or shape[1] != K or (M and K > 1 and x.stride(1) != 1):
+            raise KernelError(f"{what}: x must be bfloat16 [rows, {K}] with contiguous rows, got {x.dtype} "
+                              f"{tuple(shape)}")
+        others = (x,)
     out_type = _FP8_DTYPES.get(out.dtype)
-    if (out_type is None or out_shape != (M, features) or (M and features > 1 and out.stride(1) != 1)):
+    if out_type is None or out.shape != (M, features) or (M and features > 1 and out.stride(1) != 1):
         raise KernelError(f"{what}: out must be bfloat16 or float32 [{M}, {features}] with contiguous rows, got "
-                          f"{out.dtype} {tuple(out_shape)}")
-    if w.gated and (out_type != 1 or activation not in FUSED_ACTIVATIONS):
-        raise KernelError(f"{what}: a gated product has a bfloat16 result and one of the activations "
-                          f"{FUSED_ACTIVATIONS}")
+                          f"{out.dtype} {tuple(out.shape)}")
+    act = 0
+    if w.gated:
+        if out_type != 1 or activation not in FUSED_ACTIVATIONS:
+            raise KernelError(f"{what}: a gated product has a bfloat16 result and one of the activations "
+                              f"{FUSED_ACTIVATIONS}")
+        act = GATE_ACTIVATIONS[activation]
+    starts_at = row_w_at = 0
     if row_w is not None:
         _want(row_w, torch.float32, "row_w")
         if row_w.numel() != M:
             raise KernelError(f"{what}: row_w must have a number per row")
-    if tile not in (0, 16, 32, 64, -1) or not 0 <= split <= 8:
+        others, row_w_at = (*others, row_w), row_w.data_ptr()
+    if starts is not None:
+        others, starts_at = (*others, starts), starts.data_ptr()
+    if (tile or split) and (tile not in (0, 16, 32, 64, -1) or not 0 <= split <= 8):
         raise KernelError(f"{what}: no tiles of {tile} rows, shared by {split}")
-    device = x.device
-    err = error_word(device)
-    _same_device(what, *(x if held else (x,)), w.codes, w.scales, starts, out, row_w, err)
+    _same_device(what, out, *others)
+    if w._index != out.get_device():
+        _same_device(what, w.codes)
     if M == 0:
         return
-    behind = (*w._held, starts.data_ptr() if starts is not None else 0,
-              row_w.data_ptr() if row_w is not None else 0, out.data_ptr(), out.stride(0), out_type, M, features, K,
-              w.experts or 1, w.gated, GATE_ACTIVATIONS[activation] if w.gated else 0, limit, slope, up_offset,
-              tile, split, num_sms(device), err.data_ptr(), _stream_at(out))
+    device = out.device
+    behind = (*w._held, starts_at, row_w_at, out.data_ptr(), out.stride(0), out_type, M, features, K,
+              w.experts or 1, w.gated, act, limit, slope, up_offset, tile, split, num_sms(device),
+              error_word(device).data_ptr(), _stream_at(out))
     global _launches
     p = _profiler
     if p is not None:
@@ -3088,7 +3101,8 @@ def _fp8_product(what: str, x, w: Fp8Weight, starts, out, row_w, activation, lim
     if code == -1 and not held:
         # the rows' codes and behind them their scales
         pitch = -(-K // 16) * 16
-        scratch = torch.empty(M * pitch + 4 * -(-K // FP8_GROUP) * M, dtype=torch.uint8, device=device)
+        scratch = torch.empty_strided((M * (pitch + 4 * -(-K // FP8_GROUP)),), (1,), dtype=torch.uint8,
+                                      device=device)
         at = scratch.data_ptr()
         code = _fp8_product_call(x.data_ptr(), x.stride(0), at, pitch, at + M * pitch, M, *behind)
         _launches += 1          # two kernels
