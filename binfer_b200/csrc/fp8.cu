@@ -411,22 +411,25 @@ extern "C" int bf_gemm_fp8_few(const void*, long long, const float*, long long, 
                                int, int, int, float, float, float, int, int, int, int, int*, cudaStream_t);
 extern "C" int bf_gemm_fp8_pair(const void*, long long, const float*, long long, const void*, long long,
                                 const float*, const int*, const float*, void*, long long, int, int, int, int,
-                                int, int, int, float, float, float, int, int*, cudaStream_t);
+                                int, int, int, float, float, float, int, int, int*, cudaStream_t);
 
-// How a product runs: the most rows of a tile of gemm_fp8_few.cu, or -1 for gemm_fp8_pair.cu.  Without
-// experts tiles of 32 rows as long as they are all resident (157 rows, 6,144 x 4,096: 18.6 us against 23.3
-// with tiles of 64 and 22.3 on pairs; 256 rows, 4,096 x 12,288: 42 / 40 / 51), then 64 if those hold all
-// rows (64 rows, 24,576 x 4,096 gated: 28 against 36 and 44), then pairs (157 rows of the same: 61 / 51 /
-// 46).  With experts by the rows that one has on average (64 experts, 2,048 x 2,048 gated, 8 to 128 rows
-// each: 47 / 51 / 55 us with tiles of 16 / 32 / 64 and 84 on pairs, 77 / 62 / 60 / 92, 128 / 90 / 84 / 104,
-// 228 / 156 / 136 / 126).
-static int fp8_tile(int rows, int features, bool gated, int experts, int num_sms) {
+// How a product runs: the most rows of a tile of gemm_fp8_few.cu, or -1 for gemm_fp8_pair.cu.
+// Without experts: tiles of 32 rows while there is one for every SM at most, or two with few groups (157
+// rows, 6,144 x 4,096: 17.0 us against 22.1 with tiles of 64 and 17.9 on pairs; 4,096 x 12,288: 37.1 / 37.9 /
+// 32.0); then 64 if those hold all rows (64 rows, 24,576 x 4,096 gated: 30.8 / 26.9 / 43.7); up to 96 rows 32
+// again (34.3 / 47.6 / 44.8); then pairs (157 rows of the same: 55.7 / 49.1 / 45.8).
+// With experts by the rows that one has on average (64 experts, 2,048 x 2,048 gated, 8 to 128 rows each: 47 /
+// 51 / 55 us with tiles of 16 / 32 / 64 and 84 on pairs, 77 / 62 / 60 / 92, 128 / 90 / 84 / 104, 228 / 156 /
+// 136 / 126).
+static int fp8_tile(int rows, int features, int K, bool gated, int experts, int num_sms) {
   const int each = (rows + experts - 1) / experts;
   if (each <= 16) return 16;
   if (experts > 1) return each <= 24 ? 32 : each <= 112 ? 64 : -1;
+  if (each <= 32) return 32;
   const long long tiles = (rows + 31LL) / 32 * ((features + (gated ? 63 : 127)) / (gated ? 64 : 128));
-  if (each <= 32 || tiles <= 2 * num_sms) return 32;
-  return each <= 64 ? 64 : -1;
+  if (tiles <= num_sms || (tiles <= 2 * num_sms && K <= 48 * BF_FP8_GROUP)) return 32;
+  if (each <= 64) return 64;
+  return each <= 96 && tiles <= 4 * num_sms ? 32 : -1;
 }
 // CTAs that share a tile of 128 weight rows: as many (a power of two: clusters of other sizes leave SMs
 // of a GPC empty) as are resident together, two to an SM, each with two groups at least.
@@ -436,6 +439,16 @@ static int fp8_split(int rows, int features, int K, bool gated, int nb, int num_
   int c = 1;
   while (nb <= 64 && c < 8 && tiles * 2 * c <= 2 * num_sms && groups >= 4 * c) c *= 2;
   return c;
+}
+
+// Pairs that share a tile of 256 x 256, each with four groups at least: two while those are resident together
+// (157 rows, 4,096 x 12,288: 50.8 -> 32.0 us; 512 rows: 54.2 -> 37.2), four for the fewest tiles (64 rows, 1,024
+// x 4,096: 19.5 / 15.2 / 13.2; with 16 tiles, whose clusters of eight CTAs run in two turns, 21.4 / 16.6 / 27.4).
+static int fp8_pair_split(int rows, int features, int K, bool gated, int num_sms) {
+  const long long tiles = (rows + 255LL) / 256 * ((features + (gated ? 127 : 255)) / (gated ? 128 : 256));
+  const int groups = (K + BF_FP8_GROUP - 1) / BF_FP8_GROUP;
+  if (tiles * 16 <= num_sms && groups >= 16) return 4;
+  return tiles * 4 <= num_sms * 9LL / 10 && groups >= 8 ? 2 : 1;
 }
 
 struct Fp8ProductCall {
@@ -463,10 +476,11 @@ struct Fp8ProductCall {
 BF_EXPORT int bf_fp8_product(const Fp8ProductCall* call) {
   const Fp8ProductCall& c = *call;
   if (c.rows <= 0 || c.features <= 0) return 0;
-  const int tile = c.tile ? c.tile : fp8_tile(c.rows, c.features, c.gated != 0, c.experts, c.num_sms);
-  const int split = c.starts || tile < 0 ? 1
+  const int tile = c.tile ? c.tile : fp8_tile(c.rows, c.features, c.K, c.gated != 0, c.experts, c.num_sms);
+  const int split = c.starts ? 1
                     : c.split ? c.split
-                              : fp8_split(c.rows, c.features, c.K, c.gated != 0, tile, c.num_sms);
+                    : tile < 0 ? fp8_pair_split(c.rows, c.features, c.K, c.gated != 0, c.num_sms)
+                               : fp8_split(c.rows, c.features, c.K, c.gated != 0, tile, c.num_sms);
   if (c.x && !c.codes) {
     // asked for without scratch: the rows stay in the CTAs that read them, where they fit
     if (tile != 16 || c.starts) return -1;
@@ -481,7 +495,7 @@ BF_EXPORT int bf_fp8_product(const Fp8ProductCall* call) {
   if (tile < 0)
     return bf_gemm_fp8_pair(c.codes, c.ldc, c.scales, c.lds, c.w, c.ldw, c.sw, c.starts, c.row_w, c.out, c.ldo,
                             c.out_dtype, c.rows, c.features, c.K, c.experts, c.gated, c.act, c.limit, c.slope,
-                            c.up_offset, c.num_sms, c.err, c.stream);
+                            c.up_offset, split, c.num_sms, c.err, c.stream);
   return bf_gemm_fp8_few(c.codes, c.ldc, c.scales, c.lds, c.w, c.ldw, c.sw, c.starts, c.row_w, c.out, c.ldo,
                          c.out_dtype, c.rows, c.features, c.K, c.experts, c.gated, c.act, c.limit, c.slope,
                          c.up_offset, tile, split, 0, c.num_sms, c.err, c.stream);

@@ -14,10 +14,16 @@
 //                whole 128-byte lines (these two warpgroups take 232 registers a thread, which the
 //                first leaves them: 128 x 40 + 256 x 232 = 384 x 168)
 //
+// SPLIT: few tiles leave SMs idle, and `split` pairs share one, a cluster of twice as many CTAs: each adds up
+// its part of the groups, the parts meet in the shared memory that the ring had, a pair owning a slice of
+// the columns, and are added to that pair's own in the pairs' order.
+//
 // Gated: a CTA's half of the weight rows are 64 gate rows and the 64 up rows of the same outputs, so a
 // thread holds both.  With experts a tile's rows are one expert's.
 //
 // Every wait is bounded; no load uses multicast.
+#include <type_traits>
+
 #include "common.cuh"
 #include "fp8.cuh"
 #include "fp8_umma.cuh"
@@ -37,6 +43,7 @@ constexpr int PF_TURN = 32 * 64;              // a warp's rows on their way out:
 struct PairParams {
   int rows, features, K, groups;
   int experts, tiles_f, w_blocks, table_bytes;
+  int split;                            // SPLIT: 2 or 4
   const int* starts;
   const float* sx;
   long long lds;
@@ -58,13 +65,14 @@ __device__ __forceinline__ void pair_umma_fp8(uint32_t tmem_d, uint64_t a_desc, 
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(elected)
       : "memory");
 }
-__device__ __forceinline__ void pair_commit_by(uint64_t* bar, uint32_t elected) {
+// arrives on the barrier at this offset in both CTAs of the pair (`both`: their bits)
+__device__ __forceinline__ void pair_commit_by(uint64_t* bar, uint32_t both, uint32_t elected) {
   asm volatile(
       "{\n\t.reg .pred q;\n\t"
       "setp.ne.b32 q, %2, 0;\n\t"
       "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
       "[%0], %1;\n\t}" ::"r"(smem_u32(bar)),
-      "h"((uint16_t)3), "r"(elected)
+      "h"((uint16_t)both), "r"(elected)
       : "memory");
 }
 
@@ -107,7 +115,7 @@ __device__ __forceinline__ void turn_and_store(uint8_t* buf, const uint4 (&v)[4]
   __syncwarp();
 }
 
-template <typename OutT, bool GATED>
+template <typename OutT, bool GATED, bool SPLIT>
 __global__ void __launch_bounds__(PF_THREADS, 1)
 fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                 OutT* __restrict__ out, const PairParams p) {
@@ -126,8 +134,10 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   uint8_t* tiles = turn + PF_SUMS * PF_TURN;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = pair_rank();
-  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const uint32_t cluster_rank = pair_rank(), rank = cluster_rank & 1u, leader = cluster_rank & ~1u;
+  const int split = SPLIT ? p.split : 1, share = SPLIT ? (int)(cluster_rank >> 1) : 0;
+  const int pair = (int)blockIdx.x / (2 * split), pairs = (int)gridDim.x / (2 * split);
+  const int g0 = p.groups * share / split, g1 = p.groups * (share + 1) / split;
   const int w_rows = (GATED ? 2 : 1) * p.features;
 
   if (threadIdx.x == 0) {
@@ -166,13 +176,13 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   if (warp == 0) {
     // --------------------------------------------------------------- copies
     if (lane == 0) {
-      const uint32_t full_leader = pair_map(smem_u32(full), 0);
+      const uint32_t full_leader = pair_map(smem_u32(full), leader);
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
       for (int u = pair; u < units && ok && !*abort; u += pairs) {
         const RowTile t = row_tile(tables, p.experts, p.tiles_f, PF_TILE, u);
-        for (int g = 0; g < p.groups; ++g) {
+        for (int g = g0; g < g1; ++g) {
           if (!mbar_wait(empty + stage, phase ^ 1, abort)) {
             ok = false;
             break;
@@ -209,12 +219,12 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   } else if (warp == 1) {
     // ------------------------------------------------------------- products
     if (rank == 0) {
-      const uint32_t idesc = fp8_idesc(PF_TILE, 256), elected = elect_one();
+      const uint32_t idesc = fp8_idesc(PF_TILE, 256), elected = elect_one(), both = 3u << leader;
       int stage = 0, buf = 0;
       uint32_t phase = 0, buf_phase = 0;
       bool ok = true, seen = false;                         // a look at the next group's tiles
       for (int u = pair; u < units && ok; u += pairs) {
-        for (int g = 0; g < p.groups; ++g) {
+        for (int g = g0; g < g1; ++g) {
           if (!mbar_seen_or_wait_warp(seen, full + stage, phase, abort) ||
               !mbar_wait_warp(acc_empty + buf, buf_phase ^ 1, abort)) {
             ok = false;
@@ -228,8 +238,8 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
           for (int k = 0; k < FK / 32; ++k)
             pair_umma_fp8(tmem_base + (uint32_t)(buf * 256), a_desc + (uint64_t)(2 * k),
                           b_desc + (uint64_t)(2 * k), idesc, k > 0 ? 1u : 0u, elected);
-          pair_commit_by(acc_full + buf, elected);
-          pair_commit_by(empty + stage, elected);
+          pair_commit_by(acc_full + buf, both, elected);
+          pair_commit_by(empty + stage, both, elected);
           if (++stage == PF_STAGES) {
             stage = 0;
             phase ^= 1;
@@ -243,6 +253,11 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       }
     }
   }
+  if (SPLIT) {
+    __syncwarp();
+    pair_sync();                               // the ring is free in every CTA
+    pair_sync();                               // every part is in place
+  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
     // ----------------------------------------------------------------- sums
@@ -251,7 +266,8 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     const int col_a = GATED ? (part >> 1) * 128 + (part & 1) * 32 : part * 64;
     const int col_b = col_a + (GATED ? 64 : 32);
     const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t acc_empty_leader = pair_map(smem_u32(acc_empty), 0);
+    const uint32_t acc_empty_leader = pair_map(smem_u32(acc_empty), leader);
+    bool met = false;                          // (SPLIT) the cluster's two barriers are behind
     uint8_t* my_turn = turn + (warp - 4) * PF_TURN;
     const bool vec = ((uintptr_t)out & 15) == 0 && p.ldo * (int)sizeof(OutT) % 16 == 0;
     int buf = 0;
@@ -260,20 +276,20 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       const RowTile t = row_tile(tables, p.experts, p.tiles_f, PF_TILE, u);
       const int row_w0 = t.row0 + (int)rank * 128 + quarter * 32;      // the warp's first row
       const int row = min(row_w0 + lane, t.row_end - 1);               // (rows behind the last are not stored)
-      const float* sx = p.sx + row;
+      const float* sx = p.sx + (long long)g0 * p.lds + row;
       // plain: the columns lie in one block of 128 weight rows; gated: in a gate's and an up's
       const long long block = (long long)t.expert * (GATED ? 2 : 1) * p.w_blocks;
       const float* swa =
-          p.sw + (block + (GATED ? t.ft : min(t.ft * 2 + (part >> 1), p.w_blocks - 1))) * p.groups;
+          p.sw + (block + (GATED ? t.ft : min(t.ft * 2 + (part >> 1), p.w_blocks - 1))) * p.groups + g0;
       const long long to_b = GATED ? (long long)p.w_blocks * p.groups : 0;
       float acc[64];
 #pragma unroll
       for (int j = 0; j < 64; ++j) acc[j] = 0.f;
       bool ok = true;
       float s = *sx, wa = *swa, wb = GATED ? swa[to_b] : 0.f;
-      for (int g = 0; g < p.groups; ++g) {
+      for (int g = g0; g < g1; ++g) {
         const float fa = fp8_factor(s, wa), fb = GATED ? fp8_factor(s, wb) : fa;
-        if (g + 1 < p.groups) {                              // the next group's, under this one's wait
+        if (g + 1 < g1) {                                    // the next group's, under this one's wait
           sx += p.lds;
           ++swa;
           s = *sx;
@@ -303,10 +319,44 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
           buf_phase ^= 1;
         }
       }
+      bool mine = true;                                      // to store
+      if constexpr (SPLIT) {
+        // part p's 64 columns belong to pair p split / 4: [sender][four columns][row][4]
+        const int owner = split == 4 ? part : part >> 1, slice4 = 64 / split, first4 = split == 4 ? 0 : (part & 1) * 16;
+        const int lane_row = quarter * 32 + lane;
+        pair_sync();                                         // the ring is free in every CTA
+        mine = owner == share;
+        if (!mine) {
+          const int slot = share < owner ? share : share - 1;
+          const uint32_t to = pair_map(smem_u32(tiles) + (uint32_t)(((slot * slice4 + first4) * 128 + lane_row) * 16),
+                                       (uint32_t)(2 * owner) + rank);
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + (uint32_t)(j * 128 * 16)),
+                         "f"(acc[4 * j]), "f"(acc[4 * j + 1]), "f"(acc[4 * j + 2]), "f"(acc[4 * j + 3])
+                         : "memory");
+        }
+        pair_sync();                                         // every part is in place
+        met = true;
+        if (mine) {
+          // (this pair's own part first, then the others' in their order)
+          for (int slot = 0; slot < split - 1; ++slot) {
+            const uint8_t* from = tiles + ((slot * slice4 + first4) * 128 + lane_row) * 16;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float4 v = *reinterpret_cast<const float4*>(from + j * 128 * 16);
+              acc[4 * j] += v.x;
+              acc[4 * j + 1] += v.y;
+              acc[4 * j + 2] += v.z;
+              acc[4 * j + 3] += v.w;
+            }
+          }
+        }
+      }
       if (!ok) break;
       const float w = p.row_w ? p.row_w[row] : 1.f;
       const int n_rows = t.row_end - row_w0;
-      if (n_rows > 0) {
+      if (n_rows > 0 && mine) {
         OutT* dst = out + (long long)row_w0 * p.ldo;
         constexpr int COLS = 64 / (int)sizeof(OutT);         // of 64 bytes
 #pragma unroll
@@ -330,6 +380,10 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         }
       }
     }
+    if (SPLIT && !met) {
+      pair_sync();
+      pair_sync();
+    }
   }
 
   // ------------------------------------------------------------------ wind-down
@@ -339,7 +393,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       atomicOr(p.err, BF_ERR_WAIT);
       // the peer leaves its waits at once instead of running each of them out
       asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(
-                       pair_map(smem_u32(const_cast<int*>(abort)), rank ^ 1u)),
+                       pair_map(smem_u32(const_cast<int*>(abort)), cluster_rank ^ 1u)),
                    "r"(1)
                    : "memory");
     }
@@ -361,7 +415,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   }
 }
 
-template <typename OutT, bool GATED>
+template <typename OutT, bool GATED, bool SPLIT>
 int pair_launch(const void* x, long long ldx, const void* w, long long ldw, OutT* out, PairParams p,
                 int num_sms, cudaStream_t stream) {
   p.tiles_f = (p.features + (GATED ? 127 : PF_TILE - 1)) / (GATED ? 128 : PF_TILE);
@@ -376,7 +430,7 @@ int pair_launch(const void* x, long long ldx, const void* w, long long ldw, OutT
   const size_t smem_max =
       1024 + ((PF_BARS + row_tables_bytes(FP8_MAX_EXPERTS) + 1023) & ~1023) + PF_SUMS * PF_TURN +
       (size_t)PF_STAGES * PF_STAGE;
-  auto kern = fp8_pair_kernel<OutT, GATED>;
+  auto kern = fp8_pair_kernel<OutT, GATED, SPLIT>;
   static bool configured_on[BF_MAX_DEVICES];
   bool& configured = configured_on[bf_current_device()];
   if (!configured) {
@@ -390,7 +444,8 @@ int pair_launch(const void* x, long long ldx, const void* w, long long ldw, OutT
   if ((e = fp8_map(&mx, x, p.rows, p.K, ldx, 128)) ||
       (e = fp8_map(&mw, w, (long long)p.experts * (GATED ? 2 : 1) * p.features, p.K, ldw, GATED ? 64 : 128)))
     return e;
-  const long long pairs = units < num_sms / 2 ? units : num_sms / 2;
+  if (SPLIT && (p.starts || units * 2 * p.split > num_sms || p.groups < p.split)) return (int)cudaErrorInvalidValue;
+  const long long pairs = SPLIT ? units * p.split : units < num_sms / 2 ? units : num_sms / 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * pairs));
   cfg.blockDim = dim3(PF_THREADS);
@@ -400,7 +455,7 @@ int pair_launch(const void* x, long long ldx, const void* w, long long ldw, OutT
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = bf_pdl_enabled();
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.x = SPLIT ? 2 * p.split : 2;
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
@@ -412,12 +467,13 @@ int pair_launch(const void* x, long long ldx, const void* w, long long ldw, OutT
 
 }  // namespace
 
-// Arguments as bf_gemm_fp8_few's.
+// Arguments as bf_gemm_fp8_few's; split: pairs that share a tile, 1, 2 or 4 (without experts, where tiles * 2 *
+// split is at most num_sms and there are as many groups; else 1 is taken).
 BF_EXPORT int bf_gemm_fp8_pair(const void* x, long long ldx, const float* sx, long long lds, const void* w,
                                long long ldw, const float* sw, const int* starts, const float* row_w,
                                void* out, long long ldo, int out_dtype, int rows, int features, int K,
                                int experts, int gated, int act, float limit, float slope, float up_offset,
-                               int num_sms, int* err, cudaStream_t stream) {
+                               int split, int num_sms, int* err, cudaStream_t stream) {
   if (rows <= 0 || features <= 0) return 0;
   if (K <= 0 || experts < 1 || experts > FP8_MAX_EXPERTS || (!starts && experts != 1) || ldx % 16 || ldw % 16 ||
       (((uintptr_t)x | (uintptr_t)w) & 15) || num_sms < 2 ||
@@ -437,9 +493,16 @@ BF_EXPORT int bf_gemm_fp8_pair(const void* x, long long ldx, const float* sx, lo
   p.act = act;
   p.gk = BfGateConst{limit, slope, up_offset};
   p.err = err;
-  if (gated)
-    return pair_launch<__nv_bfloat16, true>(x, ldx, w, ldw, (__nv_bfloat16*)out, p, num_sms, stream);
-  if (out_dtype == BF_DTYPE_F32)
-    return pair_launch<float, false>(x, ldx, w, ldw, (float*)out, p, num_sms, stream);
-  return pair_launch<__nv_bfloat16, false>(x, ldx, w, ldw, (__nv_bfloat16*)out, p, num_sms, stream);
+  const long long tiles = (rows + 255LL) / 256 * ((features + (gated ? 127 : 255)) / (gated ? 128 : 256));
+  p.split = split == 2 || split == 4 ? split : 1;
+  if (starts || tiles * 2 * p.split > num_sms || p.split > (K + FK - 1) / FK) p.split = 1;
+  auto go = [&](auto* o, auto is_gated) {
+    using T = std::remove_pointer_t<decltype(o)>;
+    constexpr bool G = decltype(is_gated)::value;
+    return p.split > 1 ? pair_launch<T, G, true>(x, ldx, w, ldw, o, p, num_sms, stream)
+                       : pair_launch<T, G, false>(x, ldx, w, ldw, o, p, num_sms, stream);
+  };
+  if (gated) return go((__nv_bfloat16*)out, std::true_type{});
+  if (out_dtype == BF_DTYPE_F32) return go((float*)out, std::false_type{});
+  return go((__nv_bfloat16*)out, std::false_type{});
 }

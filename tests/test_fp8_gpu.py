@@ -435,3 +435,18 @@ def test_rows_that_are_there_already(cuda_device, M):
             call(x, a)
             call(rows, b)
             assert torch.equal(a, b) and a.any()
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("split", [2, 4])
+@pytest.mark.parametrize("M,K,N", [(1, 512, 128), (157, 1100, 300), (256, 2048, 1024), (300, 640, 130), (513, 4096, 256)])
+def test_linear_shared_by_pairs(cuda_device, M, K, N, split, gated):
+    out, ref = _linear(cuda_device, M, K, N, gated=gated, seed=split, tile=-1, split=split)
+    _check(out, *ref)
+
+
+@pytest.mark.parametrize("M,K,N", [(157, 4096, 6144), (300, 12288, 4096), (512, 2048, 1024), (700, 4096, 4096)])
+def test_middle_sizes_as_chosen(cuda_device, M, K, N):
+    for out_type in (BF16, F32):
+        out, ref = _linear(cuda_device, M, K, N, out_type=out_type)
+        _check(out, *ref)
