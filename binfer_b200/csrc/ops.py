@@ -2916,8 +2916,7 @@ def fp8_rows(x: torch.Tensor) -> Fp8Rows:
     NaN.  (The codes' rows are padded to 16 bytes: ``codes`` need not be contiguous.)"""
     dtype = _fp8_matrix("fp8_rows", "x", x)
     _same_device("fp8_rows", x)
-    shape, device = x.shape, x.device
-    T, K = shape
+    (T, K), device = x.shape, x.device
     codes, scales = _fp8_empty_rows(T, K, device)
     if T:
         _run("fp8_rows", _fp8_rows_call, x.data_ptr(), x.stride(0), codes.data_ptr(), -(-K // 16) * 16,
@@ -2960,16 +2959,20 @@ def fp8_rows_read(codes: torch.Tensor, scales: torch.Tensor, out: torch.Tensor) 
     dtype = _fp8_matrix("fp8_rows_read", "out", out)
     shape = out.shape
     T, K = shape
-    if codes.dtype != E4M3 or codes.shape != shape or (T and not _fp8_codes_lie(codes)):
-        raise KernelError("fp8_rows_read: codes must be float8_e4m3fn of out's shape, their rows contiguous and "
-                          "on 16-byte boundaries")
-    if scales.dtype != torch.float32 or scales.shape != (-(-K // FP8_GROUP), T) or (
-            T > 1 and scales.stride(1) != 1):
-        raise KernelError("fp8_rows_read: scales must be float32 [ceil(K / 128), T] with contiguous rows")
+    if codes.dtype != E4M3 or codes.shape != shape:
+        raise KernelError(f"fp8_rows_read: codes must be float8_e4m3fn of out's shape, got {codes.dtype} "
+                          f"{tuple(codes.shape)}")
+    if scales.dtype != torch.float32 or scales.shape != (-(-K // FP8_GROUP), T):
+        raise KernelError("fp8_rows_read: scales must be float32 [ceil(K / 128), T]")
+    (pitch, one), (lds, s_one), at = codes.stride(), scales.stride(), codes.data_ptr()
+    if T and ((one != 1 and K > 1) or pitch % 16 or pitch < K or at % 16 or (s_one != 1 and T > 1)):
+        raise KernelError("fp8_rows_read: rows of codes must be contiguous and on 16-byte boundaries, rows of scales "
+                          "contiguous")
     _same_device("fp8_rows_read", codes, scales, out)
-    if T:
-        _run("fp8_read", _fp8_read_call, codes.data_ptr(), codes.stride(0), scales.data_ptr(), scales.stride(0),
-             out.data_ptr(), out.stride(0), dtype, 0, 1, T, K, num_sms(out.device), _stream_at(out))
+    if T == 0:
+        return
+    _run("fp8_read", _fp8_read_call, at, pitch, scales.data_ptr(), lds, out.data_ptr(), out.stride(0), dtype, 0, 1, T,
+         K, num_sms(out.device), _stream_at(out))
 
 
 class Fp8Weight:
@@ -2999,11 +3002,16 @@ class Fp8Weight:
             laid = _fp8_empty_codes(codes.shape, codes.device)
             laid.view(torch.uint8).copy_(codes.view(torch.uint8))
             codes = laid
+        self._take(codes, scales, gated)
+
+    def _take(self, codes: torch.Tensor, scales: torch.Tensor, gated: bool) -> "Fp8Weight":
         self.codes, self.scales, self.gated = codes, scales, bool(gated)
+        *lead, self.rows, self.K = codes.shape
         self.experts = lead[0] if lead else 0
-        self.rows, self.features, self.K, self.device = n, features, k, codes.device
+        self.features, self.device = self.rows // 2 if gated else self.rows, codes.device
         self._held = (codes.data_ptr(), codes.stride(-2), scales.data_ptr())
         self._index = codes.get_device()
+        return self
 
     @property
     def shape(self):
@@ -3018,14 +3026,18 @@ def fp8_weight(w: torch.Tensor, gated: bool = False) -> Fp8Weight:
         raise KernelError("fp8_weight: w must have rows that are equally far apart, a gated one as many up rows "
                           "as gate rows")
     _same_device("fp8_weight", w)
-    *lead, n, k = w.shape
-    halves = 2 if gated else 1
-    codes = _fp8_empty_codes(w.shape, w.device)
-    scales = torch.empty((*lead, halves * -(-(n // halves) // FP8_GROUP), -(-k // FP8_GROUP)),
-                         dtype=torch.float32, device=w.device)
+    shape, device = w.shape, w.device
+    n, k, mats, halves = shape[-2], shape[-1], shape[0] if len(shape) == 3 else 1, 2 if gated else 1
+    if mats > FP8_MAX_EXPERTS:
+        raise KernelError(f"fp8_weight: at most {FP8_MAX_EXPERTS} experts")
+    blocks, groups = halves * -(-(n // halves) // FP8_GROUP), -(-k // FP8_GROUP)
+    codes = _fp8_empty_codes(shape, device)
+    size, strides = ((blocks, groups), (groups, 1)) if len(shape) == 2 else (
+        (mats, blocks, groups), (blocks * groups, groups, 1))
+    scales = torch.empty_strided(size, strides, dtype=torch.float32, device=device)
     _run("fp8_blocks", _fp8_blocks_call, w.data_ptr(), w.stride(-2), codes.data_ptr(), codes.stride(-2),
-         scales.data_ptr(), dtype, (lead[0] if lead else 1) * halves, n // halves, k, _stream_at(w))
-    return Fp8Weight(codes, scales, gated)
+         scales.data_ptr(), dtype, mats * halves, n // halves, k, _stream_at(w))
+    return Fp8Weight.__new__(Fp8Weight)._take(codes, scales, gated)
 
 
 def fp8_weight_read(w: Fp8Weight, out: torch.Tensor) -> None:
