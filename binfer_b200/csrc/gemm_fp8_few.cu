@@ -2,9 +2,8 @@
 // sum_{k in t} cx[m, k] cw[n, k] over the groups t of 128 columns (the format: fp8.cuh).
 //
 // The weight's rows are the product's rows (128 of them = 128 lanes of tensor memory) and the
-// activations' rows its columns, of which a tile has as many as there are, rounded up to 16: a decode
-// step's eight rows cost a sixteenth of what they would as the product's rows, and an expert with 37
-// rows pays for 48.  One tcgen05.mma.kind::f8f6f4 takes K = 32; the four of a group go into columns of
+// activations' rows its columns, of which a tile has as many as there are, rounded up to 16: nothing is
+// multiplied for rows that are not there, and an expert with 37 rows pays for 48.  One tcgen05.mma.kind::f8f6f4 takes K = 32; the four of a group go into columns of
 // tensor memory of their own, a ring of them, and the epilogue's warps add each group's sums, times its
 // two scales, into registers (float; the scales cannot ride along in tensor memory).
 //
@@ -13,9 +12,15 @@
 //   warp 2       the factors sx sw of every column of a group, into shared memory
 //   warps 4-11   the sums, times the factors, into registers; the result
 //
-// What bounds it with few rows is the weights' bytes; a tile is 128 rows of the weight, so that a
-// narrow weight alone does not give every SM work: then a cluster of `split` CTAs shares a tile, each a
-// part of the groups, and the parts meet in shared memory, added in the order of the ranks.
+// What bounds it with few rows is the weights' bytes (8 rows, 24,576 x 4,096 gated: 20.5 us with the rows'
+// codes, 5.4 TB/s) or, of narrow weights, the way from the last of them to the end: a group passes 350
+// cycles of the issuing warp and 230 and more of the sums', the parts of a cluster meet in 1 us (4,096 x 4,096:
+// 7.6 us, of which 1.5 are the rows' codes).  A tile is 128 rows of the weight, so that a narrow weight alone does
+// not give every SM work: then a cluster of `split` CTAs shares a tile, each a part of the groups, and the
+// parts meet in shared memory, added in the order of the ranks.
+// With more rows it is what a group costs beside its products (157 rows, 6,144 x 4,096: 17 us; the tensor
+// pipe is busy 4 % of the time at 8 rows).  The factors come by broadcast loads from shared memory, of which an
+// SM takes 128 bytes a cycle: with tiles of 128 columns that was the bound (1,030 cycles a group), so 64 is the most.
 // With experts the tiles are dealt out to persistent CTAs.
 //
 // RESIDENT: at most eight rows come as bfloat16, and every CTA puts its columns of them into 8 bits by
@@ -564,7 +569,7 @@ int few_launch(const void* x, long long ldx, const void* w, long long ldw, OutT*
   const long long tiles_r = (p.rows + NB - 1) / NB, room = (long long)FEW_PER_SM * num_sms;
   // (at most: `starts` may hold anything)
   const long long units = tiles_r * p.experts * p.tiles_f;
-  if (units > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+  if (units > 0x7fffffffLL || (long long)p.experts * HALVES * p.features > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
   if (p.starts || units * p.split > room || p.split > p.groups) p.split = 1;
   if (RESIDENT) {
     p.x = (const __nv_bfloat16*)x;

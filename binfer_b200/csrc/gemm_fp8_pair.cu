@@ -5,14 +5,20 @@
 // of the weight rows.  Here the activations are the product's rows, so that a thread has one row's
 // scale and the weight's scale is one number a group: one multiplication a group of 128 instead of one
 // factor per column.  The sums of a group (256 columns) go into one of two buffers of tensor memory;
-// eight warps per CTA, two to a quarter of the lanes, add them times the factor into 128 registers each
+// sixteen warps per CTA, four to a quarter of the lanes, add them times the factor into 64 registers each
 // while the products fill the other buffer.
 //
 //   warp 0       TMA: 128 activation rows and 128 weight rows x 128 bytes per stage
 //   warp 1       (leader) the products; TMEM allocation
-//   warps 4-11   the sums into registers; the result, turned in shared memory so that a warp writes
-//                whole 128-byte lines (these two warpgroups take 232 registers a thread, which the
-//                first leaves them: 128 x 40 + 256 x 232 = 384 x 168)
+//   warps 4-19   the sums into registers; the result, turned in shared memory so that a warp writes
+//                64 bytes a row (these four warpgroups take 104 registers a thread, which the first
+//                leaves them: 128 x 40 + 512 x 104 of the launch's 640 x 96)
+//
+// What bounds it: a group's 512 cycles of products and, per buffer, 700 more from the last product to the
+// sums' warps and back to the next (the pair's CTAs signal one another), over two buffers, which is all that
+// tensor memory has room for; the results of a tile, 5,000 cycles gated, which two groups of the next cover; and
+// the clock (2,048 rows, 24,576 x 4,096 gated: 210 us of 218 with the rows' codes, 1.96 PFLOP/s, tensor pipe busy
+// 46 % of the time; 1.67 GHz at 900 W when it runs on).  Eight warps with 128 sums each took 236 us.
 //
 // SPLIT: few tiles leave SMs idle, and `split` pairs share one, a cluster of twice as many CTAs: each adds up
 // its part of the groups, the parts meet in the shared memory that the ring had, a pair owning a slice of
@@ -172,92 +178,92 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   uint32_t next_phase = 0;
 
   if (warp < 4) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-  if (warp == 0) {
-    // --------------------------------------------------------------- copies
-    if (lane == 0) {
-      const uint32_t full_leader = pair_map(smem_u32(full), leader);
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int u = pair; u < units && ok && !*abort; u += pairs) {
-        const RowTile t = row_tile(tables, p.experts, p.tiles_f, PF_TILE, u);
-        for (int g = g0; g < g1; ++g) {
-          if (!mbar_wait(empty + stage, phase ^ 1, abort)) {
-            ok = false;
-            break;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 0) {
+      // --------------------------------------------------------------- copies
+      if (lane == 0) {
+        const uint32_t full_leader = pair_map(smem_u32(full), leader);
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int u = pair; u < units && ok && !*abort; u += pairs) {
+          const RowTile t = row_tile(tables, p.experts, p.tiles_f, PF_TILE, u);
+          for (int g = g0; g < g1; ++g) {
+            if (!mbar_wait(empty + stage, phase ^ 1, abort)) {
+              ok = false;
+              break;
+            }
+            uint8_t* dst = tiles + (size_t)stage * PF_STAGE;
+            const uint32_t bar = full_leader + 8u * (uint32_t)stage;
+            if (rank == 0) mbar_expect_tx(full + stage, 2u * (uint32_t)PF_STAGE);
+            pair_tma_load(dst, &map_x, bar, g * FK, t.row0 + (int)rank * 128);
+            if (GATED) {
+              const int o = t.expert * w_rows + t.ft * 128 + (int)rank * 64;
+              pair_tma_load(dst + PF_HALF, &map_w, bar, g * FK, o);
+              pair_tma_load(dst + PF_HALF + PF_HALF / 2, &map_w, bar, g * FK, o + p.features);
+            } else {
+              pair_tma_load(dst + PF_HALF, &map_w, bar, g * FK,
+                            t.expert * w_rows + t.ft * PF_TILE + (int)rank * 128);
+            }
+            if (++stage == PF_STAGES) {
+              stage = 0;
+              phase ^= 1;
+            }
           }
-          uint8_t* dst = tiles + (size_t)stage * PF_STAGE;
-          const uint32_t bar = full_leader + 8u * (uint32_t)stage;
-          if (rank == 0) mbar_expect_tx(full + stage, 2u * (uint32_t)PF_STAGE);
-          pair_tma_load(dst, &map_x, bar, g * FK, t.row0 + (int)rank * 128);
-          if (GATED) {
-            const int o = t.expert * w_rows + t.ft * 128 + (int)rank * 64;
-            pair_tma_load(dst + PF_HALF, &map_w, bar, g * FK, o);
-            pair_tma_load(dst + PF_HALF + PF_HALF / 2, &map_w, bar, g * FK, o + p.features);
-          } else {
-            pair_tma_load(dst + PF_HALF, &map_w, bar, g * FK,
-                          t.expert * w_rows + t.ft * PF_TILE + (int)rank * 128);
-          }
+        }
+        next = stage;
+        next_phase = phase;
+        // every arrival that the leader's commits send to this CTA's barriers lands before it ends
+        for (int s = 0; s < PF_STAGES && ok && !*abort; ++s) {
+          ok = mbar_wait(empty + stage, phase ^ 1, abort);
           if (++stage == PF_STAGES) {
             stage = 0;
             phase ^= 1;
           }
         }
       }
-      next = stage;
-      next_phase = phase;
-      // every arrival that the leader's commits send to this CTA's barriers lands before it ends
-      for (int s = 0; s < PF_STAGES && ok && !*abort; ++s) {
-        ok = mbar_wait(empty + stage, phase ^ 1, abort);
-        if (++stage == PF_STAGES) {
-          stage = 0;
-          phase ^= 1;
-        }
-      }
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------- products
-    if (rank == 0) {
-      const uint32_t idesc = fp8_idesc(PF_TILE, 256), elected = elect_one(), both = 3u << leader;
-      int stage = 0, buf = 0;
-      uint32_t phase = 0, buf_phase = 0;
-      bool ok = true, seen = false;                         // a look at the next group's tiles
-      for (int u = pair; u < units && ok; u += pairs) {
-        for (int g = g0; g < g1; ++g) {
-          if (!mbar_seen_or_wait_warp(seen, full + stage, phase, abort) ||
-              !mbar_wait_warp(acc_empty + buf, buf_phase ^ 1, abort)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t a_addr = smem_u32(tiles + (size_t)stage * PF_STAGE);
-          const uint64_t a_desc = umma_desc_k_sw128(a_addr);
-          const uint64_t b_desc = umma_desc_k_sw128(a_addr + PF_HALF);
+    } else if (warp == 1) {
+      // ------------------------------------------------------------- products
+      if (rank == 0) {
+        const uint32_t idesc = fp8_idesc(PF_TILE, 256), elected = elect_one(), both = 3u << leader;
+        int stage = 0, buf = 0;
+        uint32_t phase = 0, buf_phase = 0;
+        bool ok = true, seen = false;                         // a look at the next group's tiles
+        for (int u = pair; u < units && ok; u += pairs) {
+          for (int g = g0; g < g1; ++g) {
+            if (!mbar_seen_or_wait_warp(seen, full + stage, phase, abort) ||
+                !mbar_wait_warp(acc_empty + buf, buf_phase ^ 1, abort)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t a_addr = smem_u32(tiles + (size_t)stage * PF_STAGE);
+            const uint64_t a_desc = umma_desc_k_sw128(a_addr);
+            const uint64_t b_desc = umma_desc_k_sw128(a_addr + PF_HALF);
 #pragma unroll
-          for (int k = 0; k < FK / 32; ++k)
-            pair_umma_fp8(tmem_base + (uint32_t)(buf * 256), a_desc + (uint64_t)(2 * k),
-                          b_desc + (uint64_t)(2 * k), idesc, k > 0 ? 1u : 0u, elected);
-          pair_commit_by(acc_full + buf, both, elected);
-          pair_commit_by(empty + stage, both, elected);
-          if (++stage == PF_STAGES) {
-            stage = 0;
-            phase ^= 1;
+            for (int k = 0; k < FK / 32; ++k)
+              pair_umma_fp8(tmem_base + (uint32_t)(buf * 256), a_desc + (uint64_t)(2 * k),
+                            b_desc + (uint64_t)(2 * k), idesc, k > 0 ? 1u : 0u, elected);
+            pair_commit_by(acc_full + buf, both, elected);
+            pair_commit_by(empty + stage, both, elected);
+            if (++stage == PF_STAGES) {
+              stage = 0;
+              phase ^= 1;
+            }
+            if (++buf == 2) {
+              buf = 0;
+              buf_phase ^= 1;
+            }
+            seen = mbar_look(full + stage, phase);
           }
-          if (++buf == 2) {
-            buf = 0;
-            buf_phase ^= 1;
-          }
-          seen = mbar_look(full + stage, phase);
         }
       }
     }
-  }
-  if (SPLIT) {
-    __syncwarp();
-    pair_sync();                               // the ring is free in every CTA
-    pair_sync();                               // every part is in place
-  }
+    if (SPLIT) {
+      __syncwarp();
+      pair_sync();                               // the ring is free in every CTA
+      pair_sync();                               // every part is in place
+    }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
     // ----------------------------------------------------------------- sums
@@ -424,7 +430,7 @@ int pair_launch(const void* x, long long ldx, const void* w, long long ldw, OutT
   p.table_bytes = row_tables_bytes(p.experts);
   const long long tiles_r = (p.rows + PF_TILE - 1) / PF_TILE;
   const long long units = tiles_r * p.experts * p.tiles_f;
-  if (units > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+  if (units > 0x7fffffffLL || (long long)p.experts * (GATED ? 2 : 1) * p.features > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
   const size_t smem =
       1024 + ((PF_BARS + p.table_bytes + 1023) & ~1023) + PF_SUMS * PF_TURN + (size_t)PF_STAGES * PF_STAGE;
   const size_t smem_max =

@@ -3109,7 +3109,11 @@ def _fp8_product(what: str, x, w: Fp8Weight, starts, out, row_w, activation, lim
     if held:
         code = _fp8_product_call(0, 0, codes.data_ptr(), codes.stride(0), scales.data_ptr(), scales.stride(0), *behind)
     elif M <= 8 and starts is None and FP8_RESIDENT and not torch.cuda.is_current_stream_capturing():
-        code = _fp8_product_call(x.data_ptr(), x.stride(0), 0, 0, 0, 0, *behind)
+        # (not where the result may lie on the rows: its blocks would read what others have written)
+        x_at, stride, out_at = x.data_ptr(), x.stride(0), out.data_ptr()
+        if (x_at + 2 * ((M - 1) * stride + K) <= out_at
+                or out_at + (4, 2)[out_type] * ((M - 1) * out.stride(0) + features) <= x_at):
+            code = _fp8_product_call(x_at, stride, 0, 0, 0, 0, *behind)
     if code == -1 and not held:
         # the rows' codes and behind them their scales
         pitch = -(-K // 16) * 16

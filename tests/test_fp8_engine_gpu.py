@@ -119,3 +119,14 @@ def test_what_is_refused(cuda_device, tmp_path):
         Engine(m, "float32", weights="fp8", **kw)
     with pytest.raises(ValueError, match="8 bits"):
         Engine(H.make_pabelix_dir(tmp_path / "p", "A", BF16), "bfloat16", weights="fp8", **kw)
+
+
+def test_queries_alone(cuda_device, tmp_path):
+    """A layer that reads another one's pages projects its queries only: the first rows of the stacked weight."""
+    from binfer_b200.csrc import ops
+    mixer = _runner(H.make_model_dir(tmp_path, "M", BF16)).model.blocks[0].mixer
+    w, x = mixer._w_q(), torch.randn((7, mixer.hidden), device=cuda_device).to(BF16)
+    out = torch.empty((7, mixer.q_size), dtype=BF16, device=cuda_device)
+    ops.fp8_linear(x, w, out)
+    ref, off = P8.product(x, mixer.w_qkv.codes[:mixer.q_size].to(F32).to(F64), mixer.w_qkv.scales[:w.scales.shape[0]])
+    assert ((out.to(F64) - ref).abs() <= off + ref.abs() * 2.0 ** -8).all()

@@ -450,3 +450,17 @@ def test_middle_sizes_as_chosen(cuda_device, M, K, N):
     for out_type in (BF16, F32):
         out, ref = _linear(cuda_device, M, K, N, out_type=out_type)
         _check(out, *ref)
+
+
+@pytest.mark.parametrize("M", [1, 8, 40, 300])
+def test_result_in_the_rows_place(cuda_device, M):
+    from binfer_b200.csrc import ops
+    w = ops.fp8_weight(_w((512, 512), cuda_device))
+    wide = torch.empty((M, 1024), dtype=BF16, device=cuda_device)
+    x, ref = _x(M, 512, cuda_device, M), torch.empty((M, 512), dtype=BF16, device=cuda_device)
+    ops.fp8_linear(x, w, ref)
+    wide[:, 256:768] = x
+    ops.fp8_linear(wide[:, 256:768], w, wide[:, 512:])       # half of it over the rows
+    assert torch.equal(wide[:, 512:], ref)
+    ops.fp8_linear(x, w, x)
+    assert torch.equal(x, ref)
