@@ -11,14 +11,15 @@
 //   warp 0       TMA: 128 activation rows and 128 weight rows x 128 bytes per stage
 //   warp 1       (leader) the products; TMEM allocation
 //   warps 4-19   the sums into registers; the result, turned in shared memory so that a warp writes
-//                64 bytes a row (these four warpgroups take 104 registers a thread, which the first
-//                leaves them: 128 x 40 + 512 x 104 of the launch's 640 x 96)
+//                64 bytes a row (these four warpgroups take 112 registers a thread, which the first
+//                leaves them: 128 x 32 + 512 x 112 of the launch's 640 x 96; with 104 the products of 2,048
+//                rows and 24,576 x 4,096 gated took 210 us, now 201)
 //
-// What bounds it: a group's 512 cycles of products and, per buffer, 700 more from the last product to the
-// sums' warps and back to the next (the pair's CTAs signal one another), over two buffers, which is all that
-// tensor memory has room for; the results of a tile, 5,000 cycles gated, which two groups of the next cover; and
-// the clock (2,048 rows, 24,576 x 4,096 gated: 210 us of 218 with the rows' codes, 1.96 PFLOP/s, tensor pipe busy
-// 46 % of the time; 1.67 GHz at 900 W when it runs on).  Eight warps with 128 sums each took 236 us.
+// What bounds it: the sums' warps.  A group's products take 512 cycles, its 32 packed multiply-adds a warp 278 for
+// the four warps of a scheduler, but a warp executes 126 instructions a group in a chain of waits (2,048 rows,
+// 24,576 x 4,096 gated, 201 us without the rows' codes, 2.05 PFLOP/s: without fetching operands 6 us less, without
+// the results 26, with an eighth of the multiply-adds 50; products and signals alone 110).  When it runs on, the
+// clock too (1.67 GHz at 900 W).  Eight warps with 128 sums each took 236 us.
 //
 // SPLIT: few tiles leave SMs idle, and `split` pairs share one, a cluster of twice as many CTAs: each adds up
 // its part of the groups, the parts meet in the shared memory that the ring had, a pair owning a slice of
@@ -178,7 +179,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   uint32_t next_phase = 0;
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
     if (warp == 0) {
       // --------------------------------------------------------------- copies
       if (lane == 0) {
@@ -265,7 +266,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       pair_sync();                               // every part is in place
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
     // ----------------------------------------------------------------- sums
     // A warp's 64 columns: neighbours, or (gated) the gate rows' and the up rows' of 32 outputs.
     const int quarter = warp & 3, part = (warp - 4) >> 2;
