@@ -2959,6 +2959,8 @@ def fp8_rows_read(codes: torch.Tensor, scales: torch.Tensor, out: torch.Tensor) 
     dtype = _fp8_matrix("fp8_rows_read", "out", out)
     shape = out.shape
     T, K = shape
+    if T > 1 and out.stride(0) < K:
+        raise KernelError("fp8_rows_read: out's rows must not share memory")
     if codes.dtype != E4M3 or codes.shape != shape:
         raise KernelError(f"fp8_rows_read: codes must be float8_e4m3fn of out's shape, got {codes.dtype} "
                           f"{tuple(codes.shape)}")
@@ -2980,8 +2982,9 @@ class Fp8Weight:
     and ``scales`` float32 ``[(E,) blocks, ceil(K / 128)]``, one per 128 x 128 numbers; a number stands for
     code times scale.  ``gated``: the weight is a gate weight and an up weight of N / 2 rows each, one
     behind the other, and the up rows' blocks begin anew (blocks = 2 ceil(N / 2 / 128), else ceil(N / 128)).
-    Scales are positive and finite.  Codes whose rows do not lie on 16-byte boundaries are copied."""
-    __slots__ = ("codes", "scales", "gated", "experts", "rows", "features", "K", "device", "_held", "_index")
+    Scales are positive and finite.  Codes whose rows do not lie on 16-byte boundaries are copied.  The two
+    tensors may be written to, but not replaced."""
+    __slots__ = ("_codes", "_scales", "gated", "experts", "rows", "features", "K", "device", "_held", "_index")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, gated: bool = False):
         if codes.dtype != E4M3 or codes.dim() not in (2, 3) or not codes.numel():
@@ -3005,7 +3008,7 @@ class Fp8Weight:
         self._take(codes, scales, gated)
 
     def _take(self, codes: torch.Tensor, scales: torch.Tensor, gated: bool) -> "Fp8Weight":
-        self.codes, self.scales, self.gated = codes, scales, bool(gated)
+        self._codes, self._scales, self.gated = codes, scales, bool(gated)
         *lead, self.rows, self.K = codes.shape
         self.experts = lead[0] if lead else 0
         self.features, self.device = self.rows // 2 if gated else self.rows, codes.device
@@ -3013,9 +3016,28 @@ class Fp8Weight:
         self._index = codes.get_device()
         return self
 
+    def __copy__(self) -> "Fp8Weight":
+        return Fp8Weight.__new__(Fp8Weight)._take(self._codes, self._scales, self.gated)
+
+    def __reduce__(self):       # a deep copy, or one read back, has addresses of its own
+        # (as bytes: pickle does not take 8-bit floats)
+        return _fp8_weight_again, (self._codes.view(torch.uint8), self._scales, self.gated)
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._scales
+
     @property
     def shape(self):
-        return self.codes.shape
+        return self._codes.shape
+
+
+def _fp8_weight_again(codes: torch.Tensor, scales: torch.Tensor, gated: bool) -> Fp8Weight:
+    return Fp8Weight(codes.view(E4M3), scales, gated)
 
 
 def fp8_weight(w: torch.Tensor, gated: bool = False) -> Fp8Weight:
@@ -3045,6 +3067,8 @@ def fp8_weight_read(w: Fp8Weight, out: torch.Tensor) -> None:
     dtype = _fp8_matrix("fp8_weight_read", "out", out, (2, 3))
     if out.shape != w.shape or not _fp8_stacked(out):
         raise KernelError("fp8_weight_read: out must have the weight's shape, its rows equally far apart")
+    if out.shape[0] * out.shape[-2] > 1 and out.stride(-2) < w.K:
+        raise KernelError("fp8_weight_read: out's rows must not share memory")
     _same_device("fp8_weight_read", w.codes, w.scales, out)
     at, pitch, scales_at = w._held
     _run("fp8_read", _fp8_read_call, at, pitch, scales_at, 0, out.data_ptr(), out.stride(-2), dtype, 1,
@@ -3070,9 +3094,10 @@ def _fp8_product(what: str, x, w: Fp8Weight, starts, out, row_w, activation, lim
                               f"{tuple(shape)}")
         others = (x,)
     out_type = _FP8_DTYPES.get(out.dtype)
-    if out_type is None or out.shape != (M, features) or (M and features > 1 and out.stride(1) != 1):
-        raise KernelError(f"{what}: out must be bfloat16 or float32 [{M}, {features}] with contiguous rows, got "
-                          f"{out.dtype} {tuple(out.shape)}")
+    if (out_type is None or out.shape != (M, features) or (M and features > 1 and out.stride(1) != 1)
+            or (M > 1 and out.stride(0) < features)):
+        raise KernelError(f"{what}: out must be bfloat16 or float32 [{M}, {features}] with contiguous rows of their "
+                          f"own, got {out.dtype} {tuple(out.shape)}")
     act = 0
     if w.gated:
         if out_type != 1 or activation not in FUSED_ACTIVATIONS:
@@ -3131,12 +3156,12 @@ def fp8_linear(x: torch.Tensor, w: Fp8Weight, out: torch.Tensor, activation: str
                limit: float = 0.0, slope: float = 1.0, up_offset: float = 0.0, tile: int = 0,
                split: int = 0) -> None:
     """``out [M, N] = x [M, K] w^T`` for rows in bfloat16 and a weight in 8 bits: the rows go into 8 bits as
-    :func:`fp8_rows` puts them (or are there already: ``x`` an :class:`Fp8Rows`), the products of codes are added up in float and counted with their scales, 128
-    columns after another.  A gated weight: ``out = act(g) u`` of the product's two halves, ``activation`` as
-    in :func:`gated_act_mul` ("silu" or "clamped").  ``out``: bfloat16, or float32 for a weight that is not
-    gated; it may be a column block of a wider buffer.  A row's result does not depend on the other rows'
-    values.  ``tile``, ``split``: rows of a tile (16, 32 or 64; -1: on pairs of SMs) and SMs that share one (0: chosen
-    by the library)."""
+    :func:`fp8_rows` puts them (or are there already: ``x`` an :class:`Fp8Rows`), the products of codes are
+    added up in float and counted with their scales, 128 columns after another.  A gated weight:
+    ``out = act(g) u`` of the product's two halves, ``activation`` as in :func:`gated_act_mul` ("silu" or
+    "clamped").  ``out``: bfloat16, or float32 for a weight that is not gated; it may be a column block of a
+    wider buffer.  A row's result does not depend on the other rows' values.  ``tile``, ``split``: rows of a
+    tile (16, 32 or 64; -1: on pairs of SMs) and SMs that share one (0: chosen by the library)."""
     if w.experts:
         raise KernelError("fp8_linear: the weight has experts")
     _fp8_product("fp8_linear", x, w, None, out, None, activation, limit, slope, up_offset, tile, split)

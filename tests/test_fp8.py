@@ -1,4 +1,7 @@
 """Weights in 8 bits: the restatement, and what the operators refuse before anything reaches a GPU."""
+import copy
+import pickle
+
 import pytest
 import torch
 
@@ -173,3 +176,31 @@ def test_norm_into_8_bits_refuses(ops):
         assert "CUDA" not in str(e.value)
     with pytest.raises(ops.KernelError, match="CUDA"):
         ops.add_rmsnorm_fp8(**ok)
+
+
+def test_copies_have_tensors_of_their_own(ops):
+    w = ops.Fp8Weight((torch.randn(300, 200) * 3).to(E4M3), torch.rand(4, 2), gated=True)
+    for c in (copy.deepcopy(w), pickle.loads(pickle.dumps(w))):
+        assert c.gated and c.features == 150 and c.K == 200
+        assert c.codes.data_ptr() != w.codes.data_ptr() and c.scales.data_ptr() != w.scales.data_ptr()
+        assert c._held == (c.codes.data_ptr(), 208, c.scales.data_ptr())
+        assert torch.equal(c.codes.view(torch.uint8), w.codes.view(torch.uint8)) and torch.equal(c.scales, w.scales)
+    c = copy.copy(w)
+    assert c.codes is w.codes and c.scales is w.scales and c._held == w._held
+    for name in ("codes", "scales"):
+        with pytest.raises(AttributeError):
+            setattr(w, name, getattr(w, name).clone())
+
+
+def test_results_in_rows_that_share_memory_refused(ops):
+    w, x = ops.Fp8Weight(_codes(300, 200), torch.ones(3, 2)), torch.zeros(2, 200, dtype=BF16)
+    for fn in (lambda out: ops.fp8_linear(x, w, out),
+               lambda out: ops.fp8_linear(ops.Fp8Rows(_codes(2, 208)[:, :200], torch.ones(2, 2)), w, out)):
+        for out in (torch.zeros(300, dtype=BF16).expand(2, 300),
+                    torch.zeros(700, dtype=BF16).as_strided((2, 300), (299, 1))):
+            with pytest.raises(ops.KernelError, match="of their own"):
+                fn(out)
+    with pytest.raises(ops.KernelError, match="share memory"):
+        ops.fp8_rows_read(_codes(4, 32), torch.ones(1, 4), torch.zeros(32).expand(4, 32))
+    with pytest.raises(ops.KernelError, match="share memory"):
+        ops.fp8_weight_read(w, torch.zeros(200).expand(300, 200))

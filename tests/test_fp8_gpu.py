@@ -1,5 +1,7 @@
 """Weights in 8 bits: quantising, reading back and the products against their restatement in 64 bits."""
+import copy
 import gc
+import pickle
 
 import pytest
 import torch
@@ -464,3 +466,21 @@ def test_result_in_the_rows_place(cuda_device, M):
     assert torch.equal(wide[:, 512:], ref)
     ops.fp8_linear(x, w, x)
     assert torch.equal(x, ref)
+
+
+@pytest.mark.parametrize("M", [3, 40])
+def test_copies_of_a_weight(cuda_device, M):
+    """A deep copy, or a weight read back, has its own numbers; a shallow one has those of its source."""
+    from binfer_b200.csrc import ops
+    dev = cuda_device
+    w = ops.fp8_weight(_w((300, 200), dev, 5))
+    x = _x(M, 200, dev, 6)
+    want, got = (torch.empty((M, 300), dtype=F32, device=dev) for _ in range(2))
+    ops.fp8_linear(x, w, want)
+    copies = [copy.deepcopy(w), pickle.loads(pickle.dumps(w)), copy.copy(w)]
+    w.codes.view(torch.uint8).zero_()
+    for c in copies[:2]:
+        ops.fp8_linear(x, c, got)
+        assert torch.equal(got, want)
+    ops.fp8_linear(x, copies[2], got)
+    assert not got.any()
