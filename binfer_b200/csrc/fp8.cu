@@ -334,8 +334,7 @@ BF_EXPORT int bf_fp8_blocks(const Fp8BlocksCall* call) {
   const int blocks = (mat_rows + BF_FP8_GROUP - 1) / BF_FP8_GROUP;
   if (!on_16(codes, ldc, 1) || mats > 65535 || blocks > 65535) return (int)cudaErrorInvalidValue;
   uint8_t* c = (uint8_t*)codes;
-  // (launched the ordinary way, and no kernel behind it may begin before it has ended: the products
-  // ask for weights ahead of their wait for the kernels before them)
+  // (launched the ordinary way: what a model is loaded with gains nothing by an early start)
   auto go = [&](auto kern, auto* src) {
     kern<<<dim3(groups, blocks, call->mats), F8_THREADS, 0, call->stream>>>(
         src, call->ldw, c, call->ldc, call->scales, call->mat_rows, call->K);

@@ -43,6 +43,12 @@ __device__ __forceinline__ void umma_commit_by(uint64_t* bar, uint32_t elected) 
       "r"(elected)
       : "memory");
 }
+// A tile of a matrix into L2: nothing is read by this kernel, so what a kernel before it still writes there is
+// not missed (L2 is where all SMs meet).
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y)
+               : "memory");
+}
 // A look at a barrier that does not wait.
 __device__ __forceinline__ bool mbar_look(uint64_t* bar, uint32_t parity) {
   uint32_t ok;

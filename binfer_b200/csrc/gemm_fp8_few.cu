@@ -160,25 +160,19 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  auto load_w = [&](int stage, int g, int expert, int ft) {
-    uint8_t* dst = tiles + (size_t)stage * STAGE;
-    if (GATED) {
-      tma_load_2d(dst, &map_w, full + stage, g * FK, expert * w_rows + ft * 64);
-      tma_load_2d(dst + 64 * FK, &map_w, full + stage, g * FK, expert * w_rows + p.features + ft * 64);
-    } else {
-      tma_load_2d(dst, &map_w, full + stage, g * FK, expert * w_rows + ft * 128);
-    }
-  };
-  // The weights depend on no kernel of the stream before this one: without experts the first ring of
-  // them is asked for before the wait for those.
+  // A group's rows of the weight: one box, or (gated) the gate rows' and the up rows'.
+  constexpr int BOX = GATED ? 64 : 128;
+  auto first_row = [&](int expert, int ft, int half) { return expert * w_rows + half * p.features + ft * BOX; };
   // (clusters: nothing goes to a CTA that has not begun)
   if (p.split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  const int pre = p.starts ? 0 : min(STAGES, g1 - g0);
-  if (warp == 0 && lane == 0)
-    for (int i = 0; i < pre; ++i) {
-      mbar_expect_tx(full + i, STAGE);
-      load_w(i, g0 + i, 0, cluster / ((p.rows + NB - 1) / NB));
-    }
+  // Without experts a ring's worth of the weight goes into L2 before the wait for the kernels ahead.  No further: one
+  // of those may be writing it (a weight is made, or written to, like any tensor).
+  if (warp == 0 && lane == 0 && !p.starts) {
+    const int ft = cluster / ((p.rows + NB - 1) / NB);
+    for (int g = g0; g < min(g0 + STAGES, g1); ++g)
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h) tma_prefetch_2d(&map_w, g * FK, first_row(0, ft, h));
+  }
   __syncwarp();
   bf_pdl_wait();
   BF_TRACE_POINT(10 * BF_TR_FP8_GEMM + 1);
@@ -194,21 +188,20 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   if (warp == 0) {
     // --------------------------------------------------------------- copies
     if (lane == 0) {
-      int asked = 0;
       bool ok = true;
       for (int u = cluster; u < units && ok && !*abort; u += clusters) {
         const RowTile t = row_tile(tables, p.experts, p.tiles_f, NB, u);
-        for (int g = g0; g < g1; ++g, ++asked) {
-          if (asked >= pre) {
-            if (!mbar_wait(empty + stage, phase ^ 1, abort)) {
-              ok = false;
-              break;
-            }
-            mbar_expect_tx(full + stage, STAGE);
-            load_w(stage, g, t.expert, t.ft);
+        for (int g = g0; g < g1; ++g) {
+          if (!mbar_wait(empty + stage, phase ^ 1, abort)) {
+            ok = false;
+            break;
           }
-          if (!RESIDENT)
-            tma_load_2d(tiles + (size_t)stage * STAGE + FEW_W_BYTES, &map_x, full + stage, g * FK, t.row0);
+          mbar_expect_tx(full + stage, STAGE);
+          uint8_t* dst = tiles + (size_t)stage * STAGE;
+#pragma unroll
+          for (int h = 0; h < HALVES; ++h)
+            tma_load_2d(dst + h * BOX * FK, &map_w, full + stage, g * FK, first_row(t.expert, t.ft, h));
+          if (!RESIDENT) tma_load_2d(dst + FEW_W_BYTES, &map_x, full + stage, g * FK, t.row0);
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1;

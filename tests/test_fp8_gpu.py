@@ -484,3 +484,22 @@ def test_copies_of_a_weight(cuda_device, M):
         assert torch.equal(got, want)
     ops.fp8_linear(x, copies[2], got)
     assert not got.any()
+
+
+@pytest.mark.parametrize("resident", [True, False])
+@pytest.mark.parametrize("M", [1, 8, 20, 60, 300])
+def test_a_weight_that_the_kernel_ahead_writes(cuda_device, monkeypatch, M, resident):
+    """Codes that a kernel writes which lets its successor begin early: the product waits for them."""
+    from binfer_b200.csrc import ops
+    monkeypatch.setattr(ops, "FP8_RESIDENT", resident)
+    N, K = 19000, 512
+    x, scales = _x(M, K, cuda_device, M), torch.full((-(-N // 128), K // 128), 2.0 ** -6, device=cuda_device)
+    makes = [_w((N, K), cuda_device, i).mul_(9) for i in range(3)]
+    held = [ops.fp8_rows(m).codes.view(torch.uint8).clone() for m in makes]
+    want = [P8.product(x, h.view(E4M3).to(F32).to(F64), scales) for h in held]
+    torch.cuda.synchronize()
+    out = torch.empty((M, N), dtype=F32, device=cuda_device)
+    for i in [0, 1, 2] * 4:
+        # (the codes' memory is that of the turn before, which the allocator gives out again)
+        ops.fp8_linear(x, ops.Fp8Weight(ops.fp8_rows(makes[i]).codes, scales), out)
+        _check(out, *want[i])
