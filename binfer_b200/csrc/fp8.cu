@@ -93,24 +93,18 @@ __global__ void add_rmsnorm_fp8_kernel(float* __restrict__ resid, const __nv_bfl
   __shared__ float scratch[33];
   BF_TRACE_POINT(10 * BF_TR_FP8_NORM);
   bf_pdl_trigger();
-  // (the norm's weight depends on no kernel of the stream)
-  float f[TRIPS][8];
+  // (into L2 ahead of the wait, and no further: a kernel before this one may write the norm's weight)
 #pragma unroll
   for (int k = 0; k < TRIPS; ++k) {
     const int c = (k * blockDim.x + threadIdx.x) * 8;
-    if (c < H) {
-      const float4 wa = *reinterpret_cast<const float4*>(w + c);
-      const float4 wb = *reinterpret_cast<const float4*>(w + c + 4);
-      f[k][0] = wa.x; f[k][1] = wa.y; f[k][2] = wa.z; f[k][3] = wa.w;
-      f[k][4] = wb.x; f[k][5] = wb.y; f[k][6] = wb.z; f[k][7] = wb.w;
-    }
+    if (c < H && threadIdx.x % 4 == 0) asm volatile("prefetch.global.L2 [%0];" ::"l"(w + c));
   }
   bf_pdl_wait();
   BF_TRACE_POINT(10 * BF_TR_FP8_NORM + 1);
   const int r = blockIdx.x;
   float* x = resid + (size_t)r * H;
   const __nv_bfloat16* d = delta ? delta + (size_t)r * H : nullptr;
-  float v[TRIPS][8];
+  float v[TRIPS][8], f[TRIPS][8];
   float ss = 0.f;
 #pragma unroll
   for (int k = 0; k < TRIPS; ++k) {
@@ -118,6 +112,10 @@ __global__ void add_rmsnorm_fp8_kernel(float* __restrict__ resid, const __nv_bfl
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[k][j] = 0.f;
     if (c < H) {
+      const float4 wa = *reinterpret_cast<const float4*>(w + c);
+      const float4 wb = *reinterpret_cast<const float4*>(w + c + 4);
+      f[k][0] = wa.x; f[k][1] = wa.y; f[k][2] = wa.z; f[k][3] = wa.w;
+      f[k][4] = wb.x; f[k][5] = wb.y; f[k][6] = wb.z; f[k][7] = wb.w;
       const float4 a = *reinterpret_cast<const float4*>(x + c);
       const float4 b = *reinterpret_cast<const float4*>(x + c + 4);
       v[k][0] = a.x; v[k][1] = a.y; v[k][2] = a.z; v[k][3] = a.w;

@@ -503,3 +503,27 @@ def test_a_weight_that_the_kernel_ahead_writes(cuda_device, monkeypatch, M, resi
         # (the codes' memory is that of the turn before, which the allocator gives out again)
         ops.fp8_linear(x, ops.Fp8Weight(ops.fp8_rows(makes[i]).codes, scales), out)
         _check(out, *want[i])
+
+
+@pytest.mark.parametrize("H", [512, 4096])
+def test_a_norm_s_weight_that_the_kernel_ahead_writes(cuda_device, H):
+    """The norm's weight as the last row of what a kernel makes that lets its successor begin early."""
+    from binfer_b200.csrc import ops
+    T = 8192
+    made = torch.zeros((T, H), device=cuda_device)
+    g = torch.Generator(cuda_device).manual_seed(H)
+    resid = torch.randn((3, H), generator=g, device=cuda_device)
+    rows = [ops.fp8_rows(_x(T, H, cuda_device, i)) for i in range(2)]
+    want = []
+    for r in rows:
+        w, y = torch.empty((T, H), device=cuda_device), torch.empty((3, H), dtype=BF16, device=cuda_device)
+        ops.fp8_rows_read(*r, w)
+        torch.cuda.synchronize()
+        ops.add_rmsnorm(resid.clone(), None, w[-1], y, 1e-6)
+        want.append(ops.fp8_rows(y))
+    torch.cuda.synchronize()
+    for i in [0, 1] * 6:
+        ops.fp8_rows_read(*rows[i], made)
+        got = ops.add_rmsnorm_fp8(resid, None, made[-1], 1e-6)
+        assert torch.equal(got.scales, want[i].scales)
+        assert torch.equal(got.codes.view(torch.uint8), want[i].codes.view(torch.uint8))
