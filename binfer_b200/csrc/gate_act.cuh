@@ -5,7 +5,7 @@
 // ACT 1: the tanh form of gelu in silu's place,
 //   gelu(g) = 0.5 g (1 + tanh(sqrt(2/pi) (g + 0.044715 g^3))).
 // ACT 2: clamped, with three constants: g = min(gate, limit), u = clamp(up, -limit, limit),
-//   g sigmoid(slope g) (u + up_offset).
+//   g sigmoid(slope g) (u + up_offset); a NaN stays one (the plain minimum of a NaN and the limit is the limit).
 #pragma once
 #include "common.cuh"
 
@@ -30,11 +30,21 @@ __device__ __forceinline__ float bf_mix_weight(const BfMixture& m, int t, int o,
   k.limit = m.shared_limit;
   return m.shared_gate ? m.w[(size_t)t * m.cols + m.experts] : 1.f;
 }
+__device__ __forceinline__ float bf_min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float bf_max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 template <int ACT>
 __device__ __forceinline__ float bf_gate_mul(float g, float u, const BfGateConst& k) {
   if (ACT == BF_ACT_CLAMPED) {
-    g = fminf(g, k.limit);
-    u = fminf(fmaxf(u, -k.limit), k.limit) + k.up_offset;
+    g = bf_min_nan(g, k.limit);
+    u = bf_min_nan(bf_max_nan(u, -k.limit), k.limit) + k.up_offset;
     return g / (1.f + expf(-k.slope * g)) * u;
   }
   if (ACT == BF_ACT_GELU_TANH)
@@ -50,8 +60,8 @@ __device__ __forceinline__ float bf_silu_fast(float g) { return __fdividef(g, 1.
 template <int ACT>
 __device__ __forceinline__ float bf_gate_mul_fast(float g, float u, const BfGateConst& k) {
   if (ACT == BF_ACT_CLAMPED) {
-    g = fminf(g, k.limit);
-    u = fminf(fmaxf(u, -k.limit), k.limit) + k.up_offset;
+    g = bf_min_nan(g, k.limit);
+    u = bf_min_nan(bf_max_nan(u, -k.limit), k.limit) + k.up_offset;
     return __fdividef(g, 1.f + __expf(-k.slope * g)) * u;
   }
   if (ACT == BF_ACT_GELU_TANH) {

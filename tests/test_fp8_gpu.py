@@ -527,3 +527,32 @@ def test_a_norm_s_weight_that_the_kernel_ahead_writes(cuda_device, H):
         got = ops.add_rmsnorm_fp8(resid, None, made[-1], 1e-6)
         assert torch.equal(got.scales, want[i].scales)
         assert torch.equal(got.codes.view(torch.uint8), want[i].codes.view(torch.uint8))
+
+
+@pytest.mark.parametrize("act", [dict(), dict(activation="clamped", limit=1.5, slope=1.7, up_offset=1.0)])
+@pytest.mark.parametrize("M,kw", [(6, {}), (70, {}), (300, {}), (6, dict(split=1)), (8, dict(split=2)), (20, dict(split=3)),
+                                  (300, dict(tile=-1, split=2)), (300, dict(tile=-1, split=1)), (300, dict(tile=64))])
+def test_gated_rows_that_are_not_finite(cuda_device, M, kw, act):
+    """A row with an infinity or a NaN is NaN behind either activation, by every kernel; the others are what they were."""
+    from binfer_b200.csrc import ops
+    x, w = _x(M, 1024, cuda_device, M), ops.fp8_weight(_w((400, 1024), cuda_device), True)
+    a, b = (torch.empty((M, 200), dtype=BF16, device=cuda_device) for _ in range(2))
+    ops.fp8_linear(x, w, a, **act, **kw)
+    assert torch.isfinite(a).all()
+    x[1, 7], x[4, 900], x[5, 1023] = float("inf"), float("nan"), float("-inf")
+    ops.fp8_linear(x, w, b, **act, **kw)
+    bad = torch.tensor([1, 4, 5], device=cuda_device)
+    assert torch.isnan(b[bad]).all()
+    b[bad] = a[bad]
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("tile", [0, 16, -1])
+def test_experts_rows_that_are_not_finite(cuda_device, tile):
+    from binfer_b200.csrc import ops
+    x, w = _x(90, 256, cuda_device, 1), ops.fp8_weight(_w((3, 200, 256), cuda_device), True)
+    starts, out = torch.tensor([0, 20, 21, 90], dtype=torch.int32, device=cuda_device), torch.empty((90, 100), dtype=BF16,
+                                                                                                   device=cuda_device)
+    x[20, 3] = x[89, 255] = float("nan")
+    ops.fp8_experts(x, w, starts, out, activation="clamped", limit=2.0, up_offset=1.0, tile=tile)
+    assert torch.isnan(out[[20, 89]]).all() and torch.isfinite(out[:20]).all() and torch.isfinite(out[21:89]).all()

@@ -809,3 +809,34 @@ def test_trace_replay_tool_with_four_requests(cuda_device, tmp_path):
     ref = {rid: P.forward(raw, w, toks) for rid, toks in reqs.items()}
     worst = max(H.rel_err(row, ref[rid][p]) for (rid, p), row in got.items())
     assert got and worst <= TOL[torch.float32], f"worst relative error {worst:.3g}"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("inner", [33, 256])
+def test_clamped_activation_keeps_nan(cuda_device, dtype, inner):
+    """As a clamp does: a NaN is not a number above the limit."""
+    from binfer_b200.csrc import ops
+    gu = torch.randn((4, 2 * inner), device=cuda_device).to(dtype)
+    gu[0, 3], gu[1, inner + 5], gu[2, inner - 1] = float("nan"), float("nan"), float("inf")
+    out = torch.empty((4, inner), dtype=dtype, device=cuda_device)
+    ops.gated_act_mul(gu, out, "clamped", limit=2.0, slope=1.702, up_offset=1.0)
+    bad = torch.zeros((4, inner), dtype=torch.bool, device=cuda_device)
+    bad[0, 3] = bad[1, 5] = True
+    assert torch.equal(torch.isnan(out), bad)
+
+
+@pytest.mark.parametrize("tokens", [3, 600])
+def test_products_with_the_clamped_activation_keep_nan(cuda_device, tokens):
+    from binfer_b200.csrc import ops
+    inner = 2048
+    x = torch.randn((tokens, 256), device=cuda_device).to(torch.bfloat16)
+    w = (torch.randn((2 * inner, 256), device=cuda_device) * 0.06).to(torch.bfloat16)
+    out, err = torch.empty((tokens, inner), dtype=torch.bfloat16, device=cuda_device), ops.error_word(cuda_device)
+    x[1, 9] = float("nan")
+    kw = dict(activation="clamped", limit=2.0, slope=1.702, up_offset=1.0)
+    if tokens <= 64:
+        plan = ops.gemm_swiglu_plan(inner, 256, cuda_device)
+        assert plan and ops.gemm_bf16_swiglu(x, w, out, err, plan[0], **kw)
+    else:
+        assert ops.gemm_bf16_pair(x, w, out, err, gated=True, **kw)
+    assert torch.isnan(out[1]).all() and int(torch.isnan(out).sum()) == inner
