@@ -137,9 +137,34 @@ struct Fp8Sixteen {
     return make_uint4(c[0], c[1], c[2], c[3]);
   }
 };
-// The factor of a group's sums: the product of two scales, held at the largest float, so that a sum of
-// zero stays zero where the product alone is out of range.  (NaN stays NaN.)
-__device__ __forceinline__ float fp8_factor(float sx, float sw) {
+// The factor of a group's sums is the product of two scales.  Scales that are both small or both large have products
+// below the floats of full precision, or above all of them, while the product with the sum, of up to 2^25 or down to
+// 2^-18, may well be one.  The kernels' loops take such a factor as zero, or as infinity; warps that have the time look
+// for them beside (fp8_odd), and at a tile's end the results that they concern are made anew (fp8_anew).
+__device__ __forceinline__ float fp8_loop_factor(float sx, float sw) {
+  float f;
+  asm("mul.ftz.f32 %0, %1, %2;" : "=f"(f) : "f"(sx), "f"(sw));
+  return f;
+}
+// A factor as two: the sum times `before`, and that times `after`, a power of two, within a multiply-add.  Of s1 s2 in
+// 2^-175 .. 2^-126 the first lies in 2^-75 .. 2^-26, of 2^128 .. 2^239 in 2^8 .. 2^119, so that its product with the
+// sum underflows nowhere and overflows only where the result does.  (Times less than 2^-175 a sum is less than half of
+// the smallest float: nothing, as for two groups of zeros.)
+struct Fp8Factor {
+  float before, after;
+};
+__device__ __forceinline__ Fp8Factor fp8_factor(float sx, float sw) {
   const float f = sx * sw;
-  return f > 3.4028234663852886e38f ? 3.4028234663852886e38f : f;
+  if (f > 3.4028234663852886e38f) return Fp8Factor{(sx * 0x1p-60f) * (sw * 0x1p-60f), 0x1p120f};
+  if (f < 0x1p-126f) {
+    const float before = (sx * 0x1p50f) * (sw * 0x1p50f);
+    if (before >= 0x1p-75f) return Fp8Factor{before, 0x1p-100f};
+  }
+  return Fp8Factor{f, 1.f};
+}
+// FP8_ODD and more for a product that is no positive float of full precision (the only ones that can be odd)
+#define FP8_ODD 0x7f000000u
+__device__ __forceinline__ uint32_t fp8_note(float f) { return __float_as_uint(f) - 0x00800000u; }
+__device__ __forceinline__ bool fp8_odd(float sx, float sw) {
+  return fp8_note(sx * sw) >= FP8_ODD && fp8_factor(sx, sw).after != 1.f;
 }

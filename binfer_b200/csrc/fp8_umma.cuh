@@ -3,6 +3,7 @@
 #include <cuda.h>
 #include <stdint.h>
 
+#include "fp8.cuh"
 #include "gate_act.cuh"
 #include "tma_utils.cuh"
 #include "umma_utils.cuh"
@@ -131,7 +132,7 @@ __device__ __forceinline__ RowTables row_tables_at(void* smem, int E) {
   int* p = reinterpret_cast<int*>(smem);
   return RowTables{p, p + E, p + 2 * E};
 }
-static inline int row_tables_bytes(int E) { return ((3 * E + 1) * 4 + 127) & ~127; }
+__host__ __device__ __forceinline__ int row_tables_bytes(int E) { return ((3 * E + 1) * 4 + 127) & ~127; }
 // by the whole block; a __syncthreads() behind it
 __device__ __forceinline__ void fill_row_tables(const RowTables& t, const int* starts, int E, int rows,
                                                 int tile) {
@@ -189,6 +190,41 @@ static inline int fp8_map(CUtensorMap* map, const void* base, long long rows, lo
                          estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
+}
+
+// up to four codes, of which `left` are there
+__device__ __forceinline__ uint32_t fp8_word(const uint8_t* p, int left) {
+  if (left >= 4) return *reinterpret_cast<const uint32_t*>(p);
+  uint32_t r = 0u;
+  for (int j = 0; j < left; ++j) r |= (uint32_t)p[j] << (8 * j);
+  return r;
+}
+// Whether a result has a factor that is no float of full precision (fp8.cuh) among the groups g0 .. g1 - 1, and its sum
+// over them, by multiply-adds.  scale_x(g), scale_w(g): the groups' scales; x(g, k), w(g, k): where their codes
+// k .. k + 3 lie (k a multiple of 4).  K: columns in all.  By one thread; slow, and rare.
+template <typename SX, typename SW>
+__device__ bool fp8_any_odd(int g0, int g1, SX scale_x, SW scale_w) {
+  for (int g = g0; g < g1; ++g)
+    if (fp8_odd(scale_x(g), scale_w(g))) return true;
+  return false;
+}
+template <typename SX, typename SW, typename X, typename W>
+__device__ float fp8_sum_anew(int g0, int g1, int K, SX scale_x, SW scale_w, X x, W w) {
+  float acc = 0.f;
+  for (int g = g0; g < g1; ++g) {
+    const Fp8Factor f = fp8_factor(scale_x(g), scale_w(g));
+    const int n = min(FK, K - g * FK);
+    float sum = 0.f;
+    for (int k = 0; k < n; k += 4) {
+      float a[4], b[4];
+      fp8_values4(fp8_word(x(g, k), n - k), a);
+      fp8_values4(fp8_word(w(g, k), n - k), b);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum = fmaf(a[j], b[j], sum);
+    }
+    acc = fmaf(sum * f.before, f.after, acc);
+  }
+  return acc;
 }
 
 __device__ __forceinline__ float fp8_gate(int act, float g, float u, const BfGateConst& k) {

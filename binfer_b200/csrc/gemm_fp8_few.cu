@@ -9,7 +9,7 @@
 //
 //   warp 0       TMA: 128 weight rows and NB activation rows x 128 bytes per stage
 //   warp 1       the products; TMEM allocation
-//   warp 2       the factors sx sw of every column of a group, into shared memory
+//   warp 2       the factors sx sw of every column of a group, into shared memory; whether one is no float (fp8.cuh)
 //   warps 4-11   the sums, times the factors, into registers; the result
 //
 // What bounds it with few rows is the weights' bytes (8 rows, 24,576 x 4,096 gated: 20.5 us with the rows'
@@ -67,6 +67,8 @@ struct FewParams {
   const float* sw;                     // [experts * (gated ? 2 : 1) * w_blocks, groups]
   const float* row_w;                  // per row, or null
   int split, stages, table_bytes;
+  const uint8_t *codes, *w;            // what the tensor maps show
+  long long ldw;
   const __nv_bfloat16* x;              // RESIDENT: the rows, res_groups groups of each in a CTA
   long long ldx;
   int x_vec, res_groups;
@@ -107,7 +109,8 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* factors = reinterpret_cast<float*>(base + FEW_BARS);            // [SLOTS][HALVES][NB]
-  float* exchange = factors + SLOTS * HALVES * NB;       // gated: up sums; split: the parts sent here
+  int* odd = reinterpret_cast<int*>(factors + SLOTS * HALVES * NB);      // [16]: of a tile's last group, whether it has odd factors
+  float* exchange = reinterpret_cast<float*>(odd + 16);  // gated: up sums; split: the parts sent here
   uint8_t* table_smem = reinterpret_cast<uint8_t*>(exchange) +
                         (p.split > 1 ? ((NB + p.split - 1) / p.split) * p.split * 128 * 4
                                      : GATED ? FewShape<NB>::EXCHANGE : 0);
@@ -275,9 +278,9 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
           const int row = t.row0 + j * 32 + lane;
           if (RESIDENT) {
             if (i == 0 && j == 0) ok = mbar_wait_warp(ready + (min(ga + AHEAD, g1) - 1 - g0) / per_round, 0, abort);
-            sx[i][j] = row < t.row_end ? res_sx[(g - g0) * NB + row] : 0.f;
+            sx[i][j] = row < t.row_end ? res_sx[(g - g0) * NB + row] : 1.f;
           } else {
-            sx[i][j] = row < t.row_end && j * 32 + lane < NB ? p.sx[(long long)g * p.lds + row] : 0.f;
+            sx[i][j] = row < t.row_end && j * 32 + lane < NB ? p.sx[(long long)g * p.lds + row] : 1.f;
           }
         }
 #pragma unroll
@@ -291,6 +294,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
       ask(t, g0);
     }
     for (; u < units && ok; u += clusters) {
+      bool odd_here = false;
       for (int ga = g0; ga < g1 && ok; ga += AHEAD) {
         float f[AHEAD][PER * HALVES];
 #pragma unroll
@@ -298,7 +302,10 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
 #pragma unroll
           for (int j = 0; j < PER; ++j)
 #pragma unroll
-            for (int h = 0; h < HALVES; ++h) f[i][j * HALVES + h] = fp8_factor(sx[i][j], sw[i][h]);
+            for (int h = 0; h < HALVES; ++h) {
+              f[i][j * HALVES + h] = fp8_loop_factor(sx[i][j], sw[i][h]);
+              odd_here = odd_here || fp8_odd(sx[i][j], sw[i][h]);
+            }
         if (ga + AHEAD < g1) {
           ask(t, ga + AHEAD);
         } else if (u + clusters < units) {
@@ -318,6 +325,10 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
 #pragma unroll
             for (int h = 0; h < HALVES; ++h)
               if (j * 32 + lane < NB) dst[h * NB + j * 32 + lane] = f[i][j * HALVES + h];
+          if (ga + i == g1 - 1) {
+            const int any = __any_sync(0xffffffffu, odd_here);
+            if (lane == 0) odd[slot] = any;
+          }
           __syncwarp();
           if (lane == 0) mbar_arrive(acc_full + slot);
           if (++slot == SLOTS) {
@@ -377,6 +388,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
 #pragma unroll
         for (int j = 0; j < CH; ++j) acc[i][j] = 0.f;
       bool ok = true;
+      int tile_odd = 0;
       for (int g = g0; g < g1; ++g) {
         if (!mbar_wait_warp(acc_full + slot, slot_phase, abort)) {
           ok = false;
@@ -403,6 +415,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
             }
           }
         }
+        if (g == g1 - 1) tile_odd = odd[slot];           // (before the slot goes back)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(acc_empty + slot);
@@ -411,6 +424,30 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
           slot_phase ^= 1;
         }
       }
+      const int feature = t.ft * BOX + (lane_row & (BOX - 1));
+      // (rare) what has such a factor anew: the sum over this CTA's groups
+      if (ok && tile_odd && feature < p.features) {
+        const uint8_t* wr = p.w + ((long long)t.expert * w_rows + which * p.features + feature) * p.ldw;
+        const float* swr =
+            p.sw + ((long long)t.expert * HALVES * p.w_blocks + which * p.w_blocks + (feature >> 7)) * p.groups;
+        for (int a = 0; a < CHUNKS * CH; ++a) {
+          const int c = (2 * (a / CH) + half) * CH + a % CH, row = t.row0 + c;
+          if (c >= n) continue;
+          auto scale_x = [&](int g) { return RESIDENT ? res_sx[(g - g0) * NB + c] : p.sx[g * p.lds + row]; };
+          auto scale_w = [&](int g) { return swr[g]; };
+          if (!fp8_any_odd(g0, g1, scale_x, scale_w)) continue;
+          const float v = fp8_sum_anew(
+              g0, g1, p.K, scale_x, scale_w,
+              [&](int g, int k) -> const uint8_t* {
+                if (RESIDENT) return res + ((g - g0) * FEW_RES_ROWS + c) * FK + (((k >> 4) ^ (c & 7)) << 4) + (k & 15);
+                return p.codes + row * p.ldx + g * FK + k;
+              },
+              [&](int g, int k) { return wr + g * FK + k; });
+#pragma unroll
+          for (int i = 0; i < CHUNKS * CH; ++i) acc[i / CH][i % CH] = i == a ? v : acc[i / CH][i % CH];
+        }
+      }
+      __syncwarp();
       if (p.split > 1) {
         // column j goes to rank j % split: [rank][its number there][weight row]
         const int per = (NB + p.split - 1) / p.split;
@@ -532,7 +569,7 @@ template <int NB, bool GATED, bool RESIDENT>
 size_t few_memory(const FewParams& p, int* stages) {
   const size_t extra = p.split > 1 ? (size_t)((NB + p.split - 1) / p.split) * p.split * 128 * 4
                                    : GATED ? FewShape<NB>::EXCHANGE : 0;
-  size_t fixed = FEW_BARS + (size_t)FewShape<NB>::SLOTS * (GATED ? 2 : 1) * NB * 4 + extra + p.table_bytes;
+  size_t fixed = FEW_BARS + (size_t)FewShape<NB>::SLOTS * (GATED ? 2 : 1) * NB * 4 + 16 * 4 + extra + p.table_bytes;
   if (RESIDENT) fixed += (size_t)p.res_groups * NB * 4;
   fixed = 1024 + ((fixed + 1023) & ~(size_t)1023);
   if (RESIDENT) fixed += (size_t)p.res_groups * FEW_RES_ROWS * FK;
@@ -564,9 +601,12 @@ int few_launch(const void* x, long long ldx, const void* w, long long ldw, OutT*
   const long long units = tiles_r * p.experts * p.tiles_f;
   if (units > 0x7fffffffLL || (long long)p.experts * HALVES * p.features > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
   if (p.starts || units * p.split > room || p.split > p.groups) p.split = 1;
+  p.codes = (const uint8_t*)x;
+  p.w = (const uint8_t*)w;
+  p.ldx = ldx;
+  p.ldw = ldw;
   if (RESIDENT) {
     p.x = (const __nv_bfloat16*)x;
-    p.ldx = ldx;
     p.x_vec = ldx % 8 == 0 && ((uintptr_t)x & 15) == 0;
     p.res_groups = (p.groups + p.split - 1) / p.split;
     int per_round = 32;

@@ -10,6 +10,7 @@
 //
 //   warp 0       TMA: 128 activation rows and 128 weight rows x 128 bytes per stage
 //   warp 1       (leader) the products; TMEM allocation
+//   warps 2, 3   look for products of two scales that are no floats of full precision
 //   warps 4-19   the sums into registers; the result, turned in shared memory so that a warp writes
 //                64 bytes a row (these four warpgroups take 112 registers a thread, which the first
 //                leaves them: 128 x 32 + 512 x 112 of the launch's 640 x 96; with 104 the products of 2,048
@@ -47,10 +48,13 @@ constexpr int PF_STAGES = 5;
 constexpr int PF_BARS = 512;
 constexpr int PF_TURN = 32 * 64;              // a warp's rows on their way out: 32 x 64 bytes
 
+// (128 bytes: of a longer one the compiler makes a copy, which cost 8,088 rows of a mixture 4 of 43 us)
 struct PairParams {
   int rows, features, K, groups;
-  int experts, tiles_f, w_blocks, table_bytes;
+  int experts, tiles_f, w_blocks;
   int split;                            // SPLIT: 2 or 4
+  const uint8_t *x, *w;                 // what the tensor maps show ...
+  uint32_t ldx16, ldw16;                // ... whose rows are so many times 16 bytes apart
   const int* starts;
   const float* sx;
   long long lds;
@@ -61,6 +65,7 @@ struct PairParams {
   BfGateConst gk;
   int* err;
 };
+static_assert(sizeof(PairParams) <= 128, "see above");
 
 __device__ __forceinline__ void pair_umma_fp8(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc,
                                               uint32_t idesc, uint32_t accumulate, uint32_t elected) {
@@ -136,8 +141,9 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   uint64_t* drain = acc_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* odd = abort + 1;               // not zero: some tile of this CTA has a factor that is no float (fp8.cuh)
   const RowTables tables = row_tables_at(base + PF_BARS, p.experts);
-  uint8_t* turn = base + ((PF_BARS + p.table_bytes + 1023) & ~1023);
+  uint8_t* turn = base + ((PF_BARS + row_tables_bytes(p.experts) + 1023) & ~1023);
   uint8_t* tiles = turn + PF_SUMS * PF_TURN;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -157,6 +163,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       mbar_init(acc_empty + a, 2 * PF_SUMS);   // one arrival per warp of both CTAs' sums
     }
     mbar_init(drain, 1);
+    *odd = 0;
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -260,11 +267,49 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         }
       }
     }
+    if (warp >= 2) {
+      // ------------------------------------------------- factors that are no floats
+      // Two warps that have nothing else to do look for them: the scales of a tile's rows (64 rows a warp) times
+      // those of its two blocks of the weight (SPLIT: of this pair's groups; the others of the cluster are told).
+      bool any = false;
+      for (int u = pair; u < units; u += pairs) {
+        const RowTile t = row_tile(tables, p.experts, p.tiles_f, PF_TILE, u);
+        const int row = t.row0 + (int)rank * 128 + (warp & 1) * 64 + lane;
+        const float *s0 = p.sx + min(row, t.row_end - 1), *s1 = p.sx + min(row + 32, t.row_end - 1);
+        const float* w0 = p.sw + ((long long)t.expert * (GATED ? 2 : 1) * p.w_blocks + (GATED ? t.ft : t.ft * 2)) * p.groups;
+        const float* w1 = w0 + (GATED ? (long long)p.w_blocks : t.ft * 2 + 1 < p.w_blocks ? 1LL : 0LL) * p.groups;
+        for (int first = g0; first < g1; first += 32) {
+          const int n = min(32, g1 - first);
+          const float a = w0[first + min(lane, n - 1)], b = w1[first + min(lane, n - 1)];
+          uint32_t note = 0u;
+#pragma unroll 4
+          for (int i = 0; i < n; ++i) {
+            const float wa = __shfl_sync(0xffffffffu, a, i), wb = __shfl_sync(0xffffffffu, b, i);
+            const float x0 = s0[(first + i) * p.lds], x1 = s1[(first + i) * p.lds];
+            note = max(max(fp8_note(x0 * wa), fp8_note(x0 * wb)), note);
+            note = max(max(fp8_note(x1 * wa), fp8_note(x1 * wb)), note);
+          }
+          if (__any_sync(0xffffffffu, note >= FP8_ODD))
+            for (int i = 0; i < n; ++i) {
+              const float wa = __shfl_sync(0xffffffffu, a, i), wb = __shfl_sync(0xffffffffu, b, i);
+              const float x0 = s0[(first + i) * p.lds], x1 = s1[(first + i) * p.lds];
+              any = any || fp8_odd(x0, wa) || fp8_odd(x0, wb) || fp8_odd(x1, wa) || fp8_odd(x1, wb);
+            }
+        }
+      }
+      if (any)
+        for (int q = 0; q < split; ++q)
+          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(
+                           pair_map(smem_u32(const_cast<int*>(odd)), (SPLIT ? 2u * (uint32_t)q : leader) + rank)),
+                       "r"(1)
+                       : "memory");
+    }
     if (SPLIT) {
       __syncwarp();
       pair_sync();                               // the ring is free in every CTA
       pair_sync();                               // every part is in place
     }
+    if (warp >= 2) named_sync(1, (PF_SUMS + 2) * 32);
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
     // ----------------------------------------------------------------- sums
@@ -295,7 +340,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       bool ok = true;
       float s = *sx, wa = *swa, wb = GATED ? swa[to_b] : 0.f;
       for (int g = g0; g < g1; ++g) {
-        const float fa = fp8_factor(s, wa), fb = GATED ? fp8_factor(s, wb) : fa;
+        const float fa = fp8_loop_factor(s, wa), fb = GATED ? fp8_loop_factor(s, wb) : fa;
         if (g + 1 < g1) {                                    // the next group's, under this one's wait
           sx += p.lds;
           ++swa;
@@ -391,6 +436,35 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       pair_sync();
       pair_sync();
     }
+    named_sync(1, (PF_SUMS + 2) * 32);
+    if (*odd && !*abort) {
+      // (rare) Results with such factors anew, over what the warp has stored.  A thread has its row of the warp's tiles;
+      // the weight's rows that the warp's columns are lie in one block, or (gated) in two.
+      for (int u = pair; u < units; u += pairs) {
+        const RowTile t = row_tile(tables, p.experts, p.tiles_f, PF_TILE, u);
+        const int row = t.row0 + (int)rank * 128 + quarter * 32 + lane;
+        const int o0 = GATED ? t.ft * 128 + part * 32 : t.ft * PF_TILE + part * 64;
+        if (row >= t.row_end || o0 >= p.features || (SPLIT && (split == 4 ? part : part >> 1) != share)) continue;
+        const uint8_t* xr = p.x + (size_t)row * p.ldx16 * 16;
+        const float* swa = p.sw + ((long long)t.expert * (GATED ? 2 : 1) * p.w_blocks + (o0 >> 7)) * p.groups;
+        auto scale_x = [&](int g) { return p.sx[g * p.lds + row]; };
+        auto scale_w = [&](int up) {
+          return [at = swa + (long long)up * p.w_blocks * p.groups](int g) { return at[g]; };
+        };
+        auto sum = [&](int o, int up) {
+          const uint8_t* wr = p.w + ((size_t)t.expert * w_rows + up * p.features + o) * p.ldw16 * 16;
+          return fp8_sum_anew(
+              0, p.groups, p.K, scale_x, scale_w(up), [&](int g, int k) { return xr + g * FK + k; },
+              [&](int g, int k) { return wr + g * FK + k; });
+        };
+        if (!fp8_any_odd(0, p.groups, scale_x, scale_w(0)) && (!GATED || !fp8_any_odd(0, p.groups, scale_x, scale_w(1))))
+          continue;
+        const float w = p.row_w ? p.row_w[row] : 1.f;
+        for (int o = o0; o < min(o0 + (GATED ? 32 : 64), p.features); ++o)
+          bf_st(out + (long long)row * p.ldo + o,
+                w * (GATED ? fp8_gate(p.act, sum(o, 0), sum(o, 1), p.gk) : sum(o, 0)));
+      }
+    }
   }
 
   // ------------------------------------------------------------------ wind-down
@@ -428,12 +502,15 @@ int pair_launch(const void* x, long long ldx, const void* w, long long ldw, OutT
   p.tiles_f = (p.features + (GATED ? 127 : PF_TILE - 1)) / (GATED ? 128 : PF_TILE);
   p.w_blocks = (p.features + 127) / 128;
   p.groups = (p.K + FK - 1) / FK;
-  p.table_bytes = row_tables_bytes(p.experts);
+  p.x = (const uint8_t*)x;
+  p.w = (const uint8_t*)w;
+  p.ldx16 = (uint32_t)(ldx / 16);
+  p.ldw16 = (uint32_t)(ldw / 16);
   const long long tiles_r = (p.rows + PF_TILE - 1) / PF_TILE;
   const long long units = tiles_r * p.experts * p.tiles_f;
   if (units > 0x7fffffffLL || (long long)p.experts * (GATED ? 2 : 1) * p.features > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
   const size_t smem =
-      1024 + ((PF_BARS + p.table_bytes + 1023) & ~1023) + PF_SUMS * PF_TURN + (size_t)PF_STAGES * PF_STAGE;
+      1024 + ((PF_BARS + row_tables_bytes(p.experts) + 1023) & ~1023) + PF_SUMS * PF_TURN + (size_t)PF_STAGES * PF_STAGE;
   const size_t smem_max =
       1024 + ((PF_BARS + row_tables_bytes(FP8_MAX_EXPERTS) + 1023) & ~1023) + PF_SUMS * PF_TURN +
       (size_t)PF_STAGES * PF_STAGE;
@@ -482,7 +559,7 @@ BF_EXPORT int bf_gemm_fp8_pair(const void* x, long long ldx, const float* sx, lo
                                int experts, int gated, int act, float limit, float slope, float up_offset,
                                int split, int num_sms, int* err, cudaStream_t stream) {
   if (rows <= 0 || features <= 0) return 0;
-  if (K <= 0 || experts < 1 || experts > FP8_MAX_EXPERTS || (!starts && experts != 1) || ldx % 16 || ldw % 16 ||
+  if (K <= 0 || experts < 1 || experts > FP8_MAX_EXPERTS || (!starts && experts != 1) || ldx % 16 || ldw % 16 || ldx >> 35 || ldw >> 35 ||
       (((uintptr_t)x | (uintptr_t)w) & 15) || num_sms < 2 ||
       (act != BF_ACT_SILU && act != BF_ACT_CLAMPED) || (gated && out_dtype != BF_DTYPE_BF16))
     return (int)cudaErrorInvalidValue;

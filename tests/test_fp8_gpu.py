@@ -556,3 +556,136 @@ def test_experts_rows_that_are_not_finite(cuda_device, tile):
     x[20, 3] = x[89, 255] = float("nan")
     ops.fp8_experts(x, w, starts, out, activation="clamped", limit=2.0, up_offset=1.0, tile=tile)
     assert torch.isnan(out[[20, 89]]).all() and torch.isfinite(out[:20]).all() and torch.isfinite(out[21:89]).all()
+
+
+def _scaled(dev, M, K, N, gated, sx, sw, seed=0):
+    """Rows and a weight of codes of every size, zeros among them, with the scales 2^sx[t] and 2^sw[t] of their groups of
+    columns, up to a factor of two."""
+    from binfer_b200.csrc import ops
+    g = torch.Generator(dev).manual_seed(seed)
+    T, B = K // 128, -(-N // 128) * (2 if gated else 1)
+
+    def codes(n):
+        c = torch.randint(0, 0x7f, (n, K), generator=g, device=dev, dtype=torch.uint8)
+        return (c | (torch.randint(0, 2, c.shape, generator=g, device=dev, dtype=torch.uint8) << 7)).view(E4M3)
+
+    def scales(n, e):
+        e = torch.tensor(e, dtype=F64, device=dev)
+        return (torch.exp2(e) * (1 + torch.rand((n, T), generator=g, device=dev, dtype=F64))).to(F32)
+    x = ops.Fp8Rows(codes(M), scales(M, sx).t().contiguous())
+    return x, ops.Fp8Weight(codes((2 if gated else 1) * N), scales(B, sw), gated)
+
+
+def _by_hand(x, w, gated):
+    """The product in 64 bits of rows that are in 8 bits (P8.product's sums and bounds)."""
+    a = P8.dense(x.codes.to(F32).to(F64), x.scales.t(), 1)
+    b = P8.dense(w.codes.to(F32).to(F64), w.scales, 128, gated)
+    return a @ b.t(), (a.abs() @ b.abs().t()) * ((131 + x.scales.shape[0]) * 2.0 ** -23)
+
+
+@pytest.mark.parametrize("kw", [dict(tile=16), dict(tile=16, split=3), dict(tile=32, split=1), dict(tile=64),
+                                dict(tile=-1, split=1), dict(tile=-1, split=2), dict()])
+@pytest.mark.parametrize("M", [1, 7, 61, 300])
+@pytest.mark.parametrize("sx,sw", [([-70] * 6, [-69] * 6), ([-99] * 6, [-60] * 6), ([-65, -20, -70, -100, -66, -68], [-66] * 6),
+                                   ([-100] * 6, [-30, -27, -26, -25, -24, -23]), ([70] * 6, [48] * 6)])
+def test_scales_whose_product_is_no_float(cuda_device, M, kw, sx, sw):
+    """Results that a float has room for, of scales whose product it has none for (or only some of its bits): 131
+    where P8.product has 130, for one more rounding a group; results below a float's smallest step, 2^-149, are off
+    by a step a group more."""
+    from binfer_b200.csrc import ops
+    for N in (130, 640):
+        x, w = _scaled(cuda_device, M, 768, N, False, sx, sw, M + N)
+        out = torch.full((M, N), 9.0, dtype=F32, device=cuda_device)
+        ops.fp8_linear(x, w, out, **kw)
+        ref, off = _by_hand(x, w, False)
+        # (no partial sum is above the sum of the sizes; a result above all floats is infinite, or NaN where partial
+        # sums of both signs are)
+        fits, above = off / ((131 + 6) * 2.0 ** -23) < 2.0 ** 127, ref.abs() - off >= 2.0 ** 128
+        assert (fits | above).float().mean() > 0.5 and not torch.isfinite(out[above]).any()
+        _check(out[fits], ref[fits], off[fits] + 7 * 2.0 ** -149)
+
+
+@pytest.mark.parametrize("kw", [dict(tile=16), dict(tile=16, split=2), dict(tile=32), dict(tile=64), dict(tile=-1, split=1),
+                                dict(tile=-1, split=2)])
+@pytest.mark.parametrize("M", [3, 200])
+@pytest.mark.parametrize("sx,sw", [(80, 70), (63, 66)])
+def test_scales_whose_product_is_too_large(cuda_device, M, kw, sx, sw):
+    """Sums that are not zero times a product above all floats: infinity, or a float where the sum is small.  (Each row
+    has one code that is not zero: its results are one product each.  Codes of 2^-9 at least: 2^150 times them is above
+    the floats; of 1.375 2^-5 and 1.625 2^-4 at most: 2^131 times them is not.)"""
+    from binfer_b200.csrc import ops
+    N, K = 200, 256
+    x, w = _scaled(cuda_device, M, K, N, False, [sx, -3], [sw, 2])
+    one = torch.zeros((M, K), dtype=torch.uint8, device=cuda_device)
+    one[:, 5] = torch.arange(M, device=cuda_device) % 20          # codes of 0 to 1.5 * 2^-6 in the first group
+    w.codes.view(torch.uint8)[:, 5] = (torch.arange(N, device=cuda_device) % 30).to(torch.uint8)
+    x = ops.Fp8Rows(one.view(E4M3), x.scales)
+    ref, _ = _by_hand(x, w, False)
+    out = torch.empty((M, N), dtype=F32, device=cuda_device)
+    ops.fp8_linear(x, w, out, **kw)
+    inf = ref.abs() >= 2.0 ** 128
+    near = (ref.abs() > 2.0 ** 128 * (1 - 2.0 ** -20)) & (ref.abs() < 2.0 ** 128 * (1 + 2.0 ** -20))
+    assert not near.any() and (ref == 0).any() and torch.equal(inf, (ref != 0) if sx == 80 else inf & False)
+    assert torch.isinf(out[inf & ~near]).all()
+    rest = ~inf & ~near
+    # (two scales and a factor: at most three roundings, and the multiply-add's)
+    assert ((out.to(F64) - ref).abs()[rest] <= ref.abs()[rest] * (4 * 2.0 ** -24)).all()
+
+
+def test_a_row_s_scales_do_not_touch_the_others(cuda_device):
+    from binfer_b200.csrc import ops
+    for M, kw in ((7, {}), (7, dict(split=2)), (40, dict(tile=64)), (300, dict(tile=-1, split=1))):
+        x, w = _scaled(cuda_device, M, 512, 150, True, [-3, -5, -2, -4], [-6] * 4, M)
+        a, b = (torch.empty((M, 150), dtype=BF16, device=cuda_device) for _ in range(2))
+        ops.fp8_linear(x, w, a, **kw)
+        x.scales[1, 2], x.scales[3, 0] = 2.0 ** -127, float("nan")
+        x.scales[0, 4] = 2.0 ** 127
+        ops.fp8_linear(x, w, b, **kw)
+        keep = torch.ones(M, dtype=torch.bool, device=cuda_device)
+        keep[[0, 2, 4]] = False
+        assert torch.isnan(b[0]).all() and not torch.equal(a[2], b[2])
+        assert torch.equal(a[keep], b[keep])
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("M,kw", [(1, {}), (5, {}), (5, dict(tile=16, split=2)), (40, dict(tile=32)), (40, dict(tile=64)),
+                                  (290, dict(tile=-1, split=1)), (290, dict(tile=-1, split=2))])
+def test_tiny_rows_and_weights(cuda_device, M, kw, gated):
+    """Numbers whose scales' product is below the floats of full precision, from their bfloat16 rows on and with a last
+    group that ends inside a word.  (One rounding a group more than P8.product counts.)"""
+    from binfer_b200.csrc import ops
+    K, N = 333, 200
+    x, w = (_x(M, K, cuda_device, M).to(F32) * 2.0 ** -60).to(BF16), _w(((1 + gated) * N, K), cuda_device, M)
+    w[:N] *= 2.0 ** -60
+    if gated:
+        w[N:] *= 2.0 ** 110
+    out = torch.empty((M, N), dtype=BF16 if gated else F32, device=cuda_device)
+    ops.fp8_linear(x, ops.fp8_weight(w, gated), out, **kw)
+    ref, off = P8.product(x, *P8.hold_weight(w, gated), gated)
+    assert ref.abs().max() > 2.0 ** -125
+    _check(out, ref, off * (134 / 133) + 2.0 ** -148)
+
+
+@pytest.mark.parametrize("tile", [0, 16, 64, -1])
+def test_experts_with_tiny_numbers(cuda_device, tile):
+    """An expert's weight and some rows so small that the scales' products are below the floats of full precision; the
+    other experts, and the rows beside, as they are without them."""
+    from binfer_b200.csrc import ops
+    counts, K, N = [30, 0, 300, 7], 300, 136
+    starts, R = torch.tensor([0, 30, 30, 330, 337], dtype=torch.int32, device=cuda_device), 337
+    x, w = _x(R, K, cuda_device, 1), _w((4, N, K), cuda_device, 1)
+    row_w = torch.rand(R, device=cuda_device) + 0.5
+    a, b = (torch.empty((R, N), dtype=F32, device=cuda_device) for _ in range(2))
+    ops.fp8_experts(x, ops.fp8_weight(w), starts, a, row_w=row_w, tile=tile)
+    w[2] *= 2.0 ** -58
+    small = torch.arange(R, device=cuda_device) % 3 == 1
+    x[small] *= 2.0 ** -58
+    ops.fp8_experts(x, ops.fp8_weight(w), starts, b, row_w=row_w, tile=tile)
+    for e, (i, j) in enumerate(zip(starts.tolist(), starts.tolist()[1:])):
+        if j > i:
+            ref, off = P8.product(x[i:j], *P8.hold_weight(w[e]))
+            k = row_w[i:j, None].to(F64)
+            _check(b[i:j], ref * k, (off * (134 / 133) + ref.abs() * 2.0 ** -23) * k + 2.0 ** -148)
+    rest = ~small
+    rest[30:330] = False
+    assert torch.equal(a[rest], b[rest]) and b[small].any()
