@@ -220,10 +220,10 @@ def linear_add_tanh(x: torch.Tensor, w: torch.Tensor, resid: torch.Tensor,
                     norm_b: Optional[torch.Tensor], assign: bool = False):
     """``resid += x @ w^T + bias`` (``assign``: ``=``) with the next norm, ``tanh(alpha resid) *
     norm_w + norm_b``, in the same kernel: returns the norm's output, or None, having done
-    nothing, where the cluster kernel does not run."""
+    nothing, where the cluster kernel does not run (weights in 8 bits, as for ``linear_add_norm``)."""
     M, (N, K) = x.shape[0], w.shape
-    if (not FUSE_NORM or x.dtype != torch.bfloat16 or w.dtype != torch.bfloat16
-            or not _use_cluster(M, N, K)):
+    if (not FUSE_NORM or isinstance(w, ops.Fp8Weight) or x.dtype != torch.bfloat16
+            or w.dtype != torch.bfloat16 or not _use_cluster(M, N, K)):
         return None
     plan = _plans.get((N, K))
     if plan is None:

@@ -204,3 +204,13 @@ def test_results_in_rows_that_share_memory_refused(ops):
         ops.fp8_rows_read(_codes(4, 32), torch.ones(1, 4), torch.zeros(32).expand(4, 32))
     with pytest.raises(ops.KernelError, match="share memory"):
         ops.fp8_weight_read(w, torch.zeros(200).expand(300, 200))
+
+
+def test_no_fused_epilogue_takes_a_weight_in_8_bits(ops):
+    """The products with the next norm in their epilogue leave such a weight to the plain product."""
+    from binfer_b200.parts.linear import linear_add_norm, linear_add_tanh
+    x, w = torch.zeros(2, 256, dtype=BF16), ops.Fp8Weight(_codes(128, 256), torch.ones(1, 2))
+    resid, norm_w = torch.zeros(2, 128), torch.ones(128)
+    assert linear_add_norm(x, w, resid, norm_w, 1e-6) is None
+    for assign in (False, True):
+        assert linear_add_tanh(x, w, resid, None, 0.5, norm_w, None, assign=assign) is None

@@ -130,3 +130,48 @@ def test_queries_alone(cuda_device, tmp_path):
     ops.fp8_linear(x, w, out)
     ref, off = P8.product(x, mixer.w_qkv.codes[:mixer.q_size].to(F32).to(F64), mixer.w_qkv.scales[:w.scales.shape[0]])
     assert ((out.to(F64) - ref).abs() <= off + ref.abs() * 2.0 ** -8).all()
+
+
+@pytest.mark.parametrize("norm", ["tanh_norm", "layernorm", "rmsnorm"])
+@pytest.mark.parametrize("hidden", [256, 260])
+def test_pre_norm_layers_of_every_norm(cuda_device, monkeypatch, norm, hidden):
+    """Pre-norm layers whose norms are not RMS, and rows that the norm's kernel in 8 bits does not take (a width
+    that is no multiple of eight): every product of a step is that of its inputs."""
+    import dataclasses
+    from binfer_b200.config.qwen3 import Qwen3Config
+    from binfer_b200.config.specs import NormSpec
+    from binfer_b200.csrc import ops
+    from binfer_b200.engine import StepItem, make_env, make_runner
+    from binfer_b200.engine.loading import model_from_seed
+    raw = dict(architectures=["Qwen3ForCausalLM"], model_type="qwen3", num_hidden_layers=2, hidden_size=hidden,
+               num_attention_heads=4, num_key_value_heads=2, head_dim=64, intermediate_size=384, vocab_size=200,
+               rope_theta=1e4, rms_norm_eps=1e-6, tie_word_embeddings=False, max_position_embeddings=1024,
+               hidden_act="silu", attention_bias=False)
+
+    class Config:
+        def to_spec(self):
+            spec = Qwen3Config.from_dict(raw).to_spec()
+            ns = NormSpec(kind=norm, eps=1e-5, bias_suffix=".b" if norm != "rmsnorm" else None)
+            return dataclasses.replace(spec, final_norm=ns,
+                                       layers=tuple(dataclasses.replace(l, norm=ns) for l in spec.layers))
+    env = make_env("bfloat16", weights="fp8")
+    runner = make_runner(model_from_seed(Config(), env, 3, std=0.06, norm_std=0.1), env, page_size=16, num_pages=32)
+    seen, whole = [], ops.fp8_linear
+
+    def watched(x, w, out, **kw):
+        whole(x, w, out, **kw)
+        seen.append(type(x))
+        if isinstance(x, ops.Fp8Rows):
+            rows, x = x, torch.empty(x.shape, device=cuda_device)
+            ops.fp8_rows_read(*rows, x)
+        ref, off = P8.product(x, w.codes.to(F32).to(F64), w.scales, w.gated)
+        assert ((out.to(F64) - ref).abs() <= off + ref.abs() * (torch.finfo(out.dtype).eps / 2)).all()
+    monkeypatch.setattr(ops, "fp8_linear", watched)
+    ids = H.random_tokens(70, 200, 3)
+    runner.add_request("a")
+    for a, b in ((0, 60), (60, 61), (61, 70)):
+        seen.clear()
+        logits = runner.step([StepItem("a", ids[a:b], [b - a - 1])])
+        assert len(seen) == 8 and torch.isfinite(logits).all()
+        assert seen.count(ops.Fp8Rows) == (4 if norm == "rmsnorm" and hidden == 256 else 0)
+    runner.check_errors()
