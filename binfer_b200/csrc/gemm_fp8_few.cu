@@ -46,8 +46,10 @@ constexpr int FEW_ROUNDS = 4;
 constexpr int FEW_W_BYTES = 128 * FK;
 // Two CTAs share an SM: its registers, its shared memory and its tensor memory are dealt out by halves.  A
 // step of eight rows against 24,576 x 4,096 gated took 27.5 us with one, whose 192 tiles ran in two turns.
+// With 256 columns of tensor memory each (umma_utils.cuh: why no more, and no less shared memory than 92 KB).
 constexpr int FEW_PER_SM = 2;
 constexpr size_t FEW_SMEM = 112 * 1024;
+static_assert(FEW_PER_SM * (FEW_SMEM + SMEM_OWN) <= SMEM_SM, "resident together");
 constexpr int FEW_DOES_NOT_FIT = -1;
 
 template <int NB>
@@ -97,6 +99,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   constexpr int STAGE = FEW_W_BYTES + (RESIDENT ? 0 : NB * FK);
   constexpr int HALVES = GATED ? 2 : 1;
   constexpr int TMEM_COLS = SLOTS * NB;
+  static_assert(TMEM_COLS * FEW_PER_SM <= TMEM_SM_COLS, "none waits for the other's tensor memory");
   extern __shared__ __align__(16) uint8_t smem_raw[];
   BF_TRACE_POINT(10 * BF_TR_FP8_GEMM);
   bf_pdl_trigger();
@@ -576,7 +579,8 @@ size_t few_memory(const FewParams& p, int* stages) {
   const size_t stage = FEW_W_BYTES + (RESIDENT ? 0 : NB * FK);
   const size_t n = fixed < FEW_SMEM ? (FEW_SMEM - fixed) / stage : 0;
   *stages = n > FEW_MAX_STAGES ? FEW_MAX_STAGES : (int)n;
-  return fixed + *stages * stage;
+  const size_t all = fixed + *stages * stage;      // (93 KB at least as it is)
+  return all < TMEM_LEAST_SMEM ? TMEM_LEAST_SMEM : all;
 }
 
 template <int NB, typename OutT, bool GATED, bool RESIDENT>

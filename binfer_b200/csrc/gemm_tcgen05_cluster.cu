@@ -714,6 +714,8 @@ int launch_cluster(const void* x, const void* w, OutT* out, ClusterGemmParams p,
   // (Seen once, with the shared memory capped at 110 KB for an experiment: the launch failed.)
   size_t smem = fixed + (size_t)stages * stage_bytes;
   if (smem < 120 * 1024) smem = 120 * 1024;
+  // (tiles of more than 128 rows ask for 153 KB and more)
+  if (p.tmem_cols > TMEM_SM_COLS / 2 && smem < TMEM_ALONE_SMEM) smem = TMEM_ALONE_SMEM;
   auto kern = gemm_cluster_kernel<OutT, FORM>;
   static bool configured_on[BF_MAX_DEVICES];
   bool& configured = configured_on[bf_current_device()];

@@ -572,8 +572,9 @@ int sp_launch(const CUtensorMap& map, SplitParams p, int batch, uint8_t* scratch
   p.stages = stages;
   p.floats = left < SP_MAX_FLOATS ? left : SP_MAX_FLOATS;
   size_t smem = 1024 + SP_HEAD + (size_t)p.stages * STAGE + (size_t)p.floats * SP_FLOATS;
-  // one CTA an SM: two that hold tensor memory and wait for their clusters could wait for each other
-  if (smem < 120 * 1024) smem = 120 * 1024;
+  // one CTA an SM, and no other kernel's that holds tensor memory (umma_utils.cuh): two that wait for their clusters
+  // could wait for each other
+  if (smem < TMEM_ALONE_SMEM) smem = TMEM_ALONE_SMEM;
   auto kern = sgemm_split_kernel<NT, VEC, PRE>;
   static bool configured_on[BF_MAX_DEVICES];
   bool& configured = configured_on[bf_current_device()];

@@ -13,6 +13,16 @@ namespace {
 constexpr int BM = 128;   // rows of the A tile = TMEM lanes
 constexpr int BK = 64;    // K per stage: 64 bf16 = 128 bytes = one swizzle row
 constexpr long long WAIT_LIMIT_CYCLES = 2000000000LL;
+// A CTA that allocates tensor memory and then waits, for its cluster or (dependent launch) for the kernels ahead, must
+// never wait in the allocation for another such CTA on its SM: those could wait for it in turn, without end.  So CTAs
+// that fit an SM's 228 KB of shared memory together (1 KB more than each asks for) have at most its 512 columns
+// between them: those of up to 256 columns are two to an SM at most, those of more ask for so much that no other fits.
+constexpr int TMEM_SM_COLS = 512;
+constexpr size_t SMEM_SM = 228 * 1024, SMEM_OWN = 1024;
+constexpr size_t TMEM_LEAST_SMEM = 92 * 1024;      // asked for by a CTA of up to 256 columns
+constexpr size_t TMEM_ALONE_SMEM = 136 * 1024;     // ... of more
+static_assert(3 * (TMEM_LEAST_SMEM + SMEM_OWN) > SMEM_SM, "a third CTA");
+static_assert(TMEM_LEAST_SMEM + TMEM_ALONE_SMEM + 2 * SMEM_OWN > SMEM_SM, "beside one of more than 256 columns");
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return (uint32_t)__cvta_generic_to_shared(p);
