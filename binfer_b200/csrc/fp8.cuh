@@ -140,7 +140,8 @@ struct Fp8Sixteen {
 // The factor of a group's sums is the product of two scales.  Scales that are both small or both large have products
 // below the floats of full precision, or above all of them, while the product with the sum, of up to 2^25 or down to
 // 2^-18, may well be one.  The kernels' loops take such a factor as zero, or as infinity; warps that have the time look
-// for them beside (fp8_odd), and at a tile's end the results that they concern are made anew (fp8_anew).
+// for them beside (fp8_odd), and the results that they concern are made anew behind the loops (fp8_sum_anew).  (A look
+// within the loops, even at one flag a group, cost 2 to 15 % of a product.)
 __device__ __forceinline__ float fp8_loop_factor(float sx, float sw) {
   float f;
   asm("mul.ftz.f32 %0, %1, %2;" : "=f"(f) : "f"(sx), "f"(sw));

@@ -112,8 +112,9 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* factors = reinterpret_cast<float*>(base + FEW_BARS);            // [SLOTS][HALVES][NB]
-  int* odd = reinterpret_cast<int*>(factors + SLOTS * HALVES * NB);      // [16]: of a tile's last group, whether it has odd factors
-  float* exchange = reinterpret_cast<float*>(odd + 16);  // gated: up sums; split: the parts sent here
+  // whether a factor was no float (fp8.cuh): of all tiles, the cluster's; RESIDENT: of this CTA's part of the tile
+  volatile int* odd = reinterpret_cast<volatile int*>(factors + SLOTS * HALVES * NB);
+  float* exchange = factors + SLOTS * HALVES * NB + 16;  // gated: up sums; split: the parts sent here
   uint8_t* table_smem = reinterpret_cast<uint8_t*>(exchange) +
                         (p.split > 1 ? ((NB + p.split - 1) / p.split) * p.split * 128 * 4
                                      : GATED ? FewShape<NB>::EXCHANGE : 0);
@@ -153,6 +154,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
       tables.before[1] = (p.rows + NB - 1) / NB;
     }
     *abort = 0;
+    *odd = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -271,23 +273,24 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
     uint32_t slot_phase = 0;
     bool ok = true;
     float sx[AHEAD][PER], sw[AHEAD][HALVES];
-    auto ask = [&](const RowTile& t, int ga) {
+    auto scale_x = [&](const RowTile& t, int g, int j) {       // of column j * 32 + lane
+      const int row = t.row0 + j * 32 + lane;
+      if (RESIDENT) return row < t.row_end ? res_sx[(g - g0) * NB + row] : 1.f;
+      return row < t.row_end && j * 32 + lane < NB ? p.sx[(long long)g * p.lds + row] : 1.f;
+    };
+    auto scale_w = [&](const RowTile& t, int g, int h) {
       const long long block = (long long)t.expert * HALVES * p.w_blocks + (GATED ? t.ft >> 1 : t.ft);
+      return p.sw[(block + h * p.w_blocks) * p.groups + g];
+    };
+    auto ask = [&](const RowTile& t, int ga) {
+      if (RESIDENT) ok = mbar_wait_warp(ready + (min(ga + AHEAD, g1) - 1 - g0) / per_round, 0, abort);
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
         const int g = min(ga + i, g1 - 1);
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-          const int row = t.row0 + j * 32 + lane;
-          if (RESIDENT) {
-            if (i == 0 && j == 0) ok = mbar_wait_warp(ready + (min(ga + AHEAD, g1) - 1 - g0) / per_round, 0, abort);
-            sx[i][j] = row < t.row_end ? res_sx[(g - g0) * NB + row] : 1.f;
-          } else {
-            sx[i][j] = row < t.row_end && j * 32 + lane < NB ? p.sx[(long long)g * p.lds + row] : 1.f;
-          }
-        }
+        for (int j = 0; j < PER; ++j) sx[i][j] = scale_x(t, g, j);
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h) sw[i][h] = p.sw[(block + h * p.w_blocks) * p.groups + g];
+        for (int h = 0; h < HALVES; ++h) sw[i][h] = scale_w(t, g, h);
       }
     };
     int u = cluster;
@@ -296,10 +299,11 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
       t = row_tile(tables, p.experts, p.tiles_f, NB, u);
       ask(t, g0);
     }
+    bool odd_here = false;
     for (; u < units && ok; u += clusters) {
-      bool odd_here = false;
       for (int ga = g0; ga < g1 && ok; ga += AHEAD) {
         float f[AHEAD][PER * HALVES];
+        uint32_t note = 0u;
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i)
 #pragma unroll
@@ -307,8 +311,15 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
 #pragma unroll
             for (int h = 0; h < HALVES; ++h) {
               f[i][j * HALVES + h] = fp8_loop_factor(sx[i][j], sw[i][h]);
-              odd_here = odd_here || fp8_odd(sx[i][j], sw[i][h]);
+              note = max(note, fp8_note(f[i][j * HALVES + h]));
             }
+        if (__builtin_expect(note >= FP8_ODD, 0)) {
+#pragma unroll 1
+          for (int i = 0; i < AHEAD * PER * HALVES; ++i) {
+            const int g = min(ga + i / (PER * HALVES), g1 - 1);
+            odd_here = odd_here || fp8_odd(scale_x(t, g, i / HALVES % PER), scale_w(t, g, i % HALVES));
+          }
+        }
         if (ga + AHEAD < g1) {
           ask(t, ga + AHEAD);
         } else if (u + clusters < units) {
@@ -328,10 +339,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
 #pragma unroll
             for (int h = 0; h < HALVES; ++h)
               if (j * 32 + lane < NB) dst[h * NB + j * 32 + lane] = f[i][j * HALVES + h];
-          if (ga + i == g1 - 1) {
-            const int any = __any_sync(0xffffffffu, odd_here);
-            if (lane == 0) odd[slot] = any;
-          }
+          if (RESIDENT && odd_here) *odd = 1;
           __syncwarp();
           if (lane == 0) mbar_arrive(acc_full + slot);
           if (++slot == SLOTS) {
@@ -341,6 +349,12 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
         }
       }
     }
+    if (!RESIDENT && odd_here)
+      for (int r = 0; r < p.split; ++r)
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(
+                         few_map(smem_u32(const_cast<int*>(odd)), (uint32_t)r)),
+                     "r"(1)
+                     : "memory");
   } else if (warp >= 4) {
     // ----------------------------------------------------------------- sums
     const int quarter = warp & 3, half = (warp - 4) >> 2;
@@ -391,7 +405,6 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
 #pragma unroll
         for (int j = 0; j < CH; ++j) acc[i][j] = 0.f;
       bool ok = true;
-      int tile_odd = 0;
       for (int g = g0; g < g1; ++g) {
         if (!mbar_wait_warp(acc_full + slot, slot_phase, abort)) {
           ok = false;
@@ -418,7 +431,6 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
             }
           }
         }
-        if (g == g1 - 1) tile_odd = odd[slot];           // (before the slot goes back)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(acc_empty + slot);
@@ -427,30 +439,30 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
           slot_phase ^= 1;
         }
       }
-      const int feature = t.ft * BOX + (lane_row & (BOX - 1));
-      // (rare) what has such a factor anew: the sum over this CTA's groups
-      if (ok && tile_odd && feature < p.features) {
-        const uint8_t* wr = p.w + ((long long)t.expert * w_rows + which * p.features + feature) * p.ldw;
-        const float* swr =
-            p.sw + ((long long)t.expert * HALVES * p.w_blocks + which * p.w_blocks + (feature >> 7)) * p.groups;
-        for (int a = 0; a < CHUNKS * CH; ++a) {
-          const int c = (2 * (a / CH) + half) * CH + a % CH, row = t.row0 + c;
-          if (c >= n) continue;
-          auto scale_x = [&](int g) { return RESIDENT ? res_sx[(g - g0) * NB + c] : p.sx[g * p.lds + row]; };
-          auto scale_w = [&](int g) { return swr[g]; };
-          if (!fp8_any_odd(g0, g1, scale_x, scale_w)) continue;
-          const float v = fp8_sum_anew(
-              g0, g1, p.K, scale_x, scale_w,
-              [&](int g, int k) -> const uint8_t* {
-                if (RESIDENT) return res + ((g - g0) * FEW_RES_ROWS + c) * FK + (((k >> 4) ^ (c & 7)) << 4) + (k & 15);
-                return p.codes + row * p.ldx + g * FK + k;
-              },
-              [&](int g, int k) { return wr + g * FK + k; });
+      if constexpr (RESIDENT) {
+        const int feature = t.ft * BOX + (lane_row & (BOX - 1));
+        if (__builtin_expect(ok && *odd != 0 && feature < p.features, 0)) {
+          // (rare) the sums over this CTA's groups anew
+          const uint8_t* wr = p.w + ((long long)which * p.features + feature) * p.ldw;
+          const float* swr = p.sw + (which * p.w_blocks + (feature >> 7)) * (long long)p.groups;
+          for (int a = 0; a < CHUNKS * CH; ++a) {
+            const int c = (2 * (a / CH) + half) * CH + a % CH;
+            if (c >= n) continue;
+            auto scale_x = [&](int g) { return res_sx[(g - g0) * NB + c]; };
+            auto scale_w = [&](int g) { return swr[g]; };
+            if (!fp8_any_odd(g0, g1, scale_x, scale_w)) continue;
+            const float v = fp8_sum_anew(
+                g0, g1, p.K, scale_x, scale_w,
+                [&](int g, int k) {
+                  return res + ((g - g0) * FEW_RES_ROWS + c) * FK + (((k >> 4) ^ (c & 7)) << 4) + (k & 15);
+                },
+                [&](int g, int k) { return wr + g * FK + k; });
 #pragma unroll
-          for (int i = 0; i < CHUNKS * CH; ++i) acc[i / CH][i % CH] = i == a ? v : acc[i / CH][i % CH];
+            for (int i = 0; i < CHUNKS * CH; ++i) acc[i / CH][i % CH] = i == a ? v : acc[i / CH][i % CH];
+          }
         }
+        __syncwarp();
       }
-      __syncwarp();
       if (p.split > 1) {
         // column j goes to rank j % split: [rank][its number there][weight row]
         const int per = (NB + p.split - 1) / p.split;
@@ -548,6 +560,39 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
 
   // ------------------------------------------------------------------ wind-down
   __syncthreads();
+  if (!RESIDENT && __builtin_expect(*odd != 0 && !*abort, 0)) {
+    // (rare) results with a factor that is no float anew, over what this CTA has stored
+    constexpr int WIDTH = GATED ? 64 : 128;
+    for (int u = cluster; u < units; u += clusters) {
+      const RowTile t = row_tile(tables, p.experts, p.tiles_f, NB, u);
+      const int n = min(NB, t.row_end - t.row0);
+      for (int i = threadIdx.x; i < n * WIDTH; i += FEW_THREADS) {
+        const int o = t.ft * WIDTH + i % WIDTH, c = i / WIDTH, row = t.row0 + c;
+        if (o >= p.features || (p.split > 1 && c % p.split != rank)) continue;
+        auto scale_x = [&](int g) { return p.sx[g * p.lds + row]; };
+        auto scales_w = [&](int h) {
+          return p.sw + (((long long)t.expert * HALVES + h) * p.w_blocks + (o >> 7)) * p.groups;
+        };
+        bool any = false;
+        for (int h = 0; h < HALVES; ++h)
+          any = any || fp8_any_odd(0, p.groups, scale_x, [at = scales_w(h)](int g) { return at[g]; });
+        if (!any) continue;
+        float v[2];
+#pragma unroll 1
+        for (int h = 0; h < HALVES; ++h) {
+          const uint8_t* wr = p.w + ((long long)t.expert * w_rows + h * p.features + o) * p.ldw;
+          const float sum = fp8_sum_anew(
+              0, p.groups, p.K, scale_x, [at = scales_w(h)](int g) { return at[g]; },
+              [&](int g, int k) { return p.codes + row * p.ldx + g * FK + k; },
+              [&](int g, int k) { return wr + g * FK + k; });
+          if (h == 0) v[0] = sum; else v[1] = sum;
+        }
+        float r = GATED ? fp8_gate(p.act, v[0], v[1], p.gk) : v[0];
+        if (p.row_w) r *= p.row_w[row];
+        bf_st(out + (size_t)row * p.ldo + o, r);
+      }
+    }
+  }
   BF_TRACE_POINT(10 * BF_TR_FP8_GEMM + 2);
   if (*abort) {
     if (threadIdx.x == 0) atomicOr(p.err, BF_ERR_WAIT);
