@@ -2983,7 +2983,7 @@ class Fp8Weight:
     code times scale.  ``gated``: the weight is a gate weight and an up weight of N / 2 rows each, one
     behind the other, and the up rows' blocks begin anew (blocks = 2 ceil(N / 2 / 128), else ceil(N / 128)).
     Scales are positive and finite.  Codes whose rows do not lie on 16-byte boundaries are copied.  The two
-    tensors may be written to, but not replaced."""
+    tensors may be written to, but not replaced or given other memory (refused by the calls)."""
     __slots__ = ("_codes", "_scales", "gated", "experts", "rows", "features", "K", "device", "_held", "_index")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, gated: bool = False):
@@ -3022,6 +3022,13 @@ class Fp8Weight:
     def __reduce__(self):       # a deep copy, or one read back, has addresses of its own
         # (as bytes: pickle does not take 8-bit floats)
         return _fp8_weight_again, (self._codes.view(torch.uint8), self._scales, self.gated)
+
+    def _addresses(self, what: str) -> Tuple[int, int, int]:
+        """(the codes' address, how far rows are apart, the scales' address)"""
+        held = self._held
+        if self._codes.data_ptr() != held[0] or self._scales.data_ptr() != held[2]:
+            raise KernelError(f"{what}: the weight's tensors lie elsewhere than when it was made")
+        return held
 
     @property
     def codes(self) -> torch.Tensor:
@@ -3069,8 +3076,8 @@ def fp8_weight_read(w: Fp8Weight, out: torch.Tensor) -> None:
         raise KernelError("fp8_weight_read: out must have the weight's shape, its rows equally far apart")
     if out.shape[0] * out.shape[-2] > 1 and out.stride(-2) < w.K:
         raise KernelError("fp8_weight_read: out's rows must not share memory")
+    at, pitch, scales_at = w._addresses("fp8_weight_read")
     _same_device("fp8_weight_read", w.codes, w.scales, out)
-    at, pitch, scales_at = w._held
     _run("fp8_read", _fp8_read_call, at, pitch, scales_at, 0, out.data_ptr(), out.stride(-2), dtype, 1,
          max(1, w.experts) * (2 if w.gated else 1), w.features, w.K, num_sms(out.device), _stream_at(out))
 
@@ -3114,13 +3121,14 @@ def _fp8_product(what: str, x, w: Fp8Weight, starts, out, row_w, activation, lim
         others, starts_at = (*others, starts), starts.data_ptr()
     if (tile or split) and (tile not in (0, 16, 32, 64, -1) or not 0 <= split <= 8):
         raise KernelError(f"{what}: no tiles of {tile} rows, shared by {split}")
+    held_at = w._addresses(what)
     _same_device(what, out, *others)
     if w._index != out.get_device():
         _same_device(what, w.codes)
     if M == 0:
         return
     device = out.device
-    behind = (*w._held, starts_at, row_w_at, out.data_ptr(), out.stride(0), out_type, M, features, K,
+    behind = (*held_at, starts_at, row_w_at, out.data_ptr(), out.stride(0), out_type, M, features, K,
               w.experts or 1, w.gated, act, limit, slope, up_offset, tile, split, num_sms(device),
               error_word(device).data_ptr(), _stream_at(out))
     global _launches

@@ -214,3 +214,18 @@ def test_no_fused_epilogue_takes_a_weight_in_8_bits(ops):
     assert linear_add_norm(x, w, resid, norm_w, 1e-6) is None
     for assign in (False, True):
         assert linear_add_tanh(x, w, resid, None, 0.5, norm_w, None, assign=assign) is None
+
+
+def test_weights_whose_memory_went_elsewhere_are_refused(ops):
+    """The addresses taken when the weight was made are not read where its tensors have others by now."""
+    for change in (lambda w: setattr(w.codes, "data", w.codes.clone()), lambda w: setattr(w.scales, "data", w.scales.clone()),
+                   lambda w: w.codes.untyped_storage().resize_(0), lambda w: w.scales.set_(torch.ones(3, 2))):
+        w = ops.Fp8Weight(_codes(300, 208), torch.ones(3, 2))
+        x, out = torch.zeros(2, 208, dtype=BF16), torch.zeros(2, 300, dtype=BF16)
+        for call in (lambda: ops.fp8_linear(x, w, out), lambda: ops.fp8_weight_read(w, torch.zeros(300, 208))):
+            with pytest.raises(ops.KernelError, match="CUDA"):
+                call()
+        change(w)
+        for call in (lambda: ops.fp8_linear(x, w, out), lambda: ops.fp8_weight_read(w, torch.zeros(300, 208))):
+            with pytest.raises(ops.KernelError, match="elsewhere"):
+                call()
