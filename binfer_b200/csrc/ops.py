@@ -2834,6 +2834,7 @@ def gemm_bf16_swiglu(x: torch.Tensor, w_gate_up: torch.Tensor, out: torch.Tensor
 # ------------------------------------------------------------------ weights in 8 bits
 FP8_GROUP = 128                # numbers of a row that share a scale; weights: blocks of 128 x 128
 FP8_MAX_EXPERTS = 512
+FP8_MAX_ROWS = 2 ** 31 - 2 ** 20          # the kernels count rows, and a grid's step beyond them, in 31 bits
 # BINFER_B200_FP8_RESIDENT=0: the rows go into 8 bits in a kernel of their own for few rows too
 FP8_RESIDENT = os.environ.get("BINFER_B200_FP8_RESIDENT", "1") != "0"
 E4M3 = torch.float8_e4m3fn
@@ -2877,6 +2878,11 @@ def _fp8_matrix(what: str, name: str, t: torch.Tensor, dims: Tuple[int, ...] = (
     return dtype
 
 
+def _fp8_row_count(what: str, rows: int) -> None:
+    if rows > FP8_MAX_ROWS:
+        raise KernelError(f"{what}: at most {FP8_MAX_ROWS} rows")
+
+
 def _fp8_stacked(t: torch.Tensor) -> bool:
     """Whether the rows of all of ``[E, N, K]``'s matrices are equally far apart."""
     return t.dim() == 2 or t.shape[0] < 2 or t.stride(0) == t.shape[1] * t.stride(1)
@@ -2915,6 +2921,7 @@ def fp8_rows(x: torch.Tensor) -> Fp8Rows:
     e4m3 value nearest to ``x / s``, ties to even.  A number that is not finite makes its group read as
     NaN.  (The codes' rows are padded to 16 bytes: ``codes`` need not be contiguous.)"""
     dtype = _fp8_matrix("fp8_rows", "x", x)
+    _fp8_row_count("fp8_rows", x.shape[0])
     _same_device("fp8_rows", x)
     (T, K), device = x.shape, x.device
     codes, scales = _fp8_empty_rows(T, K, device)
@@ -2959,6 +2966,7 @@ def fp8_rows_read(codes: torch.Tensor, scales: torch.Tensor, out: torch.Tensor) 
     dtype = _fp8_matrix("fp8_rows_read", "out", out)
     shape = out.shape
     T, K = shape
+    _fp8_row_count("fp8_rows_read", T)
     if T > 1 and out.stride(0) < K:
         raise KernelError("fp8_rows_read: out's rows must not share memory")
     if codes.dtype != E4M3 or codes.shape != shape:
@@ -3054,11 +3062,13 @@ def fp8_weight(w: torch.Tensor, gated: bool = False) -> Fp8Weight:
     if not w.numel() or not _fp8_stacked(w) or (gated and w.shape[-2] % 2):
         raise KernelError("fp8_weight: w must have rows that are equally far apart, a gated one as many up rows "
                           "as gate rows")
-    _same_device("fp8_weight", w)
     shape, device = w.shape, w.device
     n, k, mats, halves = shape[-2], shape[-1], shape[0] if len(shape) == 3 else 1, 2 if gated else 1
     if mats > FP8_MAX_EXPERTS:
         raise KernelError(f"fp8_weight: at most {FP8_MAX_EXPERTS} experts")
+    if n // halves > 65535 * FP8_GROUP:
+        raise KernelError(f"fp8_weight: at most {65535 * FP8_GROUP} rows")
+    _same_device("fp8_weight", w)
     blocks, groups = halves * -(-(n // halves) // FP8_GROUP), -(-k // FP8_GROUP)
     codes = _fp8_empty_codes(shape, device)
     size, strides = ((blocks, groups), (groups, 1)) if len(shape) == 2 else (
@@ -3086,6 +3096,7 @@ def _fp8_product(what: str, x, w: Fp8Weight, starts, out, row_w, activation, lim
                  split) -> None:
     shape, K, features = x.shape, w.K, w.features
     M = shape[0] if len(shape) == 2 else -1
+    _fp8_row_count(what, M)
     held = isinstance(x, Fp8Rows)
     if held:
         codes, scales = x

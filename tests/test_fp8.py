@@ -229,3 +229,15 @@ def test_weights_whose_memory_went_elsewhere_are_refused(ops):
         for call in (lambda: ops.fp8_linear(x, w, out), lambda: ops.fp8_weight_read(w, torch.zeros(300, 208))):
             with pytest.raises(ops.KernelError, match="elsewhere"):
                 call()
+
+
+def test_more_rows_than_the_kernels_count_are_refused(ops):
+    n = 2 ** 31 - 100
+    x, y = torch.zeros(1, 1, dtype=BF16).expand(n, 1), torch.zeros(1, 1).expand(n, 1)
+    w = ops.Fp8Weight(_codes(1, 1), torch.ones(1, 1))
+    e = ops.Fp8Weight(_codes(2, 1, 1), torch.ones(2, 1, 1))
+    for call in (lambda: ops.fp8_rows(x), lambda: ops.fp8_rows(y), lambda: ops.fp8_weight(x), lambda: ops.fp8_weight(y),
+                 lambda: ops.fp8_linear(x, w, x), lambda: ops.fp8_experts(x, e, torch.zeros(3, dtype=torch.int32), x),
+                 lambda: ops.fp8_rows_read(_codes(1, 1).expand(n, 1), torch.ones(1, 1).expand(1, n), y)):
+        with pytest.raises(ops.KernelError, match="at most"):
+            call()
