@@ -689,3 +689,63 @@ def test_experts_with_tiny_numbers(cuda_device, tile):
     rest = ~small
     rest[30:330] = False
     assert torch.equal(a[rest], b[rest]) and b[small].any()
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("M,groups,N,fits", [
+    # clusters of eight: 1 to 5 groups a CTA, in one or two turns
+    (1, 32, 300, True), (2, 32, 300, True), (3, 40, 128, True), (5, 32, 130, True), (8, 40, 300, True),
+    # a tile for every SM: a CTA has all groups, in one to four turns of 32, 16, 8 or 4 ...
+    (1, 32, 19200, True), (2, 20, 19200, True), (3, 32, 19200, True), (4, 9, 19200, True), (7, 16, 19200, True),
+    (8, 12, 19200, True), (8, 16, 19200, True),
+    # ... five, or more than there is room for beside four stages of the weight; more than eight rows
+    (8, 17, 19200, False), (4, 33, 19200, False), (1, 48, 19200, False), (9, 32, 300, False)])
+def test_rows_that_stay_in_the_product_s_kernel(cuda_device, monkeypatch, M, groups, N, fits, gated):
+    """One kernel where the rows fit and two elsewhere, with the same results; an odd last group either way."""
+    from binfer_b200.csrc import ops
+    if gated and N == 19200:
+        N = 9600
+    for K in (groups * 128, groups * 128 - 37):
+        x, w = _x(M, K + 3, cuda_device, M)[:, 3:], ops.fp8_weight(_w(((1 + gated) * N, K), cuda_device), gated)
+        for rows in (x, x.contiguous()):
+            outs = []
+            for resident in (True, False):
+                monkeypatch.setattr(ops, "FP8_RESIDENT", resident)
+                out = torch.full((M, N), float("nan"), dtype=BF16, device=cuda_device)
+                before = ops.launches()
+                ops.fp8_linear(rows, w, out)
+                assert ops.launches() - before == (1 if resident and fits else 2)
+                outs.append(out)
+            assert torch.equal(*outs)
+    assert ops.error_word(cuda_device).item() == 0
+
+
+@pytest.mark.parametrize("R", [40, 900])
+def test_captured_experts_with_other_rows_each_time(cuda_device, R):
+    """A captured call replayed with other rows, other shares of the experts and other weights of the rows."""
+    from binfer_b200.csrc import ops
+    E, K, N = 6, 384, 200
+    w = _w((E, 2 * N, K), cuda_device)
+    held, x = ops.fp8_weight(w, True), _x(R, K, cuda_device)
+    starts, row_w = torch.zeros(E + 1, dtype=torch.int32, device=cuda_device), torch.ones(R, device=cuda_device)
+    out = torch.empty((R, N), dtype=BF16, device=cuda_device)
+    ops.fp8_experts(x, held, starts, out, row_w=row_w)
+    torch.cuda.synchronize()
+    gc.collect()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.fp8_experts(x, held, starts, out, row_w=row_w)
+    for i, cuts in enumerate(([0, 0, 1, 1, 1, 1, 1], [0, .1, .1, .5, .9, .9, 1], [.2, .3, .4, .5, .6, .7, .8],
+                              [1, 1, 1, 1, 1, 1, 1], [0, 0, 0, 0, 0, 0, 1])):
+        s = [round(c * R) for c in cuts]
+        x.copy_(_x(R, K, cuda_device, 20 + i))
+        row_w.copy_(torch.rand(R, device=cuda_device))
+        starts.copy_(torch.tensor(s, dtype=torch.int32))
+        out.fill_(9.0)
+        g.replay()
+        for e, (a, b) in enumerate(zip(s, s[1:])):
+            if b > a:
+                ref, off = P8.product(x[a:b], *P8.hold_weight(w[e], True), True)
+                k = row_w[a:b, None].to(F64)
+                _check(out[a:b], ref * k, (off + ref.abs() * 2.0 ** -23) * k)
+        assert (out[:s[0]] == 9).all() and (out[s[-1]:] == 9).all()
