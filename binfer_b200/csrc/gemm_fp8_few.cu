@@ -37,10 +37,10 @@ namespace {
 constexpr int FEW_THREADS = 384;
 constexpr int FEW_MAX_STAGES = 12;
 constexpr int FEW_BARS = 1024;
-// RESIDENT: rows, and turns in which the CTA puts its columns of them into 8 bits (32 groups each).  With
-// more turns a kernel in front is faster (a turn is 0.6 us; one row, 4,096 x 2,048 to 12,288: 8.5 to 13.7 us
-// so and 8.0 to 12.8 us with it, but 1,024 x 2,048: 5.0 and 5.5; launched one by one, 4 us of the host's
-// time are gained at every size).
+// RESIDENT: rows, and turns in which the CTA puts its columns of them into 8 bits (32 groups each).  A turn is
+// 0.6 us, a kernel in front 1.6 with its way from end to start: within a graph the two come out alike (one row,
+// 4,096 x 2,048 to 12,288: 7.1 to 12.7 us so and 7.0 to 12.6 with it, 1,024 x 2,048: 4.5 and 5.0), one by one 4 us of
+// the host's time are gained at every size.  With more turns the kernel in front is faster.
 constexpr int FEW_RES_ROWS = 8;
 constexpr int FEW_ROUNDS = 4;
 constexpr int FEW_W_BYTES = 128 * FK;

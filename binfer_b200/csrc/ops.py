@@ -3146,13 +3146,13 @@ def _fp8_product(what: str, x, w: Fp8Weight, starts, out, row_w, activation, lim
     p = _profiler
     if p is not None:
         p.begin(what)
-    # Few rows launched one by one go as one kernel, where it takes the sizes (4 us of the host's time less: 7.5
-    # against 12); in a captured graph, where the host does not count, as two (a decode step of one request, 36
-    # layers of the 8B shape: 2.74 ms against 2.93).  The results are the same.
+    # Few rows go as one kernel where it takes the sizes: launched one by one 4 us of the host's time less (7.5 against
+    # 12), in a graph the same time (1 row, 4,096 x 2,048 / 4,096 / 12,288: 7.1 / 8.0 / 12.7 us, as two kernels 7.0 /
+    # 8.1 / 12.6; a decode step of one request, 36 layers of the 8B shape: 2.605 and 2.610 ms).  The results are the same.
     code = -1
     if held:
         code = _fp8_product_call(0, 0, codes.data_ptr(), codes.stride(0), scales.data_ptr(), scales.stride(0), *behind)
-    elif M <= 8 and starts is None and FP8_RESIDENT and not torch.cuda.is_current_stream_capturing():
+    elif M <= 8 and starts is None and FP8_RESIDENT:
         # (not where the result may lie on the rows: its blocks would read what others have written)
         x_at, stride, out_at = x.data_ptr(), x.stride(0), out.data_ptr()
         if (x_at + 2 * ((M - 1) * stride + K) <= out_at

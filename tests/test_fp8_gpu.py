@@ -749,3 +749,25 @@ def test_captured_experts_with_other_rows_each_time(cuda_device, R):
                 k = row_w[a:b, None].to(F64)
                 _check(out[a:b], ref * k, (off + ref.abs() * 2.0 ** -23) * k)
         assert (out[:s[0]] == 9).all() and (out[s[-1]:] == 9).all()
+
+
+@pytest.mark.parametrize("M", [1, 8])
+def test_one_kernel_in_a_graph_too(cuda_device, M):
+    """Which kernels a call takes depends on its sizes, not on how it is launched."""
+    from binfer_b200.csrc import ops
+    w = _w((300, 1024), cuda_device)
+    held, x = ops.fp8_weight(w), _x(M, 1024, cuda_device)
+    out, eager = (torch.empty((M, 300), dtype=F32, device=cuda_device) for _ in range(2))
+    ops.fp8_linear(x, held, out)
+    torch.cuda.synchronize()
+    gc.collect()
+    g, before = torch.cuda.CUDAGraph(), ops.launches()
+    with torch.cuda.graph(g):
+        ops.fp8_linear(x, held, out)
+    assert ops.launches() - before == 1
+    for seed in range(3):
+        x.copy_(_x(M, 1024, cuda_device, 30 + seed))
+        g.replay()
+        ops.fp8_linear(x, held, eager)
+        assert torch.equal(out, eager)
+        _check(out, *P8.product(x, *P8.hold_weight(w)))
