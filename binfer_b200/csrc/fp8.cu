@@ -1,8 +1,9 @@
 // Activations and weights into 8 bits and back (the format: fp8.cuh).
 //
 // All kernels pass over the data once, with the numbers of a group in registers between the search for
-// the largest and the rounding.  2,048 x 12,288 bfloat16 into codes: 17 us (4.4 TB/s; eight or nine integer
-// instructions a number); back as floats: 25 us (5.0 TB/s); a weight of 12,288 x 4,096: 31 and 51 us (4.9 TB/s).
+// the largest and the rounding.  2,048 x 12,288 bfloat16 into codes: 17.3 us (4.4 TB/s; eight or nine integer
+// instructions a number), float32 23.6 (5.4 TB/s); back as floats: 24 us (5.2 TB/s); a weight of 12,288 x 4,096: 31 us
+// (4.8 TB/s; float32 43, 5.8 TB/s), back as floats 47 (5.3 TB/s).
 #include "fp8.cuh"
 
 namespace {
@@ -85,7 +86,8 @@ fp8_rows_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ co
 
 // A block a row: resid (+= delta), RMSNorm, rounding to bfloat16, into 8 bits; eight numbers a thread and
 // trip, sixteen threads a group.  The sums have the order of the norm's own kernel: the codes are those of
-// its output.
+// its output.  2,048 rows of 4,096 with an addition: 18.1 us (5.1 TB/s; the norm and fp8_rows one behind the other
+// 22.1), 8 rows 2.6 (4.0): the way from the kernel ahead and two passes through a block's barrier.
 template <int TRIPS>
 __global__ void add_rmsnorm_fp8_kernel(float* __restrict__ resid, const __nv_bfloat16* __restrict__ delta,
                                        const float* __restrict__ w, uint8_t* __restrict__ codes, long long ldc,
@@ -416,12 +418,13 @@ extern "C" int bf_gemm_fp8_pair(const void*, long long, const float*, long long,
 
 // How a product runs: the most rows of a tile of gemm_fp8_few.cu, or -1 for gemm_fp8_pair.cu.
 // Without experts: tiles of 32 rows while there is one for every SM at most, or two with few groups (157
-// rows, 6,144 x 4,096: 17.0 us against 22.1 with tiles of 64 and 17.9 on pairs; 4,096 x 12,288: 37.1 / 37.9 /
-// 32.0); then 64 if those hold all rows (64 rows, 24,576 x 4,096 gated: 30.8 / 26.9 / 43.7); up to 96 rows 32
-// again (34.3 / 47.6 / 44.8); then pairs (157 rows of the same: 55.7 / 49.1 / 45.8).
-// With experts by the rows that one has on average (64 experts, 2,048 x 2,048 gated, 8 to 128 rows each: 47 /
-// 51 / 55 us with tiles of 16 / 32 / 64 and 84 on pairs, 77 / 62 / 60 / 92, 128 / 90 / 84 / 104, 228 / 156 /
-// 136 / 126).
+// rows, 6,144 x 4,096: 17.2 us against 22.3 with tiles of 64 and 18.0 on pairs; 4,096 x 12,288: 36.9 / 38.0 /
+// 32.1); then 64 if those hold all rows (64 rows, 24,576 x 4,096 gated: 33.1 / 27.0 / 42.3); up to 96 rows 32
+// again (35.2 / 48.9 / 42.8); then pairs (157 rows of the same: 57.1 / 50.0 / 43.7).
+// With experts by the rows that one has on average (64 experts, 2,048 x 2,048 gated, 8 to 128 rows each: 52 /
+// 52 / 53 us with tiles of 16 / 32 / 64 and 80 on pairs, 58 / 57 / 56 / 83, 99 / 72 / 67 / 88, 188 / 131 / 108 / 96).
+// The rows' shares lie on the device and are not known here: where few experts have all rows, theirs come in more
+// and smaller tiles than would be fastest.
 static int fp8_tile(int rows, int features, int K, bool gated, int experts, int num_sms) {
   const int each = (rows + experts - 1) / experts;
   if (each <= 16) return 16;
@@ -438,13 +441,13 @@ static int fp8_split(int rows, int features, int K, bool gated, int nb, int num_
   const long long tiles = (long long)((rows + nb - 1) / nb) * ((features + (gated ? 63 : 127)) / (gated ? 64 : 128));
   const int groups = (K + BF_FP8_GROUP - 1) / BF_FP8_GROUP;
   int c = 1;
-  while (nb <= 64 && c < 8 && tiles * 2 * c <= 2 * num_sms && groups >= 4 * c) c *= 2;
+  while (c < 8 && tiles * 2 * c <= 2 * num_sms && groups >= 4 * c) c *= 2;
   return c;
 }
 
 // Pairs that share a tile of 256 x 256, each with four groups at least: two while those are resident together
-// (157 rows, 4,096 x 12,288: 50.8 -> 32.0 us; 512 rows: 54.2 -> 37.2), four for the fewest tiles (64 rows, 1,024
-// x 4,096: 19.5 / 15.2 / 13.2; with 16 tiles, whose clusters of eight CTAs run in two turns, 21.4 / 16.6 / 27.4).
+// (157 rows, 4,096 x 12,288: 47.2 -> 32.6 us; 512 rows: 50.6 -> 37.1), four for the fewest tiles (64 rows, 1,024
+// x 4,096: 18.7 / 15.4 / 13.6; with 16 tiles, whose clusters of eight CTAs run in two turns, 19.5 / 16.4 / 27.4).
 static int fp8_pair_split(int rows, int features, int K, bool gated, int num_sms) {
   const long long tiles = (rows + 255LL) / 256 * ((features + (gated ? 127 : 255)) / (gated ? 128 : 256));
   const int groups = (K + BF_FP8_GROUP - 1) / BF_FP8_GROUP;

@@ -3,19 +3,20 @@
 //
 // The weight's rows are the product's rows (128 of them = 128 lanes of tensor memory) and the
 // activations' rows its columns, of which a tile has as many as there are, rounded up to 16: nothing is
-// multiplied for rows that are not there, and an expert with 37 rows pays for 48.  One tcgen05.mma.kind::f8f6f4 takes K = 32; the four of a group go into columns of
-// tensor memory of their own, a ring of them, and the epilogue's warps add each group's sums, times its
-// two scales, into registers (float; the scales cannot ride along in tensor memory).
+// multiplied for rows that are not there, and an expert with 37 rows pays for 48.  One
+// tcgen05.mma.kind::f8f6f4 takes K = 32; the four of a group go into columns of tensor memory of their own,
+// a ring of them, and the epilogue's warps add each group's sums, times its two scales, into registers
+// (float; the scales cannot ride along in tensor memory).
 //
 //   warp 0       TMA: 128 weight rows and NB activation rows x 128 bytes per stage
 //   warp 1       the products; TMEM allocation
 //   warp 2       the factors sx sw of every column of a group, into shared memory; whether one is no float (fp8.cuh)
 //   warps 4-11   the sums, times the factors, into registers; the result
 //
-// What bounds it with few rows is the weights' bytes (8 rows, 24,576 x 4,096 gated: 20.5 us with the rows'
-// codes, 5.4 TB/s) or, of narrow weights, the way from the last of them to the end: a group passes 350
+// What bounds it with few rows is the weights' bytes (8 rows, 24,576 x 4,096 gated: 21.2 us with the rows'
+// codes, 4.8 TB/s) or, of narrow weights, the way from the last of them to the end: a group passes 350
 // cycles of the issuing warp and 230 and more of the sums', the parts of a cluster meet in 1 us (4,096 x 4,096:
-// 7.6 us, of which 1.5 are the rows' codes).  A tile is 128 rows of the weight, so that a narrow weight alone does
+// 8.7 us, of which 1.0 are the rows' codes).  A tile is 128 rows of the weight, so that a narrow weight alone does
 // not give every SM work: then a cluster of `split` CTAs shares a tile, each a part of the groups, and the
 // parts meet in shared memory, added in the order of the ranks.
 // With more rows it is what a group costs beside its products (157 rows, 6,144 x 4,096: 17 us; the tensor
@@ -412,8 +413,7 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
         }
         tc_fence_after();
         const float* f = factors + (slot * HALVES + which) * NB;
-        // (the two halves of the warps take the chunks in turn; a warp's are all asked for before the first
-        // is waited for: one after the other, a group of 128 columns took 1,030 cycles)
+        // (the two halves of the warps take the chunks in turn, one after the other: a warp has two at most)
         const uint32_t at = tmem_base + lanes + (uint32_t)(slot * NB + half * CH);
 #pragma unroll
         for (int i = 0; i < CHUNKS; ++i) {
@@ -713,8 +713,8 @@ int few_by_width(int nb, bool resident, const void* x, long long ldx, const void
 // (gated ? 2 : 1) * features, K] (rows ldw bytes apart) with scales sw [experts, (gated ? 2 : 1) *
 // ceil(features / 128), ceil(K / 128)]; starts int [experts + 1] of the experts' first rows, or null for
 // one weight; row_w float [rows] or null; out [rows, features], rows ldo apart.  nb: most rows of a tile
-// (16, 32 or 64).  split: CTAs that share a tile (without experts, tiles * split at most
-// num_sms; else 1 is taken).
+// (16, 32 or 64).  split: CTAs that share a tile (without experts, tiles * split at most 2 * num_sms, as many as
+// are resident, and at most as many as there are groups; else 1 is taken).
 BF_EXPORT int bf_gemm_fp8_few(const void* x, long long ldx, const float* sx, long long lds, const void* w,
                               long long ldw, const float* sw, const int* starts, const float* row_w,
                               void* out, long long ldo, int out_dtype, int rows, int features, int K,

@@ -14,13 +14,13 @@
 //   warps 4-19   the sums into registers; the result, turned in shared memory so that a warp writes
 //                64 bytes a row (these four warpgroups take 112 registers a thread, which the first
 //                leaves them: 128 x 32 + 512 x 112 of the launch's 640 x 96; with 104 the products of 2,048
-//                rows and 24,576 x 4,096 gated took 210 us, now 201)
+//                rows and 24,576 x 4,096 gated took 210 us, with 112 201)
 //
 // What bounds it: the sums' warps.  A group's products take 512 cycles, its 32 packed multiply-adds a warp 278 for
 // the four warps of a scheduler, but a warp executes 126 instructions a group in a chain of waits (2,048 rows,
-// 24,576 x 4,096 gated, 201 us without the rows' codes, 2.05 PFLOP/s: without fetching operands 6 us less, without
-// the results 26, with an eighth of the multiply-adds 50; products and signals alone 110).  When it runs on, the
-// clock too (1.67 GHz at 900 W).  Eight warps with 128 sums each took 236 us.
+// 24,576 x 4,096 gated, 205 us without the rows' codes, 2.0 PFLOP/s; parts left out to time the rest, of 201 us then:
+// without fetching operands 6 us less, without the results 26, with an eighth of the multiply-adds 50; products and
+// signals alone 110).  When it runs on, the clock too (1.67 GHz at 900 W).  Eight warps with 128 sums each took 236 us.
 //
 // SPLIT: few tiles leave SMs idle, and `split` pairs share one, a cluster of twice as many CTAs: each adds up
 // its part of the groups, the parts meet in the shared memory that the ring had, a pair owning a slice of

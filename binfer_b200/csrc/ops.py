@@ -3180,7 +3180,7 @@ def fp8_linear(x: torch.Tensor, w: Fp8Weight, out: torch.Tensor, activation: str
     ``out = act(g) u`` of the product's two halves, ``activation`` as in :func:`gated_act_mul` ("silu" or
     "clamped").  ``out``: bfloat16, or float32 for a weight that is not gated; it may be a column block of a
     wider buffer.  A row's result does not depend on the other rows' values.  ``tile``, ``split``: rows of a
-    tile (16, 32 or 64; -1: on pairs of SMs) and SMs that share one (0: chosen by the library)."""
+    tile (16, 32 or 64; -1: on pairs of SMs) and CTAs, or pairs, that share one (0: chosen by the library)."""
     if w.experts:
         raise KernelError("fp8_linear: the weight has experts")
     _fp8_product("fp8_linear", x, w, None, out, None, activation, limit, slope, up_offset, tile, split)
