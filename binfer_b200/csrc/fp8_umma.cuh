@@ -192,20 +192,32 @@ static inline int fp8_map(CUtensorMap* map, const void* base, long long rows, lo
   return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
 }
 
-// up to four codes, of which `left` are there
-__device__ __forceinline__ uint32_t fp8_word(const uint8_t* p, int left) {
-  if (left >= 4) return *reinterpret_cast<const uint32_t*>(p);
-  uint32_t r = 0u;
-  for (int j = 0; j < left; ++j) r |= (uint32_t)p[j] << (8 * j);
-  return r;
+// sixteen codes, of which `left` are there (the others zero), on a 16-byte boundary
+__device__ __forceinline__ uint4 fp8_sixteen(const uint8_t* p, int left) {
+  if (left >= 16) return *reinterpret_cast<const uint4*>(p);
+  uint32_t r[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+    if (j < left) r[j >> 2] |= (uint32_t)p[j] << (8 * (j & 3));
+  return make_uint4(r[0], r[1], r[2], r[3]);
 }
-// Whether a result has a factor that is no float of full precision (fp8.cuh) among the groups g0 .. g1 - 1, and its sum
-// over them, by multiply-adds.  scale_x(g), scale_w(g): the groups' scales; x(g, k), w(g, k): where their codes
-// k .. k + 3 lie (k a multiple of 4).  K: columns in all.  By one thread; slow, and rare.
-template <typename SX, typename SW>
-__device__ bool fp8_any_odd(int g0, int g1, SX scale_x, SW scale_w) {
-  for (int g = g0; g < g1; ++g)
-    if (fp8_odd(scale_x(g), scale_w(g))) return true;
+// Whether the loop's sum of a result's groups g0 .. g1 - 1 is off because of a factor that is no float of full precision
+// (fp8.cuh; one taken as zero does no harm where the row's numbers are zeros, as in a padded batch), and that sum by
+// multiply-adds.  scale_x(g), scale_w(g): the groups' scales; x(g, k), w(g, k): where their codes k .. k + 15 lie (k a
+// multiple of 16).  K: columns in all.  By one thread; slow, and rare.
+template <typename SX, typename SW, typename X>
+__device__ bool fp8_any_odd(int g0, int g1, int K, SX scale_x, SW scale_w, X x) {
+  for (int g = g0; g < g1; ++g) {
+    if (!fp8_odd(scale_x(g), scale_w(g))) continue;
+    if (fp8_factor(scale_x(g), scale_w(g)).after > 1.f) return true;
+    uint32_t any = 0u;
+#pragma unroll 4
+    for (int k = 0; k < FK; k += 16) {
+      const uint4 c = fp8_sixteen(x(g, k), K - g * FK - k);
+      any |= c.x | c.y | c.z | c.w;
+    }
+    if (any & 0x7f7f7f7fu) return true;
+  }
   return false;
 }
 template <typename SX, typename SW, typename X, typename W>
@@ -213,14 +225,19 @@ __device__ float fp8_sum_anew(int g0, int g1, int K, SX scale_x, SW scale_w, X x
   float acc = 0.f;
   for (int g = g0; g < g1; ++g) {
     const Fp8Factor f = fp8_factor(scale_x(g), scale_w(g));
-    const int n = min(FK, K - g * FK);
     float sum = 0.f;
-    for (int k = 0; k < n; k += 4) {
-      float a[4], b[4];
-      fp8_values4(fp8_word(x(g, k), n - k), a);
-      fp8_values4(fp8_word(w(g, k), n - k), b);
+#pragma unroll 2
+    for (int k = 0; k < FK; k += 16) {
+      const uint4 a4 = fp8_sixteen(x(g, k), K - g * FK - k), b4 = fp8_sixteen(w(g, k), K - g * FK - k);
+      const uint32_t a[4] = {a4.x, a4.y, a4.z, a4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum = fmaf(a[j], b[j], sum);
+      for (int i = 0; i < 4; ++i) {
+        float u[4], v[4];
+        fp8_values4(a[i], u);
+        fp8_values4(b[i], v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum = fmaf(u[j], v[j], sum);
+      }
     }
     acc = fmaf(sum * f.before, f.after, acc);
   }

@@ -450,13 +450,11 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
             if (c >= n) continue;
             auto scale_x = [&](int g) { return res_sx[(g - g0) * NB + c]; };
             auto scale_w = [&](int g) { return swr[g]; };
-            if (!fp8_any_odd(g0, g1, scale_x, scale_w)) continue;
-            const float v = fp8_sum_anew(
-                g0, g1, p.K, scale_x, scale_w,
-                [&](int g, int k) {
-                  return res + ((g - g0) * FEW_RES_ROWS + c) * FK + (((k >> 4) ^ (c & 7)) << 4) + (k & 15);
-                },
-                [&](int g, int k) { return wr + g * FK + k; });
+            auto x_at = [&](int g, int k) {
+              return res + ((g - g0) * FEW_RES_ROWS + c) * FK + (((k >> 4) ^ (c & 7)) << 4) + (k & 15);
+            };
+            if (!fp8_any_odd(g0, g1, p.K, scale_x, scale_w, x_at)) continue;
+            const float v = fp8_sum_anew(g0, g1, p.K, scale_x, scale_w, x_at, [&](int g, int k) { return wr + g * FK + k; });
 #pragma unroll
             for (int i = 0; i < CHUNKS * CH; ++i) acc[i / CH][i % CH] = i == a ? v : acc[i / CH][i % CH];
           }
@@ -573,17 +571,17 @@ fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
         auto scales_w = [&](int h) {
           return p.sw + (((long long)t.expert * HALVES + h) * p.w_blocks + (o >> 7)) * p.groups;
         };
+        auto x_at = [&](int g, int k) { return p.codes + row * p.ldx + g * FK + k; };
         bool any = false;
         for (int h = 0; h < HALVES; ++h)
-          any = any || fp8_any_odd(0, p.groups, scale_x, [at = scales_w(h)](int g) { return at[g]; });
+          any = any || fp8_any_odd(0, p.groups, p.K, scale_x, [at = scales_w(h)](int g) { return at[g]; }, x_at);
         if (!any) continue;
         float v[2];
 #pragma unroll 1
         for (int h = 0; h < HALVES; ++h) {
           const uint8_t* wr = p.w + ((long long)t.expert * w_rows + h * p.features + o) * p.ldw;
           const float sum = fp8_sum_anew(
-              0, p.groups, p.K, scale_x, [at = scales_w(h)](int g) { return at[g]; },
-              [&](int g, int k) { return p.codes + row * p.ldx + g * FK + k; },
+              0, p.groups, p.K, scale_x, [at = scales_w(h)](int g) { return at[g]; }, x_at,
               [&](int g, int k) { return wr + g * FK + k; });
           if (h == 0) v[0] = sum; else v[1] = sum;
         }

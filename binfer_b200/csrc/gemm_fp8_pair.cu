@@ -451,13 +451,14 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         auto scale_w = [&](int up) {
           return [at = swa + (long long)up * p.w_blocks * p.groups](int g) { return at[g]; };
         };
+        auto x_at = [&](int g, int k) { return xr + g * FK + k; };
         auto sum = [&](int o, int up) {
           const uint8_t* wr = p.w + ((size_t)t.expert * w_rows + up * p.features + o) * p.ldw16 * 16;
           return fp8_sum_anew(
-              0, p.groups, p.K, scale_x, scale_w(up), [&](int g, int k) { return xr + g * FK + k; },
-              [&](int g, int k) { return wr + g * FK + k; });
+              0, p.groups, p.K, scale_x, scale_w(up), x_at, [&](int g, int k) { return wr + g * FK + k; });
         };
-        if (!fp8_any_odd(0, p.groups, scale_x, scale_w(0)) && (!GATED || !fp8_any_odd(0, p.groups, scale_x, scale_w(1))))
+        if (!fp8_any_odd(0, p.groups, p.K, scale_x, scale_w(0), x_at) &&
+            (!GATED || !fp8_any_odd(0, p.groups, p.K, scale_x, scale_w(1), x_at)))
           continue;
         const float w = p.row_w ? p.row_w[row] : 1.f;
         for (int o = o0; o < min(o0 + (GATED ? 32 : 64), p.features); ++o)
@@ -559,8 +560,8 @@ BF_EXPORT int bf_gemm_fp8_pair(const void* x, long long ldx, const float* sx, lo
                                int experts, int gated, int act, float limit, float slope, float up_offset,
                                int split, int num_sms, int* err, cudaStream_t stream) {
   if (rows <= 0 || features <= 0) return 0;
-  if (K <= 0 || experts < 1 || experts > FP8_MAX_EXPERTS || (!starts && experts != 1) || ldx % 16 || ldw % 16 || ldx >> 35 || ldw >> 35 ||
-      (((uintptr_t)x | (uintptr_t)w) & 15) || num_sms < 2 ||
+  if (K <= 0 || experts < 1 || experts > FP8_MAX_EXPERTS || (!starts && experts != 1) || ldx % 16 || ldw % 16 ||
+      ldx >> 35 || ldw >> 35 || (((uintptr_t)x | (uintptr_t)w) & 15) || num_sms < 2 ||
       (act != BF_ACT_SILU && act != BF_ACT_CLAMPED) || (gated && out_dtype != BF_DTYPE_BF16))
     return (int)cudaErrorInvalidValue;
   PairParams p = {};

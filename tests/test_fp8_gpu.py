@@ -771,3 +771,20 @@ def test_one_kernel_in_a_graph_too(cuda_device, M):
         ops.fp8_linear(x, held, eager)
         assert torch.equal(out, eager)
         _check(out, *P8.product(x, *P8.hold_weight(w)))
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("M,kw", [(6, {}), (6, dict(split=1, tile=32)), (100, dict(tile=64)), (300, dict(tile=-1, split=1)),
+                                  (300, dict(tile=-1, split=2))])
+def test_rows_of_zeros_beside_tiny_weights(cuda_device, M, kw, gated):
+    """Zeros' scale is the smallest there is, so that its product with a small weight's is no float: such rows, and groups
+    of zeros within others, count as zeros, and results of the others are what they are."""
+    from binfer_b200.csrc import ops
+    x, w = _x(M, 640, cuda_device, M), _w(((1 + gated) * 200, 640), cuda_device, M)
+    w[:, 128:256] *= 2.0 ** -40
+    x[::2] = 0
+    x[1::4, 128:256] = 0
+    out = torch.empty((M, 200), dtype=BF16 if gated else F32, device=cuda_device)
+    ops.fp8_linear(x, ops.fp8_weight(w, gated), out, **kw)
+    _check(out, *P8.product(x, *P8.hold_weight(w, gated), gated))
+    assert not out[::2].any() and out[1::2].any(dim=1).all()
