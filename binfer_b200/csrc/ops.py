@@ -1907,7 +1907,7 @@ class _Packed:
     def __call__(self, *args) -> int:
         try:
             packed = self.pack(*args)
-        except (struct.error, OverflowError) as e:
+        except struct.error as e:
             raise KernelError(f"{self.name}: an argument that its type has no room for ({e})") from None
         if self.fn is None:
             fn = getattr(lib(), self.name)

@@ -241,10 +241,3 @@ def test_more_rows_than_the_kernels_count_are_refused(ops):
                  lambda: ops.fp8_rows_read(_codes(1, 1).expand(n, 1), torch.ones(1, 1).expand(1, n), y)):
         with pytest.raises(ops.KernelError, match="at most"):
             call()
-
-
-def test_numbers_that_an_argument_has_no_room_for(ops):
-    """A launcher's arguments are packed: whatever does not fit is an error of the framework's own."""
-    for fields, value in (("f", 1e40), ("i", 2 ** 31), ("q", 2 ** 63), ("P", -2 ** 64)):
-        with pytest.raises(ops.KernelError, match="no room"):
-            ops._Packed("bf_fp8_rows", fields)(value)
